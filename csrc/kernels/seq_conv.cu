@@ -1,0 +1,442 @@
+// seq_conv.cu — short causal depthwise convolution over the tokens of a row,
+// SiLU behind it: whole sequences, their gradient, single tokens (sm_100a).
+//
+//   pre[t, d] = bias[d] + sum_{k < W} w[d, k] * x[t - (W - 1) + k, d]
+//   y = pre * sigmoid(pre)            (or pre itself)
+//
+// The tokens before the row are the W - 1 rows of `state` (oldest first, zeros
+// without one); reset[b, t] drops everything before token t, and tokens from
+// lengths[b] on are not there: they give zeros and are never read. Everything is
+// one pass over memory (2 W + 4 flops per element against 4 to 8 bytes): the
+// window slides through registers, a thread owning kV neighbouring channels over a
+// stretch of tokens, so each x is read once (plus W - 1 of every stretch).
+#include <type_traits>
+
+#include "seq_common.cuh"
+
+namespace {
+
+using namespace seqk;
+
+struct ConvArgs {
+  const void* x;
+  const void* dy;
+  const void* state;          // [B, W-1, D] or null
+  const void* dfinal;         // [B, W-1, D] or null
+  const float* w;             // [D, W]
+  const float* bias;          // [D] or null
+  const uint8_t* reset;       // [B, T] or null
+  const int* lengths;         // [B] or null
+  void* y;                    // forward: [B, T, D]; gradient: dx
+  void* final_state;          // forward: [B, W-1, D] or null; gradient: dstate or null
+  float* part;                // gradient: [rows][W + 1][D] partial sums of dw and dbias
+  int64_t x_b, x_t, dy_b, dy_t, y_b, y_t, r_b;
+  int B, T, D, silu;
+  int tt, chunks;             // tokens of a stretch, stretches of a row
+};
+
+// 16-byte vectors would hold 8 bf16 channels, and with them the window, weights
+// and sums of the gradient no longer fit the registers: 4 channels for both types.
+constexpr int kV = 4;
+
+// ---- whole sequences ----------------------------------------------------------------
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) {
+  const int groups = a.D / V;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (id >= static_cast<int64_t>(groups) * a.chunks * a.B) return;
+  const int d = static_cast<int>(id % groups) * V;
+  const int64_t rest = id / groups;
+  const int chunk = static_cast<int>(rest % a.chunks);
+  const int b = static_cast<int>(rest / a.chunks);
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  const int t0 = chunk * a.tt, t1 = min(a.T, t0 + a.tt);
+  const T* x = static_cast<const T*>(a.x) + b * a.x_b + d;
+  T* y = static_cast<T*>(a.y) + b * a.y_b + d;
+  const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+  const T* st = a.state ? static_cast<const T*>(a.state) + static_cast<int64_t>(b) * (W - 1) * a.D + d : nullptr;
+
+  float w[V][W], bias[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[i][k] = a.w[static_cast<int64_t>(d + i) * W + k];
+    bias[i] = a.bias ? a.bias[d + i] : 0.0f;
+  }
+  // the W - 1 tokens before the stretch
+  float h[W - 1][V];
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) {
+    const int t = t0 - (W - 1) + j;
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
+    if (t >= 0 && t < len) {
+      if (reset && reset[t]) {
+#pragma unroll
+        for (int q = 0; q < j; ++q)
+#pragma unroll
+          for (int i = 0; i < V; ++i) h[q][i] = 0.0f;
+      }
+      load_vec<T, V>(x + t * a.x_t, h[j]);
+    } else if (t < 0 && st) {
+      load_vec<T, V>(st + static_cast<int64_t>(W - 1 + t) * a.D, h[j]);
+    }
+  }
+  constexpr int U = 8;                    // tokens loaded ahead
+  const int live = min(t1, len);
+  for (int t = t0; t < live; t += U) {
+    float in[U][V];
+    bool cut[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      cut[u] = false;
+      if (t + u < live) {
+        load_vec<T, V>(x + (t + u) * a.x_t, in[u]);
+        if (reset) cut[u] = reset[t + u] != 0;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u < live) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float acc = bias[i];
+#pragma unroll
+          for (int j = 0; j < W - 1; ++j) {
+            if (cut[u]) h[j][i] = 0.0f;
+            acc = fmaf(w[i][j], h[j][i], acc);
+          }
+          acc = fmaf(w[i][W - 1], in[u][i], acc);
+#pragma unroll
+          for (int j = 0; j + 1 < W - 1; ++j) h[j][i] = h[j + 1][i];
+          h[W - 2][i] = in[u][i];
+          o[i] = a.silu ? acc * sigmoid(acc) : acc;
+        }
+        store_vec<T, V>(y + (t + u) * a.y_t, o);
+      }
+    }
+  }
+  float zero[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) zero[i] = 0.0f;
+  for (int t = max(t0, live); t < t1; ++t) store_vec<T, V>(y + t * a.y_t, zero);
+  // what the next token finds behind it: by the stretch of the last token
+  if (a.final_state && (len > 0 ? (len - 1 >= t0 && len - 1 < t0 + a.tt) : chunk == 0)) {
+    T* f = static_cast<T*>(a.final_state) + static_cast<int64_t>(b) * (W - 1) * a.D + d;
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) store_vec<T, V>(f + static_cast<int64_t>(j) * a.D, h[j]);
+  }
+}
+
+// ---- gradient -------------------------------------------------------------------------
+// One sweep in token order: with the window at hand pre[t] is recomputed, dpre[t] =
+// dy[t] * silu'(pre[t]) is spread onto the W pending dx of the tokens that it sees,
+// and dx[t - (W - 1)] is then complete. A stretch runs W - 1 tokens on into the next
+// one for its own last tokens; only its own tokens count for dw and dbias, whose
+// sums a block joins in shared memory and leaves as one row of `part`, summed in
+// row order by conv_reduce_kernel: no atomics, so a rerun gives the same bits.
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(256) conv_grad_kernel(ConvArgs a, int items) {
+  extern __shared__ float red[];                                // [blockDim.y][W + 1][blockDim.x * V]
+  const int groups = a.D / V;
+  const int cg = blockIdx.x * blockDim.x + threadIdx.x;
+  const int d = cg * V;
+  const bool on = cg < groups;
+  float w[V][W], bias[V], dw[V][W], db[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      w[i][k] = on ? a.w[static_cast<int64_t>(d + i) * W + k] : 0.0f;
+      dw[i][k] = 0.0f;
+    }
+    bias[i] = on && a.bias ? a.bias[d + i] : 0.0f;
+    db[i] = 0.0f;
+  }
+  if (on) {
+    for (int item = blockIdx.y * blockDim.y + threadIdx.y; item < items; item += gridDim.y * blockDim.y) {
+      const int b = item / a.chunks, chunk = item - b * a.chunks;
+      const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+      const int t0 = chunk * a.tt, t1 = min(a.T, t0 + a.tt);
+      const T* x = static_cast<const T*>(a.x) + b * a.x_b + d;
+      const T* dy = static_cast<const T*>(a.dy) + b * a.dy_b + d;
+      T* dx = static_cast<T*>(a.y) + b * a.y_b + d;
+      const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+      const int64_t ends = static_cast<int64_t>(b) * (W - 1) * a.D + d;
+      const T* st = a.state ? static_cast<const T*>(a.state) + ends : nullptr;
+      const T* df = a.dfinal ? static_cast<const T*>(a.dfinal) + ends : nullptr;
+      T* ds = a.final_state ? static_cast<T*>(a.final_state) + ends : nullptr;
+      float h[W - 1][V], pend[W][V];                 // pend[j]: dx of token t - j so far
+      unsigned seen = 0;                             // bit j: token t sees token t - 1 - j
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) {
+        const int t = t0 - (W - 1) + j;
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
+        if (t >= 0 && t < len) {
+          if (reset && reset[t]) {
+            seen = 0;
+#pragma unroll
+            for (int q = 0; q < j; ++q)
+#pragma unroll
+              for (int i = 0; i < V; ++i) h[q][i] = 0.0f;
+          }
+          load_vec<T, V>(x + t * a.x_t, h[j]);
+        } else if (t < 0 && st) {
+          load_vec<T, V>(st + static_cast<int64_t>(W - 1 + t) * a.D, h[j]);
+        }
+        seen = (seen << 1) | 1u;
+      }
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) pend[j][i] = 0.0f;
+      if (len == 0 && chunk == 0 && df) {            // an empty row hands its state on
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) load_vec<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D, pend[j + 1]);
+      }
+      const int end = t1 + W - 1;
+      constexpr int U = 4;
+      for (int tb = t0; tb < end; tb += U) {
+        float xin[U][V], gin[U][V];
+        bool cut[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int t = tb + u;
+          cut[u] = false;
+#pragma unroll
+          for (int i = 0; i < V; ++i) xin[u][i] = gin[u][i] = 0.0f;
+          if (t < end && t < len) {
+            load_vec<T, V>(x + t * a.x_t, xin[u]);
+            load_vec<T, V>(dy + t * a.dy_t, gin[u]);
+            if (reset) cut[u] = reset[t] != 0;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int t = tb + u;
+          if (t < end) {
+            if (t < len) {
+              if (cut[u]) {
+                seen = 0;
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+                  for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
+              }
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                float g = gin[u][i];
+                if (a.silu) {
+                  float pre = bias[i];
+#pragma unroll
+                  for (int j = 0; j < W - 1; ++j) pre = fmaf(w[i][j], h[j][i], pre);
+                  pre = fmaf(w[i][W - 1], xin[u][i], pre);
+                  const float s = sigmoid(pre);
+                  g *= s * fmaf(pre, 1.0f - s, 1.0f);
+                }
+                pend[0][i] = fmaf(w[i][W - 1], g, pend[0][i]);
+#pragma unroll
+                for (int j = 1; j < W; ++j)
+                  if (seen >> (j - 1) & 1u) pend[j][i] = fmaf(w[i][W - 1 - j], g, pend[j][i]);
+                if (t < t1) {
+                  db[i] += g;
+#pragma unroll
+                  for (int k = 0; k < W - 1; ++k) dw[i][k] = fmaf(h[k][i], g, dw[i][k]);
+                  dw[i][W - 1] = fmaf(xin[u][i], g, dw[i][W - 1]);
+                }
+              }
+              if (t == len - 1 && df) {              // the state behind the last token
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j)
+                  if (j == 0 || (seen >> (j - 1) & 1u)) {
+                    float e[V];
+                    load_vec<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D, e);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) pend[j][i] += e[i];
+                  }
+              }
+            }
+            const int done = t - (W - 1);
+            if (done >= t0 && done < t1) store_vec<T, V>(dx + done * a.y_t, pend[W - 1]);
+            else if (done < 0 && ds) store_vec<T, V>(ds + static_cast<int64_t>(W - 1 + done) * a.D, pend[W - 1]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+#pragma unroll
+              for (int j = W - 1; j > 0; --j) pend[j][i] = pend[j - 1][i];
+              pend[0][i] = 0.0f;
+#pragma unroll
+              for (int j = 0; j + 1 < W - 1; ++j) h[j][i] = h[j + 1][i];
+              h[W - 2][i] = xin[u][i];
+            }
+            seen = (seen << 1) | 1u;
+          }
+        }
+      }
+    }
+  }
+  // join the block's rows of sums
+  const int cols = blockDim.x * V;
+  float* mine = red + threadIdx.y * (W + 1) * cols + threadIdx.x * V;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) mine[k * cols + i] = dw[i][k];
+    mine[W * cols + i] = db[i];
+  }
+  __syncthreads();
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+  for (int e = tid; e < (W + 1) * cols; e += blockDim.x * blockDim.y) {
+    float s = 0.0f;
+    for (int r = 0; r < static_cast<int>(blockDim.y); ++r) s += red[r * (W + 1) * cols + e];
+    const int k = e / cols, c = blockIdx.x * cols + (e - k * cols);
+    if (c < a.D) a.part[(static_cast<int64_t>(blockIdx.y) * (W + 1) + k) * a.D + c] = s;
+  }
+}
+
+// dw[d, k] and dbias[d] from the rows of `part`, 8 row sums side by side, joined in order
+template <int W>
+__global__ void __launch_bounds__(256) conv_reduce_kernel(const float* part, int rows, int D, float* dw, float* dbias) {
+  __shared__ float red[8][33];
+  const int e = blockIdx.x * 32 + threadIdx.x;
+  const int total = (W + 1) * D;
+  float s = 0.0f;
+  if (e < total)
+    for (int r = threadIdx.y; r < rows; r += 8) s += part[static_cast<int64_t>(r) * total + e];
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && e < total) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) s += red[r][threadIdx.x];
+    const int k = e / D, d = e - k * D;
+    if (k < W) dw[static_cast<int64_t>(d) * W + k] = s;
+    else if (dbias) dbias[d] = s;
+  }
+}
+
+// ---- single tokens -----------------------------------------------------------------------
+// Row r is the next token of the env in slot slots[r] of the state pool (-1: none, its
+// output is zero); the slot's window is moved on in place.
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(128) conv_step_kernel(const T* x, int64_t ldx, const float* w, const float* bias, T* pool,
+                                                        const uint8_t* reset, const int* slots, int n_slots, T* y, int64_t ldy,
+                                                        int rows, int D, int silu, int* err) {
+  const int groups = D / V;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (id >= static_cast<int64_t>(groups) * rows) return;
+  const int r = static_cast<int>(id / groups), d = static_cast<int>(id - static_cast<int64_t>(r) * groups) * V;
+  const int slot = slots ? slots[r] : r;
+  float o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = 0.0f;
+  if (slot >= n_slots) {
+    surfk::report_error(err, surfk::kErrSlotIndex);
+  } else if (slot >= 0) {
+    T* st = pool + static_cast<int64_t>(slot) * (W - 1) * D + d;
+    float h[W][V];
+    load_vec<T, V>(x + r * ldx + d, h[W - 1]);
+    const bool cut = reset && reset[r];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
+      } else {
+        load_vec<T, V>(st + static_cast<int64_t>(j) * D, h[j]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float acc = bias ? bias[d + i] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) acc = fmaf(w[static_cast<int64_t>(d + i) * W + k], h[k][i], acc);
+      o[i] = silu ? acc * sigmoid(acc) : acc;
+    }
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) store_vec<T, V>(st + static_cast<int64_t>(j) * D, h[j + 1]);
+  }
+  store_vec<T, V>(y + r * ldy + d, o);
+}
+
+// ---- launches -------------------------------------------------------------------------------
+// width -> template argument; vectors of kV channels where `vec`, else one
+template <typename F> int by_width(int W, F f) {
+  switch (W) {
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+  }
+  return static_cast<int>(cudaErrorInvalidValue);
+}
+
+template <typename T, int W, int V> int launch_conv(ConvArgs a, cudaStream_t s) {
+  const int64_t n = static_cast<int64_t>(a.D / V) * a.chunks * a.B;
+  const int64_t blocks = surfk::ceil_div(n, 256);
+  if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
+  conv_kernel<T, W, V><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+  SURF_RETURN_LAUNCH();
+}
+
+template <typename T, int W, int V>
+int launch_grad(ConvArgs a, int rows, float* dw, float* dbias, cudaStream_t s) {
+  const int groups = a.D / V;
+  int bx = 1;
+  while (bx < 32 && bx < groups) bx *= 2;
+  const int by = 256 / bx;
+  const dim3 grid(static_cast<unsigned>(surfk::ceil_div(groups, bx)), static_cast<unsigned>(rows));
+  const size_t smem = static_cast<size_t>(by) * (W + 1) * bx * V * sizeof(float);
+  conv_grad_kernel<T, W, V><<<grid, dim3(bx, by), smem, s>>>(a, a.B * a.chunks);
+  const int rc = static_cast<int>(cudaGetLastError());
+  if (rc) return rc;
+  conv_reduce_kernel<W><<<static_cast<unsigned>(surfk::ceil_div((W + 1) * static_cast<int64_t>(a.D), 32)), dim3(32, 8), 0, s>>>(
+      a.part, rows, a.D, dw, dbias);
+  SURF_RETURN_LAUNCH();
+}
+
+}  // namespace
+
+// vec: D is a multiple of 4 and every row starts on a 4-element boundary
+SURF_EXPORT int surf_seq_conv(const void* args, int dtype, int W, int vec, void* stream) {
+  const ConvArgs a = *static_cast<const ConvArgs*>(args);
+  if (a.B <= 0 || a.D <= 0) return 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return by_width(W, [&](auto w) {
+    constexpr int kW = decltype(w)::value;
+    if (dtype == kBf16) return vec ? launch_conv<bf16, kW, kV>(a, s) : launch_conv<bf16, kW, 1>(a, s);
+    return vec ? launch_conv<float, kW, kV>(a, s) : launch_conv<float, kW, 1>(a, s);
+  });
+}
+
+SURF_EXPORT int surf_seq_conv_grad(const void* args, int dtype, int W, int vec, int rows, float* dw, float* dbias,
+                                   void* stream) {
+  const ConvArgs a = *static_cast<const ConvArgs*>(args);
+  if (a.D <= 0 || rows <= 0 || rows > 65535) return static_cast<int>(cudaErrorInvalidValue);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return by_width(W, [&](auto w) {
+    constexpr int kW = decltype(w)::value;
+    if (dtype == kBf16) return vec ? launch_grad<bf16, kW, kV>(a, rows, dw, dbias, s) : launch_grad<bf16, kW, 1>(a, rows, dw, dbias, s);
+    return vec ? launch_grad<float, kW, kV>(a, rows, dw, dbias, s) : launch_grad<float, kW, 1>(a, rows, dw, dbias, s);
+  });
+}
+
+SURF_EXPORT int surf_seq_conv_step(const void* x, int64_t ldx, const float* w, const float* bias, void* pool,
+                                   const uint8_t* reset, const int* slots, int n_slots, void* y, int64_t ldy, int rows, int D,
+                                   int W, int silu, int dtype, int vec, int* err, void* stream) {
+  if (rows <= 0 || D <= 0) return 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return by_width(W, [&](auto wc) {
+    constexpr int kW = decltype(wc)::value;
+    auto go = [&](auto t, auto v) {
+      using T = decltype(t);
+      constexpr int V = decltype(v)::value;
+      const int64_t n = static_cast<int64_t>(D / V) * rows;
+      conv_step_kernel<T, kW, V><<<static_cast<unsigned>(surfk::ceil_div(n, 128)), 128, 0, s>>>(
+          static_cast<const T*>(x), ldx, w, bias, static_cast<T*>(pool), reset, slots, n_slots, static_cast<T*>(y), ldy, rows,
+          D, silu, err);
+      SURF_RETURN_LAUNCH();
+    };
+    if (dtype == kBf16) return vec ? go(bf16{}, std::integral_constant<int, kV>{}) : go(bf16{}, std::integral_constant<int, 1>{});
+    return vec ? go(float{}, std::integral_constant<int, kV>{}) : go(float{}, std::integral_constant<int, 1>{});
+  });
+}

@@ -1,0 +1,352 @@
+// seq_scan.cu — selective state space scan: whole sequences and single tokens (sm_100a).
+//
+//   delta = softplus(dt + bias)
+//   h[n] <- exp(delta * A[d, n]) * h[n] + delta * x * B[n]        (32-bit state)
+//   out  = (sum_n C[n] * h[n] + D[d] * x) * silu(z)
+//
+// for every channel d of every row, token by token. reset[b, t] empties the state
+// before token t; tokens from lengths[b] on leave it alone, give zeros and are never
+// read. A block takes a stretch of channels through its tokens in tiles of kTile: the
+// tile's x, dt, z, B, C arrive by asynchronous copies while the tile before is worked
+// on, delta and delta * x are made once per channel, and the recurrence runs with the
+// states in registers (4 states of K channels a thread).
+//
+// Long rows with too few channels to fill the GPU are cut into chunks: a first pass
+// leaves each chunk's state from an empty start and its sum of delta (the chunk's
+// whole decay is exp(A * sum), 0 across a reset), a small kernel strings the chunks
+// together, and the scan then runs in all chunks at once.
+#include "seq_scan.cuh"
+
+namespace {
+
+using namespace seqk;
+
+constexpr int kTile = 16;
+constexpr int kThreads = 128;
+
+template <typename T, int LN> struct Layout {
+  static constexpr int K = LN < 4 ? LN : 4;              // channels of a thread
+  static constexpr int CH = kThreads / LN * K;           // channels of a block
+  static constexpr int NP = 4 * LN;                      // states, padded
+  struct Smem {
+    alignas(16) T x[2][kTile * CH], dt[2][kTile * CH], z[2][kTile * CH], B[2][kTile * NP], C[2][kTile * NP];
+    alignas(16) float delta[kTile * CH], u[kTile * CH], y[kTile * CH], Bf[kTile * NP], Cf[kTile * NP];
+    int cut[kTile];
+  };
+};
+
+// kCarry: only the chunk's end state from an empty start and its sum of delta.
+template <typename T, int LN, bool kAsync, bool kCarry>
+__global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_per_group) {
+  using L = Layout<T, LN>;
+  constexpr int K = L::K, CH = L::CH, NP = L::NP;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  typename L::Smem& sm = *reinterpret_cast<typename L::Smem*>(smem_raw);
+  const int blocks = blocks_per_group * a.G;
+  const int b = blockIdx.x / blocks, blk = blockIdx.x - b * blocks;
+  const int g = blk / blocks_per_group, per_group = a.dim / a.G;
+  const int c0 = (blk - g * blocks_per_group) * CH;
+  const int nch = min(CH, per_group - c0);
+  const int d0 = g * per_group + c0;                     // first channel of the block
+  const int chunk = blockIdx.y;
+  const int t_lo = chunk * a.chunk, t_hi = min(a.T, t_lo + a.chunk);
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  const int t_live = min(t_hi, len);
+
+  const int lane = threadIdx.x & 31;
+  const int nl = lane & (LN - 1);
+  const int ch = threadIdx.x / LN * K;                   // the thread's first channel within the block
+  const int n0 = nl * 4;
+
+  float A2[K][4], h[K][4], sumd[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const bool on = ch + k < nch;
+    const int64_t row = static_cast<int64_t>(d0 + ch + k) * a.N;
+    const float4 v = on ? load_state4<LN>(a.A + row, n0, a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
+    A2[k][0] = v.x * kLog2e; A2[k][1] = v.y * kLog2e; A2[k][2] = v.z * kLog2e; A2[k][3] = v.w * kLog2e;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!kCarry && on) {
+      const int64_t bd = static_cast<int64_t>(a.dim) * a.N;
+      if (a.chunks > 1) s = load_state4<LN>(a.carry + (static_cast<int64_t>(b) * a.chunks + chunk) * bd + row, n0, a.N);
+      else if (a.state) s = load_state4<LN>(a.state + b * bd + row, n0, a.N);
+    }
+    h[k][0] = s.x; h[k][1] = s.y; h[k][2] = s.z; h[k][3] = s.w;
+    sumd[k] = 0.0f;
+  }
+  const T* gx = static_cast<const T*>(a.x) + b * a.x_b + d0;
+  const T* gdt = static_cast<const T*>(a.dt) + b * a.dt_b + d0;
+  const T* gz = a.z ? static_cast<const T*>(a.z) + b * a.z_b + d0 : nullptr;
+  const T* gB = static_cast<const T*>(a.B) + b * a.B_b + g * a.B_g;
+  const T* gC = static_cast<const T*>(a.C) + b * a.C_b + g * a.C_g;
+  T* gout = static_cast<T*>(a.out) + b * a.out_b + d0;
+  const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+
+  auto fetch = [&](int t, int buf) {
+    const int rows = min(kTile, t_live - t);
+    if (rows > 0) {
+      copy_rows<T, kThreads, kAsync>(sm.x[buf], CH, gx + t * a.x_t, a.x_t, rows, nch);
+      copy_rows<T, kThreads, kAsync>(sm.dt[buf], CH, gdt + t * a.dt_t, a.dt_t, rows, nch);
+      copy_rows<T, kThreads, kAsync>(sm.B[buf], NP, gB + t * a.B_t, a.B_t, rows, a.N);
+      if (!kCarry) {
+        copy_rows<T, kThreads, kAsync>(sm.C[buf], NP, gC + t * a.C_t, a.C_t, rows, a.N);
+        if (gz) copy_rows<T, kThreads, kAsync>(sm.z[buf], CH, gz + t * a.z_t, a.z_t, rows, nch);
+      }
+    }
+    cp_async_commit();
+  };
+
+  bool any_cut = false;
+  fetch(t_lo, 0);
+  int buf = 0;
+  for (int t0 = t_lo; t0 < t_live; t0 += kTile, buf ^= 1) {
+    cp_async_wait<0>();
+    __syncthreads();
+    fetch(t0 + kTile, buf ^ 1);
+    const int rows = min(kTile, t_live - t0);
+    // delta and delta * x of the tile, B and C in 32 bits
+    for (int i = threadIdx.x; i < kTile * CH; i += kThreads) {
+      const int r = i / CH, c = i - r * CH;
+      float dv = 0.0f, uv = 0.0f;
+      if (r < rows && c < nch) {
+        dv = to_f(sm.dt[buf][i]) + (a.bias ? a.bias[d0 + c] : 0.0f);
+        if (a.softplus) dv = softplus(dv);
+        uv = dv * to_f(sm.x[buf][i]);
+      }
+      sm.delta[i] = dv;
+      sm.u[i] = uv;
+    }
+    for (int i = threadIdx.x; i < kTile * NP; i += kThreads) {
+      const int r = i / NP, n = i - r * NP;
+      const bool in = r < rows && n < a.N;
+      sm.Bf[i] = in ? to_f(sm.B[buf][i]) : 0.0f;
+      if (!kCarry) sm.Cf[i] = in ? to_f(sm.C[buf][i]) : 0.0f;
+    }
+    if (threadIdx.x < kTile) sm.cut[threadIdx.x] = reset && threadIdx.x < rows && reset[t0 + threadIdx.x] ? 1 : 0;
+    __syncthreads();
+    for (int r = 0; r < rows; ++r) {
+      if (sm.cut[r]) {
+        any_cut = true;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[k][i] = 0.0f;
+      }
+      if (!kCarry && a.saved && (r & (kSave - 1)) == 0) {
+        float* s = a.saved + ((static_cast<int64_t>(b) * ((a.T + kSave - 1) / kSave) + (t0 + r) / kSave) * a.dim + d0 + ch) * a.N;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (ch + k < nch) store_state4(s + static_cast<int64_t>(k) * a.N, n0, a.N, h[k]);
+      }
+      float dl[K], u[K], acc[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        dl[k] = sm.delta[r * CH + ch + k];
+        u[k] = sm.u[r * CH + ch + k];
+        acc[k] = 0.0f;
+        if (kCarry) sumd[k] += dl[k];
+      }
+      const float4 Bv = *reinterpret_cast<const float4*>(sm.Bf + r * NP + n0);
+      const float Bt[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
+      float Ct[4] = {0.f, 0.f, 0.f, 0.f};
+      if (!kCarry) {
+        const float4 Cv = *reinterpret_cast<const float4*>(sm.Cf + r * NP + n0);
+        Ct[0] = Cv.x; Ct[1] = Cv.y; Ct[2] = Cv.z; Ct[3] = Cv.w;
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          h[k][i] = fmaf(exp2_hw(dl[k] * A2[k][i]), h[k][i], u[k] * Bt[i]);
+          if (!kCarry) acc[k] = fmaf(h[k][i], Ct[i], acc[k]);
+        }
+      if (!kCarry) {
+        reduce_lanes<LN, K>(acc, lane);
+        if (reduced_writer<LN, K>(lane)) sm.y[r * CH + ch + reduced_channel<LN, K>(lane)] = acc[0];
+      }
+    }
+    __syncthreads();
+    if (!kCarry) {
+      constexpr int V = kAsync ? kVec16<T> : 1;
+      for (int i = threadIdx.x; i < rows * (CH / V); i += kThreads) {
+        const int r = i / (CH / V), c = (i - r * (CH / V)) * V;
+        if (c >= nch) continue;
+        float o[V], xv[V];
+        load_vec<T, V>(sm.x[buf] + r * CH + c, xv);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = sm.y[r * CH + c + j] + (a.D ? a.D[d0 + c + j] * xv[j] : 0.0f);
+        if (gz) {
+          float zv[V];
+          load_vec<T, V>(sm.z[buf] + r * CH + c, zv);
+#pragma unroll
+          for (int j = 0; j < V; ++j) o[j] *= zv[j] * sigmoid(zv[j]);
+        }
+        store_vec<T, V>(gout + (t0 + r) * a.out_t + c, o);
+      }
+    }
+  }
+  cp_async_wait<0>();
+  if (!kCarry) {
+    for (int t = max(t_lo, t_live); t < t_hi; ++t)
+      for (int c = threadIdx.x; c < nch; c += kThreads) gout[t * a.out_t + c] = from_f<T>(0.0f);
+  }
+  if (kCarry || (a.final_state && chunk == a.chunks - 1)) {
+    float* dst = kCarry ? a.carry + (static_cast<int64_t>(b) * a.chunks + chunk) * a.dim * a.N
+                        : a.final_state + static_cast<int64_t>(b) * a.dim * a.N;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (ch + k < nch) store_state4(dst + static_cast<int64_t>(d0 + ch + k) * a.N, n0, a.N, h[k]);
+  }
+  if (kCarry) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (nl == 0 && ch + k < nch) a.sumd[(static_cast<int64_t>(b) * a.chunks + chunk) * a.dim + d0 + ch + k] = sumd[k];
+    if (threadIdx.x == 0) a.cut[static_cast<int64_t>(b) * a.chunks + chunk] = any_cut;   // the same from every block
+  }
+}
+
+// carry[b, c] <- the state before chunk c. One thread per (b, d, n); kAhead chunks loaded at a time.
+__global__ void __launch_bounds__(256) carry_kernel(ScanArgs a) {
+  const int64_t per = static_cast<int64_t>(a.dim) * a.N;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (id >= per * a.batch) return;
+  const int b = static_cast<int>(id / per);
+  const int64_t dn = id - b * per;
+  const int d = static_cast<int>(dn / a.N);
+  const float A2 = a.A[dn] * kLog2e;
+  float h = a.state ? a.state[id] : 0.0f;
+  float* carry = a.carry + static_cast<int64_t>(b) * a.chunks * per + dn;
+  const float* sumd = a.sumd + static_cast<int64_t>(b) * a.chunks * a.dim + d;
+  const uint8_t* cut = a.cut + static_cast<int64_t>(b) * a.chunks;
+  constexpr int kAhead = 8;
+  for (int c = 0; c < a.chunks; c += kAhead) {
+    float e[kAhead], p[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (c + j < a.chunks) {
+        e[j] = carry[(c + j) * per];
+        p[j] = cut[c + j] ? 0.0f : exp2_hw(A2 * sumd[static_cast<int64_t>(c + j) * a.dim]);
+      }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (c + j < a.chunks) {
+        carry[(c + j) * per] = h;
+        h = cut[c + j] ? e[j] : fmaf(p[j], h, e[j]);
+      }
+  }
+}
+
+template <typename T, int LN, bool kAsync> int launch_scan(const ScanArgs& a, cudaStream_t s) {
+  using L = Layout<T, LN>;
+  const int bpg = static_cast<int>(surfk::ceil_div(a.dim / a.G, L::CH));
+  const int64_t gx = static_cast<int64_t>(bpg) * a.G * a.batch;
+  if (gx > 0x7fffffffLL || a.chunks > 65535) return static_cast<int>(cudaErrorInvalidValue);
+  constexpr size_t smem = sizeof(typename L::Smem);
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(a.chunks));
+  if (a.chunks > 1) {
+    if (const int rc = allow_smem<scan_kernel<T, LN, kAsync, true>>(smem)) return rc;
+    scan_kernel<T, LN, kAsync, true><<<grid, kThreads, smem, s>>>(a, bpg);
+    const int64_t n = static_cast<int64_t>(a.batch) * a.dim * a.N;
+    carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(n, 256)), 256, 0, s>>>(a);
+  }
+  if (const int rc = allow_smem<scan_kernel<T, LN, kAsync, false>>(smem)) return rc;
+  scan_kernel<T, LN, kAsync, false><<<grid, kThreads, smem, s>>>(a, bpg);
+  SURF_RETURN_LAUNCH();
+}
+
+// ---- single tokens -----------------------------------------------------------------------
+// Row r is the next token of the env in slot slots[r] of the state pool (-1: none, its output
+// is zero); the slot's state is moved on in place. LN lanes hold a channel's states.
+struct StepArgs {
+  const void *x, *dt, *z, *B, *C;
+  const float *A, *D, *bias;
+  float* pool;                                 // [slots, D, N]
+  const uint8_t* reset;                        // [rows] or null
+  const int* slots;                            // [rows] or null: row r is slot r
+  void* out;
+  int* err;
+  int64_t x_r, dt_r, z_r, B_r, B_g, C_r, C_g, out_r;
+  int rows, dim, N, G, softplus, n_slots;
+};
+
+template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel(StepArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int nl = lane & (LN - 1), n0 = nl * 4;
+  const int64_t id = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LN;
+  const bool in = id < static_cast<int64_t>(a.rows) * a.dim;
+  const int r = in ? static_cast<int>(id / a.dim) : 0;
+  const int d = in ? static_cast<int>(id - static_cast<int64_t>(r) * a.dim) : 0;
+  const int slot = a.slots ? a.slots[r] : r;
+  const bool bad = slot >= a.n_slots;
+  const bool on = in && slot >= 0 && !bad;
+  float acc[1] = {0.0f};
+  float x = 0.0f;
+  if (on) {
+    const int g = d / (a.dim / a.G);
+    x = to_f(static_cast<const T*>(a.x)[r * a.x_r + d]);
+    float dv = to_f(static_cast<const T*>(a.dt)[r * a.dt_r + d]) + (a.bias ? a.bias[d] : 0.0f);
+    if (a.softplus) dv = softplus(dv);
+    const float u = dv * x;
+    float* st = a.pool + (static_cast<int64_t>(slot) * a.dim + d) * a.N;
+    float4 h4 = a.reset && a.reset[r] ? make_float4(0.f, 0.f, 0.f, 0.f) : load_state4<LN>(st, n0, a.N);
+    const float4 A4 = load_state4<LN>(a.A + static_cast<int64_t>(d) * a.N, n0, a.N);
+    const T* B = static_cast<const T*>(a.B) + r * a.B_r + g * a.B_g;
+    const T* C = static_cast<const T*>(a.C) + r * a.C_r + g * a.C_g;
+    float h[4] = {h4.x, h4.y, h4.z, h4.w};
+    const float Av[4] = {A4.x, A4.y, A4.z, A4.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n0 + i < a.N) {
+        h[i] = fmaf(exp2_hw(dv * (Av[i] * kLog2e)), h[i], u * to_f(B[n0 + i]));
+        acc[0] = fmaf(h[i], to_f(C[n0 + i]), acc[0]);
+      }
+    }
+    store_state4(st, n0, a.N, h);
+  }
+#pragma unroll
+  for (int off = LN / 2; off >= 1; off /= 2) acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], off);
+  if (!in || nl != 0) return;
+  float o = 0.0f;
+  if (on) {
+    o = acc[0] + (a.D ? a.D[d] * x : 0.0f);
+    if (a.z) {
+      const float z = to_f(static_cast<const T*>(a.z)[r * a.z_r + d]);
+      o *= z * sigmoid(z);
+    }
+  } else if (bad) {
+    surfk::report_error(a.err, surfk::kErrSlotIndex);
+  }
+  static_cast<T*>(a.out)[r * a.out_r + d] = from_f<T>(o);
+}
+
+}  // namespace
+
+// aligned: the per-group channel count and N are whole 16-byte pieces, and so are all bases and strides
+SURF_EXPORT int surf_seq_scan(const void* args, int dtype, int aligned, void* stream) {
+  const ScanArgs a = *static_cast<const ScanArgs*>(args);
+  if (a.batch <= 0 || a.dim <= 0) return 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return by_lanes(a.N, [&](auto ln) {
+    constexpr int LN = decltype(ln)::value;
+    if (dtype == kBf16) return aligned ? launch_scan<bf16, LN, true>(a, s) : launch_scan<bf16, LN, false>(a, s);
+    return aligned ? launch_scan<float, LN, true>(a, s) : launch_scan<float, LN, false>(a, s);
+  });
+}
+
+SURF_EXPORT int surf_seq_scan_step(const void* args, int dtype, void* stream) {
+  const StepArgs a = *static_cast<const StepArgs*>(args);
+  if (a.rows <= 0 || a.dim <= 0) return 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return by_lanes(a.N, [&](auto ln) {
+    constexpr int LN = decltype(ln)::value;
+    const int64_t blocks = surfk::ceil_div(static_cast<int64_t>(a.rows) * a.dim * LN, 128);
+    if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
+    if (dtype == kBf16) step_kernel<bf16, LN><<<static_cast<unsigned>(blocks), 128, 0, s>>>(a);
+    else step_kernel<float, LN><<<static_cast<unsigned>(blocks), 128, 0, s>>>(a);
+    SURF_RETURN_LAUNCH();
+  });
+}
+
+SURF_EXPORT int surf_seq_args_size(int which) {
+  return static_cast<int>(which == 0 ? sizeof(ScanArgs) : sizeof(StepArgs));
+}

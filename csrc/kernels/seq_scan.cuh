@@ -1,0 +1,101 @@
+// seq_scan.cuh — arguments and thread layout shared by the selective scan's
+// forward (seq_scan.cu) and gradient (seq_scan_grad.cu).
+#pragma once
+#include <type_traits>
+
+#include "seq_common.cuh"
+
+namespace seqk {
+
+// States are kept for the gradient before every kSave-th token.
+constexpr int kSave = 8;
+
+// Everything 8 bytes wide first, then 32-bit numbers: the binding packs it flat.
+struct ScanArgs {
+  const void *x, *dt, *z, *B, *C, *dout;       // z null: no gate
+  const float *A, *D, *bias, *state, *dfinal;  // D, bias, state, dfinal may be null
+  const uint8_t* reset;                        // [B, T] or null
+  const int* lengths;                          // [B] or null
+  void* out;                                   // forward
+  float *final_state, *saved;                  // [B, D, N]; [B, ceil(T / kSave), D, N] (null: not kept)
+  float *carry, *sumd;                         // [B, chunks, D, N], [B, chunks, D]: length split only
+  uint8_t* cut;                                // [B, chunks]
+  void *dx, *ddt, *dz, *dB, *dC;               // gradient: dense [B, T, D] and [B, T, G, N]
+  float *part_bc;                              // [blocks of a group][B, T, G, 2 N]
+  float *part_a, *part_v;                      // [B * chunks][D, N], [B * chunks][2][D] (dD, ddt_bias)
+  float *dA, *dD, *dbias, *dstate;
+  int64_t x_b, x_t, dt_b, dt_t, z_b, z_t, B_b, B_t, B_g, C_b, C_t, C_g, do_b, do_t, out_b, out_t, r_b;
+  int batch, T, dim, N, G, softplus;
+  int chunk, chunks;                           // tokens of a chunk (a multiple of 16), chunks of a row
+};
+
+// A warp's 32 lanes are 32 / LN channel rows of LN lanes; a lane holds 4 states of
+// each of K channels, so 4 * LN >= N states of a channel sit in LN neighbouring lanes.
+template <int LN> __device__ __forceinline__ float4 load_state4(const float* p, int n0, int N) {
+  if ((N & 3) == 0) return n0 < N ? *reinterpret_cast<const float4*>(p + n0) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 v;
+  v.x = n0 + 0 < N ? p[n0 + 0] : 0.0f;
+  v.y = n0 + 1 < N ? p[n0 + 1] : 0.0f;
+  v.z = n0 + 2 < N ? p[n0 + 2] : 0.0f;
+  v.w = n0 + 3 < N ? p[n0 + 3] : 0.0f;
+  return v;
+}
+__device__ __forceinline__ void store_state4(float* p, int n0, int N, const float (&h)[4]) {
+  if ((N & 3) == 0) {
+    if (n0 < N) *reinterpret_cast<float4*>(p + n0) = make_float4(h[0], h[1], h[2], h[3]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n0 + i < N) p[n0 + i] = h[i];
+}
+
+// Sums v[0..K) over the LN lanes of a channel row, halving what a lane carries with
+// every exchange (K = 4, LN = 4: 3 exchanges instead of 8). Afterwards v[0] is the sum of
+// channel reduced_channel<LN, K>(lane); with LN > K several lanes hold the same one.
+template <int LN, int K> __device__ __forceinline__ void reduce_lanes(float (&v)[K], int lane) {
+  int k = K;
+#pragma unroll
+  for (int off = LN / 2; off >= 1; off /= 2) {
+    if (k > 1) {
+      k /= 2;
+#pragma unroll
+      for (int i = 0; i < K / 2; ++i) {
+        if (i < k) {
+          const bool up = lane & off;
+          const float give = up ? v[i] : v[i + k];
+          const float keep = up ? v[i + k] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+        }
+      }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+    }
+  }
+}
+template <int LN, int K> __device__ __forceinline__ int reduced_channel(int lane) {
+  int c = 0, k = K;
+#pragma unroll
+  for (int off = LN / 2; off >= 1; off /= 2)
+    if (k > 1) {
+      k /= 2;
+      if (lane & off) c += k;
+    }
+  return c;
+}
+// the lane that writes the channel's sum
+template <int LN, int K> __device__ __forceinline__ bool reduced_writer(int lane) {
+  return (lane & (LN / K - 1)) == 0;
+}
+
+// states -> lanes of a channel row; f gets the count as a compile-time constant
+template <typename F> int by_lanes(int N, F f) {
+  if (N < 1 || N > 64) return static_cast<int>(cudaErrorInvalidValue);
+  if (N <= 4) return f(std::integral_constant<int, 1>{});
+  if (N <= 8) return f(std::integral_constant<int, 2>{});
+  if (N <= 16) return f(std::integral_constant<int, 4>{});
+  if (N <= 32) return f(std::integral_constant<int, 8>{});
+  return f(std::integral_constant<int, 16>{});
+}
+
+}  // namespace seqk

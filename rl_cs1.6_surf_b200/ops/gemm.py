@@ -58,7 +58,7 @@ _err_flags: dict = {}
 ERROR_CODES = {1: "GEMM producer wait timed out", 2: "GEMM MMA wait timed out", 3: "GEMM epilogue wait timed out",
                4: "GEMM accumulator wait timed out", 5: "GEMM resident-operand wait timed out",
                0x100: "row gather index out of range", 0x101: "frame-stack index out of range",
-               0x102: "PPO loss sample index out of range"}
+               0x102: "PPO loss sample index out of range", 0x103: "state slot index out of range"}
 
 
 def error_flag(device) -> torch.Tensor:

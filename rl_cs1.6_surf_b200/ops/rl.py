@@ -22,6 +22,7 @@ import torch
 from . import _lib
 from ..rewards import spec as _spec  # noqa: F401  (registers surf_permutation_pool of libsurf_rl.so)
 from . import gemm as _gemm  # noqa: F401  (registers the libsurf_nn.so signatures the optimizer uses)
+from . import ssm as _ssm, tokens as _tokens  # noqa: F401  (register the libsurf_seq.so signatures)
 from ._lib import check, ptr, stream_ptr
 
 RLIB = "libsurf_rl.so"

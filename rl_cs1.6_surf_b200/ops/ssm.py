@@ -1,0 +1,499 @@
+"""Sequence operators of a policy's memory core (csrc/kernels/seq_conv.cu,
+seq_scan.cu, seq_scan_grad.cu) and their PyTorch oracles.
+
+* ``causal_conv`` — short depthwise convolution over the tokens of a row, SiLU
+  behind it;
+* ``selective_scan`` — the selective state space recurrence
+  h <- exp(delta A) h + delta x B, out = (C . h + D x) silu(z);
+
+each over whole sequences [B, T, ...], with its gradient (``*_grad``), and for
+single tokens of many envs (``*_step``: one state per slot of a pool, moved on in
+place). The weights are float32; tokens and windows are bfloat16 or float32, the
+scan's state always float32.
+
+``reset`` [B, T] (bool or uint8) empties window and state before the marked tokens
+(episode starts); ``lengths`` [B] (int32) says how many tokens of a row are there:
+the others give zeros, change nothing and are never read. ``state`` is what the row
+starts from (None: empty), ``final`` what the next call starts from.
+
+Inputs may be strided views (slices of a projection) as long as the last axis is
+dense; 16-byte aligned rows are copied asynchronously, others element by element.
+"""
+from __future__ import annotations
+
+import struct
+from collections import namedtuple
+from ctypes import c_char_p
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import KernelError, check, stream_ptr
+from .gemm import error_flag
+
+SLIB = "libsurf_seq.so"
+_V, _I, _L = _lib._V, _lib._I, _lib._L
+_lib.register(SLIB, {
+    "surf_seq_conv": (_I, [c_char_p, _I, _I, _I, _V]),
+    "surf_seq_conv_grad": (_I, [c_char_p, _I, _I, _I, _I, _V, _V, _V]),
+    "surf_seq_conv_step": (_I, [_V, _L, _V, _V, _V, _V, _V, _I, _V, _L, _I, _I, _I, _I, _I, _I, _V, _V]),
+    "surf_seq_scan": (_I, [c_char_p, _I, _I, _V]),
+    "surf_seq_scan_grad": (_I, [c_char_p, _I, _I, _V]),
+    "surf_seq_scan_grad_blocks": (_I, [_I, _I]),
+    "surf_seq_scan_step": (_I, [c_char_p, _I, _V]),
+    "surf_seq_args_size": (_I, [_I]),
+})
+_lib._KERNELS_PER_CALL["surf_seq_conv_grad"] = 2
+
+MAX_WIDTH, MAX_STATE, SAVE_EVERY = 4, 64, 8
+
+ConvGrads = namedtuple("ConvGrads", "dx dweight dbias dstate")
+Scan = namedtuple("Scan", "out final saved")
+ScanGrads = namedtuple("ScanGrads", "dx ddt dz dB dC dA dD ddt_bias dstate")
+
+_CONV = struct.Struct("18q6i")
+_SCAN = struct.Struct("48q8i")
+_STEP = struct.Struct("21q6i")
+
+
+def _p(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _dtype_code(t: torch.Tensor, what: str) -> int:
+    if t.dtype == torch.bfloat16:
+        return 1
+    if t.dtype == torch.float32:
+        return 0
+    raise TypeError(f"{what}: tokens must be bfloat16 or float32, not {t.dtype}")
+
+
+def _tokens(what: str, name: str, t: Optional[torch.Tensor], shape: tuple, like: torch.Tensor) -> None:
+    """An input with the tokens' type: shape, type, device and a dense last axis."""
+    if t is None:
+        return
+    if t.shape != shape:
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != like.dtype:
+        raise TypeError(f"{what}: {name} is {t.dtype}, the tokens are {like.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{what}: {name} is on {t.device}, the tokens on {like.device}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{what}: {name} needs a dense last axis")
+
+
+def _dense(what: str, name: str, t: Optional[torch.Tensor], shape: tuple, dtype, device) -> None:
+    """A contiguous input (weights, states, masks)."""
+    if t is None:
+        return
+    if t.shape != shape:
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, the tokens on {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous")
+
+
+def _flags(what: str, t: Optional[torch.Tensor], shape: tuple, device) -> None:
+    if t is None:
+        return
+    if t.dtype != torch.bool and t.dtype != torch.uint8:
+        raise TypeError(f"{what}: reset must be bool or uint8, not {t.dtype}")
+    _dense(what, "reset", t, shape, t.dtype, device)
+
+
+def _on_device(t: torch.Tensor):
+    """Launches go to the tensors' device, whatever the current one is."""
+    return torch.cuda.device(t.device)
+
+
+def _aligned(elems: int, *tensors) -> bool:
+    """Every row of the tensors starts on a boundary of ``elems`` elements."""
+    bytes_, bits = 0, 0
+    for t in tensors:
+        if t is not None:
+            bytes_ |= t.data_ptr() // t.element_size() | (t.data_ptr() % t.element_size())
+            for n, s in zip(t.shape[:-1], t.stride()):
+                if n > 1:
+                    bits |= s
+    return (bytes_ | bits) % elems == 0
+
+
+# ---- causal convolution -----------------------------------------------------------
+def _conv_check(what, x, weight, bias, state, reset, lengths):
+    _lib.require_cuda(x, what)
+    if x.dim() != 3:
+        raise ValueError(f"{what}: x must be [batch, tokens, channels]")
+    code = _dtype_code(x, what)
+    b, t, d = x.shape
+    if weight.dim() != 2 or not 2 <= weight.shape[1] <= MAX_WIDTH:
+        raise ValueError(f"{what}: weight must be [channels, width] with a width of 2 to {MAX_WIDTH}")
+    w = weight.shape[1]
+    _tokens(what, "x", x, x.shape, x)
+    _dense(what, "weight", weight, (d, w), torch.float32, x.device)
+    _dense(what, "bias", bias, (d,), torch.float32, x.device)
+    _dense(what, "state", state, (b, w - 1, d), x.dtype, x.device)
+    _flags(what, reset, (b, t), x.device)
+    _dense(what, "lengths", lengths, (b,), torch.int32, x.device)
+    return code, b, t, d, w
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                state: Optional[torch.Tensor] = None, reset: Optional[torch.Tensor] = None,
+                lengths: Optional[torch.Tensor] = None, silu: bool = True, out: Optional[torch.Tensor] = None):
+    """(y [B, T, D], final [B, W-1, D]): y[t] = silu(bias + sum_k weight[:, k] x[t - (W-1) + k])
+    over the tokens that t sees; ``state`` and ``final`` hold the W - 1 tokens before
+    and behind the row, oldest first."""
+    what = "causal_conv"
+    code, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
+    if out is None:
+        out = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+    else:
+        _tokens(what, "out", out, x.shape, x)
+    final = torch.empty((b, w - 1, d), dtype=x.dtype, device=x.device)
+    if b == 0 or d == 0:
+        return out, final
+    vec = d % 4 == 0 and _aligned(4, x, out, state)
+    tt = 16
+    args = _CONV.pack(_p(x), 0, _p(state), 0, _p(weight), _p(bias), _p(reset), _p(lengths), out.data_ptr(),
+                      final.data_ptr(), 0, x.stride(0), x.stride(1), 0, 0, out.stride(0), out.stride(1), t,
+                      b, t, d, int(silu), tt, max(1, -(-t // tt)))
+    with _on_device(x):
+        check(_lib.lib(SLIB).surf_seq_conv(args, code, w, int(vec), stream_ptr(x.device)), "surf_seq_conv")
+    return out, final
+
+
+def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                     state: Optional[torch.Tensor] = None, reset: Optional[torch.Tensor] = None,
+                     lengths: Optional[torch.Tensor] = None, silu: bool = True,
+                     dfinal: Optional[torch.Tensor] = None) -> ConvGrads:
+    """Gradients of ``causal_conv`` for the gradient ``dy`` of y and ``dfinal`` of
+    final (None: zero): dx and dstate in the tokens' type, dweight and dbias float32."""
+    what = "causal_conv_grad"
+    code, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
+    _tokens(what, "dy", dy, x.shape, x)
+    _dense(what, "dfinal", dfinal, (b, w - 1, d), x.dtype, x.device)
+    dev = x.device
+    dx = torch.empty((b, t, d), dtype=x.dtype, device=dev)
+    dstate = torch.empty((b, w - 1, d), dtype=x.dtype, device=dev) if state is not None else None
+    if b == 0 or d == 0:
+        return ConvGrads(dx, torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dstate)
+    dw = torch.empty((d, w), dtype=torch.float32, device=dev)
+    db = torch.empty(d, dtype=torch.float32, device=dev) if bias is not None else None
+    vec = d % 4 == 0 and _aligned(4, x, dy, state, dfinal)
+    tt = 16
+    chunks = max(1, -(-t // tt))
+    groups = d // 4 if vec else d
+    bx = min(32, 1 << (groups - 1).bit_length())
+    # rows of partial sums: about four blocks per SM, none without work
+    rows = max(1, min(-(-b * chunks // (256 // bx)), -(-592 // -(-groups // bx))))
+    part = torch.empty((rows, w + 1, d), dtype=torch.float32, device=dev)
+    args = _CONV.pack(_p(x), dy.data_ptr(), _p(state), _p(dfinal), _p(weight), _p(bias), _p(reset), _p(lengths),
+                      dx.data_ptr(), _p(dstate), part.data_ptr(), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1),
+                      t * d, d, t, b, t, d, int(silu), tt, chunks)
+    with _on_device(x):
+        check(_lib.lib(SLIB).surf_seq_conv_grad(args, code, w, int(vec), rows, _p(dw), _p(db), stream_ptr(dev)),
+              "surf_seq_conv_grad")
+    return ConvGrads(dx, dw, db, dstate)
+
+
+def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], state: torch.Tensor, *,
+                     reset: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None, silu: bool = True,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token x [R, D] for each of R envs: y [R, D]. ``state`` [S, W-1, D] is the pool
+    of windows, ``slots`` [R] (int32) each row's place in it (None: row r is slot r; below
+    0: no env, its output is zero), moved on in place. No two rows may name one slot."""
+    what = "causal_conv_step"
+    _lib.require_cuda(x, what)
+    if x.dim() != 2:
+        raise ValueError(f"{what}: x must be [rows, channels]")
+    code = _dtype_code(x, what)
+    r, d = x.shape
+    dev = x.device
+    if weight.dim() != 2 or not 2 <= weight.shape[1] <= MAX_WIDTH:
+        raise ValueError(f"{what}: weight must be [channels, width] with a width of 2 to {MAX_WIDTH}")
+    w = weight.shape[1]
+    _tokens(what, "x", x, x.shape, x)
+    _dense(what, "weight", weight, (d, w), torch.float32, dev)
+    _dense(what, "bias", bias, (d,), torch.float32, dev)
+    _dense(what, "state", state, (state.shape[0], w - 1, d), x.dtype, dev)
+    _flags(what, reset, (r,), dev)
+    _dense(what, "slots", slots, (r,), torch.int32, dev)
+    if slots is None and state.shape[0] < r:
+        raise ValueError(f"{what}: {r} rows, but {state.shape[0]} slots")
+    if out is None:
+        out = torch.empty((r, d), dtype=x.dtype, device=dev)
+    else:
+        _tokens(what, "out", out, x.shape, x)
+    if r == 0 or d == 0:
+        return out
+    vec = d % 4 == 0 and _aligned(4, x, out, state)
+    with _on_device(x):
+        check(_lib.lib(SLIB).surf_seq_conv_step(
+            x.data_ptr(), x.stride(0), weight.data_ptr(), _p(bias), state.data_ptr(), _p(reset), _p(slots),
+            state.shape[0], out.data_ptr(), out.stride(0), r, d, w, int(silu), code, int(vec),
+            error_flag(dev).data_ptr(), stream_ptr(dev)), "surf_seq_conv_step")
+    return out
+
+
+# ---- selective scan ---------------------------------------------------------------
+def _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths):
+    _lib.require_cuda(x, what)
+    if x.dim() != 3:
+        raise ValueError(f"{what}: x must be [batch, tokens, channels]")
+    code = _dtype_code(x, what)
+    b, t, d = x.shape
+    dev = x.device
+    if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATE:
+        raise ValueError(f"{what}: A must be [channels, states] with 1 to {MAX_STATE} states")
+    n = A.shape[1]
+    if B.dim() != 4 or B.shape[2] < 1 or d % B.shape[2]:
+        raise ValueError(f"{what}: B must be [batch, tokens, groups, states], its groups dividing the channels")
+    g = B.shape[2]
+    for name, v in (("x", x), ("dt", dt), ("z", z)):
+        _tokens(what, name, v, (b, t, d), x)
+    for name, v in (("B", B), ("C", C)):
+        _tokens(what, name, v, (b, t, g, n), x)
+    f32 = torch.float32
+    _dense(what, "A", A, (d, n), f32, dev)
+    _dense(what, "D", D, (d,), f32, dev)
+    _dense(what, "dt_bias", dt_bias, (d,), f32, dev)
+    _dense(what, "state", state, (b, d, n), f32, dev)
+    _flags(what, reset, (b, t), dev)
+    _dense(what, "lengths", lengths, (b,), torch.int32, dev)
+    return code, b, t, d, n, g
+
+
+def _scan_aligned(d, g, n, x, *tensors) -> bool:
+    """16-byte pieces throughout: a group's channels, its states and every row."""
+    v = 16 // x.element_size()
+    return (d // g) % v == 0 and n % v == 0 and _aligned(v, x, *tensors)
+
+
+def _chunks(b: int, t: int, d: int, n: int, g: int):
+    """(tokens of a chunk, chunks): a row is cut only where its channels do not fill the GPU."""
+    lanes = 1 if n <= 4 else 2 if n <= 8 else 4 if n <= 16 else 8 if n <= 32 else 16
+    per_block = 128 // lanes * min(lanes, 4)
+    blocks = b * g * -(-(d // g) // per_block)
+    want = max(1, min(592 // blocks if blocks else 1, t // 64))
+    if want <= 1:
+        return max(16, -(-t // 16) * 16), 1
+    chunk = -(-t // want)
+    chunk = -(-chunk // 16) * 16
+    return chunk, -(-t // chunk)
+
+
+def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+                   D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                   dt_bias: Optional[torch.Tensor] = None, softplus: bool = True,
+                   state: Optional[torch.Tensor] = None, reset: Optional[torch.Tensor] = None,
+                   lengths: Optional[torch.Tensor] = None, train: bool = False,
+                   out: Optional[torch.Tensor] = None) -> Scan:
+    """The recurrence over x, dt, z [B, T, D], B, C [B, T, G, N] (each group of D / G
+    channels shares a row of them), A [D, N]: ``out`` [B, T, D] and ``final`` [B, D, N].
+    delta = softplus(dt + dt_bias), or the sum itself with ``softplus=False``. ``train``
+    keeps in ``saved`` the states that ``selective_scan_grad`` starts from: 4 D N bytes
+    for every 8 tokens."""
+    what = "selective_scan"
+    code, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
+    dev = x.device
+    if out is None:
+        out = torch.empty((b, t, d), dtype=x.dtype, device=dev)
+    else:
+        _tokens(what, "out", out, x.shape, x)
+    final = torch.empty((b, d, n), dtype=torch.float32, device=dev)
+    saved = torch.empty((b, -(-t // SAVE_EVERY), d, n), dtype=torch.float32, device=dev) if train else None
+    if b == 0 or d == 0:
+        return Scan(out, final, saved)
+    chunk, chunks = _chunks(b, t, d, n, g)
+    carry = sumd = cut = None
+    if chunks > 1:
+        carry = torch.empty((b, chunks, d, n), dtype=torch.float32, device=dev)
+        sumd = torch.empty((b, chunks, d), dtype=torch.float32, device=dev)
+        cut = torch.empty((b, chunks), dtype=torch.uint8, device=dev)
+    args = _SCAN.pack(
+        x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), 0, A.data_ptr(), _p(D), _p(dt_bias), _p(state), 0,
+        _p(reset), _p(lengths), out.data_ptr(), final.data_ptr(), _p(saved), _p(carry), _p(sumd), _p(cut),
+        0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+        x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
+        0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
+        0, 0, out.stride(0), out.stride(1), t, b, t, d, n, g, int(softplus), chunk, chunks)
+    aligned = _scan_aligned(d, g, n, x, dt, z, B, C, out)
+    with _on_device(x):
+        check(_lib.lib(SLIB).surf_seq_scan(args, code, int(aligned), stream_ptr(dev)), "surf_seq_scan")
+    if chunks > 1:
+        _lib.add_launches(2)
+    return Scan(out, final, saved)
+
+
+def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+                        C: torch.Tensor, *, saved: torch.Tensor, D: Optional[torch.Tensor] = None,
+                        z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None,
+                        softplus: bool = True, state: Optional[torch.Tensor] = None,
+                        reset: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                        dfinal: Optional[torch.Tensor] = None) -> ScanGrads:
+    """Gradients of ``selective_scan`` for the gradient ``dout`` of out and ``dfinal`` of
+    final (None: zero). The tokens' gradients come in the tokens' type (summed in 32 bits
+    first where heads share them), the weights' and the state's in float32; None for an
+    input that was None."""
+    what = "selective_scan_grad"
+    code, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
+    dev, f32 = x.device, torch.float32
+    _tokens(what, "dout", dout, x.shape, x)
+    _dense(what, "dfinal", dfinal, (b, d, n), f32, dev)
+    if saved is None:
+        raise ValueError(f"{what}: needs the states that selective_scan(train=True) saved")
+    _dense(what, "saved", saved, (b, -(-t // SAVE_EVERY), d, n), f32, dev)
+
+    def like(v, shape, dtype):
+        return None if v is None else torch.empty(shape, dtype=dtype, device=dev)
+
+    dx, ddt, dz = (like(v, (b, t, d), x.dtype) for v in (x, dt, z))
+    dB, dC = (like(v, (b, t, g, n), x.dtype) for v in (B, C))
+    dA, dD, dbias = like(A, (d, n), f32), like(D, (d,), f32), like(dt_bias, (d,), f32)
+    dstate = like(state, (b, d, n), f32)
+    if b == 0 or d == 0:
+        for v in (dA, dD, dbias):
+            if v is not None:
+                v.zero_()
+        return ScanGrads(dx, ddt, dz, dB, dC, dA, dD, dbias, dstate)
+    chunk, chunks = _chunks(b, t, d, n, g)
+    L = _lib.lib(SLIB)
+    carry = sumd = cut = None
+    if chunks > 1:
+        carry = torch.empty((b, chunks, d, n), dtype=f32, device=dev)
+        sumd = torch.empty((b, chunks, d), dtype=f32, device=dev)
+        cut = torch.empty((b, chunks), dtype=torch.uint8, device=dev)
+    part_bc = torch.empty(L.surf_seq_scan_grad_blocks(d // g, n) * b * t * g * 2 * n, dtype=f32, device=dev)
+    part_a = torch.empty(b * chunks * d * (n + 2), dtype=f32, device=dev)
+    args = _SCAN.pack(
+        x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), dout.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias),
+        _p(state), _p(dfinal), _p(reset), _p(lengths), 0, 0, saved.data_ptr(), _p(carry), _p(sumd), _p(cut),
+        dx.data_ptr(), ddt.data_ptr(), _p(dz), dB.data_ptr(), dC.data_ptr(), part_bc.data_ptr(), part_a.data_ptr(),
+        part_a.data_ptr() + 4 * b * chunks * d * n, dA.data_ptr(), _p(dD), _p(dbias), _p(dstate),
+        x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
+        0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
+        dout.stride(0), dout.stride(1), 0, 0, t, b, t, d, n, g, int(softplus), chunk, chunks)
+    aligned = _scan_aligned(d, g, n, x, dt, z, B, C, dout)
+    with _on_device(x):
+        check(L.surf_seq_scan_grad(args, code, int(aligned), stream_ptr(dev)), "surf_seq_scan_grad")
+    _lib.add_launches(4 if chunks > 1 else 2)
+    return ScanGrads(dx, ddt, dz, dB, dC, dA, dD, dbias, dstate)
+
+
+def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                        state: torch.Tensor, *, D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                        dt_bias: Optional[torch.Tensor] = None, softplus: bool = True,
+                        reset: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token for each of R envs: x, dt, z [R, D], B, C [R, G, N] -> out [R, D].
+    ``state`` [S, D, N] is the pool of states, ``slots`` [R] (int32) each row's place in
+    it (None: row r is slot r; below 0: no env, its output is zero), moved on in place.
+    No two rows may name one slot."""
+    what = "selective_scan_step"
+    _lib.require_cuda(x, what)
+    if x.dim() != 2:
+        raise ValueError(f"{what}: x must be [rows, channels]")
+    code = _dtype_code(x, what)
+    r, d = x.shape
+    dev = x.device
+    if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATE:
+        raise ValueError(f"{what}: A must be [channels, states] with 1 to {MAX_STATE} states")
+    n = A.shape[1]
+    if B.dim() != 3 or B.shape[1] < 1 or d % B.shape[1]:
+        raise ValueError(f"{what}: B must be [rows, groups, states], its groups dividing the channels")
+    g = B.shape[1]
+    for name, v in (("x", x), ("dt", dt), ("z", z)):
+        _tokens(what, name, v, (r, d), x)
+    for name, v in (("B", B), ("C", C)):
+        _tokens(what, name, v, (r, g, n), x)
+    f32 = torch.float32
+    _dense(what, "A", A, (d, n), f32, dev)
+    _dense(what, "D", D, (d,), f32, dev)
+    _dense(what, "dt_bias", dt_bias, (d,), f32, dev)
+    _dense(what, "state", state, (state.shape[0], d, n), f32, dev)
+    _flags(what, reset, (r,), dev)
+    _dense(what, "slots", slots, (r,), torch.int32, dev)
+    if slots is None and state.shape[0] < r:
+        raise ValueError(f"{what}: {r} rows, but {state.shape[0]} slots")
+    if out is None:
+        out = torch.empty((r, d), dtype=x.dtype, device=dev)
+    else:
+        _tokens(what, "out", out, x.shape, x)
+    if r == 0 or d == 0:
+        return out
+    args = _STEP.pack(x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias),
+                      state.data_ptr(), _p(reset), _p(slots), out.data_ptr(), error_flag(dev).data_ptr(), x.stride(0),
+                      dt.stride(0), 0 if z is None else z.stride(0), B.stride(0), B.stride(1), C.stride(0), C.stride(1),
+                      out.stride(0), r, d, n, g, int(softplus), state.shape[0])
+    with _on_device(x):
+        check(_lib.lib(SLIB).surf_seq_scan_step(args, code, stream_ptr(dev)), "surf_seq_scan_step")
+    return out
+
+
+# ---- oracles ------------------------------------------------------------------------
+def _real(lengths, b, t, device):
+    if lengths is None:
+        return torch.ones(b, t, dtype=torch.bool, device=device)
+    return torch.arange(t, device=device)[None, :] < lengths.to(device)[:, None]
+
+
+def causal_conv_reference(x, weight, bias=None, *, state=None, reset=None, lengths=None, silu=True):
+    """``causal_conv`` token by token, in the type of its inputs (differentiable)."""
+    b, t, d = x.shape
+    w = weight.shape[1]
+    real = _real(lengths, b, t, x.device)
+    past = [x.new_zeros(b, d) for _ in range(w - 1)] if state is None else [state[:, j] for j in range(w - 1)]
+    ys = []
+    for i in range(t):
+        on = real[:, i:i + 1]
+        seen = past
+        if reset is not None:
+            seen = [torch.where(reset[:, i:i + 1].bool(), torch.zeros_like(h), h) for h in past]
+        taps = seen + [torch.where(on, x[:, i], torch.zeros_like(x[:, i]))]
+        pre = sum(weight[:, k] * taps[k] for k in range(w))
+        if bias is not None:
+            pre = pre + bias
+        y = pre * torch.sigmoid(pre) if silu else pre
+        ys.append(torch.where(on, y, torch.zeros_like(y)))
+        past = [torch.where(on, taps[k + 1], past[k]) for k in range(w - 1)]
+    return (torch.stack(ys, 1) if ys else x.new_zeros(b, 0, d)), torch.stack(past, 1)
+
+
+def selective_scan_reference(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=True, state=None, reset=None,
+                             lengths=None):
+    """``selective_scan`` token by token, in the type of its inputs (differentiable):
+    (out, final)."""
+    b, t, d = x.shape
+    rep = d // B.shape[2]
+    real = _real(lengths, b, t, x.device)
+    h = x.new_zeros(b, d, A.shape[1]) if state is None else state
+    outs = []
+    for i in range(t):
+        on = real[:, i:i + 1]
+        off = torch.zeros_like(x[:, i])
+        xi, v = torch.where(on, x[:, i], off), torch.where(on, dt[:, i], off)
+        Bi, Ci = (torch.where(on[..., None], m[:, i], torch.zeros_like(m[:, i])).repeat_interleave(rep, 1) for m in (B, C))
+        if dt_bias is not None:
+            v = v + dt_bias
+        if softplus:
+            v = torch.nn.functional.softplus(v)
+        past = h if reset is None else torch.where(reset[:, i, None, None].bool(), torch.zeros_like(h), h)
+        new = torch.exp(v[..., None] * A) * past + (v * xi)[..., None] * Bi
+        h = torch.where(on[..., None], new, h)
+        y = (h * Ci).sum(-1)
+        if D is not None:
+            y = y + D * xi
+        if z is not None:
+            zi = torch.where(on, z[:, i], off)
+            y = y * zi * torch.sigmoid(zi)
+        outs.append(torch.where(on, y, torch.zeros_like(y)))
+    return (torch.stack(outs, 1) if outs else x.new_zeros(b, 0, d)), h
+
+
+__all__ = ["causal_conv", "causal_conv_grad", "causal_conv_step", "selective_scan", "selective_scan_grad",
+           "selective_scan_step", "causal_conv_reference", "selective_scan_reference", "ConvGrads", "Scan", "ScanGrads",
+           "KernelError"]

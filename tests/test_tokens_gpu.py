@@ -1,0 +1,154 @@
+"""The answer sampler against its rule by sorting: the same answers (whole numbers of
+weight make every sum exact, so they are equal, not close), log-probabilities to two
+roundings of 32 bits; empty rows, ties, infinities, NaN, limits per row; frequencies."""
+import pytest
+import torch
+
+from surfb200.models.policy import HeadLayout
+from surfb200.ops import _lib
+from surfb200.ops import tokens as TK
+
+pytestmark = pytest.mark.gpu
+
+
+def _same(logits, u, **kw):
+    tok, logp = TK.sample_tokens(logits, u, **kw)
+    # the rule's exponential on the same device, so that weights are the same numbers
+    et, ep = _by_rule(logits, u, **kw)
+    assert torch.equal(tok, et)
+    assert torch.allclose(logp, ep, rtol=2.0 ** -22, atol=1e-6)
+    assert torch.equal(torch.isinf(logp), tok < 0)
+    return tok, logp
+
+
+def _by_rule(logits, u, **kw):
+    """sample_tokens_reference with the exponentials of the GPU."""
+    keep = torch.exp
+
+    def gpu_exp(x):
+        return keep(x.cuda()).cpu() if x.dtype == torch.float32 else keep(x)
+
+    torch.exp = gpu_exp
+    try:
+        cpu = {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+        t, p = TK.sample_tokens_reference(logits.cpu(), u.cpu(), **cpu)
+    finally:
+        torch.exp = keep
+    return t.cuda(), p.cuda()
+
+
+RULES = [dict(), dict(top_k=1), dict(top_k=5), dict(top_p=0.9), dict(top_p=0.5, top_k=40), dict(min_p=0.1),
+         dict(temperature=0.0), dict(temperature=0.3, top_p=0.99, min_p=0.01), dict(temperature=3.0, top_k=1000, top_p=0.7),
+         dict(top_p=0.0), dict(min_p=1.0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rule", RULES, ids=str)
+@pytest.mark.parametrize("rows,vocab", [(5, 2), (7, 31), (3, 33), (4, 1000), (2, 8193), (1, 40001)])
+def test_equals_the_rule(rows, vocab, rule, dtype):
+    gen = torch.Generator("cuda").manual_seed(rows * vocab)
+    z = (3 * torch.randn(rows, vocab + 3, generator=gen, device="cuda")).to(dtype)[:, 1:vocab + 1]
+    z[torch.rand(rows, vocab, generator=gen, device="cuda") < 0.1] = float("-inf")
+    u = torch.rand(rows, 1, generator=gen, device="cuda")
+    _same(z, u, **rule)
+
+
+@pytest.mark.parametrize("vocab", [9, 3000, 20000, 131072])
+def test_ties_go_to_the_lowest_index(vocab):
+    z = torch.zeros(4, vocab, device="cuda")
+    z[1, vocab // 2:] = -0.0                                    # equal to +0
+    z[2] = torch.arange(vocab, device="cuda") % 3
+    z[3, :vocab // 2] = -1.0
+    for rule in (dict(top_k=4), dict(top_p=0.25), dict(top_k=vocab // 2 + 1, top_p=0.5), dict(temperature=0.0), dict()):
+        for q in (0.0, 0.37, 0.9999):
+            _same(z, torch.full((4, 1), q, device="cuda"), **rule)
+    tok, _ = TK.sample_tokens(z, torch.full((4, 1), 0.9999, device="cuda"), top_k=2)
+    assert tok[:, 0].tolist() == [1, 1, 5, vocab // 2 + 1]
+
+
+@pytest.mark.parametrize("vocab", [20, 5000])
+def test_empty_rows_infinities_and_nan(vocab):
+    inf = float("inf")
+    z = torch.zeros(6, vocab, device="cuda")
+    z[0] = -inf
+    z[1] = float("nan")
+    z[2, :] = -inf
+    z[2, 7] = torch.finfo(torch.float32).min                     # the only candidate
+    z[3, 3] = z[3, 9] = inf                                      # share everything
+    z[4, ::2] = float("nan")
+    z[5] = torch.finfo(torch.float32).min                        # masked by the lowest value: all equal
+    for rule in (dict(), dict(top_k=3), dict(top_p=0.9), dict(top_k=3, top_p=0.4, min_p=0.2)):
+        tok, logp = _same(z, torch.full((6, 1), 0.6, device="cuda"), **rule)
+        assert tok[:3, 0].tolist() == [-1, -1, 7] and logp[2, 0] == 0
+        assert tok[3, 0] in (3, 9) and tok[4, 0] % 2 == 1
+
+
+def test_limits_per_row():
+    gen = torch.Generator("cuda").manual_seed(1)
+    z = 2 * torch.randn(8, 700, generator=gen, device="cuda")
+    u = torch.rand(8, 1, generator=gen, device="cuda")
+    r = torch.arange(8, device="cuda")
+    _same(z, u, temperature=0.2 * r.float(), top_k=(r * 3).int(), top_p=1 - 0.1 * r.float(), min_p=0.02 * r.float())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_heads(dtype):
+    layout = HeadLayout()
+    gen = torch.Generator("cuda").manual_seed(2)
+    z = torch.randn(300, 64, generator=gen, device="cuda").to(dtype)
+    u = torch.rand(300, len(layout.sizes), generator=gen, device="cuda")
+    for rule in RULES:
+        tok, _ = _same(z, u, heads=layout.sizes, **rule)
+        assert (tok < torch.tensor(layout.sizes, device="cuda")).all()
+    big = torch.randn(3, 200, generator=gen, device="cuda").to(dtype)
+    _same(big, u[:3, :3].contiguous(), heads=(100, 1, 60), top_p=0.8)
+
+
+def test_numbers_at_the_ends():
+    z = torch.randn(1, 100, device="cuda").expand(4, 100)
+    u = torch.tensor([[0.0], [1.0 - 2.0 ** -24], [1.0], [-1.0]], device="cuda")
+    tok, _ = TK.sample_tokens(z, u)
+    assert tok[:, 0].tolist() == [0, 99, 99, 0]
+
+
+def test_frequencies():
+    """200,000 draws of 50 answers under top-p: each count within 6 standard deviations
+    (a chance of about 1e-7 for all of them)."""
+    gen = torch.Generator("cuda").manual_seed(5)
+    z = 1.5 * torch.randn(50, generator=gen, device="cuda")
+    n = 200_000
+    tok, logp = TK.sample_tokens(z.expand(n, 50), torch.rand(n, 1, generator=gen, device="cuda"), temperature=0.9, top_p=0.9)
+    p = torch.softmax(z.double() / 0.9, 0)
+    order = torch.argsort(p, descending=True)
+    kept = torch.zeros(50, dtype=torch.bool, device="cuda")
+    kept[order] = (p[order].cumsum(0) - p[order]) < 0.9
+    q = torch.where(kept, p, 0.0) / p[kept].sum()
+    count = torch.bincount(tok[:, 0].long(), minlength=50).double()
+    assert ((count - n * q).abs() <= 6 * (n * q * (1 - q)).sqrt() + 1e-9).all()
+    assert torch.allclose(logp[:, 0].double(), q[tok[:, 0].long()].log(), atol=1e-5)
+
+
+def test_outputs_in_place_and_refusals():
+    z = torch.randn(3, 40, device="cuda")
+    u = torch.rand(3, 1, device="cuda")
+    out = torch.empty(3, 1, dtype=torch.int32, device="cuda")
+    logp = torch.empty(3, 1, device="cuda")
+    a, b = TK.sample_tokens(z, u, out=out, logp=logp)
+    assert a is out and b is logp
+    assert TK.sample_tokens(z[:0], u[:0])[0].shape == (0, 1)
+    with pytest.raises(_lib.KernelError):
+        TK.sample_tokens(z.cpu(), u.cpu())
+    with pytest.raises(TypeError, match="bfloat16 or float32"):
+        TK.sample_tokens(z.half(), u)
+    with pytest.raises(ValueError, match="u must be"):
+        TK.sample_tokens(z, u[:2])
+    with pytest.raises(ValueError, match="dense last axis"):
+        TK.sample_tokens(z.t(), torch.rand(40, 1, device="cuda"))
+    with pytest.raises(ValueError, match="heads"):
+        TK.sample_tokens(z, u, heads=(41,))
+    with pytest.raises(ValueError, match="negative"):
+        TK.sample_tokens(z, u, top_p=1.5)
+    with pytest.raises(ValueError, match="top_k must be"):
+        TK.sample_tokens(z, u, top_k=torch.ones(3, device="cuda"))
+    with pytest.raises(ValueError, match="at most"):
+        TK.sample_tokens(torch.empty(1, TK.MAX_VOCAB + 1, device="cuda"), u[:1])
