@@ -62,23 +62,36 @@ template <int N> __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// dst[r][0, cols) = src[r * stride + (0, cols)] for `rows` rows (dst row pitch:
-// `pitch` elements), by all NT threads. kAsync: 16-byte pieces (cols, pitch and
-// stride are multiples of a piece, both bases aligned), in flight on return;
-// else element by element, done on return.
-template <typename T, int NT, bool kAsync>
-__device__ __forceinline__ void copy_rows(T* dst, int pitch, const T* src, int64_t stride, int rows, int cols) {
-  if constexpr (kAsync) {
-    constexpr int V = kVec16<T>;
-    const int per = cols / V;
-    for (int i = threadIdx.x; i < rows * per; i += NT) {
-      const int r = i / per, c = (i - r * per) * V;
-      cp_async16(dst + r * pitch + c, src + r * stride + c);
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
+}
+
+// How rows may be copied: pieces of 16 or 4 bytes (bases, strides and the row's length
+// are multiples of it), else element by element.
+enum : int { kPlain = 0, kPieces4 = 4, kPieces16 = 16 };
+
+// dst[r][0, cols) = src[r * stride + (0, cols)] for `rows` rows of pitch P, by all NT
+// threads; in pieces it is still in flight on return.
+template <typename T, int NT, int P>
+__device__ __forceinline__ void copy_rows(T* dst, const T* src, int64_t stride, int rows, int cols, int mode) {
+  if (mode == kPieces16) {
+    constexpr int V = kVec16<T>, W = (P + V - 1) / V;
+    for (int i = threadIdx.x; i < rows * W; i += NT) {
+      const int r = i / W, c = (i - r * W) * V;
+      if (c < cols) cp_async16(dst + r * P + c, src + r * stride + c);
+    }
+  } else if (mode == kPieces4) {
+    constexpr int V = 4 / static_cast<int>(sizeof(T)), W = P / V;
+    for (int i = threadIdx.x; i < rows * W; i += NT) {
+      const int r = i / W, c = (i - r * W) * V;
+      if (c < cols) cp_async4(dst + r * P + c, src + r * stride + c);
     }
   } else {
-    for (int i = threadIdx.x; i < rows * cols; i += NT) {
-      const int r = i / cols, c = i - r * cols;
-      dst[r * pitch + c] = src[r * stride + c];
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows * P; i += NT) {
+      const int r = i / P, c = i - r * P;
+      if (c < cols) dst[i] = src[r * stride + c];
     }
   }
 }
@@ -107,7 +120,50 @@ __device__ __forceinline__ float exp2_hw(float x) {
 }
 __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + exp2_hw(-kLog2e * v)); }
 
-// log(1 + e^v)
-__device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
+// log(1 + e^v) = max(v, 0) + log(1 + e^-|v|); with s = e / (2 + e) <= 1/3 the logarithm is
+// 2 atanh(s) = 2 s g(s^2), g fitted on [0, 1/9] to 4e-9: as exact for small e as for e = 1.
+__device__ __forceinline__ float softplus(float v) {
+  const float e = exp2_hw(-kLog2e * fabsf(v));
+  const float s = __fdividef(e, 2.0f + e), q = s * s;
+  float g = fmaf(q, 0.14089155197143555f, 0.13980303704738617f);
+  g = fmaf(g, q, 0.20012454688549042f);
+  g = fmaf(g, q, 0.3333315849304199f);
+  g = fmaf(g, q, 1.0f);
+  return fmaf(2.0f * s, g, fmaxf(v, 0.0f));
+}
 
+// ---- pairs of floats in one 64-bit register: one instruction for both ---------------
+struct f2 { unsigned long long v; };
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+// four floats of shared memory as two pairs
+__device__ __forceinline__ void load_pairs(const float* p, f2& a, f2& b) {
+  const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(p);
+  a.v = q.x;
+  b.v = q.y;
+}
+__device__ __forceinline__ f2 exp2_hw2(f2 x) {
+  float lo, hi;
+  unpack2(x, lo, hi);
+  return pack2(exp2_hw(lo), exp2_hw(hi));
+}
 }  // namespace seqk

@@ -25,21 +25,25 @@ constexpr int kTile = 16;
 constexpr int kThreads = 128;
 
 template <typename T, int LN> struct Layout {
-  static constexpr int K = LN < 4 ? LN : 4;              // channels of a thread
+  static constexpr int K = LN < 4 ? 2 : 4;               // channels of a thread, taken in pairs
   static constexpr int CH = kThreads / LN * K;           // channels of a block
   static constexpr int NP = 4 * LN;                      // states, padded
   struct Smem {
     alignas(16) T x[2][kTile * CH], dt[2][kTile * CH], z[2][kTile * CH], B[2][kTile * NP], C[2][kTile * NP];
-    alignas(16) float delta[kTile * CH], u[kTile * CH], y[kTile * CH], Bf[kTile * NP], Cf[kTile * NP];
-    int cut[kTile];
+    alignas(16) float delta[kTile * CH], u[kTile * CH];  // u: delta * x, then y = C . h of the token
+    alignas(16) float Bd[kTile * NP * 2], Cd[kTile * NP * 2];    // 32-bit, every value twice
   };
 };
 
 // kCarry: only the chunk's end state from an empty start and its sum of delta.
-template <typename T, int LN, bool kAsync, bool kCarry>
+//
+// The recurrence of a token costs 4 multiply-adds and an exponential per state. Two
+// channels share an instruction (f32x2), which leaves the exponential unit's 16 a cycle
+// and SM as the bound.
+template <typename T, int LN, bool kCarry>
 __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_per_group) {
   using L = Layout<T, LN>;
-  constexpr int K = L::K, CH = L::CH, NP = L::NP;
+  constexpr int K = L::K, P = K / 2, CH = L::CH, NP = L::NP;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   typename L::Smem& sm = *reinterpret_cast<typename L::Smem*>(smem_raw);
   const int blocks = blocks_per_group * a.G;
@@ -58,22 +62,46 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
   const int ch = threadIdx.x / LN * K;                   // the thread's first channel within the block
   const int n0 = nl * 4;
 
-  float A2[K][4], h[K][4], sumd[K];
+  f2 A2[P][4], h[P][4], sumd[P];                         // pairs of channels (ch + 2 p, ch + 2 p + 1)
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const bool on = ch + k < nch;
-    const int64_t row = static_cast<int64_t>(d0 + ch + k) * a.N;
-    const float4 v = on ? load_state4<LN>(a.A + row, n0, a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
-    A2[k][0] = v.x * kLog2e; A2[k][1] = v.y * kLog2e; A2[k][2] = v.z * kLog2e; A2[k][3] = v.w * kLog2e;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!kCarry && on) {
-      const int64_t bd = static_cast<int64_t>(a.dim) * a.N;
-      if (a.chunks > 1) s = load_state4<LN>(a.carry + (static_cast<int64_t>(b) * a.chunks + chunk) * bd + row, n0, a.N);
-      else if (a.state) s = load_state4<LN>(a.state + b * bd + row, n0, a.N);
+  for (int p = 0; p < P; ++p) {
+    float4 av[2], hv[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool on = ch + 2 * p + e < nch;
+      const int64_t row = static_cast<int64_t>(d0 + ch + 2 * p + e) * a.N, bd = static_cast<int64_t>(a.dim) * a.N;
+      av[e] = hv[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (on) {
+        av[e] = load_state4(a.A + row, n0, a.N);
+        if (!kCarry) {
+          if (a.chunks > 1) hv[e] = load_state4(a.carry + (static_cast<int64_t>(b) * a.chunks + chunk) * bd + row, n0, a.N);
+          else if (a.state) hv[e] = load_state4(a.state + b * bd + row, n0, a.N);
+        }
+      }
     }
-    h[k][0] = s.x; h[k][1] = s.y; h[k][2] = s.z; h[k][3] = s.w;
-    sumd[k] = 0.0f;
+    const float a0[4] = {av[0].x, av[0].y, av[0].z, av[0].w}, a1[4] = {av[1].x, av[1].y, av[1].z, av[1].w};
+    const float h0[4] = {hv[0].x, hv[0].y, hv[0].z, hv[0].w}, h1[4] = {hv[1].x, hv[1].y, hv[1].z, hv[1].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      A2[p][i] = pack2(a0[i] * kLog2e, a1[i] * kLog2e);
+      h[p][i] = pack2(h0[i], h1[i]);
+    }
+    sumd[p] = pack2(0.0f, 0.0f);
   }
+  auto store_h = [&](float* dst) {                       // dst: the first channel's states
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (ch + k >= nch) continue;
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        unpack2(h[k / 2][i], lo, hi);
+        v[i] = k & 1 ? hi : lo;
+      }
+      store_state4(dst + static_cast<int64_t>(k) * a.N, n0, a.N, v);
+    }
+  };
   const T* gx = static_cast<const T*>(a.x) + b * a.x_b + d0;
   const T* gdt = static_cast<const T*>(a.dt) + b * a.dt_b + d0;
   const T* gz = a.z ? static_cast<const T*>(a.z) + b * a.z_b + d0 : nullptr;
@@ -81,20 +109,31 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
   const T* gC = static_cast<const T*>(a.C) + b * a.C_b + g * a.C_g;
   T* gout = static_cast<T*>(a.out) + b * a.out_b + d0;
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+  float* saved = a.saved ? a.saved + (static_cast<int64_t>(b) * ((a.T + kSave - 1) / kSave) * a.dim + d0 + ch) * a.N : nullptr;
 
   auto fetch = [&](int t, int buf) {
     const int rows = min(kTile, t_live - t);
     if (rows > 0) {
-      copy_rows<T, kThreads, kAsync>(sm.x[buf], CH, gx + t * a.x_t, a.x_t, rows, nch);
-      copy_rows<T, kThreads, kAsync>(sm.dt[buf], CH, gdt + t * a.dt_t, a.dt_t, rows, nch);
-      copy_rows<T, kThreads, kAsync>(sm.B[buf], NP, gB + t * a.B_t, a.B_t, rows, a.N);
+      copy_rows<T, kThreads, CH>(sm.x[buf], gx + t * a.x_t, a.x_t, rows, nch, a.mode_d);
+      copy_rows<T, kThreads, CH>(sm.dt[buf], gdt + t * a.dt_t, a.dt_t, rows, nch, a.mode_d);
+      copy_rows<T, kThreads, NP>(sm.B[buf], gB + t * a.B_t, a.B_t, rows, a.N, a.mode_n);
       if (!kCarry) {
-        copy_rows<T, kThreads, kAsync>(sm.C[buf], NP, gC + t * a.C_t, a.C_t, rows, a.N);
-        if (gz) copy_rows<T, kThreads, kAsync>(sm.z[buf], CH, gz + t * a.z_t, a.z_t, rows, nch);
+        copy_rows<T, kThreads, NP>(sm.C[buf], gC + t * a.C_t, a.C_t, rows, a.N, a.mode_n);
+        if (gz) copy_rows<T, kThreads, CH>(sm.z[buf], gz + t * a.z_t, a.z_t, rows, nch, a.mode_d);
       }
     }
     cp_async_commit();
   };
+
+  // before and behind the recurrence a thread works on 4 channels of every kStep-th token
+  constexpr int kQuads = CH / 4, kStep = kThreads / kQuads;
+  const int ec = threadIdx.x % kQuads * 4, er = threadIdx.x / kQuads;
+  float bias[4], skip[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    bias[j] = a.bias && ec + j < nch ? a.bias[d0 + ec + j] : 0.0f;
+    skip[j] = a.D && ec + j < nch ? a.D[d0 + ec + j] : 0.0f;
+  }
 
   bool any_cut = false;
   fetch(t_lo, 0);
@@ -104,84 +143,100 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
     __syncthreads();
     fetch(t0 + kTile, buf ^ 1);
     const int rows = min(kTile, t_live - t0);
-    // delta and delta * x of the tile, B and C in 32 bits
-    for (int i = threadIdx.x; i < kTile * CH; i += kThreads) {
-      const int r = i / CH, c = i - r * CH;
-      float dv = 0.0f, uv = 0.0f;
-      if (r < rows && c < nch) {
-        dv = to_f(sm.dt[buf][i]) + (a.bias ? a.bias[d0 + c] : 0.0f);
-        if (a.softplus) dv = softplus(dv);
-        uv = dv * to_f(sm.x[buf][i]);
+    // bit r: token r starts an episode (every warp finds them for itself)
+    static_assert(kTile <= 32, "a warp's lanes look at a tile's tokens");
+    const unsigned cuts = __ballot_sync(0xffffffffu, reset && lane < rows && reset[t0 + lane]);
+    any_cut |= cuts != 0;
+    // delta and delta * x; zeros past the tile's last token, where the state then stays as it is
+#pragma unroll 4
+    for (int r = er; r < kTile; r += kStep) {
+      float dv[4], xv[4], uv[4];
+      load_vec<T, 4>(sm.dt[buf] + r * CH + ec, dv);
+      load_vec<T, 4>(sm.x[buf] + r * CH + ec, xv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dv[j] += bias[j];
+        if (a.softplus) dv[j] = softplus(dv[j]);
+        const bool in = r < rows && ec + j < nch;
+        dv[j] = in ? dv[j] : 0.0f;
+        uv[j] = in ? dv[j] * xv[j] : 0.0f;
       }
-      sm.delta[i] = dv;
-      sm.u[i] = uv;
+      store_vec<float, 4>(sm.delta + r * CH + ec, dv);
+      store_vec<float, 4>(sm.u + r * CH + ec, uv);
     }
     for (int i = threadIdx.x; i < kTile * NP; i += kThreads) {
-      const int r = i / NP, n = i - r * NP;
+      const int r = i / NP, n = i % NP;
       const bool in = r < rows && n < a.N;
-      sm.Bf[i] = in ? to_f(sm.B[buf][i]) : 0.0f;
-      if (!kCarry) sm.Cf[i] = in ? to_f(sm.C[buf][i]) : 0.0f;
-    }
-    if (threadIdx.x < kTile) sm.cut[threadIdx.x] = reset && threadIdx.x < rows && reset[t0 + threadIdx.x] ? 1 : 0;
-    __syncthreads();
-    for (int r = 0; r < rows; ++r) {
-      if (sm.cut[r]) {
-        any_cut = true;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) h[k][i] = 0.0f;
-      }
-      if (!kCarry && a.saved && (r & (kSave - 1)) == 0) {
-        float* s = a.saved + ((static_cast<int64_t>(b) * ((a.T + kSave - 1) / kSave) + (t0 + r) / kSave) * a.dim + d0 + ch) * a.N;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (ch + k < nch) store_state4(s + static_cast<int64_t>(k) * a.N, n0, a.N, h[k]);
-      }
-      float dl[K], u[K], acc[K];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        dl[k] = sm.delta[r * CH + ch + k];
-        u[k] = sm.u[r * CH + ch + k];
-        acc[k] = 0.0f;
-        if (kCarry) sumd[k] += dl[k];
-      }
-      const float4 Bv = *reinterpret_cast<const float4*>(sm.Bf + r * NP + n0);
-      const float Bt[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
-      float Ct[4] = {0.f, 0.f, 0.f, 0.f};
+      const float Bv = in ? to_f(sm.B[buf][i]) : 0.0f;
+      *reinterpret_cast<float2*>(sm.Bd + 2 * i) = make_float2(Bv, Bv);
       if (!kCarry) {
-        const float4 Cv = *reinterpret_cast<const float4*>(sm.Cf + r * NP + n0);
-        Ct[0] = Cv.x; Ct[1] = Cv.y; Ct[2] = Cv.z; Ct[3] = Cv.w;
+        const float Cv = in ? to_f(sm.C[buf][i]) : 0.0f;
+        *reinterpret_cast<float2*>(sm.Cd + 2 * i) = make_float2(Cv, Cv);
+      }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int r = 0; r < kTile; ++r) {
+      if (cuts >> r & 1u) {
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[p][i].v = 0;
+      }
+      if (!kCarry && (r % kSave) == 0 && saved && r < rows)
+        store_h(saved + static_cast<int64_t>((t0 + r) / kSave) * a.dim * a.N);
+      f2 dl[P], u[P], y[P], Bt[4], Ct[4];
+      if constexpr (P == 2) {
+        load_pairs(sm.delta + r * CH + ch, dl[0], dl[1]);
+        load_pairs(sm.u + r * CH + ch, u[0], u[1]);
+      } else {
+        dl[0].v = *reinterpret_cast<const unsigned long long*>(sm.delta + r * CH + ch);
+        u[0].v = *reinterpret_cast<const unsigned long long*>(sm.u + r * CH + ch);
+      }
+      load_pairs(sm.Bd + (r * NP + n0) * 2, Bt[0], Bt[1]);
+      load_pairs(sm.Bd + (r * NP + n0) * 2 + 4, Bt[2], Bt[3]);
+      if (!kCarry) {
+        load_pairs(sm.Cd + (r * NP + n0) * 2, Ct[0], Ct[1]);
+        load_pairs(sm.Cd + (r * NP + n0) * 2 + 4, Ct[2], Ct[3]);
       }
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int p = 0; p < P; ++p) {
+        if (kCarry) sumd[p] = add2(sumd[p], dl[p]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          h[k][i] = fmaf(exp2_hw(dl[k] * A2[k][i]), h[k][i], u[k] * Bt[i]);
-          if (!kCarry) acc[k] = fmaf(h[k][i], Ct[i], acc[k]);
+          h[p][i] = fma2(exp2_hw2(mul2(dl[p], A2[p][i])), h[p][i], mul2(u[p], Bt[i]));
+          if (!kCarry) y[p] = i == 0 ? mul2(h[p][i], Ct[i]) : fma2(h[p][i], Ct[i], y[p]);
         }
+      }
       if (!kCarry) {
+        float acc[K];
+#pragma unroll
+        for (int p = 0; p < P; ++p) unpack2(y[p], acc[2 * p], acc[2 * p + 1]);
         reduce_lanes<LN, K>(acc, lane);
-        if (reduced_writer<LN, K>(lane)) sm.y[r * CH + ch + reduced_channel<LN, K>(lane)] = acc[0];
+        // u of this token and these channels has been read by the lanes whose sums are here
+        if (reduced_writer<LN, K>(lane)) {
+#pragma unroll
+          for (int q = 0; q < kReduced<LN, K>; ++q) sm.u[r * CH + ch + reduced_channel<LN, K>(lane) + q] = acc[q];
+        }
       }
     }
     __syncthreads();
     if (!kCarry) {
-      constexpr int V = kAsync ? kVec16<T> : 1;
-      for (int i = threadIdx.x; i < rows * (CH / V); i += kThreads) {
-        const int r = i / (CH / V), c = (i - r * (CH / V)) * V;
-        if (c >= nch) continue;
-        float o[V], xv[V];
-        load_vec<T, V>(sm.x[buf] + r * CH + c, xv);
+#pragma unroll 4
+      for (int r = er; r < rows; r += kStep) {
+        if (ec >= nch) break;
+        float o[4], xv[4];
+        load_vec<float, 4>(sm.u + r * CH + ec, o);
+        load_vec<T, 4>(sm.x[buf] + r * CH + ec, xv);
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = sm.y[r * CH + c + j] + (a.D ? a.D[d0 + c + j] * xv[j] : 0.0f);
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(skip[j], xv[j], o[j]);
         if (gz) {
-          float zv[V];
-          load_vec<T, V>(sm.z[buf] + r * CH + c, zv);
+          float zv[4];
+          load_vec<T, 4>(sm.z[buf] + r * CH + ec, zv);
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] *= zv[j] * sigmoid(zv[j]);
+          for (int j = 0; j < 4; ++j) o[j] *= zv[j] * sigmoid(zv[j]);
         }
-        store_vec<T, V>(gout + (t0 + r) * a.out_t + c, o);
+        store_quad<T>(gout + (t0 + r) * a.out_t + ec, o, nch - ec, a.mode_d == kPieces16);
       }
     }
   }
@@ -190,17 +245,18 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
     for (int t = max(t_lo, t_live); t < t_hi; ++t)
       for (int c = threadIdx.x; c < nch; c += kThreads) gout[t * a.out_t + c] = from_f<T>(0.0f);
   }
-  if (kCarry || (a.final_state && chunk == a.chunks - 1)) {
-    float* dst = kCarry ? a.carry + (static_cast<int64_t>(b) * a.chunks + chunk) * a.dim * a.N
-                        : a.final_state + static_cast<int64_t>(b) * a.dim * a.N;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (ch + k < nch) store_state4(dst + static_cast<int64_t>(d0 + ch + k) * a.N, n0, a.N, h[k]);
-  }
+  if (kCarry) store_h(a.carry + ((static_cast<int64_t>(b) * a.chunks + chunk) * a.dim + d0 + ch) * a.N);
+  else if (a.final_state && chunk == a.chunks - 1) store_h(a.final_state + (static_cast<int64_t>(b) * a.dim + d0 + ch) * a.N);
   if (kCarry) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (nl == 0 && ch + k < nch) a.sumd[(static_cast<int64_t>(b) * a.chunks + chunk) * a.dim + d0 + ch + k] = sumd[k];
+    for (int p = 0; p < P; ++p) {
+      float v[2];
+      unpack2(sumd[p], v[0], v[1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (nl == 0 && ch + 2 * p + e < nch)
+          a.sumd[(static_cast<int64_t>(b) * a.chunks + chunk) * a.dim + d0 + ch + 2 * p + e] = v[e];
+    }
     if (threadIdx.x == 0) a.cut[static_cast<int64_t>(b) * a.chunks + chunk] = any_cut;   // the same from every block
   }
 }
@@ -236,7 +292,7 @@ __global__ void __launch_bounds__(256) carry_kernel(ScanArgs a) {
   }
 }
 
-template <typename T, int LN, bool kAsync> int launch_scan(const ScanArgs& a, cudaStream_t s) {
+template <typename T, int LN> int launch_scan(const ScanArgs& a, cudaStream_t s) {
   using L = Layout<T, LN>;
   const int bpg = static_cast<int>(surfk::ceil_div(a.dim / a.G, L::CH));
   const int64_t gx = static_cast<int64_t>(bpg) * a.G * a.batch;
@@ -244,13 +300,13 @@ template <typename T, int LN, bool kAsync> int launch_scan(const ScanArgs& a, cu
   constexpr size_t smem = sizeof(typename L::Smem);
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(a.chunks));
   if (a.chunks > 1) {
-    if (const int rc = allow_smem<scan_kernel<T, LN, kAsync, true>>(smem)) return rc;
-    scan_kernel<T, LN, kAsync, true><<<grid, kThreads, smem, s>>>(a, bpg);
+    if (const int rc = allow_smem<scan_kernel<T, LN, true>>(smem)) return rc;
+    scan_kernel<T, LN, true><<<grid, kThreads, smem, s>>>(a, bpg);
     const int64_t n = static_cast<int64_t>(a.batch) * a.dim * a.N;
     carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(n, 256)), 256, 0, s>>>(a);
   }
-  if (const int rc = allow_smem<scan_kernel<T, LN, kAsync, false>>(smem)) return rc;
-  scan_kernel<T, LN, kAsync, false><<<grid, kThreads, smem, s>>>(a, bpg);
+  if (const int rc = allow_smem<scan_kernel<T, LN, false>>(smem)) return rc;
+  scan_kernel<T, LN, false><<<grid, kThreads, smem, s>>>(a, bpg);
   SURF_RETURN_LAUNCH();
 }
 
@@ -288,8 +344,8 @@ template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel
     if (a.softplus) dv = softplus(dv);
     const float u = dv * x;
     float* st = a.pool + (static_cast<int64_t>(slot) * a.dim + d) * a.N;
-    float4 h4 = a.reset && a.reset[r] ? make_float4(0.f, 0.f, 0.f, 0.f) : load_state4<LN>(st, n0, a.N);
-    const float4 A4 = load_state4<LN>(a.A + static_cast<int64_t>(d) * a.N, n0, a.N);
+    float4 h4 = a.reset && a.reset[r] ? make_float4(0.f, 0.f, 0.f, 0.f) : load_state4(st, n0, a.N);
+    const float4 A4 = load_state4(a.A + static_cast<int64_t>(d) * a.N, n0, a.N);
     const T* B = static_cast<const T*>(a.B) + r * a.B_r + g * a.B_g;
     const T* C = static_cast<const T*>(a.C) + r * a.C_r + g * a.C_g;
     float h[4] = {h4.x, h4.y, h4.z, h4.w};
@@ -321,15 +377,13 @@ template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel
 
 }  // namespace
 
-// aligned: the per-group channel count and N are whole 16-byte pieces, and so are all bases and strides
-SURF_EXPORT int surf_seq_scan(const void* args, int dtype, int aligned, void* stream) {
+SURF_EXPORT int surf_seq_scan(const void* args, int dtype, void* stream) {
   const ScanArgs a = *static_cast<const ScanArgs*>(args);
   if (a.batch <= 0 || a.dim <= 0) return 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_lanes(a.N, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
-    if (dtype == kBf16) return aligned ? launch_scan<bf16, LN, true>(a, s) : launch_scan<bf16, LN, false>(a, s);
-    return aligned ? launch_scan<float, LN, true>(a, s) : launch_scan<float, LN, false>(a, s);
+    return dtype == kBf16 ? launch_scan<bf16, LN>(a, s) : launch_scan<float, LN>(a, s);
   });
 }
 

@@ -27,11 +27,12 @@ struct ScanArgs {
   int64_t x_b, x_t, dt_b, dt_t, z_b, z_t, B_b, B_t, B_g, C_b, C_t, C_g, do_b, do_t, out_b, out_t, r_b;
   int batch, T, dim, N, G, softplus;
   int chunk, chunks;                           // tokens of a chunk (a multiple of 16), chunks of a row
+  int mode_d, mode_n;                          // how rows of channels and of states are copied (copy_rows)
 };
 
 // A warp's 32 lanes are 32 / LN channel rows of LN lanes; a lane holds 4 states of
 // each of K channels, so 4 * LN >= N states of a channel sit in LN neighbouring lanes.
-template <int LN> __device__ __forceinline__ float4 load_state4(const float* p, int n0, int N) {
+__device__ __forceinline__ float4 load_state4(const float* p, int n0, int N) {
   if ((N & 3) == 0) return n0 < N ? *reinterpret_cast<const float4*>(p + n0) : make_float4(0.f, 0.f, 0.f, 0.f);
   float4 v;
   v.x = n0 + 0 < N ? p[n0 + 0] : 0.0f;
@@ -83,9 +84,21 @@ template <int LN, int K> __device__ __forceinline__ int reduced_channel(int lane
     }
   return c;
 }
-// the lane that writes the channel's sum
+// the lanes that write sums, and how many each of them holds
 template <int LN, int K> __device__ __forceinline__ bool reduced_writer(int lane) {
-  return (lane & (LN / K - 1)) == 0;
+  return LN <= K || (lane & (LN / K - 1)) == 0;
+}
+template <int LN, int K> constexpr int kReduced = K > LN ? K / LN : 1;
+
+// up to 4 channels of a row: one store where it is aligned and whole
+template <typename T> __device__ __forceinline__ void store_quad(T* p, const float (&v)[4], int left, bool whole) {
+  if (whole && left >= 4) {
+    store_vec<T, 4>(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = from_f<T>(v[j]);
+  }
 }
 
 // states -> lanes of a channel row; f gets the count as a compile-time constant

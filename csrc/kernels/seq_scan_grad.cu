@@ -24,16 +24,16 @@ namespace {
 using namespace seqk;
 
 template <typename T, int LN> struct GradLayout {
-  static constexpr int K = LN < 2 ? 1 : 2;
   static constexpr int NT = LN < 4 ? 128 : 256;
-  static constexpr int CH = NT / LN * K;
+  static constexpr int CH = NT / LN * 2;                  // two channels a thread, one f32x2 pair
   static constexpr int NP = 4 * LN;
   static constexpr int R = kSave;                         // tokens of a tile
   struct Smem {
     alignas(16) T x[2][R * CH], dt[2][R * CH], z[2][R * CH], dout[2][R * CH], B[2][R * NP], C[2][R * NP];
-    alignas(16) float delta[R * CH], u[R * CH], g[R * CH], y[R * CH], ub[R * CH], qa[R * CH], Bf[R * NP], Cf[R * NP];
+    alignas(16) float delta[R * CH], u[R * CH], g[R * CH], y[R * CH], ub[R * CH], qa[R * CH];
+    alignas(16) float Bd[R * NP * 2], Cd[R * NP * 2];     // 32-bit, every value twice
     alignas(16) float red[NT / 32][R][2 * NP];            // the warps' sums of dB and dC
-    int cut[R];
+    alignas(16) float bias[CH], skip[CH];
   };
 };
 
@@ -65,20 +65,25 @@ template <int LN> __device__ __forceinline__ void reduce_rows(float (&v)[8], int
   }
 }
 // The backward sweep's decays, made again: as an ordinary expression the compiler would
-// keep the forward run's (4 K values for each of the tile's tokens) and spill.
-__device__ __forceinline__ float exp2_again(float x) {
-  float y;
-  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// keep the forward run's (8 values for each of the tile's tokens) and spill.
+__device__ __forceinline__ f2 exp2_again(f2 x) {
+  float lo, hi;
+  unpack2(x, lo, hi);
+  asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(lo));
+  asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(hi));
+  return pack2(lo, hi);
 }
 
 template <int LN> constexpr int kRowSums = LN <= 4 ? 1 : (LN == 8 ? 2 : 4);
 
-template <typename T, int LN, bool kAsync, bool kCarry>
-__global__ void __launch_bounds__(GradLayout<T, LN>::NT, kCarry ? 1 : 512 / GradLayout<T, LN>::NT)
+// Per state and token the two sweeps cost 13 multiply-adds and two exponentials, the
+// sums across lanes about 6 instructions more: the issue rate and the exponential unit
+// (16 a cycle and SM) bound it alike.
+template <typename T, int LN, bool kCarry>
+__global__ void __launch_bounds__(GradLayout<T, LN>::NT, (kCarry ? 768 : 512) / GradLayout<T, LN>::NT)
 scan_grad_kernel(ScanArgs a, int blocks_per_group) {
   using L = GradLayout<T, LN>;
-  constexpr int K = L::K, CH = L::CH, NP = L::NP, R = L::R, NT = L::NT;
+  constexpr int CH = L::CH, NP = L::NP, R = L::R, NT = L::NT;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   typename L::Smem& sm = *reinterpret_cast<typename L::Smem*>(smem_raw);
   const int blocks = blocks_per_group * a.G;
@@ -95,25 +100,36 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nl = lane & (LN - 1);
-  const int ch = threadIdx.x / LN * K;
+  const int ch = threadIdx.x / LN * 2;
   const int n0 = nl * 4;
 
-  float A2[K][4], dh[K][4], dA[K][4], sumd[K];
+  // 4 states of the two channels, from memory into pairs and back
+  auto load_h = [&](const float* src, f2 (&v)[4], float scale) {
+    float4 q[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const bool on = ch + k < nch;
-    const int64_t row = static_cast<int64_t>(d0 + ch + k) * a.N, bd = static_cast<int64_t>(a.dim) * a.N;
-    const float4 v = on ? load_state4<LN>(a.A + row, n0, a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
-    A2[k][0] = v.x * kLog2e; A2[k][1] = v.y * kLog2e; A2[k][2] = v.z * kLog2e; A2[k][3] = v.w * kLog2e;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!kCarry && on) {
-      if (a.chunks > 1) s = load_state4<LN>(a.carry + bchunk * bd + row, n0, a.N);
-      else if (a.dfinal) s = load_state4<LN>(a.dfinal + b * bd + row, n0, a.N);
-    }
-    dh[k][0] = s.x; dh[k][1] = s.y; dh[k][2] = s.z; dh[k][3] = s.w;
-    dA[k][0] = dA[k][1] = dA[k][2] = dA[k][3] = 0.0f;
-    sumd[k] = 0.0f;
-  }
+    for (int e = 0; e < 2; ++e)
+      if (src && ch + e < nch) q[e] = load_state4(src + static_cast<int64_t>(d0 + ch + e) * a.N, n0, a.N);
+    v[0] = pack2(q[0].x * scale, q[1].x * scale);
+    v[1] = pack2(q[0].y * scale, q[1].y * scale);
+    v[2] = pack2(q[0].z * scale, q[1].z * scale);
+    v[3] = pack2(q[0].w * scale, q[1].w * scale);
+  };
+  auto store_h = [&](float* dst, const f2 (&v)[4]) {
+    float q[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack2(v[i], q[0][i], q[1][i]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (ch + e < nch) store_state4(dst + static_cast<int64_t>(d0 + ch + e) * a.N, n0, a.N, q[e]);
+  };
+  const int64_t per_row = static_cast<int64_t>(a.dim) * a.N;
+
+  f2 A2[4], dh[4], dA[4], sumd = pack2(0.0f, 0.0f);
+  load_h(a.A, A2, kLog2e);
+  load_h(kCarry ? nullptr : a.chunks > 1 ? a.carry + bchunk * per_row : a.dfinal ? a.dfinal + b * per_row : nullptr, dh, 1.0f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dA[i] = pack2(0.0f, 0.0f);
+
   const T* gx = static_cast<const T*>(a.x) + b * a.x_b + d0;
   const T* gdt = static_cast<const T*>(a.dt) + b * a.dt_b + d0;
   const T* gz = a.z ? static_cast<const T*>(a.z) + b * a.z_b + d0 : nullptr;
@@ -125,150 +141,162 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
   T* gddt = static_cast<T*>(a.ddt) + dense;
   T* gdz = a.dz ? static_cast<T*>(a.dz) + dense : nullptr;
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
-  const int64_t save_rows = (a.T + kSave - 1) / kSave;
+  const float* saved = kCarry ? nullptr : a.saved + static_cast<int64_t>(b) * ((a.T + kSave - 1) / kSave) * per_row;
 
   auto fetch = [&](int t, int buf) {
     const int rows = min(R, t_live - t);
     if (t >= t_lo && rows > 0) {
       if (!kCarry) {
-        copy_rows<T, NT, kAsync>(sm.x[buf], CH, gx + t * a.x_t, a.x_t, rows, nch);
-        copy_rows<T, NT, kAsync>(sm.B[buf], NP, gB + t * a.B_t, a.B_t, rows, a.N);
+        copy_rows<T, NT, CH>(sm.x[buf], gx + t * a.x_t, a.x_t, rows, nch, a.mode_d);
+        copy_rows<T, NT, NP>(sm.B[buf], gB + t * a.B_t, a.B_t, rows, a.N, a.mode_n);
       }
-      copy_rows<T, NT, kAsync>(sm.dt[buf], CH, gdt + t * a.dt_t, a.dt_t, rows, nch);
-      copy_rows<T, NT, kAsync>(sm.dout[buf], CH, gdo + t * a.do_t, a.do_t, rows, nch);
-      copy_rows<T, NT, kAsync>(sm.C[buf], NP, gC + t * a.C_t, a.C_t, rows, a.N);
-      if (gz) copy_rows<T, NT, kAsync>(sm.z[buf], CH, gz + t * a.z_t, a.z_t, rows, nch);
+      copy_rows<T, NT, CH>(sm.dt[buf], gdt + t * a.dt_t, a.dt_t, rows, nch, a.mode_d);
+      copy_rows<T, NT, CH>(sm.dout[buf], gdo + t * a.do_t, a.do_t, rows, nch, a.mode_d);
+      copy_rows<T, NT, NP>(sm.C[buf], gC + t * a.C_t, a.C_t, rows, a.N, a.mode_n);
+      if (gz) copy_rows<T, NT, CH>(sm.z[buf], gz + t * a.z_t, a.z_t, rows, nch, a.mode_d);
     }
     cp_async_commit();
   };
-  auto load_saved = [&](int t, float (&h0)[K][4]) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const float* s = a.saved + ((b * save_rows + t / kSave) * a.dim + d0 + ch + k) * a.N;
-      const float4 v = t >= t_lo && ch + k < nch ? load_state4<LN>(s, n0, a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
-      h0[k][0] = v.x; h0[k][1] = v.y; h0[k][2] = v.z; h0[k][3] = v.w;
-    }
-  };
 
-  // the epilogue's channels of this thread, and their sums of g x and ddt
-  constexpr int VE = kAsync ? 4 : 1;
-  const int ec = static_cast<int>(threadIdx.x % (CH / VE)) * VE;
-  float sD[VE], sV[VE];
-#pragma unroll
-  for (int j = 0; j < VE; ++j) sD[j] = sV[j] = 0.0f;
+  // before and behind the sweeps a thread works on 4 channels of every kStep-th token
+  constexpr int kQuads = CH / 4, kStep = NT / kQuads;
+  const int ec = threadIdx.x % kQuads * 4, er = threadIdx.x / kQuads;
+  float sD[4] = {0.f, 0.f, 0.f, 0.f}, sV[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int c = threadIdx.x; c < CH; c += NT) {
+    sm.bias[c] = a.bias && c < nch ? a.bias[d0 + c] : 0.0f;
+    sm.skip[c] = a.D && c < nch ? a.D[d0 + c] : 0.0f;
+  }
 
   bool any_cut = false;
   const int last = t_live > t_lo ? t_lo + (t_live - 1 - t_lo) / R * R : t_lo - R;
-  float h0[K][4];
-  if (!kCarry) load_saved(last, h0);
   fetch(last, 0);
   int buf = 0;
   for (int t0 = last; t0 >= t_lo; t0 -= R, buf ^= 1) {
+    f2 h[R + 1][4];                                        // h[r]: the state before token r, h[R] behind the last
+    if (!kCarry) load_h(saved + t0 / kSave * per_row, h[0], 1.0f);
     cp_async_wait<0>();
     __syncthreads();
     fetch(t0 - R, buf ^ 1);
     const int rows = min(R, t_live - t0);
-    for (int i = threadIdx.x; i < R * CH; i += NT) {
-      const int r = i / CH, c = i - r * CH;
-      float dv = 0.0f, uv = 0.0f, gv = 0.0f;
-      if (r < rows && c < nch) {
-        dv = to_f(sm.dt[buf][i]) + (a.bias ? a.bias[d0 + c] : 0.0f);
-        if (a.softplus) dv = softplus(dv);
-        if (!kCarry) uv = dv * to_f(sm.x[buf][i]);
-        gv = to_f(sm.dout[buf][i]);
-        if (gz) {
-          const float z = to_f(sm.z[buf][i]);
-          gv *= z * sigmoid(z);
-        }
+    // bit r: token r starts an episode (every warp finds them for itself)
+    const unsigned cuts = __ballot_sync(0xffffffffu, reset && lane < rows && reset[t0 + lane]);
+    any_cut |= cuts != 0;
+    for (int r = er; r < R; r += kStep) {
+      float dv[4], gv[4], uv[4], bias[4];
+      const int at = r * CH + ec;
+      load_vec<float, 4>(sm.bias + ec, bias);
+      load_vec<T, 4>(sm.dt[buf] + at, dv);
+      load_vec<T, 4>(sm.dout[buf] + at, gv);
+      if (!kCarry) load_vec<T, 4>(sm.x[buf] + at, uv);
+      if (gz) {
+        float zv[4];
+        load_vec<T, 4>(sm.z[buf] + at, zv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) gv[j] *= zv[j] * sigmoid(zv[j]);
       }
-      sm.delta[i] = dv;
-      if (!kCarry) sm.u[i] = uv;
-      sm.g[i] = gv;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dv[j] += bias[j];
+        if (a.softplus) dv[j] = softplus(dv[j]);
+        const bool in = r < rows && ec + j < nch;          // past the last token nothing changes
+        dv[j] = in ? dv[j] : 0.0f;
+        gv[j] = in ? gv[j] : 0.0f;
+        uv[j] = !kCarry && in ? dv[j] * uv[j] : 0.0f;
+      }
+      store_vec<float, 4>(sm.delta + at, dv);
+      store_vec<float, 4>(sm.g + at, gv);
+      if (!kCarry) store_vec<float, 4>(sm.u + at, uv);
     }
     for (int i = threadIdx.x; i < R * NP; i += NT) {
-      const int r = i / NP, n = i - r * NP;
+      const int r = i / NP, n = i % NP;
       const bool in = r < rows && n < a.N;
-      if (!kCarry) sm.Bf[i] = in ? to_f(sm.B[buf][i]) : 0.0f;
-      sm.Cf[i] = in ? to_f(sm.C[buf][i]) : 0.0f;
+      const float Cv = in ? to_f(sm.C[buf][i]) : 0.0f;
+      *reinterpret_cast<float2*>(sm.Cd + 2 * i) = make_float2(Cv, Cv);
+      if (!kCarry) {
+        const float Bv = in ? to_f(sm.B[buf][i]) : 0.0f;
+        *reinterpret_cast<float2*>(sm.Bd + 2 * i) = make_float2(Bv, Bv);
+      }
     }
-    if (threadIdx.x < R) sm.cut[threadIdx.x] = reset && threadIdx.x < rows && reset[t0 + threadIdx.x] ? 1 : 0;
     __syncthreads();
+    auto pair_at = [&](const float* p) {
+      f2 v;
+      v.v = *reinterpret_cast<const unsigned long long*>(p);
+      return v;
+    };
     if constexpr (kCarry) {
-      for (int r = rows - 1; r >= 0; --r) {
-        const bool cut = sm.cut[r];
-        any_cut |= cut;
-        const float4 Cv = *reinterpret_cast<const float4*>(sm.Cf + r * NP + n0);
-        const float Ct[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const float dl = sm.delta[r * CH + ch + k], gv = sm.g[r * CH + ch + k];
-          sumd[k] += dl;
+      for (int r = R - 1; r >= 0; --r) {
+        f2 Ct[4];
+        load_pairs(sm.Cd + (r * NP + n0) * 2, Ct[0], Ct[1]);
+        load_pairs(sm.Cd + (r * NP + n0) * 2 + 4, Ct[2], Ct[3]);
+        const f2 dl = pair_at(sm.delta + r * CH + ch), gv = pair_at(sm.g + r * CH + ch);
+        sumd = add2(sumd, dl);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float v = fmaf(gv, Ct[i], dh[k][i]);
-            dh[k][i] = cut ? 0.0f : v * exp2_hw(dl * A2[k][i]);
-          }
+        for (int i = 0; i < 4; ++i) dh[i] = mul2(fma2(gv, Ct[i], dh[i]), exp2_hw2(mul2(dl, A2[i])));
+        if (cuts >> r & 1u) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dh[i].v = 0;
         }
       }
     } else {
-      // the states of the tile: h[r] before token r, h[R] behind the last (tokens past the
-      // row's end have delta = 0 and change nothing)
-      float h[R + 1][K][4];
+      auto sweeps = [&](auto with_cuts) {
+        constexpr bool kCuts = decltype(with_cuts)::value;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+        for (int r = 0; r < R; ++r) {
+          f2 Bt[4];
+          load_pairs(sm.Bd + (r * NP + n0) * 2, Bt[0], Bt[1]);
+          load_pairs(sm.Bd + (r * NP + n0) * 2 + 4, Bt[2], Bt[3]);
+          const f2 dl = pair_at(sm.delta + r * CH + ch), u = pair_at(sm.u + r * CH + ch);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[0][k][i] = h0[k][i];
-      load_saved(t0 - R, h0);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float4 Bv = *reinterpret_cast<const float4*>(sm.Bf + r * NP + n0);
-        const float Bt[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
-        const bool cut = sm.cut[r];
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const float dl = sm.delta[r * CH + ch + k], u = sm.u[r * CH + ch + k];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            h[r + 1][k][i] = fmaf(exp2_hw(dl * A2[k][i]), cut ? 0.0f : h[r][k][i], u * Bt[i]);
-        }
-      }
-#pragma unroll
-      for (int r = R - 1; r >= 0; --r) {
-        if (r < rows) {
-          const float4 Bv = *reinterpret_cast<const float4*>(sm.Bf + r * NP + n0);
-          const float4 Cv = *reinterpret_cast<const float4*>(sm.Cf + r * NP + n0);
-          const float Bt[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, Ct[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
-          float y[K], ub[K], qa[K], bc[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) bc[i] = 0.0f;
-          const bool cut = sm.cut[r];
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            const float dl = sm.delta[r * CH + ch + k], u = sm.u[r * CH + ch + k], gv = sm.g[r * CH + ch + k];
-            y[k] = ub[k] = qa[k] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float ad = exp2_again(dl * A2[k][i]);
-              const float v = fmaf(gv, Ct[i], dh[k][i]);
-              y[k] = fmaf(h[r + 1][k][i], Ct[i], y[k]);
-              bc[4 + i] = fmaf(h[r + 1][k][i], gv, bc[4 + i]);
-              bc[i] = fmaf(v, u, bc[i]);
-              ub[k] = fmaf(v, Bt[i], ub[k]);
-              const float va = v * ad;
-              const float q = va * (cut ? 0.0f : h[r][k][i]);
-              qa[k] = fmaf(q, A2[k][i], qa[k]);
-              dA[k][i] = fmaf(q, dl, dA[k][i]);
-              dh[k][i] = cut ? 0.0f : va;
-            }
+          for (int i = 0; i < 4; ++i) {
+            f2 before = h[r][i];
+            if (kCuts && (cuts >> r & 1u)) before.v = 0;
+            h[r + 1][i] = fma2(exp2_hw2(mul2(dl, A2[i])), before, mul2(u, Bt[i]));
           }
-          reduce_lanes<LN, K>(y, lane);
-          reduce_lanes<LN, K>(ub, lane);
-          reduce_lanes<LN, K>(qa, lane);
-          if (reduced_writer<LN, K>(lane)) {
-            const int at = r * CH + ch + reduced_channel<LN, K>(lane);
-            sm.y[at] = y[0];
-            sm.ub[at] = ub[0];
-            sm.qa[at] = qa[0] * kLn2;
+        }
+#pragma unroll
+        for (int r = R - 1; r >= 0; --r) {
+          f2 Bt[4], Ct[4];
+          load_pairs(sm.Bd + (r * NP + n0) * 2, Bt[0], Bt[1]);
+          load_pairs(sm.Bd + (r * NP + n0) * 2 + 4, Bt[2], Bt[3]);
+          load_pairs(sm.Cd + (r * NP + n0) * 2, Ct[0], Ct[1]);
+          load_pairs(sm.Cd + (r * NP + n0) * 2 + 4, Ct[2], Ct[3]);
+          const f2 dl = pair_at(sm.delta + r * CH + ch), u = pair_at(sm.u + r * CH + ch), gv = pair_at(sm.g + r * CH + ch);
+          float ul, uh, gl, gh, bc[8];
+          unpack2(u, ul, uh);
+          unpack2(gv, gl, gh);
+          f2 y, ub, qa;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f2 v = fma2(gv, Ct[i], dh[i]);
+            float lo, hi;
+            unpack2(v, lo, hi);
+            bc[i] = fmaf(hi, uh, lo * ul);
+            unpack2(h[r + 1][i], lo, hi);
+            bc[4 + i] = fmaf(hi, gh, lo * gl);
+            y = i == 0 ? mul2(h[r + 1][i], Ct[i]) : fma2(h[r + 1][i], Ct[i], y);
+            ub = i == 0 ? mul2(v, Bt[i]) : fma2(v, Bt[i], ub);
+            f2 va = mul2(v, exp2_again(mul2(dl, A2[i])));
+            f2 q = mul2(va, h[r][i]);
+            if (kCuts && (cuts >> r & 1u)) va.v = q.v = 0;
+            qa = i == 0 ? mul2(q, A2[i]) : fma2(q, A2[i], qa);
+            dA[i] = fma2(q, dl, dA[i]);
+            dh[i] = va;
+          }
+          float s3[3][2];
+          unpack2(y, s3[0][0], s3[0][1]);
+          unpack2(ub, s3[1][0], s3[1][1]);
+          unpack2(qa, s3[2][0], s3[2][1]);
+#pragma unroll
+          for (int e = 0; e < 3; ++e) reduce_lanes<LN, 2>(s3[e], lane);
+          if (reduced_writer<LN, 2>(lane)) {
+            const int at = r * CH + ch + reduced_channel<LN, 2>(lane);
+#pragma unroll
+            for (int e = 0; e < kReduced<LN, 2>; ++e) {
+              sm.y[at + e] = s3[0][e];
+              sm.ub[at + e] = s3[1][e];
+              sm.qa[at + e] = s3[2][e];
+            }
           }
           int first;
           bool writer;
@@ -281,53 +309,66 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
             }
           }
         }
-      }
+      };
+      if (cuts) sweeps(std::true_type{});
+      else sweeps(std::false_type{});
       __syncthreads();
-      for (int r = threadIdx.x / (CH / VE); r < rows; r += NT / (CH / VE)) {
+      for (int r = er; r < rows; r += kStep) {
         if (ec >= nch) break;
-        float xv[VE], tv[VE], zv[VE], ov[VE], dx[VE], ddt[VE], dz[VE];
+        float xv[4], tv[4], ov[4], gv[4], dl[4], y[4], ub[4], qa[4], dx[4], ddt[4], bias[4], skip[4];
+        load_vec<float, 4>(sm.bias + ec, bias);
+        load_vec<float, 4>(sm.skip + ec, skip);
         const int at = r * CH + ec;
-        load_vec<T, VE>(sm.x[buf] + at, xv);
-        load_vec<T, VE>(sm.dt[buf] + at, tv);
-        load_vec<T, VE>(sm.dout[buf] + at, ov);
-        if (gz) load_vec<T, VE>(sm.z[buf] + at, zv);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const float D = a.D ? a.D[d0 + ec + j] : 0.0f;
-          const float gv = sm.g[at + j], ub = sm.ub[at + j];
-          if (gz) {
-            const float s = sigmoid(zv[j]);
-            dz[j] = ov[j] * fmaf(D, xv[j], sm.y[at + j]) * s * fmaf(zv[j], 1.0f - s, 1.0f);
-          }
-          dx[j] = fmaf(ub, sm.delta[at + j], gv * D);
-          const float dd = fmaf(ub, xv[j], sm.qa[at + j]);
-          ddt[j] = a.softplus ? dd * sigmoid(tv[j] + (a.bias ? a.bias[d0 + ec + j] : 0.0f)) : dd;
-          sD[j] = fmaf(gv, xv[j], sD[j]);
-          sV[j] += ddt[j];
-        }
         const int64_t o = static_cast<int64_t>(t0 + r) * a.dim + ec;
-        store_vec<T, VE>(gdx + o, dx);
-        store_vec<T, VE>(gddt + o, ddt);
-        if (gz) store_vec<T, VE>(gdz + o, dz);
+        load_vec<T, 4>(sm.x[buf] + at, xv);
+        load_vec<T, 4>(sm.dt[buf] + at, tv);
+        load_vec<float, 4>(sm.g + at, gv);
+        load_vec<float, 4>(sm.delta + at, dl);
+        load_vec<float, 4>(sm.ub + at, ub);
+        load_vec<float, 4>(sm.qa + at, qa);
+        if (gz) {
+          float zv[4], dz[4];
+          load_vec<T, 4>(sm.z[buf] + at, zv);
+          load_vec<T, 4>(sm.dout[buf] + at, ov);
+          load_vec<float, 4>(sm.y + at, y);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float s = sigmoid(zv[j]);
+            dz[j] = ov[j] * fmaf(skip[j], xv[j], y[j]) * s * fmaf(zv[j], 1.0f - s, 1.0f);
+          }
+          store_quad<T>(gdz + o, dz, nch - ec, a.mode_d == kPieces16);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          dx[j] = fmaf(ub[j], dl[j], gv[j] * skip[j]);
+          ddt[j] = fmaf(ub[j], xv[j], qa[j] * kLn2);
+          if (a.softplus) ddt[j] *= sigmoid(tv[j] + bias[j]);
+          if (ec + j < nch) {
+            sD[j] = fmaf(gv[j], xv[j], sD[j]);
+            sV[j] += ddt[j];
+          }
+        }
+        store_quad<T>(gdx + o, dx, nch - ec, a.mode_d == kPieces16);
+        store_quad<T>(gddt + o, ddt, nch - ec, a.mode_d == kPieces16);
       }
-      for (int i = threadIdx.x; i < rows * 2 * a.N; i += NT) {
-        const int r = i / (2 * a.N), q = i - r * (2 * a.N);
-        const int at = q < a.N ? q : NP + q - a.N;
+      for (int i = threadIdx.x; i < rows * 2 * NP; i += NT) {
+        const int r = i / (2 * NP), q = i % (2 * NP), n = q % NP;
+        if (n >= a.N) continue;
         float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NT / 32; ++w) s += sm.red[w][r][at];
-        a.part_bc[(((static_cast<int64_t>(sub) * a.batch + b) * a.T + t0 + r) * a.G + g) * (2 * a.N) + q] = s;
+        for (int w = 0; w < NT / 32; ++w) s += sm.red[w][r][q];
+        a.part_bc[(((static_cast<int64_t>(sub) * a.batch + b) * a.T + t0 + r) * a.G + g) * (2 * a.N) + (q < NP ? n : a.N + n)] = s;
       }
     }
   }
   cp_async_wait<0>();
   if constexpr (kCarry) {
+    store_h(a.carry + bchunk * per_row, dh);
+    float v[2];
+    unpack2(sumd, v[0], v[1]);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (ch + k < nch) {
-        store_state4(a.carry + (bchunk * a.dim + d0 + ch + k) * a.N, n0, a.N, dh[k]);
-        if (nl == 0) a.sumd[bchunk * a.dim + d0 + ch + k] = sumd[k];
-      }
+    for (int e = 0; e < 2; ++e)
+      if (nl == 0 && ch + e < nch) a.sumd[bchunk * a.dim + d0 + ch + e] = v[e];
     if (threadIdx.x == 0) a.cut[bchunk] = any_cut;               // the same from every block
   } else {
     for (int t = max(t_lo, t_live); t < t_hi; ++t) {             // tokens that are not there
@@ -339,25 +380,20 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
       for (int q = threadIdx.x; q < 2 * a.N; q += NT)
         a.part_bc[(((static_cast<int64_t>(sub) * a.batch + b) * a.T + t) * a.G + g) * (2 * a.N) + q] = 0.0f;
     }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (ch + k < nch) {
-        const int64_t row = static_cast<int64_t>(d0 + ch + k) * a.N;
-        if (a.dstate && a.chunks == 1) store_state4(a.dstate + static_cast<int64_t>(b) * a.dim * a.N + row, n0, a.N, dh[k]);
-        store_state4(a.part_a + bchunk * a.dim * a.N + row, n0, a.N, dA[k]);
-      }
+    if (a.dstate && a.chunks == 1) store_h(a.dstate + b * per_row, dh);
+    store_h(a.part_a + bchunk * per_row, dA);
     // the channels' sums over the threads that share them: within the warp, then in warp order
-    constexpr int kSpan = CH / VE, kWide = kSpan < 32 ? 32 : kSpan, kRows = NT / kWide;
+    constexpr int kWide = kQuads < 32 ? 32 : kQuads, kRows = NT / kWide;
     static_assert(kRows <= R, "the sums of a block fit one array of the tile");
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
+    for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int off = 16; off >= kSpan; off /= 2) {
+      for (int off = 16; off >= kQuads; off /= 2) {
         sD[j] += __shfl_xor_sync(0xffffffffu, sD[j], off);
         sV[j] += __shfl_xor_sync(0xffffffffu, sV[j], off);
       }
-      if (kSpan >= 32 || lane < kSpan) {
+      if (kQuads >= 32 || lane < kQuads) {
         sm.delta[(threadIdx.x / kWide) * CH + ec + j] = sD[j];
         sm.u[(threadIdx.x / kWide) * CH + ec + j] = sV[j];
       }
@@ -445,7 +481,7 @@ __global__ void __launch_bounds__(256) finish_weights_kernel(ScanArgs a) {
   }
 }
 
-template <typename T, int LN, bool kAsync> int launch_grad(const ScanArgs& a, cudaStream_t s) {
+template <typename T, int LN> int launch_grad(const ScanArgs& a, cudaStream_t s) {
   using L = GradLayout<T, LN>;
   const int bpg = static_cast<int>(surfk::ceil_div(a.dim / a.G, L::CH));
   const int64_t gx = static_cast<int64_t>(bpg) * a.G * a.batch;
@@ -453,12 +489,12 @@ template <typename T, int LN, bool kAsync> int launch_grad(const ScanArgs& a, cu
   constexpr size_t smem = sizeof(typename L::Smem);
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(a.chunks));
   if (a.chunks > 1) {
-    if (const int rc = allow_smem<scan_grad_kernel<T, LN, kAsync, true>>(smem)) return rc;
-    scan_grad_kernel<T, LN, kAsync, true><<<grid, L::NT, smem, s>>>(a, bpg);
+    if (const int rc = allow_smem<scan_grad_kernel<T, LN, true>>(smem)) return rc;
+    scan_grad_kernel<T, LN, true><<<grid, L::NT, smem, s>>>(a, bpg);
     grad_carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(static_cast<int64_t>(a.batch) * a.dim * a.N, 256)), 256, 0, s>>>(a);
   }
-  if (const int rc = allow_smem<scan_grad_kernel<T, LN, kAsync, false>>(smem)) return rc;
-  scan_grad_kernel<T, LN, kAsync, false><<<grid, L::NT, smem, s>>>(a, bpg);
+  if (const int rc = allow_smem<scan_grad_kernel<T, LN, false>>(smem)) return rc;
+  scan_grad_kernel<T, LN, false><<<grid, L::NT, smem, s>>>(a, bpg);
   const int64_t n = static_cast<int64_t>(a.batch) * a.T * a.G * 2 * a.N;
   const int64_t blocks = surfk::ceil_div(n, 256);
   finish_bc_kernel<T><<<static_cast<unsigned>(blocks < 148 * 16 ? (blocks > 0 ? blocks : 1) : 148 * 16), 256, 0, s>>>(a, bpg);
@@ -468,14 +504,13 @@ template <typename T, int LN, bool kAsync> int launch_grad(const ScanArgs& a, cu
 
 }  // namespace
 
-SURF_EXPORT int surf_seq_scan_grad(const void* args, int dtype, int aligned, void* stream) {
+SURF_EXPORT int surf_seq_scan_grad(const void* args, int dtype, void* stream) {
   const ScanArgs a = *static_cast<const ScanArgs*>(args);
   if (a.batch <= 0 || a.dim <= 0) return static_cast<int>(cudaErrorInvalidValue);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_lanes(a.N, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
-    if (dtype == kBf16) return aligned ? launch_grad<bf16, LN, true>(a, s) : launch_grad<bf16, LN, false>(a, s);
-    return aligned ? launch_grad<float, LN, true>(a, s) : launch_grad<float, LN, false>(a, s);
+    return dtype == kBf16 ? launch_grad<bf16, LN>(a, s) : launch_grad<float, LN>(a, s);
   });
 }
 

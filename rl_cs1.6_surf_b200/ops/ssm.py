@@ -38,8 +38,8 @@ _lib.register(SLIB, {
     "surf_seq_conv": (_I, [c_char_p, _I, _I, _I, _V]),
     "surf_seq_conv_grad": (_I, [c_char_p, _I, _I, _I, _I, _V, _V, _V]),
     "surf_seq_conv_step": (_I, [_V, _L, _V, _V, _V, _V, _V, _I, _V, _L, _I, _I, _I, _I, _I, _I, _V, _V]),
-    "surf_seq_scan": (_I, [c_char_p, _I, _I, _V]),
-    "surf_seq_scan_grad": (_I, [c_char_p, _I, _I, _V]),
+    "surf_seq_scan": (_I, [c_char_p, _I, _V]),
+    "surf_seq_scan_grad": (_I, [c_char_p, _I, _V]),
     "surf_seq_scan_grad_blocks": (_I, [_I, _I]),
     "surf_seq_scan_step": (_I, [c_char_p, _I, _V]),
     "surf_seq_args_size": (_I, [_I]),
@@ -53,7 +53,7 @@ Scan = namedtuple("Scan", "out final saved")
 ScanGrads = namedtuple("ScanGrads", "dx ddt dz dB dC dA dD ddt_bias dstate")
 
 _CONV = struct.Struct("18q6i")
-_SCAN = struct.Struct("48q8i")
+_SCAN = struct.Struct("48q10i")
 _STEP = struct.Struct("21q6i")
 
 
@@ -267,16 +267,24 @@ def _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths):
     return code, b, t, d, n, g
 
 
-def _scan_aligned(d, g, n, x, *tensors) -> bool:
-    """16-byte pieces throughout: a group's channels, its states and every row."""
-    v = 16 // x.element_size()
-    return (d // g) % v == 0 and n % v == 0 and _aligned(v, x, *tensors)
+def _piece(cols: int, *tensors) -> int:
+    """Bytes of the pieces that rows of ``cols`` elements may be copied in (copy_rows): 16
+    or 4 where the row's length, every base and every stride is a multiple of it, else 0."""
+    size = next(t for t in tensors if t is not None).element_size()
+    bits = cols * size
+    for t in tensors:
+        if t is not None:
+            bits |= t.data_ptr()
+            for n, s in zip(t.shape[:-1], t.stride()):
+                if n > 1:
+                    bits |= s * size
+    return 16 if bits % 16 == 0 else 4 if bits % 4 == 0 else 0
 
 
 def _chunks(b: int, t: int, d: int, n: int, g: int):
     """(tokens of a chunk, chunks): a row is cut only where its channels do not fill the GPU."""
     lanes = 1 if n <= 4 else 2 if n <= 8 else 4 if n <= 16 else 8 if n <= 32 else 16
-    per_block = 128 // lanes * min(lanes, 4)
+    per_block = 128 // lanes * (4 if lanes >= 4 else 2)
     blocks = b * g * -(-(d // g) // per_block)
     want = max(1, min(592 // blocks if blocks else 1, t // 64))
     if want <= 1:
@@ -320,10 +328,10 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
         x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
         0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
-        0, 0, out.stride(0), out.stride(1), t, b, t, d, n, g, int(softplus), chunk, chunks)
-    aligned = _scan_aligned(d, g, n, x, dt, z, B, C, out)
+        0, 0, out.stride(0), out.stride(1), t, b, t, d, n, g, int(softplus), chunk, chunks,
+        _piece(d // g, x, dt, z, out), _piece(n, B, C))
     with _on_device(x):
-        check(_lib.lib(SLIB).surf_seq_scan(args, code, int(aligned), stream_ptr(dev)), "surf_seq_scan")
+        check(_lib.lib(SLIB).surf_seq_scan(args, code, stream_ptr(dev)), "surf_seq_scan")
     if chunks > 1:
         _lib.add_launches(2)
     return Scan(out, final, saved)
@@ -376,10 +384,10 @@ def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A
         part_a.data_ptr() + 4 * b * chunks * d * n, dA.data_ptr(), _p(dD), _p(dbias), _p(dstate),
         x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
         0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
-        dout.stride(0), dout.stride(1), 0, 0, t, b, t, d, n, g, int(softplus), chunk, chunks)
-    aligned = _scan_aligned(d, g, n, x, dt, z, B, C, dout)
+        dout.stride(0), dout.stride(1), 0, 0, t, b, t, d, n, g, int(softplus), chunk, chunks,
+        _piece(d // g, x, dt, z, dout), _piece(n, B, C))
     with _on_device(x):
-        check(L.surf_seq_scan_grad(args, code, int(aligned), stream_ptr(dev)), "surf_seq_scan_grad")
+        check(L.surf_seq_scan_grad(args, code, stream_ptr(dev)), "surf_seq_scan_grad")
     _lib.add_launches(4 if chunks > 1 else 2)
     return ScanGrads(dx, ddt, dz, dB, dC, dA, dD, dbias, dstate)
 
