@@ -132,6 +132,16 @@ __device__ __forceinline__ float softplus(float v) {
   return fmaf(2.0f * s, g, fmaxf(v, 0.0f));
 }
 
+// dt -> delta for 4 channels
+__device__ __forceinline__ void step_of(float (&v)[4], const float (&bias)[4], int through_softplus) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] += bias[j];
+  if (through_softplus) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = softplus(v[j]);
+  }
+}
+
 // ---- pairs of floats in one 64-bit register: one instruction for both ---------------
 struct f2 { unsigned long long v; };
 __device__ __forceinline__ f2 pack2(float lo, float hi) {

@@ -136,33 +136,36 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
   }
 
   bool any_cut = false;
-  fetch(t_lo, 0);
-  int buf = 0;
-  for (int t0 = t_lo; t0 < t_live; t0 += kTile, buf ^= 1) {
+  int buf = 1;
+  for (int t0 = t_lo - kTile; t0 < t_live; t0 += kTile, buf ^= 1) {
     cp_async_wait<0>();
     __syncthreads();
     fetch(t0 + kTile, buf ^ 1);
+    if (t0 < t_lo) continue;                             // the first round only fetches
     const int rows = min(kTile, t_live - t0);
     // bit r: token r starts an episode (every warp finds them for itself)
     static_assert(kTile <= 32, "a warp's lanes look at a tile's tokens");
     const unsigned cuts = __ballot_sync(0xffffffffu, reset && lane < rows && reset[t0 + lane]);
     any_cut |= cuts != 0;
-    // delta and delta * x; zeros past the tile's last token, where the state then stays as it is
-#pragma unroll 4
+    // delta and delta * x (channels past the block's last are never looked at)
+#pragma unroll 2
     for (int r = er; r < kTile; r += kStep) {
-      float dv[4], xv[4], uv[4];
+      float dv[4], xv[4];
       load_vec<T, 4>(sm.dt[buf] + r * CH + ec, dv);
       load_vec<T, 4>(sm.x[buf] + r * CH + ec, xv);
+      step_of(dv, bias, a.softplus);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        dv[j] += bias[j];
-        if (a.softplus) dv[j] = softplus(dv[j]);
-        const bool in = r < rows && ec + j < nch;
-        dv[j] = in ? dv[j] : 0.0f;
-        uv[j] = in ? dv[j] * xv[j] : 0.0f;
-      }
+      for (int j = 0; j < 4; ++j) xv[j] *= dv[j];
       store_vec<float, 4>(sm.delta + r * CH + ec, dv);
-      store_vec<float, 4>(sm.u + r * CH + ec, uv);
+      store_vec<float, 4>(sm.u + r * CH + ec, xv);
+    }
+    if (rows < kTile) {                                  // past the last token the state stays as it is
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int r = er; r < kTile; r += kStep)
+        if (r >= rows) {
+          store_vec<float, 4>(sm.delta + r * CH + ec, zero);
+          store_vec<float, 4>(sm.u + r * CH + ec, zero);
+        }
     }
     for (int i = threadIdx.x; i < kTile * NP; i += kThreads) {
       const int r = i / NP, n = i % NP;
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
     }
     __syncthreads();
     if (!kCarry) {
-#pragma unroll 4
+#pragma unroll 2
       for (int r = er; r < rows; r += kStep) {
         if (ec >= nch) break;
         float o[4], xv[4];

@@ -31,6 +31,7 @@ template <typename T, int LN> struct GradLayout {
   struct Smem {
     alignas(16) T x[2][R * CH], dt[2][R * CH], z[2][R * CH], dout[2][R * CH], B[2][R * NP], C[2][R * NP];
     alignas(16) float delta[R * CH], u[R * CH], g[R * CH], y[R * CH], ub[R * CH], qa[R * CH];
+    alignas(16) float dgate[R * CH], dstep[R * CH];       // dout silu'(z), d delta / d dt
     alignas(16) float Bd[R * NP * 2], Cd[R * NP * 2];     // 32-bit, every value twice
     alignas(16) float red[NT / 32][R][2 * NP];            // the warps' sums of dB and dC
     alignas(16) float bias[CH], skip[CH];
@@ -169,39 +170,50 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
 
   bool any_cut = false;
   const int last = t_live > t_lo ? t_lo + (t_live - 1 - t_lo) / R * R : t_lo - R;
-  fetch(last, 0);
-  int buf = 0;
-  for (int t0 = last; t0 >= t_lo; t0 -= R, buf ^= 1) {
+  int buf = 1;
+  for (int t0 = last + R; t0 >= t_lo; t0 -= R, buf ^= 1) {
     f2 h[R + 1][4];                                        // h[r]: the state before token r, h[R] behind the last
-    if (!kCarry) load_h(saved + t0 / kSave * per_row, h[0], 1.0f);
+    if (!kCarry && t0 <= last) load_h(saved + t0 / kSave * per_row, h[0], 1.0f);
     cp_async_wait<0>();
     __syncthreads();
     fetch(t0 - R, buf ^ 1);
+    if (t0 > last) continue;                               // the first round only fetches
     const int rows = min(R, t_live - t0);
     // bit r: token r starts an episode (every warp finds them for itself)
     const unsigned cuts = __ballot_sync(0xffffffffu, reset && lane < rows && reset[t0 + lane]);
     any_cut |= cuts != 0;
     for (int r = er; r < R; r += kStep) {
-      float dv[4], gv[4], uv[4], bias[4];
+      float dv[4], gv[4], uv[4], dg[4], ds[4], bias[4];
       const int at = r * CH + ec;
       load_vec<float, 4>(sm.bias + ec, bias);
       load_vec<T, 4>(sm.dt[buf] + at, dv);
       load_vec<T, 4>(sm.dout[buf] + at, gv);
-      if (!kCarry) load_vec<T, 4>(sm.x[buf] + at, uv);
       if (gz) {
         float zv[4];
         load_vec<T, 4>(sm.z[buf] + at, zv);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) gv[j] *= zv[j] * sigmoid(zv[j]);
+        for (int j = 0; j < 4; ++j) {
+          const float s = sigmoid(zv[j]), w = gv[j] * s;
+          dg[j] = w * fmaf(zv[j], 1.0f - s, 1.0f);
+          gv[j] = w * zv[j];
+        }
+        if (!kCarry) store_vec<float, 4>(sm.dgate + at, dg);
       }
+      if (!kCarry && a.softplus) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        dv[j] += bias[j];
-        if (a.softplus) dv[j] = softplus(dv[j]);
-        const bool in = r < rows && ec + j < nch;          // past the last token nothing changes
-        dv[j] = in ? dv[j] : 0.0f;
-        gv[j] = in ? gv[j] : 0.0f;
-        uv[j] = !kCarry && in ? dv[j] * uv[j] : 0.0f;
+        for (int j = 0; j < 4; ++j) ds[j] = sigmoid(dv[j] + bias[j]);
+        store_vec<float, 4>(sm.dstep + at, ds);
+      }
+      step_of(dv, bias, a.softplus);
+      if (!kCarry) {
+        load_vec<T, 4>(sm.x[buf] + at, uv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) uv[j] *= dv[j];
+      }
+      if (r >= rows || ec + 4 > nch) {                     // what is not there adds nothing and changes nothing
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (r >= rows || ec + j >= nch) dv[j] = gv[j] = uv[j] = 0.0f;
       }
       store_vec<float, 4>(sm.delta + at, dv);
       store_vec<float, 4>(sm.g + at, gv);
@@ -315,38 +327,38 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
       __syncthreads();
       for (int r = er; r < rows; r += kStep) {
         if (ec >= nch) break;
-        float xv[4], tv[4], ov[4], gv[4], dl[4], y[4], ub[4], qa[4], dx[4], ddt[4], bias[4], skip[4];
-        load_vec<float, 4>(sm.bias + ec, bias);
-        load_vec<float, 4>(sm.skip + ec, skip);
+        float xv[4], gv[4], dl[4], y[4], ub[4], qa[4], dx[4], ddt[4], skip[4];
         const int at = r * CH + ec;
         const int64_t o = static_cast<int64_t>(t0 + r) * a.dim + ec;
         load_vec<T, 4>(sm.x[buf] + at, xv);
-        load_vec<T, 4>(sm.dt[buf] + at, tv);
+        load_vec<float, 4>(sm.skip + ec, skip);
+        if (gz) {
+          float dz[4];
+          load_vec<float, 4>(sm.y + at, y);
+          load_vec<float, 4>(sm.dgate + at, dz);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dz[j] *= fmaf(skip[j], xv[j], y[j]);
+          store_quad<T>(gdz + o, dz, nch - ec, a.mode_d == kPieces16);
+        }
         load_vec<float, 4>(sm.g + at, gv);
         load_vec<float, 4>(sm.delta + at, dl);
         load_vec<float, 4>(sm.ub + at, ub);
         load_vec<float, 4>(sm.qa + at, qa);
-        if (gz) {
-          float zv[4], dz[4];
-          load_vec<T, 4>(sm.z[buf] + at, zv);
-          load_vec<T, 4>(sm.dout[buf] + at, ov);
-          load_vec<float, 4>(sm.y + at, y);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float s = sigmoid(zv[j]);
-            dz[j] = ov[j] * fmaf(skip[j], xv[j], y[j]) * s * fmaf(zv[j], 1.0f - s, 1.0f);
-          }
-          store_quad<T>(gdz + o, dz, nch - ec, a.mode_d == kPieces16);
-        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           dx[j] = fmaf(ub[j], dl[j], gv[j] * skip[j]);
           ddt[j] = fmaf(ub[j], xv[j], qa[j] * kLn2);
-          if (a.softplus) ddt[j] *= sigmoid(tv[j] + bias[j]);
-          if (ec + j < nch) {
-            sD[j] = fmaf(gv[j], xv[j], sD[j]);
-            sV[j] += ddt[j];
-          }
+        }
+        if (a.softplus) {
+          float ds[4];
+          load_vec<float, 4>(sm.dstep + at, ds);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ddt[j] *= ds[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {                      // channels past the last are never looked at
+          sD[j] = fmaf(gv[j], xv[j], sD[j]);
+          sV[j] += ddt[j];
         }
         store_quad<T>(gdx + o, dx, nch - ec, a.mode_d == kPieces16);
         store_quad<T>(gddt + o, ddt, nch - ec, a.mode_d == kPieces16);
