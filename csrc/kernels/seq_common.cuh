@@ -97,13 +97,15 @@ __device__ __forceinline__ void copy_rows(T* dst, const T* src, int64_t stride, 
 }
 
 // ---- launches -----------------------------------------------------------------------
-// Raises the kernel's dynamic shared-memory limit once per device.
-template <auto Kern> int allow_smem(size_t bytes) {
+// Raises the kernel's dynamic shared-memory limit (and, if wide, its cluster limit to 16
+// blocks) once per device.
+template <auto Kern, bool kWide = false> int allow_smem(size_t bytes) {
   static bool done[64] = {};
   int dev = 0;
   if (const cudaError_t e = cudaGetDevice(&dev)) return static_cast<int>(e);
   if (dev < 64 && done[dev]) return 0;
-  const cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (kWide && e == cudaSuccess) e = cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess && dev < 64) done[dev] = true;
   return static_cast<int>(e);
 }

@@ -150,36 +150,50 @@ template <typename T> __global__ void __launch_bounds__(128) small_kernel(TokenA
 // ---- many candidates: a cluster of CS blocks, the row's slices in shared memory -----------
 // One exponential per candidate: e is kept in shared memory in the logit's place, and all
 // later passes work on its bits (e orders the candidates except where several logits share
-// an e; only there the logits are looked at again).
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kMaxSlice = 32768;
-constexpr int kBinShift = 17;                        // 64 bins an octave of e, 40 octaves
-constexpr int kBins = 2592;                          // > 40 * 64, whole shares for 1, 2, 4, 8 blocks
-constexpr int kList = 1024;
+// an e; only there the logits are looked at again). What bounds it is the number of
+// instructions for a candidate, about 25 for the exponential and the weight, 20 for the
+// histogram and 15 for the sums of what is kept: small blocks (4 on an SM) so that the
+// phases of one fill the waits of another.
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxCluster = 16, kMaxSlice = 16384;
+constexpr int kBinShift = 18;                        // 32 bins an octave of e, 40 octaves
+constexpr int kBins = 1312;                          // > 40 * 32, whole shares for 1 .. 16 blocks
+constexpr int kList = 512;
+constexpr int kAllKept = 1 << 30, kNoBin = -1;
 
-struct Found { u64 mass_before; unsigned count_before, count; int bin; };
-struct Cut { uint32_t key; unsigned count_before; u64 ties, mass_upto; };     // kept: keys above, `ties` equal ones
+struct Found { u64 mass_before; unsigned count_before; int bin; };
+struct Cut { u64 ties, mass_upto; uint32_t key; unsigned pad; };     // kept: keys above, `ties` equal ones
 
 struct TokenSmem {
-  unsigned hist_lo[kBins], hist_hi[kBins], hist_c[kBins];      // weight in two words, count
-  u64 list_w[kList];
-  uint32_t list_key[kList];
+  unsigned hist_lo[kBins + 1], hist_hi[kBins + 1], hist_c[kBins + 1];      // weight in two words, count
+  uint32_t list_key[kList], list_e[kList];           // of the bin where the limit falls
   int list_at[kList];
-  u64 warp_m[kWarps], share_m[8], x_m[8];
-  unsigned warp_c[kWarps], share_c[8], x_c[8];
-  float x_max[8], red[kWarps];
+  u64 warp_m[kWarps], share_m[kMaxCluster], x_m[kMaxCluster];
+  unsigned warp_c[kWarps], share_c[kMaxCluster], x_c[kMaxCluster];
+  float x_max[kMaxCluster], red[kWarps];
   Found found;
   Cut cut;
   unsigned list_n;
 };
 
-// w = floor(e * 2^40) from the bits of e in [0, 1]
-__device__ __forceinline__ u64 weight_of_bits(uint32_t e) {
-  return (static_cast<u64>((e & 0x7fffffu) | 0x800000u) << 17) >> min(127u - (e >> 23), 63u);
-}
 __device__ __forceinline__ int bin_of_bits(uint32_t e) { return static_cast<int>((0x3f800000u - e) >> kBinShift); }
 
-template <typename T, int CS> __global__ void __launch_bounds__(kThreads) large_kernel(TokenArgs a, int slice) {
+// w = floor(e * 2^40), e in [0, 1], as w1 * 2^23 + w0: the additions of 2^23 that round down
+// leave the whole part in the low bits of a float (what is left is exact in between).
+__device__ __forceinline__ void split_weight(float e, uint32_t& w1, uint32_t& w0) {
+  const float t = __fmaf_rd(e, 131072.0f, 8388608.0f);
+  const float rest = __fmaf_rn(e, 131072.0f, -__fsub_rn(t, 8388608.0f));
+  w1 = __float_as_uint(t) - 0x4b000000u;
+  w0 = __float_as_uint(__fmaf_rd(rest, 8388608.0f, 8388608.0f)) - 0x4b000000u;
+}
+__device__ __forceinline__ u64 whole_weight(float e) {
+  uint32_t w1, w0;
+  split_weight(e, w1, w0);
+  return (static_cast<u64>(w1) << 23) + w0;
+}
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+
+template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) large_kernel(TokenArgs a, int slice) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   TokenSmem& sm = *reinterpret_cast<TokenSmem*>(smem_raw);
   float* zs = reinterpret_cast<float*>(smem_raw + (sizeof(TokenSmem) + 15) / 16 * 16);
@@ -207,33 +221,28 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads) large_
   constexpr int W = kVec16<T>;
   const int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T));
   const int off = (W - head) % W;
-  const int total_slots = (off + n + 3) / 4 * 4;
+  const int slots = (off + n + 3) / 4 * 4;
   float mx = -INFINITY;
-  for (int i = threadIdx.x; i < off; i += kThreads) zs[i] = -INFINITY;
-  for (int i = off + n + threadIdx.x; i < total_slots; i += kThreads) zs[i] = -INFINITY;
-  for (int i = threadIdx.x; i < min(head, n); i += kThreads) {
-    const float z = clean(to_f(row[i]));
-    zs[off + i] = z;
-    mx = fmaxf(mx, z);
+  if (threadIdx.x < off) zs[threadIdx.x] = -INFINITY;
+  if (threadIdx.x < slots - off - n) zs[off + n + threadIdx.x] = -INFINITY;
+  if (threadIdx.x < min(head, n)) {
+    zs[off + threadIdx.x] = to_f(row[threadIdx.x]);
+    mx = fmaxf(mx, to_f(row[threadIdx.x]));          // passes NaN over
   }
   const int whole = n > head ? (n - head) / W * W : 0;
-#pragma unroll 2
+#pragma unroll 4
   for (int i = threadIdx.x * W; i < whole; i += kThreads * W) {
     float v[W];
     load_vec<T, W>(row + head + i, v);
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      v[j] = clean(v[j]);
-      mx = fmaxf(mx, v[j]);
-    }
+    for (int j = 0; j < W; ++j) mx = fmaxf(mx, v[j]);
 #pragma unroll
     for (int j = 0; j < W; j += 4)
       *reinterpret_cast<float4*>(zs + off + head + i + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
   }
-  for (int i = head + whole + threadIdx.x; i < n; i += kThreads) {
-    const float z = clean(to_f(row[i]));
-    zs[off + i] = z;
-    mx = fmaxf(mx, z);
+  if (const int i = head + whole + threadIdx.x; i < n) {
+    zs[off + i] = to_f(row[i]);
+    mx = fmaxf(mx, to_f(row[i]));
   }
   auto clear = [&] {
     for (int i = threadIdx.x; i < kBins; i += kThreads) sm.hist_lo[i] = sm.hist_hi[i] = sm.hist_c[i] = 0;
@@ -241,6 +250,7 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads) large_
   };
   mx = warp_max(mx);
   if (lane == 0) sm.red[warp] = mx;
+  if (threadIdx.x == 0) sm.list_n = 0;
   clear();
   if constexpr (CS > 1) cluster.barrier_wait();
   if (warp == 0) {
@@ -251,7 +261,6 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads) large_
   float m = sm.x_max[0];
 #pragma unroll
   for (int c = 1; c < CS; ++c) m = fmaxf(m, sm.x_max[c]);
-
   if (m == -INFINITY) {                      // the same in every block of the cluster
     if (rank == 0 && threadIdx.x == 0) {
       a.token[id] = -1;
@@ -260,245 +269,308 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads) large_
     return;
   }
 
+  // every warp owns a run of the slice, so that sums over warps are in index order
+  const int run = (slots + kWarps * 128 - 1) / (kWarps * 128) * 128;
+  const int w_lo = min(slots, warp * run), w_hi = min(slots, w_lo + run);
   const bool limited = q.k || q.p < 1.0;
-  auto add = [&](int bin, u64 w) {           // two 32-bit additions: shared memory has no 64-bit one
-    const unsigned w0 = static_cast<unsigned>(w);
-    const unsigned old = atomicAdd(&sm.hist_lo[bin], w0);
-    const unsigned up = static_cast<unsigned>(w >> 32) + (old + w0 < old ? 1u : 0u);
+  auto add = [&](int bin, uint32_t w1, uint32_t w0) {    // two 32-bit additions: shared memory has no 64-bit one
+    const uint32_t x = (w1 << 23) + w0;
+    const unsigned old = atomicAdd(&sm.hist_lo[bin], x);
+    const unsigned up = (w1 >> 9) + (old + x < old ? 1u : 0u);
     if (up) atomicAdd(&sm.hist_hi[bin], up);
     if (q.k) atomicAdd(&sm.hist_c[bin], 1u);
   };
-  // logits -> e; weights into the histogram
-  for (int i = threadIdx.x * 4; i < total_slots; i += kThreads * 4) {
-    float4 v = *reinterpret_cast<float4*>(zs + i);
+  // logits -> e (0 for NaN and what min_p drops); weights into the histogram, or summed
+  const bool plain = m < INFINITY && q.inv < INFINITY;   // else equal logits need below()
+  uint32_t s1 = 0, s0 = 0;
+  u64 above = 0;
+  for (int i = w_lo + lane * 4; i < w_hi; i += 128) {
+    const float4 v = *reinterpret_cast<const float4*>(zs + i);
     float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float z = e[j];
-      e[j] = expf(below(z, m, q.inv));
-      if (!(e[j] >= q.min_p) || z == -INFINITY) e[j] = 0.0f;
+      e[j] = expf(plain ? __fmul_rn(__fsub_rn(e[j], m), q.inv) : below(e[j], m, q.inv));
+      if (!(e[j] >= q.min_p)) e[j] = 0.0f;
     }
     *reinterpret_cast<float4*>(zs + i) = make_float4(e[0], e[1], e[2], e[3]);
+    uint32_t w1[4], w0[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split_weight(e[j], w1[j], w0[j]);
     if (limited) {
+      // four additions in flight; what has no weight goes to a bin that nobody reads
+      unsigned old[4];
+      int bin[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t bits = __float_as_uint(e[j]);
-        const u64 w = weight_of_bits(bits);
-        if (w) add(bin_of_bits(bits), w);
+        bin[j] = min(bin_of_bits(__float_as_uint(e[j])), kBins);
+        old[j] = atomicAdd(&sm.hist_lo[bin[j]], (w1[j] << 23) + w0[j]);
+      }
+      if (q.k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) atomicAdd(&sm.hist_c[bin[j]], 1u);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = (w1[j] << 23) + w0[j];
+        const unsigned up = (w1[j] >> 9) + (old[j] + x < old[j] ? 1u : 0u);
+        if (up) atomicAdd(&sm.hist_hi[bin[j]], up);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s1 += w1[j];                         // at most kMaxSlice / 256 of 2^17 and 2^23
+        s0 += w0[j];
       }
     }
   }
+  above = (static_cast<u64>(s1) << 23) + s0;
   __syncthreads();
-  auto rebuild = [&] {
-    clear();
-    for (int i = threadIdx.x; i < total_slots; i += kThreads) {
-      const uint32_t bits = __float_as_uint(zs[i]);
-      const u64 w = weight_of_bits(bits);
-      if (w) add(bin_of_bits(bits), w);
-    }
-  };
 
-  // The first bin at which the running weight (by_mass) or count reaches `lim`, over the
-  // cluster's histograms; total_m, total_c: all of them. A block sums its share of the bins
-  // over the cluster; the block whose share holds the bin tells the others.
-  u64 total_m = 0;
-  unsigned total_c = 0;
-  constexpr int kShare = kBins / CS, kEach = (kShare + kThreads - 1) / kThreads;
-  auto find = [&](auto limit_of, u64 at_m, unsigned at_c) {
-    sync();
-    u64 bm[kEach], tm = 0;
-    unsigned bc[kEach], tc = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      bm[j] = 0;
-      bc[j] = 0;
-      const int bin = threadIdx.x * kEach + j;
-      if (bin < kShare) {
-#pragma unroll
-        for (int c = 0; c < CS; ++c) {
-          bm[j] += (static_cast<u64>(peer(sm.hist_hi, c)[rank * kShare + bin]) << 32) + peer(sm.hist_lo, c)[rank * kShare + bin];
-          if (q.k) bc[j] += peer(sm.hist_c, c)[rank * kShare + bin];
-        }
-      }
-      tm += bm[j];
-      tc += bc[j];
-    }
-    const u64 s_m = warp_scan(tm, lane);
-    const unsigned s_c = warp_scan(tc, lane);
-    if (lane == 31) {
-      sm.warp_m[warp] = s_m;
-      sm.warp_c[warp] = s_c;
-    }
-    __syncthreads();
-    u64 all_m = 0, cm = s_m - tm;
-    unsigned all_c = 0, cc = s_c - tc;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) {
-        cm += sm.warp_m[w];
-        cc += sm.warp_c[w];
-      }
-      all_m += sm.warp_m[w];
-      all_c += sm.warp_c[w];
-    }
-    if (threadIdx.x < CS) {
-      peer(sm.share_m, threadIdx.x)[rank] = all_m;
-      peer(sm.share_c, threadIdx.x)[rank] = all_c;
-    }
-    if (threadIdx.x == 0) sm.found.bin = -1;
-    sync();
-    total_m = at_m;
-    total_c = at_c;
-    for (int c = 0; c < CS; ++c) {
-      if (c == rank) {
-        cm += total_m;
-        cc += total_c;
-      }
-      total_m += sm.share_m[c];
-      total_c += sm.share_c[c];
-    }
-    bool by_mass;
-    const u64 lim = limit_of(by_mass);       // may depend on the totals; 0: no limit
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const u64 before = by_mass ? cm : cc, upto = by_mass ? cm + bm[j] : cc + bc[j];
-      if (before < lim && lim <= upto) {
-        const Found f{cm, cc, bc[j], rank * kShare + static_cast<int>(threadIdx.x) * kEach + j};
-        for (int c = 0; c < CS; ++c) *peer(&sm.found, c) = f;
-      }
-      cm += bm[j];
-      cc += bc[j];
-    }
-    sync();
-    return sm.found;
-  };
-
-  bool intact = true;                        // the histogram of e
-  // the place within bin f at which the limit falls
-  auto refine = [&](bool by_mass, u64 lim, Found f) {
-    if (rank == 0 && threadIdx.x == 0) sm.list_n = 0;
-    sync();
-    for (int i = threadIdx.x; i < total_slots; i += kThreads) {
-      const uint32_t bits = __float_as_uint(zs[i]);
-      if (bin_of_bits(bits) == f.bin) {
-        const u64 w = weight_of_bits(bits);
-        if (w) {
-          const unsigned at = atomicAdd(peer(&sm.list_n, 0), 1u);
-          if (at < kList) {
-            peer(sm.list_w, 0)[at] = w;
-            peer(sm.list_key, 0)[at] = key_of(clean(to_f(row[i - off])));
-            peer(sm.list_at, 0)[at] = lo + i - off;
-          }
-        }
-      }
-    }
-    sync();
-    const unsigned listed = *peer(&sm.list_n, 0);
-    if (listed <= kList) {                   // few: their order by counting, in the first block
-      if (rank == 0) {
-        for (unsigned i = threadIdx.x; i < listed; i += kThreads) {
-          const uint32_t key = sm.list_key[i];
-          const int at = sm.list_at[i];
-          u64 before = f.mass_before;
-          unsigned count = f.count_before, same = 0;
-          for (unsigned j = 0; j < listed; ++j) {
-            const uint32_t kj = sm.list_key[j];
-            const bool equal = kj == key && sm.list_at[j] < at;
-            if (kj > key || equal) {
-              before += sm.list_w[j];
-              ++count;
-            }
-            same += equal;
-          }
-          const u64 w = sm.list_w[i];
-          if (by_mass ? before < lim && lim <= before + w : count + 1 == lim) {
-            const Cut cut{key, count, static_cast<u64>(same) + 1, before + w};
-            for (int c = 0; c < CS; ++c) *peer(&sm.cut, c) = cut;
-          }
-        }
-      }
-      sync();
-      return sm.cut;
-    }
-    // many (equal or nearly equal logits): three digits of the key, by histograms
-    intact = false;
-    uint32_t prefix = 0;
-    const int b0 = f.bin;
-    Found g = f;
-    for (int level = 0; level < 3; ++level) {
-      const int shift = level == 0 ? 21 : (level == 1 ? 10 : 0), width = level == 2 ? 1024 : 2048;
-      clear();
-      for (int i = threadIdx.x; i < total_slots; i += kThreads) {
-        const uint32_t bits = __float_as_uint(zs[i]);
-        const u64 w = bin_of_bits(bits) == b0 ? weight_of_bits(bits) : 0;
-        if (w) {
-          const uint32_t key = key_of(clean(to_f(row[i - off])));
-          if (level == 0 || key >> (level == 1 ? 21 : 10) == prefix) add(width - 1 - static_cast<int>((key >> shift) & (width - 1)), w);
-        }
-      }
-      g = find([&](bool& mass) { mass = by_mass; return lim; }, g.mass_before, g.count_before);
-      prefix = (prefix << (level == 2 ? 10 : 11)) | static_cast<uint32_t>(width - 1 - g.bin);
-    }
-    // all keys here are equal, and so are their weights
-    const u64 each = weight_of_bits(__float_as_uint(expf(below(__uint_as_float(prefix & 0x80000000u ? prefix & 0x7fffffffu : ~prefix), m, q.inv))));
-    const u64 ties = by_mass ? (lim - g.mass_before + each - 1) / each : lim - g.count_before;
-    return Cut{prefix, g.count_before, ties, g.mass_before + ties * each};
-  };
-
-  // kept: keys above the cut's, and the first `ties` of those equal to it
-  Cut cut{0, 0, ~0ull, 0};
-  uint32_t e_cut = 0;
+  // Kept: everything in bins below `edge`; in bin `edge`, keys above the cut's and the first
+  // `ties` of those equal to it.
+  Cut cut{~0ull, 0, 0, 0};
+  int edge = kAllKept;
+  u64 tie_w = 0;
+  unsigned listed = 0;
+  bool by_list = true;
   if (limited) {
-    u64 lim = 0;
-    bool by_mass = true;
-    Found f = find([&](bool& mass) {
-      by_mass = !(q.k && total_c > static_cast<unsigned>(q.k));
-      mass = by_mass;
-      lim = by_mass ? (q.p < 1.0 ? mass_limit(q.p, total_m) : 0) : static_cast<u64>(q.k);
-      return lim;
-    }, 0, 0);
-    if (lim) {
-      cut = refine(by_mass, lim, f);
-      if (!by_mass && q.p < 1.0) {
-        lim = mass_limit(q.p, cut.mass_upto);
-        if (!intact) rebuild();
-        f = find([&](bool& mass) { mass = true; return lim; }, 0, 0);
-        cut = refine(true, lim, f);
+    u64 lim = 0;                             // 0: from the totals
+    bool by_mass = true, intact = true, got;
+    int level = -1;                          // of the key's digits, where the list is too short
+    uint32_t prefix = 0;
+    Found f{0, 0, 0};
+    constexpr int kShare = kBins / CS, kEach = (kShare + kThreads - 1) / kThreads;
+    for (;;) {
+      // The first bin at which the running weight (or count) reaches the limit, over the
+      // cluster's histograms: a block sums its share of the bins over the cluster, the block
+      // whose share holds the bin tells the others.
+      sync();
+      {
+        u64 bm[kEach], tm = 0;
+        unsigned bc[kEach], tc = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          bm[j] = 0;
+          bc[j] = 0;
+          const int bin = threadIdx.x * kEach + j;
+          if (bin < kShare) {
+#pragma unroll 8
+            for (int c = 0; c < CS; ++c) {
+              bm[j] += (static_cast<u64>(peer(sm.hist_hi, c)[rank * kShare + bin]) << 32) + peer(sm.hist_lo, c)[rank * kShare + bin];
+              if (q.k) bc[j] += peer(sm.hist_c, c)[rank * kShare + bin];
+            }
+          }
+          tm += bm[j];
+          tc += bc[j];
+        }
+        const u64 scan_m = warp_scan(tm, lane);
+        const unsigned scan_c = warp_scan(tc, lane);
+        if (lane == 31) {
+          sm.warp_m[warp] = scan_m;
+          sm.warp_c[warp] = scan_c;
+        }
+        __syncthreads();
+        u64 all_m = 0, cm = scan_m - tm;
+        unsigned all_c = 0, cc = scan_c - tc;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) {
+            cm += sm.warp_m[w];
+            cc += sm.warp_c[w];
+          }
+          all_m += sm.warp_m[w];
+          all_c += sm.warp_c[w];
+        }
+        if (threadIdx.x < CS) {
+          peer(sm.share_m, threadIdx.x)[rank] = all_m;
+          peer(sm.share_c, threadIdx.x)[rank] = all_c;
+        }
+        if (threadIdx.x == 0) sm.found.bin = kNoBin;
+        sync();
+        u64 total_m = f.mass_before;
+        unsigned total_c = f.count_before;
+        for (int c = 0; c < CS; ++c) {
+          if (c == rank) {
+            cm += total_m;
+            cc += total_c;
+          }
+          total_m += sm.share_m[c];
+          total_c += sm.share_c[c];
+        }
+        if (!lim) {
+          by_mass = !(q.k && total_c > static_cast<unsigned>(q.k));
+          lim = by_mass ? (q.p < 1.0 ? mass_limit(q.p, total_m) : 0) : static_cast<u64>(q.k);
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          const u64 before = by_mass ? cm : cc, upto = by_mass ? cm + bm[j] : cc + bc[j];
+          if (before < lim && lim <= upto) {
+            const Found at{cm, cc, rank * kShare + static_cast<int>(threadIdx.x) * kEach + j};
+            for (int c = 0; c < CS; ++c) *peer(&sm.found, c) = at;
+          }
+          cm += bm[j];
+          cc += bc[j];
+        }
+        sync();
+        f = sm.found;
       }
-      e_cut = __float_as_uint(expf(below(__uint_as_float(cut.key & 0x80000000u ? cut.key & 0x7fffffffu : ~cut.key), m, q.inv)));
+      if (level < 0) {
+        // the sums of what is surely kept, and the candidates of the bin where the limit falls
+        edge = lim ? f.bin : kAllKept;
+        s1 = s0 = 0;
+        for (int i = w_lo + lane * 4; i < w_hi; i += 128) {
+          const float4 v = *reinterpret_cast<const float4*>(zs + i);
+          const float e[4] = {v.x, v.y, v.z, v.w};
+          bool in_edge = false;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int bin = bin_of_bits(__float_as_uint(e[j]));
+            uint32_t w1, w0;
+            split_weight(e[j], w1, w0);
+            s1 += bin < edge ? w1 : 0u;
+            s0 += bin < edge ? w0 : 0u;
+            in_edge |= bin == edge;
+          }
+          if (in_edge) {
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t bits = __float_as_uint(zs[i + j]);
+              if (bin_of_bits(bits) != edge || !whole_weight(__uint_as_float(bits))) continue;
+              const unsigned at = atomicAdd(peer(&sm.list_n, 0), 1u);
+              if (at < kList) {
+                peer(sm.list_e, 0)[at] = bits;
+                peer(sm.list_key, 0)[at] = key_of(clean(to_f(row[i + j - off])));
+                peer(sm.list_at, 0)[at] = lo + i + j - off;
+              }
+            }
+          }
+        }
+        above = (static_cast<u64>(s1) << 23) + s0;
+        if (!lim) break;
+        sync();
+        listed = *peer(&sm.list_n, 0);
+        got = listed <= kList;
+        if (got) {
+          // their order by counting: a warp for each, all blocks with a copy of the list
+          if (rank != 0) {
+            for (unsigned i = threadIdx.x; i < listed; i += kThreads) {
+              sm.list_key[i] = peer(sm.list_key, 0)[i];
+              sm.list_e[i] = peer(sm.list_e, 0)[i];
+              sm.list_at[i] = peer(sm.list_at, 0)[i];
+            }
+          }
+          __syncthreads();
+          for (unsigned i = rank * kWarps + warp; i < listed; i += CS * kWarps) {
+            const uint32_t key = sm.list_key[i];
+            const int at = sm.list_at[i];
+            u64 before = 0;
+            unsigned count = 0, same = 0;
+            for (unsigned j = lane; j < listed; j += 32) {
+              const uint32_t kj = sm.list_key[j];
+              const bool equal_before = kj == key && sm.list_at[j] < at;
+              if (kj > key || equal_before) {
+                before += whole_weight(__uint_as_float(sm.list_e[j]));
+                ++count;
+              }
+              same += equal_before;
+            }
+            before = f.mass_before + warp_sum(before);
+            count = f.count_before + __reduce_add_sync(0xffffffffu, count);
+            same = __reduce_add_sync(0xffffffffu, same);
+            const u64 w = whole_weight(__uint_as_float(sm.list_e[i]));
+            if ((by_mass ? before < lim && lim <= before + w : count + 1 == lim) && lane < CS)
+              *peer(&sm.cut, lane) = Cut{static_cast<u64>(same) + 1, before + w, key, 0};
+          }
+          sync();
+          cut = sm.cut;
+        } else {
+          level = 0;                         // many equal or nearly equal logits: by the bytes of their keys
+          prefix = 0;
+          intact = false;
+        }
+      } else {
+        prefix = prefix << 8 | static_cast<uint32_t>(255 - f.bin);
+        got = ++level == 4;
+        if (got) {                           // all keys left are equal, and so are their weights
+          const u64 each = whole_weight(expf(below(logit_of(prefix), m, q.inv)));
+          const u64 ties = by_mass ? (lim - f.mass_before + each - 1) / each : lim - f.count_before;
+          cut = Cut{ties, f.mass_before + ties * each, prefix, 0};
+          level = -1;
+        }
+      }
+      if (got) {
+        if (by_mass || q.p >= 1.0) break;
+        by_mass = true;                      // top_p of what top_k has left
+        lim = mass_limit(q.p, cut.mass_upto);
+        f = Found{0, 0, 0};
+        if (rank == 0 && threadIdx.x == 0) sm.list_n = 0;
+        if (!intact) {
+          clear();
+          for (int i = threadIdx.x; i < slots; i += kThreads) {
+            uint32_t w1, w0;
+            split_weight(zs[i], w1, w0);
+            if (w1 | w0) add(bin_of_bits(__float_as_uint(zs[i])), w1, w0);
+          }
+        }
+      } else {
+        clear();
+        for (int i = threadIdx.x; i < slots; i += kThreads) {
+          if (bin_of_bits(__float_as_uint(zs[i])) != edge) continue;
+          uint32_t w1, w0;
+          split_weight(zs[i], w1, w0);
+          if (!(w1 | w0)) continue;
+          const uint32_t key = key_of(clean(to_f(row[i - off])));
+          if (level == 0 || key >> (32 - 8 * level) == prefix) add(255 - static_cast<int>(key >> (24 - 8 * level) & 255u), w1, w0);
+        }
+      }
     }
+    by_list = listed <= kList;
   }
-
-  // the draw: every warp owns a run of the slice, so sums are in index order
-  const int run = (total_slots + kThreads - 1) / kThreads * 32;
-  const int w_lo = min(total_slots, warp * run), w_hi = min(total_slots, w_lo + run);
-  // 0: dropped, 1: above the cut, 2: equal to it
-  auto side = [&](uint32_t bits, int i) {
-    if (!cut.key || bits > e_cut) return 1;
-    if (bits < e_cut) return 0;
+  // 0: dropped, 1: kept, 2: equal to the cut
+  auto side = [&](uint32_t e, int i) {
+    const int bin = bin_of_bits(e);
+    if (bin != edge) return bin < edge ? 1 : 0;
     const uint32_t key = key_of(clean(to_f(row[i - off])));
     return key > cut.key ? 1 : key == cut.key ? 2 : 0;
   };
-  u64 above = 0;
-  unsigned equal = 0;
-#pragma unroll 4
-  for (int i = w_lo + lane; i < w_hi; i += 32) {
-    const uint32_t bits = __float_as_uint(zs[i]);
-    const u64 w = weight_of_bits(bits);
-    if (w) {
-      const int s = side(bits, i);
-      if (s == 1) above += w;
-      else equal += s == 2;
-    }
-  }
+
+  // the runs' sums: what is surely kept, and the shares of the bin with the cut
   above = warp_sum(above);
-  equal = __reduce_add_sync(0xffffffffu, equal);
-  const u64 tie_w = cut.key ? weight_of_bits(e_cut) : 0;
   __syncthreads();
   if (lane == 0) {
     sm.warp_m[warp] = above;
-    sm.warp_c[warp] = equal;
+    sm.warp_c[warp] = 0;
   }
   __syncthreads();
+  if (edge != kAllKept) {
+    tie_w = whole_weight(expf(below(logit_of(cut.key), m, q.inv)));
+    if (by_list) {
+      for (unsigned j = threadIdx.x; j < listed; j += kThreads) {
+        const int i = sm.list_at[j] - lo;
+        const uint32_t key = sm.list_key[j];
+        if (i < 0 || i >= n || key < cut.key) continue;
+        if (key > cut.key) atomicAdd(&sm.warp_m[(off + i) / run], whole_weight(__uint_as_float(sm.list_e[j])));
+        else atomicAdd(&sm.warp_c[(off + i) / run], 1u);
+      }
+    } else {
+      u64 more = 0;
+      unsigned equal = 0;
+      for (int i = w_lo + lane; i < w_hi; i += 32) {
+        const float e = zs[i];
+        if (bin_of_bits(__float_as_uint(e)) != edge) continue;
+        const u64 w = whole_weight(e);
+        const int s = w ? side(__float_as_uint(e), i) : 0;
+        if (s == 1) more += w;
+        equal += s == 2;
+      }
+      more = warp_sum(more);
+      equal = __reduce_add_sync(0xffffffffu, equal);
+      if (lane == 0) {
+        sm.warp_m[warp] += more;
+        sm.warp_c[warp] = equal;
+      }
+    }
+    __syncthreads();
+  }
   if (threadIdx.x < CS) {
     u64 s = 0;
     unsigned c = 0;
@@ -533,9 +605,9 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads) large_
   if (at >= mass_at && at < mass_at + mine) {
     for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
       const int i = i0 + lane;
-      const uint32_t bits = i < w_hi ? __float_as_uint(zs[i]) : 0;
-      u64 w = weight_of_bits(bits);
-      const int s = w ? side(bits, i) : 0;
+      const float e = i < w_hi ? zs[i] : 0.0f;
+      u64 w = whole_weight(e);
+      const int s = w ? side(__float_as_uint(e), i) : 0;
       const unsigned eq = __ballot_sync(0xffffffffu, s == 2);
       if (s == 0 || (s == 2 && ties_at + __popc(eq & ((1u << lane) - 1u)) >= cut.ties)) w = 0;
       ties_at += __popc(eq);
@@ -555,7 +627,7 @@ template <typename T, int CS> int launch_large(const TokenArgs& a, int slice, cu
   const size_t smem = kFixed + static_cast<size_t>(slice) * sizeof(float);
   const int64_t blocks = static_cast<int64_t>(a.rows) * a.heads * CS;
   if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
-  if (const int rc = allow_smem<large_kernel<T, CS>>(kFixed + kMaxSlice * sizeof(float))) return rc;
+  if (const int rc = allow_smem<large_kernel<T, CS>, (CS > 8)>(kFixed + kMaxSlice * sizeof(float))) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kThreads);
@@ -572,21 +644,25 @@ template <typename T, int CS> int launch_large(const TokenArgs& a, int slice, cu
 }
 
 template <typename T> int launch_tokens(const TokenArgs& a, int widest, cudaStream_t s) {
+  const int64_t answers = static_cast<int64_t>(a.rows) * a.heads;
   if (widest <= 32) {
-    const int64_t blocks = surfk::ceil_div(static_cast<int64_t>(a.rows) * a.heads, 4);
+    const int64_t blocks = surfk::ceil_div(answers, 4);
     if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
     small_kernel<T><<<static_cast<unsigned>(blocks), 128, 0, s>>>(a);
     SURF_RETURN_LAUNCH();
   }
+  // slices of at most 8192 candidates (32 a thread, 4 blocks on an SM); smaller ones, down to
+  // 1024, while there are too few blocks to fill the GPU
   int cs = 1;
-  while (cs < 8 && widest > cs * 8192) cs *= 2;
+  while (cs < kMaxCluster && (widest > cs * 8192 || (answers * cs < 2 * 148 && widest > cs * 1024))) cs *= 2;
   const int slice = static_cast<int>(surfk::ceil_div(widest, cs));
   if (slice > kMaxSlice) return static_cast<int>(cudaErrorInvalidValue);
   switch (cs) {
     case 1: return launch_large<T, 1>(a, slice, s);
     case 2: return launch_large<T, 2>(a, slice, s);
     case 4: return launch_large<T, 4>(a, slice, s);
-    default: return launch_large<T, 8>(a, slice, s);
+    case 8: return launch_large<T, 8>(a, slice, s);
+    default: return launch_large<T, 16>(a, slice, s);
   }
 }
 

@@ -31,7 +31,7 @@ SLIB = "libsurf_seq.so"
 _V, _I = _lib._V, _lib._I
 _lib.register(SLIB, {"surf_sample_tokens": (_I, [c_char_p, _I, _I, _V])})
 
-MAX_HEADS, MAX_VOCAB = 16, 8 * 32768
+MAX_HEADS, MAX_VOCAB = 16, 16 * 16384
 _ARGS = struct.Struct("9q3f3i32i")
 _SCALE = float(1 << 40)
 
