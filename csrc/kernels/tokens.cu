@@ -152,20 +152,25 @@ template <typename T> __global__ void __launch_bounds__(128) small_kernel(TokenA
 // later passes work on its bits (e orders the candidates except where several logits share
 // an e; only there the logits are looked at again). What bounds it is the number of
 // instructions for a candidate, about 25 for the exponential and the weight, 20 for the
-// histogram and 15 for the sums of what is kept: small blocks (4 on an SM) so that the
-// phases of one fill the waits of another.
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMaxCluster = 16, kMaxSlice = 16384;
-constexpr int kBinShift = 18;                        // 32 bins an octave of e, 40 octaves
-constexpr int kBins = 1312;                          // > 40 * 32, whole shares for 1 .. 16 blocks
+// histogram and 15 for the sums of what is kept, and the waits at the cluster's barriers.
+//
+// With enough rows to fill the GPU a row is one block's (kStream): no barriers between
+// blocks; the row is read again from the L2 cache and its exponentials made again instead
+// of being kept (a slice of the whole row would not fit).
+constexpr int kMaxCluster = 16, kMaxSlice = 16384, kMaxStream = kMaxCluster * kMaxSlice;
 constexpr int kList = 512;
+template <bool kStream> struct Large {
+  static constexpr int kThreads = kStream ? 512 : 256, kWarps = kThreads / 32;
+  static constexpr int kBinShift = kStream ? 16 : 18;          // 128 or 32 bins an octave of e, 40 octaves
+  static constexpr int kBins = kStream ? 5136 : 1312;          // > 40 octaves, whole shares for 1 .. 16 blocks
+};
 constexpr int kAllKept = 1 << 30, kNoBin = -1;
 
 struct Found { u64 mass_before; unsigned count_before; int bin; };
 struct Cut { u64 ties, mass_upto; uint32_t key; unsigned pad; };     // kept: keys above, `ties` equal ones
 
-struct TokenSmem {
-  unsigned hist_lo[kBins + 1], hist_hi[kBins + 1], hist_c[kBins + 1];      // weight in two words, count
+template <int kBins, int kWarps> struct TokenSmem {
+  unsigned hist_lo[kBins + 32], hist_hi[kBins + 32], hist_c[kBins + 32];      // weight in two words, count
   uint32_t list_key[kList], list_e[kList];           // of the bin where the limit falls
   int list_at[kList];
   u64 warp_m[kWarps], share_m[kMaxCluster], x_m[kMaxCluster];
@@ -175,8 +180,6 @@ struct TokenSmem {
   Cut cut;
   unsigned list_n;
 };
-
-__device__ __forceinline__ int bin_of_bits(uint32_t e) { return static_cast<int>((0x3f800000u - e) >> kBinShift); }
 
 // w = floor(e * 2^40), e in [0, 1], as w1 * 2^23 + w0: the additions of 2^23 that round down
 // leave the whole part in the low bits of a float (what is left is exact in between).
@@ -193,10 +196,14 @@ __device__ __forceinline__ u64 whole_weight(float e) {
 }
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
-template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) large_kernel(TokenArgs a, int slice) {
+template <typename T, int CS, bool kStream>
+__global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream>::kThreads) large_kernel(TokenArgs a, int slice) {
+  constexpr int kThreads = Large<kStream>::kThreads, kWarps = Large<kStream>::kWarps, kBins = Large<kStream>::kBins;
+  using Smem = TokenSmem<kBins, kWarps>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  TokenSmem& sm = *reinterpret_cast<TokenSmem*>(smem_raw);
-  float* zs = reinterpret_cast<float*>(smem_raw + (sizeof(TokenSmem) + 15) / 16 * 16);
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  float* zs = reinterpret_cast<float*>(smem_raw + (sizeof(Smem) + 15) / 16 * 16);
+  auto bin_of_bits = [](uint32_t e) { return static_cast<int>((0x3f800000u - e) >> Large<kStream>::kBinShift); };
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = CS > 1 ? static_cast<int>(cluster.block_rank()) : 0;
   const int64_t id = blockIdx.x / CS;
@@ -223,11 +230,12 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
   const int off = (W - head) % W;
   const int slots = (off + n + 3) / 4 * 4;
   float mx = -INFINITY;
-  if (threadIdx.x < off) zs[threadIdx.x] = -INFINITY;
-  if (threadIdx.x < slots - off - n) zs[off + n + threadIdx.x] = -INFINITY;
+  if (!kStream && threadIdx.x < off) zs[threadIdx.x] = -INFINITY;
+  if (!kStream && threadIdx.x < slots - off - n) zs[off + n + threadIdx.x] = -INFINITY;
   if (threadIdx.x < min(head, n)) {
-    zs[off + threadIdx.x] = to_f(row[threadIdx.x]);
-    mx = fmaxf(mx, to_f(row[threadIdx.x]));          // passes NaN over
+    const float z = to_f(row[threadIdx.x]);
+    if (!kStream) zs[off + threadIdx.x] = z;
+    mx = fmaxf(mx, z);                               // passes NaN over
   }
   const int whole = n > head ? (n - head) / W * W : 0;
 #pragma unroll 4
@@ -236,13 +244,16 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
     load_vec<T, W>(row + head + i, v);
 #pragma unroll
     for (int j = 0; j < W; ++j) mx = fmaxf(mx, v[j]);
+    if (!kStream) {
 #pragma unroll
-    for (int j = 0; j < W; j += 4)
-      *reinterpret_cast<float4*>(zs + off + head + i + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      for (int j = 0; j < W; j += 4)
+        *reinterpret_cast<float4*>(zs + off + head + i + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    }
   }
   if (const int i = head + whole + threadIdx.x; i < n) {
-    zs[off + i] = to_f(row[i]);
-    mx = fmaxf(mx, to_f(row[i]));
+    const float z = to_f(row[i]);
+    if (!kStream) zs[off + i] = z;
+    mx = fmaxf(mx, z);
   }
   auto clear = [&] {
     for (int i = threadIdx.x; i < kBins; i += kThreads) sm.hist_lo[i] = sm.hist_hi[i] = sm.hist_c[i] = 0;
@@ -280,29 +291,58 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
     if (up) atomicAdd(&sm.hist_hi[bin], up);
     if (q.k) atomicAdd(&sm.hist_c[bin], 1u);
   };
-  // logits -> e (0 for NaN and what min_p drops); weights into the histogram, or summed
+  // logit -> e (0 for NaN and what min_p drops)
   const bool plain = m < INFINITY && q.inv < INFINITY;   // else equal logits need below()
+  auto exp_of = [&](float z) {
+    const float e = expf(plain ? __fmul_rn(__fsub_rn(z, m), q.inv) : below(z, m, q.inv));
+    return e >= q.min_p ? e : 0.0f;
+  };
+  // the e of candidates i .. i + 3 (slots; i a multiple of 4) and of one
+  auto four = [&](int i, float (&e)[4]) {
+    if constexpr (kStream) {
+      if (i >= off && i + 4 <= off + n) {
+        load_vec<T, 4>(row + i - off, e);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = i + j >= off && i + j < off + n ? to_f(row[i + j - off]) : -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = exp_of(e[j]);
+    } else {
+      const float4 v = *reinterpret_cast<const float4*>(zs + i);
+      e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w;
+    }
+  };
+  auto one = [&](int i) {
+    if constexpr (kStream) return i >= off && i < off + n ? exp_of(to_f(row[i - off])) : 0.0f;
+    else return zs[i];
+  };
+  // weights into the histogram, or summed; sums of a thread stay within 2^32 for 256 slots
   uint32_t s1 = 0, s0 = 0;
   u64 above = 0;
+  auto flush = [&] {
+    above += (static_cast<u64>(s1) << 23) + s0;
+    s1 = s0 = 0;
+  };
+#pragma unroll 2
   for (int i = w_lo + lane * 4; i < w_hi; i += 128) {
-    const float4 v = *reinterpret_cast<const float4*>(zs + i);
-    float e[4] = {v.x, v.y, v.z, v.w};
+    float e[4];
+    four(i, e);
+    if constexpr (!kStream) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      e[j] = expf(plain ? __fmul_rn(__fsub_rn(e[j], m), q.inv) : below(e[j], m, q.inv));
-      if (!(e[j] >= q.min_p)) e[j] = 0.0f;
+      for (int j = 0; j < 4; ++j) e[j] = exp_of(e[j]);
+      *reinterpret_cast<float4*>(zs + i) = make_float4(e[0], e[1], e[2], e[3]);
     }
-    *reinterpret_cast<float4*>(zs + i) = make_float4(e[0], e[1], e[2], e[3]);
     uint32_t w1[4], w0[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) split_weight(e[j], w1[j], w0[j]);
     if (limited) {
-      // four additions in flight; what has no weight goes to a bin that nobody reads
+      // four additions in flight; what has no weight goes to bins that nobody reads
       unsigned old[4];
       int bin[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        bin[j] = min(bin_of_bits(__float_as_uint(e[j])), kBins);
+        bin[j] = w1[j] | w0[j] ? bin_of_bits(__float_as_uint(e[j])) : kBins + lane;
         old[j] = atomicAdd(&sm.hist_lo[bin[j]], (w1[j] << 23) + w0[j]);
       }
       if (q.k) {
@@ -318,12 +358,13 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s1 += w1[j];                         // at most kMaxSlice / 256 of 2^17 and 2^23
+        s1 += w1[j];
         s0 += w0[j];
       }
+      if (kStream && ((i - w_lo) & 8191) >= 8064) flush();
     }
   }
-  above = (static_cast<u64>(s1) << 23) + s0;
+  flush();
   __syncthreads();
 
   // Kept: everything in bins below `edge`; in bin `edge`, keys above the cut's and the first
@@ -417,10 +458,11 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
       if (level < 0) {
         // the sums of what is surely kept, and the candidates of the bin where the limit falls
         edge = lim ? f.bin : kAllKept;
-        s1 = s0 = 0;
+        above = 0;
+#pragma unroll 2
         for (int i = w_lo + lane * 4; i < w_hi; i += 128) {
-          const float4 v = *reinterpret_cast<const float4*>(zs + i);
-          const float e[4] = {v.x, v.y, v.z, v.w};
+          float e[4];
+          four(i, e);
           bool in_edge = false;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -432,8 +474,9 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
             in_edge |= bin == edge;
           }
           if (in_edge) {
+#pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const uint32_t bits = __float_as_uint(zs[i + j]);
+              const uint32_t bits = __float_as_uint(e[j]);
               if (bin_of_bits(bits) != edge || !whole_weight(__uint_as_float(bits))) continue;
               const unsigned at = atomicAdd(peer(&sm.list_n, 0), 1u);
               if (at < kList) {
@@ -443,8 +486,9 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
               }
             }
           }
+          if (kStream && ((i - w_lo) & 8191) >= 8064) flush();
         }
-        above = (static_cast<u64>(s1) << 23) + s0;
+        flush();
         if (!lim) break;
         sync();
         listed = *peer(&sm.list_n, 0);
@@ -507,16 +551,18 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
           clear();
           for (int i = threadIdx.x; i < slots; i += kThreads) {
             uint32_t w1, w0;
-            split_weight(zs[i], w1, w0);
-            if (w1 | w0) add(bin_of_bits(__float_as_uint(zs[i])), w1, w0);
+            const float e = one(i);
+            split_weight(e, w1, w0);
+            if (w1 | w0) add(bin_of_bits(__float_as_uint(e)), w1, w0);
           }
         }
       } else {
         clear();
         for (int i = threadIdx.x; i < slots; i += kThreads) {
-          if (bin_of_bits(__float_as_uint(zs[i])) != edge) continue;
+          const float e = one(i);
+          if (bin_of_bits(__float_as_uint(e)) != edge) continue;
           uint32_t w1, w0;
-          split_weight(zs[i], w1, w0);
+          split_weight(e, w1, w0);
           if (!(w1 | w0)) continue;
           const uint32_t key = key_of(clean(to_f(row[i - off])));
           if (level == 0 || key >> (32 - 8 * level) == prefix) add(255 - static_cast<int>(key >> (24 - 8 * level) & 255u), w1, w0);
@@ -555,7 +601,7 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
       u64 more = 0;
       unsigned equal = 0;
       for (int i = w_lo + lane; i < w_hi; i += 32) {
-        const float e = zs[i];
+        const float e = one(i);
         if (bin_of_bits(__float_as_uint(e)) != edge) continue;
         const u64 w = whole_weight(e);
         const int s = w ? side(__float_as_uint(e), i) : 0;
@@ -602,35 +648,69 @@ template <typename T, int CS> __global__ void __launch_bounds__(kThreads, 4) lar
     ties_at += c;
   }
   const u64 mine = sm.warp_m[warp] + (min(ties_at + sm.warp_c[warp], cut.ties) - min(ties_at, cut.ties)) * tie_w;
-  if (at >= mass_at && at < mass_at + mine) {
-    for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-      const int i = i0 + lane;
-      const float e = i < w_hi ? zs[i] : 0.0f;
-      u64 w = whole_weight(e);
-      const int s = w ? side(__float_as_uint(e), i) : 0;
-      const unsigned eq = __ballot_sync(0xffffffffu, s == 2);
-      if (s == 0 || (s == 2 && ties_at + __popc(eq & ((1u << lane) - 1u)) >= cut.ties)) w = 0;
-      ties_at += __popc(eq);
-      const u64 upto = mass_at + warp_scan(w, lane);
-      if (w && upto > at && upto - w <= at) {
-        a.token[id] = lo + i - off;
-        a.logp[id] = log_share(w, total);
-      }
-      mass_at = __shfl_sync(0xffffffffu, upto, 31);
-      if (mass_at > at) break;
+  // the run that holds it, again in parts, one for each warp, and the part walked 32 at a time
+  if (threadIdx.x == 0) sm.found.bin = -1;
+  __syncthreads();
+  if (at >= mass_at && at < mass_at + mine && lane == 0) sm.found = Found{mass_at, static_cast<unsigned>(ties_at), warp};
+  __syncthreads();
+  if (sm.found.bin < 0) return;
+  mass_at = sm.found.mass_before;
+  ties_at = sm.found.count_before;
+  const int r_lo = min(slots, sm.found.bin * run), r_hi = min(slots, r_lo + run);
+  const int part = run / kWarps;             // run is a multiple of 128
+  const int p_lo = min(r_hi, r_lo + warp * part), p_hi = warp == kWarps - 1 ? r_hi : min(r_hi, p_lo + part);
+  u64 sure = 0;
+  unsigned equal = 0;
+#pragma unroll 4
+  for (int i = p_lo + lane; i < p_hi; i += 32) {
+    const float e = one(i);
+    const u64 w = whole_weight(e);
+    const int s = w ? side(__float_as_uint(e), i) : 0;
+    if (s == 1) sure += w;
+    equal += s == 2;
+  }
+  sure = warp_sum(sure);
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  __syncthreads();
+  if (lane == 0) {
+    sm.warp_m[warp] = sure;
+    sm.warp_c[warp] = equal;
+  }
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) {
+    const u64 c = sm.warp_c[w];
+    mass_at += sm.warp_m[w] + (min(ties_at + c, cut.ties) - min(ties_at, cut.ties)) * tie_w;
+    ties_at += c;
+  }
+  if (at < mass_at || at >= mass_at + sure + (min(ties_at + equal, cut.ties) - min(ties_at, cut.ties)) * tie_w) return;
+  for (int i0 = p_lo; i0 < p_hi; i0 += 32) {
+    const int i = i0 + lane;
+    const float e = i < p_hi ? one(i) : 0.0f;
+    u64 w = whole_weight(e);
+    const int s = w ? side(__float_as_uint(e), i) : 0;
+    const unsigned eq = __ballot_sync(0xffffffffu, s == 2);
+    if (s == 0 || (s == 2 && ties_at + __popc(eq & ((1u << lane) - 1u)) >= cut.ties)) w = 0;
+    ties_at += __popc(eq);
+    const u64 upto = mass_at + warp_scan(w, lane);
+    if (w && upto > at && upto - w <= at) {
+      a.token[id] = lo + i - off;
+      a.logp[id] = log_share(w, total);
     }
+    mass_at = __shfl_sync(0xffffffffu, upto, 31);
+    if (mass_at > at) break;
   }
 }
 
-template <typename T, int CS> int launch_large(const TokenArgs& a, int slice, cudaStream_t s) {
-  constexpr size_t kFixed = (sizeof(TokenSmem) + 15) / 16 * 16 + 16 * sizeof(float);   // a slice is shifted by up to 7
-  const size_t smem = kFixed + static_cast<size_t>(slice) * sizeof(float);
+template <typename T, int CS, bool kStream> int launch_large(const TokenArgs& a, int slice, cudaStream_t s) {
+  using L = Large<kStream>;
+  constexpr size_t kFixed = (sizeof(TokenSmem<L::kBins, L::kWarps>) + 15) / 16 * 16 + 16 * sizeof(float);   // a slice is shifted by up to 7
+  const size_t smem = kFixed + (kStream ? 0 : static_cast<size_t>(slice) * sizeof(float));
   const int64_t blocks = static_cast<int64_t>(a.rows) * a.heads * CS;
   if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
-  if (const int rc = allow_smem<large_kernel<T, CS>, (CS > 8)>(kFixed + kMaxSlice * sizeof(float))) return rc;
+  if (const int rc = allow_smem<large_kernel<T, CS, kStream>, (CS > 8)>(kFixed + (kStream ? 0 : kMaxSlice * sizeof(float)))) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(L::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -640,7 +720,7 @@ template <typename T, int CS> int launch_large(const TokenArgs& a, int slice, cu
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CS > 1 ? 1 : 0;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, large_kernel<T, CS>, a, slice));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, large_kernel<T, CS, kStream>, a, slice));
 }
 
 template <typename T> int launch_tokens(const TokenArgs& a, int widest, cudaStream_t s) {
@@ -651,6 +731,7 @@ template <typename T> int launch_tokens(const TokenArgs& a, int widest, cudaStre
     small_kernel<T><<<static_cast<unsigned>(blocks), 128, 0, s>>>(a);
     SURF_RETURN_LAUNCH();
   }
+  if (answers >= 148 && widest > 8192 && widest <= kMaxStream) return launch_large<T, 1, true>(a, widest, s);
   // slices of at most 8192 candidates (32 a thread, 4 blocks on an SM); smaller ones, down to
   // 1024, while there are too few blocks to fill the GPU
   int cs = 1;
@@ -658,11 +739,11 @@ template <typename T> int launch_tokens(const TokenArgs& a, int widest, cudaStre
   const int slice = static_cast<int>(surfk::ceil_div(widest, cs));
   if (slice > kMaxSlice) return static_cast<int>(cudaErrorInvalidValue);
   switch (cs) {
-    case 1: return launch_large<T, 1>(a, slice, s);
-    case 2: return launch_large<T, 2>(a, slice, s);
-    case 4: return launch_large<T, 4>(a, slice, s);
-    case 8: return launch_large<T, 8>(a, slice, s);
-    default: return launch_large<T, 16>(a, slice, s);
+    case 1: return launch_large<T, 1, false>(a, slice, s);
+    case 2: return launch_large<T, 2, false>(a, slice, s);
+    case 4: return launch_large<T, 4, false>(a, slice, s);
+    case 8: return launch_large<T, 8, false>(a, slice, s);
+    default: return launch_large<T, 16, false>(a, slice, s);
   }
 }
 

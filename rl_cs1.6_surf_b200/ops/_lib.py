@@ -81,6 +81,19 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def launch(fn, what: str, index: int, *args) -> None:
+    """``fn(*args, stream)`` on device ``index`` and its current stream, whatever the
+    current device is; raises on a non-zero status."""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            launch(fn, what, index, *args)
+        return
+    check(fn(*args, _raw_stream(index) if _raw_stream is not None else stream_ptr(index)), what)
+
+
 def ptr(t) -> int:
     return 0 if t is None else int(t.data_ptr())
 

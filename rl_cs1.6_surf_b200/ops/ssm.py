@@ -29,7 +29,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import KernelError, check, stream_ptr
+from ._lib import KernelError, launch
 from .gemm import error_flag
 
 SLIB = "libsurf_seq.so"
@@ -69,57 +69,57 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
     raise TypeError(f"{what}: tokens must be bfloat16 or float32, not {t.dtype}")
 
 
-def _tokens(what: str, name: str, t: Optional[torch.Tensor], shape: tuple, like: torch.Tensor) -> None:
+def _tokens(what: str, name: str, t: Optional[torch.Tensor], shape: tuple, dtype, index: int) -> None:
     """An input with the tokens' type: shape, type, device and a dense last axis."""
-    if t is None:
+    if t is None or (t.dtype is dtype and t.shape == shape and t.get_device() == index and t.stride(-1) == 1):
         return
     if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype != like.dtype:
-        raise TypeError(f"{what}: {name} is {t.dtype}, the tokens are {like.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{what}: {name} is on {t.device}, the tokens on {like.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {name} is {t.dtype}, the tokens are {dtype}")
+    if t.get_device() != index:
+        raise ValueError(f"{what}: {name} is on {t.device}, the tokens on cuda:{index}")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{what}: {name} needs a dense last axis")
 
 
-def _dense(what: str, name: str, t: Optional[torch.Tensor], shape: tuple, dtype, device) -> None:
+def _dense(what: str, name: str, t: Optional[torch.Tensor], shape: tuple, dtype, index: int) -> None:
     """A contiguous input (weights, states, masks)."""
-    if t is None:
+    if t is None or (t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous()):
         return
     if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{what}: {name} is on {t.device}, the tokens on {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{what}: {name} must be contiguous")
+    if t.get_device() != index:
+        raise ValueError(f"{what}: {name} is on {t.device}, the tokens on cuda:{index}")
+    raise ValueError(f"{what}: {name} must be contiguous")
 
 
-def _flags(what: str, t: Optional[torch.Tensor], shape: tuple, device) -> None:
+def _flags(what: str, t: Optional[torch.Tensor], shape: tuple, index: int) -> None:
     if t is None:
         return
-    if t.dtype != torch.bool and t.dtype != torch.uint8:
+    if t.dtype is not torch.bool and t.dtype is not torch.uint8:
         raise TypeError(f"{what}: reset must be bool or uint8, not {t.dtype}")
-    _dense(what, "reset", t, shape, t.dtype, device)
+    _dense(what, "reset", t, shape, t.dtype, index)
 
 
-def _on_device(t: torch.Tensor):
-    """Launches go to the tensors' device, whatever the current one is."""
-    return torch.cuda.device(t.device)
-
-
-def _aligned(elems: int, *tensors) -> bool:
-    """Every row of the tensors starts on a boundary of ``elems`` elements."""
-    bytes_, bits = 0, 0
+def _bits(size: int, *tensors) -> int:
+    """What the bases and the strides of the tensors' rows, in bytes, have in their low bits."""
+    bits = 0
     for t in tensors:
         if t is not None:
-            bytes_ |= t.data_ptr() // t.element_size() | (t.data_ptr() % t.element_size())
-            for n, s in zip(t.shape[:-1], t.stride()):
-                if n > 1:
-                    bits |= s
-    return (bytes_ | bits) % elems == 0
+            bits |= t.data_ptr()
+            for s in t.stride()[:-1]:
+                bits |= s * size
+    return bits
+
+
+def _piece(cols: int, size: int, *tensors) -> int:
+    """Bytes of the pieces that rows of ``cols`` elements may be copied in (copy_rows): 16
+    or 4 where the row's length, every base and every stride is a multiple of it, else 0."""
+    bits = _bits(size, *tensors) | cols * size
+    return 16 if bits & 15 == 0 else 4 if bits & 3 == 0 else 0
 
 
 # ---- causal convolution -----------------------------------------------------------
@@ -129,16 +129,17 @@ def _conv_check(what, x, weight, bias, state, reset, lengths):
         raise ValueError(f"{what}: x must be [batch, tokens, channels]")
     code = _dtype_code(x, what)
     b, t, d = x.shape
+    at = x.get_device()
     if weight.dim() != 2 or not 2 <= weight.shape[1] <= MAX_WIDTH:
         raise ValueError(f"{what}: weight must be [channels, width] with a width of 2 to {MAX_WIDTH}")
     w = weight.shape[1]
-    _tokens(what, "x", x, x.shape, x)
-    _dense(what, "weight", weight, (d, w), torch.float32, x.device)
-    _dense(what, "bias", bias, (d,), torch.float32, x.device)
-    _dense(what, "state", state, (b, w - 1, d), x.dtype, x.device)
-    _flags(what, reset, (b, t), x.device)
-    _dense(what, "lengths", lengths, (b,), torch.int32, x.device)
-    return code, b, t, d, w
+    _tokens(what, "x", x, x.shape, x.dtype, at)
+    _dense(what, "weight", weight, (d, w), torch.float32, at)
+    _dense(what, "bias", bias, (d,), torch.float32, at)
+    _dense(what, "state", state, (b, w - 1, d), x.dtype, at)
+    _flags(what, reset, (b, t), at)
+    _dense(what, "lengths", lengths, (b,), torch.int32, at)
+    return code, 4 - 2 * code, at, b, t, d, w
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -148,21 +149,20 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     over the tokens that t sees; ``state`` and ``final`` hold the W - 1 tokens before
     and behind the row, oldest first."""
     what = "causal_conv"
-    code, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
+    code, e, at, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
     if out is None:
         out = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
     else:
-        _tokens(what, "out", out, x.shape, x)
+        _tokens(what, "out", out, x.shape, x.dtype, at)
     final = torch.empty((b, w - 1, d), dtype=x.dtype, device=x.device)
     if b == 0 or d == 0:
         return out, final
-    vec = d % 4 == 0 and _aligned(4, x, out, state)
+    vec = (_bits(e, x, out, state) | d * e) % (4 * e) == 0
     tt = 16
     args = _CONV.pack(_p(x), 0, _p(state), 0, _p(weight), _p(bias), _p(reset), _p(lengths), out.data_ptr(),
                       final.data_ptr(), 0, x.stride(0), x.stride(1), 0, 0, out.stride(0), out.stride(1), t,
                       b, t, d, int(silu), tt, max(1, -(-t // tt)))
-    with _on_device(x):
-        check(_lib.lib(SLIB).surf_seq_conv(args, code, w, int(vec), stream_ptr(x.device)), "surf_seq_conv")
+    launch(_lib.lib(SLIB).surf_seq_conv, "surf_seq_conv", at, args, code, w, int(vec))
     return out, final
 
 
@@ -173,9 +173,9 @@ def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bi
     """Gradients of ``causal_conv`` for the gradient ``dy`` of y and ``dfinal`` of
     final (None: zero): dx and dstate in the tokens' type, dweight and dbias float32."""
     what = "causal_conv_grad"
-    code, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
-    _tokens(what, "dy", dy, x.shape, x)
-    _dense(what, "dfinal", dfinal, (b, w - 1, d), x.dtype, x.device)
+    code, e, at, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
+    _tokens(what, "dy", dy, x.shape, x.dtype, at)
+    _dense(what, "dfinal", dfinal, (b, w - 1, d), x.dtype, at)
     dev = x.device
     dx = torch.empty((b, t, d), dtype=x.dtype, device=dev)
     dstate = torch.empty((b, w - 1, d), dtype=x.dtype, device=dev) if state is not None else None
@@ -183,7 +183,7 @@ def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bi
         return ConvGrads(dx, torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dstate)
     dw = torch.empty((d, w), dtype=torch.float32, device=dev)
     db = torch.empty(d, dtype=torch.float32, device=dev) if bias is not None else None
-    vec = d % 4 == 0 and _aligned(4, x, dy, state, dfinal)
+    vec = (_bits(e, x, dy, state, dfinal) | d * e) % (4 * e) == 0
     tt = 16
     chunks = max(1, -(-t // tt))
     groups = d // 4 if vec else d
@@ -194,9 +194,7 @@ def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bi
     args = _CONV.pack(_p(x), dy.data_ptr(), _p(state), _p(dfinal), _p(weight), _p(bias), _p(reset), _p(lengths),
                       dx.data_ptr(), _p(dstate), part.data_ptr(), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1),
                       t * d, d, t, b, t, d, int(silu), tt, chunks)
-    with _on_device(x):
-        check(_lib.lib(SLIB).surf_seq_conv_grad(args, code, w, int(vec), rows, _p(dw), _p(db), stream_ptr(dev)),
-              "surf_seq_conv_grad")
+    launch(_lib.lib(SLIB).surf_seq_conv_grad, "surf_seq_conv_grad", at, args, code, w, int(vec), rows, _p(dw), _p(db))
     return ConvGrads(dx, dw, db, dstate)
 
 
@@ -212,30 +210,28 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
         raise ValueError(f"{what}: x must be [rows, channels]")
     code = _dtype_code(x, what)
     r, d = x.shape
-    dev = x.device
+    dev, at, e = x.device, x.get_device(), x.element_size()
     if weight.dim() != 2 or not 2 <= weight.shape[1] <= MAX_WIDTH:
         raise ValueError(f"{what}: weight must be [channels, width] with a width of 2 to {MAX_WIDTH}")
     w = weight.shape[1]
-    _tokens(what, "x", x, x.shape, x)
-    _dense(what, "weight", weight, (d, w), torch.float32, dev)
-    _dense(what, "bias", bias, (d,), torch.float32, dev)
-    _dense(what, "state", state, (state.shape[0], w - 1, d), x.dtype, dev)
-    _flags(what, reset, (r,), dev)
-    _dense(what, "slots", slots, (r,), torch.int32, dev)
+    _tokens(what, "x", x, x.shape, x.dtype, at)
+    _dense(what, "weight", weight, (d, w), torch.float32, at)
+    _dense(what, "bias", bias, (d,), torch.float32, at)
+    _dense(what, "state", state, (state.shape[0], w - 1, d), x.dtype, at)
+    _flags(what, reset, (r,), at)
+    _dense(what, "slots", slots, (r,), torch.int32, at)
     if slots is None and state.shape[0] < r:
         raise ValueError(f"{what}: {r} rows, but {state.shape[0]} slots")
     if out is None:
         out = torch.empty((r, d), dtype=x.dtype, device=dev)
     else:
-        _tokens(what, "out", out, x.shape, x)
+        _tokens(what, "out", out, x.shape, x.dtype, at)
     if r == 0 or d == 0:
         return out
-    vec = d % 4 == 0 and _aligned(4, x, out, state)
-    with _on_device(x):
-        check(_lib.lib(SLIB).surf_seq_conv_step(
-            x.data_ptr(), x.stride(0), weight.data_ptr(), _p(bias), state.data_ptr(), _p(reset), _p(slots),
-            state.shape[0], out.data_ptr(), out.stride(0), r, d, w, int(silu), code, int(vec),
-            error_flag(dev).data_ptr(), stream_ptr(dev)), "surf_seq_conv_step")
+    vec = (_bits(e, x, out, state) | d * e) % (4 * e) == 0
+    launch(_lib.lib(SLIB).surf_seq_conv_step, "surf_seq_conv_step", at, x.data_ptr(), x.stride(0), weight.data_ptr(),
+           _p(bias), state.data_ptr(), _p(reset), _p(slots), state.shape[0], out.data_ptr(), out.stride(0), r, d, w,
+           int(silu), code, int(vec), error_flag(dev).data_ptr())
     return out
 
 
@@ -246,7 +242,7 @@ def _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths):
         raise ValueError(f"{what}: x must be [batch, tokens, channels]")
     code = _dtype_code(x, what)
     b, t, d = x.shape
-    dev = x.device
+    at = x.get_device()
     if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATE:
         raise ValueError(f"{what}: A must be [channels, states] with 1 to {MAX_STATE} states")
     n = A.shape[1]
@@ -254,31 +250,17 @@ def _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths):
         raise ValueError(f"{what}: B must be [batch, tokens, groups, states], its groups dividing the channels")
     g = B.shape[2]
     for name, v in (("x", x), ("dt", dt), ("z", z)):
-        _tokens(what, name, v, (b, t, d), x)
+        _tokens(what, name, v, (b, t, d), x.dtype, at)
     for name, v in (("B", B), ("C", C)):
-        _tokens(what, name, v, (b, t, g, n), x)
+        _tokens(what, name, v, (b, t, g, n), x.dtype, at)
     f32 = torch.float32
-    _dense(what, "A", A, (d, n), f32, dev)
-    _dense(what, "D", D, (d,), f32, dev)
-    _dense(what, "dt_bias", dt_bias, (d,), f32, dev)
-    _dense(what, "state", state, (b, d, n), f32, dev)
-    _flags(what, reset, (b, t), dev)
-    _dense(what, "lengths", lengths, (b,), torch.int32, dev)
-    return code, b, t, d, n, g
-
-
-def _piece(cols: int, *tensors) -> int:
-    """Bytes of the pieces that rows of ``cols`` elements may be copied in (copy_rows): 16
-    or 4 where the row's length, every base and every stride is a multiple of it, else 0."""
-    size = next(t for t in tensors if t is not None).element_size()
-    bits = cols * size
-    for t in tensors:
-        if t is not None:
-            bits |= t.data_ptr()
-            for n, s in zip(t.shape[:-1], t.stride()):
-                if n > 1:
-                    bits |= s * size
-    return 16 if bits % 16 == 0 else 4 if bits % 4 == 0 else 0
+    _dense(what, "A", A, (d, n), f32, at)
+    _dense(what, "D", D, (d,), f32, at)
+    _dense(what, "dt_bias", dt_bias, (d,), f32, at)
+    _dense(what, "state", state, (b, d, n), f32, at)
+    _flags(what, reset, (b, t), at)
+    _dense(what, "lengths", lengths, (b,), torch.int32, at)
+    return code, 4 - 2 * code, at, b, t, d, n, g
 
 
 def _chunks(b: int, t: int, d: int, n: int, g: int):
@@ -306,12 +288,12 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     keeps in ``saved`` the states that ``selective_scan_grad`` starts from: 4 D N bytes
     for every 8 tokens."""
     what = "selective_scan"
-    code, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
+    code, e, at, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
     dev = x.device
     if out is None:
         out = torch.empty((b, t, d), dtype=x.dtype, device=dev)
     else:
-        _tokens(what, "out", out, x.shape, x)
+        _tokens(what, "out", out, x.shape, x.dtype, at)
     final = torch.empty((b, d, n), dtype=torch.float32, device=dev)
     saved = torch.empty((b, -(-t // SAVE_EVERY), d, n), dtype=torch.float32, device=dev) if train else None
     if b == 0 or d == 0:
@@ -329,9 +311,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
         0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
         0, 0, out.stride(0), out.stride(1), t, b, t, d, n, g, int(softplus), chunk, chunks,
-        _piece(d // g, x, dt, z, out), _piece(n, B, C))
-    with _on_device(x):
-        check(_lib.lib(SLIB).surf_seq_scan(args, code, stream_ptr(dev)), "surf_seq_scan")
+        _piece(d // g, e, x, dt, z, out), _piece(n, e, B, C))
+    launch(_lib.lib(SLIB).surf_seq_scan, "surf_seq_scan", at, args, code)
     if chunks > 1:
         _lib.add_launches(2)
     return Scan(out, final, saved)
@@ -348,13 +329,13 @@ def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A
     first where heads share them), the weights' and the state's in float32; None for an
     input that was None."""
     what = "selective_scan_grad"
-    code, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
+    code, e, at, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
     dev, f32 = x.device, torch.float32
-    _tokens(what, "dout", dout, x.shape, x)
-    _dense(what, "dfinal", dfinal, (b, d, n), f32, dev)
+    _tokens(what, "dout", dout, x.shape, x.dtype, at)
+    _dense(what, "dfinal", dfinal, (b, d, n), f32, at)
     if saved is None:
         raise ValueError(f"{what}: needs the states that selective_scan(train=True) saved")
-    _dense(what, "saved", saved, (b, -(-t // SAVE_EVERY), d, n), f32, dev)
+    _dense(what, "saved", saved, (b, -(-t // SAVE_EVERY), d, n), f32, at)
 
     def like(v, shape, dtype):
         return None if v is None else torch.empty(shape, dtype=dtype, device=dev)
@@ -385,9 +366,8 @@ def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A
         x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
         0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
         dout.stride(0), dout.stride(1), 0, 0, t, b, t, d, n, g, int(softplus), chunk, chunks,
-        _piece(d // g, x, dt, z, dout), _piece(n, B, C))
-    with _on_device(x):
-        check(L.surf_seq_scan_grad(args, code, stream_ptr(dev)), "surf_seq_scan_grad")
+        _piece(d // g, e, x, dt, z, dout), _piece(n, e, B, C))
+    launch(L.surf_seq_scan_grad, "surf_seq_scan_grad", at, args, code)
     _lib.add_launches(4 if chunks > 1 else 2)
     return ScanGrads(dx, ddt, dz, dB, dC, dA, dD, dbias, dstate)
 
@@ -407,7 +387,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
         raise ValueError(f"{what}: x must be [rows, channels]")
     code = _dtype_code(x, what)
     r, d = x.shape
-    dev = x.device
+    dev, at, e = x.device, x.get_device(), x.element_size()
     if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATE:
         raise ValueError(f"{what}: A must be [channels, states] with 1 to {MAX_STATE} states")
     n = A.shape[1]
@@ -415,30 +395,29 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
         raise ValueError(f"{what}: B must be [rows, groups, states], its groups dividing the channels")
     g = B.shape[1]
     for name, v in (("x", x), ("dt", dt), ("z", z)):
-        _tokens(what, name, v, (r, d), x)
+        _tokens(what, name, v, (r, d), x.dtype, at)
     for name, v in (("B", B), ("C", C)):
-        _tokens(what, name, v, (r, g, n), x)
+        _tokens(what, name, v, (r, g, n), x.dtype, at)
     f32 = torch.float32
-    _dense(what, "A", A, (d, n), f32, dev)
-    _dense(what, "D", D, (d,), f32, dev)
-    _dense(what, "dt_bias", dt_bias, (d,), f32, dev)
-    _dense(what, "state", state, (state.shape[0], d, n), f32, dev)
-    _flags(what, reset, (r,), dev)
-    _dense(what, "slots", slots, (r,), torch.int32, dev)
+    _dense(what, "A", A, (d, n), f32, at)
+    _dense(what, "D", D, (d,), f32, at)
+    _dense(what, "dt_bias", dt_bias, (d,), f32, at)
+    _dense(what, "state", state, (state.shape[0], d, n), f32, at)
+    _flags(what, reset, (r,), at)
+    _dense(what, "slots", slots, (r,), torch.int32, at)
     if slots is None and state.shape[0] < r:
         raise ValueError(f"{what}: {r} rows, but {state.shape[0]} slots")
     if out is None:
         out = torch.empty((r, d), dtype=x.dtype, device=dev)
     else:
-        _tokens(what, "out", out, x.shape, x)
+        _tokens(what, "out", out, x.shape, x.dtype, at)
     if r == 0 or d == 0:
         return out
     args = _STEP.pack(x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias),
                       state.data_ptr(), _p(reset), _p(slots), out.data_ptr(), error_flag(dev).data_ptr(), x.stride(0),
                       dt.stride(0), 0 if z is None else z.stride(0), B.stride(0), B.stride(1), C.stride(0), C.stride(1),
                       out.stride(0), r, d, n, g, int(softplus), state.shape[0])
-    with _on_device(x):
-        check(_lib.lib(SLIB).surf_seq_scan_step(args, code, stream_ptr(dev)), "surf_seq_scan_step")
+    launch(_lib.lib(SLIB).surf_seq_scan_step, "surf_seq_scan_step", at, args, code)
     return out
 
 

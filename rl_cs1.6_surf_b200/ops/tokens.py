@@ -25,7 +25,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import check, stream_ptr
+from ._lib import launch
 
 SLIB = "libsurf_seq.so"
 _V, _I = _lib._V, _lib._I
@@ -95,8 +95,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     offsets = tuple(sum(sizes[:i]) for i in range(n))
     args = _ARGS.pack(logits.data_ptr(), u.data_ptr(), tp, pp, mp, kp, out.data_ptr(), logp.data_ptr(), logits.stride(0),
                       t0, p0, m0, min(int(k0), 2 ** 31 - 1), rows, n, *offsets, *pad, *sizes, *pad)
-    with torch.cuda.device(dev):
-        check(_lib.lib(SLIB).surf_sample_tokens(args, code, widest, stream_ptr(dev)), "surf_sample_tokens")
+    launch(_lib.lib(SLIB).surf_sample_tokens, "surf_sample_tokens", logits.get_device(), args, code, widest)
     return out, logp
 
 

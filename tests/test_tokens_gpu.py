@@ -83,6 +83,25 @@ def test_empty_rows_infinities_and_nan(vocab):
         assert tok[3, 0] in (3, 9) and tok[4, 0] % 2 == 1
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_long_rows(dtype):
+    """As many rows as there are blocks to run them, each one block's: ordinary ones, ties,
+    empty ones, an odd offset."""
+    gen = torch.Generator("cuda").manual_seed(3)
+    n, vocab = 150, 9001
+    wide = (2.5 * torch.randn(n, vocab + 6, generator=gen, device="cuda")).to(dtype)
+    wide[0] = 0.0
+    wide[1] = float("-inf")
+    wide[2, 5000:] = float("nan")
+    wide[3, ::2] = 7.0
+    wide[4] = (torch.arange(vocab + 6, device="cuda") % 5).to(dtype)
+    z = wide[:, 3:vocab + 3]
+    u = torch.rand(n, 1, generator=gen, device="cuda")
+    for rule in (dict(), dict(top_p=0.9), dict(top_k=30, top_p=0.8), dict(top_k=4600, min_p=1e-4), dict(top_k=7000, top_p=0.99),
+                 dict(temperature=0.0)):
+        _same(z, u, **rule)
+
+
 def test_limits_per_row():
     gen = torch.Generator("cuda").manual_seed(1)
     z = 2 * torch.randn(8, 700, generator=gen, device="cuda")
