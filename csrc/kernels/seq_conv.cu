@@ -39,93 +39,153 @@ struct ConvArgs {
 // and sums of the gradient no longer fit the registers: 4 channels for both types.
 constexpr int kV = 4;
 
-// ---- whole sequences ----------------------------------------------------------------
-template <typename T, int W, int V>
-__global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) {
-  const int groups = a.D / V;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (id >= static_cast<int64_t>(groups) * a.chunks * a.B) return;
-  const int d = static_cast<int>(id % groups) * V;
-  const int64_t rest = id / groups;
-  const int chunk = static_cast<int>(rest % a.chunks);
-  const int b = static_cast<int>(rest / a.chunks);
-  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
-  const int t0 = chunk * a.tt, t1 = min(a.T, t0 + a.tt);
-  const T* x = static_cast<const T*>(a.x) + b * a.x_b + d;
-  T* y = static_cast<T*>(a.y) + b * a.y_b + d;
-  const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
-  const T* st = a.state ? static_cast<const T*>(a.state) + static_cast<int64_t>(b) * (W - 1) * a.D + d : nullptr;
-
-  float w[V][W], bias[V];
+// The channels' weights: V * W neighbouring numbers, in 16-byte pieces for V = 4.
+template <int W, int V> __device__ __forceinline__ void load_weights(const float* p, float (&w)[V][W]) {
+  if constexpr (V == 4) {
+    float flat[V * W];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+    for (int q = 0; q < W; ++q) {
+      const float4 v = reinterpret_cast<const float4*>(p)[q];
+      flat[4 * q] = v.x; flat[4 * q + 1] = v.y; flat[4 * q + 2] = v.z; flat[4 * q + 3] = v.w;
+    }
 #pragma unroll
-    for (int k = 0; k < W; ++k) w[i][k] = a.w[static_cast<int64_t>(d + i) * W + k];
-    bias[i] = a.bias ? a.bias[d + i] : 0.0f;
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[i][k] = flat[i * W + k];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[i][k] = p[i * W + k];
   }
-  // the W - 1 tokens before the stretch
-  float h[W - 1][V];
+}
+
+// One stretch of tokens of one row, as a thread sees it.
+template <typename T> struct Stretch {
+  const T* x;
+  const T* state;             // [W - 1] rows before the first token, or null
+  const uint8_t* reset;
+  int b, chunk, t0, t1, len;
+  __device__ __forceinline__ Stretch(const ConvArgs& a, int item, int d, int W) {
+    b = item / a.chunks;
+    chunk = item - b * a.chunks;
+    len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+    t0 = chunk * a.tt;
+    t1 = min(a.T, t0 + a.tt);
+    x = static_cast<const T*>(a.x) + b * a.x_b + d;
+    state = a.state ? static_cast<const T*>(a.state) + static_cast<int64_t>(b) * (W - 1) * a.D + d : nullptr;
+    reset = a.reset ? a.reset + b * a.r_b : nullptr;
+  }
+  __device__ __forceinline__ bool cut(int t) const { return reset && t >= 0 && t < len && reset[t]; }
+};
+
+// Bit u: token t + u starts an episode, for the U tokens from t on.
+template <typename T, int U> __device__ __forceinline__ unsigned cuts_of(const Stretch<T>& s, int t) {
+  unsigned m = 0;
+  if (s.reset) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u < s.len && s.reset[t + u]) m |= 1u << u;
+  }
+  return m;
+}
+
+// The W - 1 tokens before the stretch as its first token finds them (before its own
+// reset); returns bit j: it sees token t0 - 1 - j.
+template <typename T, int W, int V>
+__device__ __forceinline__ unsigned window_of(const ConvArgs& a, const Stretch<T>& s, float (&h)[W - 1][V]) {
+  unsigned seen = 0;
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
-    const int t = t0 - (W - 1) + j;
+    const int t = s.t0 - (W - 1) + j;
 #pragma unroll
     for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
-    if (t >= 0 && t < len) {
-      if (reset && reset[t]) {
+    if (t >= 0 && t < s.len) {
+      if (s.cut(t)) {
+        seen = 0;
 #pragma unroll
         for (int q = 0; q < j; ++q)
 #pragma unroll
           for (int i = 0; i < V; ++i) h[q][i] = 0.0f;
       }
-      load_vec<T, V>(x + t * a.x_t, h[j]);
-    } else if (t < 0 && st) {
-      load_vec<T, V>(st + static_cast<int64_t>(W - 1 + t) * a.D, h[j]);
+      load_vec<T, V>(s.x + t * a.x_t, h[j]);
+    } else if (t < 0 && s.state) {
+      load_vec<T, V>(s.state + static_cast<int64_t>(W - 1 + t) * a.D, h[j]);
     }
+    seen = (seen << 1) | 1u;
   }
-  constexpr int U = 8;                    // tokens loaded ahead
-  const int live = min(t1, len);
-  for (int t = t0; t < live; t += U) {
-    float in[U][V];
-    bool cut[U];
+  return seen;
+}
+
+// ---- whole sequences ----------------------------------------------------------------
+// A thread keeps its channels' weights and takes one stretch after the other; the tokens
+// of the next step are on their way while this step's are worked on.
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(256) conv_kernel(ConvArgs a, int items) {
+  const int cg = blockIdx.x * blockDim.x + threadIdx.x, d = cg * V;
+  if (cg >= a.D / V) return;
+  float w[V][W], bias[V];
+  load_weights<W, V>(a.w + static_cast<int64_t>(d) * W, w);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      cut[u] = false;
-      if (t + u < live) {
-        load_vec<T, V>(x + (t + u) * a.x_t, in[u]);
-        if (reset) cut[u] = reset[t + u] != 0;
-      }
-    }
+  for (int i = 0; i < V; ++i) bias[i] = a.bias ? a.bias[d + i] : 0.0f;
+  for (int item = blockIdx.y * blockDim.y + threadIdx.y; item < items; item += gridDim.y * blockDim.y) {
+    const Stretch<T> s(a, item, d, W);
+    T* __restrict__ y = static_cast<T*>(a.y) + s.b * a.y_b + d;
+    float h[W - 1][V];
+    window_of<T, W, V>(a, s, h);
+    constexpr int U = 8;
+    const int live = min(s.t1, s.len);
+    float next[U][V];
+    auto fetch = [&](int t) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (t + u < live) {
-        float o[V];
+      for (int u = 0; u < U; ++u)
+        if (t + u < live) load_vec<T, V>(s.x + (t + u) * a.x_t, next[u]);
+    };
+    fetch(s.t0);
+    for (int t = s.t0; t < live; t += U) {
+      float in[U][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float acc = bias[i];
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int j = 0; j < W - 1; ++j) {
-            if (cut[u]) h[j][i] = 0.0f;
-            acc = fmaf(w[i][j], h[j][i], acc);
+        for (int i = 0; i < V; ++i) in[u][i] = next[u][i];
+      const unsigned cuts = cuts_of<T, U>(s, t);
+      fetch(t + U);
+      auto work = [&](auto with_cuts) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (t + u < live) {
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              float acc = bias[i];
+#pragma unroll
+              for (int j = 0; j < W - 1; ++j) {
+                if (decltype(with_cuts)::value && (cuts >> u & 1u)) h[j][i] = 0.0f;
+                acc = fmaf(w[i][j], h[j][i], acc);
+              }
+              acc = fmaf(w[i][W - 1], in[u][i], acc);
+#pragma unroll
+              for (int j = 0; j + 1 < W - 1; ++j) h[j][i] = h[j + 1][i];
+              h[W - 2][i] = in[u][i];
+              o[i] = a.silu ? acc * sigmoid(acc) : acc;
+            }
+            store_vec<T, V>(y + (t + u) * a.y_t, o);
           }
-          acc = fmaf(w[i][W - 1], in[u][i], acc);
-#pragma unroll
-          for (int j = 0; j + 1 < W - 1; ++j) h[j][i] = h[j + 1][i];
-          h[W - 2][i] = in[u][i];
-          o[i] = a.silu ? acc * sigmoid(acc) : acc;
         }
-        store_vec<T, V>(y + (t + u) * a.y_t, o);
-      }
+      };
+      if (cuts) work(std::true_type{});
+      else work(std::false_type{});
     }
-  }
-  float zero[V];
+    float zero[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) zero[i] = 0.0f;
-  for (int t = max(t0, live); t < t1; ++t) store_vec<T, V>(y + t * a.y_t, zero);
-  // what the next token finds behind it: by the stretch of the last token
-  if (a.final_state && (len > 0 ? (len - 1 >= t0 && len - 1 < t0 + a.tt) : chunk == 0)) {
-    T* f = static_cast<T*>(a.final_state) + static_cast<int64_t>(b) * (W - 1) * a.D + d;
+    for (int i = 0; i < V; ++i) zero[i] = 0.0f;
+    for (int t = max(s.t0, live); t < s.t1; ++t) store_vec<T, V>(y + t * a.y_t, zero);
+    // what the next token finds behind it: by the stretch of the last token
+    if (a.final_state && (s.len > 0 ? (s.len - 1 >= s.t0 && s.len - 1 < s.t0 + a.tt) : s.chunk == 0)) {
+      T* f = static_cast<T*>(a.final_state) + static_cast<int64_t>(s.b) * (W - 1) * a.D + d;
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) store_vec<T, V>(f + static_cast<int64_t>(j) * a.D, h[j]);
+      for (int j = 0; j < W - 1; ++j) store_vec<T, V>(f + static_cast<int64_t>(j) * a.D, h[j]);
+    }
   }
 }
 
@@ -139,140 +199,130 @@ __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) {
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(256) conv_grad_kernel(ConvArgs a, int items) {
   extern __shared__ float red[];                                // [blockDim.y][W + 1][blockDim.x * V]
-  const int groups = a.D / V;
   const int cg = blockIdx.x * blockDim.x + threadIdx.x;
   const int d = cg * V;
-  const bool on = cg < groups;
+  const bool on = cg < a.D / V;
   float w[V][W], bias[V], dw[V][W], db[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      w[i][k] = on ? a.w[static_cast<int64_t>(d + i) * W + k] : 0.0f;
-      dw[i][k] = 0.0f;
-    }
     bias[i] = on && a.bias ? a.bias[d + i] : 0.0f;
     db[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) dw[i][k] = w[i][k] = 0.0f;
   }
   if (on) {
+    load_weights<W, V>(a.w + static_cast<int64_t>(d) * W, w);
     for (int item = blockIdx.y * blockDim.y + threadIdx.y; item < items; item += gridDim.y * blockDim.y) {
-      const int b = item / a.chunks, chunk = item - b * a.chunks;
-      const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
-      const int t0 = chunk * a.tt, t1 = min(a.T, t0 + a.tt);
-      const T* x = static_cast<const T*>(a.x) + b * a.x_b + d;
-      const T* dy = static_cast<const T*>(a.dy) + b * a.dy_b + d;
-      T* dx = static_cast<T*>(a.y) + b * a.y_b + d;
-      const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
-      const int64_t ends = static_cast<int64_t>(b) * (W - 1) * a.D + d;
-      const T* st = a.state ? static_cast<const T*>(a.state) + ends : nullptr;
+      const Stretch<T> s(a, item, d, W);
+      const T* dy = static_cast<const T*>(a.dy) + s.b * a.dy_b + d;
+      T* __restrict__ dx = static_cast<T*>(a.y) + s.b * a.y_b + d;
+      const int64_t ends = static_cast<int64_t>(s.b) * (W - 1) * a.D + d;
       const T* df = a.dfinal ? static_cast<const T*>(a.dfinal) + ends : nullptr;
-      T* ds = a.final_state ? static_cast<T*>(a.final_state) + ends : nullptr;
+      T* __restrict__ ds = a.final_state ? static_cast<T*>(a.final_state) + ends : nullptr;
       float h[W - 1][V], pend[W][V];                 // pend[j]: dx of token t - j so far
-      unsigned seen = 0;                             // bit j: token t sees token t - 1 - j
-#pragma unroll
-      for (int j = 0; j < W - 1; ++j) {
-        const int t = t0 - (W - 1) + j;
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
-        if (t >= 0 && t < len) {
-          if (reset && reset[t]) {
-            seen = 0;
-#pragma unroll
-            for (int q = 0; q < j; ++q)
-#pragma unroll
-              for (int i = 0; i < V; ++i) h[q][i] = 0.0f;
-          }
-          load_vec<T, V>(x + t * a.x_t, h[j]);
-        } else if (t < 0 && st) {
-          load_vec<T, V>(st + static_cast<int64_t>(W - 1 + t) * a.D, h[j]);
-        }
-        seen = (seen << 1) | 1u;
-      }
+      unsigned seen = window_of<T, W, V>(a, s, h);   // bit j: token t sees token t - 1 - j
+      constexpr unsigned kAll = (1u << (W - 1)) - 1u;
 #pragma unroll
       for (int j = 0; j < W; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) pend[j][i] = 0.0f;
-      if (len == 0 && chunk == 0 && df) {            // an empty row hands its state on
+      if (s.len == 0 && s.chunk == 0 && df) {        // an empty row hands its state on
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) load_vec<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D, pend[j + 1]);
       }
-      const int end = t1 + W - 1;
+      const int end = s.t1 + W - 1;
       constexpr int U = 4;
-      for (int tb = t0; tb < end; tb += U) {
-        float xin[U][V], gin[U][V];
-        bool cut[U];
+      float nx[U][V], ng[U][V];
+      auto fetch = [&](int t) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int t = tb + u;
-          cut[u] = false;
+          if (t + u < end && t + u < s.len) {
+            load_vec<T, V>(s.x + (t + u) * a.x_t, nx[u]);
+            load_vec<T, V>(dy + (t + u) * a.dy_t, ng[u]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < V; ++i) xin[u][i] = gin[u][i] = 0.0f;
-          if (t < end && t < len) {
-            load_vec<T, V>(x + t * a.x_t, xin[u]);
-            load_vec<T, V>(dy + t * a.dy_t, gin[u]);
-            if (reset) cut[u] = reset[t] != 0;
+            for (int i = 0; i < V; ++i) nx[u][i] = ng[u][i] = 0.0f;
           }
         }
+      };
+      fetch(s.t0);
+      for (int tb = s.t0; tb < end; tb += U) {
+        float xin[U][V], gin[U][V];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int t = tb + u;
-          if (t < end) {
-            if (t < len) {
-              if (cut[u]) {
-                seen = 0;
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < W - 1; ++j)
+          for (int i = 0; i < V; ++i) {
+            xin[u][i] = nx[u][i];
+            gin[u][i] = ng[u][i];
+          }
+        const unsigned cuts = cuts_of<T, U>(s, tb);
+        fetch(tb + U);
+        // kPlain: U tokens of the stretch's own, no reset in sight, the row goes on
+        auto work = [&](auto is_plain) {
+          constexpr bool kPlain = decltype(is_plain)::value;
 #pragma unroll
-                  for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
+          for (int u = 0; u < U; ++u) {
+            const int t = tb + u;
+            if (kPlain || t < end) {
+              if (kPlain || t < s.len) {
+                if (!kPlain && (cuts >> u & 1u)) {
+                  seen = 0;
+#pragma unroll
+                  for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                  float g = gin[u][i];
+                  if (a.silu) {
+                    float pre = bias[i];
+#pragma unroll
+                    for (int j = 0; j < W - 1; ++j) pre = fmaf(w[i][j], h[j][i], pre);
+                    pre = fmaf(w[i][W - 1], xin[u][i], pre);
+                    const float sg = sigmoid(pre);
+                    g *= sg * fmaf(pre, 1.0f - sg, 1.0f);
+                  }
+                  pend[0][i] = fmaf(w[i][W - 1], g, pend[0][i]);
+#pragma unroll
+                  for (int j = 1; j < W; ++j)
+                    if (kPlain || (seen >> (j - 1) & 1u)) pend[j][i] = fmaf(w[i][W - 1 - j], g, pend[j][i]);
+                  if (kPlain || t < s.t1) {
+                    db[i] += g;
+#pragma unroll
+                    for (int k = 0; k < W - 1; ++k) dw[i][k] = fmaf(h[k][i], g, dw[i][k]);
+                    dw[i][W - 1] = fmaf(xin[u][i], g, dw[i][W - 1]);
+                  }
+                }
+                if (!kPlain && t == s.len - 1 && df) {             // the state behind the last token
+#pragma unroll
+                  for (int j = 0; j < W - 1; ++j)
+                    if (j == 0 || (seen >> (j - 1) & 1u)) {
+                      float e[V];
+                      load_vec<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D, e);
+#pragma unroll
+                      for (int i = 0; i < V; ++i) pend[j][i] += e[i];
+                    }
+                }
               }
+              const int done = t - (W - 1);
+              if (done >= s.t0 && done < s.t1) store_vec<T, V>(dx + done * a.y_t, pend[W - 1]);
+              else if (done < 0 && ds) store_vec<T, V>(ds + static_cast<int64_t>(W - 1 + done) * a.D, pend[W - 1]);
 #pragma unroll
               for (int i = 0; i < V; ++i) {
-                float g = gin[u][i];
-                if (a.silu) {
-                  float pre = bias[i];
 #pragma unroll
-                  for (int j = 0; j < W - 1; ++j) pre = fmaf(w[i][j], h[j][i], pre);
-                  pre = fmaf(w[i][W - 1], xin[u][i], pre);
-                  const float s = sigmoid(pre);
-                  g *= s * fmaf(pre, 1.0f - s, 1.0f);
-                }
-                pend[0][i] = fmaf(w[i][W - 1], g, pend[0][i]);
+                for (int j = W - 1; j > 0; --j) pend[j][i] = pend[j - 1][i];
+                pend[0][i] = 0.0f;
 #pragma unroll
-                for (int j = 1; j < W; ++j)
-                  if (seen >> (j - 1) & 1u) pend[j][i] = fmaf(w[i][W - 1 - j], g, pend[j][i]);
-                if (t < t1) {
-                  db[i] += g;
-#pragma unroll
-                  for (int k = 0; k < W - 1; ++k) dw[i][k] = fmaf(h[k][i], g, dw[i][k]);
-                  dw[i][W - 1] = fmaf(xin[u][i], g, dw[i][W - 1]);
-                }
+                for (int j = 0; j + 1 < W - 1; ++j) h[j][i] = h[j + 1][i];
+                h[W - 2][i] = xin[u][i];
               }
-              if (t == len - 1 && df) {              // the state behind the last token
-#pragma unroll
-                for (int j = 0; j < W - 1; ++j)
-                  if (j == 0 || (seen >> (j - 1) & 1u)) {
-                    float e[V];
-                    load_vec<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D, e);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) pend[j][i] += e[i];
-                  }
-              }
+              if (!kPlain) seen = (seen << 1) | 1u;
             }
-            const int done = t - (W - 1);
-            if (done >= t0 && done < t1) store_vec<T, V>(dx + done * a.y_t, pend[W - 1]);
-            else if (done < 0 && ds) store_vec<T, V>(ds + static_cast<int64_t>(W - 1 + done) * a.D, pend[W - 1]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-#pragma unroll
-              for (int j = W - 1; j > 0; --j) pend[j][i] = pend[j - 1][i];
-              pend[0][i] = 0.0f;
-#pragma unroll
-              for (int j = 0; j + 1 < W - 1; ++j) h[j][i] = h[j + 1][i];
-              h[W - 2][i] = xin[u][i];
-            }
-            seen = (seen << 1) | 1u;
           }
-        }
+        };
+        if (!cuts && (seen & kAll) == kAll && tb + U <= s.t1 && tb + U < s.len) work(std::true_type{});
+        else work(std::false_type{});
       }
     }
   }
@@ -370,11 +420,12 @@ template <typename F> int by_width(int W, F f) {
   return static_cast<int>(cudaErrorInvalidValue);
 }
 
-template <typename T, int W, int V> int launch_conv(ConvArgs a, cudaStream_t s) {
-  const int64_t n = static_cast<int64_t>(a.D / V) * a.chunks * a.B;
-  const int64_t blocks = surfk::ceil_div(n, 256);
-  if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
-  conv_kernel<T, W, V><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+template <typename T, int W, int V> int launch_conv(ConvArgs a, int rows, cudaStream_t s) {
+  const int groups = a.D / V;
+  int bx = 1;
+  while (bx < 32 && bx < groups) bx *= 2;
+  const dim3 grid(static_cast<unsigned>(surfk::ceil_div(groups, bx)), static_cast<unsigned>(rows));
+  conv_kernel<T, W, V><<<grid, dim3(bx, 256 / bx), 0, s>>>(a, a.B * a.chunks);
   SURF_RETURN_LAUNCH();
 }
 
@@ -397,14 +448,14 @@ int launch_grad(ConvArgs a, int rows, float* dw, float* dbias, cudaStream_t s) {
 }  // namespace
 
 // vec: D is a multiple of 4 and every row starts on a 4-element boundary
-SURF_EXPORT int surf_seq_conv(const void* args, int dtype, int W, int vec, void* stream) {
+SURF_EXPORT int surf_seq_conv(const void* args, int dtype, int W, int vec, int rows, void* stream) {
   const ConvArgs a = *static_cast<const ConvArgs*>(args);
-  if (a.B <= 0 || a.D <= 0) return 0;
+  if (a.D <= 0 || rows <= 0 || rows > 65535) return static_cast<int>(cudaErrorInvalidValue);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_width(W, [&](auto w) {
     constexpr int kW = decltype(w)::value;
-    if (dtype == kBf16) return vec ? launch_conv<bf16, kW, kV>(a, s) : launch_conv<bf16, kW, 1>(a, s);
-    return vec ? launch_conv<float, kW, kV>(a, s) : launch_conv<float, kW, 1>(a, s);
+    if (dtype == kBf16) return vec ? launch_conv<bf16, kW, kV>(a, rows, s) : launch_conv<bf16, kW, 1>(a, rows, s);
+    return vec ? launch_conv<float, kW, kV>(a, rows, s) : launch_conv<float, kW, 1>(a, rows, s);
   });
 }
 

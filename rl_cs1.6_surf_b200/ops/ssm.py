@@ -35,7 +35,7 @@ from .gemm import error_flag
 SLIB = "libsurf_seq.so"
 _V, _I, _L = _lib._V, _lib._I, _lib._L
 _lib.register(SLIB, {
-    "surf_seq_conv": (_I, [c_char_p, _I, _I, _I, _V]),
+    "surf_seq_conv": (_I, [c_char_p, _I, _I, _I, _I, _V]),
     "surf_seq_conv_grad": (_I, [c_char_p, _I, _I, _I, _I, _V, _V, _V]),
     "surf_seq_conv_step": (_I, [_V, _L, _V, _V, _V, _V, _V, _I, _V, _L, _I, _I, _I, _I, _I, _I, _V, _V]),
     "surf_seq_scan": (_I, [c_char_p, _I, _V]),
@@ -142,6 +142,18 @@ def _conv_check(what, x, weight, bias, state, reset, lengths):
     return code, 4 - 2 * code, at, b, t, d, w
 
 
+def _stretches(b: int, t: int, groups: int, per_sm: int):
+    """(tokens of a stretch, stretches of a row, rows of blocks) of the convolution: the
+    longest stretch (each reads width - 1 tokens of its neighbour again) that still gives
+    every SM 1024 threads, and ``per_sm`` blocks of 256 threads on an SM to take them."""
+    tt = 64
+    while tt > 8 and b * -(-t // tt) * groups < 148 * 1024:
+        tt //= 2
+    chunks = max(1, -(-t // tt))
+    bx = min(32, 1 << (groups - 1).bit_length())
+    return tt, chunks, max(1, min(-(-b * chunks * bx // 256), -(-148 * per_sm // -(-groups // bx)), 65535))
+
+
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
                 state: Optional[torch.Tensor] = None, reset: Optional[torch.Tensor] = None,
                 lengths: Optional[torch.Tensor] = None, silu: bool = True, out: Optional[torch.Tensor] = None):
@@ -158,11 +170,11 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if b == 0 or d == 0:
         return out, final
     vec = (_bits(e, x, out, state) | d * e) % (4 * e) == 0
-    tt = 16
+    tt, chunks, rows = _stretches(b, t, d // 4 if vec else d, 8)
     args = _CONV.pack(_p(x), 0, _p(state), 0, _p(weight), _p(bias), _p(reset), _p(lengths), out.data_ptr(),
                       final.data_ptr(), 0, x.stride(0), x.stride(1), 0, 0, out.stride(0), out.stride(1), t,
-                      b, t, d, int(silu), tt, max(1, -(-t // tt)))
-    launch(_lib.lib(SLIB).surf_seq_conv, "surf_seq_conv", at, args, code, w, int(vec))
+                      b, t, d, int(silu), tt, chunks)
+    launch(_lib.lib(SLIB).surf_seq_conv, "surf_seq_conv", at, args, code, w, int(vec), rows)
     return out, final
 
 
@@ -184,12 +196,7 @@ def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bi
     dw = torch.empty((d, w), dtype=torch.float32, device=dev)
     db = torch.empty(d, dtype=torch.float32, device=dev) if bias is not None else None
     vec = (_bits(e, x, dy, state, dfinal) | d * e) % (4 * e) == 0
-    tt = 16
-    chunks = max(1, -(-t // tt))
-    groups = d // 4 if vec else d
-    bx = min(32, 1 << (groups - 1).bit_length())
-    # rows of partial sums: about four blocks per SM, none without work
-    rows = max(1, min(-(-b * chunks // (256 // bx)), -(-592 // -(-groups // bx))))
+    tt, chunks, rows = _stretches(b, t, d // 4 if vec else d, 4)
     part = torch.empty((rows, w + 1, d), dtype=torch.float32, device=dev)
     args = _CONV.pack(_p(x), dy.data_ptr(), _p(state), _p(dfinal), _p(weight), _p(bias), _p(reset), _p(lengths),
                       dx.data_ptr(), _p(dstate), part.data_ptr(), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1),
