@@ -35,28 +35,95 @@ struct ConvArgs {
   int tt, chunks;             // tokens of a stretch, stretches of a row
 };
 
-// 16-byte vectors would hold 8 bf16 channels, and with them the window, weights
-// and sums of the gradient no longer fit the registers: 4 channels for both types.
-constexpr int kV = 4;
+// Channels of a thread: 4 in the forward (8-byte loads of bf16), 2 in the gradient, whose
+// window, weights and sums of 4 channels took 186 registers (8 warps on an SM). All the
+// arithmetic is on pairs of channels (f32x2), a lone channel being half a pair.
+constexpr int kVFwd = 4, kVGrad = 2;
+template <int V> constexpr int kPairs = (V + 1) / 2;
+template <int V> struct Pairs { f2 p[kPairs<V>]; };
 
-// The channels' weights: V * W neighbouring numbers, in 16-byte pieces for V = 4.
-template <int W, int V> __device__ __forceinline__ void load_weights(const float* p, float (&w)[V][W]) {
-  if constexpr (V == 4) {
-    float flat[V * W];
+template <int V> __device__ __forceinline__ Pairs<V> zeros() {
+  Pairs<V> r;
 #pragma unroll
-    for (int q = 0; q < W; ++q) {
+  for (int i = 0; i < kPairs<V>; ++i) r.p[i].v = 0;
+  return r;
+}
+template <int V> __device__ __forceinline__ Pairs<V> to_pairs(const float (&v)[V]) {
+  Pairs<V> r;
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) r.p[i] = pack2(v[2 * i], 2 * i + 1 < V ? v[(2 * i + 1) % V] : 0.0f);
+  return r;
+}
+template <int V> __device__ __forceinline__ void from_pairs(const Pairs<V>& r, float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    float lo, hi;
+    unpack2(r.p[i], lo, hi);
+    v[2 * i] = lo;
+    if (2 * i + 1 < V) v[(2 * i + 1) % V] = hi;
+  }
+}
+template <int V> __device__ __forceinline__ void madd(Pairs<V>& c, const Pairs<V>& x, const Pairs<V>& y) {
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) c.p[i] = fma2(x.p[i], y.p[i], c.p[i]);
+}
+
+// V channels of a row as they are in memory
+template <typename T, int V> struct Raw {
+  static constexpr int kBytes = V * static_cast<int>(sizeof(T));
+  using Word = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, std::conditional_t<kBytes == 4, uint32_t, uint16_t>>>;
+  Word w;
+  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const Word*>(p); }
+  __device__ __forceinline__ void clear() { w = Word{}; }
+  __device__ __forceinline__ Pairs<V> pairs() const {
+    float v[V];
+    if constexpr (sizeof(T) == 4) {
+      const float* q = reinterpret_cast<const float*>(&w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = q[i];
+    } else if constexpr (V == 1) {
+      v[0] = __uint_as_float(static_cast<uint32_t>(w) << 16);
+    } else {
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(&w);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        v[2 * i] = __uint_as_float(q[i] << 16);
+        v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+      }
+    }
+    return to_pairs<V>(v);
+  }
+};
+template <typename T, int V> __device__ __forceinline__ Pairs<V> load_pairs_of(const T* p) {
+  Raw<T, V> r;
+  r.load(p);
+  return r.pairs();
+}
+template <typename T, int V> __device__ __forceinline__ void store_pairs_of(T* p, const Pairs<V>& r) {
+  float v[V];
+  from_pairs<V>(r, v);
+  store_vec<T, V>(p, v);
+}
+
+// The channels' weights, tap by tap
+template <int W, int V> __device__ __forceinline__ void load_weights(const float* p, Pairs<V> (&w)[W]) {
+  float flat[V * W];
+  if constexpr (V * W % 4 == 0 && V > 1) {
+#pragma unroll
+    for (int q = 0; q < V * W / 4; ++q) {
       const float4 v = reinterpret_cast<const float4*>(p)[q];
       flat[4 * q] = v.x; flat[4 * q + 1] = v.y; flat[4 * q + 2] = v.z; flat[4 * q + 3] = v.w;
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int k = 0; k < W; ++k) w[i][k] = flat[i * W + k];
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int q = 0; q < V * W; ++q) flat[q] = p[q];
+  }
 #pragma unroll
-      for (int k = 0; k < W; ++k) w[i][k] = p[i * W + k];
+  for (int k = 0; k < W; ++k) {
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = flat[i * W + k];
+    w[k] = to_pairs<V>(v);
   }
 }
 
@@ -93,24 +160,21 @@ template <typename T, int U> __device__ __forceinline__ unsigned cuts_of(const S
 // The W - 1 tokens before the stretch as its first token finds them (before its own
 // reset); returns bit j: it sees token t0 - 1 - j.
 template <typename T, int W, int V>
-__device__ __forceinline__ unsigned window_of(const ConvArgs& a, const Stretch<T>& s, float (&h)[W - 1][V]) {
+__device__ __forceinline__ unsigned window_of(const ConvArgs& a, const Stretch<T>& s, Pairs<V> (&h)[W - 1]) {
   unsigned seen = 0;
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
     const int t = s.t0 - (W - 1) + j;
-#pragma unroll
-    for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
+    h[j] = zeros<V>();
     if (t >= 0 && t < s.len) {
       if (s.cut(t)) {
         seen = 0;
 #pragma unroll
-        for (int q = 0; q < j; ++q)
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[q][i] = 0.0f;
+        for (int q = 0; q < j; ++q) h[q] = zeros<V>();
       }
-      load_vec<T, V>(s.x + t * a.x_t, h[j]);
+      h[j] = load_pairs_of<T, V>(s.x + t * a.x_t);
     } else if (t < 0 && s.state) {
-      load_vec<T, V>(s.state + static_cast<int64_t>(W - 1 + t) * a.D, h[j]);
+      h[j] = load_pairs_of<T, V>(s.state + static_cast<int64_t>(W - 1 + t) * a.D);
     }
     seen = (seen << 1) | 1u;
   }
@@ -118,73 +182,70 @@ __device__ __forceinline__ unsigned window_of(const ConvArgs& a, const Stretch<T
 }
 
 // ---- whole sequences ----------------------------------------------------------------
-// A thread keeps its channels' weights and takes one stretch after the other; the tokens
-// of the next step are on their way while this step's are worked on.
+// A thread keeps its channels' weights and takes one stretch after the other, kU tokens
+// loaded at a time.
+constexpr int kU = 8;
+
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(256) conv_kernel(ConvArgs a, int items) {
+__global__ void __launch_bounds__(256, 4) conv_kernel(ConvArgs a, int items) {
   const int cg = blockIdx.x * blockDim.x + threadIdx.x, d = cg * V;
   if (cg >= a.D / V) return;
-  float w[V][W], bias[V];
+  Pairs<V> w[W], bias = zeros<V>();
   load_weights<W, V>(a.w + static_cast<int64_t>(d) * W, w);
+  if (a.bias) {
+    float v[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) bias[i] = a.bias ? a.bias[d + i] : 0.0f;
+    for (int i = 0; i < V; ++i) v[i] = a.bias[d + i];
+    bias = to_pairs<V>(v);
+  }
   for (int item = blockIdx.y * blockDim.y + threadIdx.y; item < items; item += gridDim.y * blockDim.y) {
     const Stretch<T> s(a, item, d, W);
-    T* __restrict__ y = static_cast<T*>(a.y) + s.b * a.y_b + d;
-    float h[W - 1][V];
+    T* y = static_cast<T*>(a.y) + s.b * a.y_b + d;
+    Pairs<V> h[W - 1];
     window_of<T, W, V>(a, s, h);
-    constexpr int U = 8;
     const int live = min(s.t1, s.len);
-    float next[U][V];
-    auto fetch = [&](int t) {
+    // `whole`: kU tokens are there and none of them starts an episode
+    auto step = [&](int t, unsigned cuts, auto whole) {
+      Raw<T, V> in[kU];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (t + u < live) load_vec<T, V>(s.x + (t + u) * a.x_t, next[u]);
-    };
-    fetch(s.t0);
-    for (int t = s.t0; t < live; t += U) {
-      float in[U][V];
+      for (int u = 0; u < kU; ++u)
+        if (decltype(whole)::value || t + u < live) in[u].load(s.x + (t + u) * a.x_t);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < kU; ++u) {
+        if (decltype(whole)::value || t + u < live) {
+          if (!decltype(whole)::value && (cuts >> u & 1u)) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) in[u][i] = next[u][i];
-      const unsigned cuts = cuts_of<T, U>(s, t);
-      fetch(t + U);
-      auto work = [&](auto with_cuts) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (t + u < live) {
-            float o[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              float acc = bias[i];
-#pragma unroll
-              for (int j = 0; j < W - 1; ++j) {
-                if (decltype(with_cuts)::value && (cuts >> u & 1u)) h[j][i] = 0.0f;
-                acc = fmaf(w[i][j], h[j][i], acc);
-              }
-              acc = fmaf(w[i][W - 1], in[u][i], acc);
-#pragma unroll
-              for (int j = 0; j + 1 < W - 1; ++j) h[j][i] = h[j + 1][i];
-              h[W - 2][i] = in[u][i];
-              o[i] = a.silu ? acc * sigmoid(acc) : acc;
-            }
-            store_vec<T, V>(y + (t + u) * a.y_t, o);
+            for (int j = 0; j < W - 1; ++j) h[j] = zeros<V>();
           }
-        }
-      };
-      if (cuts) work(std::true_type{});
-      else work(std::false_type{});
-    }
-    float zero[V];
+          const Pairs<V> now = in[u].pairs();
+          Pairs<V> acc = bias;
 #pragma unroll
-    for (int i = 0; i < V; ++i) zero[i] = 0.0f;
-    for (int t = max(s.t0, live); t < s.t1; ++t) store_vec<T, V>(y + t * a.y_t, zero);
+          for (int j = 0; j < W - 1; ++j) madd<V>(acc, w[j], h[j]);
+          madd<V>(acc, w[W - 1], now);
+#pragma unroll
+          for (int j = 0; j + 1 < W - 1; ++j) h[j] = h[j + 1];
+          h[W - 2] = now;
+          float o[V];
+          from_pairs<V>(acc, o);
+          if (a.silu) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] *= sigmoid(o[i]);
+          }
+          store_vec<T, V>(y + (t + u) * a.y_t, o);
+        }
+      }
+    };
+    for (int t = s.t0; t < live; t += kU) {
+      const unsigned cuts = cuts_of<T, kU>(s, t);
+      if (!cuts && t + kU <= live) step(t, 0, std::true_type{});
+      else step(t, cuts, std::false_type{});
+    }
+    for (int t = max(s.t0, live); t < s.t1; ++t) store_pairs_of<T, V>(y + t * a.y_t, zeros<V>());
     // what the next token finds behind it: by the stretch of the last token
     if (a.final_state && (s.len > 0 ? (s.len - 1 >= s.t0 && s.len - 1 < s.t0 + a.tt) : s.chunk == 0)) {
       T* f = static_cast<T*>(a.final_state) + static_cast<int64_t>(s.b) * (W - 1) * a.D + d;
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) store_vec<T, V>(f + static_cast<int64_t>(j) * a.D, h[j]);
+      for (int j = 0; j < W - 1; ++j) store_pairs_of<T, V>(f + static_cast<int64_t>(j) * a.D, h[j]);
     }
   }
 }
@@ -197,132 +258,118 @@ __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a, int items) {
 // sums a block joins in shared memory and leaves as one row of `part`, summed in
 // row order by conv_reduce_kernel: no atomics, so a rerun gives the same bits.
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(256) conv_grad_kernel(ConvArgs a, int items) {
+__global__ void __launch_bounds__(256, 3) conv_grad_kernel(ConvArgs a, int items) {
   extern __shared__ float red[];                                // [blockDim.y][W + 1][blockDim.x * V]
   const int cg = blockIdx.x * blockDim.x + threadIdx.x;
   const int d = cg * V;
   const bool on = cg < a.D / V;
-  float w[V][W], bias[V], dw[V][W], db[V];
+  Pairs<V> w[W], dw[W], bias = zeros<V>(), db = zeros<V>();
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = on && a.bias ? a.bias[d + i] : 0.0f;
-    db[i] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < W; ++k) dw[i][k] = w[i][k] = 0.0f;
-  }
+  for (int k = 0; k < W; ++k) dw[k] = w[k] = zeros<V>();
   if (on) {
     load_weights<W, V>(a.w + static_cast<int64_t>(d) * W, w);
+    if (a.bias) {
+      float v[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = a.bias[d + i];
+      bias = to_pairs<V>(v);
+    }
     for (int item = blockIdx.y * blockDim.y + threadIdx.y; item < items; item += gridDim.y * blockDim.y) {
       const Stretch<T> s(a, item, d, W);
       const T* dy = static_cast<const T*>(a.dy) + s.b * a.dy_b + d;
-      T* __restrict__ dx = static_cast<T*>(a.y) + s.b * a.y_b + d;
+      T* dx = static_cast<T*>(a.y) + s.b * a.y_b + d;
       const int64_t ends = static_cast<int64_t>(s.b) * (W - 1) * a.D + d;
       const T* df = a.dfinal ? static_cast<const T*>(a.dfinal) + ends : nullptr;
-      T* __restrict__ ds = a.final_state ? static_cast<T*>(a.final_state) + ends : nullptr;
-      float h[W - 1][V], pend[W][V];                 // pend[j]: dx of token t - j so far
+      T* ds = a.final_state ? static_cast<T*>(a.final_state) + ends : nullptr;
+      Pairs<V> h[W - 1], pend[W];                    // pend[j]: dx of token t - j so far
       unsigned seen = window_of<T, W, V>(a, s, h);   // bit j: token t sees token t - 1 - j
       constexpr unsigned kAll = (1u << (W - 1)) - 1u;
 #pragma unroll
-      for (int j = 0; j < W; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) pend[j][i] = 0.0f;
+      for (int j = 0; j < W; ++j) pend[j] = zeros<V>();
       if (s.len == 0 && s.chunk == 0 && df) {        // an empty row hands its state on
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) load_vec<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D, pend[j + 1]);
+        for (int j = 0; j < W - 1; ++j) pend[j + 1] = load_pairs_of<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D);
       }
       const int end = s.t1 + W - 1;
-      constexpr int U = 4;
-      float nx[U][V], ng[U][V];
-      auto fetch = [&](int t) {
+      // whole: kU tokens of the stretch's own, past its first W - 1, no reset in sight, the row goes on
+      auto step = [&](int tb, unsigned cuts, auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
+        Raw<T, V> xin[kU], gin[kU];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (t + u < end && t + u < s.len) {
-            load_vec<T, V>(s.x + (t + u) * a.x_t, nx[u]);
-            load_vec<T, V>(dy + (t + u) * a.dy_t, ng[u]);
+        for (int u = 0; u < kU; ++u) {
+          if (kWhole || (tb + u < end && tb + u < s.len)) {
+            xin[u].load(s.x + (tb + u) * a.x_t);
+            gin[u].load(dy + (tb + u) * a.dy_t);
           } else {
+            xin[u].clear();
+            gin[u].clear();
+          }
+        }
 #pragma unroll
-            for (int i = 0; i < V; ++i) nx[u][i] = ng[u][i] = 0.0f;
+        for (int u = 0; u < kU; ++u) {
+          const int t = tb + u;
+          if (kWhole || t < end) {
+            const Pairs<V> now = xin[u].pairs();
+            if (kWhole || t < s.len) {
+              if (!kWhole && (cuts >> u & 1u)) {
+                seen = 0;
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) h[j] = zeros<V>();
+              }
+              Pairs<V> g = gin[u].pairs();
+              if (a.silu) {
+                Pairs<V> pre = bias;
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) madd<V>(pre, w[j], h[j]);
+                madd<V>(pre, w[W - 1], now);
+                float p[V], q[V];
+                from_pairs<V>(pre, p);
+                from_pairs<V>(g, q);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                  const float sg = sigmoid(p[i]);
+                  q[i] *= sg * fmaf(p[i], 1.0f - sg, 1.0f);
+                }
+                g = to_pairs<V>(q);
+              }
+              madd<V>(pend[0], w[W - 1], g);
+#pragma unroll
+              for (int j = 1; j < W; ++j)
+                if (kWhole || (seen >> (j - 1) & 1u)) madd<V>(pend[j], w[W - 1 - j], g);
+              if (kWhole || t < s.t1) {
+#pragma unroll
+                for (int i = 0; i < kPairs<V>; ++i) db.p[i] = add2(db.p[i], g.p[i]);
+#pragma unroll
+                for (int k = 0; k < W - 1; ++k) madd<V>(dw[k], h[k], g);
+                madd<V>(dw[W - 1], now, g);
+              }
+              if (!kWhole && t == s.len - 1 && df) {             // the state behind the last token
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j)
+                  if (j == 0 || (seen >> (j - 1) & 1u)) {
+                    const Pairs<V> e = load_pairs_of<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D);
+#pragma unroll
+                    for (int i = 0; i < kPairs<V>; ++i) pend[j].p[i] = add2(pend[j].p[i], e.p[i]);
+                  }
+              }
+            }
+            const int done = t - (W - 1);
+            if (kWhole || (done >= s.t0 && done < s.t1)) store_pairs_of<T, V>(dx + done * a.y_t, pend[W - 1]);
+            else if (done < 0 && ds) store_pairs_of<T, V>(ds + static_cast<int64_t>(W - 1 + done) * a.D, pend[W - 1]);
+#pragma unroll
+            for (int j = W - 1; j > 0; --j) pend[j] = pend[j - 1];
+            pend[0] = zeros<V>();
+#pragma unroll
+            for (int j = 0; j + 1 < W - 1; ++j) h[j] = h[j + 1];
+            h[W - 2] = now;
+            if (!kWhole) seen = (seen << 1) | 1u;
           }
         }
       };
-      fetch(s.t0);
-      for (int tb = s.t0; tb < end; tb += U) {
-        float xin[U][V], gin[U][V];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            xin[u][i] = nx[u][i];
-            gin[u][i] = ng[u][i];
-          }
-        const unsigned cuts = cuts_of<T, U>(s, tb);
-        fetch(tb + U);
-        // kPlain: U tokens of the stretch's own, no reset in sight, the row goes on
-        auto work = [&](auto is_plain) {
-          constexpr bool kPlain = decltype(is_plain)::value;
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int t = tb + u;
-            if (kPlain || t < end) {
-              if (kPlain || t < s.len) {
-                if (!kPlain && (cuts >> u & 1u)) {
-                  seen = 0;
-#pragma unroll
-                  for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) h[j][i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                  float g = gin[u][i];
-                  if (a.silu) {
-                    float pre = bias[i];
-#pragma unroll
-                    for (int j = 0; j < W - 1; ++j) pre = fmaf(w[i][j], h[j][i], pre);
-                    pre = fmaf(w[i][W - 1], xin[u][i], pre);
-                    const float sg = sigmoid(pre);
-                    g *= sg * fmaf(pre, 1.0f - sg, 1.0f);
-                  }
-                  pend[0][i] = fmaf(w[i][W - 1], g, pend[0][i]);
-#pragma unroll
-                  for (int j = 1; j < W; ++j)
-                    if (kPlain || (seen >> (j - 1) & 1u)) pend[j][i] = fmaf(w[i][W - 1 - j], g, pend[j][i]);
-                  if (kPlain || t < s.t1) {
-                    db[i] += g;
-#pragma unroll
-                    for (int k = 0; k < W - 1; ++k) dw[i][k] = fmaf(h[k][i], g, dw[i][k]);
-                    dw[i][W - 1] = fmaf(xin[u][i], g, dw[i][W - 1]);
-                  }
-                }
-                if (!kPlain && t == s.len - 1 && df) {             // the state behind the last token
-#pragma unroll
-                  for (int j = 0; j < W - 1; ++j)
-                    if (j == 0 || (seen >> (j - 1) & 1u)) {
-                      float e[V];
-                      load_vec<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D, e);
-#pragma unroll
-                      for (int i = 0; i < V; ++i) pend[j][i] += e[i];
-                    }
-                }
-              }
-              const int done = t - (W - 1);
-              if (done >= s.t0 && done < s.t1) store_vec<T, V>(dx + done * a.y_t, pend[W - 1]);
-              else if (done < 0 && ds) store_vec<T, V>(ds + static_cast<int64_t>(W - 1 + done) * a.D, pend[W - 1]);
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-#pragma unroll
-                for (int j = W - 1; j > 0; --j) pend[j][i] = pend[j - 1][i];
-                pend[0][i] = 0.0f;
-#pragma unroll
-                for (int j = 0; j + 1 < W - 1; ++j) h[j][i] = h[j + 1][i];
-                h[W - 2][i] = xin[u][i];
-              }
-              if (!kPlain) seen = (seen << 1) | 1u;
-            }
-          }
-        };
-        if (!cuts && (seen & kAll) == kAll && tb + U <= s.t1 && tb + U < s.len) work(std::true_type{});
-        else work(std::false_type{});
+      for (int tb = s.t0; tb < end; tb += kU) {
+        const unsigned cuts = cuts_of<T, kU>(s, tb);
+        if (!cuts && (seen & kAll) == kAll && tb > s.t0 && tb + kU <= s.t1 && tb + kU < s.len) step(tb, 0, std::true_type{});
+        else step(tb, cuts, std::false_type{});
       }
     }
   }
@@ -330,10 +377,11 @@ __global__ void __launch_bounds__(256) conv_grad_kernel(ConvArgs a, int items) {
   const int cols = blockDim.x * V;
   float* mine = red + threadIdx.y * (W + 1) * cols + threadIdx.x * V;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int k = 0; k <= W; ++k) {
+    float v[V];
+    from_pairs<V>(k < W ? dw[k % W] : db, v);
 #pragma unroll
-    for (int k = 0; k < W; ++k) mine[k * cols + i] = dw[i][k];
-    mine[W * cols + i] = db[i];
+    for (int i = 0; i < V; ++i) mine[k * cols + i] = v[i];
   }
   __syncthreads();
   const int tid = threadIdx.y * blockDim.x + threadIdx.x;
@@ -410,7 +458,7 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const T* x, int64_t ldx,
 }
 
 // ---- launches -------------------------------------------------------------------------------
-// width -> template argument; vectors of kV channels where `vec`, else one
+// width -> template argument; several channels a thread where `vec`, else one
 template <typename F> int by_width(int W, F f) {
   switch (W) {
     case 2: return f(std::integral_constant<int, 2>{});
@@ -447,15 +495,15 @@ int launch_grad(ConvArgs a, int rows, float* dw, float* dbias, cudaStream_t s) {
 
 }  // namespace
 
-// vec: D is a multiple of 4 and every row starts on a 4-element boundary
+// vec: D is a multiple of 4 (gradient: of 2) and every row starts on a boundary of so many elements
 SURF_EXPORT int surf_seq_conv(const void* args, int dtype, int W, int vec, int rows, void* stream) {
   const ConvArgs a = *static_cast<const ConvArgs*>(args);
   if (a.D <= 0 || rows <= 0 || rows > 65535) return static_cast<int>(cudaErrorInvalidValue);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_width(W, [&](auto w) {
     constexpr int kW = decltype(w)::value;
-    if (dtype == kBf16) return vec ? launch_conv<bf16, kW, kV>(a, rows, s) : launch_conv<bf16, kW, 1>(a, rows, s);
-    return vec ? launch_conv<float, kW, kV>(a, rows, s) : launch_conv<float, kW, 1>(a, rows, s);
+    if (dtype == kBf16) return vec ? launch_conv<bf16, kW, kVFwd>(a, rows, s) : launch_conv<bf16, kW, 1>(a, rows, s);
+    return vec ? launch_conv<float, kW, kVFwd>(a, rows, s) : launch_conv<float, kW, 1>(a, rows, s);
   });
 }
 
@@ -466,8 +514,8 @@ SURF_EXPORT int surf_seq_conv_grad(const void* args, int dtype, int W, int vec, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_width(W, [&](auto w) {
     constexpr int kW = decltype(w)::value;
-    if (dtype == kBf16) return vec ? launch_grad<bf16, kW, kV>(a, rows, dw, dbias, s) : launch_grad<bf16, kW, 1>(a, rows, dw, dbias, s);
-    return vec ? launch_grad<float, kW, kV>(a, rows, dw, dbias, s) : launch_grad<float, kW, 1>(a, rows, dw, dbias, s);
+    if (dtype == kBf16) return vec ? launch_grad<bf16, kW, kVGrad>(a, rows, dw, dbias, s) : launch_grad<bf16, kW, 1>(a, rows, dw, dbias, s);
+    return vec ? launch_grad<float, kW, kVGrad>(a, rows, dw, dbias, s) : launch_grad<float, kW, 1>(a, rows, dw, dbias, s);
   });
 }
 
@@ -487,7 +535,7 @@ SURF_EXPORT int surf_seq_conv_step(const void* x, int64_t ldx, const float* w, c
           D, silu, err);
       SURF_RETURN_LAUNCH();
     };
-    if (dtype == kBf16) return vec ? go(bf16{}, std::integral_constant<int, kV>{}) : go(bf16{}, std::integral_constant<int, 1>{});
-    return vec ? go(float{}, std::integral_constant<int, kV>{}) : go(float{}, std::integral_constant<int, 1>{});
+    if (dtype == kBf16) return vec ? go(bf16{}, std::integral_constant<int, kVFwd>{}) : go(bf16{}, std::integral_constant<int, 1>{});
+    return vec ? go(float{}, std::integral_constant<int, kVFwd>{}) : go(float{}, std::integral_constant<int, 1>{});
   });
 }

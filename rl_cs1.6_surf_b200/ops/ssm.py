@@ -170,7 +170,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if b == 0 or d == 0:
         return out, final
     vec = (_bits(e, x, out, state) | d * e) % (4 * e) == 0
-    tt, chunks, rows = _stretches(b, t, d // 4 if vec else d, 8)
+    tt, chunks, rows = _stretches(b, t, d // 4 if vec else d, 4)
     args = _CONV.pack(_p(x), 0, _p(state), 0, _p(weight), _p(bias), _p(reset), _p(lengths), out.data_ptr(),
                       final.data_ptr(), 0, x.stride(0), x.stride(1), 0, 0, out.stride(0), out.stride(1), t,
                       b, t, d, int(silu), tt, chunks)
@@ -195,8 +195,8 @@ def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bi
         return ConvGrads(dx, torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dstate)
     dw = torch.empty((d, w), dtype=torch.float32, device=dev)
     db = torch.empty(d, dtype=torch.float32, device=dev) if bias is not None else None
-    vec = (_bits(e, x, dy, state, dfinal) | d * e) % (4 * e) == 0
-    tt, chunks, rows = _stretches(b, t, d // 4 if vec else d, 4)
+    vec = (_bits(e, x, dy, state, dfinal) | d * e) % (2 * e) == 0
+    tt, chunks, rows = _stretches(b, t, d // 2 if vec else d, 3)
     part = torch.empty((rows, w + 1, d), dtype=torch.float32, device=dev)
     args = _CONV.pack(_p(x), dy.data_ptr(), _p(state), _p(dfinal), _p(weight), _p(bias), _p(reset), _p(lengths),
                       dx.data_ptr(), _p(dstate), part.data_ptr(), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1),
