@@ -35,10 +35,16 @@ struct ConvArgs {
   int tt, chunks;             // tokens of a stretch, stretches of a row
 };
 
-// Channels of a thread: 4 in the forward (8-byte loads of bf16), 2 in the gradient, whose
-// window, weights and sums of 4 channels took 186 registers (8 warps on an SM). All the
-// arithmetic is on pairs of channels (f32x2), a lone channel being half a pair.
-constexpr int kVFwd = 4, kVGrad = 2;
+// Channels of a thread: in whole sequences 16 bytes of them in the forward, 8 in the
+// gradient (its weights, sums and pending dx fill the registers otherwise), 4 bytes where
+// rows are only aligned to that, else one. All the arithmetic is on pairs of channels
+// (f32x2), a lone channel being half a pair.
+//
+// Tokens come through a ring in shared memory, kU of them on their way to every thread by
+// asynchronous copies. A thread reads only what it has copied itself, so there are no
+// barriers; held in registers, 8 tokens cost the warps that hide the latency (gradient
+// 186 us with 2 channels a thread and 24 warps, 117 us with 16 warps and no spills).
+constexpr int kThreads = 256, kU = 8;
 template <int V> constexpr int kPairs = (V + 1) / 2;
 template <int V> struct Pairs { f2 p[kPairs<V>]; };
 
@@ -75,6 +81,11 @@ template <typename T, int V> struct Raw {
   Word w;
   __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const Word*>(p); }
   __device__ __forceinline__ void clear() { w = Word{}; }
+  static __device__ __forceinline__ void copy_async(Word* dst, const T* src) {
+    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+    if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else if constexpr (kBytes >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(kBytes) : "memory");
+  }
   __device__ __forceinline__ Pairs<V> pairs() const {
     float v[V];
     if constexpr (sizeof(T) == 4) {
@@ -146,16 +157,52 @@ template <typename T> struct Stretch {
   __device__ __forceinline__ bool cut(int t) const { return reset && t >= 0 && t < len && reset[t]; }
 };
 
-// Bit u: token t + u starts an episode, for the U tokens from t on.
-template <typename T, int U> __device__ __forceinline__ unsigned cuts_of(const Stretch<T>& s, int t) {
+// Bit u: token t + u starts an episode, for the 8 tokens from t on.
+template <typename T> __device__ __forceinline__ unsigned cuts_of(const Stretch<T>& s, int t) {
+  static_assert(kU == 8, "the flags of 8 tokens are one word");
+  if (!s.reset) return 0;
+  const uint8_t* p = s.reset + t;
+  if ((reinterpret_cast<uintptr_t>(p) & 7) == 0 && t + 8 <= s.len && *reinterpret_cast<const unsigned long long*>(p) == 0) return 0;
   unsigned m = 0;
-  if (s.reset) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (t + u < s.len && s.reset[t + u]) m |= 1u << u;
-  }
+  for (int u = 0; u < 8; ++u)
+    if (t + u < s.len && p[u]) m |= 1u << u;
   return m;
 }
+
+// The tokens of a row on their way to one thread: slot u of kU holds token t0 + u, then
+// t0 + u + kU, ... (kAsync), or the kU tokens of a step are loaded at its start.
+template <typename T, int V> struct Ring {
+  static constexpr bool kAsync = Raw<T, V>::kBytes >= 4;
+  typename Raw<T, V>::Word* slot;              // of this thread
+  const T* src;
+  int64_t stride;
+  int stop;                                    // first token that is not there
+  Raw<T, V> held[kAsync ? 1 : kU];
+  __device__ __forceinline__ void issue(int u, int t) {
+    if constexpr (kAsync)
+      if (t < stop) Raw<T, V>::copy_async(slot + u * kThreads, src + t * stride);
+  }
+  __device__ __forceinline__ void batch(int t) {
+    if constexpr (!kAsync) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        held[u].clear();
+        if (t + u < stop) held[u].load(src + (t + u) * stride);
+      }
+    }
+  }
+  // token t in slot u (anything if it is not there)
+  __device__ __forceinline__ Pairs<V> get(int u) {
+    if constexpr (kAsync) {
+      Raw<T, V> r;
+      r.w = slot[u * kThreads];
+      return r.pairs();
+    } else {
+      return held[u].pairs();
+    }
+  }
+};
 
 // The W - 1 tokens before the stretch as its first token finds them (before its own
 // reset); returns bit j: it sees token t0 - 1 - j.
@@ -182,12 +229,11 @@ __device__ __forceinline__ unsigned window_of(const ConvArgs& a, const Stretch<T
 }
 
 // ---- whole sequences ----------------------------------------------------------------
-// A thread keeps its channels' weights and takes one stretch after the other, kU tokens
-// loaded at a time.
-constexpr int kU = 8;
-
+// A thread keeps its channels' weights and takes one stretch after the other.
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(256, 4) conv_kernel(ConvArgs a, int items) {
+__global__ void __launch_bounds__(kThreads, 2) conv_kernel(ConvArgs a, int items) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  using Word = typename Raw<T, V>::Word;
   const int cg = blockIdx.x * blockDim.x + threadIdx.x, d = cg * V;
   if (cg >= a.D / V) return;
   Pairs<V> w[W], bias = zeros<V>();
@@ -204,20 +250,24 @@ __global__ void __launch_bounds__(256, 4) conv_kernel(ConvArgs a, int items) {
     Pairs<V> h[W - 1];
     window_of<T, W, V>(a, s, h);
     const int live = min(s.t1, s.len);
+    Ring<T, V> in{reinterpret_cast<Word*>(smem) + threadIdx.y * blockDim.x + threadIdx.x, s.x, a.x_t, live};
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      in.issue(u, s.t0 + u);
+      cp_async_commit();
+    }
     // `whole`: kU tokens are there and none of them starts an episode
     auto step = [&](int t, unsigned cuts, auto whole) {
-      Raw<T, V> in[kU];
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-        if (decltype(whole)::value || t + u < live) in[u].load(s.x + (t + u) * a.x_t);
+      in.batch(t);
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         if (decltype(whole)::value || t + u < live) {
+          cp_async_wait<kU - 1>();
           if (!decltype(whole)::value && (cuts >> u & 1u)) {
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) h[j] = zeros<V>();
           }
-          const Pairs<V> now = in[u].pairs();
+          const Pairs<V> now = in.get(u);
           Pairs<V> acc = bias;
 #pragma unroll
           for (int j = 0; j < W - 1; ++j) madd<V>(acc, w[j], h[j]);
@@ -232,14 +282,17 @@ __global__ void __launch_bounds__(256, 4) conv_kernel(ConvArgs a, int items) {
             for (int i = 0; i < V; ++i) o[i] *= sigmoid(o[i]);
           }
           store_vec<T, V>(y + (t + u) * a.y_t, o);
+          in.issue(u, t + u + kU);
+          cp_async_commit();
         }
       }
     };
     for (int t = s.t0; t < live; t += kU) {
-      const unsigned cuts = cuts_of<T, kU>(s, t);
+      const unsigned cuts = cuts_of<T>(s, t);
       if (!cuts && t + kU <= live) step(t, 0, std::true_type{});
       else step(t, cuts, std::false_type{});
     }
+    cp_async_wait<0>();
     for (int t = max(s.t0, live); t < s.t1; ++t) store_pairs_of<T, V>(y + t * a.y_t, zeros<V>());
     // what the next token finds behind it: by the stretch of the last token
     if (a.final_state && (s.len > 0 ? (s.len - 1 >= s.t0 && s.len - 1 < s.t0 + a.tt) : s.chunk == 0)) {
@@ -258,8 +311,10 @@ __global__ void __launch_bounds__(256, 4) conv_kernel(ConvArgs a, int items) {
 // sums a block joins in shared memory and leaves as one row of `part`, summed in
 // row order by conv_reduce_kernel: no atomics, so a rerun gives the same bits.
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(256, 3) conv_grad_kernel(ConvArgs a, int items) {
-  extern __shared__ float red[];                                // [blockDim.y][W + 1][blockDim.x * V]
+__global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int items) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  using Word = typename Raw<T, V>::Word;
+  float* red = reinterpret_cast<float*>(smem);                  // at the end: [blockDim.y][W + 1][blockDim.x * V]
   const int cg = blockIdx.x * blockDim.x + threadIdx.x;
   const int d = cg * V;
   const bool on = cg < a.D / V;
@@ -291,32 +346,33 @@ __global__ void __launch_bounds__(256, 3) conv_grad_kernel(ConvArgs a, int items
         for (int j = 0; j < W - 1; ++j) pend[j + 1] = load_pairs_of<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D);
       }
       const int end = s.t1 + W - 1;
+      Word* const slots = reinterpret_cast<Word*>(smem) + threadIdx.y * blockDim.x + threadIdx.x;
+      const int stop = min(end, s.len);
+      Ring<T, V> xin{slots, s.x, a.x_t, stop}, gin{slots + kU * kThreads, dy, a.dy_t, stop};
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        xin.issue(u, s.t0 + u);
+        gin.issue(u, s.t0 + u);
+        cp_async_commit();
+      }
       // whole: kU tokens of the stretch's own, past its first W - 1, no reset in sight, the row goes on
       auto step = [&](int tb, unsigned cuts, auto whole) {
         constexpr bool kWhole = decltype(whole)::value;
-        Raw<T, V> xin[kU], gin[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          if (kWhole || (tb + u < end && tb + u < s.len)) {
-            xin[u].load(s.x + (tb + u) * a.x_t);
-            gin[u].load(dy + (tb + u) * a.dy_t);
-          } else {
-            xin[u].clear();
-            gin[u].clear();
-          }
-        }
+        xin.batch(tb);
+        gin.batch(tb);
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
           const int t = tb + u;
           if (kWhole || t < end) {
-            const Pairs<V> now = xin[u].pairs();
+            cp_async_wait<kU - 1>();
+            const Pairs<V> now = kWhole || t < s.len ? xin.get(u) : zeros<V>();
             if (kWhole || t < s.len) {
               if (!kWhole && (cuts >> u & 1u)) {
                 seen = 0;
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) h[j] = zeros<V>();
               }
-              Pairs<V> g = gin[u].pairs();
+              Pairs<V> g = gin.get(u);
               if (a.silu) {
                 Pairs<V> pre = bias;
 #pragma unroll
@@ -363,16 +419,21 @@ __global__ void __launch_bounds__(256, 3) conv_grad_kernel(ConvArgs a, int items
             for (int j = 0; j + 1 < W - 1; ++j) h[j] = h[j + 1];
             h[W - 2] = now;
             if (!kWhole) seen = (seen << 1) | 1u;
+            xin.issue(u, t + kU);
+            gin.issue(u, t + kU);
+            cp_async_commit();
           }
         }
       };
       for (int tb = s.t0; tb < end; tb += kU) {
-        const unsigned cuts = cuts_of<T, kU>(s, tb);
+        const unsigned cuts = cuts_of<T>(s, tb);
         if (!cuts && (seen & kAll) == kAll && tb > s.t0 && tb + kU <= s.t1 && tb + kU < s.len) step(tb, 0, std::true_type{});
         else step(tb, cuts, std::false_type{});
       }
+      cp_async_wait<0>();
     }
   }
+  __syncthreads();                             // the rings are done with
   // join the block's rows of sums
   const int cols = blockDim.x * V;
   float* mine = red + threadIdx.y * (W + 1) * cols + threadIdx.x * V;
@@ -473,7 +534,8 @@ template <typename T, int W, int V> int launch_conv(ConvArgs a, int rows, cudaSt
   int bx = 1;
   while (bx < 32 && bx < groups) bx *= 2;
   const dim3 grid(static_cast<unsigned>(surfk::ceil_div(groups, bx)), static_cast<unsigned>(rows));
-  conv_kernel<T, W, V><<<grid, dim3(bx, 256 / bx), 0, s>>>(a, a.B * a.chunks);
+  constexpr size_t smem = kU * kThreads * sizeof(typename Raw<T, V>::Word);
+  conv_kernel<T, W, V><<<grid, dim3(bx, kThreads / bx), smem, s>>>(a, a.B * a.chunks);
   SURF_RETURN_LAUNCH();
 }
 
@@ -482,9 +544,11 @@ int launch_grad(ConvArgs a, int rows, float* dw, float* dbias, cudaStream_t s) {
   const int groups = a.D / V;
   int bx = 1;
   while (bx < 32 && bx < groups) bx *= 2;
-  const int by = 256 / bx;
+  const int by = kThreads / bx;
   const dim3 grid(static_cast<unsigned>(surfk::ceil_div(groups, bx)), static_cast<unsigned>(rows));
-  const size_t smem = static_cast<size_t>(by) * (W + 1) * bx * V * sizeof(float);
+  constexpr size_t kRings = 2 * kU * kThreads * sizeof(typename Raw<T, V>::Word), kSums = kThreads * (W + 1) * V * sizeof(float);
+  constexpr size_t smem = kRings > kSums ? kRings : kSums;
+  if (const int rc = allow_smem<conv_grad_kernel<T, W, V>>(smem)) return rc;
   conv_grad_kernel<T, W, V><<<grid, dim3(bx, by), smem, s>>>(a, a.B * a.chunks);
   const int rc = static_cast<int>(cudaGetLastError());
   if (rc) return rc;
@@ -495,27 +559,33 @@ int launch_grad(ConvArgs a, int rows, float* dw, float* dbias, cudaStream_t s) {
 
 }  // namespace
 
-// vec: D is a multiple of 4 (gradient: of 2) and every row starts on a boundary of so many elements
-SURF_EXPORT int surf_seq_conv(const void* args, int dtype, int W, int vec, int rows, void* stream) {
+// bytes: what a thread's channels take in a row; a multiple of it are D, every base and every stride
+SURF_EXPORT int surf_seq_conv(const void* args, int dtype, int W, int bytes, int rows, void* stream) {
   const ConvArgs a = *static_cast<const ConvArgs*>(args);
   if (a.D <= 0 || rows <= 0 || rows > 65535) return static_cast<int>(cudaErrorInvalidValue);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_width(W, [&](auto w) {
     constexpr int kW = decltype(w)::value;
-    if (dtype == kBf16) return vec ? launch_conv<bf16, kW, kVFwd>(a, rows, s) : launch_conv<bf16, kW, 1>(a, rows, s);
-    return vec ? launch_conv<float, kW, kVFwd>(a, rows, s) : launch_conv<float, kW, 1>(a, rows, s);
+    if (dtype == kBf16) {
+      if (bytes == 16) return launch_conv<bf16, kW, 8>(a, rows, s);
+      return bytes == 4 ? launch_conv<bf16, kW, 2>(a, rows, s) : launch_conv<bf16, kW, 1>(a, rows, s);
+    }
+    return bytes == 16 ? launch_conv<float, kW, 4>(a, rows, s) : launch_conv<float, kW, 1>(a, rows, s);
   });
 }
 
-SURF_EXPORT int surf_seq_conv_grad(const void* args, int dtype, int W, int vec, int rows, float* dw, float* dbias,
+SURF_EXPORT int surf_seq_conv_grad(const void* args, int dtype, int W, int bytes, int rows, float* dw, float* dbias,
                                    void* stream) {
   const ConvArgs a = *static_cast<const ConvArgs*>(args);
   if (a.D <= 0 || rows <= 0 || rows > 65535) return static_cast<int>(cudaErrorInvalidValue);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_width(W, [&](auto w) {
     constexpr int kW = decltype(w)::value;
-    if (dtype == kBf16) return vec ? launch_grad<bf16, kW, kVGrad>(a, rows, dw, dbias, s) : launch_grad<bf16, kW, 1>(a, rows, dw, dbias, s);
-    return vec ? launch_grad<float, kW, kVGrad>(a, rows, dw, dbias, s) : launch_grad<float, kW, 1>(a, rows, dw, dbias, s);
+    if (dtype == kBf16) {
+      if (bytes == 8) return launch_grad<bf16, kW, 4>(a, rows, dw, dbias, s);
+      return bytes == 4 ? launch_grad<bf16, kW, 2>(a, rows, dw, dbias, s) : launch_grad<bf16, kW, 1>(a, rows, dw, dbias, s);
+    }
+    return bytes == 8 ? launch_grad<float, kW, 2>(a, rows, dw, dbias, s) : launch_grad<float, kW, 1>(a, rows, dw, dbias, s);
   });
 }
 
@@ -535,7 +605,7 @@ SURF_EXPORT int surf_seq_conv_step(const void* x, int64_t ldx, const float* w, c
           D, silu, err);
       SURF_RETURN_LAUNCH();
     };
-    if (dtype == kBf16) return vec ? go(bf16{}, std::integral_constant<int, kVFwd>{}) : go(bf16{}, std::integral_constant<int, 1>{});
-    return vec ? go(float{}, std::integral_constant<int, kVFwd>{}) : go(float{}, std::integral_constant<int, 1>{});
+    if (dtype == kBf16) return vec ? go(bf16{}, std::integral_constant<int, 4>{}) : go(bf16{}, std::integral_constant<int, 1>{});
+    return vec ? go(float{}, std::integral_constant<int, 4>{}) : go(float{}, std::integral_constant<int, 1>{});
   });
 }

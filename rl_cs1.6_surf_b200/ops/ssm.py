@@ -142,16 +142,16 @@ def _conv_check(what, x, weight, bias, state, reset, lengths):
     return code, 4 - 2 * code, at, b, t, d, w
 
 
-def _stretches(b: int, t: int, groups: int, per_sm: int):
-    """(tokens of a stretch, stretches of a row, rows of blocks) of the convolution: the
-    longest stretch (each reads width - 1 tokens of its neighbour again) that still gives
-    every SM 1024 threads, and ``per_sm`` blocks of 256 threads on an SM to take them."""
+def _stretches(b: int, t: int, groups: int):
+    """(tokens of a stretch, stretches of a row, rows of blocks) of the convolution for
+    ``groups`` threads across a row: the longest stretch (each reads width - 1 tokens of its
+    neighbour again) that still gives every SM 512 threads, two blocks on an SM to take them."""
     tt = 64
-    while tt > 8 and b * -(-t // tt) * groups < 148 * 1024:
+    while tt > 8 and b * -(-t // tt) * groups < 148 * 512:
         tt //= 2
     chunks = max(1, -(-t // tt))
     bx = min(32, 1 << (groups - 1).bit_length())
-    return tt, chunks, max(1, min(-(-b * chunks * bx // 256), -(-148 * per_sm // -(-groups // bx)), 65535))
+    return tt, chunks, max(1, min(-(-b * chunks * bx // 256), -(-296 // -(-groups // bx)), 65535))
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -169,12 +169,13 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     final = torch.empty((b, w - 1, d), dtype=x.dtype, device=x.device)
     if b == 0 or d == 0:
         return out, final
-    vec = (_bits(e, x, out, state) | d * e) % (4 * e) == 0
-    tt, chunks, rows = _stretches(b, t, d // 4 if vec else d, 4)
+    bits = _bits(e, x, out, state) | d * e
+    size = 16 if bits & 15 == 0 else 4 if bits & 3 == 0 else 2
+    tt, chunks, rows = _stretches(b, t, d * e // size)
     args = _CONV.pack(_p(x), 0, _p(state), 0, _p(weight), _p(bias), _p(reset), _p(lengths), out.data_ptr(),
                       final.data_ptr(), 0, x.stride(0), x.stride(1), 0, 0, out.stride(0), out.stride(1), t,
                       b, t, d, int(silu), tt, chunks)
-    launch(_lib.lib(SLIB).surf_seq_conv, "surf_seq_conv", at, args, code, w, int(vec), rows)
+    launch(_lib.lib(SLIB).surf_seq_conv, "surf_seq_conv", at, args, code, w, size, rows)
     return out, final
 
 
@@ -195,13 +196,14 @@ def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bi
         return ConvGrads(dx, torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dstate)
     dw = torch.empty((d, w), dtype=torch.float32, device=dev)
     db = torch.empty(d, dtype=torch.float32, device=dev) if bias is not None else None
-    vec = (_bits(e, x, dy, state, dfinal) | d * e) % (2 * e) == 0
-    tt, chunks, rows = _stretches(b, t, d // 2 if vec else d, 3)
+    bits = _bits(e, x, dy, state, dfinal) | d * e
+    size = 8 if bits & 7 == 0 else 4 if bits & 3 == 0 else 2
+    tt, chunks, rows = _stretches(b, t, d * e // size)
     part = torch.empty((rows, w + 1, d), dtype=torch.float32, device=dev)
     args = _CONV.pack(_p(x), dy.data_ptr(), _p(state), _p(dfinal), _p(weight), _p(bias), _p(reset), _p(lengths),
                       dx.data_ptr(), _p(dstate), part.data_ptr(), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1),
                       t * d, d, t, b, t, d, int(silu), tt, chunks)
-    launch(_lib.lib(SLIB).surf_seq_conv_grad, "surf_seq_conv_grad", at, args, code, w, int(vec), rows, _p(dw), _p(db))
+    launch(_lib.lib(SLIB).surf_seq_conv_grad, "surf_seq_conv_grad", at, args, code, w, size, rows, _p(dw), _p(db))
     return ConvGrads(dx, dw, db, dstate)
 
 
