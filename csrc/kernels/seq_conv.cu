@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2) conv_kernel(ConvArgs a, int items
     // `whole`: kU tokens are there and none of them starts an episode
     auto step = [&](int t, unsigned cuts, auto whole) {
       in.batch(t);
-#pragma unroll
+#pragma unroll (decltype(whole)::value || !Ring<T, V>::kAsync ? kU : 1)
       for (int u = 0; u < kU; ++u) {
         if (decltype(whole)::value || t + u < live) {
           cp_async_wait<kU - 1>();
@@ -355,12 +355,12 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
         gin.issue(u, s.t0 + u);
         cp_async_commit();
       }
-      // whole: kU tokens of the stretch's own, past its first W - 1, no reset in sight, the row goes on
+      // whole: kU tokens of the stretch's own, no reset in sight, the row goes on
       auto step = [&](int tb, unsigned cuts, auto whole) {
         constexpr bool kWhole = decltype(whole)::value;
         xin.batch(tb);
         gin.batch(tb);
-#pragma unroll
+#pragma unroll (kWhole || !Ring<T, V>::kAsync ? kU : 1)
         for (int u = 0; u < kU; ++u) {
           const int t = tb + u;
           if (kWhole || t < end) {
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
               }
             }
             const int done = t - (W - 1);
-            if (kWhole || (done >= s.t0 && done < s.t1)) store_pairs_of<T, V>(dx + done * a.y_t, pend[W - 1]);
+            if (done >= s.t0 && (kWhole || done < s.t1)) store_pairs_of<T, V>(dx + done * a.y_t, pend[W - 1]);
             else if (done < 0 && ds) store_pairs_of<T, V>(ds + static_cast<int64_t>(W - 1 + done) * a.D, pend[W - 1]);
 #pragma unroll
             for (int j = W - 1; j > 0; --j) pend[j] = pend[j - 1];
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
       };
       for (int tb = s.t0; tb < end; tb += kU) {
         const unsigned cuts = cuts_of<T>(s, tb);
-        if (!cuts && (seen & kAll) == kAll && tb > s.t0 && tb + kU <= s.t1 && tb + kU < s.len) step(tb, 0, std::true_type{});
+        if (!cuts && (seen & kAll) == kAll && tb + kU <= s.t1 && tb + kU < s.len) step(tb, 0, std::true_type{});
         else step(tb, cuts, std::false_type{});
       }
       cp_async_wait<0>();
@@ -480,11 +480,9 @@ __global__ void __launch_bounds__(256) conv_reduce_kernel(const float* part, int
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(128) conv_step_kernel(const T* x, int64_t ldx, const float* w, const float* bias, T* pool,
                                                         const uint8_t* reset, const int* slots, int n_slots, T* y, int64_t ldy,
-                                                        int rows, int D, int silu, int* err) {
-  const int groups = D / V;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (id >= static_cast<int64_t>(groups) * rows) return;
-  const int r = static_cast<int>(id / groups), d = static_cast<int>(id - static_cast<int64_t>(r) * groups) * V;
+                                                        int D, int silu, int* err) {
+  const int r = blockIdx.x, d = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+  if (d >= D) return;
   const int slot = slots ? slots[r] : r;
   float o[V];
 #pragma unroll
@@ -599,10 +597,10 @@ SURF_EXPORT int surf_seq_conv_step(const void* x, int64_t ldx, const float* w, c
     auto go = [&](auto t, auto v) {
       using T = decltype(t);
       constexpr int V = decltype(v)::value;
-      const int64_t n = static_cast<int64_t>(D / V) * rows;
-      conv_step_kernel<T, kW, V><<<static_cast<unsigned>(surfk::ceil_div(n, 128)), 128, 0, s>>>(
-          static_cast<const T*>(x), ldx, w, bias, static_cast<T*>(pool), reset, slots, n_slots, static_cast<T*>(y), ldy, rows,
-          D, silu, err);
+      const int threads = D / V < 128 ? (D / V + 31) / 32 * 32 : 128;
+      const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(surfk::ceil_div(D / V, threads)));
+      conv_step_kernel<T, kW, V><<<grid, threads, 0, s>>>(static_cast<const T*>(x), ldx, w, bias, static_cast<T*>(pool), reset,
+                                                          slots, n_slots, static_cast<T*>(y), ldy, D, silu, err);
       SURF_RETURN_LAUNCH();
     };
     if (dtype == kBf16) return vec ? go(bf16{}, std::integral_constant<int, 4>{}) : go(bf16{}, std::integral_constant<int, 1>{});

@@ -328,54 +328,81 @@ struct StepArgs {
   int rows, dim, N, G, softplus, n_slots;
 };
 
-template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel(StepArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int nl = lane & (LN - 1), n0 = nl * 4;
-  const int64_t id = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LN;
-  const bool in = id < static_cast<int64_t>(a.rows) * a.dim;
-  const int r = in ? static_cast<int>(id / a.dim) : 0;
-  const int d = in ? static_cast<int>(id - static_cast<int64_t>(r) * a.dim) : 0;
-  const int slot = a.slots ? a.slots[r] : r;
-  const bool bad = slot >= a.n_slots;
-  const bool on = in && slot >= 0 && !bad;
-  float acc[1] = {0.0f};
-  float x = 0.0f;
-  if (on) {
-    const int g = d / (a.dim / a.G);
-    x = to_f(static_cast<const T*>(a.x)[r * a.x_r + d]);
-    float dv = to_f(static_cast<const T*>(a.dt)[r * a.dt_r + d]) + (a.bias ? a.bias[d] : 0.0f);
-    if (a.softplus) dv = softplus(dv);
-    const float u = dv * x;
-    float* st = a.pool + (static_cast<int64_t>(slot) * a.dim + d) * a.N;
-    float4 h4 = a.reset && a.reset[r] ? make_float4(0.f, 0.f, 0.f, 0.f) : load_state4(st, n0, a.N);
-    const float4 A4 = load_state4(a.A + static_cast<int64_t>(d) * a.N, n0, a.N);
-    const T* B = static_cast<const T*>(a.B) + r * a.B_r + g * a.B_g;
-    const T* C = static_cast<const T*>(a.C) + r * a.C_r + g * a.C_g;
-    float h[4] = {h4.x, h4.y, h4.z, h4.w};
-    const float Av[4] = {A4.x, A4.y, A4.z, A4.w};
+// One pass over the states, 8 bytes a state to move: a thread keeps its A, D and bias for
+// kRows rows (4 where there are rows enough to fill the GPU all the same), whose states it
+// loads before it works on the first.
+template <typename T, int LN, int kRows> __global__ void __launch_bounds__(128) step_kernel(StepArgs a) {
+  const int n0 = (threadIdx.x & (LN - 1)) * 4;
+  const int d = (blockIdx.y * 128 + threadIdx.x) / LN;
+  const bool in = d < a.dim;
+  const int r0 = blockIdx.x * kRows;
+  const int g = in && a.G > 1 ? d / (a.dim / a.G) : 0;
+  float A2[4] = {0.f, 0.f, 0.f, 0.f}, skip = 0.0f, bias = 0.0f;
+  float4 h4[kRows];
+  int slot[kRows];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (n0 + i < a.N) {
-        h[i] = fmaf(exp2_hw(dv * (Av[i] * kLog2e)), h[i], u * to_f(B[n0 + i]));
-        acc[0] = fmaf(h[i], to_f(C[n0 + i]), acc[0]);
+  for (int j = 0; j < kRows; ++j) {
+    const int r = r0 + j;
+    slot[j] = in && r < a.rows ? (a.slots ? a.slots[r] : r) : -1;
+    h4[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (slot[j] >= 0 && slot[j] < a.n_slots && !(a.reset && a.reset[r]))
+      h4[j] = load_state4(a.pool + (static_cast<int64_t>(slot[j]) * a.dim + d) * a.N, n0, a.N);
+  }
+  if (in) {
+    const float4 v = load_state4(a.A + static_cast<int64_t>(d) * a.N, n0, a.N);
+    A2[0] = v.x * kLog2e; A2[1] = v.y * kLog2e; A2[2] = v.z * kLog2e; A2[3] = v.w * kLog2e;
+    if (a.D) skip = a.D[d];
+    if (a.bias) bias = a.bias[d];
+  }
+#pragma unroll
+  for (int j = 0; j < kRows; ++j) {
+    const int r = r0 + j;
+    if (r >= a.rows) break;                              // the same for the whole block
+    const bool on = slot[j] >= 0 && slot[j] < a.n_slots;
+    float acc = 0.0f, x = 0.0f;
+    if (on) {
+      x = to_f(static_cast<const T*>(a.x)[r * a.x_r + d]);
+      float dv = to_f(static_cast<const T*>(a.dt)[r * a.dt_r + d]) + bias;
+      if (a.softplus) dv = softplus(dv);
+      const float u = dv * x;
+      const T* B = static_cast<const T*>(a.B) + r * a.B_r + g * a.B_g + n0;
+      const T* C = static_cast<const T*>(a.C) + r * a.C_r + g * a.C_g + n0;
+      float h[4] = {h4[j].x, h4[j].y, h4[j].z, h4[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (n0 + i < a.N) {
+          h[i] = fmaf(exp2_hw(dv * A2[i]), h[i], u * to_f(B[i]));
+          acc = fmaf(h[i], to_f(C[i]), acc);
+        }
       }
+      store_state4(a.pool + (static_cast<int64_t>(slot[j]) * a.dim + d) * a.N, n0, a.N, h);
     }
-    store_state4(st, n0, a.N, h);
-  }
 #pragma unroll
-  for (int off = LN / 2; off >= 1; off /= 2) acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], off);
-  if (!in || nl != 0) return;
-  float o = 0.0f;
-  if (on) {
-    o = acc[0] + (a.D ? a.D[d] * x : 0.0f);
-    if (a.z) {
-      const float z = to_f(static_cast<const T*>(a.z)[r * a.z_r + d]);
-      o *= z * sigmoid(z);
+    for (int off = LN / 2; off >= 1; off /= 2) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (in && n0 == 0) {
+      float o = 0.0f;
+      if (on) {
+        o = fmaf(skip, x, acc);
+        if (a.z) {
+          const float z = to_f(static_cast<const T*>(a.z)[r * a.z_r + d]);
+          o *= z * sigmoid(z);
+        }
+      } else if (slot[j] >= a.n_slots) {
+        surfk::report_error(a.err, surfk::kErrSlotIndex);
+      }
+      static_cast<T*>(a.out)[r * a.out_r + d] = from_f<T>(o);
     }
-  } else if (bad) {
-    surfk::report_error(a.err, surfk::kErrSlotIndex);
   }
-  static_cast<T*>(a.out)[r * a.out_r + d] = from_f<T>(o);
+}
+
+template <typename T, int LN> int launch_step(const StepArgs& a, cudaStream_t s) {
+  const unsigned across = static_cast<unsigned>(surfk::ceil_div(static_cast<int64_t>(a.dim) * LN, 128));
+  if (across > 65535) return static_cast<int>(cudaErrorInvalidValue);
+  if (static_cast<int64_t>(across) * a.rows >= 4 * 148 * 12)
+    step_kernel<T, LN, 4><<<dim3(static_cast<unsigned>(surfk::ceil_div(a.rows, 4)), across), 128, 0, s>>>(a);
+  else
+    step_kernel<T, LN, 1><<<dim3(static_cast<unsigned>(a.rows), across), 128, 0, s>>>(a);
+  SURF_RETURN_LAUNCH();
 }
 
 }  // namespace
@@ -396,11 +423,7 @@ SURF_EXPORT int surf_seq_scan_step(const void* args, int dtype, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_lanes(a.N, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
-    const int64_t blocks = surfk::ceil_div(static_cast<int64_t>(a.rows) * a.dim * LN, 128);
-    if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
-    if (dtype == kBf16) step_kernel<bf16, LN><<<static_cast<unsigned>(blocks), 128, 0, s>>>(a);
-    else step_kernel<float, LN><<<static_cast<unsigned>(blocks), 128, 0, s>>>(a);
-    SURF_RETURN_LAUNCH();
+    return dtype == kBf16 ? launch_step<bf16, LN>(a, s) : launch_step<float, LN>(a, s);
   });
 }
 
