@@ -54,7 +54,7 @@ ScanGrads = namedtuple("ScanGrads", "dx ddt dz dB dC dA dD ddt_bias dstate")
 
 _CONV = struct.Struct("18q6i")
 _SCAN = struct.Struct("48q10i")
-_STEP = struct.Struct("21q6i")
+_STEP = struct.Struct("21q8i")
 
 
 def _p(t) -> int:
@@ -425,7 +425,8 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     args = _STEP.pack(x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias),
                       state.data_ptr(), _p(reset), _p(slots), out.data_ptr(), error_flag(dev).data_ptr(), x.stride(0),
                       dt.stride(0), 0 if z is None else z.stride(0), B.stride(0), B.stride(1), C.stride(0), C.stride(1),
-                      out.stride(0), r, d, n, g, int(softplus), state.shape[0])
+                      out.stride(0), r, d, n, g, int(softplus), state.shape[0],
+                      (_bits(e, B, C) | n * e) % (4 * e) == 0, 0)
     launch(_lib.lib(SLIB).surf_seq_scan_step, "surf_seq_scan_step", at, args, code)
     return out
 
