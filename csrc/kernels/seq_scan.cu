@@ -363,15 +363,12 @@ template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel
   }
   float* pool = a.pool + static_cast<int64_t>(slot) * a.dim * a.N;
   const bool cut = a.reset && a.reset[r];
-  float4 h4[K], A4[K];
+  float4 h4[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int d = base + k * kRowsOfWarp;
-    h4[k] = A4[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (d < a.dim) {
-      if (!cut) h4[k] = load_state4(pool + static_cast<int64_t>(d) * a.N, n0, a.N);
-      A4[k] = load_state4(a.A + static_cast<int64_t>(d) * a.N, n0, a.N);
-    }
+    h4[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d < a.dim && !cut) h4[k] = load_state4(pool + static_cast<int64_t>(d) * a.N, n0, a.N);
   }
   alignas(16) Quad<T> B, C;
   const T* rowB = static_cast<const T*>(a.B) + r * a.B_r + n0;
@@ -398,7 +395,8 @@ template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel
         B.load(rowB + g * a.B_g, a.N - n0, a.whole);
         C.load(rowC + g * a.C_g, a.N - n0, a.whole);
       }
-      const float Av[4] = {A4[k].x, A4[k].y, A4[k].z, A4[k].w};
+      const float4 A4 = load_state4(a.A + static_cast<int64_t>(d) * a.N, n0, a.N);
+      const float Av[4] = {A4.x, A4.y, A4.z, A4.w};
       float h[4] = {h4[k].x, h4[k].y, h4[k].z, h4[k].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {                      // states past the N-th stay zero: A, B and h are there
