@@ -25,46 +25,60 @@ using namespace seqk;
 
 template <typename T, int LN> struct GradLayout {
   static constexpr int NT = LN < 4 ? 128 : 256;
-  static constexpr int CH = NT / LN * 2;                  // two channels a thread, one f32x2 pair
+  static constexpr int CH = NT / LN * 2;                  // two channels a thread, 4 states of each in two f32x2 pairs
   static constexpr int NP = 4 * LN;
   static constexpr int R = kSave;                         // tokens of a tile
   struct Smem {
     alignas(16) T x[2][R * CH], dt[2][R * CH], z[2][R * CH], dout[2][R * CH], B[2][R * NP], C[2][R * NP];
     alignas(16) float delta[R * CH], u[R * CH], g[R * CH], y[R * CH], ub[R * CH], qa[R * CH];
     alignas(16) float dgate[R * CH], dstep[R * CH];       // dout silu'(z), d delta / d dt
-    alignas(16) float Bd[R * NP * 2], Cd[R * NP * 2];     // 32-bit, every value twice
+    alignas(16) float Bf[R * 4 * NP], Cf[R * 4 * NP];     // 32-bit, in the four orders of the lanes
     alignas(16) float red[NT / 32][R][2 * NP];            // the warps' sums of dB and dC
     alignas(16) float bias[CH], skip[CH];
   };
 };
 
-// Sums v[0..8) over the 32 / LN channel rows of a warp, halving what a lane carries with
-// every exchange. Returns how many sums the lane holds (in v[0..)), the first of them
-// being value `first`; lanes with `writer` false hold copies.
-template <int LN> __device__ __forceinline__ void reduce_rows(float (&v)[8], int lane, int& first, bool& writer) {
-  int k = 8;
-  first = 0;
-  writer = true;
+// The order of a lane's 4 states. Sums over the 32 / LN channel rows of a warp halve what a
+// lane carries with every exchange; so that no lane has to choose which half it gives, lanes
+// hold their states in different orders: slot s is state s ^ order_of(lane).
+template <int LN> __device__ __forceinline__ int order_of(int lane) {
+  return (LN <= 16 && (lane & LN) ? 2 : 0) | (LN <= 8 && (lane & (2 * LN)) ? 1 : 0);
+}
+__device__ __forceinline__ float4 in_order(float4 v, int order) {
+  if (order & 2) v = make_float4(v.z, v.w, v.x, v.y);
+  if (order & 1) v = make_float4(v.y, v.x, v.w, v.z);
+  return v;
+}
+
+// dB and dC of one token: b and c summed over the warp's channel rows into red[0, NP) and
+// red[NP, 2 NP).
+template <int LN> __device__ __forceinline__ void reduce_rows(float (&b)[4], float (&c)[4], int lane, int n, float* red) {
+  constexpr int NP = 4 * LN;
+  constexpr unsigned kFull = 0xffffffffu;
+  b[0] += __shfl_xor_sync(kFull, b[2], LN);
+  b[1] += __shfl_xor_sync(kFull, b[3], LN);
+  c[0] += __shfl_xor_sync(kFull, c[2], LN);
+  c[1] += __shfl_xor_sync(kFull, c[3], LN);
+  if constexpr (LN <= 8) {
+    b[0] += __shfl_xor_sync(kFull, b[1], 2 * LN);
+    c[0] += __shfl_xor_sync(kFull, c[1], 2 * LN);
+  } else {
+    red[n ^ 1] = b[1];
+    red[NP + (n ^ 1)] = c[1];
+  }
+  if constexpr (LN <= 4) {
+    const bool up = lane & (4 * LN);
+    float keep = up ? c[0] : b[0];
+    keep += __shfl_xor_sync(kFull, up ? b[0] : c[0], 4 * LN);
 #pragma unroll
-  for (int off = 16; off >= LN; off /= 2) {
-    const bool up = lane & off;
-    if (k > 1) {
-      k /= 2;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i < k) {
-          const float give = up ? v[i] : v[i + k];
-          const float keep = up ? v[i + k] : v[i];
-          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
-        }
-      }
-      if (up) first += k;
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
-      if (up) writer = false;
-    }
+    for (int off = 8 * LN; off <= 16; off *= 2) keep += __shfl_xor_sync(kFull, keep, off);
+    if (LN == 4 || lane < 8 * LN) red[(up ? NP : 0) + n] = keep;
+  } else {
+    red[n] = b[0];
+    red[NP + n] = c[0];
   }
 }
+
 // The backward sweep's decays, made again: as an ordinary expression the compiler would
 // keep the forward run's (8 values for each of the tile's tokens) and spill.
 __device__ __forceinline__ f2 exp2_again(f2 x) {
@@ -75,11 +89,16 @@ __device__ __forceinline__ f2 exp2_again(f2 x) {
   return pack2(lo, hi);
 }
 
-template <int LN> constexpr int kRowSums = LN <= 4 ? 1 : (LN == 8 ? 2 : 4);
+__device__ __forceinline__ float sum_of(f2 v) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  return lo + hi;
+}
 
-// Per state and token the two sweeps cost 13 multiply-adds and two exponentials, the
-// sums across lanes about 6 instructions more: the issue rate and the exponential unit
-// (16 a cycle and SM) bound it alike.
+// Per state and token the two sweeps cost 13 multiply-adds (in pairs of states) and two
+// exponentials, the sums across lanes 13 exchanges for 8 states: shared memory's 128 bytes
+// a cycle (exchanges and loads, about 40 of its cycles for 256 states), the exponential unit
+// (32 cycles) and the issue rate bound it alike.
 template <typename T, int LN, bool kCarry>
 __global__ void __launch_bounds__(GradLayout<T, LN>::NT, (kCarry ? 768 : 512) / GradLayout<T, LN>::NT)
 scan_grad_kernel(ScanArgs a, int blocks_per_group) {
@@ -104,32 +123,35 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
   const int ch = threadIdx.x / LN * 2;
   const int n0 = nl * 4;
 
+  const int order = order_of<LN>(lane);
   // 4 states of the two channels, from memory into pairs and back
-  auto load_h = [&](const float* src, f2 (&v)[4], float scale) {
-    float4 q[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  auto load_h = [&](const float* src, f2 (&v)[2][2], float scale) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (src && ch + e < nch) q[e] = load_state4(src + static_cast<int64_t>(d0 + ch + e) * a.N, n0, a.N);
-    v[0] = pack2(q[0].x * scale, q[1].x * scale);
-    v[1] = pack2(q[0].y * scale, q[1].y * scale);
-    v[2] = pack2(q[0].z * scale, q[1].z * scale);
-    v[3] = pack2(q[0].w * scale, q[1].w * scale);
+    for (int k = 0; k < 2; ++k) {
+      float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (src && ch + k < nch) q = in_order(load_state4(src + static_cast<int64_t>(d0 + ch + k) * a.N, n0, a.N), order);
+      v[k][0] = pack2(q.x * scale, q.y * scale);
+      v[k][1] = pack2(q.z * scale, q.w * scale);
+    }
   };
-  auto store_h = [&](float* dst, const f2 (&v)[4]) {
-    float q[2][4];
+  auto store_h = [&](float* dst, const f2 (&v)[2][2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) unpack2(v[i], q[0][i], q[1][i]);
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (ch + e < nch) store_state4(dst + static_cast<int64_t>(d0 + ch + e) * a.N, n0, a.N, q[e]);
+    for (int k = 0; k < 2; ++k) {
+      float4 q;
+      unpack2(v[k][0], q.x, q.y);
+      unpack2(v[k][1], q.z, q.w);
+      q = in_order(q, order);
+      const float f[4] = {q.x, q.y, q.z, q.w};
+      if (ch + k < nch) store_state4(dst + static_cast<int64_t>(d0 + ch + k) * a.N, n0, a.N, f);
+    }
   };
   const int64_t per_row = static_cast<int64_t>(a.dim) * a.N;
 
-  f2 A2[4], dh[4], dA[4], sumd = pack2(0.0f, 0.0f);
+  f2 A2[2][2], dh[2][2], dA[2][2];
+  float sumd[2] = {0.0f, 0.0f};
   load_h(a.A, A2, kLog2e);
   load_h(kCarry ? nullptr : a.chunks > 1 ? a.carry + bchunk * per_row : a.dfinal ? a.dfinal + b * per_row : nullptr, dh, 1.0f);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) dA[i] = pack2(0.0f, 0.0f);
+  dA[0][0].v = dA[0][1].v = dA[1][0].v = dA[1][1].v = 0;
 
   const T* gx = static_cast<const T*>(a.x) + b * a.x_b + d0;
   const T* gdt = static_cast<const T*>(a.dt) + b * a.dt_b + d0;
@@ -172,7 +194,7 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
   const int last = t_live > t_lo ? t_lo + (t_live - 1 - t_lo) / R * R : t_lo - R;
   int buf = 1;
   for (int t0 = last + R; t0 >= t_lo; t0 -= R, buf ^= 1) {
-    f2 h[R + 1][4];                                        // h[r]: the state before token r, h[R] behind the last
+    f2 h[R + 1][2][2];                                     // h[r]: the state before token r, h[R] behind the last
     if (!kCarry && t0 <= last) load_h(saved + t0 / kSave * per_row, h[0], 1.0f);
     cp_async_wait<0>();
     __syncthreads();
@@ -222,32 +244,39 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
     for (int i = threadIdx.x; i < R * NP; i += NT) {
       const int r = i / NP, n = i % NP;
       const bool in = r < rows && n < a.N;
-      const float Cv = in ? to_f(sm.C[buf][i]) : 0.0f;
-      *reinterpret_cast<float2*>(sm.Cd + 2 * i) = make_float2(Cv, Cv);
-      if (!kCarry) {
-        const float Bv = in ? to_f(sm.B[buf][i]) : 0.0f;
-        *reinterpret_cast<float2*>(sm.Bd + 2 * i) = make_float2(Bv, Bv);
+      const float Cv = in ? to_f(sm.C[buf][i]) : 0.0f, Bv = !kCarry && in ? to_f(sm.B[buf][i]) : 0.0f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        sm.Cf[(r * 4 + q) * NP + (n ^ q)] = Cv;
+        if (!kCarry) sm.Bf[(r * 4 + q) * NP + (n ^ q)] = Bv;
       }
     }
     __syncthreads();
-    auto pair_at = [&](const float* p) {
-      f2 v;
-      v.v = *reinterpret_cast<const unsigned long long*>(p);
-      return v;
+    const float* const Bl = sm.Bf + order * NP + n0;
+    const float* const Cl = sm.Cf + order * NP + n0;
+    auto twice = [](const float* p, f2 (&v)[2], float (&x)[2]) {       // the two channels' numbers
+      const float2 q = *reinterpret_cast<const float2*>(p);
+      x[0] = q.x;
+      x[1] = q.y;
+      v[0] = pack2(q.x, q.x);
+      v[1] = pack2(q.y, q.y);
     };
     if constexpr (kCarry) {
 #pragma unroll
       for (int r = R - 1; r >= 0; --r) {
-        f2 Ct[4];
-        load_pairs(sm.Cd + (r * NP + n0) * 2, Ct[0], Ct[1]);
-        load_pairs(sm.Cd + (r * NP + n0) * 2 + 4, Ct[2], Ct[3]);
-        const f2 dl = pair_at(sm.delta + r * CH + ch), gv = pair_at(sm.g + r * CH + ch);
-        sumd = add2(sumd, dl);
+        f2 Ct[2], dl[2], gv[2];
+        float dx[2], gx2[2];
+        load_pairs(Cl + r * 4 * NP, Ct[0], Ct[1]);
+        twice(sm.delta + r * CH + ch, dl, dx);
+        twice(sm.g + r * CH + ch, gv, gx2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dh[i] = mul2(fma2(gv, Ct[i], dh[i]), exp2_hw2(mul2(dl, A2[i])));
-        if (cuts >> r & 1u) {
+        for (int k = 0; k < 2; ++k) {
+          sumd[k] += dx[k];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) dh[i].v = 0;
+          for (int q = 0; q < 2; ++q) {
+            dh[k][q] = mul2(fma2(gv[k], Ct[q], dh[k][q]), exp2_hw2(mul2(dl[k], A2[k][q])));
+            if (cuts >> r & 1u) dh[k][q].v = 0;
+          }
         }
       }
     } else {
@@ -255,50 +284,50 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
         constexpr bool kCuts = decltype(with_cuts)::value;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          f2 Bt[4];
-          load_pairs(sm.Bd + (r * NP + n0) * 2, Bt[0], Bt[1]);
-          load_pairs(sm.Bd + (r * NP + n0) * 2 + 4, Bt[2], Bt[3]);
-          const f2 dl = pair_at(sm.delta + r * CH + ch), u = pair_at(sm.u + r * CH + ch);
+          f2 Bt[2], dl[2], u[2];
+          float x0[2], x1[2];
+          load_pairs(Bl + r * 4 * NP, Bt[0], Bt[1]);
+          twice(sm.delta + r * CH + ch, dl, x0);
+          twice(sm.u + r * CH + ch, u, x1);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f2 before = h[r][i];
-            if (kCuts && (cuts >> r & 1u)) before.v = 0;
-            h[r + 1][i] = fma2(exp2_hw2(mul2(dl, A2[i])), before, mul2(u, Bt[i]));
-          }
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              f2 before = h[r][k][q];
+              if (kCuts && (cuts >> r & 1u)) before.v = 0;
+              h[r + 1][k][q] = fma2(exp2_hw2(mul2(dl[k], A2[k][q])), before, mul2(u[k], Bt[q]));
+            }
         }
 #pragma unroll
         for (int r = R - 1; r >= 0; --r) {
-          f2 Bt[4], Ct[4];
-          load_pairs(sm.Bd + (r * NP + n0) * 2, Bt[0], Bt[1]);
-          load_pairs(sm.Bd + (r * NP + n0) * 2 + 4, Bt[2], Bt[3]);
-          load_pairs(sm.Cd + (r * NP + n0) * 2, Ct[0], Ct[1]);
-          load_pairs(sm.Cd + (r * NP + n0) * 2 + 4, Ct[2], Ct[3]);
-          const f2 dl = pair_at(sm.delta + r * CH + ch), u = pair_at(sm.u + r * CH + ch), gv = pair_at(sm.g + r * CH + ch);
-          float ul, uh, gl, gh, bc[8];
-          unpack2(u, ul, uh);
-          unpack2(gv, gl, gh);
-          f2 y, ub, qa;
+          f2 Bt[2], Ct[2], dl[2], u[2], gv[2], dB[2], dC[2];
+          float x0[2], x1[2], x2[2], s3[3][2];
+          load_pairs(Bl + r * 4 * NP, Bt[0], Bt[1]);
+          load_pairs(Cl + r * 4 * NP, Ct[0], Ct[1]);
+          twice(sm.delta + r * CH + ch, dl, x0);
+          twice(sm.u + r * CH + ch, u, x1);
+          twice(sm.g + r * CH + ch, gv, x2);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f2 v = fma2(gv, Ct[i], dh[i]);
-            float lo, hi;
-            unpack2(v, lo, hi);
-            bc[i] = fmaf(hi, uh, lo * ul);
-            unpack2(h[r + 1][i], lo, hi);
-            bc[4 + i] = fmaf(hi, gh, lo * gl);
-            y = i == 0 ? mul2(h[r + 1][i], Ct[i]) : fma2(h[r + 1][i], Ct[i], y);
-            ub = i == 0 ? mul2(v, Bt[i]) : fma2(v, Bt[i], ub);
-            f2 va = mul2(v, exp2_again(mul2(dl, A2[i])));
-            f2 q = mul2(va, h[r][i]);
-            if (kCuts && (cuts >> r & 1u)) va.v = q.v = 0;
-            qa = i == 0 ? mul2(q, A2[i]) : fma2(q, A2[i], qa);
-            dA[i] = fma2(q, dl, dA[i]);
-            dh[i] = va;
+          for (int k = 0; k < 2; ++k) {
+            f2 y, ub, qa;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const f2 v = fma2(gv[k], Ct[q], dh[k][q]), now = h[r + 1][k][q];
+              dB[q] = k == 0 ? mul2(v, u[k]) : fma2(v, u[k], dB[q]);
+              dC[q] = k == 0 ? mul2(now, gv[k]) : fma2(now, gv[k], dC[q]);
+              y = q == 0 ? mul2(now, Ct[q]) : fma2(now, Ct[q], y);
+              ub = q == 0 ? mul2(v, Bt[q]) : fma2(v, Bt[q], ub);
+              f2 va = mul2(v, exp2_again(mul2(dl[k], A2[k][q])));
+              f2 w = mul2(va, h[r][k][q]);
+              if (kCuts && (cuts >> r & 1u)) va.v = w.v = 0;
+              qa = q == 0 ? mul2(w, A2[k][q]) : fma2(w, A2[k][q], qa);
+              dA[k][q] = fma2(w, dl[k], dA[k][q]);
+              dh[k][q] = va;
+            }
+            s3[0][k] = sum_of(y);
+            s3[1][k] = sum_of(ub);
+            s3[2][k] = sum_of(qa);
           }
-          float s3[3][2];
-          unpack2(y, s3[0][0], s3[0][1]);
-          unpack2(ub, s3[1][0], s3[1][1]);
-          unpack2(qa, s3[2][0], s3[2][1]);
 #pragma unroll
           for (int e = 0; e < 3; ++e) reduce_lanes<LN, 2>(s3[e], lane);
           if (reduced_writer<LN, 2>(lane)) {
@@ -310,16 +339,12 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
               sm.qa[at + e] = s3[2][e];
             }
           }
-          int first;
-          bool writer;
-          reduce_rows<LN>(bc, lane, first, writer);
-          if (writer) {
-#pragma unroll
-            for (int i = 0; i < kRowSums<LN>; ++i) {
-              const int q = first + i;
-              sm.red[warp][r][(q < 4 ? 0 : NP) + n0 + (q & 3)] = bc[i];
-            }
-          }
+          float b4[4], c4[4];
+          unpack2(dB[0], b4[0], b4[1]);
+          unpack2(dB[1], b4[2], b4[3]);
+          unpack2(dC[0], c4[0], c4[1]);
+          unpack2(dC[1], c4[2], c4[3]);
+          reduce_rows<LN>(b4, c4, lane, n0 + order, sm.red[warp][r]);
         }
       };
       if (cuts) sweeps(std::true_type{});
@@ -376,11 +401,9 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
   cp_async_wait<0>();
   if constexpr (kCarry) {
     store_h(a.carry + bchunk * per_row, dh);
-    float v[2];
-    unpack2(sumd, v[0], v[1]);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (nl == 0 && ch + e < nch) a.sumd[bchunk * a.dim + d0 + ch + e] = v[e];
+      if (nl == 0 && ch + e < nch) a.sumd[bchunk * a.dim + d0 + ch + e] = sumd[e];
     if (threadIdx.x == 0) a.cut[bchunk] = any_cut;               // the same from every block
   } else {
     for (int t = max(t_lo, t_live); t < t_hi; ++t) {             // tokens that are not there
