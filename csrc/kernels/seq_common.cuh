@@ -96,6 +96,23 @@ __device__ __forceinline__ void copy_rows(T* dst, const T* src, int64_t stride, 
   }
 }
 
+// One thread's share of a tile's rows of channels in 16-byte pieces: piece column `c`, rows
+// r0, r0 + kStep, ... of R. The pointer moves with the tiles, so a tile costs no index
+// arithmetic.
+template <typename T, int NT, int CH, int R> struct RowPieces {
+  static constexpr int kPer = CH / kVec16<T>, kStep = NT / kPer;         // pieces of a row, rows between two of a thread's
+  static constexpr int kCount = (R + kStep - 1) / kStep;
+  static __device__ __forceinline__ int column() { return static_cast<int>(threadIdx.x) % kPer * kVec16<T>; }
+  static __device__ __forceinline__ int row() { return static_cast<int>(threadIdx.x) / kPer; }
+  // dst: the tile; src: this thread's first piece; rows: how many are there
+  static __device__ __forceinline__ void copy(T* dst, const T* src, int64_t stride, int rows) {
+    T* d = dst + row() * CH + column();
+#pragma unroll
+    for (int k = 0; k < kCount; ++k)
+      if (row() + k * kStep < rows) cp_async16(d + k * kStep * CH, src + k * kStep * stride);
+  }
+};
+
 // ---- launches -----------------------------------------------------------------------
 // Raises the kernel's dynamic shared-memory limit (and, if wide, its cluster limit to 16
 // blocks) once per device.

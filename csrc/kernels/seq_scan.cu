@@ -111,15 +111,35 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
   float* saved = a.saved ? a.saved + (static_cast<int64_t>(b) * ((a.T + kSave - 1) / kSave) * a.dim + d0 + ch) * a.N : nullptr;
 
+  // rows of channels in 16-byte pieces: this thread's first piece of the next tile
+  using Pieces = RowPieces<T, kThreads, CH, kTile>;
+  const bool pieces = a.mode_d == kPieces16, mine = Pieces::column() < nch;
+  const T *px = gx + (t_lo + Pieces::row()) * a.x_t + Pieces::column(), *pdt = gdt + (t_lo + Pieces::row()) * a.dt_t + Pieces::column();
+  const T* pz = gz ? gz + (t_lo + Pieces::row()) * a.z_t + Pieces::column() : nullptr;
   auto fetch = [&](int t, int buf) {
     const int rows = min(kTile, t_live - t);
     if (rows > 0) {
-      copy_rows<T, kThreads, CH>(sm.x[buf], gx + t * a.x_t, a.x_t, rows, nch, a.mode_d);
-      copy_rows<T, kThreads, CH>(sm.dt[buf], gdt + t * a.dt_t, a.dt_t, rows, nch, a.mode_d);
-      copy_rows<T, kThreads, NP>(sm.B[buf], gB + t * a.B_t, a.B_t, rows, a.N, a.mode_n);
-      if (!kCarry) {
-        copy_rows<T, kThreads, NP>(sm.C[buf], gC + t * a.C_t, a.C_t, rows, a.N, a.mode_n);
-        if (gz) copy_rows<T, kThreads, CH>(sm.z[buf], gz + t * a.z_t, a.z_t, rows, nch, a.mode_d);
+      if (pieces) {
+        if (mine) {
+          Pieces::copy(sm.x[buf], px, a.x_t, rows);
+          Pieces::copy(sm.dt[buf], pdt, a.dt_t, rows);
+          if (!kCarry && gz) Pieces::copy(sm.z[buf], pz, a.z_t, rows);
+        }
+        px += kTile * a.x_t;
+        pdt += kTile * a.dt_t;
+        if (!kCarry && gz) pz += kTile * a.z_t;
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < (kCarry || !gz ? 2 : 3); ++i) {
+          const int64_t stride = i == 0 ? a.x_t : i == 1 ? a.dt_t : a.z_t;
+          copy_rows<T, kThreads, CH>(i == 0 ? sm.x[buf] : i == 1 ? sm.dt[buf] : sm.z[buf], (i == 0 ? gx : i == 1 ? gdt : gz) + t * stride, stride,
+                                     rows, nch, a.mode_d);
+        }
+      }
+#pragma unroll 1
+      for (int i = 0; i < (kCarry ? 1 : 2); ++i) {
+        const int64_t stride = i == 0 ? a.B_t : a.C_t;
+        copy_rows<T, kThreads, NP>(i == 0 ? sm.B[buf] : sm.C[buf], (i == 0 ? gB : gC) + t * stride, stride, rows, a.N, a.mode_n);
       }
     }
     cp_async_commit();

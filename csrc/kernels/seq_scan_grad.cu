@@ -35,6 +35,7 @@ template <typename T, int LN> struct GradLayout {
     alignas(16) float Bf[R * 4 * NP], Cf[R * 4 * NP];     // 32-bit, in the four orders of the lanes
     alignas(16) float red[NT / 32][R][2 * NP];            // the warps' sums of dB and dC
     alignas(16) float bias[CH], skip[CH];
+    alignas(16) float hs[2][CH * NP];                     // the states kept before a tile, as in memory
   };
 };
 
@@ -44,6 +45,8 @@ template <typename T, int LN> struct GradLayout {
 template <int LN> __device__ __forceinline__ int order_of(int lane) {
   return (LN <= 16 && (lane & LN) ? 2 : 0) | (LN <= 8 && (lane & (2 * LN)) ? 1 : 0);
 }
+// where B and C lie in that order: neighbouring channel rows read neighbouring copies
+__device__ __forceinline__ int copy_of(int order) { return (order >> 1) | (order & 1) << 1; }
 __device__ __forceinline__ float4 in_order(float4 v, int order) {
   if (order & 2) v = make_float4(v.z, v.w, v.x, v.y);
   if (order & 1) v = make_float4(v.y, v.x, v.w, v.z);
@@ -166,17 +169,48 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
   const float* saved = kCarry ? nullptr : a.saved + static_cast<int64_t>(b) * ((a.T + kSave - 1) / kSave) * per_row;
 
+  // rows of channels in 16-byte pieces: this thread's first piece of the next tile
+  using Pieces = RowPieces<T, NT, CH, R>;
+  const int last = t_live > t_lo ? t_lo + (t_live - 1 - t_lo) / R * R : t_lo - R;
+  const bool pieces = a.mode_d == kPieces16, mine = Pieces::column() < nch;
+  const T *px = gx + (last + Pieces::row()) * a.x_t + Pieces::column(), *pdt = gdt + (last + Pieces::row()) * a.dt_t + Pieces::column();
+  const T* pdo = gdo + (last + Pieces::row()) * a.do_t + Pieces::column();
+  const T* pz = gz ? gz + (last + Pieces::row()) * a.z_t + Pieces::column() : nullptr;
   auto fetch = [&](int t, int buf) {
     const int rows = min(R, t_live - t);
     if (t >= t_lo && rows > 0) {
-      if (!kCarry) {
-        copy_rows<T, NT, CH>(sm.x[buf], gx + t * a.x_t, a.x_t, rows, nch, a.mode_d);
-        copy_rows<T, NT, NP>(sm.B[buf], gB + t * a.B_t, a.B_t, rows, a.N, a.mode_n);
+      if (pieces) {
+        if (mine) {
+          if (!kCarry) Pieces::copy(sm.x[buf], px, a.x_t, rows);
+          Pieces::copy(sm.dt[buf], pdt, a.dt_t, rows);
+          Pieces::copy(sm.dout[buf], pdo, a.do_t, rows);
+          if (gz) Pieces::copy(sm.z[buf], pz, a.z_t, rows);
+        }
+        px -= R * a.x_t;
+        pdt -= R * a.dt_t;
+        pdo -= R * a.do_t;
+        if (gz) pz -= R * a.z_t;
+      } else {
+#pragma unroll 1
+        for (int i = kCarry ? 1 : 0; i < (gz ? 4 : 3); ++i) {
+          const int64_t stride = i == 0 ? a.x_t : i == 1 ? a.dt_t : i == 2 ? a.do_t : a.z_t;
+          copy_rows<T, NT, CH>(i == 0 ? sm.x[buf] : i == 1 ? sm.dt[buf] : i == 2 ? sm.dout[buf] : sm.z[buf],
+                               (i == 0 ? gx : i == 1 ? gdt : i == 2 ? gdo : gz) + t * stride, stride, rows, nch, a.mode_d);
+        }
       }
-      copy_rows<T, NT, CH>(sm.dt[buf], gdt + t * a.dt_t, a.dt_t, rows, nch, a.mode_d);
-      copy_rows<T, NT, CH>(sm.dout[buf], gdo + t * a.do_t, a.do_t, rows, nch, a.mode_d);
-      copy_rows<T, NT, NP>(sm.C[buf], gC + t * a.C_t, a.C_t, rows, a.N, a.mode_n);
-      if (gz) copy_rows<T, NT, CH>(sm.z[buf], gz + t * a.z_t, a.z_t, rows, nch, a.mode_d);
+#pragma unroll 1
+      for (int i = kCarry ? 1 : 0; i < 2; ++i) {
+        const int64_t stride = i == 0 ? a.B_t : a.C_t;
+        copy_rows<T, NT, NP>(i == 0 ? sm.B[buf] : sm.C[buf], (i == 0 ? gB : gC) + t * stride, stride, rows, a.N, a.mode_n);
+      }
+      if (!kCarry) {
+        const float* src = saved + t / kSave * per_row + static_cast<int64_t>(d0) * a.N;
+        if ((a.N & 3) == 0) {
+          for (int i = threadIdx.x * 4; i < nch * a.N; i += NT * 4) cp_async16(sm.hs[buf] + i, src + i);
+        } else {
+          for (int i = threadIdx.x; i < nch * a.N; i += NT) cp_async4(sm.hs[buf] + i, src + i);
+        }
+      }
     }
     cp_async_commit();
   };
@@ -190,12 +224,17 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
     sm.skip[c] = a.D && c < nch ? a.D[d0 + c] : 0.0f;
   }
 
+  // dB and dC of the tile: a thread sums one state of every kBcStep-th token over the warps
+  constexpr int kBcStep = NT / (2 * NP) > 0 ? NT / (2 * NP) : 1;
+  static_assert(NT % (2 * NP) == 0, "a thread keeps its state");
+  const int bq = threadIdx.x % (2 * NP), br = threadIdx.x / (2 * NP), bn = bq % NP;
+  const int64_t bc_stride = static_cast<int64_t>(a.G) * 2 * a.N;
+  float* const pbc = kCarry ? nullptr : a.part_bc + ((static_cast<int64_t>(sub) * a.batch + b) * a.T * a.G + g) * (2 * a.N) + (bq < NP ? bn : a.N + bn);
+
   bool any_cut = false;
-  const int last = t_live > t_lo ? t_lo + (t_live - 1 - t_lo) / R * R : t_lo - R;
   int buf = 1;
   for (int t0 = last + R; t0 >= t_lo; t0 -= R, buf ^= 1) {
     f2 h[R + 1][2][2];                                     // h[r]: the state before token r, h[R] behind the last
-    if (!kCarry && t0 <= last) load_h(saved + t0 / kSave * per_row, h[0], 1.0f);
     cp_async_wait<0>();
     __syncthreads();
     fetch(t0 - R, buf ^ 1);
@@ -247,13 +286,13 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
       const float Cv = in ? to_f(sm.C[buf][i]) : 0.0f, Bv = !kCarry && in ? to_f(sm.B[buf][i]) : 0.0f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        sm.Cf[(r * 4 + q) * NP + (n ^ q)] = Cv;
-        if (!kCarry) sm.Bf[(r * 4 + q) * NP + (n ^ q)] = Bv;
+        sm.Cf[(r * 4 + copy_of(q)) * NP + (n ^ q)] = Cv;
+        if (!kCarry) sm.Bf[(r * 4 + copy_of(q)) * NP + (n ^ q)] = Bv;
       }
     }
     __syncthreads();
-    const float* const Bl = sm.Bf + order * NP + n0;
-    const float* const Cl = sm.Cf + order * NP + n0;
+    const float* const Bl = sm.Bf + copy_of(order) * NP + n0;
+    const float* const Cl = sm.Cf + copy_of(order) * NP + n0;
     auto twice = [](const float* p, f2 (&v)[2], float (&x)[2]) {       // the two channels' numbers
       const float2 q = *reinterpret_cast<const float2*>(p);
       x[0] = q.x;
@@ -280,6 +319,7 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
         }
       }
     } else {
+      load_h(sm.hs[buf] - static_cast<int64_t>(d0) * a.N, h[0], 1.0f);
       auto sweeps = [&](auto with_cuts) {
         constexpr bool kCuts = decltype(with_cuts)::value;
 #pragma unroll
@@ -388,13 +428,13 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
         store_quad<T>(gdx + o, dx, nch - ec, a.mode_d == kPieces16);
         store_quad<T>(gddt + o, ddt, nch - ec, a.mode_d == kPieces16);
       }
-      for (int i = threadIdx.x; i < rows * 2 * NP; i += NT) {
-        const int r = i / (2 * NP), q = i % (2 * NP), n = q % NP;
-        if (n >= a.N) continue;
-        float s = 0.0f;
+      if (bn < a.N) {
+        for (int r = br; r < rows; r += kBcStep) {
+          float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NT / 32; ++w) s += sm.red[w][r][q];
-        a.part_bc[(((static_cast<int64_t>(sub) * a.batch + b) * a.T + t0 + r) * a.G + g) * (2 * a.N) + (q < NP ? n : a.N + n)] = s;
+          for (int w = 0; w < NT / 32; ++w) s += sm.red[w][r][bq];
+          pbc[(t0 + r) * bc_stride] = s;
+        }
       }
     }
   }
