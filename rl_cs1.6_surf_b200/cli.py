@@ -28,6 +28,8 @@ Commands (reference tools they replace in brackets):
   tas-search        batched hill climb over one action window of a run
                     (tools/tas_search.py)
   tas-chain         window-by-window search of a whole run (tools/tas_chain.py)
+  recall            train the memory core on a recall task and let it answer
+                    (no counterpart in the reference)
 
 Train flags mirror the reference's (--envs, --n-steps, --epochs, --lr,
 --gamma, --reward, --int-coef, ...): every ``TrainConfig`` field is a flag.
@@ -317,6 +319,14 @@ def cmd_gpu_health(args) -> int:
     return health_main(args)
 
 
+def cmd_recall(args) -> int:
+    from .models.memory import MemoryConfig, train_recall
+    r = train_recall(args.iterations, args.envs, args.length, MemoryConfig(dim=args.dim), args.device, args.lr, args.seed,
+                     temperature=args.temperature, top_p=args.top_p, log=print)
+    print(json.dumps(r))
+    return 0
+
+
 def cmd_render_pov(args) -> int:
     from .utils.tools import render_pov
     n = render_pov(args.traj, args.map, args.out, width=args.width, height=args.height, cell=args.cell,
@@ -517,6 +527,16 @@ def build_parser() -> argparse.ArgumentParser:
         else:
             ts.add_argument("--max-windows", type=int, default=0, help="0 = the whole run")
             ts.add_argument("--from-drop", action="store_true", help="start at the opening drop")
+    rc = sub.add_parser("recall", help="memory core on a recall task: train, then sampled answers")
+    rc.add_argument("--iterations", type=int, default=400)
+    rc.add_argument("--envs", type=int, default=128)
+    rc.add_argument("--length", type=int, default=64, help="decisions of a training row")
+    rc.add_argument("--dim", type=int, default=256, help="channels of the core")
+    rc.add_argument("--lr", type=float, default=1e-2)
+    rc.add_argument("--temperature", type=float, default=0.5)
+    rc.add_argument("--top-p", type=float, default=0.9)
+    rc.add_argument("--seed", type=int, default=0)
+    rc.add_argument("--device", default="cuda")
     gh = sub.add_parser("gpu-health", help="HBM and bf16 GEMM health check")
     gh.add_argument("--seconds", type=float, default=2.0)
     gh.add_argument("--peaks", default=None)
@@ -530,7 +550,7 @@ def main(argv=None) -> int:
           "gpu-health": cmd_gpu_health, "render-pov": cmd_render_pov, "sample-traj": cmd_sample_traj,
           "compare-runs": cmd_compare_runs, "serve-metrics": cmd_serve_metrics, "bench-env": cmd_bench_env,
           "strafe-audit": cmd_strafe_audit, "route-bound": cmd_route_bound, "tas-search": cmd_tas_search,
-          "tas-chain": cmd_tas_chain}[args.cmd]
+          "tas-chain": cmd_tas_chain, "recall": cmd_recall}[args.cmd]
     return int(fn(args) or 0)
 
 
