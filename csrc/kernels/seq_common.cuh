@@ -113,6 +113,16 @@ template <typename T, int NT, int CH, int R> struct RowPieces {
   }
 };
 
+// The same for the two short rows of a token (B and C, NP elements each): one piece for each
+// of the first 2 R NP / V threads, B's first.
+template <typename T, int NT, int NP, int R> struct TwinPieces {
+  static constexpr int kPer = NP >= kVec16<T> ? NP / kVec16<T> : 1, kEach = R * kPer;
+  static constexpr bool kFits = NP % kVec16<T> == 0 && 2 * kEach <= NT;
+  static __device__ __forceinline__ int which() { return static_cast<int>(threadIdx.x) / kEach; }        // 0: B, 1: C
+  static __device__ __forceinline__ int row() { return static_cast<int>(threadIdx.x) % kEach / kPer; }
+  static __device__ __forceinline__ int column() { return static_cast<int>(threadIdx.x) % kPer * kVec16<T>; }
+};
+
 // ---- launches -----------------------------------------------------------------------
 // Raises the kernel's dynamic shared-memory limit (and, if wide, its cluster limit to 16
 // blocks) once per device.

@@ -41,7 +41,7 @@ template <typename T, int LN> struct Layout {
 // channels share an instruction (f32x2), which leaves the exponential unit's 16 a cycle
 // and SM as the bound.
 template <typename T, int LN, bool kCarry>
-__global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_per_group) {
+__global__ void __launch_bounds__(kThreads, 4) scan_kernel(ScanArgs a, int blocks_per_group) {
   using L = Layout<T, LN>;
   constexpr int K = L::K, P = K / 2, CH = L::CH, NP = L::NP;
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -116,6 +116,11 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
   const bool pieces = a.mode_d == kPieces16, mine = Pieces::column() < nch;
   const T *px = gx + (t_lo + Pieces::row()) * a.x_t + Pieces::column(), *pdt = gdt + (t_lo + Pieces::row()) * a.dt_t + Pieces::column();
   const T* pz = gz ? gz + (t_lo + Pieces::row()) * a.z_t + Pieces::column() : nullptr;
+  using Twin = TwinPieces<T, kThreads, NP, kTile>;
+  const bool twin = Twin::kFits && a.mode_n == kPieces16 && a.N == NP;
+  const bool my_twin = kCarry ? Twin::which() == 0 : Twin::which() < 2;
+  const int64_t twin_t = Twin::which() == 0 ? a.B_t : a.C_t;
+  const T* ptwin = (Twin::which() == 0 ? gB : gC) + (t_lo + Twin::row()) * twin_t + Twin::column();
   auto fetch = [&](int t, int buf) {
     const int rows = min(kTile, t_live - t);
     if (rows > 0) {
@@ -136,10 +141,16 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs a, int blocks_p
                                      rows, nch, a.mode_d);
         }
       }
+      if (twin) {
+        if (my_twin && Twin::row() < rows)
+          cp_async16((Twin::which() == 0 ? sm.B[buf] : sm.C[buf]) + Twin::row() * NP + Twin::column(), ptwin);
+        ptwin += kTile * twin_t;
+      } else {
 #pragma unroll 1
-      for (int i = 0; i < (kCarry ? 1 : 2); ++i) {
-        const int64_t stride = i == 0 ? a.B_t : a.C_t;
-        copy_rows<T, kThreads, NP>(i == 0 ? sm.B[buf] : sm.C[buf], (i == 0 ? gB : gC) + t * stride, stride, rows, a.N, a.mode_n);
+        for (int i = 0; i < (kCarry ? 1 : 2); ++i) {
+          const int64_t stride = i == 0 ? a.B_t : a.C_t;
+          copy_rows<T, kThreads, NP>(i == 0 ? sm.B[buf] : sm.C[buf], (i == 0 ? gB : gC) + t * stride, stride, rows, a.N, a.mode_n);
+        }
       }
     }
     cp_async_commit();

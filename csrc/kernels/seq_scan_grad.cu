@@ -176,6 +176,13 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
   const T *px = gx + (last + Pieces::row()) * a.x_t + Pieces::column(), *pdt = gdt + (last + Pieces::row()) * a.dt_t + Pieces::column();
   const T* pdo = gdo + (last + Pieces::row()) * a.do_t + Pieces::column();
   const T* pz = gz ? gz + (last + Pieces::row()) * a.z_t + Pieces::column() : nullptr;
+  const float* psaved = kCarry ? nullptr : saved + last / kSave * per_row + static_cast<int64_t>(d0) * a.N;
+  const bool all_states = nch == CH && a.N == NP;
+  using Twin = TwinPieces<T, NT, NP, R>;
+  const bool twin = Twin::kFits && a.mode_n == kPieces16 && a.N == NP;
+  const bool my_twin = kCarry ? Twin::which() == 1 : Twin::which() < 2;
+  const int64_t twin_t = Twin::which() == 0 ? a.B_t : a.C_t;
+  const T* ptwin = (Twin::which() == 0 ? gB : gC) + (last + Twin::row()) * twin_t + Twin::column();
   auto fetch = [&](int t, int buf) {
     const int rows = min(R, t_live - t);
     if (t >= t_lo && rows > 0) {
@@ -198,18 +205,28 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
                                (i == 0 ? gx : i == 1 ? gdt : i == 2 ? gdo : gz) + t * stride, stride, rows, nch, a.mode_d);
         }
       }
+      if (twin) {
+        if (my_twin && Twin::row() < rows)
+          cp_async16((Twin::which() == 0 ? sm.B[buf] : sm.C[buf]) + Twin::row() * NP + Twin::column(), ptwin);
+        ptwin -= R * twin_t;
+      } else {
 #pragma unroll 1
-      for (int i = kCarry ? 1 : 0; i < 2; ++i) {
-        const int64_t stride = i == 0 ? a.B_t : a.C_t;
-        copy_rows<T, NT, NP>(i == 0 ? sm.B[buf] : sm.C[buf], (i == 0 ? gB : gC) + t * stride, stride, rows, a.N, a.mode_n);
+        for (int i = kCarry ? 1 : 0; i < 2; ++i) {
+          const int64_t stride = i == 0 ? a.B_t : a.C_t;
+          copy_rows<T, NT, NP>(i == 0 ? sm.B[buf] : sm.C[buf], (i == 0 ? gB : gC) + t * stride, stride, rows, a.N, a.mode_n);
+        }
       }
       if (!kCarry) {
-        const float* src = saved + t / kSave * per_row + static_cast<int64_t>(d0) * a.N;
-        if ((a.N & 3) == 0) {
-          for (int i = threadIdx.x * 4; i < nch * a.N; i += NT * 4) cp_async16(sm.hs[buf] + i, src + i);
+        if (all_states) {
+          constexpr int kStates = CH * NP / (4 * NT);
+#pragma unroll
+          for (int k = 0; k < kStates; ++k) cp_async16(sm.hs[buf] + (threadIdx.x + k * NT) * 4, psaved + (threadIdx.x + k * NT) * 4);
+        } else if ((a.N & 3) == 0) {
+          for (int i = threadIdx.x * 4; i < nch * a.N; i += NT * 4) cp_async16(sm.hs[buf] + i, psaved + i);
         } else {
-          for (int i = threadIdx.x; i < nch * a.N; i += NT) cp_async4(sm.hs[buf] + i, src + i);
+          for (int i = threadIdx.x; i < nch * a.N; i += NT) cp_async4(sm.hs[buf] + i, psaved + i);
         }
+        psaved -= per_row;
       }
     }
     cp_async_commit();
