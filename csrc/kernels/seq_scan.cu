@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(ScanArgs a, int block
         if (kCarry) sumd[p] = add2(sumd[p], dl[p]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          h[p][i] = fma2(exp2_hw2(mul2(dl[p], A2[p][i])), h[p][i], mul2(u[p], Bt[i]));
+          h[p][i] = fma2(decay2(dl[p], A2[p][i]), h[p][i], mul2(u[p], Bt[i]));
           if (!kCarry) y[p] = i == 0 ? mul2(h[p][i], Ct[i]) : fma2(h[p][i], Ct[i], y[p]);
         }
       }
@@ -418,7 +418,7 @@ template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int d = base + k * kRowsOfWarp, from = row * LN + k * (LN / K);
-    const float dl = __shfl_sync(0xffffffffu, dv, from) * kLog2e, u = __shfl_sync(0xffffffffu, ux, from);
+    const float dl = __shfl_sync(0xffffffffu, dv, from), u = __shfl_sync(0xffffffffu, ux, from);
     acc[k] = 0.0f;
     if (d < a.dim) {
       if (a.G > 1) {
@@ -431,7 +431,7 @@ template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel
       float h[4] = {h4[k].x, h4[k].y, h4[k].z, h4[k].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {                      // states past the N-th stay zero: A, B and h are there
-        h[i] = fmaf(exp2_hw(dl * Av[i]), h[i], u * to_f(B.v[i]));
+        h[i] = fmaf(decay(dl, Av[i] * kLog2e), h[i], u * to_f(B.v[i]));
         acc[k] = fmaf(h[i], to_f(C.v[i]), acc[k]);
       }
       store_state4(pool + static_cast<int64_t>(d) * a.N, n0, a.N, h);

@@ -84,9 +84,9 @@ template <int LN> __device__ __forceinline__ void reduce_rows(float (&b)[4], flo
 
 // The backward sweep's decays, made again: as an ordinary expression the compiler would
 // keep the forward run's (8 values for each of the tile's tokens) and spill.
-__device__ __forceinline__ f2 exp2_again(f2 x) {
+__device__ __forceinline__ f2 decay2_again(f2 delta, f2 A2) {
   float lo, hi;
-  unpack2(x, lo, hi);
+  unpack2(decay_arg(delta, A2), lo, hi);
   asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(lo));
   asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(hi));
   return pack2(lo, hi);
@@ -330,7 +330,7 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
           sumd[k] += dx[k];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            dh[k][q] = mul2(fma2(gv[k], Ct[q], dh[k][q]), exp2_hw2(mul2(dl[k], A2[k][q])));
+            dh[k][q] = mul2(fma2(gv[k], Ct[q], dh[k][q]), decay2(dl[k], A2[k][q]));
             if (cuts >> r & 1u) dh[k][q].v = 0;
           }
         }
@@ -352,7 +352,7 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
             for (int q = 0; q < 2; ++q) {
               f2 before = h[r][k][q];
               if (kCuts && (cuts >> r & 1u)) before.v = 0;
-              h[r + 1][k][q] = fma2(exp2_hw2(mul2(dl[k], A2[k][q])), before, mul2(u[k], Bt[q]));
+              h[r + 1][k][q] = fma2(decay2(dl[k], A2[k][q]), before, mul2(u[k], Bt[q]));
             }
         }
 #pragma unroll
@@ -374,7 +374,7 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
               dC[q] = k == 0 ? mul2(now, gv[k]) : fma2(now, gv[k], dC[q]);
               y = q == 0 ? mul2(now, Ct[q]) : fma2(now, Ct[q], y);
               ub = q == 0 ? mul2(v, Bt[q]) : fma2(v, Bt[q], ub);
-              f2 va = mul2(v, exp2_again(mul2(dl[k], A2[k][q])));
+              f2 va = mul2(v, decay2_again(dl[k], A2[k][q]));
               f2 w = mul2(va, h[r][k][q]);
               if (kCuts && (cuts >> r & 1u)) va.v = w.v = 0;
               qa = q == 0 ? mul2(w, A2[k][q]) : fma2(w, A2[k][q], qa);
