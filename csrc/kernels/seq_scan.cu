@@ -295,35 +295,16 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(ScanArgs a, int block
   }
 }
 
-// carry[b, c] <- the state before chunk c. One thread per (b, d, n); kAhead chunks loaded at a time.
-__global__ void __launch_bounds__(256) carry_kernel(ScanArgs a) {
+// carry[b, c] <- the state before chunk c. One thread per (b, d, n).
+__global__ void __launch_bounds__(128) carry_kernel(ScanArgs a) {
   const int64_t per = static_cast<int64_t>(a.dim) * a.N;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (id >= per * a.batch) return;
   const int b = static_cast<int>(id / per);
-  const int64_t dn = id - b * per;
+  const int64_t dn = id - b * per, row = static_cast<int64_t>(b) * a.chunks;
   const int d = static_cast<int>(dn / a.N);
-  const float A2 = a.A[dn] * kLog2e;
-  float h = a.state ? a.state[id] : 0.0f;
-  float* carry = a.carry + static_cast<int64_t>(b) * a.chunks * per + dn;
-  const float* sumd = a.sumd + static_cast<int64_t>(b) * a.chunks * a.dim + d;
-  const uint8_t* cut = a.cut + static_cast<int64_t>(b) * a.chunks;
-  constexpr int kAhead = 8;
-  for (int c = 0; c < a.chunks; c += kAhead) {
-    float e[kAhead], p[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (c + j < a.chunks) {
-        e[j] = carry[(c + j) * per];
-        p[j] = cut[c + j] ? 0.0f : exp2_hw(A2 * sumd[static_cast<int64_t>(c + j) * a.dim]);
-      }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (c + j < a.chunks) {
-        carry[(c + j) * per] = h;
-        h = cut[c + j] ? e[j] : fmaf(p[j], h, e[j]);
-      }
-  }
+  string_chunks<false>(a.state ? a.state[id] : 0.0f, a.A[dn] * kLog2e, a.carry + row * per + dn, per, a.sumd + row * a.dim + d, a.dim,
+                       a.cut + row, a.chunks);
 }
 
 template <typename T, int LN> int launch_scan(const ScanArgs& a, cudaStream_t s) {
@@ -337,7 +318,7 @@ template <typename T, int LN> int launch_scan(const ScanArgs& a, cudaStream_t s)
     if (const int rc = allow_smem<scan_kernel<T, LN, true>>(smem)) return rc;
     scan_kernel<T, LN, true><<<grid, kThreads, smem, s>>>(a, bpg);
     const int64_t n = static_cast<int64_t>(a.batch) * a.dim * a.N;
-    carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(n, 256)), 256, 0, s>>>(a);
+    carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(n, 128)), 128, 0, s>>>(a);
   }
   if (const int rc = allow_smem<scan_kernel<T, LN, false>>(smem)) return rc;
   scan_kernel<T, LN, false><<<grid, kThreads, smem, s>>>(a, bpg);

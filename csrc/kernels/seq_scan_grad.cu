@@ -505,34 +505,15 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
 }
 
 // carry[b, c] <- the adjoint behind chunk c, dstate <- the one before the first token
-__global__ void __launch_bounds__(256) grad_carry_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(128) grad_carry_kernel(ScanArgs a) {
   const int64_t per = static_cast<int64_t>(a.dim) * a.N;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (id >= per * a.batch) return;
   const int b = static_cast<int>(id / per);
-  const int64_t dn = id - b * per;
+  const int64_t dn = id - b * per, row = static_cast<int64_t>(b) * a.chunks;
   const int d = static_cast<int>(dn / a.N);
-  const float A2 = a.A[dn] * kLog2e;
-  float dh = a.dfinal ? a.dfinal[id] : 0.0f;
-  float* carry = a.carry + static_cast<int64_t>(b) * a.chunks * per + dn;
-  const float* sumd = a.sumd + static_cast<int64_t>(b) * a.chunks * a.dim + d;
-  const uint8_t* cut = a.cut + static_cast<int64_t>(b) * a.chunks;
-  constexpr int kAhead = 8;
-  for (int c = a.chunks - 1; c >= 0; c -= kAhead) {
-    float e[kAhead], p[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (c - j >= 0) {
-        e[j] = carry[(c - j) * per];
-        p[j] = cut[c - j] ? 0.0f : exp2_hw(A2 * sumd[static_cast<int64_t>(c - j) * a.dim]);
-      }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (c - j >= 0) {
-        carry[(c - j) * per] = dh;
-        dh = cut[c - j] ? e[j] : fmaf(p[j], dh, e[j]);
-      }
-  }
+  const float dh = string_chunks<true>(a.dfinal ? a.dfinal[id] : 0.0f, a.A[dn] * kLog2e, a.carry + row * per + dn, per,
+                                       a.sumd + row * a.dim + d, a.dim, a.cut + row, a.chunks);
   if (a.dstate) a.dstate[id] = dh;
 }
 
@@ -583,7 +564,7 @@ template <typename T, int LN> int launch_grad(const ScanArgs& a, cudaStream_t s)
   if (a.chunks > 1) {
     if (const int rc = allow_smem<scan_grad_kernel<T, LN, true>>(smem)) return rc;
     scan_grad_kernel<T, LN, true><<<grid, L::NT, smem, s>>>(a, bpg);
-    grad_carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(static_cast<int64_t>(a.batch) * a.dim * a.N, 256)), 256, 0, s>>>(a);
+    grad_carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(static_cast<int64_t>(a.batch) * a.dim * a.N, 128)), 128, 0, s>>>(a);
   }
   if (const int rc = allow_smem<scan_grad_kernel<T, LN, false>>(smem)) return rc;
   scan_grad_kernel<T, LN, false><<<grid, L::NT, smem, s>>>(a, bpg);
