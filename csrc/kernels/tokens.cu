@@ -163,6 +163,7 @@ template <bool kStream> struct Large {
   static constexpr int kThreads = kStream ? 512 : 256, kWarps = kThreads / 32;
   static constexpr int kBinShift = kStream ? 16 : 18;          // 128 or 32 bins an octave of e, 40 octaves
   static constexpr int kBins = kStream ? 5136 : 1312;          // > 40 octaves, whole shares for 1 .. 16 blocks
+  static constexpr int kNoWeight = 40 * (1 << (23 - kBinShift)) + 1;   // the first bin of e < 2^-40 alone
 };
 constexpr int kAllKept = 1 << 30, kNoBin = -1;
 
@@ -182,23 +183,26 @@ template <int kBins, int kWarps> struct TokenSmem {
 };
 
 // w = floor(e * 2^40), e in [0, 1], as w1 * 2^23 + w0: the additions of 2^23 that round down
-// leave the whole part in the low bits of a float (what is left is exact in between).
+// leave the whole part in the low bits of a float (what is left is exact in between). Both
+// come with the bits of 2^23 on top (kTop), which sums take off at their end.
+constexpr uint32_t kTop = 0x4b000000u;
 __device__ __forceinline__ void split_weight(float e, uint32_t& w1, uint32_t& w0) {
   const float t = __fmaf_rd(e, 131072.0f, 8388608.0f);
   const float rest = __fmaf_rn(e, 131072.0f, -__fsub_rn(t, 8388608.0f));
-  w1 = __float_as_uint(t) - 0x4b000000u;
-  w0 = __float_as_uint(__fmaf_rd(rest, 8388608.0f, 8388608.0f)) - 0x4b000000u;
+  w1 = __float_as_uint(t);
+  w0 = __float_as_uint(__fmaf_rd(rest, 8388608.0f, 8388608.0f));
 }
 __device__ __forceinline__ u64 whole_weight(float e) {
   uint32_t w1, w0;
   split_weight(e, w1, w0);
-  return (static_cast<u64>(w1) << 23) + w0;
+  return (static_cast<u64>(w1 - kTop) << 23) + (w0 - kTop);
 }
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 template <typename T, int CS, bool kStream>
 __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream>::kThreads) large_kernel(TokenArgs a, int slice) {
   constexpr int kThreads = Large<kStream>::kThreads, kWarps = Large<kStream>::kWarps, kBins = Large<kStream>::kBins;
+  constexpr int kNoWeight = Large<kStream>::kNoWeight;
   using Smem = TokenSmem<kBins, kWarps>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
@@ -284,10 +288,9 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
   const int run = (slots + kWarps * 128 - 1) / (kWarps * 128) * 128;
   const int w_lo = min(slots, warp * run), w_hi = min(slots, w_lo + run);
   const bool limited = q.k || q.p < 1.0;
-  auto add = [&](int bin, uint32_t w1, uint32_t w0) {    // two 32-bit additions: shared memory has no 64-bit one
-    const uint32_t x = (w1 << 23) + w0;
-    const unsigned old = atomicAdd(&sm.hist_lo[bin], x);
-    const unsigned up = (w1 >> 9) + (old + x < old ? 1u : 0u);
+  auto add = [&](int bin, u64 w) {           // two 32-bit additions: shared memory has no 64-bit one
+    const unsigned x = static_cast<unsigned>(w), old = atomicAdd(&sm.hist_lo[bin], x);
+    const unsigned up = static_cast<unsigned>(w >> 32) + (old + x < old ? 1u : 0u);
     if (up) atomicAdd(&sm.hist_hi[bin], up);
     if (q.k) atomicAdd(&sm.hist_c[bin], 1u);
   };
@@ -296,6 +299,19 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
   auto exp_of = [&](float z) {
     const float e = expf(plain ? __fmul_rn(__fsub_rn(z, m), q.inv) : below(z, m, q.inv));
     return e >= q.min_p ? e : 0.0f;
+  };
+  auto exp_of_four = [&](float (&z)[4]) {
+    if (plain) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[j] = fmaxf(expf(__fmul_rn(__fsub_rn(z[j], m), q.inv)), 0.0f);      // NaN: 0
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[j] = fmaxf(expf(below(z[j], m, q.inv)), 0.0f);
+    }
+    if (q.min_p > 0.0f) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[j] = z[j] >= q.min_p ? z[j] : 0.0f;
+    }
   };
   // the e of candidates i .. i + 3 (slots; i a multiple of 4) and of one
   auto four = [&](int i, float (&e)[4]) {
@@ -306,8 +322,7 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] = i + j >= off && i + j < off + n ? to_f(row[i + j - off]) : -INFINITY;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = exp_of(e[j]);
+      exp_of_four(e);
     } else {
       const float4 v = *reinterpret_cast<const float4*>(zs + i);
       e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w;
@@ -320,39 +335,41 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
   // weights into the histogram, or summed; sums of a thread stay within 2^32 for 256 slots
   uint32_t s1 = 0, s0 = 0;
   u64 above = 0;
+  uint32_t added = 0;                        // candidates in s1 and s0
   auto flush = [&] {
-    above += (static_cast<u64>(s1) << 23) + s0;
-    s1 = s0 = 0;
+    above += (static_cast<u64>(s1 - added * kTop) << 23) + (s0 - added * kTop);
+    s1 = s0 = added = 0;
   };
+  const int no_bin = kNoWeight + lane;       // bins that nobody reads take what has no weight
 #pragma unroll 2
   for (int i = w_lo + lane * 4; i < w_hi; i += 128) {
     float e[4];
     four(i, e);
     if constexpr (!kStream) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = exp_of(e[j]);
+      exp_of_four(e);
       *reinterpret_cast<float4*>(zs + i) = make_float4(e[0], e[1], e[2], e[3]);
     }
     uint32_t w1[4], w0[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) split_weight(e[j], w1[j], w0[j]);
     if (limited) {
-      // four additions in flight; what has no weight goes to bins that nobody reads
+      // four additions in flight
       unsigned old[4];
       int bin[4];
+      uint32_t x[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        bin[j] = w1[j] | w0[j] ? bin_of_bits(__float_as_uint(e[j])) : kBins + lane;
-        old[j] = atomicAdd(&sm.hist_lo[bin[j]], (w1[j] << 23) + w0[j]);
+        bin[j] = min(bin_of_bits(__float_as_uint(e[j])), no_bin);
+        x[j] = (w1[j] << 23) + (w0[j] - kTop);             // the low word: kTop << 23 is gone
+        old[j] = atomicAdd(&sm.hist_lo[bin[j]], x[j]);
       }
       if (q.k) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) atomicAdd(&sm.hist_c[bin[j]], 1u);
+        for (int j = 0; j < 4; ++j) atomicAdd(&sm.hist_c[bin[j]], w1[j] != kTop || w0[j] != kTop ? 1u : 0u);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t x = (w1[j] << 23) + w0[j];
-        const unsigned up = (w1[j] >> 9) + (old[j] + x < old[j] ? 1u : 0u);
+        const unsigned up = ((w1[j] & 0x7fffffu) >> 9) + (old[j] + x[j] < old[j] ? 1u : 0u);
         if (up) atomicAdd(&sm.hist_hi[bin[j]], up);
       }
     } else {
@@ -361,6 +378,7 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
         s1 += w1[j];
         s0 += w0[j];
       }
+      added += 4;
       if (kStream && ((i - w_lo) & 8191) >= 8064) flush();
     }
   }
@@ -457,7 +475,10 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
       }
       if (level < 0) {
         // the sums of what is surely kept, and the candidates of the bin where the limit falls
+        // (bins by the e above which they lie: all bits of smaller bins are larger)
         edge = lim ? f.bin : kAllKept;
+        const float e_sure = lim ? __uint_as_float(0x3f800000u - (static_cast<uint32_t>(edge) << Large<kStream>::kBinShift)) : -1.0f;
+        const float e_edge = lim ? __uint_as_float(0x3f800000u - (static_cast<uint32_t>(edge + 1) << Large<kStream>::kBinShift)) : -1.0f;
         above = 0;
 #pragma unroll 2
         for (int i = w_lo + lane * 4; i < w_hi; i += 128) {
@@ -466,13 +487,14 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
           bool in_edge = false;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int bin = bin_of_bits(__float_as_uint(e[j]));
             uint32_t w1, w0;
             split_weight(e[j], w1, w0);
-            s1 += bin < edge ? w1 : 0u;
-            s0 += bin < edge ? w0 : 0u;
-            in_edge |= bin == edge;
+            const bool sure = e[j] > e_sure;
+            s1 += sure ? w1 : kTop;
+            s0 += sure ? w0 : kTop;
+            in_edge |= !sure && e[j] > e_edge;
           }
+          added += 4;
           if (in_edge) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -550,10 +572,8 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
         if (!intact) {
           clear();
           for (int i = threadIdx.x; i < slots; i += kThreads) {
-            uint32_t w1, w0;
             const float e = one(i);
-            split_weight(e, w1, w0);
-            if (w1 | w0) add(bin_of_bits(__float_as_uint(e)), w1, w0);
+            if (const u64 w = whole_weight(e)) add(bin_of_bits(__float_as_uint(e)), w);
           }
         }
       } else {
@@ -561,11 +581,10 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
         for (int i = threadIdx.x; i < slots; i += kThreads) {
           const float e = one(i);
           if (bin_of_bits(__float_as_uint(e)) != edge) continue;
-          uint32_t w1, w0;
-          split_weight(e, w1, w0);
-          if (!(w1 | w0)) continue;
+          const u64 w = whole_weight(e);
+          if (!w) continue;
           const uint32_t key = key_of(clean(to_f(row[i - off])));
-          if (level == 0 || key >> (32 - 8 * level) == prefix) add(255 - static_cast<int>(key >> (24 - 8 * level) & 255u), w1, w0);
+          if (level == 0 || key >> (32 - 8 * level) == prefix) add(255 - static_cast<int>(key >> (24 - 8 * level) & 255u), w);
         }
       }
     }
