@@ -197,6 +197,11 @@ __device__ __forceinline__ u64 whole_weight(float e) {
   split_weight(e, w1, w0);
   return (static_cast<u64>(w1 - kTop) << 23) + (w0 - kTop);
 }
+// *p += v in shared memory where v is not zero, without a branch
+__device__ __forceinline__ void add_some(unsigned* p, unsigned v) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(p));
+  asm volatile("{\n.reg .pred some;\nsetp.ne.u32 some, %1, 0;\n@some red.shared.add.u32 [%0], %1;\n}" ::"r"(at), "r"(v) : "memory");
+}
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 template <typename T, int CS, bool kStream>
@@ -369,8 +374,7 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const unsigned up = ((w1[j] & 0x7fffffu) >> 9) + (old[j] + x[j] < old[j] ? 1u : 0u);
-        if (up) atomicAdd(&sm.hist_hi[bin[j]], up);
+        add_some(&sm.hist_hi[bin[j]], ((w1[j] & 0x7fffffu) >> 9) + (old[j] + x[j] < old[j] ? 1u : 0u));
       }
     } else {
 #pragma unroll
@@ -751,10 +755,12 @@ template <typename T> int launch_tokens(const TokenArgs& a, int widest, cudaStre
     SURF_RETURN_LAUNCH();
   }
   if (answers >= 148 && widest > 8192 && widest <= kMaxStream) return launch_large<T, 1, true>(a, widest, s);
-  // slices of at most 8192 candidates (32 a thread, 4 blocks on an SM); smaller ones, down to
-  // 1024, while there are too few blocks to fill the GPU
+  // slices of at most 8192 candidates (32 a thread, 4 blocks on an SM), of 16384 once the
+  // blocks fill the GPU. Wider clusters cost more at their barriers than their blocks save:
+  // 64 rows of 32768 take 24 us in clusters of 4, 32 us in clusters of 8; 64 of 131072 57 us
+  // in clusters of 8, 65 us in clusters of 16; one of 32768 18.5 us in 4 blocks, 18.1 in 16.
   int cs = 1;
-  while (cs < kMaxCluster && (widest > cs * 8192 || (answers * cs < 2 * 148 && widest > cs * 1024))) cs *= 2;
+  while (cs < kMaxCluster && widest > cs * (answers * cs >= 148 ? kMaxSlice : 8192)) cs *= 2;
   const int slice = static_cast<int>(surfk::ceil_div(widest, cs));
   if (slice > kMaxSlice) return static_cast<int>(cudaErrorInvalidValue);
   switch (cs) {

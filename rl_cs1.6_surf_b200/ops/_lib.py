@@ -82,16 +82,20 @@ def stream_ptr(device=None) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)    # the tensors exist: CUDA is up
 
 
 def launch(fn, what: str, index: int, *args) -> None:
     """``fn(*args, stream)`` on device ``index`` and its current stream, whatever the
     current device is; raises on a non-zero status."""
-    if torch.cuda.current_device() != index:
+    if _current_device() != index:
         with torch.cuda.device(index):
             launch(fn, what, index, *args)
         return
-    check(fn(*args, _raw_stream(index) if _raw_stream is not None else stream_ptr(index)), what)
+    code = fn(*args, _raw_stream(index) if _raw_stream is not None else stream_ptr(index))
+    _launches[0] += _KERNELS_PER_CALL.get(what, 1)
+    if code:
+        raise KernelError(f"{what} failed with CUDA error {code}")
 
 
 def ptr(t) -> int:

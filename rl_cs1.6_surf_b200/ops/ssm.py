@@ -58,7 +58,7 @@ _STEP = struct.Struct("21q8i")
 
 
 def _p(t) -> int:
-    return 0 if t is None else t.data_ptr()
+    return t.data_ptr() if t is not None else 0
 
 
 def _dtype_code(t: torch.Tensor, what: str) -> int:
@@ -391,42 +391,48 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     it (None: row r is slot r; below 0: no env, its output is zero), moved on in place.
     No two rows may name one slot."""
     what = "selective_scan_step"
-    _lib.require_cuda(x, what)
+    if not x.is_cuda:
+        _lib.require_cuda(x, what)
     if x.dim() != 2:
         raise ValueError(f"{what}: x must be [rows, channels]")
+    dtype, f32 = x.dtype, torch.float32
     code = _dtype_code(x, what)
-    r, d = x.shape
-    dev, at, e = x.device, x.get_device(), x.element_size()
+    r, d = shape = x.shape
+    at = x.get_device()
     if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATE:
         raise ValueError(f"{what}: A must be [channels, states] with 1 to {MAX_STATE} states")
     n = A.shape[1]
     if B.dim() != 3 or B.shape[1] < 1 or d % B.shape[1]:
         raise ValueError(f"{what}: B must be [rows, groups, states], its groups dividing the channels")
     g = B.shape[1]
-    for name, v in (("x", x), ("dt", dt), ("z", z)):
-        _tokens(what, name, v, (r, d), x.dtype, at)
-    for name, v in (("B", B), ("C", C)):
-        _tokens(what, name, v, (r, g, n), x.dtype, at)
-    f32 = torch.float32
+    pools = state.shape[0]
+    _tokens(what, "x", x, shape, dtype, at)
+    _tokens(what, "dt", dt, shape, dtype, at)
+    _tokens(what, "z", z, shape, dtype, at)
+    _tokens(what, "B", B, (r, g, n), dtype, at)
+    _tokens(what, "C", C, (r, g, n), dtype, at)
     _dense(what, "A", A, (d, n), f32, at)
     _dense(what, "D", D, (d,), f32, at)
     _dense(what, "dt_bias", dt_bias, (d,), f32, at)
-    _dense(what, "state", state, (state.shape[0], d, n), f32, at)
+    _dense(what, "state", state, (pools, d, n), f32, at)
     _flags(what, reset, (r,), at)
     _dense(what, "slots", slots, (r,), torch.int32, at)
-    if slots is None and state.shape[0] < r:
-        raise ValueError(f"{what}: {r} rows, but {state.shape[0]} slots")
+    if slots is None and pools < r:
+        raise ValueError(f"{what}: {r} rows, but {pools} slots")
     if out is None:
-        out = torch.empty((r, d), dtype=x.dtype, device=dev)
+        out = torch.empty(shape, dtype=dtype, device=x.device)
     else:
-        _tokens(what, "out", out, x.shape, x.dtype, at)
+        _tokens(what, "out", out, shape, dtype, at)
     if r == 0 or d == 0:
         return out
-    args = _STEP.pack(x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias),
-                      state.data_ptr(), _p(reset), _p(slots), out.data_ptr(), error_flag(dev).data_ptr(), x.stride(0),
-                      dt.stride(0), 0 if z is None else z.stride(0), B.stride(0), B.stride(1), C.stride(0), C.stride(1),
-                      out.stride(0), r, d, n, g, int(softplus), state.shape[0],
-                      (_bits(e, B, C) | n * e) % (4 * e) == 0, 0)
+    e = 4 - 2 * code
+    pB, pC = B.data_ptr(), C.data_ptr()
+    B0, B1, _ = B.stride()
+    C0, C1, _ = C.stride()
+    whole = (pB | pC | (B0 | B1 | C0 | C1 | n) * e) % (4 * e) == 0
+    args = _STEP.pack(x.data_ptr(), dt.data_ptr(), _p(z), pB, pC, A.data_ptr(), _p(D), _p(dt_bias), state.data_ptr(),
+                      _p(reset), _p(slots), out.data_ptr(), error_flag(x.device).data_ptr(), x.stride(0), dt.stride(0),
+                      0 if z is None else z.stride(0), B0, B1, C0, C1, out.stride(0), r, d, n, g, softplus, pools, whole, 0)
     launch(_lib.lib(SLIB).surf_seq_scan_step, "surf_seq_scan_step", at, args, code)
     return out
 
