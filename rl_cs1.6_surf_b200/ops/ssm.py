@@ -96,6 +96,12 @@ def _dense(what: str, name: str, t: Optional[torch.Tensor], shape: tuple, dtype,
     raise ValueError(f"{what}: {name} must be contiguous")
 
 
+def _even(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """``t`` on a 16-byte boundary, where the kernels read their 32-bit operands four at a
+    time: itself, unless it is a view that starts elsewhere."""
+    return t if t is None or t.data_ptr() & 15 == 0 else t.clone()
+
+
 def _flags(what: str, t: Optional[torch.Tensor], shape: tuple, index: int) -> None:
     if t is None:
         return
@@ -162,6 +168,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     and behind the row, oldest first."""
     what = "causal_conv"
     code, e, at, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
+    weight = _even(weight)
     if out is None:
         out = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
     else:
@@ -189,6 +196,7 @@ def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bi
     code, e, at, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
     _tokens(what, "dy", dy, x.shape, x.dtype, at)
     _dense(what, "dfinal", dfinal, (b, w - 1, d), x.dtype, at)
+    weight = _even(weight)
     dev = x.device
     dx = torch.empty((b, t, d), dtype=x.dtype, device=dev)
     dstate = torch.empty((b, w - 1, d), dtype=x.dtype, device=dev) if state is not None else None
@@ -298,6 +306,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     for every 8 tokens."""
     what = "selective_scan"
     code, e, at, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
+    A, state = _even(A), _even(state)
     dev = x.device
     if out is None:
         out = torch.empty((b, t, d), dtype=x.dtype, device=dev)
@@ -345,6 +354,7 @@ def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A
     if saved is None:
         raise ValueError(f"{what}: needs the states that selective_scan(train=True) saved")
     _dense(what, "saved", saved, (b, -(-t // SAVE_EVERY), d, n), f32, at)
+    A, saved, dfinal = _even(A), _even(saved), _even(dfinal)
 
     def like(v, shape, dtype):
         return None if v is None else torch.empty(shape, dtype=dtype, device=dev)
@@ -425,6 +435,9 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
         _tokens(what, "out", out, shape, dtype, at)
     if r == 0 or d == 0:
         return out
+    A = _even(A)
+    if state.data_ptr() & 15:
+        raise ValueError(f"{what}: the state pool must start on a 16-byte boundary")
     e = 4 - 2 * code
     pB, pC = B.data_ptr(), C.data_ptr()
     B0, B1, _ = B.stride()

@@ -310,6 +310,73 @@ def test_graph_replay():
         assert torch.equal(out, w)
 
 
+def _shifted(t, by):
+    """The same values in a view that starts ``by`` elements into its storage."""
+    flat = torch.empty(t.numel() + by, dtype=t.dtype, device=t.device)
+    flat[by:] = t.reshape(-1)
+    return flat[by:].view(t.shape)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("by", [1, 2])
+def test_operands_on_odd_addresses(by, dtype):
+    """Views that start off the 16-byte boundaries, every operand: the same numbers."""
+    c = _conv_case(2, 30, 24, 4, True, False, dtype)
+    k = {n: _shifted(v, by) if isinstance(v, torch.Tensor) and n != "x" else v for n, v in c.items()}
+    k["x"] = _shifted(c["x"].contiguous(), by)
+    kw = lambda q: dict(state=q["state"], reset=q["reset"])  # noqa: E731
+    one = 2.0 ** -8 if dtype == torch.bfloat16 else 1e-6
+    want, got = (ssm.causal_conv(q["x"], q["weight"], q["bias"], **kw(q)) for q in (c, k))
+    assert rel(got[0], want[0]) <= one and torch.equal(got[1], want[1])
+    want, got = (ssm.causal_conv_grad(q["dy"], q["x"], q["weight"], q["bias"], dfinal=q["dfinal"], **kw(q)) for q in (c, k))
+    assert all(rel(p, q) <= one for p, q in zip(got, want))
+    c = _scan_case(2, 60, 40, 16, 1, True, False, dtype)
+    k = {n: _shifted(v.contiguous(), by) if isinstance(v, torch.Tensor) else v for n, v in c.items()}
+    (r, g), (r2, g2) = _scan_run(c), _scan_run(k)
+    assert rel(r2.out, r.out) <= TOL[dtype] and rel(r2.final, r.final) <= 1e-6
+    assert all(rel(p, q) <= TOL[p.dtype] for p, q in zip(g2, g))
+    with pytest.raises(ValueError, match="16-byte"):
+        ssm.selective_scan_step(c["x"][:, 0], c["dt"][:, 0], c["A"], c["B"][:, 0], c["C"][:, 0], k["state"])
+
+
+def test_offsets_past_32_bits():
+    """Rows 2^31 elements apart, in one allocation: the same as packed together."""
+    far = (1 << 31) + 8
+    buf = torch.zeros(far + 64 * 64, dtype=torch.bfloat16, device="cuda")
+    c = _scan_case(2, 40, 32, 16, 1, True, False, torch.bfloat16)
+    xz = buf.as_strided((2, 40, 64), (far, 64, 1))
+    xz[..., :32], xz[..., 32:] = c["x"], c["z"]
+    k = dict(c, x=xz[..., :32], z=xz[..., 32:])
+    (r, g), (r2, g2) = _scan_run(c), _scan_run(k)
+    assert torch.equal(r.out, r2.out) and all(torch.equal(p, q) for p, q in zip(g, g2))
+    w = torch.randn(32, 4, device="cuda")
+    y, f = ssm.causal_conv(c["x"], w)
+    y2, f2 = ssm.causal_conv(k["x"], w)
+    assert torch.equal(y, y2) and torch.equal(f, f2)
+    a, b = (ssm.causal_conv_grad(c["dout"], q["x"], w) for q in (c, k))
+    assert torch.equal(a.dx, b.dx) and torch.equal(a.dweight, b.dweight)
+
+
+def test_a_reset_forgets_what_is_not_finite():
+    """An episode that ended in infinities and NaN leaves nothing to the next one."""
+    c = _scan_case(1, 24, 16, 16, 1, False, False, torch.float32)
+    c["reset"] = torch.zeros(1, 24, dtype=torch.bool, device="cuda")
+    c["reset"][0, 11] = True
+    bad = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    bad["x"][0, 7] = float("inf")
+    bad["x"][0, 8] = float("nan")
+    (r, g), (r2, g2) = _scan_run(c), _scan_run(bad)
+    assert torch.equal(r.out[0, 11:], r2.out[0, 11:]) and torch.equal(r.final, r2.final)
+    for name in ("dx", "ddt", "dz", "dB", "dC"):
+        assert torch.equal(getattr(g, name)[0, 11:], getattr(g2, name)[0, 11:]), name
+    k = _conv_case(1, 24, 16, 4, False, False, torch.float32)
+    k["x"] = k["x"].clone()
+    y, _ = ssm.causal_conv(k["x"], k["weight"], reset=c["reset"])
+    k["x"][0, 9:11] = float("nan")
+    y2, _ = ssm.causal_conv(k["x"], k["weight"], reset=c["reset"])
+    assert torch.equal(y[0, 11:], y2[0, 11:])
+
+
 def test_refusals():
     c = _scan_case(2, 8, 16, 16, 1, False, False, torch.float32)
     a = [c[k] for k in ("x", "dt", "A", "B", "C")]

@@ -123,6 +123,17 @@ def test_heads(dtype):
     _same(big, u[:3, :3].contiguous(), heads=(100, 1, 60), top_p=0.8)
 
 
+def test_offsets_past_32_bits():
+    far = (1 << 31) + 4
+    buf = torch.zeros(far + 20000, dtype=torch.bfloat16, device="cuda")
+    for vocab in (30, 20000):
+        z = buf.as_strided((2, vocab), (far, 1))
+        z.copy_(torch.randn(2, vocab, device="cuda"))
+        u = torch.rand(2, 1, device="cuda")
+        a, b = TK.sample_tokens(z, u, top_p=0.9), TK.sample_tokens(z.contiguous(), u, top_p=0.9)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_numbers_at_the_ends():
     z = torch.randn(1, 100, device="cuda").expand(4, 100)
     u = torch.tensor([[0.0], [1.0 - 2.0 ** -24], [1.0], [-1.0]], device="cuda")
