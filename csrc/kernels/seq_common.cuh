@@ -28,27 +28,39 @@ template <typename T> constexpr int kVec16 = 16 / static_cast<int>(sizeof(T));
 template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
   if constexpr (V == 1) {
     v[0] = to_f(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    if constexpr (V == 4) {
+      const float4 q = *reinterpret_cast<const float4*>(p);
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+      const float2 q = *reinterpret_cast<const float2*>(p);
+      v[0] = q.x; v[1] = q.y;
+    }
   } else {
-    constexpr int kBytes = V * static_cast<int>(sizeof(T));
-    alignas(16) T raw[V];
-    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(p);
-    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
-    else *reinterpret_cast<uint32_t*>(raw) = *reinterpret_cast<const uint32_t*>(p);
+    uint32_t w[V / 2];
+    if constexpr (V == 8) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+    else if constexpr (V == 4) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+    else w[0] = *reinterpret_cast<const uint32_t*>(p);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = to_f(raw[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
   }
 }
 template <typename T, int V> __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
   if constexpr (V == 1) {
     *p = from_f<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
   } else {
-    constexpr int kBytes = V * static_cast<int>(sizeof(T));
-    alignas(16) T raw[V];
+    uint32_t w[V / 2];
 #pragma unroll
-    for (int i = 0; i < V; ++i) raw[i] = from_f<T>(v[i]);
-    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(raw);
-    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(raw);
-    else *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(raw);
+    for (int i = 0; i < V / 2; ++i) w[i] = surfk::pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    if constexpr (V == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
 }
 
@@ -155,13 +167,21 @@ __device__ __forceinline__ float exp2_hw(float x) {
 constexpr float kExp2Shift = 3e-8f;
 // exp(delta * A) with A2 = A log2(e)
 __device__ __forceinline__ float decay(float delta, float A2) { return exp2_hw(fmaf(delta, A2, kExp2Shift)); }
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + exp2_hw(-kLog2e * v)); }
+// 1 / x by the hardware's approximation (relative error 2^-23; 0 for infinity). The divisors
+// here lie between 1 and infinity: a division, even the approximate one, guards a range that
+// they never reach with four instructions more.
+__device__ __forceinline__ float rcp_hw(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sigmoid(float v) { return rcp_hw(1.0f + exp2_hw(-kLog2e * v)); }
 
 // log(1 + e^v) = max(v, 0) + log(1 + e^-|v|); with s = e / (2 + e) <= 1/3 the logarithm is
 // 2 atanh(s) = 2 s g(s^2), g fitted on [0, 1/9] to 4e-9: as exact for small e as for e = 1.
 __device__ __forceinline__ float softplus(float v) {
   const float e = exp2_hw(-kLog2e * fabsf(v));
-  const float s = __fdividef(e, 2.0f + e), q = s * s;
+  const float s = e * rcp_hw(2.0f + e), q = s * s;
   float g = fmaf(q, 0.14089155197143555f, 0.13980303704738617f);
   g = fmaf(g, q, 0.20012454688549042f);
   g = fmaf(g, q, 0.3333315849304199f);
