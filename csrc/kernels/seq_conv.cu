@@ -204,18 +204,15 @@ template <typename T, int V> struct Ring {
   }
 };
 
-// The W - 1 tokens before the stretch as its first token finds them (before its own
-// reset); returns bit j: it sees token t0 - 1 - j.
+// The W - 1 tokens before the stretch as its first token finds them (before its own reset).
 template <typename T, int W, int V>
-__device__ __forceinline__ unsigned window_of(const ConvArgs& a, const Stretch<T>& s, Pairs<V> (&h)[W - 1]) {
-  unsigned seen = 0;
+__device__ __forceinline__ void window_of(const ConvArgs& a, const Stretch<T>& s, Pairs<V> (&h)[W - 1]) {
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
     const int t = s.t0 - (W - 1) + j;
     h[j] = zeros<V>();
     if (t >= 0 && t < s.len) {
       if (s.cut(t)) {
-        seen = 0;
 #pragma unroll
         for (int q = 0; q < j; ++q) h[q] = zeros<V>();
       }
@@ -223,9 +220,7 @@ __device__ __forceinline__ unsigned window_of(const ConvArgs& a, const Stretch<T
     } else if (t < 0 && s.state) {
       h[j] = load_pairs_of<T, V>(s.state + static_cast<int64_t>(W - 1 + t) * a.D);
     }
-    seen = (seen << 1) | 1u;
   }
-  return seen;
 }
 
 // ---- whole sequences ----------------------------------------------------------------
@@ -256,14 +251,15 @@ __global__ void __launch_bounds__(kThreads, 2) conv_kernel(ConvArgs a, int items
       in.issue(u, s.t0 + u);
       cp_async_commit();
     }
-    // `whole`: kU tokens are there and none of them starts an episode
-    auto step = [&](int t, unsigned cuts, auto whole) {
+    // whole: kU tokens are there; resets: one of them starts an episode
+    auto step = [&](int t, unsigned cuts, auto whole, auto resets) {
+      constexpr bool kWhole = decltype(whole)::value, kResets = decltype(resets)::value;
       in.batch(t);
-#pragma unroll (decltype(whole)::value || !Ring<T, V>::kAsync ? kU : 1)
+#pragma unroll (kWhole || !Ring<T, V>::kAsync ? kU : 1)
       for (int u = 0; u < kU; ++u) {
-        if (decltype(whole)::value || t + u < live) {
+        if (kWhole || t + u < live) {
           cp_async_wait<kU - 1>();
-          if (!decltype(whole)::value && (cuts >> u & 1u)) {
+          if (kResets && (cuts >> u & 1u)) {
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) h[j] = zeros<V>();
           }
@@ -289,8 +285,9 @@ __global__ void __launch_bounds__(kThreads, 2) conv_kernel(ConvArgs a, int items
     };
     for (int t = s.t0; t < live; t += kU) {
       const unsigned cuts = cuts_of<T>(s, t);
-      if (!cuts && t + kU <= live) step(t, 0, std::true_type{});
-      else step(t, cuts, std::false_type{});
+      if (t + kU > live) step(t, cuts, std::false_type{}, std::true_type{});
+      else if (cuts) step(t, cuts, std::true_type{}, std::true_type{});
+      else step(t, 0, std::true_type{}, std::false_type{});
     }
     cp_async_wait<0>();
     for (int t = max(s.t0, live); t < s.t1; ++t) store_pairs_of<T, V>(y + t * a.y_t, zeros<V>());
@@ -337,14 +334,20 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
       const T* df = a.dfinal ? static_cast<const T*>(a.dfinal) + ends : nullptr;
       T* ds = a.final_state ? static_cast<T*>(a.final_state) + ends : nullptr;
       Pairs<V> h[W - 1], pend[W];                    // pend[j]: dx of token t - j so far
-      unsigned seen = window_of<T, W, V>(a, s, h);   // bit j: token t sees token t - 1 - j
-      constexpr unsigned kAll = (1u << (W - 1)) - 1u;
+      window_of<T, W, V>(a, s, h);
 #pragma unroll
       for (int j = 0; j < W; ++j) pend[j] = zeros<V>();
       if (s.len == 0 && s.chunk == 0 && df) {        // an empty row hands its state on
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) pend[j + 1] = load_pairs_of<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D);
       }
+      // Tokens from `from` on still wait for their dx. A reset at token t ends the wait of all
+      // before it: theirs is written there and then, and what is added to them later is not.
+      int from = s.chunk == 0 && ds ? -(W - 1) : s.t0;
+      auto emit = [&](int t, const Pairs<V>& v) {
+        if (t >= 0) store_pairs_of<T, V>(dx + t * a.y_t, v);
+        else store_pairs_of<T, V>(ds + static_cast<int64_t>(W - 1 + t) * a.D, v);
+      };
       const int end = s.t1 + W - 1;
       Word* const slots = reinterpret_cast<Word*>(smem) + threadIdx.y * blockDim.x + threadIdx.x;
       const int stop = min(end, s.len);
@@ -355,9 +358,10 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
         gin.issue(u, s.t0 + u);
         cp_async_commit();
       }
-      // whole: kU tokens of the stretch's own, no reset in sight, the row goes on
-      auto step = [&](int tb, unsigned cuts, auto whole) {
-        constexpr bool kWhole = decltype(whole)::value;
+      // whole: kU tokens of the stretch's own, the row goes on behind them; resets: one of them
+      // starts an episode
+      auto step = [&](int tb, unsigned cuts, auto whole, auto resets) {
+        constexpr bool kWhole = decltype(whole)::value, kResets = decltype(resets)::value;
         xin.batch(tb);
         gin.batch(tb);
 #pragma unroll (kWhole || !Ring<T, V>::kAsync ? kU : 1)
@@ -367,10 +371,13 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
             cp_async_wait<kU - 1>();
             const Pairs<V> now = kWhole || t < s.len ? xin.get(u) : zeros<V>();
             if (kWhole || t < s.len) {
-              if (!kWhole && (cuts >> u & 1u)) {
-                seen = 0;
+              if (kResets && (cuts >> u & 1u)) {
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) h[j] = zeros<V>();
+#pragma unroll
+                for (int j = W - 1; j > 0; --j)
+                  if (t - j >= from && t - j < s.t1) emit(t - j, pend[j]);
+                from = max(from, t);
               }
               Pairs<V> g = gin.get(u);
               if (a.silu) {
@@ -390,8 +397,7 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
               }
               madd<V>(pend[0], w[W - 1], g);
 #pragma unroll
-              for (int j = 1; j < W; ++j)
-                if (kWhole || (seen >> (j - 1) & 1u)) madd<V>(pend[j], w[W - 1 - j], g);
+              for (int j = 1; j < W; ++j) madd<V>(pend[j], w[W - 1 - j], g);
               if (kWhole || t < s.t1) {
 #pragma unroll
                 for (int i = 0; i < kPairs<V>; ++i) db.p[i] = add2(db.p[i], g.p[i]);
@@ -401,24 +407,21 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
               }
               if (!kWhole && t == s.len - 1 && df) {             // the state behind the last token
 #pragma unroll
-                for (int j = 0; j < W - 1; ++j)
-                  if (j == 0 || (seen >> (j - 1) & 1u)) {
-                    const Pairs<V> e = load_pairs_of<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D);
+                for (int j = 0; j < W - 1; ++j) {
+                  const Pairs<V> e = load_pairs_of<T, V>(df + static_cast<int64_t>(W - 2 - j) * a.D);
 #pragma unroll
-                    for (int i = 0; i < kPairs<V>; ++i) pend[j].p[i] = add2(pend[j].p[i], e.p[i]);
-                  }
+                  for (int i = 0; i < kPairs<V>; ++i) pend[j].p[i] = add2(pend[j].p[i], e.p[i]);
+                }
               }
             }
             const int done = t - (W - 1);
-            if (done >= s.t0 && (kWhole || done < s.t1)) store_pairs_of<T, V>(dx + done * a.y_t, pend[W - 1]);
-            else if (done < 0 && ds) store_pairs_of<T, V>(ds + static_cast<int64_t>(W - 1 + done) * a.D, pend[W - 1]);
+            if (done >= from && (kWhole || done < s.t1)) emit(done, pend[W - 1]);
 #pragma unroll
             for (int j = W - 1; j > 0; --j) pend[j] = pend[j - 1];
             pend[0] = zeros<V>();
 #pragma unroll
             for (int j = 0; j + 1 < W - 1; ++j) h[j] = h[j + 1];
             h[W - 2] = now;
-            if (!kWhole) seen = (seen << 1) | 1u;
             xin.issue(u, t + kU);
             gin.issue(u, t + kU);
             cp_async_commit();
@@ -427,8 +430,9 @@ __global__ void __launch_bounds__(kThreads, 2) conv_grad_kernel(ConvArgs a, int 
       };
       for (int tb = s.t0; tb < end; tb += kU) {
         const unsigned cuts = cuts_of<T>(s, tb);
-        if (!cuts && (seen & kAll) == kAll && tb + kU <= s.t1 && tb + kU < s.len) step(tb, 0, std::true_type{});
-        else step(tb, cuts, std::false_type{});
+        if (tb + kU > s.t1 || tb + kU >= s.len) step(tb, cuts, std::false_type{}, std::true_type{});
+        else if (cuts) step(tb, cuts, std::true_type{}, std::true_type{});
+        else step(tb, 0, std::true_type{}, std::false_type{});
       }
       cp_async_wait<0>();
     }
