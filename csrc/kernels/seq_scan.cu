@@ -166,7 +166,9 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(ScanArgs a, int block
     skip[j] = a.D && ec + j < nch ? a.D[d0 + ec + j] : 0.0f;
   }
 
-  bool any_cut = false;
+  // the tile's reset flags, a token a lane, on their way a tile ahead
+  auto flag_of = [&](int t) { return reset && lane < kTile && t + lane < t_live && reset[t + lane] != 0; };
+  bool any_cut = false, flag = flag_of(t_lo);
   int buf = 1;
   for (int t0 = t_lo - kTile; t0 < t_live; t0 += kTile, buf ^= 1) {
     cp_async_wait<0>();
@@ -176,8 +178,9 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(ScanArgs a, int block
     const int rows = min(kTile, t_live - t0);
     // bit r: token r starts an episode (every warp finds them for itself)
     static_assert(kTile <= 32, "a warp's lanes look at a tile's tokens");
-    const unsigned cuts = __ballot_sync(0xffffffffu, reset && lane < rows && reset[t0 + lane]);
+    const unsigned cuts = __ballot_sync(0xffffffffu, flag);
     any_cut |= cuts != 0;
+    flag = flag_of(t0 + kTile);
     // delta and delta * x (channels past the block's last are never looked at)
 #pragma unroll 2
     for (int r = er; r < kTile; r += kStep) {
@@ -209,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(ScanArgs a, int block
       }
     }
     __syncthreads();
-#pragma unroll 4
+#pragma unroll 8
     for (int r = 0; r < kTile; ++r) {
       if (cuts >> r & 1u) {
 #pragma unroll
