@@ -22,11 +22,10 @@ namespace {
 using namespace seqk;
 
 constexpr int kTile = 16;
-constexpr int kThreads = 128;
 
-template <typename T, int LN> struct Layout {
+template <typename T, int LN, int kThreads> struct Layout {
   static constexpr int K = LN < 4 ? 2 : 4;               // channels of a thread, taken in pairs
-  static constexpr int CH = kThreads / LN * K;           // channels of a block
+  static constexpr int CH = scan_channels<LN>(kThreads); // channels of a block
   static constexpr int NP = 4 * LN;                      // states, padded
   struct Smem {
     alignas(16) T x[2][kTile * CH], dt[2][kTile * CH], z[2][kTile * CH], B[2][kTile * NP], C[2][kTile * NP];
@@ -40,9 +39,9 @@ template <typename T, int LN> struct Layout {
 // The recurrence of a token costs 4 multiply-adds and an exponential per state. Two
 // channels share an instruction (f32x2), which leaves the exponential unit's 16 a cycle
 // and SM as the bound.
-template <typename T, int LN, bool kCarry>
-__global__ void __launch_bounds__(kThreads, 4) scan_kernel(ScanArgs a, int blocks_per_group) {
-  using L = Layout<T, LN>;
+template <typename T, int LN, int kThreads, bool kCarry>
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) scan_kernel(ScanArgs a, int blocks_per_group) {
+  using L = Layout<T, LN, kThreads>;
   constexpr int K = L::K, P = K / 2, CH = L::CH, NP = L::NP;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   typename L::Smem& sm = *reinterpret_cast<typename L::Smem*>(smem_raw);
@@ -310,22 +309,29 @@ __global__ void __launch_bounds__(128) carry_kernel(ScanArgs a) {
                        a.cut + row, a.chunks);
 }
 
-template <typename T, int LN> int launch_scan(const ScanArgs& a, cudaStream_t s) {
-  using L = Layout<T, LN>;
+template <typename T, int LN, int kThreads> int launch_scan(const ScanArgs& a, cudaStream_t s) {
+  using L = Layout<T, LN, kThreads>;
   const int bpg = static_cast<int>(surfk::ceil_div(a.dim / a.G, L::CH));
   const int64_t gx = static_cast<int64_t>(bpg) * a.G * a.batch;
   if (gx > 0x7fffffffLL || a.chunks > 65535) return static_cast<int>(cudaErrorInvalidValue);
   constexpr size_t smem = sizeof(typename L::Smem);
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(a.chunks));
   if (a.chunks > 1) {
-    if (const int rc = allow_smem<scan_kernel<T, LN, true>>(smem)) return rc;
-    scan_kernel<T, LN, true><<<grid, kThreads, smem, s>>>(a, bpg);
+    if (const int rc = allow_smem<scan_kernel<T, LN, kThreads, true>>(smem)) return rc;
+    scan_kernel<T, LN, kThreads, true><<<grid, kThreads, smem, s>>>(a, bpg);
     const int64_t n = static_cast<int64_t>(a.batch) * a.dim * a.N;
     carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(n, 128)), 128, 0, s>>>(a);
   }
-  if (const int rc = allow_smem<scan_kernel<T, LN, false>>(smem)) return rc;
-  scan_kernel<T, LN, false><<<grid, kThreads, smem, s>>>(a, bpg);
+  if (const int rc = allow_smem<scan_kernel<T, LN, kThreads, false>>(smem)) return rc;
+  scan_kernel<T, LN, kThreads, false><<<grid, kThreads, smem, s>>>(a, bpg);
   SURF_RETURN_LAUNCH();
+}
+
+// whether a group's channels leave half of an ordinary block idle
+template <int LN> bool small_blocks(int per_group) { return 2 * per_group <= scan_channels<LN>(kScanBlock<LN>); }
+
+template <typename T, int LN> int launch_scan(const ScanArgs& a, cudaStream_t s) {
+  return small_blocks<LN>(a.dim / a.G) ? launch_scan<T, LN, kSmallBlock<LN>>(a, s) : launch_scan<T, LN, kScanBlock<LN>>(a, s);
 }
 
 // ---- single tokens -----------------------------------------------------------------------
@@ -456,6 +462,15 @@ SURF_EXPORT int surf_seq_scan_step(const void* args, int dtype, void* stream) {
   return by_lanes(a.N, [&](auto ln) {
     constexpr int LN = decltype(ln)::value;
     return dtype == kBf16 ? launch_step<bf16, LN>(a, s) : launch_step<float, LN>(a, s);
+  });
+}
+
+// The forward's blocks of a row, in threads (the caller cuts rows where they do not fill the GPU).
+SURF_EXPORT int surf_seq_scan_threads(int per_group, int groups, int N) {
+  return by_lanes(N, [&](auto ln) {
+    constexpr int LN = decltype(ln)::value;
+    const int threads = small_blocks<LN>(per_group) ? kSmallBlock<LN> : kScanBlock<LN>;
+    return static_cast<int>(surfk::ceil_div(per_group, scan_channels<LN>(threads))) * groups * threads;
   });
 }
 

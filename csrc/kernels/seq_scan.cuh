@@ -141,6 +141,16 @@ template <typename T> __device__ __forceinline__ void store_quad(T* p, const flo
   }
 }
 
+// Threads of a block. A block's channels lie in one group, so a group that fills at most half
+// of the ordinary block's channels gets blocks of one warp (two for the widest states, whose
+// rows of channels stay whole 16-byte pieces): 119 x 1047 tokens of 4 groups of 5 channels
+// would leave 59 of 64 channel places idle.
+template <int LN> constexpr int kSmallBlock = LN == 16 ? 64 : 32;
+template <int LN> constexpr int kScanBlock = 128;
+template <int LN> constexpr int kGradBlock = LN < 4 ? 128 : 256;
+template <int LN> constexpr int scan_channels(int threads) { return threads / LN * (LN < 4 ? 2 : 4); }
+template <int LN> constexpr int grad_channels(int threads) { return threads / LN * 2; }
+
 // states -> lanes of a channel row; f gets the count as a compile-time constant
 template <typename F> int by_lanes(int N, F f) {
   if (N < 1 || N > 64) return static_cast<int>(cudaErrorInvalidValue);

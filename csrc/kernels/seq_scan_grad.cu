@@ -23,9 +23,9 @@ namespace {
 
 using namespace seqk;
 
-template <typename T, int LN> struct GradLayout {
-  static constexpr int NT = LN < 4 ? 128 : 256;
-  static constexpr int CH = NT / LN * 2;                  // two channels a thread, 4 states of each in two f32x2 pairs
+template <typename T, int LN, int kThreads> struct GradLayout {
+  static constexpr int NT = kThreads;
+  static constexpr int CH = grad_channels<LN>(NT);        // two channels a thread, 4 states of each in two f32x2 pairs
   static constexpr int NP = 4 * LN;
   static constexpr int R = kSave;                         // tokens of a tile
   struct Smem {
@@ -102,11 +102,10 @@ __device__ __forceinline__ float sum_of(f2 v) {
 // exponentials, the sums across lanes 13 exchanges for 8 states: shared memory's 128 bytes
 // a cycle (exchanges and loads, about 40 of its cycles for 256 states), the exponential unit
 // (32 cycles) and the issue rate bound it alike.
-template <typename T, int LN, bool kCarry>
-__global__ void __launch_bounds__(GradLayout<T, LN>::NT, (kCarry ? 768 : 512) / GradLayout<T, LN>::NT)
-scan_grad_kernel(ScanArgs a, int blocks_per_group) {
-  using L = GradLayout<T, LN>;
-  constexpr int CH = L::CH, NP = L::NP, R = L::R, NT = L::NT;
+template <typename T, int LN, int NT, bool kCarry>
+__global__ void __launch_bounds__(NT, (kCarry ? 768 : 512) / NT) scan_grad_kernel(ScanArgs a, int blocks_per_group) {
+  using L = GradLayout<T, LN, NT>;
+  constexpr int CH = L::CH, NP = L::NP, R = L::R;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   typename L::Smem& sm = *reinterpret_cast<typename L::Smem*>(smem_raw);
   const int blocks = blocks_per_group * a.G;
@@ -243,10 +242,10 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
 
   // dB and dC of the tile: a thread sums one state of every kBcStep-th token over the warps
   constexpr int kBcStep = NT / (2 * NP) > 0 ? NT / (2 * NP) : 1;
-  static_assert(NT % (2 * NP) == 0, "a thread keeps its state");
   const int bq = threadIdx.x % (2 * NP), br = threadIdx.x / (2 * NP), bn = bq % NP;
   const int64_t bc_stride = static_cast<int64_t>(a.G) * 2 * a.N;
-  float* const pbc = kCarry ? nullptr : a.part_bc + ((static_cast<int64_t>(sub) * a.batch + b) * a.T * a.G + g) * (2 * a.N) + (bq < NP ? bn : a.N + bn);
+  float* const pbc = kCarry ? nullptr : a.part_bc + ((static_cast<int64_t>(sub) * a.batch + b) * a.T * a.G + g) * (2 * a.N) +
+                                        (NT < 2 * NP ? 0 : bq < NP ? bn : a.N + bn);
 
   bool any_cut = false;
   int buf = 1;
@@ -445,12 +444,23 @@ scan_grad_kernel(ScanArgs a, int blocks_per_group) {
         store_quad<T>(gdx + o, dx, nch - ec, a.mode_d == kPieces16);
         store_quad<T>(gddt + o, ddt, nch - ec, a.mode_d == kPieces16);
       }
-      if (bn < a.N) {
-        for (int r = br; r < rows; r += kBcStep) {
+      if constexpr (NT >= 2 * NP) {
+        if (bn < a.N) {
+          for (int r = br; r < rows; r += kBcStep) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NT / 32; ++w) s += sm.red[w][r][bq];
+            pbc[(t0 + r) * bc_stride] = s;
+          }
+        }
+      } else {
+        for (int i = threadIdx.x; i < rows * 2 * NP; i += NT) {
+          const int r = i / (2 * NP), q = i % (2 * NP), n = q % NP;
+          if (n >= a.N) continue;
           float s = 0.0f;
 #pragma unroll
-          for (int w = 0; w < NT / 32; ++w) s += sm.red[w][r][bq];
-          pbc[(t0 + r) * bc_stride] = s;
+          for (int w = 0; w < NT / 32; ++w) s += sm.red[w][r][q];
+          pbc[(t0 + r) * bc_stride + (q < NP ? n : a.N + n)] = s;
         }
       }
     }
@@ -554,25 +564,32 @@ __global__ void __launch_bounds__(256) finish_weights_kernel(ScanArgs a) {
   }
 }
 
-template <typename T, int LN> int launch_grad(const ScanArgs& a, cudaStream_t s) {
-  using L = GradLayout<T, LN>;
+template <typename T, int LN, int NT> int launch_grad(const ScanArgs& a, cudaStream_t s) {
+  using L = GradLayout<T, LN, NT>;
   const int bpg = static_cast<int>(surfk::ceil_div(a.dim / a.G, L::CH));
   const int64_t gx = static_cast<int64_t>(bpg) * a.G * a.batch;
   if (gx > 0x7fffffffLL || a.chunks > 65535) return static_cast<int>(cudaErrorInvalidValue);
   constexpr size_t smem = sizeof(typename L::Smem);
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(a.chunks));
   if (a.chunks > 1) {
-    if (const int rc = allow_smem<scan_grad_kernel<T, LN, true>>(smem)) return rc;
-    scan_grad_kernel<T, LN, true><<<grid, L::NT, smem, s>>>(a, bpg);
+    if (const int rc = allow_smem<scan_grad_kernel<T, LN, NT, true>>(smem)) return rc;
+    scan_grad_kernel<T, LN, NT, true><<<grid, NT, smem, s>>>(a, bpg);
     grad_carry_kernel<<<static_cast<unsigned>(surfk::ceil_div(static_cast<int64_t>(a.batch) * a.dim * a.N, 128)), 128, 0, s>>>(a);
   }
-  if (const int rc = allow_smem<scan_grad_kernel<T, LN, false>>(smem)) return rc;
-  scan_grad_kernel<T, LN, false><<<grid, L::NT, smem, s>>>(a, bpg);
+  if (const int rc = allow_smem<scan_grad_kernel<T, LN, NT, false>>(smem)) return rc;
+  scan_grad_kernel<T, LN, NT, false><<<grid, NT, smem, s>>>(a, bpg);
   const int64_t n = static_cast<int64_t>(a.batch) * a.T * a.G * 2 * a.N;
   const int64_t blocks = surfk::ceil_div(n, 256);
   finish_bc_kernel<T><<<static_cast<unsigned>(blocks < 148 * 16 ? (blocks > 0 ? blocks : 1) : 148 * 16), 256, 0, s>>>(a, bpg);
   finish_weights_kernel<<<static_cast<unsigned>(surfk::ceil_div(static_cast<int64_t>(a.dim) * (a.N + 2), 32)), dim3(32, 8), 0, s>>>(a);
   SURF_RETURN_LAUNCH();
+}
+
+// whether a group's channels leave half of an ordinary block idle
+template <int LN> bool small_blocks(int per_group) { return 2 * per_group <= grad_channels<LN>(kGradBlock<LN>); }
+
+template <typename T, int LN> int launch_grad(const ScanArgs& a, cudaStream_t s) {
+  return small_blocks<LN>(a.dim / a.G) ? launch_grad<T, LN, kSmallBlock<LN>>(a, s) : launch_grad<T, LN, kGradBlock<LN>>(a, s);
 }
 
 }  // namespace
@@ -590,6 +607,7 @@ SURF_EXPORT int surf_seq_scan_grad(const void* args, int dtype, void* stream) {
 // channel blocks of a group (the caller sizes part_bc with it)
 SURF_EXPORT int surf_seq_scan_grad_blocks(int per_group, int N) {
   return by_lanes(N, [&](auto ln) {
-    return static_cast<int>(surfk::ceil_div(per_group, GradLayout<float, decltype(ln)::value>::CH));
+    constexpr int LN = decltype(ln)::value;
+    return static_cast<int>(surfk::ceil_div(per_group, grad_channels<LN>(small_blocks<LN>(per_group) ? kSmallBlock<LN> : kGradBlock<LN>)));
   });
 }

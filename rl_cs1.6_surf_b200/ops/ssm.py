@@ -41,6 +41,7 @@ _lib.register(SLIB, {
     "surf_seq_scan": (_I, [c_char_p, _I, _V]),
     "surf_seq_scan_grad": (_I, [c_char_p, _I, _V]),
     "surf_seq_scan_grad_blocks": (_I, [_I, _I]),
+    "surf_seq_scan_threads": (_I, [_I, _I, _I]),
     "surf_seq_scan_step": (_I, [c_char_p, _I, _V]),
     "surf_seq_args_size": (_I, [_I]),
 })
@@ -282,10 +283,8 @@ def _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths):
 
 def _chunks(b: int, t: int, d: int, n: int, g: int):
     """(tokens of a chunk, chunks): a row is cut only where its channels do not fill the GPU."""
-    lanes = 1 if n <= 4 else 2 if n <= 8 else 4 if n <= 16 else 8 if n <= 32 else 16
-    per_block = 128 // lanes * (4 if lanes >= 4 else 2)
-    blocks = b * g * -(-(d // g) // per_block)
-    want = max(1, min(592 // blocks if blocks else 1, t // 64))
+    threads = b * _lib.lib(SLIB).surf_seq_scan_threads(d // g, g, n)
+    want = max(1, min(148 * 512 // threads if threads else 1, t // 64))
     if want <= 1:
         return max(16, -(-t // 16) * 16), 1
     chunk = -(-t // want)
