@@ -527,37 +527,38 @@ __global__ void __launch_bounds__(128) grad_carry_kernel(ScanArgs a) {
   if (a.dstate) a.dstate[id] = dh;
 }
 
-// dB, dC: the sum over a group's channel blocks, in block order
-template <typename T> __global__ void __launch_bounds__(256) finish_bc_kernel(ScanArgs a, int blocks) {
-  const int64_t n = static_cast<int64_t>(a.batch) * a.T * a.G * 2 * a.N;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    float s = 0.0f;
-    for (int k = 0; k < blocks; ++k) s += a.part_bc[k * n + i];
-    const int64_t row = i / (2 * a.N);
-    const int q = static_cast<int>(i - row * (2 * a.N));
-    if (q < a.N) static_cast<T*>(a.dB)[row * a.N + q] = from_f<T>(s);
-    else static_cast<T*>(a.dC)[row * a.N + q - a.N] = from_f<T>(s);
+// The last sums, in a fixed order. Blocks below bc_blocks: dB and dC, over a group's channel
+// blocks. The others: dA, dD and ddt_bias over rows and chunks, 32 numbers a block, 8 row
+// sums side by side.
+template <typename T> __global__ void __launch_bounds__(256) finish_kernel(ScanArgs a, int blocks, int bc_blocks) {
+  if (static_cast<int>(blockIdx.x) < bc_blocks) {
+    const int64_t n = static_cast<int64_t>(a.batch) * a.T * a.G * 2 * a.N;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(bc_blocks) * 256) {
+      float s = 0.0f;
+      for (int k = 0; k < blocks; ++k) s += a.part_bc[k * n + i];
+      const int64_t row = i / (2 * a.N);
+      const int q = static_cast<int>(i - row * (2 * a.N));
+      if (q < a.N) static_cast<T*>(a.dB)[row * a.N + q] = from_f<T>(s);
+      else static_cast<T*>(a.dC)[row * a.N + q - a.N] = from_f<T>(s);
+    }
+    return;
   }
-}
-
-// dA, dD, ddt_bias: the sum over rows and chunks, 8 row sums side by side, joined in order
-__global__ void __launch_bounds__(256) finish_weights_kernel(ScanArgs a) {
   __shared__ float red[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t na = static_cast<int64_t>(a.dim) * a.N, total = na + 2 * static_cast<int64_t>(a.dim);
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x;
+  const int64_t e = static_cast<int64_t>(blockIdx.x - bc_blocks) * 32 + tx;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.chunks;
   float s = 0.0f;
   if (e < total) {
     const float* p = e < na ? a.part_a + e : a.part_v + (e - na);
     const int64_t step = e < na ? na : 2 * static_cast<int64_t>(a.dim);
-    for (int64_t r = threadIdx.y; r < rows; r += 8) s += p[r * step];
+    for (int64_t r = ty; r < rows; r += 8) s += p[r * step];
   }
-  red[threadIdx.y][threadIdx.x] = s;
+  red[ty][tx] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && e < total) {
+  if (ty == 0 && e < total) {
 #pragma unroll
-    for (int r = 1; r < 8; ++r) s += red[r][threadIdx.x];
+    for (int r = 1; r < 8; ++r) s += red[r][tx];
     if (e < na) a.dA[e] = s;
     else if (e - na < a.dim) { if (a.dD) a.dD[e - na] = s; }
     else if (a.dbias) a.dbias[e - na - a.dim] = s;
@@ -578,10 +579,10 @@ template <typename T, int LN, int NT> int launch_grad(const ScanArgs& a, cudaStr
   }
   if (const int rc = allow_smem<scan_grad_kernel<T, LN, NT, false>>(smem)) return rc;
   scan_grad_kernel<T, LN, NT, false><<<grid, NT, smem, s>>>(a, bpg);
-  const int64_t n = static_cast<int64_t>(a.batch) * a.T * a.G * 2 * a.N;
-  const int64_t blocks = surfk::ceil_div(n, 256);
-  finish_bc_kernel<T><<<static_cast<unsigned>(blocks < 148 * 16 ? (blocks > 0 ? blocks : 1) : 148 * 16), 256, 0, s>>>(a, bpg);
-  finish_weights_kernel<<<static_cast<unsigned>(surfk::ceil_div(static_cast<int64_t>(a.dim) * (a.N + 2), 32)), dim3(32, 8), 0, s>>>(a);
+  const int64_t bc = surfk::ceil_div(static_cast<int64_t>(a.batch) * a.T * a.G * 2 * a.N, 256);
+  const int bc_blocks = static_cast<int>(bc < 148 * 16 ? bc : 148 * 16);
+  const int64_t weights = surfk::ceil_div(static_cast<int64_t>(a.dim) * (a.N + 2), 32);
+  finish_kernel<T><<<static_cast<unsigned>(bc_blocks + weights), 256, 0, s>>>(a, bpg, bc_blocks);
   SURF_RETURN_LAUNCH();
 }
 

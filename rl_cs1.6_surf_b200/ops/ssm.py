@@ -292,6 +292,17 @@ def _chunks(b: int, t: int, d: int, n: int, g: int):
     return chunk, -(-t // chunk)
 
 
+def _workspace(dev, *floats):
+    """One allocation for pieces of so many 32-bit numbers: (it, the pieces' addresses)."""
+    at, total = [], 0
+    for n in floats:
+        at.append(4 * total)
+        total += (n + 3) // 4 * 4
+    ws = torch.empty(total, dtype=torch.float32, device=dev)
+    base = ws.data_ptr()
+    return ws, [base + o for o in at]
+
+
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
                    D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
                    dt_bias: Optional[torch.Tensor] = None, softplus: bool = True,
@@ -316,20 +327,17 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     if b == 0 or d == 0:
         return Scan(out, final, saved)
     chunk, chunks = _chunks(b, t, d, n, g)
-    carry = sumd = cut = None
-    if chunks > 1:
-        carry = torch.empty((b, chunks, d, n), dtype=torch.float32, device=dev)
-        sumd = torch.empty((b, chunks, d), dtype=torch.float32, device=dev)
-        cut = torch.empty((b, chunks), dtype=torch.uint8, device=dev)
+    ws, (carry, sumd, cut) = _workspace(dev, b * chunks * d * n, b * chunks * d, b * chunks) if chunks > 1 else (None, (0, 0, 0))
     args = _SCAN.pack(
         x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), 0, A.data_ptr(), _p(D), _p(dt_bias), _p(state), 0,
-        _p(reset), _p(lengths), out.data_ptr(), final.data_ptr(), _p(saved), _p(carry), _p(sumd), _p(cut),
+        _p(reset), _p(lengths), out.data_ptr(), final.data_ptr(), _p(saved), carry, sumd, cut,
         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
         x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
         0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
         0, 0, out.stride(0), out.stride(1), t, b, t, d, n, g, int(softplus), chunk, chunks,
         _piece(d // g, e, x, dt, z, out), _piece(n, e, B, C))
     launch(_lib.lib(SLIB).surf_seq_scan, "surf_seq_scan", at, args, code)
+    del ws                                     # the stream's next user comes after the launch
     if chunks > 1:
         _lib.add_launches(2)
     return Scan(out, final, saved)
@@ -369,24 +377,21 @@ def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A
         return ScanGrads(dx, ddt, dz, dB, dC, dA, dD, dbias, dstate)
     chunk, chunks = _chunks(b, t, d, n, g)
     L = _lib.lib(SLIB)
-    carry = sumd = cut = None
-    if chunks > 1:
-        carry = torch.empty((b, chunks, d, n), dtype=f32, device=dev)
-        sumd = torch.empty((b, chunks, d), dtype=f32, device=dev)
-        cut = torch.empty((b, chunks), dtype=torch.uint8, device=dev)
-    part_bc = torch.empty(L.surf_seq_scan_grad_blocks(d // g, n) * b * t * g * 2 * n, dtype=f32, device=dev)
-    part_a = torch.empty(b * chunks * d * (n + 2), dtype=f32, device=dev)
+    split = b * chunks if chunks > 1 else 0
+    ws, (part_bc, part_a, part_v, carry, sumd, cut) = _workspace(
+        dev, L.surf_seq_scan_grad_blocks(d // g, n) * b * t * g * 2 * n, b * chunks * d * n, b * chunks * d * 2,
+        split * d * n, split * d, split)
     args = _SCAN.pack(
         x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), dout.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias),
-        _p(state), _p(dfinal), _p(reset), _p(lengths), 0, 0, saved.data_ptr(), _p(carry), _p(sumd), _p(cut),
-        dx.data_ptr(), ddt.data_ptr(), _p(dz), dB.data_ptr(), dC.data_ptr(), part_bc.data_ptr(), part_a.data_ptr(),
-        part_a.data_ptr() + 4 * b * chunks * d * n, dA.data_ptr(), _p(dD), _p(dbias), _p(dstate),
+        _p(state), _p(dfinal), _p(reset), _p(lengths), 0, 0, saved.data_ptr(), carry, sumd, cut,
+        dx.data_ptr(), ddt.data_ptr(), _p(dz), dB.data_ptr(), dC.data_ptr(), part_bc, part_a, part_v, dA.data_ptr(), _p(dD), _p(dbias), _p(dstate),
         x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
         0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
         dout.stride(0), dout.stride(1), 0, 0, t, b, t, d, n, g, int(softplus), chunk, chunks,
         _piece(d // g, e, x, dt, z, dout), _piece(n, e, B, C))
     launch(L.surf_seq_scan_grad, "surf_seq_scan_grad", at, args, code)
-    _lib.add_launches(4 if chunks > 1 else 2)
+    del ws
+    _lib.add_launches(3 if chunks > 1 else 1)
     return ScanGrads(dx, ddt, dz, dB, dC, dA, dD, dbias, dstate)
 
 
