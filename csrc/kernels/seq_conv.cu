@@ -8,8 +8,14 @@
 // without one); reset[b, t] drops everything before token t, and tokens from
 // lengths[b] on are not there: they give zeros and are never read. Everything is
 // one pass over memory (2 W + 4 flops per element against 4 to 8 bytes): the
-// window slides through registers, a thread owning kV neighbouring channels over a
+// window slides through registers, a thread owning neighbouring channels over a
 // stretch of tokens, so each x is read once (plus W - 1 of every stretch).
+//
+// Measured on a B200, bf16, W = 4: forward 256 x 128 x 1024 37 us (134 MB, 3.6 TB/s),
+// gradient 82 us (201 MB, 2.5 TB/s), a prompt of 16385 x 1024 18 us (67 MB, 3.7 TB/s); one
+// token of 64 envs 2.5 us. What bounds them is instructions at 16 warps on an SM (14 an
+// element in the forward, 36 in the gradient, a sigmoid's 5 and its derivative's 10 among
+// them): with the SiLU left out they take 27 and 54 us.
 #include <type_traits>
 
 #include "seq_common.cuh"
@@ -42,8 +48,8 @@ struct ConvArgs {
 //
 // Tokens come through a ring in shared memory, kU of them on their way to every thread by
 // asynchronous copies. A thread reads only what it has copied itself, so there are no
-// barriers; held in registers, 8 tokens cost the warps that hide the latency (gradient
-// 186 us with 2 channels a thread and 24 warps, 117 us with 16 warps and no spills).
+// barriers; held in registers, the 8 tokens of 4 channels cost the warps that hide the
+// latency (256 x 128 x 1024: forward 67 us, gradient 186 us; with the ring 41 and 110 us).
 constexpr int kThreads = 256, kU = 8;
 template <int V> constexpr int kPairs = (V + 1) / 2;
 template <int V> struct Pairs { f2 p[kPairs<V>]; };

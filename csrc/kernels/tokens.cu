@@ -104,6 +104,8 @@ template <typename V> __device__ __forceinline__ V warp_scan(V v, int lane) {   
 }
 
 // ---- up to 32 candidates: one warp, a lane each ---------------------------------------
+// Ranks and the weight before a candidate by looking at every other lane in turn: 2 sizes'
+// shuffles a head, all in registers (2048 rows of six heads 8.9 us, 410 KB: latency).
 template <typename T> __global__ void __launch_bounds__(128) small_kernel(TokenArgs a) {
   const int64_t id = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
@@ -150,13 +152,17 @@ template <typename T> __global__ void __launch_bounds__(128) small_kernel(TokenA
 // ---- many candidates: a cluster of CS blocks, the row's slices in shared memory -----------
 // One exponential per candidate: e is kept in shared memory in the logit's place, and all
 // later passes work on its bits (e orders the candidates except where several logits share
-// an e; only there the logits are looked at again). What bounds it is the number of
-// instructions for a candidate, about 25 for the exponential and the weight, 20 for the
-// histogram and 15 for the sums of what is kept, and the waits at the cluster's barriers.
+// an e; only there the logits are looked at again).
 //
 // With enough rows to fill the GPU a row is one block's (kStream): no barriers between
 // blocks; the row is read again from the L2 cache and its exponentials made again instead
 // of being kept (a slice of the whole row would not fit).
+//
+// Measured on a B200: 256 rows of 131072 bf16 under top_p 155 us (67 MB; without a limit
+// 60 us), as clusters 325 us; one row of 32768 f32 under top_k and top_p 18 us, 64 rows of
+// them 24 us. What bounds many rows is instructions, 106 for a candidate under top_p (two
+// exponentials, two weights in whole numbers, one place in the histogram) at 0.7 a cycle;
+// what bounds a few rows is the cluster's barriers, about ten of a microsecond each.
 constexpr int kMaxCluster = 16, kMaxSlice = 16384, kMaxStream = kMaxCluster * kMaxSlice;
 constexpr int kList = 512;
 template <bool kStream> struct Large {
