@@ -3,14 +3,16 @@
     python bench/profile_kernels.py --only march|conv1_fwd|conv2_dgrad|fc_wgrad|col2im|im2col|conv1_ifwd|
                                            conv1_iwgrad|conv2_ifwd|
                                            conv2_iwgrad|conv2_idgrad|conv3_ifwd|conv3_iwgrad|conv3_idgrad|sample|gae|
-                                           ppo_loss|reward|adam|p2p1|edt|geodesic|geodesic_race|surfnz|framestack [--reps 2]
+                                           ppo_loss|reward|adam|p2p1|edt|geodesic|geodesic_race|surfnz|framestack|
+                                           seq_conv|seq_scan|seq_scan_step|sample_tokens [--reps 2]
 
 Each case builds its inputs (a few GB on the device at most, larger than L2
 where the kernel streams memory), warms up once, then launches the kernel
 ``--reps`` times and prints the CUDA-event time per launch. Pair it with
 ``ncu --set full --clock-control none -k regex:<kernel> -s 1 -c 1``.
 Shapes: the benchmark's 2048 envs x 128 x 64 rays, 2048-row sampling,
-128 x 2048 GAE, 32,768-row loss; the convolution cases use 4,096 images
+128 x 2048 GAE, 32,768-row loss; a rollout's rows (256 x 128) for the sequence operators, forward
+and gradient in one case; the convolution cases use 4,096 images
 (operands still larger than L2) to keep the captures small.
 """
 from __future__ import annotations
@@ -287,6 +289,35 @@ def main():
         info["voxels"] = nx * ny * nz
         info["dims"] = [nx, ny, nz]
         info["passes"] = st.get("passes")
+    elif k in ("seq_conv", "seq_scan"):
+        from surfb200.ops import ssm
+        bf = torch.bfloat16
+        B, T, D = (256, 128, 1024) if k == "seq_conv" else (256, 128, 512)
+        xz = torch.randn(B, T, 2 * D, device=dev).to(bf)
+        x, z = xz[..., :D], xz[..., D:]
+        dy = torch.randn(B, T, D, device=dev).to(bf)
+        if k == "seq_conv":
+            w, b = torch.randn(D, 4, device=dev) / 2, torch.zeros(D, device=dev)
+            info["ms"] = _time(lambda: ssm.causal_conv(x, w, b), args.reps)
+            info["grad_ms"] = _time(lambda: ssm.causal_conv_grad(dy, x, w, b), args.reps)
+        else:
+            A = -torch.arange(1, 17, device=dev).float().expand(D, 16).contiguous()
+            bc = torch.randn(B, T, 1, 32, device=dev).to(bf)
+            a = (x, (torch.randn(B, T, D, device=dev) / 2 - 4).to(bf), A, bc[..., :16], bc[..., 16:])
+            saved = ssm.selective_scan(*a, z=z, train=True).saved
+            info["ms"] = _time(lambda: ssm.selective_scan(*a, z=z, train=True), args.reps)
+            info["grad_ms"] = _time(lambda: ssm.selective_scan_grad(dy, *a, z=z, saved=saved), args.reps)
+    elif k == "seq_scan_step":
+        from surfb200.ops import ssm
+        bf = torch.bfloat16
+        x, dt, z = (torch.randn(2048, 1024, device=dev).to(bf) for _ in range(3))
+        A = -torch.arange(1, 17, device=dev).float().expand(1024, 16).contiguous()
+        bc, pool = torch.randn(2048, 1, 32, device=dev).to(bf), torch.randn(2048, 1024, 16, device=dev)
+        info["ms"] = _time(lambda: ssm.selective_scan_step(x, dt, A, bc[..., :16], bc[..., 16:], pool, z=z), args.reps)
+    elif k == "sample_tokens":
+        from surfb200.ops.tokens import sample_tokens
+        logits, u = (2.5 * torch.randn(256, 131072, device=dev)).to(torch.bfloat16), torch.rand(256, 1, device=dev)
+        info["ms"] = _time(lambda: sample_tokens(logits, u, top_p=0.95), args.reps)
     elif k == "geodesic":
         from surfb200.ops.geodesic import geodesic
         occ = torch.zeros(128, 256, 256, dtype=torch.uint8, device=dev)

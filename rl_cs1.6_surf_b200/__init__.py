@@ -7,8 +7,10 @@ Layers (bottom up):
                 procedural BSP maps, zones, spawn pools.
 * ``ops``       hand-written sm_100a CUDA kernels (SDF depth render, SDF/EDT
                 bake, geodesic bake, tcgen05 GEMMs, action sampling, GAE,
-                PPO loss, curiosity hash, fused Adam) behind a C ABI.
-* ``models``    the policy networks (Nature CNN vision policy, eyeless MLP).
+                PPO loss, curiosity hash, fused Adam, causal convolution,
+                selective scan, answer sampling) behind a C ABI.
+* ``models``    the policy networks (Nature CNN vision policy, eyeless MLP,
+                memory core).
 * ``rewards``   race / progress / coverage / speed rewards (GPU + CPU oracle).
 * ``parallel``  data parallelism over NVLink: NCCL baseline and fused P2P
                 all-reduce + clip + Adam, curiosity-count and moment merges.
