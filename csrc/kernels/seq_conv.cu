@@ -11,8 +11,8 @@
 // window slides through registers, a thread owning neighbouring channels over a
 // stretch of tokens, so each x is read once (plus W - 1 of every stretch).
 //
-// Measured on a B200, bf16, W = 4: forward 256 x 128 x 1024 37 us (134 MB, 3.6 TB/s),
-// gradient 82 us (201 MB, 2.5 TB/s), a prompt of 16385 x 1024 18 us (67 MB, 3.7 TB/s); one
+// Measured on a B200, bf16, W = 4, with resets: forward 256 x 128 x 1024 32 us (134 MB, 4.2
+// TB/s), gradient 75 us (201 MB, 2.7 TB/s), a prompt of 16385 x 1024 18 us (67 MB, 3.8 TB/s); one
 // token of 64 envs 2.5 us. What bounds them is instructions at 16 warps on an SM (14 an
 // element in the forward, 36 in the gradient, a sigmoid's 5 and its derivative's 10 among
 // them): with the SiLU left out they take 27 and 54 us.
@@ -40,6 +40,7 @@ struct ConvArgs {
   int B, T, D, silu;
   int tt, chunks;             // tokens of a stretch, stretches of a row
 };
+static_assert(sizeof(ConvArgs) == 18 * 8 + 6 * 4, "as the caller packs it");
 
 // Channels of a thread: in whole sequences 16 bytes of them in the forward, 8 in the
 // gradient (its weights, sums and pending dx fill the registers otherwise), 4 bytes where

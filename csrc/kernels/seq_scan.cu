@@ -358,6 +358,7 @@ struct StepArgs {
   int rows, dim, N, G, softplus, n_slots;
   int whole, pad;                              // rows of B and C start on 4-element boundaries, N is a multiple of 4
 };
+static_assert(sizeof(StepArgs) == 21 * 8 + 8 * 4, "as the caller packs it");
 
 // Four neighbouring values of a row of B or C as they are in memory, zeros past the N-th
 template <typename T> struct Quad {
@@ -481,8 +482,4 @@ SURF_EXPORT int surf_seq_scan_threads(int per_group, int groups, int N) {
     const int threads = small_blocks<LN>(per_group) ? kSmallBlock<LN> : kScanBlock<LN>;
     return static_cast<int>(surfk::ceil_div(per_group, scan_channels<LN>(threads))) * groups * threads;
   });
-}
-
-SURF_EXPORT int surf_seq_args_size(int which) {
-  return static_cast<int>(which == 0 ? sizeof(ScanArgs) : sizeof(StepArgs));
 }

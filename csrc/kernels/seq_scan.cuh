@@ -29,6 +29,7 @@ struct ScanArgs {
   int chunk, chunks;                           // tokens of a chunk (a multiple of 16), chunks of a row
   int mode_d, mode_n;                          // how rows of channels and of states are copied (copy_rows)
 };
+static_assert(sizeof(ScanArgs) == 48 * 8 + 10 * 4, "as the caller packs it");
 
 // A warp's 32 lanes are 32 / LN channel rows of LN lanes; a lane holds 4 states of
 // each of K channels, so 4 * LN >= N states of a channel sit in LN neighbouring lanes.

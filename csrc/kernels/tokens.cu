@@ -38,6 +38,7 @@ struct TokenArgs {
   int rows, heads;
   int offset[kMaxHeads], size[kMaxHeads];
 };
+static_assert(sizeof(TokenArgs) == 9 * 8 + 6 * 4 + 2 * kMaxHeads * 4, "as the caller packs it");
 
 struct Rule {                 // of one row
   float inv, min_p;
@@ -159,8 +160,8 @@ template <typename T> __global__ void __launch_bounds__(128) small_kernel(TokenA
 // of being kept (a slice of the whole row would not fit).
 //
 // Measured on a B200: 256 rows of 131072 bf16 under top_p 155 us (67 MB; without a limit
-// 60 us); at a temperature of 0.7 133 us, as clusters 215 us; one row of 32768 f32 under top_k and top_p 18 us, 64 rows of
-// them 24 us. What bounds many rows is instructions, 106 for a candidate under top_p (two
+// 60 us), as clusters 325 us; at a temperature of 0.7 133 us, as clusters 215 us; one row of
+// 32768 f32 under top_k and top_p 18 us, 64 rows of them 24 us. What bounds many rows is instructions, 106 for a candidate under top_p (two
 // exponentials, two weights in whole numbers, one place in the histogram) at 0.7 a cycle;
 // what bounds a few rows is the cluster's barriers, about ten of a microsecond each.
 constexpr int kMaxCluster = 16, kMaxSlice = 16384, kMaxStream = kMaxCluster * kMaxSlice;
