@@ -43,7 +43,6 @@ _lib.register(SLIB, {
     "surf_seq_scan_grad_blocks": (_I, [_I, _I]),
     "surf_seq_scan_threads": (_I, [_I, _I, _I]),
     "surf_seq_scan_step": (_I, [c_char_p, _I, _V]),
-    "surf_seq_args_size": (_I, [_I]),
 })
 _lib._KERNELS_PER_CALL["surf_seq_conv_grad"] = 2
 
@@ -152,9 +151,13 @@ def _conv_check(what, x, weight, bias, state, reset, lengths):
 def _stretches(b: int, t: int, groups: int):
     """(tokens of a stretch, stretches of a row, rows of blocks) of the convolution for
     ``groups`` threads across a row: the longest stretch (each reads width - 1 tokens of its
-    neighbour again) that still gives every SM 512 threads, two blocks on an SM to take them."""
-    tt = 64
-    while tt > 8 and b * -(-t // tt) * groups < 148 * 512:
+    neighbour again) that still gives every SM 256 threads, two blocks on an SM to take them.
+
+    Forward and gradient, bf16, us at 128, 256 and 512 threads: 256 x 128 x 1024 35 + 62,
+    31 + 62, 34 + 66; 1 x 16385 x 1024 21 + 43, 18 + 36, 19 + 39. Stretches of at most 64
+    tokens take 58 + 124 at 256 x 512 x 512, of 128 56 + 118, of 256 64 + 113."""
+    tt = 128
+    while tt > 8 and b * -(-t // tt) * groups < 148 * 256:
         tt //= 2
     chunks = max(1, -(-t // tt))
     bx = min(32, 1 << (groups - 1).bit_length())
@@ -282,14 +285,25 @@ def _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths):
 
 
 def _chunks(b: int, t: int, d: int, n: int, g: int):
-    """(tokens of a chunk, chunks): a row is cut only where its channels do not fill the GPU."""
+    """(tokens of a chunk, chunks): a row is cut where its channels leave room on the GPU for
+    three times as many threads (512 an SM), since the pass that leaves the chunks' ends costs
+    nearly half of the scan itself; a chunk has 16 tokens at least. A row below 128 is done
+    before the host has launched the two kernels more: 5 x 77 x 194 f32 cut and whole 20 + 39
+    and 23 + 52 us on the device, but 41 + 74 and 28 + 59 us a call.
+
+    Forward and gradient, bf16, 16 states, us whole and cut: 64 x 1024 x 512 in 2 323 + 797 and
+    467 + 1045; 48 rows in 3 323 + 795 and 312 + 716; 16 x 512 x 512 in 8 133 + 266 and 69 + 152;
+    16 x 128 x 512 in 8 36 + 69 and 28 + 55. Chunks of 64, 32 and 16 tokens at 4 x 512 x 256:
+    36 + 55, 24 + 36, 20 + 32. 256 and 1024 threads an SM at 2 x 4096 x 1024: 137 + 261 and
+    112 + 257, against 110 + 249."""
     threads = b * _lib.lib(SLIB).surf_seq_scan_threads(d // g, g, n)
-    want = max(1, min(148 * 512 // threads if threads else 1, t // 64))
-    if want <= 1:
-        return max(16, -(-t // 16) * 16), 1
-    chunk = -(-t // want)
-    chunk = -(-chunk // 16) * 16
-    return chunk, -(-t // chunk)
+    want = min(148 * 512 // threads if threads else 1, t // 16)
+    if want >= 3 and t >= 128:
+        chunk = -(-t // want)
+        chunk = -(-chunk // 16) * 16
+        if t > 2 * chunk:
+            return chunk, -(-t // chunk)
+    return max(16, -(-t // 16) * 16), 1
 
 
 def _workspace(dev, *floats):
