@@ -121,11 +121,16 @@ def _bits(size: int, *tensors) -> int:
     return bits
 
 
-def _piece(cols: int, size: int, *tensors) -> int:
-    """Bytes of the pieces that rows of ``cols`` elements may be copied in (copy_rows): 16
-    or 4 where the row's length, every base and every stride is a multiple of it, else 0."""
-    bits = _bits(size, *tensors) | cols * size
+def _piece(bits: int) -> int:
+    """Bytes of the pieces that rows may be copied in (copy_rows): 16 or 4 where the row's
+    length, every base and every stride, whose low bits these are, is a multiple of it, else 0."""
     return 16 if bits & 15 == 0 else 4 if bits & 3 == 0 else 0
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A new dense tensor of ``t``'s shape and type (half the host time of ``torch.empty``,
+    of which a training step needs a dozen)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 # ---- causal convolution -----------------------------------------------------------
@@ -174,10 +179,10 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     code, e, at, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
     weight = _even(weight)
     if out is None:
-        out = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+        out = _like(x)
     else:
         _tokens(what, "out", out, x.shape, x.dtype, at)
-    final = torch.empty((b, w - 1, d), dtype=x.dtype, device=x.device)
+    final = x.new_empty((b, w - 1, d))
     if b == 0 or d == 0:
         return out, final
     bits = _bits(e, x, out, state) | d * e
@@ -201,17 +206,16 @@ def causal_conv_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bi
     _tokens(what, "dy", dy, x.shape, x.dtype, at)
     _dense(what, "dfinal", dfinal, (b, w - 1, d), x.dtype, at)
     weight = _even(weight)
-    dev = x.device
-    dx = torch.empty((b, t, d), dtype=x.dtype, device=dev)
-    dstate = torch.empty((b, w - 1, d), dtype=x.dtype, device=dev) if state is not None else None
+    dx = _like(x)
+    dstate = torch.empty_like(state) if state is not None else None
     if b == 0 or d == 0:
         return ConvGrads(dx, torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dstate)
-    dw = torch.empty((d, w), dtype=torch.float32, device=dev)
-    db = torch.empty(d, dtype=torch.float32, device=dev) if bias is not None else None
+    dw = torch.empty_like(weight)
+    db = torch.empty_like(bias) if bias is not None else None
     bits = _bits(e, x, dy, state, dfinal) | d * e
     size = 8 if bits & 7 == 0 else 4 if bits & 3 == 0 else 2
     tt, chunks, rows = _stretches(b, t, d * e // size)
-    part = torch.empty((rows, w + 1, d), dtype=torch.float32, device=dev)
+    part = weight.new_empty((rows, w + 1, d))
     args = _CONV.pack(_p(x), dy.data_ptr(), _p(state), _p(dfinal), _p(weight), _p(bias), _p(reset), _p(lengths),
                       dx.data_ptr(), _p(dstate), part.data_ptr(), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1),
                       t * d, d, t, b, t, d, int(silu), tt, chunks)
@@ -244,7 +248,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     if slots is None and state.shape[0] < r:
         raise ValueError(f"{what}: {r} rows, but {state.shape[0]} slots")
     if out is None:
-        out = torch.empty((r, d), dtype=x.dtype, device=dev)
+        out = _like(x)
     else:
         _tokens(what, "out", out, x.shape, x.dtype, at)
     if r == 0 or d == 0:
@@ -270,10 +274,12 @@ def _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths):
     if B.dim() != 4 or B.shape[2] < 1 or d % B.shape[2]:
         raise ValueError(f"{what}: B must be [batch, tokens, groups, states], its groups dividing the channels")
     g = B.shape[2]
-    for name, v in (("x", x), ("dt", dt), ("z", z)):
-        _tokens(what, name, v, (b, t, d), x.dtype, at)
-    for name, v in (("B", B), ("C", C)):
-        _tokens(what, name, v, (b, t, g, n), x.dtype, at)
+    dtype, shape = x.dtype, x.shape
+    _tokens(what, "x", x, shape, dtype, at)
+    _tokens(what, "dt", dt, shape, dtype, at)
+    _tokens(what, "z", z, shape, dtype, at)
+    _tokens(what, "B", B, (b, t, g, n), dtype, at)
+    _tokens(what, "C", C, (b, t, g, n), dtype, at)
     f32 = torch.float32
     _dense(what, "A", A, (d, n), f32, at)
     _dense(what, "D", D, (d,), f32, at)
@@ -306,13 +312,28 @@ def _chunks(b: int, t: int, d: int, n: int, g: int):
     return max(16, -(-t // 16) * 16), 1
 
 
-def _workspace(dev, *floats):
-    """One allocation for pieces of so many 32-bit numbers: (it, the pieces' addresses)."""
+def _scan_inputs(x, dt, z, B, C):
+    """(addresses, strides of rows, what the strides and addresses of x, dt and z, and of B
+    and C, have in their low bits, in bytes) of the scan's tokens, in the kernel's order."""
+    e = x.element_size()
+    px, pdt, pz, pB, pC = x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr()
+    x0, x1, _ = x.stride()
+    t0, t1, _ = dt.stride()
+    z0, z1, _ = (0, 0, 0) if z is None else z.stride()
+    B0, B1, B2, _ = B.stride()
+    C0, C1, C2, _ = C.stride()
+    return ((px, pdt, pz, pB, pC), (x0, x1, t0, t1, z0, z1, B0, B1, B2, C0, C1, C2),
+            px | pdt | pz | (x0 | x1 | t0 | t1 | z0 | z1) * e, pB | pC | (B0 | B1 | B2 | C0 | C1 | C2) * e)
+
+
+def _workspace(like, *floats):
+    """One allocation for pieces of so many 32-bit numbers, by ``like``'s device: (it, the
+    pieces' addresses)."""
     at, total = [], 0
     for n in floats:
         at.append(4 * total)
         total += (n + 3) // 4 * 4
-    ws = torch.empty(total, dtype=torch.float32, device=dev)
+    ws = like.new_empty(total)
     base = ws.data_ptr()
     return ws, [base + o for o in at]
 
@@ -331,25 +352,25 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     what = "selective_scan"
     code, e, at, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
     A, state = _even(A), _even(state)
-    dev = x.device
     if out is None:
-        out = torch.empty((b, t, d), dtype=x.dtype, device=dev)
+        out = _like(x)
     else:
         _tokens(what, "out", out, x.shape, x.dtype, at)
-    final = torch.empty((b, d, n), dtype=torch.float32, device=dev)
-    saved = torch.empty((b, -(-t // SAVE_EVERY), d, n), dtype=torch.float32, device=dev) if train else None
+    final = A.new_empty((b, d, n))
+    saved = A.new_empty((b, -(-t // SAVE_EVERY), d, n)) if train else None
     if b == 0 or d == 0:
         return Scan(out, final, saved)
     chunk, chunks = _chunks(b, t, d, n, g)
-    ws, (carry, sumd, cut) = _workspace(dev, b * chunks * d * n, b * chunks * d, b * chunks) if chunks > 1 else (None, (0, 0, 0))
+    ws, (carry, sumd, cut) = _workspace(A, b * chunks * d * n, b * chunks * d, b * chunks) if chunks > 1 else (None, (0, 0, 0))
+    where, strides, bits_d, bits_n = _scan_inputs(x, dt, z, B, C)
+    o0, o1, _ = out.stride()
+    to = out.data_ptr()
     args = _SCAN.pack(
-        x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), 0, A.data_ptr(), _p(D), _p(dt_bias), _p(state), 0,
-        _p(reset), _p(lengths), out.data_ptr(), final.data_ptr(), _p(saved), carry, sumd, cut,
+        *where, 0, A.data_ptr(), _p(D), _p(dt_bias), _p(state), 0,
+        _p(reset), _p(lengths), to, final.data_ptr(), _p(saved), carry, sumd, cut,
         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
-        x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
-        0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
-        0, 0, out.stride(0), out.stride(1), t, b, t, d, n, g, int(softplus), chunk, chunks,
-        _piece(d // g, e, x, dt, z, out), _piece(n, e, B, C))
+        *strides, 0, 0, o0, o1, t, b, t, d, n, g, softplus, chunk, chunks,
+        _piece(bits_d | to | (o0 | o1 | d // g) * e), _piece(bits_n | n * e))
     launch(_lib.lib(SLIB).surf_seq_scan, "surf_seq_scan", at, args, code)
     del ws                                     # the stream's next user comes after the launch
     if chunks > 1:
@@ -369,7 +390,7 @@ def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A
     input that was None."""
     what = "selective_scan_grad"
     code, e, at, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
-    dev, f32 = x.device, torch.float32
+    f32 = torch.float32
     _tokens(what, "dout", dout, x.shape, x.dtype, at)
     _dense(what, "dfinal", dfinal, (b, d, n), f32, at)
     if saved is None:
@@ -377,13 +398,9 @@ def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A
     _dense(what, "saved", saved, (b, -(-t // SAVE_EVERY), d, n), f32, at)
     A, saved, dfinal = _even(A), _even(saved), _even(dfinal)
 
-    def like(v, shape, dtype):
-        return None if v is None else torch.empty(shape, dtype=dtype, device=dev)
-
-    dx, ddt, dz = (like(v, (b, t, d), x.dtype) for v in (x, dt, z))
-    dB, dC = (like(v, (b, t, g, n), x.dtype) for v in (B, C))
-    dA, dD, dbias = like(A, (d, n), f32), like(D, (d,), f32), like(dt_bias, (d,), f32)
-    dstate = like(state, (b, d, n), f32)
+    dx, ddt, dz = _like(x), _like(dt), None if z is None else _like(z)
+    dB, dC, dA = _like(B), _like(C), torch.empty_like(A)
+    dD, dbias, dstate = (None if v is None else torch.empty_like(v) for v in (D, dt_bias, state))
     if b == 0 or d == 0:
         for v in (dA, dD, dbias):
             if v is not None:
@@ -393,16 +410,17 @@ def selective_scan_grad(dout: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A
     L = _lib.lib(SLIB)
     split = b * chunks if chunks > 1 else 0
     ws, (part_bc, part_a, part_v, carry, sumd, cut) = _workspace(
-        dev, L.surf_seq_scan_grad_blocks(d // g, n) * b * t * g * 2 * n, b * chunks * d * n, b * chunks * d * 2,
+        A, L.surf_seq_scan_grad_blocks(d // g, n) * b * t * g * 2 * n, b * chunks * d * n, b * chunks * d * 2,
         split * d * n, split * d, split)
+    where, strides, bits_d, bits_n = _scan_inputs(x, dt, z, B, C)
+    o0, o1, _ = dout.stride()
+    of = dout.data_ptr()
     args = _SCAN.pack(
-        x.data_ptr(), dt.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), dout.data_ptr(), A.data_ptr(), _p(D), _p(dt_bias),
+        *where, of, A.data_ptr(), _p(D), _p(dt_bias),
         _p(state), _p(dfinal), _p(reset), _p(lengths), 0, 0, saved.data_ptr(), carry, sumd, cut,
         dx.data_ptr(), ddt.data_ptr(), _p(dz), dB.data_ptr(), dC.data_ptr(), part_bc, part_a, part_v, dA.data_ptr(), _p(dD), _p(dbias), _p(dstate),
-        x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), 0 if z is None else z.stride(0),
-        0 if z is None else z.stride(1), B.stride(0), B.stride(1), B.stride(2), C.stride(0), C.stride(1), C.stride(2),
-        dout.stride(0), dout.stride(1), 0, 0, t, b, t, d, n, g, int(softplus), chunk, chunks,
-        _piece(d // g, e, x, dt, z, dout), _piece(n, e, B, C))
+        *strides, o0, o1, 0, 0, t, b, t, d, n, g, softplus, chunk, chunks,
+        _piece(bits_d | of | (o0 | o1 | d // g) * e), _piece(bits_n | n * e))
     launch(L.surf_seq_scan_grad, "surf_seq_scan_grad", at, args, code)
     del ws
     _lib.add_launches(3 if chunks > 1 else 1)
@@ -448,7 +466,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     if slots is None and pools < r:
         raise ValueError(f"{what}: {r} rows, but {pools} slots")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
+        out = _like(x)
     else:
         _tokens(what, "out", out, shape, dtype, at)
     if r == 0 or d == 0:

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import struct
 from ctypes import c_char_p
+from itertools import accumulate
 from typing import Optional, Sequence
 
 import torch
@@ -86,13 +87,13 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
         if t is not None and (t.shape != (rows, n) or t.dtype != dt or t.device != dev or not t.is_contiguous()):
             raise ValueError(f"sample_tokens: {name} must be a contiguous {dt} tensor [{rows}, {n}] on {dev}")
     if out is None:
-        out = torch.empty((rows, n), dtype=torch.int32, device=dev)
+        out = torch.empty_like(u, dtype=torch.int32)
     if logp is None:
-        logp = torch.empty((rows, n), dtype=f32, device=dev)
+        logp = torch.empty_like(u)
     if rows == 0:
         return out, logp
     pad = (0,) * (MAX_HEADS - n)
-    offsets = tuple(sum(sizes[:i]) for i in range(n))
+    offsets = (0, *accumulate(sizes[:-1]))
     args = _ARGS.pack(logits.data_ptr(), u.data_ptr(), tp, pp, mp, kp, out.data_ptr(), logp.data_ptr(), logits.stride(0),
                       t0, p0, m0, min(int(k0), 2 ** 31 - 1), rows, n, *offsets, *pad, *sizes, *pad)
     launch(_lib.lib(SLIB).surf_sample_tokens, "surf_sample_tokens", logits.get_device(), args, code, widest)
