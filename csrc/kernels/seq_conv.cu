@@ -15,7 +15,7 @@
 // TB/s), gradient 75 us (201 MB, 2.7 TB/s), a prompt of 16385 x 1024 18 us (67 MB, 3.8 TB/s); one
 // token of 64 envs 2.5 us. What bounds them is instructions at 16 warps on an SM (14 an
 // element in the forward, 36 in the gradient, a sigmoid's 5 and its derivative's 10 among
-// them): with the SiLU left out they take 27 and 54 us.
+// them): the SiLU takes 10 and 28 us of them.
 #include <type_traits>
 
 #include "seq_common.cuh"
