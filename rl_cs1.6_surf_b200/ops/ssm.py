@@ -303,7 +303,7 @@ def _chunks(b: int, t: int, d: int, n: int, g: int):
     36 + 55, 24 + 36, 20 + 32. 256 and 1024 threads an SM at 2 x 4096 x 1024: 137 + 261 and
     112 + 257, against 110 + 249."""
     threads = b * _lib.lib(SLIB).surf_seq_scan_threads(d // g, g, n)
-    want = min(148 * 512 // threads if threads else 1, t // 16)
+    want = min(148 * 512 // threads if threads else 1, -(-t // 16))
     if want >= 3 and t >= 128:
         chunk = -(-t // want)
         chunk = -(-chunk // 16) * 16

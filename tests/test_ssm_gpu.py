@@ -88,6 +88,20 @@ def test_conv_and_gradient(case, dtype):
     assert all(torch.equal(p, q) for p, q in zip(g, again))
 
 
+@pytest.mark.parametrize("t", [128, 129])
+def test_conv_over_the_longest_stretches(t):
+    """As many rows as fill the GPU without cutting: stretches of 128 tokens, one more behind."""
+    assert ssm._stretches(304, t, 128)[0] == 128
+    c = _conv_case(304, t, 512, 4, True, True, torch.float32)
+    kw = dict(state=c["state"], reset=c["reset"], lengths=c["lengths"])
+    y, final = ssm.causal_conv(c["x"], c["weight"], c["bias"], **kw)
+    g = ssm.causal_conv_grad(c["dy"], c["x"], c["weight"], c["bias"], dfinal=c["dfinal"], **kw)
+    ey, ef, eg = _conv_exact(c)
+    assert rel(y, ey) <= 1e-6 and torch.equal(final.double(), ef.detach())
+    assert rel(g.dx, eg[0]) <= 1e-6 and rel(g.dstate, eg[3]) <= 1e-6
+    assert rel(g.dweight, eg[1]) <= 1e-5 and rel(g.dbias, eg[2]) <= 1e-5
+
+
 def test_conv_without_state_bias_or_silu():
     c = _conv_case(2, 37, 20, 3, True, False, torch.float32)
     y, final = ssm.causal_conv(c["x"], c["weight"], reset=c["reset"], silu=False)
@@ -186,6 +200,21 @@ def test_scan_and_gradient(case, dtype):
                                     z=c["z"], dt_bias=c["dt_bias"], state=c["state"], reset=c["reset"],
                                     lengths=c["lengths"], dfinal=c["dfinal"])
     assert all(torch.equal(p, q) for p, q in zip(g, again))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,t,chunks", [(2, 127, 1), (2, 128, 8), (2, 129, 9), (2, 145, 10), (19, 200, None)])
+def test_scan_about_the_rule_that_cuts(b, t, chunks, dtype):
+    """Lengths where rows begin to be cut, a last chunk of one token, few and many chunks."""
+    d = 64 if b == 2 else 1000
+    got = ssm._chunks(b, t, d, 16, 1)[1]
+    assert got == chunks if chunks else got != 2
+    c = _scan_case(b, t, d, 16, 1, True, True, dtype)
+    r, g = _scan_run(c)
+    out, final, grads = _scan_exact(c)
+    assert rel(r.out, out) <= TOL[dtype] and rel(r.final, final) <= TOL[torch.float32]
+    for k, v in _named(g).items():
+        assert rel(v, grads[k]) <= TOL[v.dtype], k
 
 
 @pytest.mark.parametrize("softplus", [True, False])

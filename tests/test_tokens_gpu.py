@@ -102,6 +102,26 @@ def test_many_long_rows(dtype):
         _same(z, u, **rule)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_long_rows_under_a_count(dtype):
+    """Most candidates far below the limit: one kept per row, infinite ones, a limit on the
+    boundary of two equal ones, per-row limits of which some are none."""
+    gen = torch.Generator("cuda").manual_seed(4)
+    n, vocab = 149, 12345
+    z = torch.randn(n, vocab, generator=gen, device="cuda").to(dtype)
+    z[0, 77] = z[0, 9000] = float("inf")
+    z[1, 1:] = float("-inf")
+    z[2, 12344] = 30.0
+    z[3, 5:8] = 20.0
+    z[4] = -1000.0
+    z[4, 128:256] = 1000.0
+    u = torch.rand(n, 1, generator=gen, device="cuda")
+    k = torch.arange(n, device="cuda", dtype=torch.int32) % 7
+    for rule in (dict(top_k=2), dict(top_k=k), dict(top_k=k, temperature=0.05), dict(top_k=64, top_p=0.5, min_p=0.01),
+                 dict(top_k=12000)):
+        _same(z, u, **rule)
+
+
 def test_limits_per_row():
     gen = torch.Generator("cuda").manual_seed(1)
     z = 2 * torch.randn(8, 700, generator=gen, device="cuda")
