@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 from ctypes import c_double, c_float, c_int, c_int64, c_void_p
 
+import numpy as np
 import torch
 
 from .._native import load
@@ -129,3 +130,47 @@ def add_launches(n: int) -> None:
 def require_cuda(t: torch.Tensor, what: str) -> None:
     if not t.is_cuda:
         raise KernelError(f"{what}: the CUDA kernel needs CUDA tensors (use the *_reference CPU oracle on CPU)")
+
+
+class _Extent:
+    """Where a tensor's elements lie, for numpy's overlap test; the memory is never touched."""
+
+    def __init__(self, t: torch.Tensor):
+        e = t.element_size()
+        self.__array_interface__ = {"version": 3, "typestr": f"|V{e}", "data": (t.data_ptr(), False),
+                                    "shape": tuple(t.shape), "strides": tuple(s * e for s in t.stride())}
+
+
+def _span(t: torch.Tensor) -> tuple:
+    """(first address, the one behind the last) of a tensor's elements."""
+    at = t.data_ptr()
+    if t.is_contiguous():
+        return at, at + t.nbytes
+    return at, at + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors share an element's memory: exact for strided views, so that
+    interleaved columns of one buffer do not count."""
+    if not a.numel() or not b.numel():
+        return False
+    return bool(np.shares_memory(np.asarray(_Extent(a)), np.asarray(_Extent(b))))
+
+
+def require_apart(what: str, name: str, out: torch.Tensor, inputs: dict, in_place: tuple = ()) -> None:
+    """Refuse an ``out`` whose elements share memory with one another or with an input: other
+    threads read the inputs while it is written. It may be one of the inputs named in
+    ``in_place`` itself, where a thread reads an element before it writes it."""
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError(f"{what}: {name} has elements that share memory")
+    lo, hi = _span(out)
+    for key, t in inputs.items():
+        if not isinstance(t, torch.Tensor):
+            continue
+        at, end = _span(t)
+        if end <= lo or hi <= at:
+            continue
+        if key in in_place and t.data_ptr() == out.data_ptr() and t.shape == out.shape and t.stride() == out.stride():
+            continue
+        if overlap(out, t):
+            raise ValueError(f"{what}: {name} shares memory with {key}")

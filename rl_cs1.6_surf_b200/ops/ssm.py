@@ -174,7 +174,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                 lengths: Optional[torch.Tensor] = None, silu: bool = True, out: Optional[torch.Tensor] = None):
     """(y [B, T, D], final [B, W-1, D]): y[t] = silu(bias + sum_k weight[:, k] x[t - (W-1) + k])
     over the tokens that t sees; ``state`` and ``final`` hold the W - 1 tokens before
-    and behind the row, oldest first."""
+    and behind the row, oldest first. ``out`` must not share memory with an input: a token is
+    read by the stretches of the W - 1 behind it too."""
     what = "causal_conv"
     code, e, at, b, t, d, w = _conv_check(what, x, weight, bias, state, reset, lengths)
     weight = _even(weight)
@@ -182,6 +183,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         out = _like(x)
     else:
         _tokens(what, "out", out, x.shape, x.dtype, at)
+        _lib.require_apart(what, "out", out, dict(x=x, weight=weight, bias=bias, state=state, reset=reset, lengths=lengths))
     final = x.new_empty((b, w - 1, d))
     if b == 0 or d == 0:
         return out, final
@@ -228,7 +230,8 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token x [R, D] for each of R envs: y [R, D]. ``state`` [S, W-1, D] is the pool
     of windows, ``slots`` [R] (int32) each row's place in it (None: row r is slot r; below
-    0: no env, its output is zero), moved on in place. No two rows may name one slot."""
+    0: no env, its output is zero), moved on in place. No two rows may name one slot. ``out``
+    may be x itself, and shares no memory with an input otherwise."""
     what = "causal_conv_step"
     _lib.require_cuda(x, what)
     if x.dim() != 2:
@@ -251,6 +254,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
         out = _like(x)
     else:
         _tokens(what, "out", out, x.shape, x.dtype, at)
+        _lib.require_apart(what, "out", out, dict(x=x, weight=weight, bias=bias, state=state, reset=reset, slots=slots), ("x",))
     if r == 0 or d == 0:
         return out
     vec = (_bits(e, x, out, state) | d * e) % (4 * e) == 0
@@ -348,7 +352,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     channels shares a row of them), A [D, N]: ``out`` [B, T, D] and ``final`` [B, D, N].
     delta = softplus(dt + dt_bias), or the sum itself with ``softplus=False``. ``train``
     keeps in ``saved`` the states that ``selective_scan_grad`` starts from: 4 D N bytes
-    for every 8 tokens."""
+    for every 8 tokens. ``out`` may be x, dt or z itself, and shares no memory otherwise."""
     what = "selective_scan"
     code, e, at, b, t, d, n, g = _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths)
     A, state = _even(A), _even(state)
@@ -356,6 +360,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         out = _like(x)
     else:
         _tokens(what, "out", out, x.shape, x.dtype, at)
+        _lib.require_apart(what, "out", out, dict(x=x, dt=dt, z=z, A=A, B=B, C=C, D=D, dt_bias=dt_bias, state=state, reset=reset,
+                                                  lengths=lengths), ("x", "dt", "z"))
     final = A.new_empty((b, d, n))
     saved = A.new_empty((b, -(-t // SAVE_EVERY), d, n)) if train else None
     if b == 0 or d == 0:
@@ -435,7 +441,8 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     """One token for each of R envs: x, dt, z [R, D], B, C [R, G, N] -> out [R, D].
     ``state`` [S, D, N] is the pool of states, ``slots`` [R] (int32) each row's place in
     it (None: row r is slot r; below 0: no env, its output is zero), moved on in place.
-    No two rows may name one slot."""
+    No two rows may name one slot. ``out`` may be x, dt or z itself, and shares no memory with
+    an input otherwise."""
     what = "selective_scan_step"
     if not x.is_cuda:
         _lib.require_cuda(x, what)
@@ -469,6 +476,8 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
         out = _like(x)
     else:
         _tokens(what, "out", out, shape, dtype, at)
+        _lib.require_apart(what, "out", out, dict(x=x, dt=dt, z=z, A=A, B=B, C=C, D=D, dt_bias=dt_bias, state=state, reset=reset,
+                                                  slots=slots), ("x", "dt", "z"))
     if r == 0 or d == 0:
         return out
     A = _even(A)

@@ -447,3 +447,25 @@ def test_phase_clock_nvtx_ranges_balance(monkeypatch):
     assert calls == [] and set(got) == {"env", "total"} and got["total"] >= got["env"] >= 0.0
     line = PhaseClock.timing_line(3, {"env": 1.25, "total": 2.0})
     assert line == "TIMING iter=3 env=1.2 total=2.0"
+
+
+def test_overlap_of_strided_views():
+    """Whether views share an element: the overlap test of outputs, against sets of addresses."""
+    from surfb200.ops import _lib
+    buf = torch.zeros(400)
+    views = [buf[:60].view(3, 4, 5), buf.as_strided((3, 4, 5), (20, 5, 1), 1), buf.as_strided((3, 4, 5), (40, 10, 1)),
+             buf.as_strided((3, 4, 5), (40, 10, 1), 5), buf.as_strided((3, 4, 5), (40, 10, 1), 4), buf[60:120].view(3, 4, 5),
+             buf.as_strided((3, 4, 5), (40, 5, 1), 20), buf.as_strided((3, 4, 5), (40, 5, 1)), buf.as_strided((4, 3, 5), (5, 40, 1)),
+             buf[:0].view(0, 4, 5), buf.as_strided((3, 4, 5), (0, 5, 1), 19)]
+    where = [{v.storage_offset() + sum(i * s for i, s in zip(at, v.stride())) for at in np.ndindex(*v.shape)} for v in views]
+    for a, p in zip(views, where):
+        for b, q in zip(views, where):
+            assert _lib.overlap(a, b) == bool(p & q)
+    wide = torch.zeros(3, 8, dtype=torch.bfloat16)
+    assert not _lib.overlap(wide[:, :4], wide[:, 4:]) and _lib.overlap(wide[:, :4], wide[:, 3:])
+    x, z = wide[:, :4], wide[:, 4:]
+    _lib.require_apart("op", "out", z, dict(x=x, state=None))
+    _lib.require_apart("op", "out", x, dict(x=x), ("x",))
+    for out, inputs, place in ((x, dict(x=x), ()), (wide[:, 1:5], dict(x=x), ("x",)), (torch.zeros(1, 4).expand(3, 4), dict(x=x), ())):
+        with pytest.raises(ValueError, match="share"):
+            _lib.require_apart("op", "out", out, inputs, place)

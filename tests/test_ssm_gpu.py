@@ -440,3 +440,44 @@ def test_refusals():
         ssm.causal_conv(k["x"], k["weight"].bfloat16())
     with pytest.raises(ValueError, match="slots"):
         ssm.causal_conv_step(k["x"][:, 0], k["weight"], None, torch.zeros(1, 3, 16, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_outputs_apart_from_inputs(dtype):
+    """An output over an input is refused where other threads still read it; beside the input in
+    the same buffer, or in the place of an input that only its writer reads, it is taken."""
+    c = _conv_case(3, 70, 24, 4, True, True, dtype)
+    kw = dict(state=c["state"], reset=c["reset"], lengths=c["lengths"])
+    want, _ = ssm.causal_conv(c["x"], c["weight"], c["bias"], **kw)
+    buf = torch.zeros(3, 70, 48, device="cuda", dtype=dtype)
+    x = buf[..., 24:]
+    x.copy_(c["x"])
+    for out in (x, buf[..., 23:47], buf[..., 1:25], c["state"].new_zeros(1, 70, 24).expand(3, 70, 24)):
+        with pytest.raises(ValueError, match="share"):
+            ssm.causal_conv(x, c["weight"], c["bias"], out=out, **kw)
+    assert torch.equal(ssm.causal_conv(x, c["weight"], c["bias"], out=buf[..., :24], **kw)[0], want)
+    pool = torch.zeros(3, 3, 24, device="cuda", dtype=dtype)
+    with pytest.raises(ValueError, match="memory with state"):
+        ssm.causal_conv_step(c["x"][:, 0], c["weight"], c["bias"], pool, out=pool[:, 0])
+    row = torch.nan_to_num(c["x"][:, 0])
+    want = ssm.causal_conv_step(row, c["weight"], c["bias"], pool.clone())
+    assert torch.equal(ssm.causal_conv_step(row, c["weight"], c["bias"], pool, out=row), want)
+
+    for t in (70, 300):                                     # whole and cut
+        c = _scan_case(2, t, 40, 16, 1, True, True, dtype)
+        a = {k: c[k].contiguous() for k in ("x", "dt", "A", "B", "C", "z")}
+        kw = dict(D=c["D"], dt_bias=c["dt_bias"], state=c["state"], reset=c["reset"], lengths=c["lengths"])
+        want = ssm.selective_scan(*[a[k] for k in ("x", "dt", "A", "B", "C")], z=a["z"], **kw).out
+        for place in ("x", "dt", "z"):
+            q = {k: v.clone() for k, v in a.items()}
+            got = ssm.selective_scan(*[q[k] for k in ("x", "dt", "A", "B", "C")], z=q["z"], out=q[place], **kw).out
+            assert got is q[place] and torch.equal(got, want)
+            q = {k: v[:, 0].clone() if k != "A" else v for k, v in a.items()}
+            q = {k: torch.nan_to_num(v) for k, v in q.items()}
+            step = lambda pool, **o: ssm.selective_scan_step(*[q[k] for k in ("x", "dt", "A", "B", "C")], pool, z=q["z"], **o)  # noqa: E731
+            first = step(c["state"].clone())
+            assert torch.equal(step(c["state"].clone(), out=q[place]), first)
+        wide = torch.zeros(2, t, 60, device="cuda", dtype=dtype)
+        wide[..., :40] = torch.nan_to_num(a["x"])
+        with pytest.raises(ValueError, match="memory with x"):
+            ssm.selective_scan(wide[..., :40], *[a[k] for k in ("dt", "A", "B", "C")], out=wide[..., 20:])
