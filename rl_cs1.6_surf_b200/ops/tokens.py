@@ -53,7 +53,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     (float32 or bfloat16, rows any stride apart) with uniform numbers ``u`` [R, H] in
     [0, 1). Without ``heads`` the row is one answer (H = 1); with them its columns are the
     heads' categories side by side, each an answer of its own. ``temperature``, ``top_p``,
-    ``min_p`` (float32) and ``top_k`` (int32; 0: no limit) are numbers or tensors [R]."""
+    ``min_p`` (float32) and ``top_k`` (int32; 0: no limit) are numbers or tensors [R]. ``out`` and
+    ``logp`` must not share memory with an input: other blocks of a row's cluster still read its
+    number when the answer is written."""
     _lib.require_cuda(logits, "sample_tokens")
     if logits.dim() != 2:
         raise ValueError("sample_tokens: logits must be [rows, candidates]")
@@ -86,6 +88,12 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     for name, t, dt in (("out", out, torch.int32), ("logp", logp, f32)):
         if t is not None and (t.shape != (rows, n) or t.dtype != dt or t.device != dev or not t.is_contiguous()):
             raise ValueError(f"sample_tokens: {name} must be a contiguous {dt} tensor [{rows}, {n}] on {dev}")
+    if out is not None or logp is not None:
+        inputs = dict(logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        if out is not None:
+            _lib.require_apart("sample_tokens", "out", out, dict(inputs, logp=logp))
+        if logp is not None:
+            _lib.require_apart("sample_tokens", "logp", logp, inputs)
     if out is None:
         out = torch.empty_like(u, dtype=torch.int32)
     if logp is None:

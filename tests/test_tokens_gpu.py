@@ -202,3 +202,23 @@ def test_outputs_in_place_and_refusals():
         TK.sample_tokens(z, u, top_k=torch.ones(3, device="cuda"))
     with pytest.raises(ValueError, match="at most"):
         TK.sample_tokens(torch.empty(1, TK.MAX_VOCAB + 1, device="cuda"), u[:1])
+
+
+def test_outputs_apart_from_inputs():
+    """Outputs over the numbers, the logits, a limit or one another are refused; beside them in
+    one buffer they are taken."""
+    z = torch.randn(3, 40000, device="cuda")
+    u, t = torch.rand(3, 1, device="cuda"), torch.ones(3, device="cuda")
+    k = torch.full((3,), 9, dtype=torch.int32, device="cuda")
+    for kw in (dict(logp=u), dict(out=u.view(torch.int32)), dict(logp=t.view(3, 1), temperature=t), dict(out=k.view(3, 1), top_k=k),
+               dict(logp=z[0, 8:11].view(3, 1))):
+        with pytest.raises(ValueError, match="memory with"):
+            TK.sample_tokens(z, u, **kw)
+    both = torch.zeros(3, 1, device="cuda")
+    with pytest.raises(ValueError, match="out shares memory with logp"):
+        TK.sample_tokens(z, u, out=both.view(torch.int32), logp=both)
+    buf = torch.zeros(9, device="cuda")
+    buf[3:6] = u[:, 0]
+    a = TK.sample_tokens(z, buf[3:6].view(3, 1), out=buf[:3].view(torch.int32).view(3, 1), logp=buf[6:].view(3, 1))
+    b = TK.sample_tokens(z, u)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
