@@ -165,7 +165,14 @@ __device__ __forceinline__ float exp2_hw(float x) {
 // argument 3e-8 larger takes it out (mean -4e-10 for x in [-0.02, -0.002], 2e-9 in
 // [-0.1, -0.02]) at no cost: the multiplication that makes it becomes a multiply-add.
 constexpr float kExp2Shift = 3e-8f;
-// exp(delta * A) with A2 = A log2(e)
+// The rate of a state, A log2(e). -inf (a state that forgets at once) becomes the largest finite
+// rate: with a step of zero, which a dt of -inf is and every token that fills up a row's last
+// tile, it would be 0 * -inf, not a number. Steps above 4e-37 forget all the same.
+__device__ __forceinline__ float rate_of(float A) {
+  const float r = A * kLog2e;
+  return r < -3.4028235e38f ? -3.4028235e38f : r;
+}
+// exp(delta * A) with A2 = rate_of(A); exactly 1 for a step of zero
 __device__ __forceinline__ float decay(float delta, float A2) { return exp2_hw(fmaf(delta, A2, kExp2Shift)); }
 // 1 / x by the hardware's approximation (relative error 2^-23; 0 for infinity). The divisors
 // here lie between 1 and infinity: a division, even the approximate one, guards a range that

@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) scan_kernel(ScanArgs
     const float h0[4] = {hv[0].x, hv[0].y, hv[0].z, hv[0].w}, h1[4] = {hv[1].x, hv[1].y, hv[1].z, hv[1].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      A2[p][i] = pack2(a0[i] * kLog2e, a1[i] * kLog2e);
+      A2[p][i] = pack2(rate_of(a0[i]), rate_of(a1[i]));
       h[p][i] = pack2(h0[i], h1[i]);
     }
     sumd[p] = pack2(0.0f, 0.0f);
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(128) carry_kernel(ScanArgs a) {
   const int b = static_cast<int>(id / per);
   const int64_t dn = id - b * per, row = static_cast<int64_t>(b) * a.chunks;
   const int d = static_cast<int>(dn / a.N);
-  string_chunks<false>(a.state ? a.state[id] : 0.0f, a.A[dn] * kLog2e, a.carry + row * per + dn, per, a.sumd + row * a.dim + d, a.dim,
+  string_chunks<false>(a.state ? a.state[id] : 0.0f, rate_of(a.A[dn]), a.carry + row * per + dn, per, a.sumd + row * a.dim + d, a.dim,
                        a.cut + row, a.chunks);
 }
 
@@ -431,7 +431,7 @@ template <typename T, int LN> __global__ void __launch_bounds__(128) step_kernel
       float h[4] = {h4[k].x, h4[k].y, h4[k].z, h4[k].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {                      // states past the N-th stay zero: A, B and h are there
-        h[i] = fmaf(decay(dl, Av[i] * kLog2e), h[i], u * to_f(B.v[i]));
+        h[i] = fmaf(decay(dl, rate_of(Av[i])), h[i], u * to_f(B.v[i]));
         acc[k] = fmaf(h[i], to_f(C.v[i]), acc[k]);
       }
       store_state4(pool + static_cast<int64_t>(d) * a.N, n0, a.N, h);

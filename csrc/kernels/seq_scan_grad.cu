@@ -132,13 +132,14 @@ __global__ void __launch_bounds__(NT, (kCarry ? 768 : 512) / NT) scan_grad_kerne
 
   const int order = order_of<LN>(lane);
   // 4 states of the two channels, from memory into pairs and back
-  auto load_h = [&](const float* src, f2 (&v)[2][2], float scale) {
+  auto load_h = [&](const float* src, f2 (&v)[2][2], auto rate) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
       if (src && ch + k < nch) q = in_order(load_state4(src + static_cast<int64_t>(d0 + ch + k) * a.N, n0, a.N), order);
-      v[k][0] = pack2(q.x * scale, q.y * scale);
-      v[k][1] = pack2(q.z * scale, q.w * scale);
+      if constexpr (decltype(rate)::value) q = make_float4(rate_of(q.x), rate_of(q.y), rate_of(q.z), rate_of(q.w));
+      v[k][0] = pack2(q.x, q.y);
+      v[k][1] = pack2(q.z, q.w);
     }
   };
   auto store_h = [&](float* dst, const f2 (&v)[2][2]) {
@@ -156,8 +157,8 @@ __global__ void __launch_bounds__(NT, (kCarry ? 768 : 512) / NT) scan_grad_kerne
 
   f2 A2[2][2], dh[2][2], dA[2][2];
   float sumd[2] = {0.0f, 0.0f};
-  load_h(a.A, A2, kLog2e);
-  load_h(kCarry ? nullptr : a.chunks > 1 ? a.carry + bchunk * per_row : a.dfinal ? a.dfinal + b * per_row : nullptr, dh, 1.0f);
+  load_h(a.A, A2, std::true_type{});
+  load_h(kCarry ? nullptr : a.chunks > 1 ? a.carry + bchunk * per_row : a.dfinal ? a.dfinal + b * per_row : nullptr, dh, std::false_type{});
   dA[0][0].v = dA[0][1].v = dA[1][0].v = dA[1][1].v = 0;
 
   const T* gx = static_cast<const T*>(a.x) + b * a.x_b + d0;
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(NT, (kCarry ? 768 : 512) / NT) scan_grad_kerne
         }
       }
     } else {
-      load_h(sm.hs[buf] - static_cast<int64_t>(d0) * a.N, h[0], 1.0f);
+      load_h(sm.hs[buf] - static_cast<int64_t>(d0) * a.N, h[0], std::false_type{});
       auto sweeps = [&](auto with_cuts) {
         constexpr bool kCuts = decltype(with_cuts)::value;
 #pragma unroll
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(128) grad_carry_kernel(ScanArgs a) {
   const int b = static_cast<int>(id / per);
   const int64_t dn = id - b * per, row = static_cast<int64_t>(b) * a.chunks;
   const int d = static_cast<int>(dn / a.N);
-  const float dh = string_chunks<true>(a.dfinal ? a.dfinal[id] : 0.0f, a.A[dn] * kLog2e, a.carry + row * per + dn, per,
+  const float dh = string_chunks<true>(a.dfinal ? a.dfinal[id] : 0.0f, rate_of(a.A[dn]), a.carry + row * per + dn, per,
                                        a.sumd + row * a.dim + d, a.dim, a.cut + row, a.chunks);
   if (a.dstate) a.dstate[id] = dh;
 }

@@ -481,3 +481,55 @@ def test_outputs_apart_from_inputs(dtype):
         wide[..., :40] = torch.nan_to_num(a["x"])
         with pytest.raises(ValueError, match="memory with x"):
             ssm.selective_scan(wide[..., :40], *[a[k] for k in ("dt", "A", "B", "C")], out=wide[..., 20:])
+
+
+def _state_error(c):
+    """The largest relative error of a 32-bit state of this case, from its own steps: a decay is
+    off by 2^-22 (hardware exponential) and 2^-23 |delta A| (its argument), its product and sum by
+    2^-24 each; a state sums these over min(T, 1 / (1 - largest decay)) tokens. What a gradient
+    multiplies, a state and an adjoint, is off by twice that."""
+    t = c["x"].shape[1]
+    real = ssm._real(c["lengths"], c["x"].shape[0], t, "cuda")
+    v = torch.nn.functional.softplus((c["dt"].double() + c["dt_bias"].double())[real])
+    rate = c["A"].double().abs()
+    rate = rate[rate.isfinite()]
+    memory = min(t, 1 / (1 - float(torch.exp(-v.min() * rate.min()))))
+    return memory * (2.0 ** -22 + 2.0 ** -23 * float(v.max() * rate.max()) + 2.0 ** -23)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [4, 8, 16, 24, 64])
+@pytest.mark.parametrize("t", [5, 16, 23, 300])
+def test_missing_tokens_leave_alone_what_forgets_at_once(t, n, dtype):
+    """States with a rate of -inf hold the last token only. The tokens that fill up a row's last
+    tile, and a chunk behind its end, are steps of zero: 0 * -inf must not reach the states nor the
+    adjoints."""
+    c = _scan_case(3, t, 40, n, 1, False, False, dtype, seed=t)
+    c["lengths"] = torch.tensor([t, max(1, t // 3), 0], dtype=torch.int32, device="cuda")
+    for k in ("x", "z", "dt", "B", "C", "dout"):
+        c[k] = _hide(c[k].contiguous(), c["lengths"])
+    c["A"][:, ::2] = float("-inf")
+    r, g = _scan_run(c)
+    out, final, grads = _scan_exact(c)
+    tol = {torch.bfloat16: TOL[torch.bfloat16], torch.float32: _state_error(c)}
+    assert rel(r.out, out) <= tol[dtype] and rel(r.final, final) <= tol[torch.float32]
+    got = _named(g)
+    for k in ("x", "z", "B", "C", "A", "D", "state"):               # ddelta = q A is 0 * -inf by the formula
+        assert rel(got[k], grads[k]) <= 2 * tol[got[k].dtype], k
+
+
+def test_steps_of_zero_leave_the_state_to_the_bit():
+    """exp(0 A) is exactly 1: after any number of steps of zero the state, and the adjoint on the
+    way back, are the same bits."""
+    for n in (4, 8, 16, 32, 64):
+        st = torch.randn(2, 48, n, device="cuda")
+        A = -(1 + 9 * torch.rand(48, n, device="cuda"))
+        x = torch.zeros(2, 37, 48, device="cuda")
+        dt = torch.full((2, 37, 48), float("-inf"), device="cuda")
+        B = torch.randn(2, 37, 1, n, device="cuda")
+        r = ssm.selective_scan(x, dt, A, B, B, state=st, train=True)
+        g = ssm.selective_scan_grad(x, x, dt, A, B, B, saved=r.saved, state=st, dfinal=st)
+        assert torch.equal(r.final, st) and torch.equal(g.dstate, st)
+        pool = st.clone()
+        ssm.selective_scan_step(x[:, 0], dt[:, 0], A, B[:, 0], B[:, 0], pool)
+        assert torch.equal(pool, st)
