@@ -196,7 +196,9 @@ def backward(net: MemoryNet, k: SequenceCache, dlogits: torch.Tensor) -> None:
 
 def step(net: MemoryNet, x: torch.Tensor, state: MemoryState, reset: Optional[torch.Tensor] = None,
          slots: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Logits [R, out_pad] (fp32) of one decision of R envs; their slots of ``state`` move on."""
+    """Logits [R, out_pad] (fp32) of one decision of R envs; their slots of ``state`` move on. A
+    slot out of range is reported through ``ops.gemm.check_error_flag``, which the caller looks
+    at when it synchronises; its row's core output is zero."""
     from ..ops import gemm as G
     c = net.cfg
     R = x.shape[0]
@@ -213,7 +215,8 @@ def step(net: MemoryNet, x: torch.Tensor, state: MemoryState, reset: Optional[to
 def act(net: MemoryNet, x: torch.Tensor, state: MemoryState, u: torch.Tensor, reset: Optional[torch.Tensor] = None,
         slots: Optional[torch.Tensor] = None, **rule):
     """(answers int32 [R], log-probabilities [R]) of one decision, drawn with the numbers
-    ``u`` [R, 1] under ``rule`` (temperature, top_k, top_p, min_p of ``sample_tokens``)."""
+    ``u`` [R, 1] under ``rule`` (temperature, top_k, top_p, min_p of ``sample_tokens``); errors
+    as of ``step``."""
     from ..ops.tokens import sample_tokens
     logits = step(net, x, state, reset, slots)
     token, logp = sample_tokens(logits[:, :net.cfg.answers], u, **rule)
@@ -256,7 +259,10 @@ def train_recall(iterations: int = 400, envs: int = 128, length: int = 64, cfg: 
                  lr: float = 1e-2, seed: int = 0, longest: int = 48, act_steps: int = 96, temperature: float = 0.5, top_p: float = 0.9,
                  log=None) -> dict:
     """Train a memory core on the recall task and let it answer, decision by decision, with
-    sampled answers: {"loss": first and last, "accuracy": of the sampled answers}."""
+    sampled answers: {"loss": first and last, "accuracy": of the sampled answers}. An error that
+    a kernel reported (a wait that ran out, an index out of range) is raised every 25 iterations
+    and at the end."""
+    from ..ops.gemm import check_error_flag
     from ..ops.rl import Adam
     dev = torch.device(device)
     net = MemoryNet(cfg or MemoryConfig(), dev, seed)
@@ -289,6 +295,8 @@ def train_recall(iterations: int = 400, envs: int = 128, length: int = 64, cfg: 
             net.collect_grads(params)
         opt.step()
         losses.append(loss.detach())
+        if gpu and (it + 1) % 25 == 0:
+            check_error_flag(dev)
         if log is not None and (it + 1) % 25 == 0:
             log(f"iteration {it + 1}: loss {float(loss):.4f}")
     right = asked_n = 0
@@ -306,4 +314,6 @@ def train_recall(iterations: int = 400, envs: int = 128, length: int = 64, cfg: 
             answer = sample_tokens_reference(logits[:, 0, :c.answers], u, temperature=temperature, top_p=top_p)[0][:, 0]
         right += int(((answer == t) & (t >= 0)).sum())
         asked_n += int((t >= 0).sum())
+    if gpu:
+        check_error_flag(dev)
     return {"loss": [float(losses[0]), float(losses[-1])], "accuracy": right / max(1, asked_n), "questions": asked_n}

@@ -230,8 +230,9 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token x [R, D] for each of R envs: y [R, D]. ``state`` [S, W-1, D] is the pool
     of windows, ``slots`` [R] (int32) each row's place in it (None: row r is slot r; below
-    0: no env, its output is zero), moved on in place. No two rows may name one slot. ``out``
-    may be x itself, and shares no memory with an input otherwise."""
+    0: no env, its output is zero), moved on in place. No two rows may name one slot. A slot past
+    the pool gives zeros and is reported through ``ops.gemm.check_error_flag``. ``out`` may be x
+    itself, and shares no memory with an input otherwise."""
     what = "causal_conv_step"
     _lib.require_cuda(x, what)
     if x.dim() != 2:
@@ -441,8 +442,9 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     """One token for each of R envs: x, dt, z [R, D], B, C [R, G, N] -> out [R, D].
     ``state`` [S, D, N] is the pool of states, ``slots`` [R] (int32) each row's place in
     it (None: row r is slot r; below 0: no env, its output is zero), moved on in place.
-    No two rows may name one slot. ``out`` may be x, dt or z itself, and shares no memory with
-    an input otherwise."""
+    No two rows may name one slot. A slot past the pool gives zeros and is reported through
+    ``ops.gemm.check_error_flag``. ``out`` may be x, dt or z itself, and shares no memory with an
+    input otherwise."""
     what = "selective_scan_step"
     if not x.is_cuda:
         _lib.require_cuda(x, what)

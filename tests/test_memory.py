@@ -121,3 +121,26 @@ def test_steps_follow_the_sequence():
 def test_learns_to_recall():
     r = M.train_recall(400)
     assert r["loss"][0] > 1.5 and r["loss"][1] < 1.0 and r["accuracy"] > 0.9, r
+
+
+@pytest.mark.gpu
+def test_reported_errors_are_raised(monkeypatch):
+    """What a kernel reports while the core trains or answers ends the run, and is not left for
+    whoever looks at the flag next."""
+    from surfb200.ops import _lib
+    from surfb200.ops import gemm as G
+    G.check_error_flag("cuda")
+    cfg = M.MemoryConfig(dim=32, rank=8)
+    for iterations in (1, 25):
+        G.error_flag("cuda").fill_(3)
+        with monkeypatch.context() as m, pytest.raises(_lib.KernelError, match="epilogue wait"):
+            if iterations == 25:                                     # raised before the answers
+                m.setattr(M, "act", None)
+            M.train_recall(iterations, envs=8, length=8, cfg=cfg, act_steps=1)
+    G.check_error_flag("cuda")
+    net = _small("cuda")
+    state = M.MemoryState(net, 2)
+    x = torch.zeros(2, 16, dtype=torch.bfloat16, device="cuda")
+    M.act(net, x, state, torch.zeros(2, 1, device="cuda"), slots=torch.tensor([1, 2], dtype=torch.int32, device="cuda"))
+    with pytest.raises(_lib.KernelError, match="state slot"):
+        G.check_error_flag("cuda")
