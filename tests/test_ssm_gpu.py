@@ -533,3 +533,21 @@ def test_steps_of_zero_leave_the_state_to_the_bit():
         pool = st.clone()
         ssm.selective_scan_step(x[:, 0], dt[:, 0], A, B[:, 0], B[:, 0], pool)
         assert torch.equal(pool, st)
+
+
+@pytest.mark.parametrize("n,g", [(16, 1), (5, 2), (64, 1)])
+def test_scan_slot_out_of_range_is_reported(n, g):
+    """The row's output is zero, its neighbours' states are where they were, the rows beside it
+    are answered, and the error is there to be raised."""
+    G.check_error_flag("cuda")
+    c = _scan_case(3, 1, 24, n, g, False, False, torch.float32)
+    pool = torch.full((4, 24, n), 2.0, device="cuda")
+    slots = torch.tensor([1, 3, 0], dtype=torch.int32, device="cuda")
+    args = [c[k][:, 0] if k != "A" else c[k] for k in ("x", "dt", "A", "B", "C")]
+    y = ssm.selective_scan_step(*args, pool[:3], z=c["z"][:, 0], slots=slots)
+    torch.cuda.synchronize()
+    assert not y[1].any() and y[0].any() and y[2].any()
+    assert (pool[2:] == 2).all() and (pool[:2] != 2).any()
+    with pytest.raises(_lib.KernelError, match="state slot"):
+        G.check_error_flag("cuda")
+    G.check_error_flag("cuda")
