@@ -83,7 +83,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     kp, k0 = _per_row("top_k", top_k, rows, torch.int32, dev)
     pp, p0 = _per_row("top_p", top_p, rows, f32, dev)
     mp, m0 = _per_row("min_p", min_p, rows, f32, dev)
-    if t0 < 0 or k0 < 0 or not 0 <= p0 <= 1 or not 0 <= m0 <= 1:
+    if not t0 >= 0 or k0 < 0 or not 0 <= p0 <= 1 or not 0 <= m0 <= 1:
         raise ValueError("sample_tokens: temperature and top_k must not be negative, top_p and min_p lie in [0, 1]")
     for name, t, dt in (("out", out, torch.int32), ("logp", logp, f32)):
         if t is not None and (t.shape != (rows, n) or t.dtype != dt or t.device != dev or not t.is_contiguous()):

@@ -222,3 +222,10 @@ def test_outputs_apart_from_inputs():
     a = TK.sample_tokens(z, buf[3:6].view(3, 1), out=buf[:3].view(torch.int32).view(3, 1), logp=buf[6:].view(3, 1))
     b = TK.sample_tokens(z, u)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("rule", ["temperature", "top_p", "min_p"])
+def test_a_rule_that_is_not_a_number_is_refused(rule):
+    z, u = torch.randn(3, 40, device="cuda"), torch.rand(3, 1, device="cuda")
+    with pytest.raises(ValueError, match="negative"):
+        TK.sample_tokens(z, u, **{rule: float("nan")})
