@@ -551,3 +551,49 @@ def test_scan_slot_out_of_range_is_reported(n, g):
     with pytest.raises(_lib.KernelError, match="state slot"):
         G.check_error_flag("cuda")
     G.check_error_flag("cuda")
+
+
+# B, T, D, N, groups, reset, ragged, rows in chunks: channels of a group on both sides of what
+# makes a block ordinary (129, 65, 33, 17 for 1..4, 5..16, 17..32, 33..64 states) or narrow, for
+# every count of lanes, in 16-byte and 4-byte pieces and element by element, whole and cut
+BLOCKS = [
+    (2, 37, 304, 4, 1, True, True, False), (3, 50, 258, 3, 2, True, True, False), (2, 23, 128, 4, 1, True, True, False),
+    (1, 300, 320, 4, 1, True, False, True), (2, 260, 24, 2, 1, True, True, True),
+    (2, 70, 200, 8, 1, True, True, False), (3, 45, 133, 7, 1, True, True, False), (2, 19, 128, 8, 2, False, True, False),
+    (2, 300, 256, 8, 1, True, True, True), (1, 200, 12, 8, 1, False, False, True),
+    (2, 41, 136, 16, 1, True, True, False), (2, 33, 65, 13, 1, True, True, False),
+    (2, 41, 104, 32, 1, True, True, False), (3, 35, 74, 20, 2, True, True, False), (1, 39, 32, 24, 1, True, False, False),
+    (2, 200, 80, 24, 1, True, True, True), (1, 260, 16, 32, 2, True, False, True),
+    (2, 33, 32, 64, 2, True, True, False), (3, 40, 10, 40, 1, True, True, False), (2, 29, 72, 64, 1, True, True, False),
+    (2, 200, 16, 48, 1, True, True, True), (1, 260, 51, 64, 1, True, False, True),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", BLOCKS, ids=str)
+def test_scan_in_every_kind_of_block(case, dtype):
+    b, t, d, n, g = case[:5]
+    assert (ssm._chunks(b, t, d, n, g)[1] > 2) == case[7]
+    c = _scan_case(*case[:7], dtype, seed=11)
+    r, gr = _scan_run(c)
+    out, final, grads = _scan_exact(c)
+    tol = {torch.bfloat16: TOL[torch.bfloat16], torch.float32: _state_error(c)}
+    assert rel(r.out, out) <= tol[dtype] and rel(r.final, final) <= tol[torch.float32]
+    for k, v in _named(gr).items():
+        assert rel(v, grads[k]) <= 2 * tol[v.dtype], k
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scan_in_three_chunks(dtype):
+    """The fewest chunks that a row is cut into, and never two."""
+    assert ssm._chunks(19, 200, 1000, 16, 1) == (80, 3)
+    for b in range(1, 80):
+        for t in (127, 128, 129, 200, 1000):
+            assert ssm._chunks(b, t, 1000, 16, 1)[1] != 2
+    c = _scan_case(19, 200, 1000, 16, 1, True, True, dtype)
+    r, g = _scan_run(c)
+    out, final, grads = _scan_exact(c)
+    tol = {torch.bfloat16: TOL[torch.bfloat16], torch.float32: _state_error(c)}
+    assert rel(r.out, out) <= tol[dtype] and rel(r.final, final) <= tol[torch.float32]
+    for k, v in _named(g).items():
+        assert rel(v, grads[k]) <= 2 * tol[v.dtype], k
