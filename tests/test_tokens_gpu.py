@@ -229,3 +229,42 @@ def test_a_rule_that_is_not_a_number_is_refused(rule):
     z, u = torch.randn(3, 40, device="cuda"), torch.rand(3, 1, device="cuda")
     with pytest.raises(ValueError, match="negative"):
         TK.sample_tokens(z, u, **{rule: float("nan")})
+
+
+def _same_in(rows, logits, u, **kw):
+    """``_same`` for a few of the rows of one call (the rule by sorting is slow)."""
+    tok, logp = TK.sample_tokens(logits, u, **kw)
+    et, ep = _by_rule(logits[rows], u[rows], **{k: v[rows] if isinstance(v, torch.Tensor) else v for k, v in kw.items()})
+    assert torch.equal(tok[rows], et)
+    assert torch.allclose(logp[rows], ep, rtol=2.0 ** -22, atol=1e-6)
+
+
+LONG = [dict(), dict(top_p=0.95), dict(top_p=0.9, temperature=0.3), dict(top_k=50, top_p=0.9), dict(top_k=60000), dict(min_p=0.05),
+        dict(top_k=100000, top_p=0.99, temperature=2.0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rule", LONG, ids=str)
+@pytest.mark.parametrize("rows,vocab", [(148, 131072), (149, 262144), (160, 129001)])
+def test_rows_as_long_as_they_come(rows, vocab, rule, dtype):
+    """A block for each row, its threads adding more weights than 32 bits hold: logits close
+    together, so that nearly all of them are of the largest's order, some masked, ties."""
+    gen = torch.Generator("cuda").manual_seed(vocab)
+    z = (0.5 * torch.randn(rows, vocab, generator=gen, device="cuda")).to(dtype)
+    z[torch.rand(rows, vocab, generator=gen, device="cuda") < 0.02] = float("-inf")
+    z[1] = 0.25
+    z[2] *= 6
+    _same_in([0, 1, 2, rows - 1], z, torch.rand(rows, 1, generator=gen, device="cuda"), **rule)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rule", LONG, ids=str)
+@pytest.mark.parametrize("rows,vocab", [(80, 20001), (40, 40000), (64, 131072), (20, 200003), (1, 262144), (3, 131073)])
+def test_slices_of_every_size(rows, vocab, rule, dtype):
+    """Clusters of 2 to 16 blocks whose slices are longer than 8192 candidates (rows enough to
+    fill the GPU), and as long as they come in few rows."""
+    gen = torch.Generator("cuda").manual_seed(vocab)
+    z = (0.5 * torch.randn(rows, vocab + 1, generator=gen, device="cuda")).to(dtype)[:, 1:]
+    z[torch.rand(rows, vocab, generator=gen, device="cuda") < 0.02] = float("-inf")
+    z[rows // 2] *= 6
+    _same_in(sorted({0, rows // 2, rows - 1}), z, torch.rand(rows, 1, generator=gen, device="cuda"), **rule)
