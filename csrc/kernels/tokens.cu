@@ -153,7 +153,8 @@ template <typename T> __global__ void __launch_bounds__(128) small_kernel(TokenA
 // ---- many candidates: a cluster of CS blocks, the row's slices in shared memory -----------
 // One exponential per candidate: e is kept in shared memory in the logit's place, and all
 // later passes work on its bits (e orders the candidates except where several logits share
-// an e; only there the logits are looked at again).
+// an e; only there the logits are looked at again). That rests on an expf that never falls as
+// its argument rises: so it is here, every argument from -0 to -104 looked at.
 //
 // With enough rows to fill the GPU a row is one block's (kStream): no barriers between
 // blocks; the row is read again from the L2 cache and its exponentials made again instead

@@ -268,3 +268,20 @@ def test_slices_of_every_size(rows, vocab, rule, dtype):
     z[torch.rand(rows, vocab, generator=gen, device="cuda") < 0.02] = float("-inf")
     z[rows // 2] *= 6
     _same_in(sorted({0, rows // 2, rows - 1}), z, torch.rand(rows, 1, generator=gen, device="cuda"), **rule)
+
+
+@pytest.mark.parametrize("rows", [1, 150])
+def test_order_across_the_bins(rows):
+    """Logits a few representable numbers on both sides of every border of the histogram over
+    exp(z): the limit by count falls between neighbours as their logits say, wherever it is."""
+    border = torch.tensor([2.0 ** -o * (1 - j / 256) for o in range(36) for j in range(128)], dtype=torch.float64)
+    at = border.log().float().cuda()
+    bits = at.view(torch.int32)[:, None] + torch.arange(-6, 7, device="cuda", dtype=torch.int32)
+    bits = torch.where((at == 0)[:, None], 0, bits)
+    z = bits.view(torch.float32).flatten()
+    gen = torch.Generator("cuda").manual_seed(6)
+    z = z[torch.randperm(z.numel(), generator=gen, device="cuda")][None].expand(rows, -1)
+    for k in torch.randint(1, z.shape[1], (12,), generator=gen, device="cuda").tolist() + [14, 15, 27]:
+        u = torch.full((rows, 1), 1 - 2.0 ** -24, device="cuda")
+        _same_in([0], z, u, top_k=k)
+        _same_in([0], z, torch.rand(rows, 1, generator=gen, device="cuda"), top_k=k, top_p=0.7)
