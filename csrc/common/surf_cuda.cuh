@@ -19,7 +19,7 @@ inline __host__ __device__ int64_t ceil_div(int64_t a, int64_t b) { return (a + 
 // pipeline's bounded waits; the index checks of the data-driven gathers use
 // the codes below (the offending access is skipped, its output zeroed).
 enum ErrCode : int { kErrGatherIndex = 0x100, kErrStackIndex = 0x101, kErrLossIndex = 0x102,
-               kErrSlotIndex = 0x103 };
+                     kErrSlotIndex = 0x103 };
 __device__ __forceinline__ void report_error(int* err, int code) {
   if (err) atomicCAS(err, 0, code);
 }

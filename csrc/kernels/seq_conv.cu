@@ -11,11 +11,15 @@
 // window slides through registers, a thread owning neighbouring channels over a
 // stretch of tokens, so each x is read once (plus W - 1 of every stretch).
 //
-// Measured on a B200, bf16, W = 4, with resets: forward 256 x 128 x 1024 32 us (134 MB, 4.2
-// TB/s), gradient 75 us (201 MB, 2.7 TB/s), a prompt of 16385 x 1024 18 us (67 MB, 3.8 TB/s); one
-// token of 64 envs 2.5 us. What bounds them is instructions at 16 warps on an SM (14 an
-// element in the forward, 36 in the gradient, a sigmoid's 5 and its derivative's 10 among
-// them): the SiLU takes 10 and 28 us of them.
+// Measured on a B200, W = 4, with resets, back to back: forward 256 x 128 x 1024 bf16 33 us (134
+// MB, 4.1 TB/s), f32 50 us (268 MB, 5.3 TB/s), gradient 76 us (201 MB, 2.6 TB/s) and 97 us (403
+// MB, 4.2 TB/s), a prompt of 16385 x 1024 18 us (67 MB, 3.7 TB/s) and 23 us (134 MB, 5.8 TB/s);
+// one token of 64 envs 2.9 us. In bf16 neither the issue slots (0.49 and 0.59 of a cycle and
+// scheduler in forward and gradient) nor DRAM is full: the 16 warps of an SM wait, most of all
+// for results of their own arithmetic. Of the 14 instructions an element of the forward and 36
+// of the gradient a sigmoid takes 5 and its derivative 10, an exponential and a reciprocal in a
+// row; the SiLU takes 10 and 28 us. The wait and the copies of every token keep a thread's tokens
+// apart, so that these chains do not overlap; fewer waits have not been tried.
 #include <type_traits>
 
 #include "seq_common.cuh"

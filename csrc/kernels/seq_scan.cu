@@ -16,12 +16,14 @@
 // whole decay is exp(A * sum), 0 across a reset), a small kernel strings the chunks
 // together, and the scan then runs in all chunks at once.
 //
-// Measured on a B200, bf16, 16 states: 256 x 128 x 512 121 us (131 us with the states kept
-// for the gradient), a prompt of 8191 x 1024 in 74 chunks 119 us (first pass 51, stringing 9,
-// scan 60 us), one token of 2048 envs x 1024 67 us (285 MB, 4.3 TB/s). The exponentials alone
-// take the SMs' units 60 us for 256 x 128 x 512 (2^28 of them, 16 a cycle and SM); the rest
-// is the work on every (token, channel), which shares the issue slots with the recurrence,
-// and waits at 16 warps on an SM (24 warps with tiles of 8 tokens were no faster: 120 us
+// Measured on a B200, 16 states, back to back: 256 x 128 x 512 bf16 117 us, f32 143 us (127 and
+// 158 us with the states kept for the gradient), a prompt of 8191 x 1024 in 74 chunks 114 and
+// 138 us (launched one by one: first pass 49, stringing 13, scan 62 us), one token of 2048 envs
+// x 1024 67 us in both types (285 MB, 4.3 TB/s). The recurrence's exponentials alone take the
+// SMs' units 60 us for 256 x 128 x 512 (2^28 of them, 16 a cycle and SM), softplus and gate,
+// four of their kind a (token, channel), 15 us more; the rest is the other work on every (token,
+// channel), which shares the issue slots with the recurrence, and waits at 16 warps on an SM
+// (0.52 issued a cycle and scheduler; 24 warps with tiles of 8 tokens were no faster: 120 us
 // against 121 us for every 2^28 at 1184 rows).
 #include "seq_scan.cuh"
 

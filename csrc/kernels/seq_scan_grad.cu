@@ -18,8 +18,9 @@
 // Long rows are cut into chunks as in the forward: a first pass leaves each chunk's
 // adjoint from nothing behind it, a small kernel strings the chunks together.
 //
-// Measured on a B200, bf16, 16 states: 256 x 128 x 512 376 us, 2 x 4096 x 1024 in 37 chunks
-// 268 us (first pass 65, stringing 10, sweeps 185, last sums 8 us). The two sweeps alone take
+// Measured on a B200, 16 states, back to back: 256 x 128 x 512 bf16 369 us, f32 397 us, 2 x 4096
+// x 1024 in 37 chunks 257 and 270 us (launched one by one, bf16: first pass 65, stringing 10,
+// sweeps 187, last sums 7 us). The two sweeps alone take
 // 404 cycles for 512 states (exponentials 256, multiply-adds about 260 on their own units),
 // 206 us for 256 x 128 x 512; the other half is the work on every (token, channel) around
 // them (80 of 240 M warp instructions) and the waits between the two at 16 warps on an SM.
@@ -89,7 +90,9 @@ template <int LN> __device__ __forceinline__ void reduce_rows(float (&b)[4], flo
 }
 
 // The backward sweep's decays, made again: as an ordinary expression the compiler would
-// keep the forward run's (8 values for each of the tile's tokens) and spill.
+// keep the forward run's (8 values for each of the tile's tokens), for which there are no
+// registers: the nine states of a thread's two channels take 72 of its 128, and every instance
+// spills 128 to 248 bytes of what lies around the sweeps as it is.
 __device__ __forceinline__ f2 decay2_again(f2 delta, f2 A2) {
   float lo, hi;
   unpack2(decay_arg(delta, A2), lo, hi);

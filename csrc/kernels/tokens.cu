@@ -106,7 +106,8 @@ template <typename V> __device__ __forceinline__ V warp_scan(V v, int lane) {   
 
 // ---- up to 32 candidates: one warp, a lane each ---------------------------------------
 // Ranks and the weight before a candidate by looking at every other lane in turn: 2 sizes'
-// shuffles a head, all in registers (2048 rows of six heads 8.9 us, 410 KB: latency).
+// shuffles a head, all in registers (2048 rows of six heads 9.4 us, 410 KB: the two
+// loops' chains of shuffles, in warps most of whose lanes are idle).
 template <typename T> __global__ void __launch_bounds__(128) small_kernel(TokenArgs a) {
   const int64_t id = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
@@ -160,11 +161,13 @@ template <typename T> __global__ void __launch_bounds__(128) small_kernel(TokenA
 // blocks; the row is read again from the L2 cache and its exponentials made again instead
 // of being kept (a slice of the whole row would not fit).
 //
-// Measured on a B200: 256 rows of 131072 bf16 under top_p 155 us (67 MB; without a limit
-// 60 us), as clusters 325 us; at a temperature of 0.7 133 us, as clusters 215 us; one row of
-// 32768 f32 under top_k and top_p 18 us, 64 rows of them 24 us. What bounds many rows is instructions, 106 for a candidate under top_p (two
-// exponentials, two weights in whole numbers, one place in the histogram) at 0.7 a cycle;
-// what bounds a few rows is the cluster's barriers, about ten of a microsecond each.
+// Measured on a B200: 256 rows of 131072 under top_p 155 us in bf16 (67 MB), 160 us in f32 (134
+// MB; bf16 without a limit 56 us), as clusters 325 us; at a temperature of 0.7 133 us, as
+// clusters 215 us; one row of 32768 under top_k and top_p 18 us in both types, 64 rows of them in
+// f32 24 us. What bounds many rows is instructions, 106 for a candidate under top_p (two
+// exponentials, two weights in whole numbers, one place in the histogram) at 0.7 a cycle; what
+// bounds a few rows is the cluster's barriers, thirteen of them under top_k with top_p, five of
+// these for the second limit.
 constexpr int kMaxCluster = 16, kMaxSlice = 16384, kMaxStream = kMaxCluster * kMaxSlice;
 constexpr int kList = 512;
 template <bool kStream> struct Large {
@@ -533,8 +536,9 @@ __global__ void __launch_bounds__(Large<kStream>::kThreads, 1024 / Large<kStream
         // Under top_k most warps' 128 candidates lie below the edge's bin altogether; in a
         // stream their exponentials are spared by the arguments (0.001 below the edge's: a
         // thousand times the exponential's error). 256 rows of 131072 bf16 of normal logits:
-        // top_k 50 134 -> 116 us, with top_p 182 -> 142; under top_p alone, whose set is wide,
-        // the vote costs more than it spares (155 -> 164) and is not taken.
+        // top_k 50 134 -> 114 us, with top_p 182 -> 141. Under top_p alone it is not taken: it
+        // costs a wide set 155 -> 164 us (top_p 0.95 at a temperature of 1), where it would spare a
+        // narrow one 126 -> 106 us (at 0.3). A rule on where the limit lies has not been built.
         if (kStream && q.k) {
           const float d_edge = lim ? logf(e_edge) - 0.001f : -INFINITY;
 #pragma unroll 2

@@ -186,6 +186,8 @@ def backward(net: MemoryNet, k: SequenceCache, dlogits: torch.Tensor) -> None:
     dproj[:, c.rank + c.state:] = s.dC.view(n, c.state)
     _wgrad(G, ddt, k.proj[:, :c.rank], net.g("dt.w"), n)
     _wgrad(G, dproj, k.xc.view(n, c.dim), net.g("x.w"), n)
+    # the two paths into xc, each rounded to bf16 as its kernel stores it, and their sum once more:
+    # 2^-9 each, as of the activations that they belong to
     dxc = s.dx.add_(G.gemm(dproj, net.w16("x.w"), b_mn=True).view(B, T, c.dim))
     g = ssm.causal_conv_grad(dxc, k.xz[..., :c.dim], net.p("conv.w"), net.p("conv.b"), state=k.conv0, reset=k.reset)
     net.g("conv.w").add_(g.dweight)

@@ -16,6 +16,9 @@ scan's state always float32.
 the others give zeros, change nothing and are never read. ``state`` is what the row
 starts from (None: empty), ``final`` what the next call starts from.
 
+None of them records a graph for autograd: gradients come from the ``*_grad`` functions
+alone, and an input that requires one gets none.
+
 Inputs may be strided views (slices of a projection) as long as the last axis is
 dense; 16-byte aligned rows are copied asynchronously, others element by element.
 """
@@ -298,9 +301,11 @@ def _scan_check(what, x, dt, A, B, C, D, z, dt_bias, state, reset, lengths):
 def _chunks(b: int, t: int, d: int, n: int, g: int):
     """(tokens of a chunk, chunks): a row is cut where its channels leave room on the GPU for
     three times as many threads (512 an SM), since the pass that leaves the chunks' ends costs
-    nearly half of the scan itself; a chunk has 16 tokens at least. A row below 128 is done
-    before the host has launched the two kernels more: 5 x 77 x 194 f32 cut and whole 20 + 39
-    and 23 + 52 us on the device, but 41 + 74 and 28 + 59 us a call.
+    nearly half of the scan itself; a chunk has 16 tokens at least. A row below 128 stays whole
+    for the sake of calls one by one, where the host has not launched the two kernels more before
+    it is done: 5 x 77 x 194 f32 cut and whole 41 + 74 and 28 + 59 us a call. On the device alone,
+    as in a graph, it is the other way (20 + 39 and 23 + 52 us). Other lengths on that side were
+    not measured; 128 is where a row gives eight chunks.
 
     Forward and gradient, bf16, 16 states, us whole and cut: 64 x 1024 x 512 in 2 323 + 797 and
     467 + 1045; 48 rows in 3 323 + 795 and 312 + 716; 16 x 512 x 512 in 8 133 + 266 and 69 + 152;
