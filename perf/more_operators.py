@@ -90,7 +90,7 @@ def draw(rng):
                     activation=rng.choice(["none", "silu", "silu"]), dtype=dtype)
     groups = rng.choice([1, 2, 4, 8])
     heads = groups * rng.choice([1, 1, 1, 2, 3])
-    keys, values = (rng.choice([16, 32, 64, 64, 128, rng.randint(1, 128)]) for _ in range(2))
+    keys, values = (rng.choice([16, 32, 64, 64, 128, rng.randint(4, 128)]) for _ in range(2))
     case = dict(op=op, groups=groups, heads=heads, keys=keys, values=values, dtype=dtype)
     if op == "delta_step":
         rows = _log_int(rng, 1, max(1, min(2048, (1 << 26) // (heads * keys * values))))
