@@ -1,0 +1,337 @@
+// policy_loss.cu — clipped policy loss with a KL term from rows of logits, and its gradient
+// (sm_100a).
+//
+// Row n: logits z, temperature t, y = z / t, lse = log sum e^y, p = e^(y - lse); of its answer a
+//   lp = y_a - lse,  r = exp(lp - old),  d = ref - lp,  H = -sum p log p
+//   L  = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl (e^d - d - 1) - ent H
+//   loss = sum_n w_n L_n
+// and with c = w (kl (1 - e^d) - [r A <= clip(r) A] r A)
+//   dz_j = (c ([j = a] - p_j) + w ent p_j (log p_j + H)) / t.
+//
+// One pass over memory: a row's logits stay in shared memory (registers, where a warp takes a
+// row) between the pass that sums and the one that writes the gradient.
+#include <cooperative_groups.h>
+
+#include "seq_common.cuh"
+
+namespace {
+
+using namespace seqk;
+namespace cg = cooperative_groups;
+
+struct LossArgs {
+  const void* z;
+  const void* answers;         // int32 or int64
+  const float *old_logp, *adv, *ref, *weight;       // ref, weight: null for none, 1 / rows
+  void* dz;                    // or null
+  float* rows;                 // [3, R]: log-probability, KL, entropy
+  float* each;                 // [R]: w L
+  float* loss;
+  int* err;
+  int64_t z_ld, d_ld;
+  int64_t n;
+  int v, wide;                 // candidates; 1: int64 answers
+  float lo, hi, kl, ent, inv_t, share;
+};
+static_assert(sizeof(LossArgs) == 11 * 8 + 3 * 8 + 8 * 4, "as the caller packs it");
+
+struct Row {
+  int64_t n;
+  int a;                       // the answer, -1: counts nothing
+};
+
+__device__ __forceinline__ Row row_of(const LossArgs& p, int64_t n, bool report) {
+  const int64_t a = p.wide ? static_cast<const int64_t*>(p.answers)[n] : static_cast<const int*>(p.answers)[n];
+  if (a >= p.v && report) surfk::report_error(p.err, surfk::kErrLossIndex);
+  return {n, a >= 0 && a < p.v ? static_cast<int>(a) : -1};
+}
+
+// running maximum m, sum of e^(y - m) and of (y - m) e^(y - m)
+struct Sums { float m, s, t; };
+// NaN logits count as -inf
+__device__ __forceinline__ float clean(float z) { return z == z ? z : -INFINITY; }
+// the exponent of z under the maximum m: 0 for the largest, infinite ones among them
+__device__ __forceinline__ float below(float z, float m, float inv_t) { return z == m ? 0.0f : (z - m) * inv_t; }
+__device__ __forceinline__ void add(Sums& a, float z, float inv_t) {
+  const float y = below(z, a.m, inv_t), e = __expf(y);
+  a.s += e;
+  if (e > 0.0f) a.t = fmaf(e, y, a.t);
+}
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float inv_t) {
+  const float m = fmaxf(a.m, b.m);
+  Sums r{m, 0.0f, 0.0f};
+  if (a.s > 0.0f) {
+    const float y = below(a.m, m, inv_t), f = expf(y);
+    r.s = a.s * f;
+    if (f > 0.0f) r.t = f * fmaf(a.s, y, a.t);
+  }
+  if (b.s > 0.0f) {
+    const float y = below(b.m, m, inv_t), f = expf(y);
+    r.s = fmaf(b.s, f, r.s);
+    if (f > 0.0f) r.t += f * fmaf(b.s, y, b.t);
+  }
+  return r;
+}
+
+// What the gradient needs of a row: dz = k_p p + k_e p log p (+ k_a at the answer), times 1 / t inside
+struct Slopes {
+  int a;
+  float m, log_s, inv_s, kp, ke, ka;
+};
+
+// The row's numbers from its sums; `za` the answer's logit. Written by one thread.
+__device__ __forceinline__ Slopes finish(const LossArgs& p, const Row& row, const Sums& s, float za, bool write) {
+  Slopes g{-1, s.m, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  float lp = 0.0f, kl = 0.0f, ent = 0.0f, each = 0.0f;
+  if (row.a >= 0 && za > -INFINITY) {
+    const float w = p.weight ? p.weight[row.n] : p.share, adv = p.adv[row.n];
+    // the logarithm of the sum and what is subtracted from it in 64 bits: log-probabilities and
+    // small KL terms are differences of larger numbers
+    const double log_s = log(static_cast<double>(s.s));
+    const double y = za == s.m ? 0.0 : (static_cast<double>(za) - s.m) * p.inv_t;
+    const double l = y - log_s;
+    lp = static_cast<float>(l);
+    ent = static_cast<float>(log_s - static_cast<double>(s.t) / s.s);
+    const float ratio = expf(static_cast<float>(l - p.old_logp[row.n]));
+    const float held = fminf(fmaxf(ratio, 1.0f - p.lo), 1.0f + p.hi);
+    const float free = adv == 0.0f ? 0.0f : ratio * adv, cut = held * adv;
+    float c = free <= cut ? -free : 0.0f;
+    each = -fminf(free, cut);
+    if (p.ref) {
+      const double d = p.ref[row.n] - l;
+      const double e = expm1(d);
+      kl = static_cast<float>(e - d);
+      each = fmaf(p.kl, kl, each);
+      c = fmaf(p.kl, -static_cast<float>(e), c);
+    }
+    each = w * fmaf(-p.ent, ent, each);
+    c *= w;
+    g.a = row.a;
+    g.log_s = static_cast<float>(log_s);
+    g.inv_s = 1.0f / s.s;
+    g.ka = c * p.inv_t;
+    g.ke = w * p.ent * p.inv_t;
+    g.kp = fmaf(g.ke, ent, -g.ka);
+  }
+  if (write) {
+    p.rows[row.n] = lp;
+    p.rows[p.n + row.n] = kl;
+    p.rows[2 * p.n + row.n] = ent;
+    p.each[row.n] = each;
+  }
+  return g;
+}
+__device__ __forceinline__ float slope(const Slopes& g, float z, int j, float inv_t) {
+  const float y = below(z, g.m, inv_t), pr = __expf(y) * g.inv_s;
+  float d = pr > 0.0f ? pr * fmaf(g.ke, y - g.log_s, g.kp) : 0.0f;
+  if (j == g.a) d += g.ka;
+  return g.a < 0 ? 0.0f : d;
+}
+
+// The rows' losses summed in a fixed order: a kernel of its own, since a counter of arrivals would
+// have to be shared by calls on different streams or cleared by a launch too.
+constexpr int kSumThreads = 512;
+__global__ void __launch_bounds__(kSumThreads) loss_sum(const float* each, int64_t n, float* loss) {
+  __shared__ double red[kSumThreads / 32];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += kSumThreads) s += each[i];
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kSumThreads / 32; ++i) s += red[i];
+    *loss = static_cast<float>(s);
+  }
+}
+
+// ---- a warp for a row -----------------------------------------------------------------
+constexpr int kWarpThreads = 256;
+
+template <typename T, int H> __global__ void __launch_bounds__(kWarpThreads) loss_warp(LossArgs p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * (kWarpThreads / 32) + (threadIdx.x >> 5);
+  if (n < p.n) {
+    const Row row = row_of(p, n, lane == 0);
+    const T* z = static_cast<const T*>(p.z) + n * p.z_ld;
+    float v[H], m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      v[k] = k * 32 + lane < p.v ? clean(to_f(z[k * 32 + lane])) : -INFINITY;
+      m = fmaxf(m, v[k]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    Sums s{m, 0.0f, 0.0f};
+    float za = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      if (v[k] > -INFINITY) add(s, v[k], p.inv_t);
+      if (k * 32 + lane == row.a) za = v[k];
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      s.s += __shfl_xor_sync(0xffffffffu, s.s, o);
+      s.t += __shfl_xor_sync(0xffffffffu, s.t, o);
+      za = fmaxf(za, __shfl_xor_sync(0xffffffffu, za, o));
+    }
+    const Slopes g = finish(p, row, s, za, lane == 0);
+    if (p.dz) {
+      T* d = static_cast<T*>(p.dz) + n * p.d_ld;
+#pragma unroll
+      for (int k = 0; k < H; ++k)
+        if (k * 32 + lane < p.v) d[k * 32 + lane] = from_f<T>(slope(g, v[k], k * 32 + lane, p.inv_t));
+    }
+  }
+}
+
+// ---- a cluster of blocks for a row ------------------------------------------------------
+constexpr int kRowThreads = 512;
+
+// A block takes candidates [lo, hi) of its row; shared memory mirrors their place within 16 bytes
+// of global memory, so that all but the ends move in pieces of 16 bytes.
+template <typename T> __global__ void __launch_bounds__(kRowThreads) loss_row(LossArgs p, int per) {
+  constexpr int V = kVec16<T>;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ Sums part[kRowThreads / 32], mine;
+  __shared__ float answer;
+  __shared__ Slopes slopes;
+  cg::cluster_group cl = cg::this_cluster();
+  const int ranks = cl.num_blocks(), rank = cl.block_rank();
+  const int64_t n = blockIdx.x / ranks;
+  const Row row = row_of(p, n, rank == 0 && threadIdx.x == 0);
+  const int first = min(rank * per, p.v), count = min(per, p.v - first);
+  const T* z = static_cast<const T*>(p.z) + n * p.z_ld + first;
+  T* hold = reinterpret_cast<T*>(smem) + (reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T);
+  const int head = min(count, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) / sizeof(T)) % V);
+  const int whole = (count - head) / V;
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < whole; i += kRowThreads) {
+    float v[V];
+    load_vec<T, V>(z + head + i * V, v);
+    *reinterpret_cast<uint4*>(hold + head + i * V) = *reinterpret_cast<const uint4*>(z + head + i * V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = fmaxf(m, clean(v[j]));
+  }
+  const int rest = count - whole * V;                  // the ends: [0, head) and behind the pieces
+  for (int i = threadIdx.x; i < rest; i += kRowThreads) {
+    const int at = i < head ? i : i + whole * V;
+    hold[at] = z[at];
+    m = fmaxf(m, clean(to_f(z[at])));
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5].m = m;
+  __syncthreads();
+  for (int i = 0; i < kRowThreads / 32; ++i) m = fmaxf(m, part[i].m);
+  __syncthreads();
+  Sums s{m, 0.0f, 0.0f};
+  if (m > -INFINITY) {
+    for (int i = threadIdx.x; i < whole; i += kRowThreads) {
+      float v[V];
+      load_vec<T, V>(hold + head + i * V, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float q = clean(v[j]);
+        if (q > -INFINITY) add(s, q, p.inv_t);
+      }
+    }
+    for (int i = threadIdx.x; i < rest; i += kRowThreads) {
+      const float q = clean(to_f(hold[i < head ? i : i + whole * V]));
+      if (q > -INFINITY) add(s, q, p.inv_t);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    s.s += __shfl_xor_sync(0xffffffffu, s.s, o);
+    s.t += __shfl_xor_sync(0xffffffffu, s.t, o);
+  }
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kRowThreads / 32; ++i) {
+      s.s += part[i].s;
+      s.t += part[i].t;
+    }
+    mine = s;
+    answer = row.a >= first && row.a < first + count ? clean(to_f(hold[row.a - first])) : -INFINITY;
+  }
+  if (ranks > 1) cl.sync(); else __syncthreads();
+  if (threadIdx.x == 0) {
+    Sums all = mine;
+    float za = answer;
+    if (ranks > 1) {
+      all = *cl.map_shared_rank(&mine, 0);
+      za = *cl.map_shared_rank(&answer, 0);
+      for (int i = 1; i < ranks; ++i) {
+        all = join(all, *cl.map_shared_rank(&mine, i), p.inv_t);
+        za = fmaxf(za, *cl.map_shared_rank(&answer, i));
+      }
+    }
+    slopes = finish(p, row, all, za, rank == 0);
+  }
+  if (ranks > 1) cl.sync(); else __syncthreads();      // the others' shared memory is read no more
+  if (p.dz) {
+    const Slopes g = slopes;
+    const int at_answer = g.a - first;
+    T* d = static_cast<T*>(p.dz) + n * p.d_ld + first;
+    const bool same = ((reinterpret_cast<uintptr_t>(d) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
+    Slopes q = g;
+    q.a = g.a < 0 ? -1 : 0;
+    for (int i = threadIdx.x; i < whole; i += kRowThreads) {
+      const int at = head + i * V;
+      float v[V];
+      load_vec<T, V>(hold + at, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = slope(q, clean(v[j]), at + j == at_answer ? 0 : 1, p.inv_t);
+      if (same) {
+        store_vec<T, V>(d + at, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[at + j] = from_f<T>(v[j]);
+      }
+    }
+    for (int i = threadIdx.x; i < rest; i += kRowThreads) {
+      const int at = i < head ? i : i + whole * V;
+      d[at] = from_f<T>(slope(q, clean(to_f(hold[at])), at == at_answer ? 0 : 1, p.inv_t));
+    }
+  }
+}
+
+template <typename T> int run(const LossArgs& a, int ranks, int per, cudaStream_t s) {
+  if (ranks == 0) {
+    const unsigned grid = static_cast<unsigned>((a.n + kWarpThreads / 32 - 1) / (kWarpThreads / 32));
+    if (a.v <= 32) loss_warp<T, 1><<<grid, kWarpThreads, 0, s>>>(a);
+    else if (a.v <= 128) loss_warp<T, 4><<<grid, kWarpThreads, 0, s>>>(a);
+    else if (a.v <= 512) loss_warp<T, 16><<<grid, kWarpThreads, 0, s>>>(a);
+    else return static_cast<int>(cudaErrorInvalidValue);
+    if (const cudaError_t e = cudaGetLastError()) return static_cast<int>(e);
+    loss_sum<<<1, kSumThreads, 0, s>>>(a.each, a.n, a.loss);
+    return static_cast<int>(cudaGetLastError());
+  }
+  const size_t smem = (static_cast<size_t>(per) * sizeof(T) + 31) / 16 * 16;
+  if (smem > 200 * 1024 || ranks > 8) return static_cast<int>(cudaErrorInvalidValue);
+  if (const int e = allow_smem<loss_row<T>>(200 * 1024)) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.n * ranks));
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (const cudaError_t e = cudaLaunchKernelEx(&cfg, loss_row<T>, a, per)) return static_cast<int>(e);
+  loss_sum<<<1, kSumThreads, 0, s>>>(a.each, a.n, a.loss);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace
+
+// args: a LossArgs; ranks: blocks of a row (0: a warp), per: candidates of a block
+SURF_EXPORT int surf_policy_loss(const void* args, int dtype, int ranks, int per, void* stream) {
+  const LossArgs& a = *static_cast<const LossArgs*>(args);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == kBf16 ? run<bf16>(a, ranks, per, s) : run<float>(a, ranks, per, s);
+}

@@ -61,9 +61,10 @@ def _targets():
                            [str(CSRC / "sim" / "tests" / "gates.cpp")], [], [])}
     groups = {
         "libsurf_vision.so": kern("march.cu", "sdf.cu", "geodesic.cu"),
-        "libsurf_rl.so": kern("rl.cu", "reward.cu"),
+        "libsurf_rl.so": kern("rl.cu", "reward.cu", "policy_loss.cu"),
         "libsurf_nn.so": kern("gemm_tc.cu", "conv_shift.cu", "nn_ops.cu", "adam.cu"),
         "libsurf_seq.so": kern("seq_conv.cu", "seq_scan.cu", "seq_scan_grad.cu", "tokens.cu"),
+        "libsurf_delta.so": kern("delta.cu", "delta_grad.cu", "group_norm.cu"),
         "libsurf_comm.so": comm("p2p.cu"),
     }
     for name, srcs in groups.items():

@@ -5,6 +5,8 @@
 * ``adv_moments`` — per-minibatch advantage moments for a whole epoch;
 * ``ppo_loss`` — clipped PPO objective with its gradient w.r.t. the logits,
   value and log-std in closed form;
+* ``policy_loss`` — clipped policy loss with a KL term for sampled answers,
+  from their logits, with its gradient (csrc/kernels/policy_loss.cu);
 * ``Adam`` — global-norm clip fused with Adam on the flat parameter buffer.
 
 Each ``*_reference`` function is the fp32 PyTorch statement of the same rule
@@ -14,6 +16,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
+from collections import namedtuple
 from ctypes import c_float, c_int, c_int64, c_uint64, c_void_p
 from typing import Optional
 
@@ -40,7 +44,9 @@ _lib.register(RLIB, {
                               c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
                               c_float, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
                               c_void_p, c_int64, c_void_p, c_void_p]),
+    "surf_policy_loss": (c_int, [ctypes.c_char_p, c_int, c_int, c_int, c_void_p]),
 })
+_lib._KERNELS_PER_CALL["surf_policy_loss"] = 2
 
 LOG_SQRT_2PI = 0.9189385332046727
 
@@ -281,6 +287,117 @@ def ppo_loss_reference(logits_value, value_col: int, act, old_logp, adv, ret, la
     vl = 0.5 * (value - ret).pow(2).mean()
     el = -ent.mean()
     return pg + vf_coef * vl + ent_coef * el, pg, vl, -el
+
+
+# ---- policy loss over sampled answers ----------------------------------------------------
+MAX_ANSWERS = 262144               # candidates of a row, as of ``ops.tokens.sample_tokens``
+_LOSS = struct.Struct("11q3q2i6f")
+PolicyLoss = namedtuple("PolicyLoss", "loss logp kl entropy dlogits")
+
+
+def _loss_rows(name: str, t, rows: int, device) -> None:
+    if t is not None and (t.shape != (rows,) or t.dtype != torch.float32 or t.device != device or not t.is_contiguous()):
+        raise ValueError(f"policy_loss: {name} must be a contiguous float32 tensor [{rows}] on {device}")
+
+
+def _loss_blocks(rows: int, v: int, e: int):
+    """(blocks of a row, candidates of a block); no block: a warp takes the row."""
+    if v <= 512:
+        return 0, v
+    ranks = 1
+    while ranks < 8 and (v * e > ranks * 100 * 1024 or (rows * ranks < 148 and v * e > ranks * 16384)):
+        ranks *= 2
+    return ranks, -(-v // (ranks * 16)) * 16
+
+
+def policy_loss(logits: torch.Tensor, answers: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor, *,
+                ref_logp: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None, clip: float = 0.2,
+                clip_high: Optional[float] = None, kl_coef: float = 0.0, ent_coef: float = 0.0, temperature: float = 1.0,
+                grad: bool = True, out: Optional[torch.Tensor] = None) -> PolicyLoss:
+    """Clipped policy loss of one answer a row, with its gradient: with lp the log-probability of
+    ``answers`` [R] (int32 or int64) under softmax(``logits`` [R, V] / ``temperature``),
+    r = exp(lp - ``old_logp``), d = ``ref_logp`` - lp and H the entropy,
+
+        loss = sum_n weights[n] (-min(r A, clip(r, 1 - clip, 1 + clip_high) A) + kl_coef (e^d - d - 1) - ent_coef H)
+
+    ``weights`` None: 1 / R each; ``clip_high`` None: ``clip``; ``ref_logp`` None: no KL term. Logits are
+    bfloat16 or float32, their rows any stride apart; NaN counts as -inf. A row whose answer is
+    negative or has a logit of -inf counts nothing and gets zeros. An answer past the row does too, and is
+    reported through ``ops.gemm.check_error_flag``. ``logp``, ``kl`` and ``entropy`` [R] are float32, ``dlogits`` has
+    the logits' type (None without ``grad``) and may be written to ``out``, the logits themselves among others. The
+    temperature must be positive: an answer that was taken greedily has no probability to move.
+    Where r A ties with its clipped value its gradient passes."""
+    what = "policy_loss"
+    _lib.require_cuda(logits, what)
+    if logits.dim() != 2:
+        raise ValueError(f"{what}: logits must be [rows, candidates]")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{what}: logits must be bfloat16 or float32, not {logits.dtype}")
+    rows, v = logits.shape
+    dev, e = logits.device, logits.element_size()
+    if not 1 <= v <= MAX_ANSWERS:
+        raise ValueError(f"{what}: 1 to {MAX_ANSWERS} candidates, not {v}")
+    if v > 1 and logits.stride(1) != 1:
+        raise ValueError(f"{what}: logits need a dense last axis")
+    if answers.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: answers must be int32 or int64, not {answers.dtype}")
+    if answers.shape != (rows,) or answers.device != dev or not answers.is_contiguous():
+        raise ValueError(f"{what}: answers must be a contiguous tensor [{rows}] on {dev}")
+    for name, t in (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp), ("weights", weights)):
+        _loss_rows(name, t, rows, dev)
+    high = clip if clip_high is None else clip_high
+    if not 0 <= clip <= 1 or not 0 <= high < math.inf:
+        raise ValueError(f"{what}: clip lies in [0, 1], clip_high in [0, inf)")
+    if not 0 < temperature < math.inf:
+        raise ValueError(f"{what}: the temperature must be positive and finite")
+    if not (math.isfinite(kl_coef) and math.isfinite(ent_coef)):
+        raise ValueError(f"{what}: kl_coef and ent_coef must be finite")
+    if out is not None:
+        if not grad:
+            raise ValueError(f"{what}: out without grad")
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (v > 1 and out.stride(1) != 1):
+            raise ValueError(f"{what}: out must be like the logits, with a dense last axis")
+        _lib.require_apart(what, "out", out, dict(logits=logits, answers=answers, old_logp=old_logp, advantages=advantages,
+                                                  ref_logp=ref_logp, weights=weights), ("logits",))
+    elif grad:
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(logits.shape)
+    stats = torch.empty(4 * rows + 1, dtype=torch.float32, device=dev)
+    loss = stats[4 * rows]
+    result = PolicyLoss(loss, stats[:rows], stats[rows:2 * rows], stats[2 * rows:3 * rows], out)
+    if rows == 0:
+        loss.zero_()
+        return result
+    base = stats.data_ptr()
+    args = _LOSS.pack(logits.data_ptr(), answers.data_ptr(), old_logp.data_ptr(), advantages.data_ptr(), ptr(ref_logp), ptr(weights),
+                      ptr(out), base, base + 12 * rows, base + 16 * rows, _error_flag(dev).data_ptr(),
+                      logits.stride(0), out.stride(0) if out is not None else 0, rows, v, int(answers.dtype == torch.int64),
+                      clip, high, kl_coef, ent_coef, 1.0 / temperature, 1.0 / rows)
+    _lib.launch(_lib.lib(RLIB).surf_policy_loss, "surf_policy_loss", logits.get_device(), args,
+                int(logits.dtype == torch.bfloat16), *_loss_blocks(rows, v, e))
+    return result
+
+
+def policy_loss_reference(logits, answers, old_logp, advantages, *, ref_logp=None, weights=None, clip=0.2, clip_high=None,
+                          kl_coef=0.0, ent_coef=0.0, temperature=1.0):
+    """The scalar loss from its definition, in the logits' type (differentiable)."""
+    rows = logits.shape[0]
+    z = torch.where(logits.isnan(), torch.full_like(logits, float("-inf")), logits) / temperature
+    at = answers.long().clamp(min=0)
+    on = (answers >= 0) & (z.gather(1, at[:, None])[:, 0] > float("-inf"))
+    z = torch.where(on[:, None], z, torch.zeros_like(z))
+    logp = torch.log_softmax(z, 1)
+    lp = logp.gather(1, at[:, None])[:, 0]
+    live = logp > float("-inf")
+    safe = torch.where(live, logp, torch.zeros_like(logp))
+    ent = -(torch.where(live, torch.exp(safe), torch.zeros_like(safe)) * safe).sum(1)
+    ratio = torch.exp(lp - old_logp)
+    held = torch.clamp(ratio, 1 - clip, 1 + (clip if clip_high is None else clip_high))
+    each = -torch.minimum(ratio * advantages, held * advantages) - ent_coef * ent
+    if ref_logp is not None:
+        d = ref_logp - lp
+        each = each + kl_coef * (torch.exp(d) - d - 1)
+    w = weights if weights is not None else torch.full_like(each, 1.0 / max(1, rows))
+    return torch.where(on, w * each, torch.zeros_like(each)).sum()
 
 
 # ---- optimizer ------------------------------------------------------------------------------
