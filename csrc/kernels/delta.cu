@@ -7,38 +7,119 @@ namespace {
 using namespace delta;
 
 // ---- sequences --------------------------------------------------------------------------
+constexpr int kPrep = 2;                               // warps that make chunks ready
+
 template <typename T, int DK> struct Forward {
+  // chunks ready, in the making or on their way: three for each of the warps, two where they would not fit
+  static constexpr int kStages = sizeof(T) == 4 && DK == 128 ? 2 * kPrep : 3 * kPrep;
   using Keys = Tile<T, DK>;
-  using Values = Tile<T, 128>;                         // pitch of the values' rows, whatever their number
-  static constexpr size_t kBytes = sizeof(Chunk<T>) + (2 * Keys::kSize + Values::kSize) * sizeof(bf16) +
-                                   static_cast<size_t>(kTile) * (128 + 16 / sizeof(T)) * sizeof(T);
+  static_assert(kStages % kPrep == 0, "a stage's barriers are one warp's");
+  struct Stage {
+    Chunk<T, Planes<T>::kShort> c;
+    int t0, n, fresh;
+    alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize];
+  };
+  struct Shared {
+    Stage stage[kStages];
+    alignas(16) Scratch scratch[kPrep];
+  };
+  static constexpr int kRow = 16 + 16 / static_cast<int>(sizeof(T));     // pitch of a warp's outputs
+  // behind them: the values' rows of each stage, the outputs of each warp
+  static __host__ __device__ constexpr int pitch_v(int warps) { return warps * 16 + 16 / static_cast<int>(sizeof(T)); }
+  static __host__ __device__ constexpr size_t bytes(int warps) {
+    return sizeof(Shared) + (static_cast<size_t>(kStages) * kTile * pitch_v(warps) + static_cast<size_t>(warps) * kTile * kRow) * sizeof(T);
+  }
 };
 
-// A block for a sequence's value head, a warp for 16 of its values: their rows of the state are
-// the warp's accumulators from the first token to the last.
-template <typename T, int DK> __global__ void __launch_bounds__(256) delta_forward(DeltaArgs a) {
-  constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, kSteps = DK / 16;
+// A block for up to 128 values of a sequence's value head. Two warps make the chunks ready in turn
+// (tiles, decays, P, the inverse: nothing of it waits for the state), the others hold 16 values'
+// rows of the state each, as accumulators from the first token to the last. They meet at
+// numbered barriers: stage s is ready (1 + s), stage s is free (1 + kStages + s).
+template <typename T, int DK> __global__ void __launch_bounds__(320) delta_forward(DeltaArgs a) {
+  constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort, kSteps = DK / 16;
+  using F = Forward<T, DK>;
   using Keys = Tile<T, DK>;
-  using Values = Tile<T, 128>;
+  constexpr int kStages = F::kStages;
   extern __shared__ __align__(16) char smem[];
-  Chunk<T>& c = *reinterpret_cast<Chunk<T>*>(smem);
-  bf16* tk = reinterpret_cast<bf16*>(smem + sizeof(Chunk<T>));
-  bf16* tq = tk + Keys::kSize;
-  bf16* tv = tq + Keys::kSize;
-  T* so = reinterpret_cast<T*>(tv + Values::kSize);
-  constexpr int kOut = 128 + 16 / static_cast<int>(sizeof(T));
+  typename F::Shared& sh = *reinterpret_cast<typename F::Shared*>(smem);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x / 32 - kPrep;
+  const int pitch_v = F::pitch_v(warps), threads = (warps + 1) * 32;
+  T* values = reinterpret_cast<T*>(smem + sizeof(typename F::Shared));
   const int bi = blockIdx.x / a.heads, h = blockIdx.x % a.heads, gr = h / (a.heads / a.groups);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = lane >> 2, col = (lane & 3) * 2;
-  const int v0 = warp * 16;
+  const int vb = blockIdx.y * warps * 16, mine = min(warps * 16, a.values - vb);
   const int length = a.lengths ? max(0, min(a.lengths[bi], a.length)) : a.length;
-  const uint8_t* reset = a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr;
-  const T* q = static_cast<const T*>(a.q) + bi * a.q_b + gr * a.q_g;
-  const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
-  const T* v = static_cast<const T*>(a.v) + bi * a.v_b + h * a.v_h;
-  const T* dt = static_cast<const T*>(a.dt) + bi * a.dt_b + h;
-  const T* gb = static_cast<const T*>(a.b) + bi * a.b_b + h;
+
+  if (warp >= warps) {
+    const int w = warp - warps;
+    const T* q = static_cast<const T*>(a.q) + bi * a.q_b + gr * a.q_g;
+    const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
+    const T* v = static_cast<const T*>(a.v) + bi * a.v_b + h * a.v_h + vb;
+    const T* dt = static_cast<const T*>(a.dt) + bi * a.dt_b + h;
+    const T* gb = static_cast<const T*>(a.b) + bi * a.b_b + h;
+    const float rate = rate_at(a.A, h), bias = a.bias ? a.bias[h] : 0.0f;
+    Chunks walk(a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length);
+    // at chunk `to`, or past the last: index is then their number
+    int index = -1;
+    bool more = true;
+    auto advance = [&](int to) {
+      while (more && index < to) {
+        more = walk.next();
+        ++index;
+      }
+    };
+    // chunk i's tokens on their way to its stage, its gates in registers
+    float raw_dt = 0.0f, raw_b = 0.0f;
+    int at = 0, n = 0;
+    auto fetch = [&](int i) {
+      at = i % kStages;
+      typename F::Stage& st = sh.stage[at];
+      if (i >= kStages) bar_sync(1 + kStages + at, threads);
+      const int t0 = walk.t0;
+      n = walk.n;
+      if (lane == 0) {
+        st.t0 = t0;
+        st.n = n;
+        st.fresh = walk.fresh;
+      }
+      Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k, lane, 32);
+      Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k, lane, 32);
+      load_rows(values + at * kTile * pitch_v, pitch_v, kTile, warps * 16, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
+      cp_async_commit();
+      if (lane < n) {
+        raw_dt = to_f(dt[(t0 + lane) * a.dt_t]);
+        raw_b = to_f(gb[(t0 + lane) * a.b_t]);
+      }
+    };
+    auto finish = [&] {                                // the end is the warp's to say whose chunk it would be
+      if (index % kPrep != w) return;
+      const int to = index % kStages;
+      if (index >= kStages) bar_sync(1 + kStages + to, threads);
+      if (lane == 0) sh.stage[to].n = 0;
+      __syncwarp();
+      bar_arrive(1 + to, threads);
+    };
+    advance(w);
+    if (!more) return finish();
+    fetch(w);
+    for (int i = w;; i += kPrep) {
+      typename F::Stage& st = sh.stage[at];
+      const int here = at;
+      Gate e{};
+      if (lane < n) e = gate_of(raw_dt, raw_b, bias, rate);
+      advance(i + kPrep);
+      if (more) fetch(i + kPrep);
+      else cp_async_commit();
+      cp_async_wait<1>();
+      __syncwarp();
+      prepare<T, DK, false>(st.c, sh.scratch[w], nullptr, st.tk, st.tq, e.g, e.beta, a.scale, a.unit);
+      bar_arrive(1 + here, threads);
+      if (!more) return finish();
+    }
+  }
+
+  const int row = lane >> 2, col = (lane & 3) * 2, vl = warp * 16, v0 = vb + vl;
   T* out = static_cast<T*>(a.out) + bi * a.o_b + h * a.o_h;
-  const float rate = rate_at(a.A, h), bias = a.bias ? a.bias[h] : 0.0f;
+  T* so = values + kStages * kTile * pitch_v + warp * kTile * F::kRow;
   const int64_t head_size = static_cast<int64_t>(a.values) * a.keys;
   const int64_t head_at = (static_cast<int64_t>(bi) * a.heads + h) * head_size;
   const bool pairs = (a.keys & 1) == 0;
@@ -51,10 +132,10 @@ template <typename T, int DK> __global__ void __launch_bounds__(256) delta_forwa
 #pragma unroll
       for (int e = 0; e < 2; ++e) f(s[n][2 * e], s[n][2 * e + 1], v0 + row + 8 * e, 8 * n + col);
   };
-  auto store = [&](float* to) {
+  auto store = [&](float* to, int pitch) {
     each([&](float x, float y, int r, int kc) {
       if (r >= a.values || kc >= a.keys) return;
-      float* p = to + static_cast<int64_t>(r) * a.keys + kc;
+      float* p = to + r * pitch + kc;
       if (pairs) {
         *reinterpret_cast<float2*>(p) = make_float2(x, y);
       } else {
@@ -65,40 +146,27 @@ template <typename T, int DK> __global__ void __launch_bounds__(256) delta_forwa
   };
   each([&](float& x, float& y, int r, int kc) {
     const bool on = a.state && r < a.values;
-    const float* p = a.state + head_at + static_cast<int64_t>(r) * a.keys + kc;
+    const float* p = a.state + head_at + r * a.keys + kc;
     x = on && kc < a.keys ? p[0] : 0.0f;
     y = on && kc + 1 < a.keys ? p[1] : 0.0f;
   });
 
   const int tiles = (a.length + kTile - 1) / kTile;
-  int t0 = 0;
-  while (t0 < length) {
-    const int n = chunk_tokens(reset, t0, length);
-    const bool fresh = reset && reset[t0];
-    if (a.saved && t0 % kTile == 0)
-      store(a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * head_size);
-    if (fresh) each([&](float& x, float& y, int, int) { x = y = 0.0f; });
-    __syncthreads();
-    Keys::load(tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k, threadIdx.x, blockDim.x);
-    Keys::load(tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k, threadIdx.x, blockDim.x);
-    Values::load(tv, v + t0 * a.v_t, a.v_t, n, a.values, a.piece_v, threadIdx.x, blockDim.x);
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncthreads();
-    if (warp == 0) {
-      float g = 0.0f, beta = 0.0f;
-      if (lane < n) {
-        const Gate e = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
-        g = e.g;
-        beta = e.beta;
-      }
-      prepare<T, DK, false>(c, tk, tq, g, beta, a.scale, a.unit);
-    }
-    __syncthreads();
+  for (int i = 0;; ++i) {
+    const int at = i % kStages;
+    typename F::Stage& st = sh.stage[at];
+    bar_sync(1 + at, threads);
+    const int t0 = st.t0, n = st.n;
+    if (n == 0) break;
+    const Chunk<T, NS>& c = st.c;
+    float* saved = a.saved ? a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values * (a.keys + kTile) : nullptr;
+    if (saved && t0 % kTile == 0) store(saved, a.keys + kTile);
+    if (st.fresh) each([&](float& x, float& y, int, int) { x = y = 0.0f; });
+    const T* tv = values + at * kTile * pitch_v;
 
     // K S^T and Q S^T, transposed: rows values, columns tokens
     float sk[2][4] = {}, sq[2][4] = {};
-    const uint32_t ka = smem_of(tk) + at_rows(lane, Keys::kPitch), qa = smem_of(tq) + at_rows(lane, Keys::kPitch);
+    const uint32_t ka = smem_of(st.tk) + at_rows(lane, Keys::kPitch), qa = smem_of(st.tq) + at_rows(lane, Keys::kPitch);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       Frag<NI> f;
@@ -107,7 +175,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(256) delta_forwa
       load_planes<NT, false>(b, ka + i * 32, Keys::kPlane * 2);
       mma_planes<NI, NT>(sk[0], sk[1], f.r, b);
       load_planes<NT, false>(b, qa + i * 32, Keys::kPlane * 2);
-      mma_planes<NI, NT>(sq[0], sq[1], f.r, b);
+      mma_planes<NS, NT>(sq[0], sq[1], f.r, b);
     }
     float w[2][4] = {};
     {
@@ -115,8 +183,8 @@ template <typename T, int DK> __global__ void __launch_bounds__(256) delta_forwa
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int tok = t * 8 + col + (e & 1), r = v0 + row + (e >> 1) * 8;
-          sk[t][e] = tile_at<T>(tv, Values::kPlane, tok * Values::kPitch + r) - c.head[tok] * c.rk[tok] * sk[t][e];
+          const int tok = t * 8 + col + (e & 1), r = vl + row + (e >> 1) * 8;
+          sk[t][e] = to_f(tv[tok * pitch_v + r]) - c.head[tok] * c.rk[tok] * sk[t][e];
           sq[t][e] *= a.scale * c.head[tok] * c.rq[tok];
         }
       Frag<NI> f;
@@ -125,20 +193,30 @@ template <typename T, int DK> __global__ void __launch_bounds__(256) delta_forwa
       load_planes<NI, false>(b, smem_of(c.inv) + at_rows(lane, kSide), kTile * kSide * 2);
       mma_planes<NI, NI>(w[0], w[1], f.r, b);
     }
+    if (saved) {
+      float* p = saved + a.keys + t0 % kTile;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int tok = t * 8 + col + (e & 1), r = v0 + row + (e >> 1) * 8;
+          if (tok < n && r < a.values) p[r * (a.keys + kTile) + tok] = w[t][e];
+        }
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[t][e] *= c.beta[t * 8 + col + (e & 1)];
     {
-      Frag<NI> f;
+      Frag<NS> f;
       f.from(w[0], w[1]);
-      uint32_t b[NI][4];
-      load_planes<NI, false>(b, smem_of(c.p) + at_rows(lane, kSide), kTile * kSide * 2);
-      mma_planes<NI, NI>(sq[0], sq[1], f.r, b);
+      uint32_t b[NS][4];
+      load_planes<NS, false>(b, smem_of(c.p) + at_rows(lane, kSide), kTile * kSide * 2);
+      mma_planes<NS, NS>(sq[0], sq[1], f.r, b);
     }
     // the state
-    const float end = c.head[kTile - 1];
     {
+      const float end = c.head[kTile - 1];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -148,7 +226,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(256) delta_forwa
         }
       Frag<NI> f;
       f.from(w[0], w[1]);
-      const uint32_t kt = smem_of(tk) + at_cols(lane, Keys::kPitch);
+      const uint32_t kt = smem_of(st.tk) + at_cols(lane, Keys::kPitch);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
@@ -161,37 +239,42 @@ template <typename T, int DK> __global__ void __launch_bounds__(256) delta_forwa
         mma_planes<NI, NT>(s[2 * i], s[2 * i + 1], f.r, b);
       }
     }
+    bar_arrive(1 + kStages + at, threads);
     // the outputs, by tokens
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) so[(t * 8 + col + (e & 1)) * kOut + v0 + row + (e >> 1) * 8] = from_f<T>(sq[t][e]);
+      for (int e = 0; e < 4; ++e) so[(t * 8 + col + (e & 1)) * F::kRow + row + (e >> 1) * 8] = from_f<T>(sq[t][e]);
     __syncwarp();
+    T* to = out + t0 * a.o_t + v0;
     if (a.piece_v == 16) {
       constexpr int V = kVec16<T>;
-      for (int i = lane; i < n * (16 / V); i += 32) {
-        const int r = i / (16 / V), cc = v0 + i % (16 / V) * V;
-        if (cc < a.values)
-          *reinterpret_cast<uint4*>(out + (t0 + r) * a.o_t + cc) = *reinterpret_cast<const uint4*>(so + r * kOut + cc);
+      for (int j = lane; j < n * (16 / V); j += 32) {
+        const int r = j / (16 / V), cc = j % (16 / V) * V;
+        if (v0 + cc < a.values) *reinterpret_cast<uint4*>(to + r * a.o_t + cc) = *reinterpret_cast<const uint4*>(so + r * F::kRow + cc);
       }
     } else {
-      for (int i = lane; i < n * 16; i += 32) {
-        const int r = i / 16, cc = v0 + i % 16;
-        if (cc < a.values) out[(t0 + r) * a.o_t + cc] = so[r * kOut + cc];
+      for (int j = lane; j < n * 16; j += 32) {
+        const int r = j / 16, cc = j % 16;
+        if (v0 + cc < a.values) to[r * a.o_t + cc] = so[r * F::kRow + cc];
       }
     }
-    t0 += n;
+    __syncwarp();
   }
-  store(a.final_ + head_at);
+  store(a.final_ + head_at, a.keys);
   // tokens that are not there give zeros
-  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(a.length - length) * a.values; i += blockDim.x)
-    out[(length + i / a.values) * a.o_t + i % a.values] = from_f<T>(0.0f);
+  for (int t = length + warp; t < a.length; t += warps)
+    for (int j = lane; j < mine; j += 32) out[t * a.o_t + vb + j] = from_f<T>(0.0f);
 }
 
 template <typename T, int DK> int forward(const DeltaArgs& a, cudaStream_t s) {
   using F = Forward<T, DK>;
-  if (const int e = allow_smem<delta_forward<T, DK>>(F::kBytes)) return e;
-  delta_forward<T, DK><<<a.batch * a.heads, (a.values + 15) / 16 * 32, F::kBytes, s>>>(a);
+  if (const int e = allow_smem<delta_forward<T, DK>>(F::bytes(8))) return e;
+  // values of a block: all, or fewer where that leaves SMs without one
+  int warps = (a.values + 15) / 16;
+  while (warps > 1 && a.batch * a.heads * (((a.values + 15) / 16 + warps - 1) / warps) < 148) warps = (warps + 1) / 2;
+  const int blocks = ((a.values + 15) / 16 + warps - 1) / warps;
+  delta_forward<T, DK><<<dim3(a.batch * a.heads, blocks), (warps + kPrep) * 32, F::bytes(warps), s>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T> int forward_by(const DeltaArgs& a, cudaStream_t s) {

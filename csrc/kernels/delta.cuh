@@ -30,7 +30,7 @@ namespace delta {
 
 using namespace seqk;
 
-constexpr int kTile = 16;                     // tokens of a chunk at most; states are kept before each tile
+constexpr int kTile = 16;                     // tokens of a chunk at most, and of the tiles that it ends with
 constexpr float kNormEps = 1e-6f;             // added to the square of a key's or query's length
 
 struct DeltaArgs {
@@ -44,19 +44,19 @@ struct DeltaArgs {
   const void* dout;
   const float* dfinal;
   void *dq, *dk, *dv, *ddt, *db;
-  float *dstate, *part_q, *part_k, *part_h;
+  float *dstate, *part_q, *part_k, *part_g, *part_h;
   float *dA, *dbias;
   int64_t q_b, q_t, q_g, k_b, k_t, k_g, v_b, v_t, v_h, dt_b, dt_t, b_b, b_t, o_b, o_t, o_h, do_b, do_t, do_h;
   float scale;
   int batch, length, groups, heads, keys, values, unit, piece_k, piece_v;
 };
-static_assert(sizeof(DeltaArgs) == 26 * 8 + 19 * 8 + 10 * 4, "as the caller packs it");
+static_assert(sizeof(DeltaArgs) == 27 * 8 + 19 * 8 + 10 * 4, "as the caller packs it");
 
-// Planes of a token (its own type: exact) and of a 32-bit number that is an operand. bfloat16 tokens:
-// one plane, and two for what is computed, 16 bits of mantissa against the 8 of the results; the
-// sums, states and decays keep 32 bits. 32-bit tokens: three planes of either, 24 bits.
-template <typename T> struct Planes { static constexpr int kToken = 1, kInner = 2; };
-template <> struct Planes<float> { static constexpr int kToken = 3, kInner = 3; };
+// Planes of a token (its own type: exact) and of a 32-bit number that is an operand: kInner on the way
+// from state to state and into anything that stays 32-bit, 24 bits of mantissa; kShort where the
+// result is rounded to the tokens' type at once, 16 bits against bfloat16's 8.
+template <typename T> struct Planes { static constexpr int kToken = 1, kInner = 3, kShort = 2; };
+template <> struct Planes<float> { static constexpr int kToken = 3, kInner = 3, kShort = 3; };
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
@@ -121,16 +121,16 @@ __device__ __forceinline__ uint32_t a_cols(int lane, int pitch) {
   return (((lane & 16) >> 1) + (lane & 7)) * pitch * 2 + (lane & 8) * 2;
 }
 
-// c0, c1 (columns 0-7 and 8-15) += A B over 16 of k. NA and NB planes; products of planes i and j
-// with i + j >= max(NA, NB) are below what the planes leave out.
-template <int NA, int NB>
+// c0, c1 (columns 0-7 and 8-15) += A B over 16 of k, of the first PA and PB planes; products of
+// planes i and j with i + j >= max(PA, PB) are below what the planes leave out.
+template <int PA, int PB, int NA, int NB>
 __device__ __forceinline__ void mma_planes(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
-  constexpr int kMost = NA > NB ? NA : NB;
+  static_assert(PA <= NA && PB <= NB, "planes that are there");
 #pragma unroll
-  for (int i = 0; i < NA; ++i)
+  for (int i = 0; i < PA; ++i)
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-      if (i + j < kMost) {
+    for (int j = 0; j < PB; ++j)
+      if (i + j < (PA > PB ? PA : PB)) {
         mma(c0, a[i], b[j][0], b[j][1]);
         mma(c1, a[i], b[j][2], b[j][3]);
       }
@@ -183,119 +183,179 @@ template <typename T> __device__ __forceinline__ float tile_at(const bf16* t, in
   return v;
 }
 
+// By one warp: rows [0, n) of `cols` elements as they are, `pitch` apart; the rest of `rows` x `width` zero.
+// A row's pieces are spread over a power of two of lanes.
+template <typename T>
+__device__ __forceinline__ void load_rows(T* dst, int pitch, int rows, int width, const T* src, int64_t stride, int n, int cols, bool pieces) {
+  constexpr int V = kVec16<T>;
+  const int lane = threadIdx.x & 31;
+  if (pieces) {
+    const int w = width / V, bits = min(5, 32 - __clz(w - 1)), c0 = (lane & ((1 << bits) - 1)) * V;
+    for (int r = lane >> bits; r < rows; r += 32 >> bits)
+      for (int c = c0; c < width; c += 32 * V) {
+        T* d = dst + r * pitch + c;
+        if (r < n && c < cols) cp_async16(d, src + r * stride + c);
+        else *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
+      }
+  } else {
+    for (int i = lane; i < rows * width; i += 32) {
+      const int r = i / width, c = i - r * width;
+      dst[r * pitch + c] = r < n && c < cols ? src[r * stride + c] : from_f<T>(0.0f);
+    }
+  }
+}
+
 // ---- a chunk's matrices -----------------------------------------------------------------
 constexpr int kSide = kTile + 8;                       // pitch of 16 x 16 matrices of planes
-template <typename T> struct Chunk {
-  static constexpr int kInner = Planes<T>::kInner;
+constexpr int kMat = kTile + 4;                        // and of 32-bit numbers
+template <typename T, int NP> struct Chunk {           // NP: planes of P
   float beta[kTile], head[kTile], tail[kTile], rk[kTile], rq[kTile];
-  float scratch[3][kTile][20];                         // K K^T, Q K^T, Q Q^T; then M beta, M, P
-  alignas(16) bf16 inv[kInner][kTile][kSide];          // (I + M beta)^-1
-  alignas(16) bf16 p[kInner][kTile][kSide];            // P
+  float g_hi[kTile], g_lo[kTile];                      // running sums of the log decays
+  alignas(16) bf16 inv[Planes<T>::kInner][kTile][kSide];         // (I + M beta)^-1
+  alignas(16) bf16 p[NP][kTile][kSide];                // P
 };
+using Scratch = float[2][kTile][kMat];
+struct Wide { float m[kTile][kMat], p[kTile][kMat], d[kTile][kMat]; };   // M, P, D as 32-bit numbers
 
 // By one warp, from the tiles of K and Q and each lane's gates (lane < 16: token lane's log decay and
-// beta, zero behind the chunk). scratch holds M and P as 32-bit numbers then and, with kKeep, D.
-template <typename T, int DK, bool kKeep>
-__device__ __forceinline__ void prepare(Chunk<T>& c, const bf16* tk, const bf16* tq, float g, float beta, float scale, int unit) {
+// beta, zero behind the chunk); with kKeep into `wide` too.
+//
+// Running sums are kept as two floats, of which differences lose nothing: the larger halves' is
+// exact where they are close. Decays below e^-104 are 0 in 32 bits; -10^4 stands for all of them.
+// The inverse goes by blocks of 8: [[A, 0], [C, B]]^-1 = [[A', 0], [-B' C A', B']], the blocks' own
+// column by column.
+template <typename T, int DK, bool kKeep, int NP>
+__device__ __forceinline__ void prepare(Chunk<T, NP>& c, Scratch& s, Wide* wide, const bf16* tk, const bf16* tq, float g, float beta,
+                                        float scale, int unit) {
   constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner;
   using Keys = Tile<T, DK>;
   const int lane = threadIdx.x & 31, row = lane >> 2, col = (lane & 3) * 2;
+  float kk[2][4] = {}, qk[2][4] = {};
   {
-    float kk[2][4] = {}, qk[2][4] = {}, qq[2][4] = {};
+    float qq[2][4] = {};
     const uint32_t ka = smem_of(tk), qa = smem_of(tq);
     const uint32_t b_at = at_rows(lane, Keys::kPitch), a_at = a_rows(lane, Keys::kPitch);
 #pragma unroll
-    for (int s = 0; s < DK / 16; ++s) {
+    for (int i = 0; i < DK / 16; ++i) {
       uint32_t ak[NT][4], aq[NT][4], bk[NT][4];
-      load_planes<NT, false>(ak, ka + a_at + s * 32, Keys::kPlane * 2);
-      load_planes<NT, false>(aq, qa + a_at + s * 32, Keys::kPlane * 2);
-      load_planes<NT, false>(bk, ka + b_at + s * 32, Keys::kPlane * 2);
+      load_planes<NT, false>(ak, ka + a_at + i * 32, Keys::kPlane * 2);
+      load_planes<NT, false>(aq, qa + a_at + i * 32, Keys::kPlane * 2);
+      load_planes<NT, false>(bk, ka + b_at + i * 32, Keys::kPlane * 2);
       mma_planes<NT, NT>(kk[0], kk[1], ak, bk);
       mma_planes<NT, NT>(qk[0], qk[1], aq, bk);
-      load_planes<NT, false>(bk, qa + b_at + s * 32, Keys::kPlane * 2);
-      mma_planes<NT, NT>(qq[0], qq[1], aq, bk);
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = row + (e >> 1) * 8, j = t * 8 + col + (e & 1);
-        c.scratch[0][i][j] = kk[t][e];
-        c.scratch[1][i][j] = qk[t][e];
-        c.scratch[2][i][j] = qq[t][e];
+      if (unit) {
+        load_planes<NT, false>(bk, qa + b_at + i * 32, Keys::kPlane * 2);
+        mma_planes<NT, NT>(qq[0], qq[1], aq, bk);
       }
+    }
+    // the lanes that hold the diagonals
+    if (row == col || row == col + 1) {
+      const bool odd = row != col;
+      c.rk[row] = unit ? rsqrtf((odd ? kk[0][1] : kk[0][0]) + kNormEps) : 1.0f;
+      c.rk[row + 8] = unit ? rsqrtf((odd ? kk[1][3] : kk[1][2]) + kNormEps) : 1.0f;
+      c.rq[row] = unit ? rsqrtf((odd ? qq[0][1] : qq[0][0]) + kNormEps) : 1.0f;
+      c.rq[row + 8] = unit ? rsqrtf((odd ? qq[1][3] : qq[1][2]) + kNormEps) : 1.0f;
+    }
+  }
+  {
+    double sum = fmaxf(g, -1e4f);
+#pragma unroll
+    for (int o = 1; o < kTile; o <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, sum, o, kTile);
+      if ((lane & 15) >= o) sum += x;
+    }
+    const double all = __shfl_sync(0xffffffffu, sum, 15);
+    if (lane < kTile) {
+      const float hi = static_cast<float>(sum);
+      c.g_hi[lane] = hi;
+      c.g_lo[lane] = static_cast<float>(sum - hi);
+      c.beta[lane] = beta;
+      c.head[lane] = exp2_hw(fmaf(hi, kLog2e, kExp2Shift));
+      c.tail[lane] = exp2_hw(fmaf(static_cast<float>(all - sum), kLog2e, kExp2Shift));
+    }
   }
   __syncwarp();
-  const int j = lane & 15;
-  const bool upper = lane >= 16;
-  const float rk = unit ? rsqrtf(c.scratch[0][j][j] + kNormEps) : 1.0f;
-  const float rq = unit ? rsqrtf(c.scratch[2][j][j] + kNormEps) : 1.0f;
-  __syncwarp();
-  // lanes 0-15 make M's column, 16-31 P's; d: the sum of the decays behind token j up to token i
-  float d = 0.0f, h = 0.0f, last = 1.0f, decay[kKeep ? kTile : 1];
 #pragma unroll
-  for (int i = 0; i < kTile; ++i) {
-    const float gi = __shfl_sync(0xffffffffu, g, i);
-    const float ri = __shfl_sync(0xffffffffu, upper ? rq : rk, i + (lane & 16));
-    if (i <= j) h += gi;
-    if (i > j) d += gi;
-    float x = 0.0f;
-    if (i > j || (upper && i == j)) {
-      last = exp2_hw(fmaf(d, kLog2e, kExp2Shift));
-      x = c.scratch[upper ? 1 : 0][i][j] * (last * ri * rk) * (upper ? scale : 1.0f);
+  for (int r = 0; r < 2; ++r) {
+    const int i = row + 8 * r;
+    const float hi = c.g_hi[i], lo = c.g_lo[i], rk = c.rk[i], rq = scale * c.rq[i];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int j = 8 * t + col;
+      float x[2] = {}, y[2] = {}, d[2] = {};
+      if (t <= r) {
+        const float2 hj = *reinterpret_cast<const float2*>(&c.g_hi[j]), lj = *reinterpret_cast<const float2*>(&c.g_lo[j]);
+        const float2 rj = *reinterpret_cast<const float2*>(&c.rk[j]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float sum = (hi - (e ? hj.y : hj.x)) + (lo - (e ? lj.y : lj.x));
+          const float dec = exp2_hw(fmaf(sum, kLog2e, kExp2Shift)), f = dec * (e ? rj.y : rj.x);
+          d[e] = i >= j + e ? dec : 0.0f;
+          x[e] = i > j + e ? kk[t][2 * r + e] * (f * rk) : 0.0f;
+          y[e] = i >= j + e ? qk[t][2 * r + e] * (f * rq) : 0.0f;
+        }
+      }
+      const float2 bj = *reinterpret_cast<const float2*>(&c.beta[j]);
+      *reinterpret_cast<float2*>(&s[0][i][j]) = make_float2(x[0] * bj.x, x[1] * bj.y);
+      uint32_t p[NP];
+      split2<NP>(y[0], y[1], p);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) *reinterpret_cast<uint32_t*>(&c.p[n][i][j]) = p[n];
+      if constexpr (kKeep) {
+        *reinterpret_cast<float2*>(&wide->m[i][j]) = make_float2(x[0], x[1]);
+        *reinterpret_cast<float2*>(&wide->p[i][j]) = make_float2(y[0], y[1]);
+        *reinterpret_cast<float2*>(&wide->d[i][j]) = make_float2(d[0], d[1]);
+      }
     }
-    if constexpr (kKeep) decay[i] = i == j ? 1.0f : i > j ? last : 0.0f;
-    c.scratch[upper ? 1 : 0][i][j] = x;
-    if (upper) {
-      float y = x, z = 0.0f;
+  }
+  __syncwarp();
+  if (lane < kTile) {
+    const int b = lane & 8, j = lane & 7;
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = i == j ? 1.0f : 0.0f;
+      const float4 lo = *reinterpret_cast<const float4*>(&s[0][b + i][b]), hi = *reinterpret_cast<const float4*>(&s[0][b + i][b + 4]);
+      const float a[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int e = 0; e < i; ++e) v = fmaf(-a[e], t[e], v);
+      t[i] = v;
+      s[1][b + i][b + j] = v;
+    }
+  }
+  __syncwarp();
+  const int j = lane & 7, r0 = (lane >> 3) * 2;
+  auto product = [&](const float* left, int pitch_r, const float* right, float& x, float& y) {
+    x = y = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const float4 l0 = *reinterpret_cast<const float4*>(left + r0 * kMat + e), l1 = *reinterpret_cast<const float4*>(left + (r0 + 1) * kMat + e);
+      const float* r = right + e * pitch_r + j;
+      const float b0 = r[0], b1 = r[pitch_r], b2 = r[2 * pitch_r], b3 = r[3 * pitch_r];
+      x = fmaf(l0.x, b0, fmaf(l0.y, b1, fmaf(l0.z, b2, fmaf(l0.w, b3, x))));
+      y = fmaf(l1.x, b0, fmaf(l1.y, b1, fmaf(l1.z, b2, fmaf(l1.w, b3, y))));
+    }
+  };
+  float x, y;
+  product(&s[0][8][0], kMat, &s[1][0][0], x, y);       // C A'
+  s[0][r0][8 + j] = x;
+  s[0][r0 + 1][8 + j] = y;
+  __syncwarp();
+  product(&s[1][8][8], kMat, &s[0][0][8], x, y);
+  s[1][8 + r0][j] = -x;
+  s[1][8 + r0 + 1][j] = -y;
+  __syncwarp();
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float2 v = t <= r ? *reinterpret_cast<const float2*>(&s[1][row + 8 * r][8 * t + col]) : make_float2(0.0f, 0.0f);
       uint32_t p[NI];
-      split2<NI>(y, z, p);
+      split2<NI>(v.x, v.y, p);
 #pragma unroll
-      for (int n = 0; n < NI; ++n) c.p[n][i][j] = __ushort_as_bfloat16(static_cast<unsigned short>(p[n]));
-    } else {
-      c.scratch[2][i][j] = x * beta;
+      for (int n = 0; n < NI; ++n) *reinterpret_cast<uint32_t*>(&c.inv[n][row + 8 * r][8 * t + col]) = p[n];
     }
-  }
-  if (!upper) {
-    c.beta[j] = beta;
-    c.head[j] = exp2_hw(fmaf(h, kLog2e, kExp2Shift));
-    c.tail[j] = last;
-    c.rk[j] = rk;
-    c.rq[j] = rq;
-  }
   __syncwarp();
-  // column j of (I + M beta)^-1, row by row
-  float t[kTile];
-#pragma unroll
-  for (int i = 0; i < kTile; ++i) {
-    float s = i == j ? 1.0f : 0.0f;
-#pragma unroll
-    for (int m = 0; m < i; m += 4) {
-      const float4 a = *reinterpret_cast<const float4*>(&c.scratch[2][i][m]);
-      s = fmaf(-a.x, t[m], s);
-      if (m + 1 < i) s = fmaf(-a.y, t[m + 1], s);
-      if (m + 2 < i) s = fmaf(-a.z, t[m + 2], s);
-      if (m + 3 < i) s = fmaf(-a.w, t[m + 3], s);
-    }
-    t[i] = s;
-  }
-  if (!upper) {
-#pragma unroll
-    for (int i = 0; i < kTile; ++i) {
-      uint32_t p[NI];
-      split2<NI>(t[i], 0.0f, p);
-#pragma unroll
-      for (int n = 0; n < NI; ++n) c.inv[n][i][j] = __ushort_as_bfloat16(static_cast<unsigned short>(p[n]));
-    }
-  }
-  __syncwarp();
-  if constexpr (kKeep) {
-    if (!upper) {
-#pragma unroll
-      for (int i = 0; i < kTile; ++i) c.scratch[2][i][j] = decay[i];
-    }
-    __syncwarp();
-  }
 }
 
 // A log decay and its gate from a token's dt and b.
@@ -311,16 +371,72 @@ __device__ __forceinline__ Gate gate_of(float dt, float b, float bias, float rat
 // A[h]; -inf as the lowest finite number, so that a step of zero decays by e^0
 __device__ __forceinline__ float rate_at(const float* A, int h) { return fmaxf(A[h], -3.4028235e38f); }
 
-// The tokens [t0, t0 + n) of a chunk: up to the end of its tile, the row's end, the next reset.
-__device__ __forceinline__ int chunk_tokens(const uint8_t* reset, int t0, int length) {
-  const int lane = threadIdx.x & 31;
-  int n = min(kTile - t0 % kTile, length - t0);
-  if (reset) {
-    const bool cut = lane > 0 && lane < n && reset[t0 + lane];
-    const unsigned cuts = __ballot_sync(0xffffffffu, cut);
-    if (cuts) n = __ffs(cuts) - 1;
+// The chunks of a row in order: a tile's begin at its first token and at each reset. All lanes of a
+// warp; the next tile's marks are on their way while one is taken.
+struct Chunks {
+  const uint8_t* reset;
+  int length, tile, t0, n;
+  bool fresh;
+  unsigned left, marks, coming;
+  __device__ __forceinline__ unsigned look(int t) const {                // this lane's mark of the tile at t
+    const int lane = threadIdx.x & 31;
+    return reset && lane < kTile && t + lane < length ? reset[t + lane] : 0u;
   }
-  return n;
-}
+  __device__ __forceinline__ Chunks(const uint8_t* reset_, int length_) : reset(reset_), length(length_), tile(-kTile), t0(0), n(0), fresh(false), left(0) {
+    coming = look(0);
+  }
+  __device__ __forceinline__ bool next() {
+    if (!left) {
+      tile += kTile;
+      if (tile >= length) return false;
+      marks = __ballot_sync(0xffffffffu, coming != 0);
+      left = marks | 1u;
+      coming = look(tile + kTile);
+    }
+    const int at = __ffs(left) - 1;
+    left &= left - 1;
+    t0 = tile + at;
+    n = (left ? tile + __ffs(left) - 1 : min(tile + kTile, length)) - t0;
+    fresh = (marks >> at) & 1u;
+    return true;
+  }
+};
+
+// The same from the row's end.
+struct ChunksBack {
+  const uint8_t* reset;
+  int length, tile, t0, n, end;
+  bool fresh;
+  unsigned left, marks, coming;
+  __device__ __forceinline__ unsigned look(int t) const {
+    const int lane = threadIdx.x & 31;
+    return reset && t >= 0 && lane < kTile && t + lane < length ? reset[t + lane] : 0u;
+  }
+  __device__ __forceinline__ ChunksBack(const uint8_t* reset_, int length_) : reset(reset_), length(length_), t0(0), n(0), fresh(false), left(0) {
+    tile = (length + kTile - 1) / kTile * kTile;
+    coming = look(tile - kTile);
+  }
+  __device__ __forceinline__ bool next() {
+    if (!left) {
+      tile -= kTile;
+      if (tile < 0) return false;
+      marks = __ballot_sync(0xffffffffu, coming != 0);
+      left = marks | 1u;
+      end = min(tile + kTile, length);
+      coming = look(tile - kTile);
+    }
+    const int at = 31 - __clz(left);
+    left ^= 1u << at;
+    t0 = tile + at;
+    n = end - t0;
+    end = t0;
+    fresh = (marks >> at) & 1u;
+    return true;
+  }
+};
+
+// ---- hardware barriers by number ----------------------------------------------------------
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 }  // namespace delta

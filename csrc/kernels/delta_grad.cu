@@ -11,30 +11,54 @@
 //   dg_m = sum_{j < m <= i} E_ij + sum_{i >= m} e_i + sum_{j < m} f_j + end <dS, S>.
 // These are sums of what each pair's decay contributes; none is a difference of larger ones.
 //
-// A block for a sequence's value head. By values (a warp for 16 rows of S and dS, dS its
-// accumulators): the chain from dS to dS. By keys (a warp for 16 columns): dq and dk, which sum
-// over the values; the chain's results pass through shared memory as planes.
+// A block for up to 64 values of a sequence's value head: two warps make the chunks ready in turn, as
+// in the forward pass, four carry them out, one makes the matrices and gates of 16 x 16. By values
+// (a warp for 16 rows of dS, its accumulators): the chain from dS to dS; by keys (a warp for a
+// quarter of the columns): dq and dk, which sum over the values; the chain's results pass
+// through shared memory as planes. S and W are the forward pass's. Blocks of one head, and heads
+// that share keys, leave parts of dq and dk that a second kernel sums in order.
 #include "delta.cuh"
 
 namespace {
 
 using namespace delta;
 
+constexpr int kPrep = 2, kMain = 4, kValues = 64;      // warps of each kind (and one more); values of a block
+constexpr int kThreads = (kPrep + kMain + 1) * 32;
+// barriers: stage s ready (1 + s), stage s free (1 + kStages + s), the chain's results, the matrices
+enum : int { kBarChain = 14, kBarMatrices = 15 };
+
 template <typename T, int DK> struct Backward {
-  static constexpr int NI = Planes<T>::kInner;
+  static constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort;
+  // a stage for each warp that makes chunks ready, so that its barriers are that warp's alone; where
+  // two do not fit, one warp and one stage
+  static constexpr int kStages = DK == 128 && sizeof(T) == 4 ? 1 : kPrep;
   using Keys = Tile<T, DK>;
-  using Values = Tile<T, 128>;
-  static constexpr int kState = DK + 8;                // pitch of S and dS
+  using Values = Tile<T, kValues>;
+  static constexpr int kPitchS = DK + 4, kPitchD = DK + 8, kPitchV = kValues + 16 / static_cast<int>(sizeof(T));
+  static constexpr int kColumns = DK / kMain < 16 ? 16 : DK / kMain;     // of a warp by keys
+  struct Stage {
+    Chunk<T, NI> c;
+    Wide wide;
+    int t0, n, fresh;
+    alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize], tdo[Values::kSize];
+    alignas(16) T tv[kTile * kPitchV];
+    alignas(16) float w[kValues][kMat];                // rows values, columns tokens
+    alignas(16) float s[kValues][kPitchS];
+  };
   struct Shared {
-    Chunk<T> c;
-    alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize], tv[Values::kSize], tdo[Values::kSize];
-    alignas(16) bf16 w[NI][128][kSide], z[NI][128][kSide];       // rows values, columns tokens
-    alignas(16) bf16 x1[NI][kTile][kSide], x2[NI][kTile][kSide], x3[NI][kTile][kSide];
-    float zw[kTile][kTile + 1], ow[kTile][kTile + 1];            // Z W^T and dO W^T
-    float by_value[8][3][kTile];                       // of each warp: W.dU, head's and tail's terms of k
-    float by_key[8][3][kTile];                         // head's term of q, q.dq, k.dk
-    float inner[8];                                    // <dS, S>
-    alignas(16) bf16 st[NI][128][kState];              // S, then dS
+    Stage stage[kStages];
+    alignas(16) Scratch scratch[kPrep];
+    alignas(16) bf16 w[NI][kValues][kSide], z[NI][kValues][kSide];
+    alignas(16) bf16 d[NS][kValues][kPitchD];          // dS
+    alignas(16) bf16 x1[NS][kTile][kSide], x2[NS][kTile][kSide], x3[NS][kTile][kSide];
+    // of each warp, for chunks in turn: Z W^T and dO W^T, sums over its values: W.dU, Z.V, the tails' terms
+    alignas(16) float part[2][kMain][2][kTile][kMat];
+    float by_value[2][kMain][3][kTile], inner[2][kMain];
+    float by_key[2][kMain][kTile];                     // the heads' terms of q
+    float nq[kTile], nk[kTile];                        // q.dq and k.dk but for those
+    alignas(16) float e[3][kTile][kMat];
+    alignas(16) T out[kMain][kTile][16 + 16 / sizeof(T)];
   };
   static constexpr size_t kBytes = sizeof(Shared);
   static_assert(kBytes <= 227 * 1024, "a block's shared memory");
@@ -49,150 +73,320 @@ __device__ __forceinline__ float column_sum(float v) { // over a column's eight 
   v += __shfl_xor_sync(0xffffffffu, v, 8);
   return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
-
-template <int N, int R> __device__ __forceinline__ void put_planes(bf16 (&m)[N][kTile][R], int i, int j, float x) {
-  uint32_t p[N];
-  split2<N>(x, 0.0f, p);
+template <int N, int R, int P> __device__ __forceinline__ void put_planes(bf16 (&m)[N][R][P], int i, int j, const uint32_t (&p)[N]) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) m[n][i][j] = __ushort_as_bfloat16(static_cast<unsigned short>(p[n]));
+  for (int n = 0; n < N; ++n) *reinterpret_cast<uint32_t*>(&m[n][i][j]) = p[n];
+}
+template <int N, int NF, int R, int P> __device__ __forceinline__ void put_frag(bf16 (&m)[N][R][P], int i, int j, const Frag<NF>& f) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(&m[n][i + (e & 1) * 8][j + (e >> 1) * 8]) = f.r[n][e];
+}
+// A warp's 16 x 16 of `out` (rows tokens) to the first n rows of memory, `cols` of its columns.
+template <typename T, int P>
+__device__ __forceinline__ void put_rows(T* to, int64_t stride, const T (&out)[kTile][P], int n, int cols, bool pieces) {
+  const int lane = threadIdx.x & 31;
+  if (pieces) {
+    constexpr int V = kVec16<T>;
+    for (int j = lane; j < n * (16 / V); j += 32) {
+      const int r = j / (16 / V), c = j % (16 / V) * V;
+      if (c < cols) *reinterpret_cast<uint4*>(to + r * stride + c) = *reinterpret_cast<const uint4*>(&out[r][c]);
+    }
+  } else {
+    for (int j = lane; j < n * 16; j += 32)
+      if (j % 16 < cols) to[j / 16 * stride + j % 16] = out[j / 16][j % 16];
+  }
 }
 
-template <typename T, int DK> __global__ void __launch_bounds__(256) delta_backward(DeltaArgs a) {
-  constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, kSteps = DK / 16;
+template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_backward(DeltaArgs a) {
   using B = Backward<T, DK>;
+  constexpr int NT = B::NT, NI = B::NI, NS = B::NS, kSteps = DK / 16, kStages = B::kStages;
   using Keys = typename B::Keys;
   using Values = typename B::Values;
   extern __shared__ __align__(16) char smem[];
   typename B::Shared& sh = *reinterpret_cast<typename B::Shared*>(smem);
-  Chunk<T>& c = sh.c;
-  const int bi = blockIdx.x / a.heads, h = blockIdx.x % a.heads, rep = a.heads / a.groups, gr = h / rep;
+  const int bi = blockIdx.x / a.heads, h = blockIdx.x % a.heads, gr = h / (a.heads / a.groups);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = lane >> 2, col = (lane & 3) * 2;
-  const int vwarps = (a.values + 15) / 16, kwarps = (a.keys + 15) / 16, warps = blockDim.x / 32;
-  const int v0 = warp * 16, k0 = warp * 16;
-  const bool by_v = warp < vwarps, by_k = warp < kwarps;
+  const int vb = blockIdx.y * kValues, mine = min(kValues, a.values - vb), splits = gridDim.y;
   const int length = a.lengths ? max(0, min(a.lengths[bi], a.length)) : a.length;
-  const uint8_t* reset = a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr;
-  const T* q = static_cast<const T*>(a.q) + bi * a.q_b + gr * a.q_g;
-  const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
-  const T* v = static_cast<const T*>(a.v) + bi * a.v_b + h * a.v_h;
+  const int tiles = (a.length + kTile - 1) / kTile;
+  const int64_t row0 = static_cast<int64_t>(bi) * a.length;
   const T* dt = static_cast<const T*>(a.dt) + bi * a.dt_b + h;
   const T* gb = static_cast<const T*>(a.b) + bi * a.b_b + h;
-  const T* dout = static_cast<const T*>(a.dout) + bi * a.do_b + h * a.do_h;
-  // gradients are dense
-  const int64_t row0 = static_cast<int64_t>(bi) * a.length;
-  T* dq = static_cast<T*>(a.dq) + (row0 * a.groups + gr) * a.keys;
-  T* dk = static_cast<T*>(a.dk) + (row0 * a.groups + gr) * a.keys;
-  float* pq = a.part_q ? a.part_q + (row0 * a.heads + h) * a.keys : nullptr;
-  float* pk = a.part_q ? a.part_k + (row0 * a.heads + h) * a.keys : nullptr;
-  const int64_t qk_t = static_cast<int64_t>(pq ? a.heads : a.groups) * a.keys, v_t = static_cast<int64_t>(a.heads) * a.values;
-  T* dv = static_cast<T*>(a.dv) + (row0 * a.heads + h) * a.values;
-  T* ddt = static_cast<T*>(a.ddt) + row0 * a.heads + h;
-  T* db = static_cast<T*>(a.db) + row0 * a.heads + h;
   const float rate = rate_at(a.A, h), bias = a.bias ? a.bias[h] : 0.0f;
-  const int64_t head_size = static_cast<int64_t>(a.values) * a.keys;
-  const int64_t head_at = (static_cast<int64_t>(bi) * a.heads + h) * head_size;
-  const int tiles = (a.length + kTile - 1) / kTile;
 
-  // d[n]: rows v0 + row, + 8; keys 8 n + col, + 1
+  if (warp >= kMain && warp < kMain + kPrep) {
+    const int w = warp - kMain, pitch = a.keys + kTile;
+    if (w >= kStages) return;
+    const T* q = static_cast<const T*>(a.q) + bi * a.q_b + gr * a.q_g;
+    const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
+    const T* v = static_cast<const T*>(a.v) + bi * a.v_b + h * a.v_h + vb;
+    const T* dout = static_cast<const T*>(a.dout) + bi * a.do_b + h * a.do_h + vb;
+    ChunksBack walk(a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length);
+    for (int i = 0;; ++i) {
+      const bool more = walk.next();
+      const int at = i % kStages;
+      if (at != w) {
+        if (!more) return;
+        continue;
+      }
+      typename B::Stage& st = sh.stage[at];
+      if (i >= kStages) bar_sync(1 + kStages + at, kThreads - (kPrep - 1) * 32);
+      const int t0 = walk.t0, n = more ? walk.n : 0;
+      if (lane == 0) {
+        st.t0 = t0;
+        st.n = n;
+        st.fresh = walk.fresh;
+      }
+      if (!more) {
+        __syncwarp();
+        bar_arrive(1 + at, kThreads - (kPrep - 1) * 32);
+        return;
+      }
+      Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k, lane, 32);
+      Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k, lane, 32);
+      cp_async_commit();
+      Values::load(st.tdo, dout + t0 * a.do_t, a.do_t, n, mine, a.piece_v, lane, 32);
+      load_rows(st.tv, B::kPitchV, kTile, kValues, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
+      const float* saved = a.saved + (((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values + vb) * pitch;
+      const bool pieces = a.keys % 4 == 0;
+      load_rows(&st.w[0][0], kMat, kValues, kTile, saved + a.keys + t0 % kTile, pitch, mine, n, pieces && t0 % 4 == 0 && n % 4 == 0);
+      if (!walk.fresh) load_rows(&st.s[0][0], B::kPitchS, kValues, DK, saved, pitch, mine, a.keys, pieces);
+      cp_async_commit();
+      Gate e{};
+      if (lane < n) e = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
+      cp_async_wait<1>();
+      __syncwarp();
+      prepare<T, DK, true>(st.c, sh.scratch[w], &st.wide, st.tk, st.tq, e.g, e.beta, a.scale, a.unit);
+      cp_async_wait<0>();
+      __syncwarp();
+      bar_arrive(1 + at, kThreads - (kPrep - 1) * 32);
+    }
+  }
+
+  const int stage_threads = kThreads - (kPrep - 1) * 32, team = (kMain + 1) * 32;
+  if (warp == kMain + kPrep) {
+    // the matrices and gates of 16 x 16
+    const int64_t g_t = static_cast<int64_t>(a.heads) * splits, g_at = row0 * g_t + static_cast<int64_t>(h) * splits + blockIdx.y;
+    double sum_a = 0.0, sum_bias = 0.0;
+    for (int i = 0;; ++i) {
+      const int at = i % kStages, turn = i & 1;
+      typename B::Stage& st = sh.stage[at];
+      bar_sync(1 + at, stage_threads);
+      const int t0 = st.t0, n = st.n;
+      if (n == 0) break;
+      Gate gate{};
+      if (lane < n) gate = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
+      bar_sync(kBarChain, team);
+      // lane: row r, columns j0 .. j0 + 7 of Z W^T and dO W^T. By rows: sums of E's part of P, of M, and Z.R
+      const int r = lane >> 1, j0 = (lane & 1) * 8;
+      const float rqr = st.c.rq[r], rkr = st.c.rk[r];
+      float row_p = 0.0f, row_m = 0.0f, zr = 0.0f;
+#pragma unroll
+      for (int j = j0; j < j0 + 8; j += 4) {
+        auto four = [](float (&x)[4], const float* from) { *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from); };
+        float zw[4] = {}, ow[4] = {}, bt[4], rk[4], d[4], p[4], m[4], ep[4], em[4], mz[4], pd[4], md[4];
+#pragma unroll
+        for (int x = 0; x < kMain; ++x) {
+          float y[4];
+          four(y, &sh.part[turn][x][0][r][j]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) zw[e] += y[e];
+          four(y, &sh.part[turn][x][1][r][j]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ow[e] += y[e];
+        }
+        four(bt, &st.c.beta[j]);
+        four(rk, &st.c.rk[j]);
+        four(d, &st.wide.d[r][j]);
+        four(p, &st.wide.p[r][j]);
+        four(m, &st.wide.m[r][j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = j + e;
+          const float dp = c <= r ? ow[e] * bt[e] : 0.0f, dm = c < r ? -zw[e] * bt[e] : 0.0f;
+          ep[e] = dp * p[e];
+          em[e] = dm * m[e];
+          pd[e] = a.scale * dp * d[e];
+          md[e] = dm * d[e];
+          mz[e] = c < r ? m[e] * zw[e] : 0.0f;
+          row_p += ep[e];
+          row_m += em[e];
+          zr += c == r ? zw[e] : mz[e] * bt[e];
+        }
+        *reinterpret_cast<float4*>(&sh.e[0][r][j]) = make_float4(ep[0], ep[1], ep[2], ep[3]);
+        *reinterpret_cast<float4*>(&sh.e[1][r][j]) = make_float4(em[0], em[1], em[2], em[3]);
+        *reinterpret_cast<float4*>(&sh.e[2][r][j]) = make_float4(mz[0], mz[1], mz[2], mz[3]);
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          uint32_t y[NS];
+          split2<NS>(pd[e] * rk[e], pd[e + 1] * rk[e + 1], y);
+          put_planes(sh.x1, r, j + e, y);
+          split2<NS>(pd[e] * rqr, pd[e + 1] * rqr, y);
+          put_planes(sh.x2, r, j + e, y);
+#pragma unroll
+          for (int o = e; o < e + 2; ++o)
+            if (j + o <= r) {                          // below the diagonal, and what it gives above it
+              split2<NS>(md[o] * rk[o], md[o] * rkr, y);
+#pragma unroll
+              for (int x = 0; x < NS; ++x) {
+                if (j + o < r) sh.x3[x][j + o][r] = __ushort_as_bfloat16(static_cast<unsigned short>(y[x] >> 16));
+                sh.x3[x][r][j + o] = __ushort_as_bfloat16(static_cast<unsigned short>(y[x]));
+              }
+            }
+        }
+      }
+      row_p += __shfl_xor_sync(0xffffffffu, row_p, 1);
+      row_m += __shfl_xor_sync(0xffffffffu, row_m, 1);
+      zr += __shfl_xor_sync(0xffffffffu, zr, 1);
+      __syncwarp();
+      // lane: column and token c; columns from below
+      const int c = lane & 15;
+      float wd = 0.0f, zv = 0.0f, f = 0.0f, inner = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kMain; ++x) {
+        wd += sh.by_value[turn][x][0][c];
+        zv += sh.by_value[turn][x][1][c];
+        f += sh.by_value[turn][x][2][c];
+        inner += sh.inner[turn][x];
+      }
+      float column = 0.0f, below = 0.0f, dbeta = wd;
+#pragma unroll
+      for (int y = kTile - 1; y >= 0; --y) {
+        const float ep = sh.e[0][y][c], em = sh.e[1][y][c];
+        dbeta -= sh.e[2][y][c];
+        column += ep + em;
+        if (y > c) below += ep + em;
+        __syncwarp();
+        if (lane < kTile) sh.e[0][y][c] = y > c ? below : 0.0f;
+      }
+      row_p = __shfl_sync(0xffffffffu, row_p, 2 * c);
+      row_m = __shfl_sync(0xffffffffu, row_m, 2 * c);
+      zr = __shfl_sync(0xffffffffu, zr, 2 * c);
+      // the head's term of k, -Z.(head K S^T) = Z.R - Z.V
+      const float keep = st.fresh ? 0.0f : zr - zv;
+      if (lane < kTile) {
+        sh.nq[c] = row_p;
+        sh.nk[c] = keep + f + row_m + column;
+      }
+      bar_sync(kBarMatrices, team);
+      float e = keep;
+#pragma unroll
+      for (int x = 0; x < kMain; ++x) e += sh.by_key[turn][x][c];
+      float dg = st.c.head[kTile - 1] * inner;
+#pragma unroll
+      for (int j = 0; j < kTile; ++j) {
+        const float ej = __shfl_sync(0xffffffffu, e, j), fj = __shfl_sync(0xffffffffu, f, j);
+        dg += j >= c ? ej : fj + sh.e[0][c][j];
+      }
+      if (lane < n) {
+        const float back = dg * rate * sigmoid(gate.pre), b_back = dbeta * gate.beta * (1.0f - gate.beta);
+        const int64_t to = g_at + (t0 + lane) * g_t;
+        if (a.part_g) {
+          *reinterpret_cast<float2*>(a.part_g + 2 * to) = make_float2(back, b_back);
+        } else {
+          static_cast<T*>(a.ddt)[to] = from_f<T>(back);
+          static_cast<T*>(a.db)[to] = from_f<T>(b_back);
+        }
+        sum_a += static_cast<double>(dg) * gate.delta;
+        sum_bias += back;
+      }
+      __syncwarp();
+      bar_arrive(1 + kStages + at, stage_threads);
+    }
+    for (int o = 16; o; o >>= 1) {
+      sum_a += __shfl_xor_sync(0xffffffffu, sum_a, o);
+      sum_bias += __shfl_xor_sync(0xffffffffu, sum_bias, o);
+    }
+    if (lane == 0) {
+      const int64_t to = (static_cast<int64_t>(blockIdx.x) * splits + blockIdx.y) * 2;
+      a.part_h[to] = static_cast<float>(sum_a);
+      a.part_h[to + 1] = static_cast<float>(sum_bias);
+    }
+    for (int t = length + lane; t < a.length; t += 32) {
+      const int64_t to = g_at + t * g_t;
+      if (a.part_g) *reinterpret_cast<float2*>(a.part_g + 2 * to) = make_float2(0.0f, 0.0f);
+      else static_cast<T*>(a.ddt)[to] = static_cast<T*>(a.db)[to] = from_f<T>(0.0f);
+    }
+    return;
+  }
+
+  // gradients are dense; parts of dq and dk by heads and blocks
+  const int qk_heads = a.part_q ? a.heads * splits : a.groups, qk_head = a.part_q ? h * splits + static_cast<int>(blockIdx.y) : gr;
+  const int64_t qk_t = static_cast<int64_t>(qk_heads) * a.keys, qk_at = (row0 * qk_heads + qk_head) * a.keys;
+  const int64_t v_t = static_cast<int64_t>(a.heads) * a.values;
+  T* dv = static_cast<T*>(a.dv) + (row0 * a.heads + h) * a.values + vb;
+  const bool pieces_v = a.values * sizeof(T) % 16 == 0, pieces_k = a.keys * sizeof(T) % 16 == 0;
+  const int vl = warp * 16, c0 = warp * B::kColumns, vsteps = (mine + 15) / 16;
+  const bool by_v = vl < mine, by_k = c0 < DK && c0 < a.keys;
+  constexpr int kPairs = B::kColumns / 16;
+  float* dstate = a.dstate ? a.dstate + ((static_cast<int64_t>(bi) * a.heads + h) * a.values + vb) * a.keys : nullptr;
+  const float* dfinal = a.dfinal ? a.dfinal + ((static_cast<int64_t>(bi) * a.heads + h) * a.values + vb) * a.keys : nullptr;
+
+  // d[n]: rows vl + row, + 8; keys 8 n + col, + 1
   float d[DK / 8][4];
 #pragma unroll
   for (int n = 0; n < DK / 8; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int r = v0 + row + (e >> 1) * 8, kc = 8 * n + col + (e & 1);
-      d[n][e] = a.dfinal && r < a.values && kc < a.keys ? a.dfinal[head_at + static_cast<int64_t>(r) * a.keys + kc] : 0.0f;
+      const int r = vl + row + (e >> 1) * 8, kc = 8 * n + col + (e & 1);
+      d[n][e] = dfinal && r < mine && kc < a.keys ? dfinal[r * a.keys + kc] : 0.0f;
     }
-  double sum_a = 0.0, sum_bias = 0.0;
+  // what a warp without values or columns leaves
+  for (int turn = 0; turn < 2; ++turn) {
+    for (int i = lane; i < 2 * kTile * kMat; i += 32) (&sh.part[turn][warp][0][0][0])[i] = 0.0f;
+    for (int i = lane; i < 3 * kTile; i += 32) (&sh.by_value[turn][warp][0][0])[i] = 0.0f;
+    if (lane < kTile) sh.by_key[turn][warp][lane] = 0.0f;
+    if (lane == 0) sh.inner[turn][warp] = 0.0f;
+  }
+  __syncwarp();
 
-  int t1 = length;                                     // the chunk's end
-  while (t1 > 0) {
-    // its start: the tile's, or the last reset before its end
-    int t0 = (t1 - 1) / kTile * kTile;
-    bool fresh = false;
-    if (reset) {
-      const unsigned cuts = __ballot_sync(0xffffffffu, lane < t1 - t0 && reset[t0 + lane]);
-      if (cuts) {
-        t0 += 31 - __clz(cuts);
-        fresh = true;
-      }
-    }
-    const int n = t1 - t0;
-    const float* S = !fresh ? a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * head_size : nullptr;
-    __syncthreads();
-    Keys::load(sh.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k, threadIdx.x, blockDim.x);
-    Keys::load(sh.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k, threadIdx.x, blockDim.x);
-    Values::load(sh.tv, v + t0 * a.v_t, a.v_t, n, a.values, a.piece_v, threadIdx.x, blockDim.x);
-    Values::load(sh.tdo, dout + t0 * a.do_t, a.do_t, n, a.values, a.piece_v, threadIdx.x, blockDim.x);
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncthreads();
-    Gate gate{};
-    if (warp == 0) {
-      if (lane < n) gate = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
-      prepare<T, DK, true>(c, sh.tk, sh.tq, gate.g, gate.beta, a.scale, a.unit);
-    }
-    __syncthreads();
-
-    float z[2][4] = {};
+  for (int i = 0;; ++i) {
+    const int at = i % kStages, turn = i & 1;
+    typename B::Stage& st = sh.stage[at];
+    const Chunk<T, NI>& c = st.c;
+    bar_sync(1 + at, stage_threads);
+    const int t0 = st.t0, n = st.n;
+    if (n == 0) break;
+    const bool fresh = st.fresh;
     if (by_v) {
-      // K S^T and K dS^T (rows values, columns tokens), <dS, S>; S's planes to shared memory
-      float sk[2][4] = {}, dsk[2][4] = {}, inner = 0.0f;
-      const uint32_t ka = smem_of(sh.tk) + at_rows(lane, Keys::kPitch);
+      // K dS^T (rows values, columns tokens), <dS, S>; dS's planes to shared memory
+      float ds[2][4] = {}, inner = 0.0f;
+      const uint32_t ka = smem_of(st.tk) + at_rows(lane, Keys::kPitch);
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        float s[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = v0 + row + (e >> 1) * 8, kc = 16 * i + 8 * t + col + (e & 1);
-            s[t][e] = S && r < a.values && kc < a.keys ? S[static_cast<int64_t>(r) * a.keys + kc] : 0.0f;
-            inner = fmaf(s[t][e], d[2 * i + t][e], inner);
-          }
-        uint32_t b[NT][4];
-        load_planes<NT, false>(b, ka + i * 32, Keys::kPlane * 2);
+      for (int x = 0; x < kSteps; ++x) {
         Frag<NI> f;
-        f.from(s[0], s[1]);
-        mma_planes<NI, NT>(sk[0], sk[1], f.r, b);
+        f.from(d[2 * x], d[2 * x + 1]);
+        uint32_t b[NT][4];
+        load_planes<NT, false>(b, ka + x * 32, Keys::kPlane * 2);
+        mma_planes<NI, NT>(ds[0], ds[1], f.r, b);
+        put_frag(sh.d, vl + row, 16 * x + col, f);
+        if (!fresh)
 #pragma unroll
-        for (int p = 0; p < NI; ++p)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint32_t*>(&sh.st[p][v0 + row + (e & 1) * 8][16 * i + (e >> 1) * 8 + col]) = f.r[p][e];
-        f.from(d[2 * i], d[2 * i + 1]);
-        mma_planes<NI, NT>(dsk[0], dsk[1], f.r, b);
+            for (int e = 0; e < 2; ++e) {
+              const float2 s = *reinterpret_cast<const float2*>(&st.s[vl + row + 8 * e][16 * x + 8 * t + col]);
+              inner = fmaf(s.x, d[2 * x + t][2 * e], fmaf(s.y, d[2 * x + t][2 * e + 1], inner));
+            }
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, o);
-      if (lane == 0) sh.inner[warp] = inner;
-      // W
-      float w[2][4] = {}, du[2][4] = {};
+      if (lane == 0) sh.inner[turn][warp] = inner;
+      // dU, Z
+      float w[2][4], du[2][4] = {}, z[2][4] = {};
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = t * 8 + col + (e & 1), r = v0 + row + (e >> 1) * 8;
-          sk[t][e] *= c.head[tok] * c.rk[tok];
-          dsk[t][e] *= c.tail[tok] * c.rk[tok];
-          z[t][e] = tile_at<T>(sh.tv, Values::kPlane, tok * Values::kPitch + r) - sk[t][e];
+        for (int e = 0; e < 2; ++e) {
+          const float2 y = *reinterpret_cast<const float2*>(&st.w[vl + row + 8 * e][8 * t + col]);
+          w[t][2 * e] = y.x;
+          w[t][2 * e + 1] = y.y;
         }
       {
-        Frag<NI> f;
-        f.from(z[0], z[1]);
-        uint32_t b[NI][4];
-        load_planes<NI, false>(b, smem_of(c.inv) + at_rows(lane, kSide), kTile * kSide * 2);
-        mma_planes<NI, NI>(w[0], w[1], f.r, b);
-        f.from(w[0], w[1]);
-#pragma unroll
-        for (int p = 0; p < NI; ++p)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint32_t*>(&sh.w[p][v0 + row + (e & 1) * 8][(e >> 1) * 8 + col]) = f.r[p][e];
-      }
-      // dU, Z
-      {
         uint32_t o[NT][4], b[NI][4];
-        load_planes<NT, true>(o, smem_of(sh.tdo) + a_cols(lane, Values::kPitch) + v0 * 2, Values::kPlane * 2);
+        load_planes<NT, true>(o, smem_of(st.tdo) + a_cols(lane, Values::kPitch) + vl * 2, Values::kPlane * 2);
         load_planes<NI, true>(b, smem_of(c.p) + at_cols(lane, kSide), kTile * kSide * 2);
         mma_planes<NT, NI>(du[0], du[1], o, b);
         float x[2][4];
@@ -200,310 +394,239 @@ template <typename T, int DK> __global__ void __launch_bounds__(256) delta_backw
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            du[t][e] += dsk[t][e];
-            x[t][e] = c.beta[t * 8 + col + (e & 1)] * du[t][e];
-            z[t][e] = 0.0f;
+            const int tok = t * 8 + col + (e & 1);
+            ds[t][e] *= c.tail[tok] * c.rk[tok];
+            du[t][e] += ds[t][e];
+            x[t][e] = c.beta[tok] * du[t][e];
           }
         Frag<NI> f;
         f.from(x[0], x[1]);
         load_planes<NI, true>(b, smem_of(c.inv) + at_cols(lane, kSide), kTile * kSide * 2);
         mma_planes<NI, NI>(z[0], z[1], f.r, b);
         f.from(z[0], z[1]);
-#pragma unroll
-        for (int p = 0; p < NI; ++p)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint32_t*>(&sh.z[p][v0 + row + (e & 1) * 8][(e >> 1) * 8 + col]) = f.r[p][e];
+        put_frag(sh.z, vl + row, col, f);
+        f.from(w[0], w[1]);
+        put_frag(sh.w, vl + row, col, f);
       }
-      // sums over the warp's values, by tokens; dv
+      // sums over the warp's values, by tokens
+      T (&so)[kTile][16 + 16 / sizeof(T)] = sh.out[warp];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int tok = t * 8 + col + e;
+          const float v0 = to_f(st.tv[tok * B::kPitchV + vl + row]), v1 = to_f(st.tv[tok * B::kPitchV + vl + row + 8]);
           const float wd = column_sum(fmaf(w[t][e], du[t][e], w[t][e + 2] * du[t][e + 2]));
-          const float keep = column_sum(fmaf(z[t][e], sk[t][e], z[t][e + 2] * sk[t][e + 2]));
-          const float send = column_sum(fmaf(w[t][e], dsk[t][e], w[t][e + 2] * dsk[t][e + 2]));
+          const float zv = column_sum(fmaf(z[t][e], v0, z[t][e + 2] * v1));
+          const float send = column_sum(fmaf(w[t][e], ds[t][e], w[t][e + 2] * ds[t][e + 2]));
           if (row == 0) {
-            sh.by_value[warp][0][tok] = wd;
-            sh.by_value[warp][1][tok] = -keep;
-            sh.by_value[warp][2][tok] = c.beta[tok] * send;
+            sh.by_value[turn][warp][0][tok] = wd;
+            sh.by_value[turn][warp][1][tok] = zv;
+            sh.by_value[turn][warp][2][tok] = c.beta[tok] * send;
           }
-          if (tok < n) {
-            if (v0 + row < a.values) dv[(t0 + tok) * v_t + v0 + row] = from_f<T>(z[t][e]);
-            if (v0 + row + 8 < a.values) dv[(t0 + tok) * v_t + v0 + row + 8] = from_f<T>(z[t][e + 2]);
+          so[tok][row] = from_f<T>(z[t][e]);
+          so[tok][row + 8] = from_f<T>(z[t][e + 2]);
+        }
+      __syncwarp();
+      put_rows(dv + t0 * v_t + vl, v_t, so, n, mine - vl, pieces_v);
+      // the warp's part of Z W^T and dO W^T
+      {
+        uint32_t b[NI][4], x[NI][4], o[NT][4];
+        float zw[2][4] = {}, ow[2][4] = {};
+        load_planes<NI, true>(b, smem_of(sh.w) + at_cols(lane, kSide) + vl * kSide * 2, kValues * kSide * 2);
+        load_planes<NI, true>(x, smem_of(sh.z) + a_cols(lane, kSide) + vl * kSide * 2, kValues * kSide * 2);
+        mma_planes<NI, NI>(zw[0], zw[1], x, b);
+        load_planes<NT, false>(o, smem_of(st.tdo) + a_rows(lane, Values::kPitch) + vl * 2, Values::kPlane * 2);
+        mma_planes<NT, NI>(ow[0], ow[1], o, b);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            *reinterpret_cast<float2*>(&sh.part[turn][warp][0][row + 8 * e][8 * t + col]) = make_float2(zw[t][2 * e], zw[t][2 * e + 1]);
+            *reinterpret_cast<float2*>(&sh.part[turn][warp][1][row + 8 * e][8 * t + col]) = make_float2(ow[t][2 * e], ow[t][2 * e + 1]);
           }
-        }
-    }
-    __syncthreads();
-
-    // by keys: S^T dO and S^T Z
-    float aq[2][4] = {}, ak[2][4] = {};
-    if (by_k) {
-      for (int i = 0; i < vwarps; ++i) {
-        uint32_t b[NI][4], o[NT][4], zz[NI][4];
-        load_planes<NI, true>(b, smem_of(sh.st) + at_cols(lane, B::kState) + (i * 16 * B::kState + k0) * 2, 128 * B::kState * 2);
-        load_planes<NT, false>(o, smem_of(sh.tdo) + a_rows(lane, Values::kPitch) + i * 32, Values::kPlane * 2);
-        mma_planes<NT, NI>(aq[0], aq[1], o, b);
-        load_planes<NI, true>(zz, smem_of(sh.z) + a_cols(lane, kSide) + i * 16 * kSide * 2, 128 * kSide * 2);
-        mma_planes<NI, NI>(ak[0], ak[1], zz, b);
       }
-      float e0 = 0.0f, e1 = 0.0f;
+      // dS one chunk on
+      if (fresh) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int x = 0; x < DK / 8; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = row + (e >> 1) * 8;
-          aq[t][e] *= a.scale * c.head[tok];
-          ak[t][e] *= -c.head[tok];
-          const float x = aq[t][e] * tile_at<T>(sh.tq, Keys::kPlane, tok * Keys::kPitch + k0 + t * 8 + col + (e & 1));
-          if (e < 2) e0 += x;
-          else e1 += x;
-        }
-      e0 = quad_sum(e0);
-      e1 = quad_sum(e1);
-      if ((lane & 3) == 0) {
-        sh.by_key[warp][0][row] = e0 * c.rq[row];
-        sh.by_key[warp][0][row + 8] = e1 * c.rq[row + 8];
-      }
-    }
-    // Z W^T and dO W^T
-    for (int m = warp; m < 2; m += warps) {
-      float r[2][4] = {};
-      for (int i = 0; i < vwarps; ++i) {
-        uint32_t b[NI][4];
-        load_planes<NI, true>(b, smem_of(sh.w) + at_cols(lane, kSide) + i * 16 * kSide * 2, 128 * kSide * 2);
-        if (m == 0) {
-          uint32_t x[NI][4];
-          load_planes<NI, true>(x, smem_of(sh.z) + a_cols(lane, kSide) + i * 16 * kSide * 2, 128 * kSide * 2);
-          mma_planes<NI, NI>(r[0], r[1], x, b);
-        } else {
-          uint32_t x[NT][4];
-          load_planes<NT, false>(x, smem_of(sh.tdo) + a_rows(lane, Values::kPitch) + i * 32, Values::kPlane * 2);
-          mma_planes<NT, NI>(r[0], r[1], x, b);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) (m ? sh.ow : sh.zw)[row + (e >> 1) * 8][t * 8 + col + (e & 1)] = r[t][e];
-    }
-    __syncthreads();
-
-    // dS to shared memory and one chunk on; a warp makes the 16 x 16 matrices of dq and dk
-    if (by_v) {
-      const float end = c.head[kTile - 1];
-      Frag<NI> fz, fo;
-      float x[2][4];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = t * 8 + col + (e & 1), r = v0 + row + (e >> 1) * 8;
-          z[t][e] *= -c.head[tok] * c.rk[tok];
-          x[t][e] = a.scale * c.head[tok] * c.rq[tok] * tile_at<T>(sh.tdo, Values::kPlane, tok * Values::kPitch + r);
-        }
-      fz.from(z[0], z[1]);
-      fo.from(x[0], x[1]);
-      const uint32_t kt = smem_of(sh.tk) + at_cols(lane, Keys::kPitch), qt = smem_of(sh.tq) + at_cols(lane, Keys::kPitch);
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        Frag<NI> f;
-        f.from(d[2 * i], d[2 * i + 1]);
-#pragma unroll
-        for (int p = 0; p < NI; ++p)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint32_t*>(&sh.st[p][v0 + row + (e & 1) * 8][16 * i + (e >> 1) * 8 + col]) = f.r[p][e];
-        if (fresh) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[2 * i][e] = d[2 * i + 1][e] = 0.0f;
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d[2 * i][e] *= end;
-          d[2 * i + 1][e] *= end;
-        }
-        uint32_t b[NT][4];
-        load_planes<NT, true>(b, kt + i * 32, Keys::kPlane * 2);
-        mma_planes<NI, NT>(d[2 * i], d[2 * i + 1], fz.r, b);
-        load_planes<NT, true>(b, qt + i * 32, Keys::kPlane * 2);
-        mma_planes<NI, NT>(d[2 * i], d[2 * i + 1], fo.r, b);
-      }
-    }
-    if (warp == warps - 1) {
-      for (int x = lane; x < kTile * kTile; x += 32) {
-        const int i = x / kTile, j = x % kTile;
-        const float dec = i >= j ? c.scratch[2][i][j] : 0.0f;
-        const float pd = a.scale * sh.ow[i][j] * c.beta[j] * dec;
-        const int lo = min(i, j), hi = max(i, j);
-        const float md = i == j ? 0.0f : -sh.zw[hi][lo] * c.beta[lo] * c.scratch[2][hi][lo];
-        put_planes<NI>(sh.x1, i, j, i >= j ? pd * c.rk[j] : 0.0f);
-        put_planes<NI>(sh.x2, j, i, i >= j ? pd * c.rq[i] : 0.0f);
-        put_planes<NI>(sh.x3, i, j, md * c.rk[j]);
-      }
-    }
-    __syncthreads();
-
-    if (by_k) {
-      float as[2][4] = {};
-      for (int i = 0; i < vwarps; ++i) {
-        uint32_t b[NI][4], ww[NI][4];
-        load_planes<NI, true>(b, smem_of(sh.st) + at_cols(lane, B::kState) + (i * 16 * B::kState + k0) * 2, 128 * B::kState * 2);
-        load_planes<NI, true>(ww, smem_of(sh.w) + a_cols(lane, kSide) + i * 16 * kSide * 2, 128 * kSide * 2);
-        mma_planes<NI, NI>(as[0], as[1], ww, b);
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = row + (e >> 1) * 8;
-          ak[t][e] = fmaf(c.tail[tok] * c.beta[tok], as[t][e], ak[t][e]);
-        }
-      uint32_t bk[NT][4], x[NI][4];
-      load_planes<NT, true>(bk, smem_of(sh.tk) + at_cols(lane, Keys::kPitch) + k0 * 2, Keys::kPlane * 2);
-      load_planes<NI, false>(x, smem_of(sh.x1) + a_rows(lane, kSide), kTile * kSide * 2);
-      mma_planes<NI, NT>(aq[0], aq[1], x, bk);
-      load_planes<NI, false>(x, smem_of(sh.x3) + a_rows(lane, kSide), kTile * kSide * 2);
-      mma_planes<NI, NT>(ak[0], ak[1], x, bk);
-      load_planes<NT, true>(bk, smem_of(sh.tq) + at_cols(lane, Keys::kPitch) + k0 * 2, Keys::kPlane * 2);
-      load_planes<NI, false>(x, smem_of(sh.x2) + a_rows(lane, kSide), kTile * kSide * 2);
-      mma_planes<NI, NT>(ak[0], ak[1], x, bk);
-      if (a.unit) {
-        float nq[2] = {}, nk[2] = {};
+          for (int e = 0; e < 4; ++e) d[x][e] = 0.0f;
+      } else {
+        const float end = c.head[kTile - 1];
+        float x[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int at = (row + (e >> 1) * 8) * Keys::kPitch + k0 + t * 8 + col + (e & 1);
-            nq[e >> 1] = fmaf(aq[t][e], tile_at<T>(sh.tq, Keys::kPlane, at), nq[e >> 1]);
-            nk[e >> 1] = fmaf(ak[t][e], tile_at<T>(sh.tk, Keys::kPlane, at), nk[e >> 1]);
+            const int tok = t * 8 + col + (e & 1), r = vl + row + (e >> 1) * 8;
+            z[t][e] *= -c.head[tok] * c.rk[tok];
+            x[t][e] = a.scale * c.head[tok] * c.rq[tok] * tile_at<T>(st.tdo, Values::kPlane, tok * Values::kPitch + r);
           }
+        Frag<NI> fz, fo;
+        fz.from(z[0], z[1]);
+        fo.from(x[0], x[1]);
+        const uint32_t kt = smem_of(st.tk) + at_cols(lane, Keys::kPitch), qt = smem_of(st.tq) + at_cols(lane, Keys::kPitch);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          nq[e] = quad_sum(nq[e]);
-          nk[e] = quad_sum(nk[e]);
-          if ((lane & 3) == 0) {
-            sh.by_key[warp][1][row + 8 * e] = nq[e];
-            sh.by_key[warp][2][row + 8 * e] = nk[e];
+        for (int y = 0; y < kSteps; ++y) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            d[2 * y][e] *= end;
+            d[2 * y + 1][e] *= end;
           }
+          uint32_t b[NT][4];
+          load_planes<NT, true>(b, kt + y * 32, Keys::kPlane * 2);
+          mma_planes<NI, NT>(d[2 * y], d[2 * y + 1], fz.r, b);
+          load_planes<NT, true>(b, qt + y * 32, Keys::kPlane * 2);
+          mma_planes<NI, NT>(d[2 * y], d[2 * y + 1], fo.r, b);
         }
       }
     }
-    __syncthreads();
+    bar_sync(kBarChain, team);
+
+    // by keys: rows tokens, columns c0 ..
+    float aq[kPairs][2][4] = {}, ak[kPairs][2][4] = {};
+    if (by_k) {
+      float as[kPairs][2][4] = {};
+      for (int x = 0; x < vsteps; ++x) {
+        uint32_t o[NT][4], z[NS][4], w[NS][4];
+        load_planes<NS, true>(w, smem_of(sh.w) + a_cols(lane, kSide) + x * 16 * kSide * 2, kValues * kSide * 2);
+        if (!fresh) {
+          load_planes<NT, false>(o, smem_of(st.tdo) + a_rows(lane, Values::kPitch) + x * 32, Values::kPlane * 2);
+          load_planes<NS, true>(z, smem_of(sh.z) + a_cols(lane, kSide) + x * 16 * kSide * 2, kValues * kSide * 2);
+        }
+#pragma unroll
+        for (int p = 0; p < kPairs; ++p) {
+          uint32_t b[NS][4];
+          load_planes<NS, true>(b, smem_of(sh.d) + at_cols(lane, B::kPitchD) + (x * 16 * B::kPitchD + c0 + 16 * p) * 2,
+                                kValues * B::kPitchD * 2);
+          mma_planes<NS, NS>(as[p][0], as[p][1], w, b);
+          if (!fresh) {
+            uint32_t s[NI][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float* from = &st.s[16 * x + (e & 1) * 8 + col][c0 + 16 * p + (e >> 1) * 8 + row];
+              uint32_t y[NI];
+              split2<NI>(from[0], from[B::kPitchS], y);
+#pragma unroll
+              for (int m = 0; m < NI; ++m) s[m][e] = y[m];
+            }
+            mma_planes<NT, NI>(aq[p][0], aq[p][1], o, s);
+            mma_planes<NS, NS>(ak[p][0], ak[p][1], z, s);
+          }
+        }
+      }
+      float e0[2] = {};
+#pragma unroll
+      for (int p = 0; p < kPairs; ++p)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tok = row + (e >> 1) * 8;
+            aq[p][t][e] *= a.scale * c.head[tok];
+            ak[p][t][e] = fmaf(c.tail[tok] * c.beta[tok], as[p][t][e], -c.head[tok] * ak[p][t][e]);
+            e0[e >> 1] = fmaf(aq[p][t][e], tile_at<T>(st.tq, Keys::kPlane, tok * Keys::kPitch + c0 + 16 * p + t * 8 + col + (e & 1)), e0[e >> 1]);
+          }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        e0[e] = quad_sum(e0[e]);
+        if ((lane & 3) == 0) sh.by_key[turn][warp][row + 8 * e] = e0[e] * c.rq[row + 8 * e];
+      }
+    }
+    bar_sync(kBarMatrices, team);
 
     if (by_k) {
-      float nq[2] = {}, nk[2] = {};
-      if (a.unit)
+      float nq[2] = {}, nk[2] = {}, rq[2], rk[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          for (int i = 0; i < kwarps; ++i) {
-            nq[e] += sh.by_key[i][1][row + 8 * e];
-            nk[e] += sh.by_key[i][2][row + 8 * e];
+      for (int e = 0; e < 2; ++e) {
+        rq[e] = c.rq[row + 8 * e];
+        rk[e] = c.rk[row + 8 * e];
+        if (!a.unit) continue;
+        nq[e] = sh.nq[row + 8 * e];
+#pragma unroll
+        for (int x = 0; x < kMain; ++x) nq[e] += sh.by_key[turn][x][row + 8 * e];
+        nq[e] *= rq[e];                                // what takes the part along q out of dq, for q itself
+        nk[e] = sh.nk[row + 8 * e] * rk[e];
+      }
+      uint32_t x1[NS][4], x2[NS][4], x3[NS][4];
+      load_planes<NS, false>(x1, smem_of(sh.x1) + a_rows(lane, kSide), kTile * kSide * 2);
+      load_planes<NS, true>(x2, smem_of(sh.x2) + a_cols(lane, kSide), kTile * kSide * 2);
+      load_planes<NS, false>(x3, smem_of(sh.x3) + a_rows(lane, kSide), kTile * kSide * 2);
+#pragma unroll
+      for (int p = 0; p < kPairs; ++p) {
+        const int cp = c0 + 16 * p;
+        uint32_t b[NT][4];
+        load_planes<NT, true>(b, smem_of(st.tk) + at_cols(lane, Keys::kPitch) + cp * 2, Keys::kPlane * 2);
+        mma_planes<NS, NT>(aq[p][0], aq[p][1], x1, b);
+        mma_planes<NS, NT>(ak[p][0], ak[p][1], x3, b);
+        load_planes<NT, true>(b, smem_of(st.tq) + at_cols(lane, Keys::kPitch) + cp * 2, Keys::kPlane * 2);
+        mma_planes<NS, NT>(ak[p][0], ak[p][1], x2, b);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = (row + (e >> 1) * 8) * Keys::kPitch + cp + t * 8 + col + (e & 1);
+            aq[p][t][e] = rq[e >> 1] * (aq[p][t][e] - nq[e >> 1] * tile_at<T>(st.tq, Keys::kPlane, x));
+            ak[p][t][e] = rk[e >> 1] * (ak[p][t][e] - nk[e >> 1] * tile_at<T>(st.tk, Keys::kPlane, x));
           }
-          nq[e] *= c.rq[row + 8 * e] * c.rq[row + 8 * e];
-          nk[e] *= c.rk[row + 8 * e] * c.rk[row + 8 * e];
-        }
+        if (a.part_q) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = row + (e >> 1) * 8, kc = k0 + t * 8 + col + (e & 1);
-          if (tok >= n || kc >= a.keys) continue;
-          const int at = tok * Keys::kPitch + kc;
-          const float x = c.rq[tok] * (aq[t][e] - nq[e >> 1] * tile_at<T>(sh.tq, Keys::kPlane, at));
-          const float y = c.rk[tok] * (ak[t][e] - nk[e >> 1] * tile_at<T>(sh.tk, Keys::kPlane, at));
-          const int64_t to = (t0 + tok) * qk_t + kc;
-          if (pq) {
-            pq[to] = x;
-            pk[to] = y;
-          } else {
-            dq[to] = from_f<T>(x);
-            dk[to] = from_f<T>(y);
+            for (int e = 0; e < 4; ++e) {
+              const int tok = row + (e >> 1) * 8, kc = cp + t * 8 + col + (e & 1);
+              if (tok >= n || kc >= a.keys) continue;
+              a.part_q[qk_at + (t0 + tok) * qk_t + kc] = aq[p][t][e];
+              a.part_k[qk_at + (t0 + tok) * qk_t + kc] = ak[p][t][e];
+            }
+        } else {
+          T (&so)[kTile][16 + 16 / sizeof(T)] = sh.out[warp];
+#pragma unroll
+          for (int turn2 = 0; turn2 < 2; ++turn2) {
+            __syncwarp();
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) so[row + (e >> 1) * 8][t * 8 + col + (e & 1)] = from_f<T>(turn2 ? ak[p][t][e] : aq[p][t][e]);
+            __syncwarp();
+            put_rows(static_cast<T*>(turn2 ? a.dk : a.dq) + qk_at + t0 * qk_t + cp, qk_t, so, n, a.keys - cp, pieces_k);
           }
         }
-    }
-    if (warp == 0) {
-      // the gates: lane m < 16 token m's
-      const int m = lane & 15;
-      float wd = 0.0f, e = 0.0f, f = 0.0f, inner = 0.0f, dbeta, dg;
-      for (int i = 0; i < vwarps; ++i) {
-        wd += sh.by_value[i][0][m];
-        e += sh.by_value[i][1][m];
-        f += sh.by_value[i][2][m];
-        inner += sh.inner[i];
-      }
-      for (int i = 0; i < kwarps; ++i) e += sh.by_key[i][0][m];
-      dbeta = wd;
-      // column m: E's sums from below, into the place of M
-      float below = 0.0f;
-#pragma unroll
-      for (int i = kTile - 1; i >= 0; --i) {
-        if (i > m) {
-          const float zw = sh.zw[i][m], mm = c.scratch[0][i][m];
-          dbeta = fmaf(-mm, zw, dbeta);
-          below += c.beta[m] * fmaf(sh.ow[i][m], c.scratch[1][i][m], -zw * mm);
-        }
-        __syncwarp();
-        if (lane < 16) c.scratch[0][i][m] = i > m ? below : 0.0f;
-      }
-      __syncwarp();
-      dg = c.head[kTile - 1] * inner;
-#pragma unroll
-      for (int j = 0; j < kTile; ++j) {
-        const float ej = __shfl_sync(0xffffffffu, e, j), fj = __shfl_sync(0xffffffffu, f, j);
-        if (j >= m) dg += ej;
-        else dg += fj + c.scratch[0][m][j];
-      }
-      if (lane < n) {
-        const float back = dg * rate * sigmoid(gate.pre);
-        db[(t0 + lane) * static_cast<int64_t>(a.heads)] = from_f<T>(dbeta * gate.beta * (1.0f - gate.beta));
-        ddt[(t0 + lane) * static_cast<int64_t>(a.heads)] = from_f<T>(back);
-        sum_a += static_cast<double>(dg) * gate.delta;
-        sum_bias += back;
       }
     }
-    t1 = t0;
+    __syncwarp();
+    bar_arrive(1 + kStages + at, stage_threads);
   }
 
-  if (a.dstate && by_v) {
+  if (dstate && by_v) {
 #pragma unroll
     for (int n = 0; n < DK / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = v0 + row + (e >> 1) * 8, kc = 8 * n + col + (e & 1);
-        if (r < a.values && kc < a.keys) a.dstate[head_at + static_cast<int64_t>(r) * a.keys + kc] = d[n][e];
+        const int r = vl + row + (e >> 1) * 8, kc = 8 * n + col + (e & 1);
+        if (r < mine && kc < a.keys) dstate[r * a.keys + kc] = d[n][e];
       }
   }
-  if (warp == 0) {
-    for (int o = 16; o; o >>= 1) {
-      sum_a += __shfl_xor_sync(0xffffffffu, sum_a, o);
-      sum_bias += __shfl_xor_sync(0xffffffffu, sum_bias, o);
-    }
-    if (lane == 0) {
-      a.part_h[blockIdx.x * 2] = static_cast<float>(sum_a);
-      a.part_h[blockIdx.x * 2 + 1] = static_cast<float>(sum_bias);
-    }
-  }
   // tokens that are not there
-  for (int t = length; t < a.length; ++t) {
-    for (int i = threadIdx.x; i < a.keys; i += blockDim.x) {
-      if (pq) pq[t * qk_t + i] = pk[t * qk_t + i] = 0.0f;
-      else dq[t * qk_t + i] = dk[t * qk_t + i] = from_f<T>(0.0f);
+  for (int t = length + warp; t < a.length; t += kMain) {
+    for (int x = lane; x < a.keys; x += 32) {
+      const int64_t to = qk_at + t * qk_t + x;
+      if (a.part_q) a.part_q[to] = a.part_k[to] = 0.0f;
+      else static_cast<T*>(a.dq)[to] = static_cast<T*>(a.dk)[to] = from_f<T>(0.0f);
     }
-    for (int i = threadIdx.x; i < a.values; i += blockDim.x) dv[t * v_t + i] = from_f<T>(0.0f);
-    if (threadIdx.x == 0) ddt[t * static_cast<int64_t>(a.heads)] = db[t * static_cast<int64_t>(a.heads)] = from_f<T>(0.0f);
+    for (int x = lane; x < mine; x += 32) dv[t * v_t + x] = from_f<T>(0.0f);
   }
 }
 
 // dA and dbias: the sequences' in order.
-__global__ void __launch_bounds__(32) delta_rates(DeltaArgs a) {
+__global__ void __launch_bounds__(32) delta_rates(DeltaArgs a, int splits) {
   const int h = blockIdx.x, lane = threadIdx.x;
   double x = 0.0, y = 0.0;
-  for (int b = lane; b < a.batch; b += 32) {
-    x += a.part_h[(static_cast<int64_t>(b) * a.heads + h) * 2];
-    y += a.part_h[(static_cast<int64_t>(b) * a.heads + h) * 2 + 1];
+  for (int i = lane; i < a.batch * splits; i += 32) {
+    const int64_t at = ((static_cast<int64_t>(i / splits) * a.heads + h) * splits + i % splits) * 2;
+    x += a.part_h[at];
+    y += a.part_h[at + 1];
   }
   for (int o = 16; o; o >>= 1) {
     x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -515,32 +638,44 @@ __global__ void __launch_bounds__(32) delta_rates(DeltaArgs a) {
   }
 }
 
-// dq and dk of key heads that value heads share: theirs summed, in order.
-template <typename T> __global__ void __launch_bounds__(256) delta_shared(DeltaArgs a) {
-  const int64_t total = static_cast<int64_t>(a.batch) * a.length * a.groups * a.keys;
-  const int rep = a.heads / a.groups;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t head = i / a.keys, at = head * rep * a.keys + (i - head * a.keys);
+// Parts of dq and dk (of the value heads of a key head, of their blocks) and of ddt and db, summed in order.
+template <typename T> __global__ void __launch_bounds__(256) delta_parts(DeltaArgs a, int splits) {
+  const int64_t tokens = static_cast<int64_t>(a.batch) * a.length, total = tokens * a.groups * a.keys;
+  const int parts = a.heads / a.groups * splits;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = first; i < total; i += step) {
+    const int64_t head = i / a.keys, at = head * parts * a.keys + (i - head * a.keys);
     float x = 0.0f, y = 0.0f;
-    for (int r = 0; r < rep; ++r) {
+    for (int r = 0; r < parts; ++r) {
       x += a.part_q[at + static_cast<int64_t>(r) * a.keys];
       y += a.part_k[at + static_cast<int64_t>(r) * a.keys];
     }
     static_cast<T*>(a.dq)[i] = from_f<T>(x);
     static_cast<T*>(a.dk)[i] = from_f<T>(y);
   }
+  if (a.part_g)
+    for (int64_t i = first; i < tokens * a.heads; i += step) {
+      float x = 0.0f, y = 0.0f;
+      for (int r = 0; r < splits; ++r) {
+        x += a.part_g[(i * splits + r) * 2];
+        y += a.part_g[(i * splits + r) * 2 + 1];
+      }
+      static_cast<T*>(a.ddt)[i] = from_f<T>(x);
+      static_cast<T*>(a.db)[i] = from_f<T>(y);
+    }
 }
 
 template <typename T, int DK> int backward(const DeltaArgs& a, cudaStream_t s) {
   using B = Backward<T, DK>;
+  const int splits = (a.values + kValues - 1) / kValues;
+  if ((splits > 1 && !a.part_g) || (splits * a.heads != a.groups && !a.part_q)) return static_cast<int>(cudaErrorInvalidValue);
   if (const int e = allow_smem<delta_backward<T, DK>>(B::kBytes)) return e;
-  const int warps = max((a.values + 15) / 16, (a.keys + 15) / 16);
-  delta_backward<T, DK><<<a.batch * a.heads, warps * 32, B::kBytes, s>>>(a);
+  delta_backward<T, DK><<<dim3(a.batch * a.heads, splits), kThreads, B::kBytes, s>>>(a);
   if (const cudaError_t e = cudaGetLastError()) return static_cast<int>(e);
-  delta_rates<<<a.heads, 32, 0, s>>>(a);
+  delta_rates<<<a.heads, 32, 0, s>>>(a, splits);
   if (a.part_q && a.length > 0) {
     const int64_t blocks = (static_cast<int64_t>(a.batch) * a.length * a.groups * a.keys + 255) / 256;
-    delta_shared<T><<<blocks < 148 * 16 ? static_cast<unsigned>(blocks) : 148 * 16, 256, 0, s>>>(a);
+    delta_parts<T><<<blocks < 148 * 16 ? static_cast<unsigned>(blocks) : 148 * 16, 256, 0, s>>>(a, splits);
   }
   return static_cast<int>(cudaGetLastError());
 }

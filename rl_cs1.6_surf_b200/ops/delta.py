@@ -39,12 +39,13 @@ _lib.register(DLIB, {
     "surf_delta_step": (_I, [c_char_p, _I, _V]),
 })
 
-MAX_HEAD, SAVE_EVERY, NORM_EPS = 128, 16, 1e-6
+MAX_HEAD, TILE, NORM_EPS = 128, 16, 1e-6
+_VALUES = 64                                    # of a block of the gradient
 
 Delta = namedtuple("Delta", "out final saved")
 DeltaGrads = namedtuple("DeltaGrads", "dq dk dv ddt db dA ddt_bias dstate")
 
-_ARGS = struct.Struct("45qf9i")
+_ARGS = struct.Struct("46qf9i")
 _STEP = struct.Struct("22qf7i")
 
 
@@ -95,7 +96,8 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dt: torch.Ten
                 state: Optional[torch.Tensor] = None, reset: Optional[torch.Tensor] = None,
                 lengths: Optional[torch.Tensor] = None, train: bool = False, out: Optional[torch.Tensor] = None) -> Delta:
     """The rule over whole rows: ``out`` [B, T, H, V] and ``final`` [B, H, V, K]. ``train`` keeps in
-    ``saved`` the states that ``gated_delta_grad`` starts from: 4 H V K bytes for every 16 tokens. ``out`` must
+    ``saved`` what ``gated_delta_grad`` starts from, the states before and the corrections of every 16
+    tokens: 4 H V (K + 16) bytes. ``out`` must
     not share memory with an input."""
     what = "gated_delta"
     code, e, at, bsz, t, g, h, nk, nv = _check(what, q, k, v, dt, b, A, dt_bias, state, reset, lengths)
@@ -106,11 +108,11 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dt: torch.Ten
         _lib.require_apart(what, "out", out, dict(q=q, k=k, v=v, dt=dt, b=b, A=A, dt_bias=dt_bias, state=state, reset=reset,
                                                   lengths=lengths))
     final = A.new_empty((bsz, h, nv, nk))
-    saved = A.new_empty((bsz, -(-t // SAVE_EVERY), h, nv, nk)) if train else None
+    saved = A.new_empty((bsz, -(-t // TILE), h, nv, nk + TILE)) if train else None
     if bsz == 0:
         return Delta(out, final, saved)
     args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt.data_ptr(), b.data_ptr(), A.data_ptr(), _p(dt_bias), _p(state),
-                      _p(reset), _p(lengths), out.data_ptr(), final.data_ptr(), _p(saved), *(0,) * 13,
+                      _p(reset), _p(lengths), out.data_ptr(), final.data_ptr(), _p(saved), *(0,) * 14,
                       *_strides(q, k, v), *dt.stride()[:2], *b.stride()[:2], *_strides(out), 0, 0, 0,
                       nk ** -0.5 if scale is None else scale, bsz, t, g, h, nk, nv, normalize,
                       _piece(_bits(e, q, k) | nk * e), _piece(_bits(e, v, out) | nv * e))
@@ -133,26 +135,27 @@ def gated_delta_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     _dense(what, "dfinal", dfinal, (bsz, h, nv, nk), f32, at)
     if saved is None:
         raise ValueError(f"{what}: needs the states that gated_delta(train=True) saved")
-    _dense(what, "saved", saved, (bsz, -(-t // SAVE_EVERY), h, nv, nk), f32, at)
+    _dense(what, "saved", saved, (bsz, -(-t // TILE), h, nv, nk + TILE), f32, at)
     dq, dk, dv, ddt, db = (_like(x) for x in (q, k, v, dt, b))
     dA, dbias, dstate = torch.empty_like(A), None if dt_bias is None else torch.empty_like(dt_bias), \
         None if state is None else torch.empty_like(state)
     if bsz == 0:
         return DeltaGrads(dq, dk, dv, ddt, db, dA.zero_(), None if dbias is None else dbias.zero_(), dstate)
-    shared = g != h
-    n = bsz * t * h * nk if shared else 0
-    ws = A.new_empty(2 * n + 2 * bsz * h)
+    splits = -(-nv // _VALUES)
+    n = bsz * t * h * splits * nk if g != h * splits else 0         # parts that a second kernel sums
+    m = bsz * t * h * splits * 2 if splits > 1 else 0
+    ws = A.new_empty(2 * n + m + 2 * bsz * h * splits)
     base = ws.data_ptr()
     args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt.data_ptr(), b.data_ptr(), A.data_ptr(), _p(dt_bias), _p(state),
                       _p(reset), _p(lengths), 0, 0, saved.data_ptr(), dout.data_ptr(), _p(dfinal), dq.data_ptr(), dk.data_ptr(),
-                      dv.data_ptr(), ddt.data_ptr(), db.data_ptr(), _p(dstate), base if shared else 0,
-                      base + 4 * n if shared else 0, base + 8 * n, dA.data_ptr(), _p(dbias),
+                      dv.data_ptr(), ddt.data_ptr(), db.data_ptr(), _p(dstate), base if n else 0,
+                      base + 4 * n if n else 0, base + 8 * n if m else 0, base + 8 * n + 4 * m, dA.data_ptr(), _p(dbias),
                       *_strides(q, k, v), *dt.stride()[:2], *b.stride()[:2], 0, 0, 0, *_strides(dout),
                       nk ** -0.5 if scale is None else scale, bsz, t, g, h, nk, nv, normalize,
                       _piece(_bits(e, q, k) | nk * e), _piece(_bits(e, v, dout) | nv * e))
     launch(_lib.lib(DLIB).surf_delta_grad, "surf_delta_grad", at, args, code)
     del ws                                     # the stream's next user comes after the launch
-    _lib.add_launches(2 if shared else 1)
+    _lib.add_launches(2 if n else 1)
     return DeltaGrads(dq, dk, dv, ddt, db, dA, dbias, dstate)
 
 
