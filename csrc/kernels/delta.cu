@@ -7,16 +7,17 @@ namespace {
 using namespace delta;
 
 // ---- sequences --------------------------------------------------------------------------
-constexpr int kPrep = 2;                               // warps that make chunks ready
+constexpr int kPrep = 2, kMain = 4;                    // warps that make chunks ready, that carry them out at most
 
 template <typename T, int DK> struct Forward {
-  // chunks ready, in the making or on their way: three for each of the warps, two where they would not fit
-  static constexpr int kStages = sizeof(T) == 4 && DK == 128 ? 2 * kPrep : 3 * kPrep;
+  // chunks ready, in the making or on their way
+  static constexpr int kStages = 4;
   using Keys = Tile<T, DK>;
   static_assert(kStages % kPrep == 0, "a stage's barriers are one warp's");
   struct Stage {
     Chunk<T, Planes<T>::kShort> c;
-    int t0, n, fresh;
+    int t0, n, more;                                   // more: the tile's next episode follows in this stage
+    unsigned marks;
     alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize];
   };
   struct Shared {
@@ -31,11 +32,11 @@ template <typename T, int DK> struct Forward {
   }
 };
 
-// A block for up to 128 values of a sequence's value head. Two warps make the chunks ready in turn
+// A block for up to 64 values of a sequence's value head. Two warps make the chunks ready in turn
 // (tiles, decays, P, the inverse: nothing of it waits for the state), the others hold 16 values'
 // rows of the state each, as accumulators from the first token to the last. They meet at
 // numbered barriers: stage s is ready (1 + s), stage s is free (1 + kStages + s).
-template <typename T, int DK> __global__ void __launch_bounds__(320) delta_forward(DeltaArgs a) {
+template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kPrep + kMain) * 32, kBlocks) delta_forward(DeltaArgs a) {
   constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort, kSteps = DK / 16;
   using F = Forward<T, DK>;
   using Keys = Tile<T, DK>;
@@ -57,64 +58,69 @@ template <typename T, int DK> __global__ void __launch_bounds__(320) delta_forwa
     const T* dt = static_cast<const T*>(a.dt) + bi * a.dt_b + h;
     const T* gb = static_cast<const T*>(a.b) + bi * a.b_b + h;
     const float rate = rate_at(a.A, h), bias = a.bias ? a.bias[h] : 0.0f;
-    Chunks walk(a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length);
-    // at chunk `to`, or past the last: index is then their number
-    int index = -1;
-    bool more = true;
-    auto advance = [&](int to) {
-      while (more && index < to) {
-        more = walk.next();
-        ++index;
-      }
-    };
-    // chunk i's tokens on their way to its stage, its gates in registers
-    float raw_dt = 0.0f, raw_b = 0.0f;
-    int at = 0, n = 0;
-    auto fetch = [&](int i) {
-      at = i % kStages;
-      typename F::Stage& st = sh.stage[at];
-      if (i >= kStages) bar_sync(1 + kStages + at, threads);
-      const int t0 = walk.t0;
-      n = walk.n;
+    const int tiles = (length + kTile - 1) / kTile;
+    Marks look{a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length, 0u};
+    // Tokens [t0, t0 + n) on their way to a stage; their decays are made meanwhile.
+    auto fetch = [&](typename F::Stage& st, T* tv, int t0, int n, unsigned marks) {
+      Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k == 16);
+      Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k == 16);
+      load_rows(tv, pitch_v, kTile, warps * 16, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
+      cp_async_commit();
+      Gate e{};
+      if (lane < n) e = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
+      decays(st.c, e.g, e.beta, marks);
       if (lane == 0) {
         st.t0 = t0;
         st.n = n;
-        st.fresh = walk.fresh;
+        st.marks = marks;
+        st.more = 0;
       }
-      Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k, lane, 32);
-      Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k, lane, 32);
-      load_rows(values + at * kTile * pitch_v, pitch_v, kTile, warps * 16, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
-      cp_async_commit();
-      if (lane < n) {
-        raw_dt = to_f(dt[(t0 + lane) * a.dt_t]);
-        raw_b = to_f(gb[(t0 + lane) * a.b_t]);
-      }
+      return __any_sync(0xffffffffu, fmaf(e.g, 0.0f, e.beta * 0.0f) != 0.0f);
     };
-    auto finish = [&] {                                // the end is the warp's to say whose chunk it would be
-      if (index % kPrep != w) return;
-      const int to = index % kStages;
-      if (index >= kStages) bar_sync(1 + kStages + to, threads);
-      if (lane == 0) sh.stage[to].n = 0;
-      __syncwarp();
-      bar_arrive(1 + to, threads);
+    bool bad_here = false, bad_next = false;
+    unsigned marks_here = 0, marks_next = 0;
+    auto begin = [&](int i) {
+      const int at = i % kStages;
+      if (i >= kStages) bar_sync(1 + kStages + at, threads);
+      marks_next = look.get();
+      look.look((i + kPrep) * kTile);
+      bad_next = fetch(sh.stage[at], values + at * kTile * pitch_v, i * kTile, min(kTile, length - i * kTile), marks_next);
     };
-    advance(w);
-    if (!more) return finish();
-    fetch(w);
-    for (int i = w;; i += kPrep) {
+    look.look(w * kTile);
+    if (w < tiles) begin(w);
+    for (int i = w; i < tiles; i += kPrep) {
+      const int at = i % kStages, t0 = i * kTile, n = min(kTile, length - t0);
       typename F::Stage& st = sh.stage[at];
-      const int here = at;
-      Gate e{};
-      if (lane < n) e = gate_of(raw_dt, raw_b, bias, rate);
-      advance(i + kPrep);
-      if (more) fetch(i + kPrep);
+      T* tv = values + at * kTile * pitch_v;
+      marks_here = marks_next;
+      bad_here = bad_next;
+      if (i + kPrep < tiles) begin(i + kPrep);
       else cp_async_commit();
       cp_async_wait<1>();
       __syncwarp();
-      prepare<T, DK, false>(st.c, sh.scratch[w], nullptr, st.tk, st.tq, e.g, e.beta, a.scale, a.unit);
-      bar_arrive(1 + here, threads);
-      if (!more) return finish();
+      auto ready = [&](unsigned marks) {
+        prepare<T, DK, false>(st.c, sh.scratch[w], nullptr, st.tk, st.tq, marks, a.scale, a.unit);
+        bar_arrive(1 + at, threads);
+      };
+      const bool split = (marks_here & ~1u) && (bad_here || not_finite(st.tk, Keys::kPitch, DK, n) || not_finite(st.tq, Keys::kPitch, DK, n) ||
+                                                not_finite(tv, pitch_v, warps * 16, n));
+      if (!split) {
+        ready(marks_here);
+        continue;
+      }
+      for (unsigned left = marks_here | 1u; left;) {
+        const int from = __ffs(left) - 1;
+        left &= left - 1;
+        const unsigned mark = (marks_here >> from) & 1u;
+        if (from > 0) bar_sync(1 + kStages + at, threads);
+        fetch(st, tv, t0 + from, (left ? __ffs(left) - 1 : n) - from, mark);
+        if (lane == 0) st.more = left != 0;
+        cp_async_wait<0>();
+        __syncwarp();
+        ready(mark);
+      }
     }
+    return;
   }
 
   const int row = lane >> 2, col = (lane & 3) * 2, vl = warp * 16, v0 = vb + vl;
@@ -122,7 +128,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(320) delta_forwa
   T* so = values + kStages * kTile * pitch_v + warp * kTile * F::kRow;
   const int64_t head_size = static_cast<int64_t>(a.values) * a.keys;
   const int64_t head_at = (static_cast<int64_t>(bi) * a.heads + h) * head_size;
-  const bool pairs = (a.keys & 1) == 0;
+  const bool pairs = (a.keys & 1) == 0, even = (reinterpret_cast<uintptr_t>(a.state) & 7) == 0;
 
   // s[n]: rows v0 + row, + 8; keys 8 n + col, + 1
   float s[DK / 8][4];
@@ -145,53 +151,116 @@ template <typename T, int DK> __global__ void __launch_bounds__(320) delta_forwa
     });
   };
   each([&](float& x, float& y, int r, int kc) {
-    const bool on = a.state && r < a.values;
+    const bool on = a.state && r < a.values && kc < a.keys;
     const float* p = a.state + head_at + r * a.keys + kc;
-    x = on && kc < a.keys ? p[0] : 0.0f;
-    y = on && kc + 1 < a.keys ? p[1] : 0.0f;
+    if (pairs && even) {
+      const float2 v = on ? *reinterpret_cast<const float2*>(p) : make_float2(0.0f, 0.0f);
+      x = v.x;
+      y = v.y;
+    } else {
+      x = on ? p[0] : 0.0f;
+      y = on && kc + 1 < a.keys ? p[1] : 0.0f;
+    }
   });
 
   const int tiles = (a.length + kTile - 1) / kTile;
-  for (int i = 0;; ++i) {
+  for (int i = 0, more = 0; i < (length + kTile - 1) / kTile; i += more ? 0 : 1) {
     const int at = i % kStages;
     typename F::Stage& st = sh.stage[at];
     bar_sync(1 + at, threads);
     const int t0 = st.t0, n = st.n;
-    if (n == 0) break;
+    const unsigned marks = st.marks;
+    more = st.more;
     const Chunk<T, NS>& c = st.c;
     float* saved = a.saved ? a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values * (a.keys + kTile) : nullptr;
     if (saved && t0 % kTile == 0) store(saved, a.keys + kTile);
-    if (st.fresh) each([&](float& x, float& y, int, int) { x = y = 0.0f; });
+    if (marks & 1u) each([&](float& x, float& y, int, int) { x = y = 0.0f; });
     const T* tv = values + at * kTile * pitch_v;
 
-    // K S^T and Q S^T, transposed: rows values, columns tokens
-    float sk[2][4] = {}, sq[2][4] = {};
-    const uint32_t ka = smem_of(st.tk) + at_rows(lane, Keys::kPitch), qa = smem_of(st.tq) + at_rows(lane, Keys::kPitch);
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      Frag<NI> f;
-      f.from(s[2 * i], s[2 * i + 1]);
-      uint32_t b[NT][4];
-      load_planes<NT, false>(b, ka + i * 32, Keys::kPlane * 2);
-      mma_planes<NI, NT>(sk[0], sk[1], f.r, b);
-      load_planes<NT, false>(b, qa + i * 32, Keys::kPlane * 2);
-      mma_planes<NS, NT>(sq[0], sq[1], f.r, b);
+    // per-token numbers of this lane's columns
+    auto pair = [&](const float (&x)[kTile], int t) { return *reinterpret_cast<const float2*>(&x[8 * t + col]); };
+    // whether the state before the chunk reaches a token
+    auto seen = [&](int tok) { return !(marks & ((2u << tok) - 1u)); };
+    // A state that is not finite ends with its episode: with another one in the chunk the tokens behind
+    // the reset are taken once more, without it (it is not needed any longer then).
+    bool again = false;
+    if (marks & ~1u) {
+      float bad = 0.0f;
+      each([&](float x, float y, int, int) { bad = fmaf(x, 0.0f, fmaf(y, 0.0f, bad)); });
+      again = __any_sync(0xffffffffu, bad != 0.0f);
     }
-    float w[2][4] = {};
-    {
+    float sq[2][4], w[2][4];
+    auto outputs = [&] {
+      // K S^T and Q S^T, transposed: rows values, columns tokens
+      float sk[2][4] = {};
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
+        for (int e = 0; e < 4; ++e) sq[t][e] = w[t][e] = 0.0f;
+      const uint32_t ka = smem_of(st.tk) + at_rows(lane, Keys::kPitch), qa = smem_of(st.tq) + at_rows(lane, Keys::kPitch);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        Frag<NI> f;
+        f.from(s[2 * i], s[2 * i + 1]);
+        uint32_t bk[NT][4], bq[NT][4];
+        load_planes<NT, false>(bk, ka + i * 32, Keys::kPlane * 2);
+        load_planes<NT, false>(bq, qa + i * 32, Keys::kPlane * 2);
+        mma_planes2<NI, NS>(sk[0], sk[1], sq[0], sq[1], f.r, bk, bq);
+      }
+      if (marks)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!seen(8 * t + col + (e & 1))) sk[t][e] = sq[t][e] = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float2 hk = pair(c.head_k, t), hq = pair(c.head_q, t);
+        const T* from = tv + (8 * t + col) * pitch_v + vl + row;
+#pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int tok = t * 8 + col + (e & 1), r = vl + row + (e >> 1) * 8;
-          sk[t][e] = to_f(tv[tok * pitch_v + r]) - c.head[tok] * c.rk[tok] * sk[t][e];
-          sq[t][e] *= a.scale * c.head[tok] * c.rq[tok];
+          sk[t][e] = fmaf(-(e & 1 ? hk.y : hk.x), sk[t][e], to_f(from[(e & 1) * pitch_v + (e >> 1) * 8]));
+          sq[t][e] *= e & 1 ? hq.y : hq.x;
         }
+      }
       Frag<NI> f;
       f.from(sk[0], sk[1]);
       uint32_t b[NI][4];
       load_planes<NI, false>(b, smem_of(c.inv) + at_rows(lane, kSide), kTile * kSide * 2);
       mma_planes<NI, NI>(w[0], w[1], f.r, b);
+      float u[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float2 beta = pair(c.beta, t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[t][e] = w[t][e] * (e & 1 ? beta.y : beta.x);
+      }
+      Frag<NS> g;
+      g.from(u[0], u[1]);
+      uint32_t p[NS][4];
+      load_planes<NS, false>(p, smem_of(c.p) + at_rows(lane, kSide), kTile * kSide * 2);
+      mma_planes<NS, NS>(sq[0], sq[1], g.r, p);
+    };
+    outputs();
+    if (again) {
+      float o0[2][4], w0[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o0[t][e] = sq[t][e];
+          w0[t][e] = w[t][e];
+        }
+      each([&](float& x, float& y, int, int) { x = y = 0.0f; });
+      outputs();
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (seen(8 * t + col + (e & 1))) {
+            sq[t][e] = o0[t][e];
+            w[t][e] = w0[t][e];
+          }
     }
     if (saved) {
       float* p = saved + a.keys + t0 % kTile;
@@ -203,40 +272,30 @@ template <typename T, int DK> __global__ void __launch_bounds__(320) delta_forwa
           if (tok < n && r < a.values) p[r * (a.keys + kTile) + tok] = w[t][e];
         }
     }
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[t][e] *= c.beta[t * 8 + col + (e & 1)];
-    {
-      Frag<NS> f;
-      f.from(w[0], w[1]);
-      uint32_t b[NS][4];
-      load_planes<NS, false>(b, smem_of(c.p) + at_rows(lane, kSide), kTile * kSide * 2);
-      mma_planes<NS, NS>(sq[0], sq[1], f.r, b);
-    }
     // the state
     {
       const float end = c.head[kTile - 1];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t) {
+        const float2 tail = pair(c.tail_k, t), beta = pair(c.beta, t);
+        const float fx = tail.x * beta.x, fy = tail.y * beta.y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = t * 8 + col + (e & 1);
-          w[t][e] *= c.tail[tok] * c.rk[tok];
-        }
+        for (int e = 0; e < 4; ++e) w[t][e] = marks >> (8 * t + col + (e & 1) + 1) ? 0.0f : w[t][e] * (e & 1 ? fy : fx);
+      }
       Frag<NI> f;
       f.from(w[0], w[1]);
       const uint32_t kt = smem_of(st.tk) + at_cols(lane, Keys::kPitch);
+      each([&](float& x, float& y, int, int) {
+        x = marks ? 0.0f : x * end;
+        y = marks ? 0.0f : y * end;
+      });
+      // two steps at a time, so that four sums take turns
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[2 * i][e] *= end;
-          s[2 * i + 1][e] *= end;
-        }
-        uint32_t b[NT][4];
+      for (int i = 0; i < kSteps; i += 2) {
+        uint32_t b[NT][4], d[NT][4];
         load_planes<NT, true>(b, kt + i * 32, Keys::kPlane * 2);
-        mma_planes<NI, NT>(s[2 * i], s[2 * i + 1], f.r, b);
+        load_planes<NT, true>(d, kt + i * 32 + 32, Keys::kPlane * 2);
+        mma_planes2<NI, NI>(s[2 * i], s[2 * i + 1], s[2 * i + 2], s[2 * i + 3], f.r, b, d);
       }
     }
     bar_arrive(1 + kStages + at, threads);
@@ -269,12 +328,13 @@ template <typename T, int DK> __global__ void __launch_bounds__(320) delta_forwa
 
 template <typename T, int DK> int forward(const DeltaArgs& a, cudaStream_t s) {
   using F = Forward<T, DK>;
-  if (const int e = allow_smem<delta_forward<T, DK>>(F::bytes(8))) return e;
-  // values of a block: all, or fewer where that leaves SMs without one
-  int warps = (a.values + 15) / 16;
-  while (warps > 1 && a.batch * a.heads * (((a.values + 15) / 16 + warps - 1) / warps) < 148) warps = (warps + 1) / 2;
-  const int blocks = ((a.values + 15) / 16 + warps - 1) / warps;
-  delta_forward<T, DK><<<dim3(a.batch * a.heads, blocks), (warps + kPrep) * 32, F::bytes(warps), s>>>(a);
+  constexpr int kBlocks = sizeof(T) == 4 ? (DK == 128 ? 1 : 2) : DK == 128 ? 2 : 3;
+  if (const int e = allow_smem<delta_forward<T, DK, kBlocks>>(F::bytes(kMain))) return e;
+  // values of a block: as many as it takes, or fewer where that leaves SMs without one
+  const int all = (a.values + 15) / 16;
+  int warps = all < kMain ? all : kMain;
+  while (warps > 1 && static_cast<int64_t>(a.batch) * a.heads * ((all + warps - 1) / warps) < 148) warps = (warps + 1) / 2;
+  delta_forward<T, DK, kBlocks><<<dim3(a.batch * a.heads, (all + warps - 1) / warps), (warps + kPrep) * 32, F::bytes(warps), s>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T> int forward_by(const DeltaArgs& a, cudaStream_t s) {

@@ -5,15 +5,16 @@
 //   S <- e^g S,  w = v - S k,  S <- S + beta w k^T,  o = scale S q
 // with g = A softplus(dt + bias) <= 0, beta = sigmoid(b), k and q divided by their lengths.
 //
-// A chunk: up to 16 tokens of one episode within one tile of 16. With D_ij = exp(g_j+1 + .. + g_i),
-// head_i = exp(g_1 + .. + g_i), tail_i = D_last,i, end = head_last and
+// A chunk: a tile of 16 tokens, or what a row has of it. With D_ij = exp(g_j+1 + .. + g_i) within an
+// episode and 0 across a reset, head_i = exp(g_1 + .. + g_i) up to the chunk's first reset, tail_i =
+// D_last,i, end = head_last and
 //   M_ij = D_ij k_i.k_j (j < i),  P_ij = scale D_ij q_i.k_j (j <= i):
 //   R = V - head (K S^T),  W = (I + M beta)^-1 R,  U = beta W
 //   O = scale head (Q S^T) + P U,  S+ = end S + sum_i tail_i U_i k_i^T.
-// Every exponent is a sum of terms <= 0 taken afresh for its pair of tokens (never a difference of
-// running sums), so that nothing overflows and a strong decay costs the others no digits.
-// A reset ends a chunk: what stood before it is never multiplied by zero, it is not there, so
-// that infinities and NaN end with their episode.
+// Every exponent is the sum of its tokens' own terms <= 0, so that nothing overflows and a strong
+// decay costs the others no digits.
+// Infinities and NaN end with their episode: where head, tail or end is 0 nothing is multiplied by
+// it, and a chunk with a reset inside and tokens that are not finite is taken episode by episode.
 //
 // Products run on the tensor cores as mma.sync.m16n8k16 with bfloat16 operands and 32-bit sums. A
 // 32-bit number enters as the sum of its planes, each the bfloat16 next to what the ones before
@@ -68,19 +69,19 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x, y -> their planes, packed
+// x, y -> their planes, packed. What a plane leaves comes from one subtraction of mixed types a number
+// (with its sign turned: the next plane's number is turned back by its own).
 template <int N> __device__ __forceinline__ void split2(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     p[i] = surfk::pack_bf16x2(x, y);
-    if (i + 1 < N) {
-      x -= __uint_as_float(p[i] << 16);
-      y -= __uint_as_float(p[i] & 0xffff0000u);
-    }
+    if (i + 1 < N)
+      asm("{.reg .b16 lo, hi;\n mov.b32 {lo, hi}, %2;\n sub.f32.bf16 %0, lo, %0;\n sub.f32.bf16 %1, hi, %1;\n neg.f32 %0, %0;\n neg.f32 %1, %1;}"
+          : "+f"(x), "+f"(y) : "r"(p[i]));
   }
 }
 
@@ -122,18 +123,65 @@ __device__ __forceinline__ uint32_t a_cols(int lane, int pitch) {
 }
 
 // c0, c1 (columns 0-7 and 8-15) += A B over 16 of k, of the first PA and PB planes; products of
-// planes i and j with i + j >= max(PA, PB) are below what the planes leave out.
+// planes i and j with i + j >= max(PA, PB) are below what the planes leave out. An accumulator's
+// next product waits 22 cycles for the one before (one may start every 9): products of two
+// split numbers go to sums of their own by i + j.
 template <int PA, int PB, int NA, int NB>
 __device__ __forceinline__ void mma_planes(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
   static_assert(PA <= NA && PB <= NB, "planes that are there");
+  constexpr int kLevels = PA > PB ? PA : PB;
+  if constexpr (PA == 1 || PB == 1) {
 #pragma unroll
-  for (int i = 0; i < PA; ++i)
+    for (int i = 0; i < PA; ++i)
 #pragma unroll
-    for (int j = 0; j < PB; ++j)
-      if (i + j < (PA > PB ? PA : PB)) {
+      for (int j = 0; j < PB; ++j) {
         mma(c0, a[i], b[j][0], b[j][1]);
         mma(c1, a[i], b[j][2], b[j][3]);
       }
+  } else {
+    float l0[kLevels - 1][4] = {}, l1[kLevels - 1][4] = {};
+#pragma unroll
+    for (int i = PA - 1; i >= 0; --i)
+#pragma unroll
+      for (int j = PB - 1; j >= 0; --j)
+        if (i + j < kLevels && i + j > 0) {
+          mma(l0[i + j - 1], a[i], b[j][0], b[j][1]);
+          mma(l1[i + j - 1], a[i], b[j][2], b[j][3]);
+        }
+    mma(c0, a[0], b[0][0], b[0][1]);
+    mma(c1, a[0], b[0][2], b[0][3]);
+#pragma unroll
+    for (int l = kLevels - 2; l > 0; --l)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        l0[l - 1][e] += l0[l][e];
+        l1[l - 1][e] += l1[l][e];
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c0[e] += l0[0][e];
+      c1[e] += l1[0][e];
+    }
+  }
+}
+// The same for one left operand and two right ones (c += A B, d += A D), planes in turn.
+template <int PC, int PD, int NA, int NB>
+__device__ __forceinline__ void mma_planes2(float (&c0)[4], float (&c1)[4], float (&d0)[4], float (&d1)[4], const uint32_t (&a)[NA][4],
+                                            const uint32_t (&b)[NB][4], const uint32_t (&d)[NB][4]) {
+  if constexpr (NB == 1) {
+#pragma unroll
+    for (int i = 0; i < PC; ++i) {
+      mma(c0, a[i], b[0][0], b[0][1]);
+      mma(c1, a[i], b[0][2], b[0][3]);
+      if (i < PD) {
+        mma(d0, a[i], d[0][0], d[0][1]);
+        mma(d1, a[i], d[0][2], d[0][3]);
+      }
+    }
+  } else {
+    mma_planes<PC, NB>(c0, c1, a, b);
+    mma_planes<PD, NB>(d0, d1, a, d);
+  }
 }
 template <int N, bool kTrans> __device__ __forceinline__ void load_planes(uint32_t (&r)[N][4], uint32_t at, uint32_t plane) {
 #pragma unroll
@@ -144,26 +192,35 @@ template <int N, bool kTrans> __device__ __forceinline__ void load_planes(uint32
 }
 
 // ---- token tiles ------------------------------------------------------------------------
-// Rows [0, n) of `cols` elements, planes kPlane apart with a pitch of W + 8; the rest of 16 x W zero.
+// 16 bytes, or zeros (nothing is read then)
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+// By one warp: rows [0, n) of `cols` elements, planes kPlane apart with a pitch of W + 8; the rest of 16 x W zero.
 template <typename T, int W> struct Tile {
   static constexpr int kPitch = W + 8, kPlane = kTile * kPitch, kSize = Planes<T>::kToken * kPlane;
-  static __device__ __forceinline__ void load(bf16* dst, const T* src, int64_t stride, int n, int cols, int piece, int tid, int threads) {
+  static __device__ __forceinline__ void load(bf16* dst, const T* src, int64_t stride, int n, int cols, bool pieces) {
+    const int lane = threadIdx.x & 31;
     if constexpr (sizeof(T) == 2) {
-      if (piece == 16) {
-        for (int i = tid; i < kTile * W / 8; i += threads) {
-          const int r = i / (W / 8), c = i % (W / 8) * 8;
-          bf16* d = dst + r * kPitch + c;
-          if (r < n && c < cols) cp_async16(d, src + r * stride + c);
-          else *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
+      if (pieces) {
+        constexpr int kPer = W / 8, kRows = 32 / kPer;
+        const int r0 = lane / kPer, c = lane % kPer * 8;
+        const T* from = src + r0 * stride + c;
+        bf16* to = dst + r0 * kPitch + c;
+        const int rows = c < cols ? n : 0;
+#pragma unroll
+        for (int r = 0; r < kTile; r += kRows) {
+          cp_async16_or_zero(to + r * kPitch, r0 + r < rows ? from : src, r0 + r < rows);
+          from += kRows * stride;
         }
       } else {
-        for (int i = tid; i < kTile * W; i += threads) {
+        for (int i = lane; i < kTile * W; i += 32) {
           const int r = i / W, c = i % W;
           dst[r * kPitch + c] = r < n && c < cols ? src[r * stride + c] : from_f<bf16>(0.0f);
         }
       }
     } else {
-      for (int i = tid; i < kTile * W / 2; i += threads) {
+      for (int i = lane; i < kTile * W / 2; i += 32) {
         const int r = i / (W / 2), c = i % (W / 2) * 2;
         const float x = r < n && c < cols ? src[r * stride + c] : 0.0f;
         const float y = r < n && c + 1 < cols ? src[r * stride + c + 1] : 0.0f;
@@ -190,13 +247,18 @@ __device__ __forceinline__ void load_rows(T* dst, int pitch, int rows, int width
   constexpr int V = kVec16<T>;
   const int lane = threadIdx.x & 31;
   if (pieces) {
-    const int w = width / V, bits = min(5, 32 - __clz(w - 1)), c0 = (lane & ((1 << bits) - 1)) * V;
-    for (int r = lane >> bits; r < rows; r += 32 >> bits)
-      for (int c = c0; c < width; c += 32 * V) {
-        T* d = dst + r * pitch + c;
-        if (r < n && c < cols) cp_async16(d, src + r * stride + c);
-        else *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
+    const int bits = min(5, 32 - __clz(width / V - 1)), c = (lane & ((1 << bits) - 1)) * V, r0 = lane >> bits, step = 32 >> bits;
+    for (int x = c; x < width; x += 32 * V) {
+      const T* from = src + r0 * stride + x;
+      T* to = dst + r0 * pitch + x;
+      const int last = x < cols ? n : 0;
+#pragma unroll 4
+      for (int r = r0; r < rows; r += step) {
+        cp_async16_or_zero(to, r < last ? from : src, r < last);
+        from += step * stride;
+        to += step * pitch;
       }
+    }
   } else {
     for (int i = lane; i < rows * width; i += 32) {
       const int r = i / width, c = i - r * width;
@@ -210,6 +272,7 @@ constexpr int kSide = kTile + 8;                       // pitch of 16 x 16 matri
 constexpr int kMat = kTile + 4;                        // and of 32-bit numbers
 template <typename T, int NP> struct Chunk {           // NP: planes of P
   float beta[kTile], head[kTile], tail[kTile], rk[kTile], rq[kTile];
+  float head_k[kTile], head_q[kTile], tail_k[kTile];   // head rk, scale head rq, tail rk
   float g_hi[kTile], g_lo[kTile];                      // running sums of the log decays
   alignas(16) bf16 inv[Planes<T>::kInner][kTile][kSide];         // (I + M beta)^-1
   alignas(16) bf16 p[NP][kTile][kSide];                // P
@@ -217,16 +280,35 @@ template <typename T, int NP> struct Chunk {           // NP: planes of P
 using Scratch = float[2][kTile][kMat];
 struct Wide { float m[kTile][kMat], p[kTile][kMat], d[kTile][kMat]; };   // M, P, D as 32-bit numbers
 
-// By one warp, from the tiles of K and Q and each lane's gates (lane < 16: token lane's log decay and
-// beta, zero behind the chunk); with kKeep into `wide` too.
-//
-// Running sums are kept as two floats, of which differences lose nothing: the larger halves' is
-// exact where they are close. Decays below e^-104 are 0 in 32 bits; -10^4 stands for all of them.
+// The chunk's decays, by one warp, from each lane's gates (lane < 16: token lane's log decay and beta,
+// zero behind the chunk) and the chunk's resets. Running sums are kept as two floats, of which
+// differences lose nothing: the larger halves' is exact where they are close. Decays below e^-104 are
+// 0 in 32 bits; -10^4 stands for all of them.
+template <typename T, int NP> __device__ __forceinline__ void decays(Chunk<T, NP>& c, float g, float beta, unsigned marks) {
+  const int lane = threadIdx.x & 31;
+  double sum = fmaxf(g, -1e4f);
+#pragma unroll
+  for (int o = 1; o < kTile; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, sum, o, kTile);
+    if ((lane & 15) >= o) sum += x;
+  }
+  const double all = __shfl_sync(0xffffffffu, sum, 15);
+  if (lane < kTile) {
+    const float hi = static_cast<float>(sum);
+    c.g_hi[lane] = hi;
+    c.g_lo[lane] = static_cast<float>(sum - hi);
+    c.beta[lane] = beta;
+    c.head[lane] = marks & ((2u << lane) - 1u) ? 0.0f : exp2_hw(fmaf(hi, kLog2e, kExp2Shift));
+    c.tail[lane] = marks >> (lane + 1) ? 0.0f : exp2_hw(fmaf(static_cast<float>(all - sum), kLog2e, kExp2Shift));
+  }
+}
+
+// The chunk's matrices, by the same warp, from the tiles of K and Q; with kKeep into `wide` too.
 // The inverse goes by blocks of 8: [[A, 0], [C, B]]^-1 = [[A', 0], [-B' C A', B']], the blocks' own
 // column by column.
 template <typename T, int DK, bool kKeep, int NP>
-__device__ __forceinline__ void prepare(Chunk<T, NP>& c, Scratch& s, Wide* wide, const bf16* tk, const bf16* tq, float g, float beta,
-                                        float scale, int unit) {
+__device__ __forceinline__ void prepare(Chunk<T, NP>& c, Scratch& s, Wide* wide, const bf16* tk, const bf16* tq, unsigned marks, float scale,
+                                        int unit) {
   constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner;
   using Keys = Tile<T, DK>;
   const int lane = threadIdx.x & 31, row = lane >> 2, col = (lane & 3) * 2;
@@ -257,24 +339,13 @@ __device__ __forceinline__ void prepare(Chunk<T, NP>& c, Scratch& s, Wide* wide,
       c.rq[row + 8] = unit ? rsqrtf((odd ? qq[1][3] : qq[1][2]) + kNormEps) : 1.0f;
     }
   }
-  {
-    double sum = fmaxf(g, -1e4f);
-#pragma unroll
-    for (int o = 1; o < kTile; o <<= 1) {
-      const double x = __shfl_up_sync(0xffffffffu, sum, o, kTile);
-      if ((lane & 15) >= o) sum += x;
-    }
-    const double all = __shfl_sync(0xffffffffu, sum, 15);
-    if (lane < kTile) {
-      const float hi = static_cast<float>(sum);
-      c.g_hi[lane] = hi;
-      c.g_lo[lane] = static_cast<float>(sum - hi);
-      c.beta[lane] = beta;
-      c.head[lane] = exp2_hw(fmaf(hi, kLog2e, kExp2Shift));
-      c.tail[lane] = exp2_hw(fmaf(static_cast<float>(all - sum), kLog2e, kExp2Shift));
-    }
-  }
   __syncwarp();
+  if (lane < kTile) {
+    const float rk = c.rk[lane], head = c.head[lane];
+    c.head_k[lane] = head * rk;
+    c.head_q[lane] = scale * head * c.rq[lane];
+    c.tail_k[lane] = c.tail[lane] * rk;
+  }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int i = row + 8 * r;
@@ -290,9 +361,10 @@ __device__ __forceinline__ void prepare(Chunk<T, NP>& c, Scratch& s, Wide* wide,
         for (int e = 0; e < 2; ++e) {
           const float sum = (hi - (e ? hj.y : hj.x)) + (lo - (e ? lj.y : lj.x));
           const float dec = exp2_hw(fmaf(sum, kLog2e, kExp2Shift)), f = dec * (e ? rj.y : rj.x);
-          d[e] = i >= j + e ? dec : 0.0f;
-          x[e] = i > j + e ? kk[t][2 * r + e] * (f * rk) : 0.0f;
-          y[e] = i >= j + e ? qk[t][2 * r + e] * (f * rq) : 0.0f;
+          const bool one = i >= j + e && !(marks & ((2u << i) - 1u) & ~((2u << (j + e)) - 1u));          // episode
+          d[e] = one ? dec : 0.0f;
+          x[e] = one && i > j + e ? kk[t][2 * r + e] * (f * rk) : 0.0f;
+          y[e] = one ? qk[t][2 * r + e] * (f * rq) : 0.0f;
         }
       }
       const float2 bj = *reinterpret_cast<const float2*>(&c.beta[j]);
@@ -371,69 +443,33 @@ __device__ __forceinline__ Gate gate_of(float dt, float b, float bias, float rat
 // A[h]; -inf as the lowest finite number, so that a step of zero decays by e^0
 __device__ __forceinline__ float rate_at(const float* A, int h) { return fmaxf(A[h], -3.4028235e38f); }
 
-// The chunks of a row in order: a tile's begin at its first token and at each reset. All lanes of a
-// warp; the next tile's marks are on their way while one is taken.
-struct Chunks {
+// The resets of the tile at t (bit i: token t + i), as each lane's own flag, on its way until it is
+// asked for by all lanes of the warp.
+struct Marks {
   const uint8_t* reset;
-  int length, tile, t0, n;
-  bool fresh;
-  unsigned left, marks, coming;
-  __device__ __forceinline__ unsigned look(int t) const {                // this lane's mark of the tile at t
+  int length;
+  unsigned coming;
+  __device__ __forceinline__ void look(int t) {
     const int lane = threadIdx.x & 31;
-    return reset && lane < kTile && t + lane < length ? reset[t + lane] : 0u;
+    coming = reset && t >= 0 && lane < kTile && t + lane < length ? reset[t + lane] : 0u;
   }
-  __device__ __forceinline__ Chunks(const uint8_t* reset_, int length_) : reset(reset_), length(length_), tile(-kTile), t0(0), n(0), fresh(false), left(0) {
-    coming = look(0);
-  }
-  __device__ __forceinline__ bool next() {
-    if (!left) {
-      tile += kTile;
-      if (tile >= length) return false;
-      marks = __ballot_sync(0xffffffffu, coming != 0);
-      left = marks | 1u;
-      coming = look(tile + kTile);
-    }
-    const int at = __ffs(left) - 1;
-    left &= left - 1;
-    t0 = tile + at;
-    n = (left ? tile + __ffs(left) - 1 : min(tile + kTile, length)) - t0;
-    fresh = (marks >> at) & 1u;
-    return true;
-  }
+  __device__ __forceinline__ unsigned get() const { return __ballot_sync(0xffffffffu, coming != 0); }
 };
 
-// The same from the row's end.
-struct ChunksBack {
-  const uint8_t* reset;
-  int length, tile, t0, n, end;
-  bool fresh;
-  unsigned left, marks, coming;
-  __device__ __forceinline__ unsigned look(int t) const {
-    const int lane = threadIdx.x & 31;
-    return reset && t >= 0 && lane < kTile && t + lane < length ? reset[t + lane] : 0u;
+// Whether a warp's tile (rows of `pitch` elements, `width` of them, on 16-byte boundaries) holds a number
+// that is not finite: 0 times it is not 0.
+template <typename T> __device__ __forceinline__ bool not_finite(const T* tile, int pitch, int width, int n) {
+  constexpr int V = kVec16<T>;
+  const int lane = threadIdx.x & 31, per = width / V;
+  float bad = 0.0f;
+  for (int i = lane; i < n * per; i += 32) {
+    float v[V];
+    load_vec<T, V>(tile + i / per * pitch + i % per * V, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) bad = fmaf(v[j], 0.0f, bad);
   }
-  __device__ __forceinline__ ChunksBack(const uint8_t* reset_, int length_) : reset(reset_), length(length_), t0(0), n(0), fresh(false), left(0) {
-    tile = (length + kTile - 1) / kTile * kTile;
-    coming = look(tile - kTile);
-  }
-  __device__ __forceinline__ bool next() {
-    if (!left) {
-      tile -= kTile;
-      if (tile < 0) return false;
-      marks = __ballot_sync(0xffffffffu, coming != 0);
-      left = marks | 1u;
-      end = min(tile + kTile, length);
-      coming = look(tile - kTile);
-    }
-    const int at = 31 - __clz(left);
-    left ^= 1u << at;
-    t0 = tile + at;
-    n = end - t0;
-    end = t0;
-    fresh = (marks >> at) & 1u;
-    return true;
-  }
-};
+  return __any_sync(0xffffffffu, bad != 0.0f);
+}
 
 // ---- hardware barriers by number ----------------------------------------------------------
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }

@@ -40,7 +40,8 @@ template <typename T, int DK> struct Backward {
   struct Stage {
     Chunk<T, NI> c;
     Wide wide;
-    int t0, n, fresh;
+    int t0, n, more;                                   // more: the tile's next episode follows in this stage
+    unsigned marks;
     alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize], tdo[Values::kSize];
     alignas(16) T tv[kTile * kPitchV];
     alignas(16) float w[kValues][kMat];                // rows values, columns tokens
@@ -123,59 +124,86 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
     const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
     const T* v = static_cast<const T*>(a.v) + bi * a.v_b + h * a.v_h + vb;
     const T* dout = static_cast<const T*>(a.dout) + bi * a.do_b + h * a.do_h + vb;
-    ChunksBack walk(a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length);
-    for (int i = 0;; ++i) {
-      const bool more = walk.next();
-      const int at = i % kStages;
-      if (at != w) {
-        if (!more) return;
-        continue;
-      }
-      typename B::Stage& st = sh.stage[at];
-      if (i >= kStages) bar_sync(1 + kStages + at, kThreads - (kPrep - 1) * 32);
-      const int t0 = walk.t0, n = more ? walk.n : 0;
-      if (lane == 0) {
-        st.t0 = t0;
-        st.n = n;
-        st.fresh = walk.fresh;
-      }
-      if (!more) {
-        __syncwarp();
-        bar_arrive(1 + at, kThreads - (kPrep - 1) * 32);
-        return;
-      }
-      Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k, lane, 32);
-      Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k, lane, 32);
-      cp_async_commit();
-      Values::load(st.tdo, dout + t0 * a.do_t, a.do_t, n, mine, a.piece_v, lane, 32);
-      load_rows(st.tv, B::kPitchV, kTile, kValues, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
-      const float* saved = a.saved + (((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values + vb) * pitch;
+    const int count = (length + kTile - 1) / kTile, stage_threads = kThreads - (kPrep - 1) * 32;
+    Marks look{a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length, 0u};
+    look.look((count - 1 - w) * kTile);
+    for (int i = w; i < count; i += kStages) {
+      typename B::Stage& st = sh.stage[w];
+      const int tile = count - 1 - i, end = min(kTile, length - tile * kTile);
+      const unsigned marks = look.get();
+      look.look((tile - kStages) * kTile);
+      if (i >= kStages) bar_sync(1 + kStages + w, stage_threads);
+      const float* saved = a.saved + (((static_cast<int64_t>(bi) * tiles + tile) * a.heads + h) * a.values + vb) * pitch;
       const bool pieces = a.keys % 4 == 0;
-      load_rows(&st.w[0][0], kMat, kValues, kTile, saved + a.keys + t0 % kTile, pitch, mine, n, pieces && t0 % 4 == 0 && n % 4 == 0);
-      if (!walk.fresh) load_rows(&st.s[0][0], B::kPitchS, kValues, DK, saved, pitch, mine, a.keys, pieces);
-      cp_async_commit();
-      Gate e{};
-      if (lane < n) e = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
+      bool bad = false;
+      auto fetch = [&](int from, int n, unsigned mark) {
+        const int t0 = tile * kTile + from;
+        Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k == 16);
+        Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k == 16);
+        cp_async_commit();
+        Values::load(st.tdo, dout + t0 * a.do_t, a.do_t, n, mine, a.piece_v == 16);
+        load_rows(st.tv, B::kPitchV, kTile, kValues, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
+        load_rows(&st.w[0][0], kMat, kValues, kTile, saved + a.keys + from, pitch, mine, n, pieces && from % 4 == 0 && n % 4 == 0);
+        if (!(mark & 1u)) load_rows(&st.s[0][0], B::kPitchS, kValues, DK, saved, pitch, mine, a.keys, pieces);
+        cp_async_commit();
+        Gate e{};
+        if (lane < n) e = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
+        decays(st.c, e.g, e.beta, mark);
+        if (lane == 0) {
+          st.t0 = t0;
+          st.n = n;
+          st.marks = mark;
+          st.more = 0;
+        }
+        bad = __any_sync(0xffffffffu, fmaf(e.g, 0.0f, e.beta * 0.0f) != 0.0f);
+      };
+      auto ready = [&](unsigned mark) {
+        prepare<T, DK, true>(st.c, sh.scratch[w], &st.wide, st.tk, st.tq, mark, a.scale, a.unit);
+        cp_async_wait<0>();
+        __syncwarp();
+        bar_arrive(1 + w, stage_threads);
+      };
+      fetch(0, end, marks);
       cp_async_wait<1>();
       __syncwarp();
-      prepare<T, DK, true>(st.c, sh.scratch[w], &st.wide, st.tk, st.tq, e.g, e.beta, a.scale, a.unit);
-      cp_async_wait<0>();
-      __syncwarp();
-      bar_arrive(1 + at, kThreads - (kPrep - 1) * 32);
+      bool split = false;
+      if (marks & ~1u) {
+        cp_async_wait<0>();
+        __syncwarp();
+        split = bad || not_finite(st.tk, Keys::kPitch, DK, end) || not_finite(st.tq, Keys::kPitch, DK, end) ||
+                not_finite(st.tdo, Values::kPitch, kValues, end) || not_finite(st.tv, B::kPitchV, kValues, end) ||
+                not_finite(&st.w[0][0], kMat, kTile, mine);
+      }
+      if (!split) {
+        ready(marks);
+        continue;
+      }
+      for (int to = end; to > 0;) {                    // the last episode first
+        const int from = 31 - __clz((marks | 1u) & ((1u << to) - 1u));
+        if (to < end) bar_sync(1 + kStages + w, stage_threads);
+        fetch(from, to - from, (marks >> from) & 1u);
+        if (lane == 0) st.more = from > 0;
+        cp_async_wait<0>();
+        __syncwarp();
+        ready((marks >> from) & 1u);
+        to = from;
+      }
     }
+    return;
   }
 
-  const int stage_threads = kThreads - (kPrep - 1) * 32, team = (kMain + 1) * 32;
+  const int stage_threads = kThreads - (kPrep - 1) * 32, team = (kMain + 1) * 32, count = (length + kTile - 1) / kTile;
   if (warp == kMain + kPrep) {
     // the matrices and gates of 16 x 16
     const int64_t g_t = static_cast<int64_t>(a.heads) * splits, g_at = row0 * g_t + static_cast<int64_t>(h) * splits + blockIdx.y;
     double sum_a = 0.0, sum_bias = 0.0;
-    for (int i = 0;; ++i) {
-      const int at = i % kStages, turn = i & 1;
+    for (int i = 0, more = 0, turn = 0; i < count; i += more ? 0 : 1, turn ^= 1) {
+      const int at = i % kStages;
       typename B::Stage& st = sh.stage[at];
       bar_sync(1 + at, stage_threads);
       const int t0 = st.t0, n = st.n;
-      if (n == 0) break;
+      const unsigned marks = st.marks;
+      more = st.more;
       Gate gate{};
       if (lane < n) gate = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
       bar_sync(kBarChain, team);
@@ -205,12 +233,13 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int c = j + e;
-          const float dp = c <= r ? ow[e] * bt[e] : 0.0f, dm = c < r ? -zw[e] * bt[e] : 0.0f;
+          const bool one = d[e] != 0.0f;               // across a reset Z or W need not be finite
+          const float dp = one && c <= r ? ow[e] * bt[e] : 0.0f, dm = one && c < r ? -zw[e] * bt[e] : 0.0f;
           ep[e] = dp * p[e];
           em[e] = dm * m[e];
           pd[e] = a.scale * dp * d[e];
           md[e] = dm * d[e];
-          mz[e] = c < r ? m[e] * zw[e] : 0.0f;
+          mz[e] = one && c < r ? m[e] * zw[e] : 0.0f;
           row_p += ep[e];
           row_m += em[e];
           zr += c == r ? zw[e] : mz[e] * bt[e];
@@ -265,7 +294,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
       row_m = __shfl_sync(0xffffffffu, row_m, 2 * c);
       zr = __shfl_sync(0xffffffffu, zr, 2 * c);
       // the head's term of k, -Z.(head K S^T) = Z.R - Z.V
-      const float keep = st.fresh ? 0.0f : zr - zv;
+      const float keep = marks & ((2u << c) - 1u) ? 0.0f : zr - zv;
       if (lane < kTile) {
         sh.nq[c] = row_p;
         sh.nk[c] = keep + f + row_m + column;
@@ -274,7 +303,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
       float e = keep;
 #pragma unroll
       for (int x = 0; x < kMain; ++x) e += sh.by_key[turn][x][c];
-      float dg = st.c.head[kTile - 1] * inner;
+      float dg = marks ? 0.0f : st.c.head[kTile - 1] * inner;
 #pragma unroll
       for (int j = 0; j < kTile; ++j) {
         const float ej = __shfl_sync(0xffffffffu, e, j), fj = __shfl_sync(0xffffffffu, f, j);
@@ -342,14 +371,15 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
   }
   __syncwarp();
 
-  for (int i = 0;; ++i) {
-    const int at = i % kStages, turn = i & 1;
+  for (int i = 0, more = 0, turn = 0; i < count; i += more ? 0 : 1, turn ^= 1) {
+    const int at = i % kStages;
     typename B::Stage& st = sh.stage[at];
     const Chunk<T, NI>& c = st.c;
     bar_sync(1 + at, stage_threads);
     const int t0 = st.t0, n = st.n;
-    if (n == 0) break;
-    const bool fresh = st.fresh;
+    const unsigned marks = st.marks;
+    const bool fresh = marks & 1u;                     // no token sees S
+    more = st.more;
     if (by_v) {
       // K dS^T (rows values, columns tokens), <dS, S>; dS's planes to shared memory
       float ds[2][4] = {}, inner = 0.0f;
@@ -362,7 +392,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
         load_planes<NT, false>(b, ka + x * 32, Keys::kPlane * 2);
         mma_planes<NI, NT>(ds[0], ds[1], f.r, b);
         put_frag(sh.d, vl + row, 16 * x + col, f);
-        if (!fresh)
+        if (!marks)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -395,14 +425,40 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int tok = t * 8 + col + (e & 1);
-            ds[t][e] *= c.tail[tok] * c.rk[tok];
+            ds[t][e] = marks >> (tok + 1) ? 0.0f : ds[t][e] * c.tail_k[tok];
             du[t][e] += ds[t][e];
             x[t][e] = c.beta[tok] * du[t][e];
           }
         Frag<NI> f;
-        f.from(x[0], x[1]);
         load_planes<NI, true>(b, smem_of(c.inv) + at_cols(lane, kSide), kTile * kSide * 2);
-        mma_planes<NI, NI>(z[0], z[1], f.r, b);
+        // A gradient of the state that is not finite reaches the last episode's tokens alone: with
+        // others in the chunk, theirs is a sum without them.
+        float bad = 0.0f;
+        if (marks & ~1u) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad = fmaf(x[t][e], 0.0f, bad);
+        }
+        if (!__any_sync(0xffffffffu, bad != 0.0f)) {
+          f.from(x[0], x[1]);
+          mma_planes<NI, NI>(z[0], z[1], f.r, b);
+        } else {
+          for (int last = 0; last < 2; ++last) {
+            float y[2][4], to[2][4] = {};
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[t][e] = (marks >> (t * 8 + col + (e & 1) + 1) == 0) == (last != 0) ? x[t][e] : 0.0f;
+            f.from(y[0], y[1]);
+            mma_planes<NI, NI>(to[0], to[1], f.r, b);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if ((marks >> (t * 8 + col + (e & 1) + 1) == 0) == (last != 0)) z[t][e] = to[t][e];
+          }
+        }
         f.from(z[0], z[1]);
         put_frag(sh.z, vl + row, col, f);
         f.from(w[0], w[1]);
@@ -460,8 +516,8 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int tok = t * 8 + col + (e & 1), r = vl + row + (e >> 1) * 8;
-            z[t][e] *= -c.head[tok] * c.rk[tok];
-            x[t][e] = a.scale * c.head[tok] * c.rq[tok] * tile_at<T>(st.tdo, Values::kPlane, tok * Values::kPitch + r);
+            z[t][e] = marks & ((2u << tok) - 1u) ? 0.0f : -c.head_k[tok] * z[t][e];
+            x[t][e] = c.head_q[tok] * tile_at<T>(st.tdo, Values::kPlane, tok * Values::kPitch + r);
           }
         Frag<NI> fz, fo;
         fz.from(z[0], z[1]);
@@ -471,8 +527,8 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
         for (int y = 0; y < kSteps; ++y) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            d[2 * y][e] *= end;
-            d[2 * y + 1][e] *= end;
+            d[2 * y][e] = marks ? 0.0f : d[2 * y][e] * end;
+            d[2 * y + 1][e] = marks ? 0.0f : d[2 * y + 1][e] * end;
           }
           uint32_t b[NT][4];
           load_planes<NT, true>(b, kt + y * 32, Keys::kPlane * 2);
@@ -524,8 +580,9 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int tok = row + (e >> 1) * 8;
-            aq[p][t][e] *= a.scale * c.head[tok];
-            ak[p][t][e] = fmaf(c.tail[tok] * c.beta[tok], as[p][t][e], -c.head[tok] * ak[p][t][e]);
+            const bool seen = !(marks & ((2u << tok) - 1u)), sent = !(marks >> (tok + 1));
+            aq[p][t][e] = seen ? a.scale * c.head[tok] * aq[p][t][e] : 0.0f;
+            ak[p][t][e] = (seen ? -c.head[tok] * ak[p][t][e] : 0.0f) + (sent ? c.tail[tok] * c.beta[tok] * as[p][t][e] : 0.0f);
             e0[e >> 1] = fmaf(aq[p][t][e], tile_at<T>(st.tq, Keys::kPlane, tok * Keys::kPitch + c0 + 16 * p + t * 8 + col + (e & 1)), e0[e >> 1]);
           }
 #pragma unroll

@@ -28,7 +28,6 @@ _lib.register(DLIB, {"surf_group_norm": (_I, [c_char_p, _I, _I, _I, _I, _I, _I, 
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
 LANES, BLOCK, PARTS = 0, 1, 2
-_HOLD = 4                                       # pieces that a lane keeps
 _ARGS = struct.Struct("9q8q2if3iq")
 
 Norm = namedtuple("Norm", "out stats")
@@ -83,45 +82,36 @@ def _pow2(n: int) -> int:
 
 
 def _plan(n: int, p: int, c: int, g: int, e: int, v: int, grad: bool):
-    """(form, lanes, threads, blocks, bytes of shared memory, groups of a slab, parts, positions of
-    a part)."""
+    """(form, lanes of a group, pieces that a lane or thread holds, threads, blocks along the samples,
+    groups of a slab, parts, positions of a part)."""
     cg = c // g
     per_group = cg // v
     items = p * per_group
-    if items <= 32 * _HOLD:
+    if items <= 128:
         lanes = min(32, _pow2(items))
-        sets = -(-g // (32 // lanes))
-        blocks = min(-(-n // 8), max(1, 148 * (4 if grad else 16) // sets), 65535)
-        return LANES, lanes, 256, blocks, 0, 1, 1, p
-    copies = 2 if grad else 1
-    most = 200 * 1024 // copies                 # bytes of a slab that a block keeps
-    # whole groups: rows of 64 bytes or more where they fit, as wide as leaves two slabs for an SM
-    slab = 0
-    for k in range(1, g + 1):
-        if g % k or k * per_group > 256 or (per_group > 256 and (grad or k > 1)):
-            continue
-        rows = 256 // (k * per_group)
-        size = -(-p // max(1, rows)) * max(1, rows) * k * cg * e if k * per_group <= 256 else p * cg * e + 256 * v * e
-        if size > most:
-            break
-        if slab and k * cg * e > 64 and n * (g // k) < 296:
-            break
-        slab, need = k, size
-    if not slab and per_group > 256 and not grad and p * cg * e + 256 * v * e <= most:
-        slab, need = 1, p * cg * e + 256 * v * e
+        hold = _pow2(-(-items // lanes))
+        blocks = min(-(-n // 8), max(1, 148 * (6 if grad else 24) // -(-g // (32 // lanes))), 65535)
+        return LANES, lanes, hold, 256, blocks, 1, 1, p
+    # the narrowest slab of whole groups with rows of 32 bytes (a sector) that a block's registers
+    # take, twice as wide where that still leaves three for every SM
+    threads, most = (256, 4) if grad else (512, 8)
+    fits = [k for k in range(1, g + 1) if g % k == 0 and k * per_group <= threads and
+            -(-p // (threads // (k * per_group))) <= most]
+    slab = next((k for k in fits if k * cg * e >= 32), fits[-1] if fits else 0)
+    slab = next((k for k in fits if k >= 2 * slab and n * (g // k) >= 148 * 3), slab)
     if slab and n * (g // slab) >= 74:
-        threads = 256 if slab == 1 else -(-(slab * per_group) * (256 // (slab * per_group)) // 32) * 32
-        blocks = min(n, max(1, -(-148 * 6 // (g // slab)))) if grad else n
-        return BLOCK, 0, threads, blocks, need * copies, slab, 1, p
-    slab = 1
-    for k in range(1, g + 1):
-        if g % k == 0 and k * per_group <= 256:
-            slab = k
-    slabs = g // slab if not grad else -(-(c // v) // 32)
-    parts = max(1, min(-(-148 * 4 // max(1, n * slabs)), -(-p // 16)))
+        per = slab * per_group
+        hold = -(-p // (threads // per))
+        # no more threads than the pieces take
+        threads = -(-min(threads // per, -(-p // hold)) * per // 32) * 32
+        hold = max(2, _pow2(-(-p // (threads // per))))
+        return BLOCK, 0, hold, threads, min(n, max(1, 148 * 4 // (g // slab))) if grad else n, slab, 1, p
+    threads = 256
+    slab = max((k for k in range(1, g + 1) if g % k == 0 and k * per_group <= threads), default=1)
+    slabs = -(-(c // v) // 32) if grad else g // slab
+    parts = max(1, min(-(-148 * 3 // max(1, n * slabs)), -(-p // 16)))
     span = -(-p // parts)
-    threads = 256 if slab == 1 else -(-(slab * per_group) * (256 // (slab * per_group)) // 32) * 32
-    return PARTS, 0, threads, 0, 0, slab, -(-p // span), span
+    return PARTS, 0, 0, threads, 0, slab, -(-p // span), span
 
 
 def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
@@ -144,11 +134,11 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     if n == 0 or p == 0:
         return Norm(out, stats)
     v = _piece(c // g, e, _bits(e, x, out))
-    mode, lanes, threads, blocks, smem, slab, parts, span = _plan(n, p, c, g, e, v, False)
+    mode, lanes, hold, threads, blocks, slab, parts, span = _plan(n, p, c, g, e, v, False)
     part = torch.empty(n * g * parts * 3, dtype=torch.float32, device=x.device) if mode == PARTS else None
     args = _ARGS.pack(x.data_ptr(), 0, _p(weight), _p(bias), out.data_ptr(), _p(stats), _p(part), 0, 0,
                       xn, xp, 0, 0, yn, yp, n, p, c, g, eps, ACTIVATIONS[activation], slab, parts, span)
-    launch(_lib.lib(DLIB).surf_group_norm, "surf_group_norm", at, args, code, 0, v, mode, lanes, threads, blocks, smem)
+    launch(_lib.lib(DLIB).surf_group_norm, "surf_group_norm", at, args, code, 0, v, mode, lanes, hold, threads, blocks)
     if mode == PARTS:
         _lib.add_launches(1)
     return Norm(out, stats)
@@ -173,12 +163,12 @@ def group_norm_grad(dy: torch.Tensor, x: torch.Tensor, groups: int, weight: Opti
     if n == 0 or p == 0:
         return NormGrads(dx, None if dw is None else dw.zero_(), None if db is None else db.zero_())
     v = _piece(c // g, e, _bits(e, x, dy, dx))
-    mode, lanes, threads, blocks, smem, slab, parts, span = _plan(n, p, c, g, e, v, True)
+    mode, lanes, hold, threads, blocks, slab, parts, span = _plan(n, p, c, g, e, v, True)
     rows = n * parts if mode == PARTS else blocks
     part = torch.empty(rows * 2 * c + (n * g * 2 if mode == PARTS else 0), dtype=torch.float32, device=x.device)
     args = _ARGS.pack(x.data_ptr(), dy.data_ptr(), _p(weight), _p(bias), dx.data_ptr(), stats.data_ptr(), part.data_ptr(),
                       _p(dw), _p(db), xn, xp, dn, dp, yn, yp, n, p, c, g, 0.0, ACTIVATIONS[activation], slab, parts, span)
-    launch(_lib.lib(DLIB).surf_group_norm, "surf_group_norm", at, args, code, 1, v, mode, lanes, threads, blocks, smem)
+    launch(_lib.lib(DLIB).surf_group_norm, "surf_group_norm", at, args, code, 1, v, mode, lanes, hold, threads, blocks)
     _lib.add_launches((2 if mode == PARTS else 0) + (dw is not None or db is not None))
     return NormGrads(dx, dw, db)
 
