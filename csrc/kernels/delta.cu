@@ -7,13 +7,14 @@ namespace {
 using namespace delta;
 
 // ---- sequences --------------------------------------------------------------------------
-constexpr int kPrep = 2, kMain = 4;                    // warps that make chunks ready, that carry them out at most
+constexpr int kMain = 4;                               // warps that carry chunks out at most
+constexpr int kPrep = 2;                               // warps that make chunks ready
 
 template <typename T, int DK> struct Forward {
   // chunks ready, in the making or on their way
-  static constexpr int kStages = 4;
+  static constexpr int kStages = (sizeof(T) == 4 && DK == 128 ? 2 : 3) * kPrep;
   using Keys = Tile<T, DK>;
-  static_assert(kStages % kPrep == 0, "a stage's barriers are one warp's");
+  static_assert(kStages % kPrep == 0 && kStages >= 2 * kPrep, "a stage is one warp's, and its next one another");
   struct Stage {
     Chunk<T, Planes<T>::kShort> c;
     int t0, n, more;                                   // more: the tile's next episode follows in this stage
@@ -60,14 +61,14 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
     const float rate = rate_at(a.A, h), bias = a.bias ? a.bias[h] : 0.0f;
     const int tiles = (length + kTile - 1) / kTile;
     Marks look{a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length, 0u};
-    // Tokens [t0, t0 + n) on their way to a stage; their decays are made meanwhile.
-    auto fetch = [&](typename F::Stage& st, T* tv, int t0, int n, unsigned marks) {
+    // Tokens [t0, t0 + n) on their way to a stage; their decays are made meanwhile, from this lane's token.
+    auto fetch = [&](typename F::Stage& st, T* tv, int t0, int n, unsigned marks, float raw_dt, float raw_b) {
       Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k == 16);
       Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k == 16);
       load_rows(tv, pitch_v, kTile, warps * 16, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
       cp_async_commit();
       Gate e{};
-      if (lane < n) e = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
+      if (lane < n) e = gate_of(raw_dt, raw_b, bias, rate);
       decays(st.c, e.g, e.beta, marks);
       if (lane == 0) {
         st.t0 = t0;
@@ -77,16 +78,26 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
       }
       return __any_sync(0xffffffffu, fmaf(e.g, 0.0f, e.beta * 0.0f) != 0.0f);
     };
+    // resets and gates a tile of this warp's ahead of the rest
+    T raw_dt = from_f<T>(0.0f), raw_b = raw_dt;
+    auto ahead = [&](int i) {
+      look.look(i * kTile);
+      if (lane < kTile && i * kTile + lane < length) {
+        raw_dt = dt[(i * kTile + lane) * a.dt_t];
+        raw_b = gb[(i * kTile + lane) * a.b_t];
+      }
+    };
     bool bad_here = false, bad_next = false;
     unsigned marks_here = 0, marks_next = 0;
     auto begin = [&](int i) {
       const int at = i % kStages;
       if (i >= kStages) bar_sync(1 + kStages + at, threads);
       marks_next = look.get();
-      look.look((i + kPrep) * kTile);
-      bad_next = fetch(sh.stage[at], values + at * kTile * pitch_v, i * kTile, min(kTile, length - i * kTile), marks_next);
+      const float x = to_f(raw_dt), y = to_f(raw_b);
+      ahead(i + kPrep);
+      bad_next = fetch(sh.stage[at], values + at * kTile * pitch_v, i * kTile, min(kTile, length - i * kTile), marks_next, x, y);
     };
-    look.look(w * kTile);
+    ahead(w);
     if (w < tiles) begin(w);
     for (int i = w; i < tiles; i += kPrep) {
       const int at = i % kStages, t0 = i * kTile, n = min(kTile, length - t0);
@@ -113,7 +124,10 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
         left &= left - 1;
         const unsigned mark = (marks_here >> from) & 1u;
         if (from > 0) bar_sync(1 + kStages + at, threads);
-        fetch(st, tv, t0 + from, (left ? __ffs(left) - 1 : n) - from, mark);
+        const int to = left ? __ffs(left) - 1 : n;
+        const bool on = from + lane < to;
+        fetch(st, tv, t0 + from, to - from, mark, on ? to_f(dt[(t0 + from + lane) * a.dt_t]) : 0.0f,
+              on ? to_f(gb[(t0 + from + lane) * a.b_t]) : 0.0f);
         if (lane == 0) st.more = left != 0;
         cp_async_wait<0>();
         __syncwarp();
@@ -125,6 +139,7 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
 
   const int row = lane >> 2, col = (lane & 3) * 2, vl = warp * 16, v0 = vb + vl;
   T* out = static_cast<T*>(a.out) + bi * a.o_b + h * a.o_h;
+  T* out_row = out + lane / (16 / kVec16<T>) * a.o_t + v0 + lane % (16 / kVec16<T>) * kVec16<T>;       // this lane's first piece
   T* so = values + kStages * kTile * pitch_v + warp * kTile * F::kRow;
   const int64_t head_size = static_cast<int64_t>(a.values) * a.keys;
   const int64_t head_at = (static_cast<int64_t>(bi) * a.heads + h) * head_size;
@@ -181,85 +196,76 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
     auto pair = [&](const float (&x)[kTile], int t) { return *reinterpret_cast<const float2*>(&x[8 * t + col]); };
     // whether the state before the chunk reaches a token
     auto seen = [&](int tok) { return !(marks & ((2u << tok) - 1u)); };
-    // A state that is not finite ends with its episode: with another one in the chunk the tokens behind
-    // the reset are taken once more, without it (it is not needed any longer then).
-    bool again = false;
-    if (marks & ~1u) {
-      float bad = 0.0f;
-      each([&](float x, float y, int, int) { bad = fmaf(x, 0.0f, fmaf(y, 0.0f, bad)); });
-      again = __any_sync(0xffffffffu, bad != 0.0f);
-    }
-    float sq[2][4], w[2][4];
-    auto outputs = [&] {
-      // K S^T and Q S^T, transposed: rows values, columns tokens
-      float sk[2][4] = {};
+    // K S^T and Q S^T, transposed: rows values, columns tokens
+    float sk[2][4] = {}, sq[2][4] = {}, w[2][4] = {};
+    const uint32_t ka = smem_of(st.tk) + at_rows(lane, Keys::kPitch), qa = smem_of(st.tq) + at_rows(lane, Keys::kPitch);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sq[t][e] = w[t][e] = 0.0f;
-      const uint32_t ka = smem_of(st.tk) + at_rows(lane, Keys::kPitch), qa = smem_of(st.tq) + at_rows(lane, Keys::kPitch);
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        Frag<NI> f;
-        f.from(s[2 * i], s[2 * i + 1]);
-        uint32_t bk[NT][4], bq[NT][4];
-        load_planes<NT, false>(bk, ka + i * 32, Keys::kPlane * 2);
-        load_planes<NT, false>(bq, qa + i * 32, Keys::kPlane * 2);
-        mma_planes2<NI, NS>(sk[0], sk[1], sq[0], sq[1], f.r, bk, bq);
-      }
-      if (marks)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!seen(8 * t + col + (e & 1))) sk[t][e] = sq[t][e] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float2 hk = pair(c.head_k, t), hq = pair(c.head_q, t);
-        const T* from = tv + (8 * t + col) * pitch_v + vl + row;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sk[t][e] = fmaf(-(e & 1 ? hk.y : hk.x), sk[t][e], to_f(from[(e & 1) * pitch_v + (e >> 1) * 8]));
-          sq[t][e] *= e & 1 ? hq.y : hq.x;
-        }
-      }
+    for (int i = 0; i < kSteps; ++i) {
       Frag<NI> f;
-      f.from(sk[0], sk[1]);
-      uint32_t b[NI][4];
-      load_planes<NI, false>(b, smem_of(c.inv) + at_rows(lane, kSide), kTile * kSide * 2);
-      mma_planes<NI, NI>(w[0], w[1], f.r, b);
-      float u[2][4];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float2 beta = pair(c.beta, t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) u[t][e] = w[t][e] * (e & 1 ? beta.y : beta.x);
-      }
-      Frag<NS> g;
-      g.from(u[0], u[1]);
-      uint32_t p[NS][4];
-      load_planes<NS, false>(p, smem_of(c.p) + at_rows(lane, kSide), kTile * kSide * 2);
-      mma_planes<NS, NS>(sq[0], sq[1], g.r, p);
-    };
-    outputs();
-    if (again) {
-      float o0[2][4], w0[2][4];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o0[t][e] = sq[t][e];
-          w0[t][e] = w[t][e];
-        }
-      each([&](float& x, float& y, int, int) { x = y = 0.0f; });
-      outputs();
+      f.from(s[2 * i], s[2 * i + 1]);
+      uint32_t bk[NT][4], bq[NT][4];
+      load_planes<NT, false>(bk, ka + i * 32, Keys::kPlane * 2);
+      load_planes<NT, false>(bq, qa + i * 32, Keys::kPlane * 2);
+      mma_planes2<NI, NS>(sk[0], sk[1], sq[0], sq[1], f.r, bk, bq);
+    }
+    if (marks)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (seen(8 * t + col + (e & 1))) {
-            sq[t][e] = o0[t][e];
-            w[t][e] = w0[t][e];
+          if (!seen(8 * t + col + (e & 1))) sk[t][e] = sq[t][e] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float2 hk = pair(c.head_k, t), hq = pair(c.head_q, t);
+      const T* from = tv + (8 * t + col) * pitch_v + vl + row;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sk[t][e] = fmaf(-(e & 1 ? hk.y : hk.x), sk[t][e], to_f(from[(e & 1) * pitch_v + (e >> 1) * 8]));
+        sq[t][e] *= e & 1 ? hq.y : hq.x;
+      }
+    }
+    // W and P U. A state that is not finite reaches the first episode's tokens alone: with others in
+    // the chunk, theirs are sums without them.
+    bool apart = false;
+    if (marks & ~1u) {
+      float bad = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad = fmaf(sk[t][e], 0.0f, bad);
+      apart = __any_sync(0xffffffffu, bad != 0.0f);
+    }
+#pragma unroll 1
+    for (int part = 0; part < (apart ? 2 : 1); ++part) {
+      auto ours = [&](int tok) { return seen(tok) == (part != 0); };
+      float r[2][4], x[2][4] = {}, y[2][4] = {};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[t][e] = apart && !ours(8 * t + col + (e & 1)) ? 0.0f : sk[t][e];
+      Frag<NI> f;
+      f.from(r[0], r[1]);
+      uint32_t b[NI][4];
+      load_planes<NI, false>(b, smem_of(c.inv) + at_rows(lane, kSide), kTile * kSide * 2);
+      mma_planes<NI, NI>(x[0], x[1], f.r, b);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float2 beta = pair(c.beta, t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[t][e] = x[t][e] * (e & 1 ? beta.y : beta.x);
+      }
+      Frag<NS> g;
+      g.from(r[0], r[1]);
+      uint32_t p[NS][4];
+      load_planes<NS, false>(p, smem_of(c.p) + at_rows(lane, kSide), kTile * kSide * 2);
+      mma_planes<NS, NS>(y[0], y[1], g.r, p);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!apart || ours(8 * t + col + (e & 1))) {
+            w[t][e] = x[t][e];
+            sq[t][e] += y[t][e];
           }
     }
     if (saved) {
@@ -305,17 +311,17 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
 #pragma unroll
       for (int e = 0; e < 4; ++e) so[(t * 8 + col + (e & 1)) * F::kRow + row + (e >> 1) * 8] = from_f<T>(sq[t][e]);
     __syncwarp();
-    T* to = out + t0 * a.o_t + v0;
+    T* to = out_row + t0 * a.o_t;
     if (a.piece_v == 16) {
-      constexpr int V = kVec16<T>;
-      for (int j = lane; j < n * (16 / V); j += 32) {
-        const int r = j / (16 / V), cc = j % (16 / V) * V;
-        if (v0 + cc < a.values) *reinterpret_cast<uint4*>(to + r * a.o_t + cc) = *reinterpret_cast<const uint4*>(so + r * F::kRow + cc);
-      }
+      constexpr int V = kVec16<T>, kPer = 16 / V, kRows = 32 / kPer;
+#pragma unroll
+      for (int r = 0; r < kTile; r += kRows)
+        if (r + lane / kPer < n && lane % kPer * V < a.values - v0)
+          *reinterpret_cast<uint4*>(to + r * a.o_t) = *reinterpret_cast<const uint4*>(so + (r + lane / kPer) * F::kRow + lane % kPer * V);
     } else {
       for (int j = lane; j < n * 16; j += 32) {
         const int r = j / 16, cc = j % 16;
-        if (v0 + cc < a.values) to[r * a.o_t + cc] = so[r * F::kRow + cc];
+        if (v0 + cc < a.values) out[(t0 + r) * a.o_t + v0 + cc] = so[r * F::kRow + cc];
       }
     }
     __syncwarp();
@@ -328,7 +334,7 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
 
 template <typename T, int DK> int forward(const DeltaArgs& a, cudaStream_t s) {
   using F = Forward<T, DK>;
-  constexpr int kBlocks = sizeof(T) == 4 ? (DK == 128 ? 1 : 2) : DK == 128 ? 2 : 3;
+  constexpr int kBlocks = sizeof(T) == 4 && DK == 128 ? 1 : 2;
   if (const int e = allow_smem<delta_forward<T, DK, kBlocks>>(F::bytes(kMain))) return e;
   // values of a block: as many as it takes, or fewer where that leaves SMs without one
   const int all = (a.values + 15) / 16;

@@ -73,14 +73,13 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x, y -> their planes, packed. What a plane leaves comes from one subtraction of mixed types a number
-// (with its sign turned: the next plane's number is turned back by its own).
+// x, y -> their planes, packed. What a plane leaves is one multiply-add of mixed types a number.
 template <int N> __device__ __forceinline__ void split2(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     p[i] = surfk::pack_bf16x2(x, y);
     if (i + 1 < N)
-      asm("{.reg .b16 lo, hi;\n mov.b32 {lo, hi}, %2;\n sub.f32.bf16 %0, lo, %0;\n sub.f32.bf16 %1, hi, %1;\n neg.f32 %0, %0;\n neg.f32 %1, %1;}"
+      asm("{.reg .b16 lo, hi, m;\n mov.b16 m, 0xbf80;\n mov.b32 {lo, hi}, %2;\n fma.rn.f32.bf16 %0, lo, m, %0;\n fma.rn.f32.bf16 %1, hi, m, %1;}"
           : "+f"(x), "+f"(y) : "r"(p[i]));
   }
 }

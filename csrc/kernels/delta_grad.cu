@@ -25,45 +25,48 @@ using namespace delta;
 
 constexpr int kPrep = 2, kMain = 4, kValues = 64;      // warps of each kind (and one more); values of a block
 constexpr int kThreads = (kPrep + kMain + 1) * 32;
-// barriers: stage s ready (1 + s), stage s free (1 + kStages + s), the chain's results, the matrices
-enum : int { kBarChain = 14, kBarMatrices = 15 };
+// barriers: stage s ready (1 + s), stage s free (1 + kStages + s), S free for the warp of stage s (8 + s),
+// the chain's results, the matrices
+enum : int { kBarState = 8, kBarChain = 14, kBarMatrices = 15 };
 
 template <typename T, int DK> struct Backward {
   static constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort;
-  // a stage for each warp that makes chunks ready, so that its barriers are that warp's alone; where
-  // two do not fit, one warp and one stage
-  static constexpr int kStages = DK == 128 && sizeof(T) == 4 ? 1 : kPrep;
+  static constexpr int kStages = kPrep;                // one for each warp that makes chunks ready: its barriers are that warp's alone
   using Keys = Tile<T, DK>;
   using Values = Tile<T, kValues>;
   static constexpr int kPitchS = DK + 4, kPitchD = DK + 8, kPitchV = kValues + 16 / static_cast<int>(sizeof(T));
   static constexpr int kColumns = DK / kMain < 16 ? 16 : DK / kMain;     // of a warp by keys
   struct Stage {
     Chunk<T, NI> c;
-    Wide wide;
+    Wide wide;                                         // in the end E's parts of P and M, and M Z W^T
     int t0, n, more;                                   // more: the tile's next episode follows in this stage
     unsigned marks;
     alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize], tdo[Values::kSize];
     alignas(16) T tv[kTile * kPitchV];
-    alignas(16) float w[kValues][kMat];                // rows values, columns tokens
-    alignas(16) float s[kValues][kPitchS];
   };
   struct Shared {
     Stage stage[kStages];
-    alignas(16) Scratch scratch[kPrep];
-    alignas(16) bf16 w[NI][kValues][kSide], z[NI][kValues][kSide];
+    // the forward pass's S and W (rows values, columns tokens), one chunk's: two blocks fit on an SM then
+    alignas(16) float s[kValues][kPitchS];
+    alignas(16) float saved_w[kValues][kMat];
+    alignas(16) Scratch scratch[kStages];
+    alignas(16) bf16 w[NI][kValues][kTile], z[NI][kValues][kTile];       // rows values, columns tokens; see swap8
     alignas(16) bf16 d[NS][kValues][kPitchD];          // dS
     alignas(16) bf16 x1[NS][kTile][kSide], x2[NS][kTile][kSide], x3[NS][kTile][kSide];
-    // of each warp, for chunks in turn: Z W^T and dO W^T, sums over its values: W.dU, Z.V, the tails' terms
-    alignas(16) float part[2][kMain][2][kTile][kMat];
-    float by_value[2][kMain][3][kTile], inner[2][kMain];
-    float by_key[2][kMain][kTile];                     // the heads' terms of q
+    // of each warp: Z W^T and dO W^T, or its outputs
+    alignas(16) union { float product[2][kTile][kMat]; T out[kTile][16 + 16 / sizeof(T)]; } part[kMain];
+    float by_value[kMain][3][kTile], inner[kMain];     // sums over its values: W.dU, Z.V, the tails' terms; <dS, S>
+    float by_key[kMain][kTile];                        // the heads' terms of q
     float nq[kTile], nk[kTile];                        // q.dq and k.dk but for those
-    alignas(16) float e[3][kTile][kMat];
-    alignas(16) T out[kMain][kTile][16 + 16 / sizeof(T)];
   };
   static constexpr size_t kBytes = sizeof(Shared);
   static_assert(kBytes <= 227 * 1024, "a block's shared memory");
+  static constexpr int kBlocks = kBytes <= 113 * 1024 ? 2 : 1;
 };
+
+// Rows of 16 tokens lie 32 bytes apart, their halves swapped in every other four rows: eight rows of
+// 16 bytes, as ldmatrix reads them, are in all banks.
+__device__ __forceinline__ int swap8(int row, int token) { return token ^ ((row & 4) << 1); }
 
 __device__ __forceinline__ float quad_sum(float v) {   // over a row's four lanes
   v += __shfl_xor_sync(0xffffffffu, v, 1);
@@ -84,6 +87,24 @@ template <int N, int NF, int R, int P> __device__ __forceinline__ void put_frag(
 #pragma unroll
     for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(&m[n][i + (e & 1) * 8][j + (e >> 1) * 8]) = f.r[n][e];
 }
+template <int N, int NF, int R> __device__ __forceinline__ void put_tokens(bf16 (&m)[N][R][kTile], int i, int j, const Frag<NF>& f) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = i + (e & 1) * 8;
+      *reinterpret_cast<uint32_t*>(&m[n][r][swap8(r, j + (e >> 1) * 8)]) = f.r[n][e];
+    }
+}
+// Addresses of ldmatrix in such rows, of a left operand's columns (a_cols) and a right one's (at_cols).
+__device__ __forceinline__ uint32_t tokens_a(int lane) {
+  const int r = ((lane & 16) >> 1) + (lane & 7);
+  return (r * kTile + swap8(r, lane & 8)) * 2;
+}
+__device__ __forceinline__ uint32_t tokens_b(int lane) {
+  const int r = lane & 15;
+  return (r * kTile + swap8(r, (lane & 16) >> 1)) * 2;
+}
 // A warp's 16 x 16 of `out` (rows tokens) to the first n rows of memory, `cols` of its columns.
 template <typename T, int P>
 __device__ __forceinline__ void put_rows(T* to, int64_t stride, const T (&out)[kTile][P], int n, int cols, bool pieces) {
@@ -100,7 +121,7 @@ __device__ __forceinline__ void put_rows(T* to, int64_t stride, const T (&out)[k
   }
 }
 
-template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_backward(DeltaArgs a) {
+template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backward<T, DK>::kBlocks) delta_backward(DeltaArgs a) {
   using B = Backward<T, DK>;
   constexpr int NT = B::NT, NI = B::NI, NS = B::NS, kSteps = DK / 16, kStages = B::kStages;
   using Keys = typename B::Keys;
@@ -119,35 +140,41 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
 
   if (warp >= kMain && warp < kMain + kPrep) {
     const int w = warp - kMain, pitch = a.keys + kTile;
-    if (w >= kStages) return;
     const T* q = static_cast<const T*>(a.q) + bi * a.q_b + gr * a.q_g;
     const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
     const T* v = static_cast<const T*>(a.v) + bi * a.v_b + h * a.v_h + vb;
     const T* dout = static_cast<const T*>(a.dout) + bi * a.do_b + h * a.do_h + vb;
     const int count = (length + kTile - 1) / kTile, stage_threads = kThreads - (kPrep - 1) * 32;
     Marks look{a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length, 0u};
-    look.look((count - 1 - w) * kTile);
+    // resets and gates a tile of this warp's ahead of the rest
+    T raw_dt = from_f<T>(0.0f), raw_b = raw_dt;
+    auto ahead = [&](int tile) {
+      look.look(tile * kTile);
+      if (tile >= 0 && lane < kTile && tile * kTile + lane < length) {
+        raw_dt = dt[(tile * kTile + lane) * a.dt_t];
+        raw_b = gb[(tile * kTile + lane) * a.b_t];
+      }
+    };
+    ahead(count - 1 - w);
     for (int i = w; i < count; i += kStages) {
       typename B::Stage& st = sh.stage[w];
       const int tile = count - 1 - i, end = min(kTile, length - tile * kTile);
       const unsigned marks = look.get();
-      look.look((tile - kStages) * kTile);
+      const float now_dt = to_f(raw_dt), now_b = to_f(raw_b);
+      ahead(tile - kStages);
       if (i >= kStages) bar_sync(1 + kStages + w, stage_threads);
       const float* saved = a.saved + (((static_cast<int64_t>(bi) * tiles + tile) * a.heads + h) * a.values + vb) * pitch;
       const bool pieces = a.keys % 4 == 0;
       bool bad = false;
-      auto fetch = [&](int from, int n, unsigned mark) {
+      auto fetch = [&](int from, int n, unsigned mark, float x, float y) {
         const int t0 = tile * kTile + from;
         Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k == 16);
         Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k == 16);
-        cp_async_commit();
         Values::load(st.tdo, dout + t0 * a.do_t, a.do_t, n, mine, a.piece_v == 16);
         load_rows(st.tv, B::kPitchV, kTile, kValues, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
-        load_rows(&st.w[0][0], kMat, kValues, kTile, saved + a.keys + from, pitch, mine, n, pieces && from % 4 == 0 && n % 4 == 0);
-        if (!(mark & 1u)) load_rows(&st.s[0][0], B::kPitchS, kValues, DK, saved, pitch, mine, a.keys, pieces);
         cp_async_commit();
         Gate e{};
-        if (lane < n) e = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
+        if (lane < n) e = gate_of(x, y, bias, rate);
         decays(st.c, e.g, e.beta, mark);
         if (lane == 0) {
           st.t0 = t0;
@@ -156,36 +183,42 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
           st.more = 0;
         }
         bad = __any_sync(0xffffffffu, fmaf(e.g, 0.0f, e.beta * 0.0f) != 0.0f);
+        cp_async_wait<0>();
+        __syncwarp();
       };
-      auto ready = [&](unsigned mark) {
+      // matrices, then S and W as soon as the chunk before is done with its own
+      auto ready = [&](int from, int n, unsigned mark, bool first) {
         prepare<T, DK, true>(st.c, sh.scratch[w], &st.wide, st.tk, st.tq, mark, a.scale, a.unit);
+        if (!first) bar_sync(kBarState + w, (kMain + 1) * 32);
+        load_rows(&sh.saved_w[0][0], kMat, kValues, kTile, saved + a.keys + from, pitch, mine, n, pieces && from % 4 == 0 && n % 4 == 0);
+        if (!(mark & 1u)) load_rows(&sh.s[0][0], B::kPitchS, kValues, DK, saved, pitch, mine, a.keys, pieces);
+        cp_async_commit();
         cp_async_wait<0>();
         __syncwarp();
         bar_arrive(1 + w, stage_threads);
       };
-      fetch(0, end, marks);
-      cp_async_wait<1>();
-      __syncwarp();
+      fetch(0, end, marks, now_dt, now_b);
       bool split = false;
       if (marks & ~1u) {
-        cp_async_wait<0>();
-        __syncwarp();
-        split = bad || not_finite(st.tk, Keys::kPitch, DK, end) || not_finite(st.tq, Keys::kPitch, DK, end) ||
-                not_finite(st.tdo, Values::kPitch, kValues, end) || not_finite(st.tv, B::kPitchV, kValues, end) ||
-                not_finite(&st.w[0][0], kMat, kTile, mine);
+        float w_bad = 0.0f;                            // W is looked at where it lies: its place here is still in use
+        for (int x = lane; x < mine * end; x += 32) w_bad = fmaf(saved[x / end * pitch + a.keys + x % end], 0.0f, w_bad);
+        split = bad || __any_sync(0xffffffffu, w_bad != 0.0f) || not_finite(st.tk, Keys::kPitch, DK, end) ||
+                not_finite(st.tq, Keys::kPitch, DK, end) || not_finite(st.tdo, Values::kPitch, kValues, end) ||
+                not_finite(st.tv, B::kPitchV, kValues, end);
       }
       if (!split) {
-        ready(marks);
+        ready(0, end, marks, i == 0);
         continue;
       }
       for (int to = end; to > 0;) {                    // the last episode first
         const int from = 31 - __clz((marks | 1u) & ((1u << to) - 1u));
+        const unsigned mark = (marks >> from) & 1u;
         if (to < end) bar_sync(1 + kStages + w, stage_threads);
-        fetch(from, to - from, (marks >> from) & 1u);
+        const int at = tile * kTile + from + lane;
+        const bool on = from + lane < to;
+        fetch(from, to - from, mark, on ? to_f(dt[at * a.dt_t]) : 0.0f, on ? to_f(gb[at * a.b_t]) : 0.0f);
         if (lane == 0) st.more = from > 0;
-        cp_async_wait<0>();
-        __syncwarp();
-        ready((marks >> from) & 1u);
+        ready(from, to - from, mark, i == 0 && to == end);
         to = from;
       }
     }
@@ -197,7 +230,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
     // the matrices and gates of 16 x 16
     const int64_t g_t = static_cast<int64_t>(a.heads) * splits, g_at = row0 * g_t + static_cast<int64_t>(h) * splits + blockIdx.y;
     double sum_a = 0.0, sum_bias = 0.0;
-    for (int i = 0, more = 0, turn = 0; i < count; i += more ? 0 : 1, turn ^= 1) {
+    for (int i = 0, more = 0; i < count; i += more ? 0 : 1) {
       const int at = i % kStages;
       typename B::Stage& st = sh.stage[at];
       bar_sync(1 + at, stage_threads);
@@ -218,10 +251,10 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
 #pragma unroll
         for (int x = 0; x < kMain; ++x) {
           float y[4];
-          four(y, &sh.part[turn][x][0][r][j]);
+          four(y, &sh.part[x].product[0][r][j]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) zw[e] += y[e];
-          four(y, &sh.part[turn][x][1][r][j]);
+          four(y, &sh.part[x].product[1][r][j]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) ow[e] += y[e];
         }
@@ -244,9 +277,9 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
           row_m += em[e];
           zr += c == r ? zw[e] : mz[e] * bt[e];
         }
-        *reinterpret_cast<float4*>(&sh.e[0][r][j]) = make_float4(ep[0], ep[1], ep[2], ep[3]);
-        *reinterpret_cast<float4*>(&sh.e[1][r][j]) = make_float4(em[0], em[1], em[2], em[3]);
-        *reinterpret_cast<float4*>(&sh.e[2][r][j]) = make_float4(mz[0], mz[1], mz[2], mz[3]);
+        *reinterpret_cast<float4*>(&st.wide.p[r][j]) = make_float4(ep[0], ep[1], ep[2], ep[3]);
+        *reinterpret_cast<float4*>(&st.wide.m[r][j]) = make_float4(em[0], em[1], em[2], em[3]);
+        *reinterpret_cast<float4*>(&st.wide.d[r][j]) = make_float4(mz[0], mz[1], mz[2], mz[3]);
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           uint32_t y[NS];
@@ -275,20 +308,20 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
       float wd = 0.0f, zv = 0.0f, f = 0.0f, inner = 0.0f;
 #pragma unroll
       for (int x = 0; x < kMain; ++x) {
-        wd += sh.by_value[turn][x][0][c];
-        zv += sh.by_value[turn][x][1][c];
-        f += sh.by_value[turn][x][2][c];
-        inner += sh.inner[turn][x];
+        wd += sh.by_value[x][0][c];
+        zv += sh.by_value[x][1][c];
+        f += sh.by_value[x][2][c];
+        inner += sh.inner[x];
       }
       float column = 0.0f, below = 0.0f, dbeta = wd;
 #pragma unroll
       for (int y = kTile - 1; y >= 0; --y) {
-        const float ep = sh.e[0][y][c], em = sh.e[1][y][c];
-        dbeta -= sh.e[2][y][c];
+        const float ep = st.wide.p[y][c], em = st.wide.m[y][c];
+        dbeta -= st.wide.d[y][c];
         column += ep + em;
         if (y > c) below += ep + em;
         __syncwarp();
-        if (lane < kTile) sh.e[0][y][c] = y > c ? below : 0.0f;
+        if (lane < kTile) st.wide.p[y][c] = y > c ? below : 0.0f;
       }
       row_p = __shfl_sync(0xffffffffu, row_p, 2 * c);
       row_m = __shfl_sync(0xffffffffu, row_m, 2 * c);
@@ -302,12 +335,12 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
       bar_sync(kBarMatrices, team);
       float e = keep;
 #pragma unroll
-      for (int x = 0; x < kMain; ++x) e += sh.by_key[turn][x][c];
+      for (int x = 0; x < kMain; ++x) e += sh.by_key[x][c];
       float dg = marks ? 0.0f : st.c.head[kTile - 1] * inner;
 #pragma unroll
       for (int j = 0; j < kTile; ++j) {
         const float ej = __shfl_sync(0xffffffffu, e, j), fj = __shfl_sync(0xffffffffu, f, j);
-        dg += j >= c ? ej : fj + sh.e[0][c][j];
+        dg += j >= c ? ej : fj + st.wide.p[c][j];
       }
       if (lane < n) {
         const float back = dg * rate * sigmoid(gate.pre), b_back = dbeta * gate.beta * (1.0f - gate.beta);
@@ -363,15 +396,12 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
       d[n][e] = dfinal && r < mine && kc < a.keys ? dfinal[r * a.keys + kc] : 0.0f;
     }
   // what a warp without values or columns leaves
-  for (int turn = 0; turn < 2; ++turn) {
-    for (int i = lane; i < 2 * kTile * kMat; i += 32) (&sh.part[turn][warp][0][0][0])[i] = 0.0f;
-    for (int i = lane; i < 3 * kTile; i += 32) (&sh.by_value[turn][warp][0][0])[i] = 0.0f;
-    if (lane < kTile) sh.by_key[turn][warp][lane] = 0.0f;
-    if (lane == 0) sh.inner[turn][warp] = 0.0f;
-  }
+  for (int i = lane; i < 3 * kTile; i += 32) (&sh.by_value[warp][0][0])[i] = 0.0f;
+  if (lane < kTile) sh.by_key[warp][lane] = 0.0f;
+  if (lane == 0) sh.inner[warp] = 0.0f;
   __syncwarp();
 
-  for (int i = 0, more = 0, turn = 0; i < count; i += more ? 0 : 1, turn ^= 1) {
+  for (int i = 0, more = 0; i < count; i += more ? 0 : 1) {
     const int at = i % kStages;
     typename B::Stage& st = sh.stage[at];
     const Chunk<T, NI>& c = st.c;
@@ -397,20 +427,20 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float2 s = *reinterpret_cast<const float2*>(&st.s[vl + row + 8 * e][16 * x + 8 * t + col]);
+              const float2 s = *reinterpret_cast<const float2*>(&sh.s[vl + row + 8 * e][16 * x + 8 * t + col]);
               inner = fmaf(s.x, d[2 * x + t][2 * e], fmaf(s.y, d[2 * x + t][2 * e + 1], inner));
             }
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, o);
-      if (lane == 0) sh.inner[turn][warp] = inner;
+      if (lane == 0) sh.inner[warp] = inner;
       // dU, Z
       float w[2][4], du[2][4] = {}, z[2][4] = {};
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float2 y = *reinterpret_cast<const float2*>(&st.w[vl + row + 8 * e][8 * t + col]);
+          const float2 y = *reinterpret_cast<const float2*>(&sh.saved_w[vl + row + 8 * e][8 * t + col]);
           w[t][2 * e] = y.x;
           w[t][2 * e + 1] = y.y;
         }
@@ -460,12 +490,12 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
           }
         }
         f.from(z[0], z[1]);
-        put_frag(sh.z, vl + row, col, f);
+        put_tokens(sh.z, vl + row, col, f);
         f.from(w[0], w[1]);
-        put_frag(sh.w, vl + row, col, f);
+        put_tokens(sh.w, vl + row, col, f);
       }
       // sums over the warp's values, by tokens
-      T (&so)[kTile][16 + 16 / sizeof(T)] = sh.out[warp];
+      T (&so)[kTile][16 + 16 / sizeof(T)] = sh.part[warp].out;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -476,9 +506,9 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
           const float zv = column_sum(fmaf(z[t][e], v0, z[t][e + 2] * v1));
           const float send = column_sum(fmaf(w[t][e], ds[t][e], w[t][e + 2] * ds[t][e + 2]));
           if (row == 0) {
-            sh.by_value[turn][warp][0][tok] = wd;
-            sh.by_value[turn][warp][1][tok] = zv;
-            sh.by_value[turn][warp][2][tok] = c.beta[tok] * send;
+            sh.by_value[warp][0][tok] = wd;
+            sh.by_value[warp][1][tok] = zv;
+            sh.by_value[warp][2][tok] = c.beta[tok] * send;
           }
           so[tok][row] = from_f<T>(z[t][e]);
           so[tok][row + 8] = from_f<T>(z[t][e + 2]);
@@ -489,8 +519,8 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
       {
         uint32_t b[NI][4], x[NI][4], o[NT][4];
         float zw[2][4] = {}, ow[2][4] = {};
-        load_planes<NI, true>(b, smem_of(sh.w) + at_cols(lane, kSide) + vl * kSide * 2, kValues * kSide * 2);
-        load_planes<NI, true>(x, smem_of(sh.z) + a_cols(lane, kSide) + vl * kSide * 2, kValues * kSide * 2);
+        load_planes<NI, true>(b, smem_of(sh.w) + tokens_b(lane) + vl * kTile * 2, kValues * kTile * 2);
+        load_planes<NI, true>(x, smem_of(sh.z) + tokens_a(lane) + vl * kTile * 2, kValues * kTile * 2);
         mma_planes<NI, NI>(zw[0], zw[1], x, b);
         load_planes<NT, false>(o, smem_of(st.tdo) + a_rows(lane, Values::kPitch) + vl * 2, Values::kPlane * 2);
         mma_planes<NT, NI>(ow[0], ow[1], o, b);
@@ -498,8 +528,8 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            *reinterpret_cast<float2*>(&sh.part[turn][warp][0][row + 8 * e][8 * t + col]) = make_float2(zw[t][2 * e], zw[t][2 * e + 1]);
-            *reinterpret_cast<float2*>(&sh.part[turn][warp][1][row + 8 * e][8 * t + col]) = make_float2(ow[t][2 * e], ow[t][2 * e + 1]);
+            *reinterpret_cast<float2*>(&sh.part[warp].product[0][row + 8 * e][8 * t + col]) = make_float2(zw[t][2 * e], zw[t][2 * e + 1]);
+            *reinterpret_cast<float2*>(&sh.part[warp].product[1][row + 8 * e][8 * t + col]) = make_float2(ow[t][2 * e], ow[t][2 * e + 1]);
           }
       }
       // dS one chunk on
@@ -538,6 +568,8 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
         }
       }
     }
+    else
+      for (int x = lane; x < 2 * kTile * kMat; x += 32) (&sh.part[warp].product[0][0][0])[x] = 0.0f;
     bar_sync(kBarChain, team);
 
     // by keys: rows tokens, columns c0 ..
@@ -546,10 +578,10 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
       float as[kPairs][2][4] = {};
       for (int x = 0; x < vsteps; ++x) {
         uint32_t o[NT][4], z[NS][4], w[NS][4];
-        load_planes<NS, true>(w, smem_of(sh.w) + a_cols(lane, kSide) + x * 16 * kSide * 2, kValues * kSide * 2);
+        load_planes<NS, true>(w, smem_of(sh.w) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
         if (!fresh) {
           load_planes<NT, false>(o, smem_of(st.tdo) + a_rows(lane, Values::kPitch) + x * 32, Values::kPlane * 2);
-          load_planes<NS, true>(z, smem_of(sh.z) + a_cols(lane, kSide) + x * 16 * kSide * 2, kValues * kSide * 2);
+          load_planes<NS, true>(z, smem_of(sh.z) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
         }
 #pragma unroll
         for (int p = 0; p < kPairs; ++p) {
@@ -561,7 +593,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
             uint32_t s[NI][4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float* from = &st.s[16 * x + (e & 1) * 8 + col][c0 + 16 * p + (e >> 1) * 8 + row];
+              const float* from = &sh.s[16 * x + (e & 1) * 8 + col][c0 + 16 * p + (e >> 1) * 8 + row];
               uint32_t y[NI];
               split2<NI>(from[0], from[B::kPitchS], y);
 #pragma unroll
@@ -588,10 +620,11 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         e0[e] = quad_sum(e0[e]);
-        if ((lane & 3) == 0) sh.by_key[turn][warp][row + 8 * e] = e0[e] * c.rq[row + 8 * e];
+        if ((lane & 3) == 0) sh.by_key[warp][row + 8 * e] = e0[e] * c.rq[row + 8 * e];
       }
     }
     bar_sync(kBarMatrices, team);
+    bar_arrive(kBarState + (more ? at : (i + 1) % kStages), team);       // S and W: the next chunk's warp may have their place
 
     if (by_k) {
       float nq[2] = {}, nk[2] = {}, rq[2], rk[2];
@@ -602,7 +635,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
         if (!a.unit) continue;
         nq[e] = sh.nq[row + 8 * e];
 #pragma unroll
-        for (int x = 0; x < kMain; ++x) nq[e] += sh.by_key[turn][x][row + 8 * e];
+        for (int x = 0; x < kMain; ++x) nq[e] += sh.by_key[x][row + 8 * e];
         nq[e] *= rq[e];                                // what takes the part along q out of dq, for q itself
         nk[e] = sh.nk[row + 8 * e] * rk[e];
       }
@@ -638,7 +671,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads) delta_
               a.part_k[qk_at + (t0 + tok) * qk_t + kc] = ak[p][t][e];
             }
         } else {
-          T (&so)[kTile][16 + 16 / sizeof(T)] = sh.out[warp];
+          T (&so)[kTile][16 + 16 / sizeof(T)] = sh.part[warp].out;
 #pragma unroll
           for (int turn2 = 0; turn2 < 2; ++turn2) {
             __syncwarp();
