@@ -11,6 +11,7 @@
 // One pass over memory: a row's logits stay in shared memory (registers, where a warp takes a
 // row) between the pass that sums and the one that writes the gradient.
 #include <cooperative_groups.h>
+#include <type_traits>
 
 #include "seq_common.cuh"
 
@@ -46,52 +47,57 @@ __device__ __forceinline__ Row row_of(const LossArgs& p, int64_t n, bool report)
   return {n, a >= 0 && a < p.v ? static_cast<int>(a) : -1};
 }
 
-// running maximum m, sum of e^(y - m) and of (y - m) e^(y - m)
-struct Sums { float m, s, t; };
-// NaN logits count as -inf
-__device__ __forceinline__ float clean(float z) { return z == z ? z : -INFINITY; }
-// the exponent of z under the maximum m: 0 for the largest, infinite ones among them
-__device__ __forceinline__ float below(float z, float m, float inv_t) { return z == m ? 0.0f : (z - m) * inv_t; }
-__device__ __forceinline__ void add(Sums& a, float z, float inv_t) {
-  const float y = below(z, a.m, inv_t), e = __expf(y);
-  a.s += e;
-  if (e > 0.0f) a.t = fmaf(e, y, a.t);
+// A row's exponents in powers of two: with c = log2(e) / t and the maximum m, x = z c - m c and e^(y - max y)
+// = 2^x. The product m c is rounded once and is then what all of the row is measured from, so that its
+// rounding cancels; where it would be as large as the differences themselves (and for infinite
+// maxima) x is (z - m) c instead. -1000 stands for what has no probability: -inf and NaN (which the
+// maximum of two numbers drops).
+struct Shift {
+  float m, c, mc;
+  bool far;
+  __device__ __forceinline__ double from() const { return far ? static_cast<double>(m) * c : static_cast<double>(mc); }   // finite m
+};
+__device__ __forceinline__ Shift shift_of(float m, float inv_t) {
+  const float c = __fmul_rn(inv_t, kLog2e), mc = __fmul_rn(m, c);
+  return {m, c, mc, !(fabsf(mc) <= 1048576.0f)};
 }
+template <bool kFar> __device__ __forceinline__ float power_of(float z, const Shift& h) {
+  if constexpr (kFar) return z == h.m ? 0.0f : fmaxf((z - h.m) * h.c, -1000.0f);
+  else return fmaxf(fmaf(z, h.c, -h.mc), -1000.0f);
+}
+// sums of 2^x and of x 2^x, x measured from m
+struct Sums { float m, s, t; };
+template <bool kFar> __device__ __forceinline__ void add(Sums& a, float z, const Shift& h) {
+  const float x = power_of<kFar>(z, h), e = exp2_hw(x);
+  a.s += e;
+  a.t = fmaf(e, x, a.t);
+}
+// NaN logits count as -inf
+__device__ __forceinline__ float clean(float z) { return fmaxf(z, -INFINITY); }
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float inv_t) {
-  const float m = fmaxf(a.m, b.m);
-  Sums r{m, 0.0f, 0.0f};
-  if (a.s > 0.0f) {
-    const float y = below(a.m, m, inv_t), f = expf(y);
-    r.s = a.s * f;
-    if (f > 0.0f) r.t = f * fmaf(a.s, y, a.t);
-  }
-  if (b.s > 0.0f) {
-    const float y = below(b.m, m, inv_t), f = expf(y);
-    r.s = fmaf(b.s, f, r.s);
-    if (f > 0.0f) r.t += f * fmaf(b.s, y, b.t);
-  }
-  return r;
+  const Sums &hi = a.m >= b.m ? a : b, &lo = a.m >= b.m ? b : a;
+  if (!(lo.s > 0.0f) || (hi.m == INFINITY && lo.m < hi.m)) return hi;
+  const float x = hi.m == lo.m ? 0.0f : static_cast<float>(shift_of(lo.m, inv_t).from() - shift_of(hi.m, inv_t).from()), f = exp2f(x);
+  return {hi.m, fmaf(lo.s, f, hi.s), hi.t + f * fmaf(lo.s, x, lo.t)};
 }
 
-// What the gradient needs of a row: dz = k_p p + k_e p log p (+ k_a at the answer), times 1 / t inside
-struct Slopes {
-  int a;
-  float m, log_s, inv_s, kp, ke, ka;
-};
+// What the gradient needs of a row: dz = 2^x (ax x + b), + ka at the answer
+struct Slopes { float m, ax, b, ka; };
 
 // The row's numbers from its sums; `za` the answer's logit. Written by one thread.
 __device__ __forceinline__ Slopes finish(const LossArgs& p, const Row& row, const Sums& s, float za, bool write) {
-  Slopes g{-1, s.m, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  Slopes g{s.m, 0.0f, 0.0f, 0.0f};
   float lp = 0.0f, kl = 0.0f, ent = 0.0f, each = 0.0f;
   if (row.a >= 0 && za > -INFINITY) {
     const float w = p.weight ? p.weight[row.n] : p.share, adv = p.adv[row.n];
     // the logarithm of the sum and what is subtracted from it in 64 bits: log-probabilities and
     // small KL terms are differences of larger numbers
-    const double log_s = log(static_cast<double>(s.s));
-    const double y = za == s.m ? 0.0 : (static_cast<double>(za) - s.m) * p.inv_t;
-    const double l = y - log_s;
+    constexpr double kLn2d = 0.69314718055994530942;
+    const Shift h = shift_of(s.m, p.inv_t);
+    const double log_s = log(static_cast<double>(s.s)), power = static_cast<double>(s.t) / s.s;
+    const double l = (za == s.m && h.far ? 0.0 : static_cast<double>(za) * h.c - h.from()) * kLn2d - log_s;
     lp = static_cast<float>(l);
-    ent = static_cast<float>(log_s - static_cast<double>(s.t) / s.s);
+    ent = static_cast<float>(log_s - power * kLn2d);
     const float ratio = expf(static_cast<float>(l - p.old_logp[row.n]));
     const float held = fminf(fmaxf(ratio, 1.0f - p.lo), 1.0f + p.hi);
     const float free = adv == 0.0f ? 0.0f : ratio * adv, cut = held * adv;
@@ -106,12 +112,11 @@ __device__ __forceinline__ Slopes finish(const LossArgs& p, const Row& row, cons
     }
     each = w * fmaf(-p.ent, ent, each);
     c *= w;
-    g.a = row.a;
-    g.log_s = static_cast<float>(log_s);
-    g.inv_s = 1.0f / s.s;
+    // p = 2^x / s, log p = x ln 2 - log s:  (w ent p (log p + H) - c p) / t
+    const float ke = w * p.ent * p.inv_t / s.s;
     g.ka = c * p.inv_t;
-    g.ke = w * p.ent * p.inv_t;
-    g.kp = fmaf(g.ke, ent, -g.ka);
+    g.ax = ke * kLn2;
+    g.b = ke * (ent - static_cast<float>(log_s)) - g.ka / s.s;
   }
   if (write) {
     p.rows[row.n] = lp;
@@ -121,11 +126,9 @@ __device__ __forceinline__ Slopes finish(const LossArgs& p, const Row& row, cons
   }
   return g;
 }
-__device__ __forceinline__ float slope(const Slopes& g, float z, int j, float inv_t) {
-  const float y = below(z, g.m, inv_t), pr = __expf(y) * g.inv_s;
-  float d = pr > 0.0f ? pr * fmaf(g.ke, y - g.log_s, g.kp) : 0.0f;
-  if (j == g.a) d += g.ka;
-  return g.a < 0 ? 0.0f : d;
+template <bool kFar> __device__ __forceinline__ float slope(const Slopes& g, float z, const Shift& h) {
+  const float x = power_of<kFar>(z, h);
+  return exp2_hw(x) * fmaf(g.ax, x, g.b);
 }
 
 // The rows' losses summed in a fixed order: a kernel of its own, since a counter of arrivals would
@@ -150,45 +153,52 @@ constexpr int kWarpThreads = 256;
 template <typename T, int H> __global__ void __launch_bounds__(kWarpThreads) loss_warp(LossArgs p) {
   const int lane = threadIdx.x & 31;
   const int64_t n = static_cast<int64_t>(blockIdx.x) * (kWarpThreads / 32) + (threadIdx.x >> 5);
-  if (n < p.n) {
-    const Row row = row_of(p, n, lane == 0);
-    const T* z = static_cast<const T*>(p.z) + n * p.z_ld;
-    float v[H], m = -INFINITY;
+  if (n >= p.n) return;
+  const Row row = row_of(p, n, lane == 0);
+  const T* z = static_cast<const T*>(p.z) + n * p.z_ld;
+  float v[H], m = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < H; ++k) {
-      v[k] = k * 32 + lane < p.v ? clean(to_f(z[k * 32 + lane])) : -INFINITY;
-      m = fmaxf(m, v[k]);
-    }
+  for (int k = 0; k < H; ++k) {
+    v[k] = k * 32 + lane < p.v ? to_f(z[k * 32 + lane]) : -INFINITY;
+    m = fmaxf(m, v[k]);
+  }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    Sums s{m, 0.0f, 0.0f};
-    float za = -INFINITY;
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  Sums s{m, 0.0f, 0.0f};
+  const Shift h = shift_of(m, p.inv_t);
+  float za = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < H; ++k) {
-      if (v[k] > -INFINITY) add(s, v[k], p.inv_t);
-      if (k * 32 + lane == row.a) za = v[k];
-    }
+  for (int k = 0; k < H; ++k) {
+    if (h.far) add<true>(s, v[k], h);
+    else add<false>(s, v[k], h);
+    if (k * 32 + lane == row.a) za = clean(v[k]);
+  }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      s.s += __shfl_xor_sync(0xffffffffu, s.s, o);
-      s.t += __shfl_xor_sync(0xffffffffu, s.t, o);
-      za = fmaxf(za, __shfl_xor_sync(0xffffffffu, za, o));
-    }
-    const Slopes g = finish(p, row, s, za, lane == 0);
-    if (p.dz) {
-      T* d = static_cast<T*>(p.dz) + n * p.d_ld;
+  for (int o = 16; o; o >>= 1) {
+    s.s += __shfl_xor_sync(0xffffffffu, s.s, o);
+    s.t += __shfl_xor_sync(0xffffffffu, s.t, o);
+    za = fmaxf(za, __shfl_xor_sync(0xffffffffu, za, o));
+  }
+  const Slopes g = finish(p, row, s, za, lane == 0);
+  if (!p.dz) return;
+  T* d = static_cast<T*>(p.dz) + n * p.d_ld;
 #pragma unroll
-      for (int k = 0; k < H; ++k)
-        if (k * 32 + lane < p.v) d[k * 32 + lane] = from_f<T>(slope(g, v[k], k * 32 + lane, p.inv_t));
-    }
+  for (int k = 0; k < H; ++k) {
+    const int at = k * 32 + lane;
+    if (at < p.v) d[at] = from_f<T>((h.far ? slope<true>(g, v[k], h) : slope<false>(g, v[k], h)) + (at == row.a ? g.ka : 0.0f));
   }
 }
 
 // ---- a cluster of blocks for a row ------------------------------------------------------
 constexpr int kRowThreads = 512;
 
-// A block takes candidates [lo, hi) of its row; shared memory mirrors their place within 16 bytes
-// of global memory, so that all but the ends move in pieces of 16 bytes.
+__device__ __forceinline__ float max_of(const uint4& q, float m) {
+  return fmaxf(fmaxf(m, fmaxf(__uint_as_float(q.x), __uint_as_float(q.y))), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+}
+__device__ __forceinline__ __nv_bfloat162 pair_of(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+
+// A block takes candidates [first, first + count) of its row; shared memory mirrors their place within 16
+// bytes of global memory, so that all but the ends move in pieces of 16 bytes.
 template <typename T> __global__ void __launch_bounds__(kRowThreads) loss_row(LossArgs p, int per) {
   constexpr int V = kVec16<T>;
   extern __shared__ __align__(16) char smem[];
@@ -204,41 +214,54 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads) loss_row(Lo
   T* hold = reinterpret_cast<T*>(smem) + (reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T);
   const int head = min(count, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) / sizeof(T)) % V);
   const int whole = (count - head) / V;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < whole; i += kRowThreads) {
-    float v[V];
-    load_vec<T, V>(z + head + i * V, v);
-    *reinterpret_cast<uint4*>(hold + head + i * V) = *reinterpret_cast<const uint4*>(z + head + i * V);
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = fmaxf(m, clean(v[j]));
-  }
   const int rest = count - whole * V;                  // the ends: [0, head) and behind the pieces
+  float m = -INFINITY;
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat16 low = __ushort_as_bfloat16(0xff80);
+    __nv_bfloat162 top = {low, low};
+#pragma unroll 4
+    for (int i = threadIdx.x; i < whole; i += kRowThreads) {
+      const uint4 q = *reinterpret_cast<const uint4*>(z + head + i * V);
+      *reinterpret_cast<uint4*>(hold + head + i * V) = q;
+      top = __hmax2(top, __hmax2(__hmax2(pair_of(q.x), pair_of(q.y)), __hmax2(pair_of(q.z), pair_of(q.w))));
+    }
+    m = fmaxf(m, fmaxf(__low2float(top), __high2float(top)));
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < whole; i += kRowThreads) {
+      const uint4 q = *reinterpret_cast<const uint4*>(z + head + i * V);
+      *reinterpret_cast<uint4*>(hold + head + i * V) = q;
+      m = max_of(q, m);
+    }
+  }
   for (int i = threadIdx.x; i < rest; i += kRowThreads) {
     const int at = i < head ? i : i + whole * V;
     hold[at] = z[at];
-    m = fmaxf(m, clean(to_f(z[at])));
+    m = fmaxf(m, to_f(z[at]));
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5].m = m;
   __syncthreads();
+#pragma unroll
   for (int i = 0; i < kRowThreads / 32; ++i) m = fmaxf(m, part[i].m);
   __syncthreads();
   Sums s{m, 0.0f, 0.0f};
-  if (m > -INFINITY) {
+  auto sum = [&](auto far) {
+    constexpr bool kFar = decltype(far)::value;
+    const Shift h = shift_of(m, p.inv_t);
+#pragma unroll 2
     for (int i = threadIdx.x; i < whole; i += kRowThreads) {
       float v[V];
       load_vec<T, V>(hold + head + i * V, v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float q = clean(v[j]);
-        if (q > -INFINITY) add(s, q, p.inv_t);
-      }
+      for (int j = 0; j < V; ++j) add<kFar>(s, v[j], h);
     }
-    for (int i = threadIdx.x; i < rest; i += kRowThreads) {
-      const float q = clean(to_f(hold[i < head ? i : i + whole * V]));
-      if (q > -INFINITY) add(s, q, p.inv_t);
-    }
+    for (int i = threadIdx.x; i < rest; i += kRowThreads) add<kFar>(s, to_f(hold[i < head ? i : i + whole * V]), h);
+  };
+  if (m > -INFINITY) {
+    if (shift_of(m, p.inv_t).far) sum(std::true_type());
+    else sum(std::false_type());
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -270,19 +293,24 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads) loss_row(Lo
     slopes = finish(p, row, all, za, rank == 0);
   }
   if (ranks > 1) cl.sync(); else __syncthreads();      // the others' shared memory is read no more
-  if (p.dz) {
-    const Slopes g = slopes;
-    const int at_answer = g.a - first;
-    T* d = static_cast<T*>(p.dz) + n * p.d_ld + first;
-    const bool same = ((reinterpret_cast<uintptr_t>(d) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
-    Slopes q = g;
-    q.a = g.a < 0 ? -1 : 0;
+  if (!p.dz) return;
+  const Slopes g = slopes;
+  const int answer_at = row.a - first;                 // in this block's candidates, if at all
+  T* d = static_cast<T*>(p.dz) + n * p.d_ld + first;
+  const bool same = ((reinterpret_cast<uintptr_t>(d) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
+  auto write = [&](auto far) {
+    constexpr bool kFar = decltype(far)::value;
+    const Shift h = shift_of(g.m, p.inv_t);
+#pragma unroll 2
     for (int i = threadIdx.x; i < whole; i += kRowThreads) {
       const int at = head + i * V;
       float v[V];
       load_vec<T, V>(hold + at, v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = slope(q, clean(v[j]), at + j == at_answer ? 0 : 1, p.inv_t);
+      for (int j = 0; j < V; ++j) v[j] = slope<kFar>(g, v[j], h);
+      if (static_cast<unsigned>(answer_at - at) < static_cast<unsigned>(V) && row.a >= 0)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += at + j == answer_at ? g.ka : 0.0f;
       if (same) {
         store_vec<T, V>(d + at, v);
       } else {
@@ -292,9 +320,11 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads) loss_row(Lo
     }
     for (int i = threadIdx.x; i < rest; i += kRowThreads) {
       const int at = i < head ? i : i + whole * V;
-      d[at] = from_f<T>(slope(q, clean(to_f(hold[at])), at == at_answer ? 0 : 1, p.inv_t));
+      d[at] = from_f<T>(slope<kFar>(g, to_f(hold[at]), h) + (at == answer_at && row.a >= 0 ? g.ka : 0.0f));
     }
-  }
+  };
+  if (shift_of(g.m, p.inv_t).far) write(std::true_type());
+  else write(std::false_type());
 }
 
 template <typename T> int run(const LossArgs& a, int ranks, int per, cudaStream_t s) {

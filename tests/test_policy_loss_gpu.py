@@ -122,6 +122,26 @@ def test_infinite_logits_share_the_probability():
         assert torch.isfinite(r.dlogits).all() and not r.dlogits[:, 8:].any()
 
 
+@pytest.mark.parametrize("size", [1e3, 5e5, 7.3e5, 1e6, 1e8, 1e30])
+def test_large_logits(size):
+    """Logits of any size about each other: their differences are what counts. A log-probability is a
+    difference of numbers of that size, each exact, times 1 / t in 32 bits (2^-24 of the difference)."""
+    for v in (40, 3000, 140000):
+        gen = torch.Generator("cuda").manual_seed(5)
+        z = torch.randn(3, v, generator=gen, device="cuda") * min(2.0, 1e-7 * size + 1.0) + size
+        z[1] = -z[1]
+        z[2, ::2] = -size
+        a = z.argmax(1).to(torch.int32)
+        a[0] = 1
+        c = dict(logits=z, answers=a, old_logp=torch.zeros(3, device="cuda"), advantages=torch.ones(3, device="cuda"))
+        r = R.policy_loss(**c, ent_coef=0.1, clip=1.0, clip_high=1e30)
+        zd = z.double().requires_grad_()
+        want = R.policy_loss_reference(zd, a, c["old_logp"].double(), c["advantages"].double(), ent_coef=0.1, clip=1.0, clip_high=1e30)
+        lp = torch.log_softmax(zd.detach(), 1).gather(1, a.long()[:, None])[:, 0]
+        assert rel(r.logp, lp) < 1e-6
+        assert rel(r.dlogits, torch.autograd.grad(want, zd)[0]) < 1e-5
+
+
 def test_far_ratios():
     """A ratio of e^200 is infinite in 32 bits: its loss is, no advantage means no loss; small ones vanish."""
     c = make(4, 10, F32, masked=False)
