@@ -321,8 +321,9 @@ def cmd_gpu_health(args) -> int:
 
 def cmd_recall(args) -> int:
     from .models.memory import MemoryConfig, train_recall
-    r = train_recall(args.iterations, args.envs, args.length, MemoryConfig(dim=args.dim), args.device, args.lr, args.seed,
-                     temperature=args.temperature, top_p=args.top_p, log=print)
+    cfg = MemoryConfig(dim=args.dim, core=args.core, heads=args.heads, keys=args.keys)
+    r = train_recall(args.iterations, args.envs, args.length, cfg, args.device, args.lr, args.seed,
+                     temperature=args.temperature, top_p=args.top_p, objective=args.objective, log=print)
     print(json.dumps(r))
     return 0
 
@@ -532,6 +533,11 @@ def build_parser() -> argparse.ArgumentParser:
     rc.add_argument("--envs", type=int, default=128)
     rc.add_argument("--length", type=int, default=64, help="decisions of a training row")
     rc.add_argument("--dim", type=int, default=256, help="channels of the core")
+    rc.add_argument("--core", choices=("scan", "delta"), default="scan", help="selective scan or gated delta rule")
+    rc.add_argument("--heads", type=int, default=4, help="heads of the delta core")
+    rc.add_argument("--keys", type=int, default=32, help="keys of a head of the delta core")
+    rc.add_argument("--objective", choices=("answers", "policy"), default="answers",
+                    help="the asked-for answers, or what sampled answers earn (clipped policy loss)")
     rc.add_argument("--lr", type=float, default=1e-2)
     rc.add_argument("--temperature", type=float, default=0.5)
     rc.add_argument("--top-p", type=float, default=0.9)

@@ -9,8 +9,15 @@ state through all of them. One block, features -> answers:
     o  = selective_scan(c, W_dt r, A, B, C, gate z)
     logits = W_out o + b
 
-with ``ops.gemm`` for the projections and ``ops.ssm`` for the rest. Three ways to run
-it: ``forward_sequence`` / ``backward`` over rows of decisions [envs, T] with episode
+with ``ops.gemm`` for the projections and ``ops.ssm`` for the rest. With ``core="delta"`` the
+memory is a matrix per head that is written by correction (``ops.delta``):
+
+    c  = causal_conv(W_in f)       queries, keys and values of the heads, side by side
+    (dt, b) = W_g f                decay and writing strength of each head
+    o  = gated_delta(c, dt, b, A)
+    logits = W_out group_norm(o, heads, SiLU) + b
+
+Three ways to run it: ``forward_sequence`` / ``backward`` over rows of decisions [envs, T] with episode
 resets inside the rows (training, states carried from row to row), ``step`` for one
 decision of every env (rollout: one slot of the state pools per env) and ``act``, a
 step whose answers are drawn by ``ops.tokens.sample_tokens``. ``forward_reference`` is
@@ -28,7 +35,7 @@ from typing import Optional
 import numpy as np
 import torch
 
-from ..ops import ssm
+from ..ops import delta, norm, ssm
 
 
 @dataclass
@@ -40,16 +47,32 @@ class MemoryConfig:
     rank: int = 16              # of the step projection (a multiple of 8)
     answers: int = 8            # categories of the answer
     out_pad: int = 64           # columns of the output (>= answers)
+    core: str = "scan"          # or "delta"
+    heads: int = 4              # of the delta core (a multiple of 4); dim / heads values each
+    keys: int = 32              # of a head of the delta core (a multiple of 8)
+
+    @property
+    def conv_dim(self) -> int:
+        """Channels of the convolution: the core's, or the heads' queries, keys and values."""
+        return self.dim if self.core == "scan" else 2 * self.heads * self.keys + self.dim
+
+    def heads_of(self, c: torch.Tensor):
+        """(queries, keys, values) of the delta core's convolution, by heads."""
+        h, hk = self.heads, self.heads * self.keys
+        return (c[..., :hk].unflatten(-1, (h, self.keys)), c[..., hk:2 * hk].unflatten(-1, (h, self.keys)),
+                c[..., 2 * hk:].unflatten(-1, (h, self.dim // h)))
 
 
 class MemoryState:
-    """Convolution windows [S, W-1, D] and scan states [S, D, N] of S envs."""
+    """Convolution windows [S, W-1, channels] and the core's states (scan [S, D, N], delta rule
+    [S, H, values, keys]) of S envs."""
 
     def __init__(self, net: "MemoryNet", envs: int):
         c = net.cfg
         dt = torch.bfloat16 if net.device.type == "cuda" else torch.float32
-        self.conv = torch.zeros(envs, c.width - 1, c.dim, dtype=dt, device=net.device)
-        self.scan = torch.zeros(envs, c.dim, c.state, device=net.device)
+        self.conv = torch.zeros(envs, c.width - 1, c.conv_dim, dtype=dt, device=net.device)
+        core = (c.dim, c.state) if c.core == "scan" else (c.heads, c.dim // c.heads, c.keys)
+        self.scan = torch.zeros(envs, *core, device=net.device)
 
 
 class MemoryNet:
@@ -60,7 +83,16 @@ class MemoryNet:
         c = cfg
         if c.features % 8 or c.dim % 8 or c.rank % 8 or c.state % 4 or c.answers > c.out_pad:
             raise ValueError("features, dim and rank must be multiples of 8, state of 4, answers at most out_pad")
-        self.specs = [("in.w", (2 * c.dim, c.features)), ("x.w", (c.rank + 2 * c.state, c.dim)), ("dt.w", (c.dim, c.rank)),
+        if c.core not in ("scan", "delta"):
+            raise ValueError(f"core must be scan or delta, not {c.core!r}")
+        if c.core == "delta" and (c.heads % 4 or c.dim % c.heads or c.dim // c.heads > delta.MAX_HEAD or
+                                  c.keys % 8 or not 0 < c.keys <= delta.MAX_HEAD):
+            raise ValueError(f"heads must be a multiple of 4 that divides dim, with at most {delta.MAX_HEAD} values and "
+                             f"8 to {delta.MAX_HEAD} keys, a multiple of 8")
+        self.specs = [("in.w", (c.conv_dim, c.features)), ("gate.w", (2 * c.heads, c.features)), ("out.w", (c.out_pad, c.dim)),
+                      ("conv.w", (c.conv_dim, c.width)), ("conv.b", (c.conv_dim,)), ("dt.b", (c.heads,)), ("a_log", (c.heads,)),
+                      ("norm.w", (c.dim,)), ("norm.b", (c.dim,)), ("out.b", (c.out_pad,))] if c.core == "delta" else \
+                     [("in.w", (2 * c.dim, c.features)), ("x.w", (c.rank + 2 * c.state, c.dim)), ("dt.w", (c.dim, c.rank)),
                       ("out.w", (c.out_pad, c.dim)), ("conv.w", (c.dim, c.width)), ("conv.b", (c.dim,)), ("dt.b", (c.dim,)),
                       ("a_log", (c.dim, c.state)), ("skip", (c.dim,)), ("out.b", (c.out_pad,))]
         self.offsets, off = {}, 0
@@ -91,14 +123,18 @@ class MemoryNet:
         """Uniform +-1/sqrt(fan in) weights; decays exp(-delta n), n = 1 .. N, with steps
         spread over 0.001 .. 0.1, so that a channel remembers 10 to 1000 decisions."""
         c, gen = self.cfg, torch.Generator().manual_seed(seed)
-        for name in ("in.w", "x.w", "dt.w", "out.w", "conv.w"):
+        for name in ("in.w", "x.w", "dt.w", "out.w", "conv.w") if c.core == "scan" else ("in.w", "gate.w", "out.w", "conv.w"):
             shape = self.offsets[name][1]
             w = (torch.rand(shape, generator=gen) * 2 - 1) / math.sqrt(shape[1])
             if name == "out.w":
                 w[c.answers:] = 0.0
             self.p(name).copy_(w)
-        step = torch.exp(torch.rand(c.dim, generator=gen) * math.log(100.0) + math.log(0.001))
+        step = torch.exp(torch.rand(self.p("dt.b").shape, generator=gen) * math.log(100.0) + math.log(0.001))
         self.p("dt.b").copy_(torch.log(torch.expm1(step)))
+        if c.core == "delta":
+            self.p("norm.w").fill_(1.0)             # and decays exp(-step), a_log = 0
+            self.sync_bf16()
+            return
         self.p("a_log").copy_(torch.log(torch.arange(1, c.state + 1).float()).expand(c.dim, -1))
         self.p("skip").fill_(1.0)
         self.sync_bf16()
@@ -122,6 +158,14 @@ class MemoryNet:
         c = self.cfg
         P = params if params is not None else {n: self.p(n) for n, _ in self.specs}
         B, T, _ = x.shape
+        if c.core == "delta":
+            qkv, conv = ssm.causal_conv_reference(x.float() @ P["in.w"].t(), P["conv.w"], P["conv.b"], state=state.conv.float(),
+                                                  reset=reset)
+            gates = x.float() @ P["gate.w"].t()
+            o, scan = delta.gated_delta_reference(*c.heads_of(qkv), gates[..., :c.heads], gates[..., c.heads:], -torch.exp(P["a_log"]),
+                                                  dt_bias=P["dt.b"], state=state.scan, reset=reset)
+            o = norm.group_norm_reference(o.reshape(B * T, c.dim), c.heads, P["norm.w"], P["norm.b"], activation="silu")
+            return o.view(B, T, c.dim) @ P["out.w"].t() + P["out.b"], conv, scan
         xz = x.float() @ P["in.w"].t()
         xc, conv = ssm.causal_conv_reference(xz[..., :c.dim], P["conv.w"], P["conv.b"], state=state.conv.float(), reset=reset)
         proj = xc @ P["x.w"].t()
@@ -134,7 +178,7 @@ class MemoryNet:
 # ---- kernels' path ----------------------------------------------------------------------
 class SequenceCache:
     """What ``backward`` reads of a ``forward_sequence``."""
-    __slots__ = ("x", "xz", "xc", "proj", "dt", "out", "saved", "conv0", "scan0", "reset", "A")
+    __slots__ = ("x", "xz", "xc", "proj", "dt", "out", "saved", "conv0", "scan0", "reset", "A", "core", "stats")
 
 
 def forward_sequence(net: MemoryNet, x: torch.Tensor, state: MemoryState, reset: Optional[torch.Tensor], train: bool = True):
@@ -144,6 +188,8 @@ def forward_sequence(net: MemoryNet, x: torch.Tensor, state: MemoryState, reset:
     c, k = net.cfg, SequenceCache()
     B, T, _ = x.shape
     k.x, k.reset, k.conv0, k.scan0 = x.reshape(B * T, c.features), reset, state.conv, state.scan
+    if c.core == "delta":
+        return _forward_delta(net, k, state, B, T, train), k
     k.xz = G.gemm(k.x, net.w16("in.w")).view(B, T, 2 * c.dim)
     k.xc, state.conv = ssm.causal_conv(k.xz[..., :c.dim], net.p("conv.w"), net.p("conv.b"), state=k.conv0, reset=reset)
     k.proj = G.gemm(k.xc.view(B * T, c.dim), net.w16("x.w"))
@@ -154,6 +200,37 @@ def forward_sequence(net: MemoryNet, x: torch.Tensor, state: MemoryState, reset:
     k.out, k.saved, state.scan = r.out, r.saved, r.final
     logits = G.gemm(k.out.view(B * T, c.dim), net.w16("out.w"), out_dtype=torch.float32, bias=net.p("out.b"))
     return logits.view(B, T, c.out_pad), k
+
+
+def _forward_delta(net: MemoryNet, k: SequenceCache, state: MemoryState, B: int, T: int, train: bool) -> torch.Tensor:
+    from ..ops import gemm as G
+    c = net.cfg
+    k.xz = G.gemm(k.x, net.w16("in.w")).view(B, T, c.conv_dim)
+    k.xc, state.conv = ssm.causal_conv(k.xz, net.p("conv.w"), net.p("conv.b"), state=k.conv0, reset=k.reset)
+    k.dt = G.gemm(k.x, net.w16("gate.w")).view(B, T, 2 * c.heads)
+    k.A = -torch.exp(net.p("a_log"))
+    r = delta.gated_delta(*c.heads_of(k.xc), k.dt[..., :c.heads], k.dt[..., c.heads:], k.A, dt_bias=net.p("dt.b"), state=k.scan0,
+                          reset=k.reset, train=train)
+    k.core, k.saved, state.scan = r.out.view(B * T, c.dim), r.saved, r.final
+    n = norm.group_norm(k.core, c.heads, net.p("norm.w"), net.p("norm.b"), activation="silu", train=train)
+    k.out, k.stats = n.out, n.stats
+    return G.gemm(k.out, net.w16("out.w"), out_dtype=torch.float32, bias=net.p("out.b")).view(B, T, c.out_pad)
+
+
+def _backward_delta(net: MemoryNet, k: SequenceCache, dout: torch.Tensor, B: int, T: int) -> torch.Tensor:
+    """The gradient of the convolution's output, for the gradient ``dout`` [B T, dim] of the normalised heads."""
+    from .policy import _wgrad
+    from ..ops import gemm as G
+    c = net.cfg
+    n = norm.group_norm_grad(dout, k.core, c.heads, net.p("norm.w"), net.p("norm.b"), stats=k.stats, activation="silu")
+    net.g("norm.w").add_(n.dweight)
+    net.g("norm.b").add_(n.dbias)
+    d = delta.gated_delta_grad(n.dx.view(B, T, c.heads, c.dim // c.heads), *c.heads_of(k.xc), k.dt[..., :c.heads], k.dt[..., c.heads:], k.A,
+                               saved=k.saved, dt_bias=net.p("dt.b"), state=k.scan0, reset=k.reset)
+    net.g("a_log").add_(d.dA * k.A)
+    net.g("dt.b").add_(d.ddt_bias)
+    _wgrad(G, torch.cat([d.ddt, d.db], -1).view(B * T, 2 * c.heads), k.x, net.g("gate.w"), B * T)
+    return torch.cat([v.flatten(2) for v in (d.dq, d.dk, d.dv)], -1)
 
 
 def _maps(net, proj, B, T):
@@ -174,6 +251,13 @@ def backward(net: MemoryNet, k: SequenceCache, dlogits: torch.Tensor) -> None:
     _wgrad(G, dl, k.out.view(n, c.dim), net.g("out.w"), n)
     G.colsum(dl, net.g("out.b"))
     dout = G.gemm(dl, net.w16("out.w"), b_mn=True).view(B, T, c.dim)
+    if c.core == "delta":
+        g = ssm.causal_conv_grad(_backward_delta(net, k, dout.view(n, c.dim), B, T), k.xz, net.p("conv.w"), net.p("conv.b"), state=k.conv0,
+                                 reset=k.reset)
+        net.g("conv.w").add_(g.dweight)
+        net.g("conv.b").add_(g.dbias)
+        _wgrad(G, g.dx.view(n, c.conv_dim), k.x, net.g("in.w"), n)
+        return
     s = ssm.selective_scan_grad(dout, k.xc, k.dt, k.A, *_maps(net, k.proj, B, T), saved=k.saved, D=net.p("skip"),
                                 z=k.xz[..., c.dim:], dt_bias=net.p("dt.b"), state=k.scan0, reset=k.reset)
     net.g("a_log").add_(s.dA * k.A)
@@ -205,6 +289,13 @@ def step(net: MemoryNet, x: torch.Tensor, state: MemoryState, reset: Optional[to
     c = net.cfg
     R = x.shape[0]
     xz = G.gemm(x, net.w16("in.w"))
+    if c.core == "delta":
+        xc = ssm.causal_conv_step(xz, net.p("conv.w"), net.p("conv.b"), state.conv, reset=reset, slots=slots)
+        gates = G.gemm(x, net.w16("gate.w"))
+        out = delta.gated_delta_step(*c.heads_of(xc), gates[:, :c.heads], gates[:, c.heads:], -torch.exp(net.p("a_log")), state.scan,
+                                     dt_bias=net.p("dt.b"), reset=reset, slots=slots)
+        out = norm.group_norm(out.view(R, c.dim), c.heads, net.p("norm.w"), net.p("norm.b"), activation="silu").out
+        return G.gemm(out, net.w16("out.w"), out_dtype=torch.float32, bias=net.p("out.b"))
     xc = ssm.causal_conv_step(xz[:, :c.dim], net.p("conv.w"), net.p("conv.b"), state.conv, reset=reset, slots=slots)
     proj = G.gemm(xc, net.w16("x.w"))
     dt = G.gemm(proj[:, :c.rank], net.w16("dt.w"))
@@ -257,50 +348,100 @@ class RecallTask:
         return np.stack(xs, 1), np.stack(rs, 1), np.stack(ts, 1)
 
 
+def _answers_gradient(logits, targets, cfg):
+    """(cross-entropy of the asked-for answers, its gradient by all of the output's columns)."""
+    asked = targets >= 0
+    count = asked.sum().clamp(min=1)
+    lsm = torch.log_softmax(logits[..., :cfg.answers].float(), -1)
+    target = targets.clamp(min=0)[..., None]
+    loss = -(lsm.gather(-1, target)[..., 0] * asked).sum() / count
+    d = torch.zeros_like(logits)
+    d[..., :cfg.answers] = lsm.detach().exp()
+    d.scatter_add_(-1, target, torch.full_like(target, -1.0, dtype=d.dtype))
+    return loss, d * (asked[..., None] / count)
+
+
+class _Answered:
+    """Answers that the policy gave to a batch of rows, and what they were worth: a drawn answer to every
+    question, 1 for a right one, against the batch's mean."""
+
+    def __init__(self, logits, targets, cfg, u, sample):
+        z = logits.detach().reshape(-1, logits.shape[-1])[:, :cfg.answers]
+        t = targets.reshape(-1)
+        token, logp = sample(z, u)
+        asked = t >= 0
+        self.count = asked.sum().clamp(min=1)
+        right = ((token[:, 0] == t) & asked).float()
+        self.answers = torch.where(asked, token[:, 0], -1).to(torch.int32)
+        self.logp = logp[:, 0].contiguous()
+        self.advantages = right - right.sum() / self.count
+        self.weights = (asked / self.count).float()
+        self.right = right.sum() / self.count
+
+    def options(self):
+        """Of ``ops.rl.policy_loss``: the KL term holds the policy to the one that answered."""
+        return dict(ref_logp=self.logp, weights=self.weights, clip=0.2, kl_coef=0.02, ent_coef=0.005)
+
+
 def train_recall(iterations: int = 400, envs: int = 128, length: int = 64, cfg: Optional[MemoryConfig] = None, device="cuda",
                  lr: float = 1e-2, seed: int = 0, longest: int = 48, act_steps: int = 96, temperature: float = 0.5, top_p: float = 0.9,
-                 log=None) -> dict:
+                 objective: str = "answers", epochs: int = 2, log=None) -> dict:
     """Train a memory core on the recall task and let it answer, decision by decision, with
-    sampled answers: {"loss": first and last, "accuracy": of the sampled answers}. An error that
+    sampled answers: {"loss": first and last, "accuracy": of the sampled answers}. The objective is the
+    asked-for answers' cross-entropy ("answers") or what the core's own sampled answers earn ("policy": 1 for a right one,
+    ``epochs`` updates of ``ops.rl.policy_loss`` for each batch of rows). An error that
     a kernel reported (a wait that ran out, an index out of range) is raised every 25 iterations
     and at the end."""
+    from ..ops import rl as R
     from ..ops.gemm import check_error_flag
-    from ..ops.rl import Adam
+    from ..ops.tokens import sample_tokens, sample_tokens_reference
+    if objective not in ("answers", "policy"):
+        raise ValueError(f"objective must be answers or policy, not {objective!r}")
     dev = torch.device(device)
     net = MemoryNet(cfg or MemoryConfig(), dev, seed)
     c = net.cfg
-    opt = Adam(net, lr=lr, max_norm=1.0)
+    opt = R.Adam(net, lr=lr, max_norm=1.0)
     task = RecallTask(envs, c.answers, longest, c.features, seed)
     state = MemoryState(net, envs)
     gpu = dev.type == "cuda"
+    draws = torch.Generator().manual_seed(seed)
+    sample = sample_tokens if gpu else sample_tokens_reference
     losses = []
     for it in range(iterations):
         x, r, t = (torch.as_tensor(v, device=dev) for v in task.rows(length))
-        asked = t >= 0
-        count = asked.sum().clamp(min=1)
-        if gpu:
-            logits, cache = forward_sequence(net, x.bfloat16(), state, r)
-        else:
-            params = net.autograd_params()
-            logits, conv, scan = net.forward_reference(x, state, r, params)
-            state.conv, state.scan = conv.detach(), scan.detach()
-        lsm = torch.log_softmax(logits[..., :c.answers].float(), -1)
-        target = t.clamp(min=0)[..., None]
-        loss = -(lsm.gather(-1, target)[..., 0] * asked).sum() / count
-        if gpu:
-            d = torch.zeros_like(logits)
-            d[..., :c.answers] = lsm.exp()
-            d.scatter_add_(-1, target, torch.full_like(lsm[..., :1], -1.0))
-            backward(net, cache, (d * (asked[..., None] / count)).bfloat16())
-        else:
-            loss.backward()
-            net.collect_grads(params)
-        opt.step()
+        began, answered = (state.conv, state.scan), None
+        for epoch in range(epochs if objective == "policy" else 1):
+            state.conv, state.scan = began
+            if gpu:
+                logits, cache = forward_sequence(net, x.bfloat16(), state, r)
+            else:
+                params = net.autograd_params()
+                logits, conv, scan = net.forward_reference(x, state, r, params)
+                state.conv, state.scan = conv.detach(), scan.detach()
+            if objective == "answers":
+                loss, d = _answers_gradient(logits, t, c)
+            else:
+                if answered is None:
+                    answered = _Answered(logits, t, c, torch.rand(t.numel(), 1, generator=draws).to(dev), sample)
+                z = logits.reshape(-1, c.out_pad)[:, :c.answers]
+                if gpu:
+                    d = torch.zeros_like(logits)
+                    loss = R.policy_loss(z, answered.answers, answered.logp, answered.advantages, out=d.view(-1, c.out_pad)[:, :c.answers],
+                                         **answered.options()).loss
+                else:
+                    loss = R.policy_loss_reference(z, answered.answers, answered.logp, answered.advantages, **answered.options())
+            if gpu:
+                backward(net, cache, d.bfloat16())
+            else:
+                loss.backward()
+                net.collect_grads(params)
+            opt.step()
         losses.append(loss.detach())
         if gpu and (it + 1) % 25 == 0:
             check_error_flag(dev)
         if log is not None and (it + 1) % 25 == 0:
-            log(f"iteration {it + 1}: loss {float(loss):.4f}")
+            share = "" if answered is None else f", {float(answered.right):.3f} of the answers right"
+            log(f"iteration {it + 1}: loss {float(loss):.4f}{share}")
     right = asked_n = 0
     state, task = MemoryState(net, envs), RecallTask(envs, c.answers, longest, c.features, seed + 1)
     gen = torch.Generator().manual_seed(seed)
@@ -310,7 +451,6 @@ def train_recall(iterations: int = 400, envs: int = 128, length: int = 64, cfg: 
         if gpu:
             answer, _ = act(net, x.bfloat16(), state, u.to(dev), reset=r, temperature=temperature, top_p=top_p)
         else:
-            from ..ops.tokens import sample_tokens_reference
             with torch.no_grad():
                 logits, state.conv, state.scan = net.forward_reference(x[:, None], state, r[:, None])
             answer = sample_tokens_reference(logits[:, 0, :c.answers], u, temperature=temperature, top_p=top_p)[0][:, 0]
