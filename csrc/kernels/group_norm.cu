@@ -43,25 +43,79 @@ struct NormArgs {
 };
 static_assert(sizeof(NormArgs) == 9 * 8 + 8 * 8 + 6 * 4 + 8, "as the caller packs it");
 
-__device__ __forceinline__ float act_of(float v, int act) {
-  if (act == kSilu) return v * sigmoid(v);
-  return act == kRelu ? fmaxf(v, 0.0f) : v;
-}
-__device__ __forceinline__ float slope_of(float v, int act) {
-  if (act == kSilu) {
-    const float s = sigmoid(v);
-    return s * fmaf(v, 1.0f - s, 1.0f);
+// V numbers; from two on in pairs, one instruction for both.
+template <int V> struct Nums {
+  f2 p[V / 2];
+  template <typename F> __device__ __forceinline__ static Nums of(F f) {
+    Nums r;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = f(i);
+    return r;
   }
-  return act == kRelu && !(v > 0.0f) ? 0.0f : 1.0f;
+  __device__ __forceinline__ static Nums all(float x) { return of([&](int) { return pack2(x, x); }); }
+  __device__ __forceinline__ static Nums get(const float (&v)[V]) { return of([&](int i) { return pack2(v[2 * i], v[2 * i + 1]); }); }
+  __device__ __forceinline__ void put(float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) unpack2(p[i], v[2 * i], v[2 * i + 1]);
+  }
+  template <typename F> __device__ __forceinline__ Nums each(F f) const {
+    return of([&](int i) {
+      float a, b;
+      unpack2(p[i], a, b);
+      return pack2(f(a), f(b));
+    });
+  }
+  __device__ __forceinline__ float sum() const {
+    f2 s = p[0];
+#pragma unroll
+    for (int i = 1; i < V / 2; ++i) s = add2(s, p[i]);
+    float a, b;
+    unpack2(s, a, b);
+    return a + b;
+  }
+};
+template <> struct Nums<1> {
+  float p;
+  __device__ __forceinline__ static Nums all(float x) { return {x}; }
+  __device__ __forceinline__ static Nums get(const float (&v)[1]) { return {v[0]}; }
+  __device__ __forceinline__ void put(float (&v)[1]) const { v[0] = p; }
+  template <typename F> __device__ __forceinline__ Nums each(F f) const { return {f(p)}; }
+  __device__ __forceinline__ float sum() const { return p; }
+};
+template <int V> __device__ __forceinline__ Nums<V> operator+(const Nums<V>& a, const Nums<V>& b) {
+  if constexpr (V == 1) return {a.p + b.p};
+  else return Nums<V>::of([&](int i) { return add2(a.p[i], b.p[i]); });
 }
-// relu as torch's: NaN stays
-__device__ __forceinline__ float apply(float x, float mean, float rstd, float w, float b, int act) {
-  const float pre = fmaf((x - mean) * rstd, w, b);
-  return act == kRelu && !(pre > 0.0f) ? (pre == pre ? 0.0f : pre) : act_of(pre, act);
+template <int V> __device__ __forceinline__ Nums<V> operator*(const Nums<V>& a, const Nums<V>& b) {
+  if constexpr (V == 1) return {a.p * b.p};
+  else return Nums<V>::of([&](int i) { return mul2(a.p[i], b.p[i]); });
 }
-__device__ __forceinline__ float gradient(float x, float dy, float mean, float rstd, float w, float b, int act, float& xh) {
-  xh = (x - mean) * rstd;
-  return act == kNone ? dy : dy * slope_of(fmaf(xh, w, b), act);
+template <int V> __device__ __forceinline__ Nums<V> fma(const Nums<V>& a, const Nums<V>& b, const Nums<V>& c) {
+  if constexpr (V == 1) return {fmaf(a.p, b.p, c.p)};
+  else return Nums<V>::of([&](int i) { return fma2(a.p[i], b.p[i], c.p[i]); });
+}
+template <int V> __device__ __forceinline__ Nums<V> sigmoid_of(const Nums<V>& v) {
+  return ((v * Nums<V>::all(-kLog2e)).each([](float x) { return exp2_hw(x); }) + Nums<V>::all(1.0f)).each([](float x) { return rcp_hw(x); });
+}
+
+// act(xh w + b) with xh = (x - mean) rstd; NaN stays under relu
+template <int V>
+__device__ __forceinline__ Nums<V> apply(const Nums<V>& x, float mean, float rstd, const Nums<V>& w, const Nums<V>& b, int act) {
+  const Nums<V> pre = fma((x + Nums<V>::all(-mean)) * Nums<V>::all(rstd), w, b);
+  if (act == kSilu) return pre * sigmoid_of(pre);
+  return act == kRelu ? pre.each([](float v) { return v < 0.0f ? 0.0f : v; }) : pre;
+}
+// dy act'(pre)
+template <int V>
+__device__ __forceinline__ Nums<V> gradient(const Nums<V>& x, const Nums<V>& dy, float mean, float rstd, const Nums<V>& w, const Nums<V>& b,
+                                            int act, Nums<V>& xh) {
+  const Nums<V> one = Nums<V>::all(1.0f);
+  xh = (x + Nums<V>::all(-mean)) * Nums<V>::all(rstd);
+  if (act == kNone) return dy;
+  const Nums<V> pre = fma(xh, w, b);
+  if (act == kRelu) return dy * pre.each([](float v) { return v > 0.0f ? 1.0f : 0.0f; });
+  const Nums<V> s = sigmoid_of(pre);
+  return dy * (s * fma(pre, fma(s, Nums<V>::all(-1.0f), one), one));
 }
 
 // (count, mean, sum of squares about it) of two sets
@@ -94,7 +148,8 @@ template <typename T, int V> struct Piece {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = 0;
   }
-  __device__ __forceinline__ void get(float (&v)[V]) const {
+  __device__ __forceinline__ Nums<V> get() const {
+    float v[V];
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = __uint_as_float(w[i]);
@@ -107,16 +162,30 @@ template <typename T, int V> struct Piece {
         v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
       }
     }
+    return Nums<V>::get(v);
   }
 };
+template <typename T, int V> __device__ __forceinline__ void store(T* p, const Nums<V>& x) {
+  float v[V];
+  x.put(v);
+  store_vec<T, V>(p, v);
+}
+template <typename T, int V> __device__ __forceinline__ Nums<V> load(const T* p) {
+  Piece<T, V> r;
+  r.load(p);
+  return r.get();
+}
 template <int V> struct Weights {
-  float w[V], b[V];
+  Nums<V> w, b;
   __device__ __forceinline__ void load(const float* pw, const float* pb, int c, bool on) {
+    float x[V], y[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      w[j] = pw && on ? pw[c + j] : 1.0f;
-      b[j] = pb && on ? pb[c + j] : 0.0f;
+      x[j] = pw && on ? pw[c + j] : 1.0f;
+      y[j] = pb && on ? pb[c + j] : 0.0f;
     }
+    w = Nums<V>::get(x);
+    b = Nums<V>::get(y);
   }
 };
 
@@ -125,11 +194,11 @@ constexpr int kLaneThreads = 256;
 
 // L lanes for a (sample, group): lane l holds pieces l, l + L, ... of at most H L; piece q is position
 // q / (pieces of a group), whose channels follow. A block's warps take the samples of one set of
-// 32 / L groups in turn, two at a time where a lane has one piece, so that a lane's channels stay
+// 32 / L groups in turn, several at a time where a lane has one piece, so that a lane's channels stay
 // the same and their sums stay in registers.
 template <typename T, int V, int L, int H, bool kGrad>
 __global__ void __launch_bounds__(kLaneThreads) norm_lanes(NormArgs a) {
-  constexpr int kSets = 32 / L, kWarps = kLaneThreads / 32, U = H == 1 ? 2 : 1;
+  constexpr int kSets = 32 / L, kWarps = kLaneThreads / 32, U = H == 1 ? (kGrad ? 2 : 4) : 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L;
   const int gi = blockIdx.x * kSets + lane / L, cg = a.c / a.g, per = cg / V;
   const int items = static_cast<int>(a.p) * per;
@@ -148,11 +217,13 @@ __global__ void __launch_bounds__(kLaneThreads) norm_lanes(NormArgs a) {
     wb[k].load(a.w, a.b, c, have[k]);
   }
   const float inv = 1.0f / (static_cast<float>(a.p) * cg);
-  float sw[kGrad ? H : 1][V] = {}, sb[kGrad ? H : 1][V] = {};
+  Nums<V> sw[kGrad ? H : 1], sb[kGrad ? H : 1];
+#pragma unroll
+  for (int k = 0; k < (kGrad ? H : 1); ++k) sw[k] = sb[k] = Nums<V>::all(0.0f);
   const int64_t step = static_cast<int64_t>(gridDim.y) * kWarps;
   for (int64_t n0 = static_cast<int64_t>(blockIdx.y) * kWarps + warp; n0 < a.n; n0 += U * step) {
     Piece<T, V> rx[U][H], rd[U][H];
-    float mean[U], rstd[U];
+    float2 st[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t n = n0 + u * step;
@@ -166,12 +237,8 @@ __global__ void __launch_bounds__(kLaneThreads) norm_lanes(NormArgs a) {
           else rd[u][k].zero();
         }
       }
-      mean[u] = rstd[u] = 0.0f;
-      if (kGrad && live && on) {
-        const float2 st = *reinterpret_cast<const float2*>(a.stats + (n * a.g + gi) * 2);
-        mean[u] = st.x;
-        rstd[u] = st.y;
-      }
+      st[u] = make_float2(0.0f, 0.0f);
+      if (kGrad && live && on) st[u] = *reinterpret_cast<const float2*>(a.stats + (n * a.g + gi) * 2);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -181,62 +248,36 @@ __global__ void __launch_bounds__(kLaneThreads) norm_lanes(NormArgs a) {
       if constexpr (!kGrad) {
         float s = 0.0f, q = 0.0f;
 #pragma unroll
-        for (int k = 0; k < H; ++k) {
-          float v[V];
-          rx[u][k].get(v);
-#pragma unroll
-          for (int j = 0; j < V; ++j) s += v[j];
-        }
-        const float m = lanes_sum<L>(s) * inv;
+        for (int k = 0; k < H; ++k) s += rx[u][k].get().sum();
+        const float mean = lanes_sum<L>(s) * inv;
 #pragma unroll
         for (int k = 0; k < H; ++k) {
-          float v[V];
-          rx[u][k].get(v);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float d = v[j] - m;
-            if (have[k]) q = fmaf(d, d, q);
-          }
+          const Nums<V> d = rx[u][k].get() + Nums<V>::all(-mean);
+          if (have[k]) q += (d * d).sum();
         }
-        const float r = rsqrtf(lanes_sum<L>(q) * inv + a.eps);
-        if (a.stats && live && on && l == 0) *reinterpret_cast<float2*>(a.stats + (n * a.g + gi) * 2) = make_float2(m, r);
+        const float rstd = rsqrtf(lanes_sum<L>(q) * inv + a.eps);
+        if (a.stats && live && on && l == 0) *reinterpret_cast<float2*>(a.stats + (n * a.g + gi) * 2) = make_float2(mean, rstd);
 #pragma unroll
-        for (int k = 0; k < H; ++k) {
-          if (!live || !have[k]) continue;
-          float v[V];
-          rx[u][k].get(v);
-#pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = apply(v[j], m, r, wb[k].w[j], wb[k].b[j], a.act);
-          store_vec<T, V>(y + yo[k], v);
-        }
+        for (int k = 0; k < H; ++k)
+          if (live && have[k]) store<T, V>(y + yo[k], apply<V>(rx[u][k].get(), mean, rstd, wb[k].w, wb[k].b, a.act));
       } else {
-        float xh[H][V], d[H][V], s1 = 0.0f, s2 = 0.0f;
+        // pieces that are not there have dy = 0
+        Nums<V> xh[H], d[H];
+        float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int k = 0; k < H; ++k) {
-          float v[V], e[V];
-          rx[u][k].get(v);
-          rd[u][k].get(e);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float g = gradient(v[j], e[j], mean[u], rstd[u], wb[k].w[j], wb[k].b[j], a.act, xh[k][j]);
-            if (live && have[k]) {
-              sw[k][j] = fmaf(g, xh[k][j], sw[k][j]);
-              sb[k][j] += g;
-            }
-            d[k][j] = have[k] ? g * wb[k].w[j] : 0.0f;
-            s1 += d[k][j];
-            s2 = fmaf(d[k][j], xh[k][j], s2);
-          }
+          const Nums<V> e = gradient<V>(rx[u][k].get(), rd[u][k].get(), st[u].x, st[u].y, wb[k].w, wb[k].b, a.act, xh[k]);
+          sw[k] = fma(e, xh[k], sw[k]);
+          sb[k] = sb[k] + e;
+          d[k] = e * wb[k].w;
+          s1 += d[k].sum();
+          s2 += (d[k] * xh[k]).sum();
         }
         const float m1 = lanes_sum<L>(s1) * inv, m2 = lanes_sum<L>(s2) * inv;
 #pragma unroll
-        for (int k = 0; k < H; ++k) {
-          if (!live || !have[k]) continue;
-          float v[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = rstd[u] * (d[k][j] - fmaf(xh[k][j], m2, m1));
-          store_vec<T, V>(y + yo[k], v);
-        }
+        for (int k = 0; k < H; ++k)
+          if (live && have[k])
+            store<T, V>(y + yo[k], (d[k] + fma(xh[k], Nums<V>::all(-m2), Nums<V>::all(-m1))) * Nums<V>::all(st[u].y));
       }
     }
   }
@@ -249,9 +290,12 @@ __global__ void __launch_bounds__(kLaneThreads) norm_lanes(NormArgs a) {
     for (int turn = 0; turn < 2; ++turn) {
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < H; ++k)
+      for (int k = 0; k < H; ++k) {
+        float v[V];
+        (turn ? sb[k] : sw[k]).put(v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[warp][(lane / L * L * H + l + k * L) * V + j] = turn ? sb[k][j] : sw[k][j];
+        for (int j = 0; j < V; ++j) sum[warp][(lane / L * L * H + l + k * L) * V + j] = v[j];
+      }
       __syncthreads();
       for (int c = threadIdx.x; c < width; c += kLaneThreads) {
         const int set = c / cg, in = c - set * cg;
@@ -307,123 +351,147 @@ struct Place {
   }
 };
 
-// Slabs (the faster index, so that a sample's are read together) of samples.
+// A thread's pieces of a sample on their way to places of its own in shared memory, a sample ahead;
+// pieces of two bytes are loaded when they are needed.
+template <typename T, int V, int H> struct Ahead {
+  static constexpr int kBytes = V * static_cast<int>(sizeof(T));
+  static constexpr bool kAsync = kBytes >= 4;
+  static __device__ __forceinline__ void copy(char* to, const T* from, int64_t step, int count) {
+    if constexpr (kAsync) {
+#pragma unroll
+      for (int k = 0; k < H; ++k)
+        if (k < count) {
+          const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to + static_cast<size_t>(k * blockDim.x) * kBytes));
+          if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from + k * step) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from + k * step), "n"(kBytes) : "memory");
+        }
+    }
+  }
+  static __device__ __forceinline__ void take(Piece<T, V> (&r)[H], const char* from, const T* memory, int64_t step, int count) {
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      if (k >= count) r[k].zero();
+      else if constexpr (kAsync) r[k].load(reinterpret_cast<const T*>(from + static_cast<size_t>(k * blockDim.x) * kBytes));
+      else r[k].load(memory + k * step);
+    }
+  }
+};
+
+// A slab of samples blockIdx.x / slabs, + gridDim.x / slabs, ... (slabs are the faster index, so that a
+// sample's are read together); the next sample is on its way while one is normalised.
 template <typename T, int V, int H> __global__ void __launch_bounds__(kBlockThreads) norm_block(NormArgs a) {
+  using A = Ahead<T, V, H>;
+  extern __shared__ __align__(16) char smem[];
   __shared__ float red[kBlockThreads], res[kBlockThreads];
   const int slabs = (a.g + a.slab - 1) / a.slab;
   const Place at(a, blockIdx.x % slabs, V);
-  const int64_t n = blockIdx.x / slabs;
+  const int64_t blocks = gridDim.x / slabs;
   const float inv = 1.0f / (static_cast<float>(a.p) * (a.c / a.g));
   const int count = at.on ? max(0, static_cast<int>((a.p - at.row + at.rows - 1) / at.rows)) : 0;       // this thread's pieces
-  Piece<T, V> r[H];
-  const T* x = static_cast<const T*>(a.x) + n * a.xs_n + at.row * a.xs_p + at.c0;
-#pragma unroll
-  for (int k = 0; k < H; ++k) {
-    if (k < count) r[k].load(x + k * (at.rows * a.xs_p));
-    else r[k].zero();
-  }
+  const T* x = static_cast<const T*>(a.x) + at.row * a.xs_p + at.c0;
+  const int64_t step = at.rows * a.xs_p;
+  char* mine = smem + threadIdx.x * A::kBytes;
+  const size_t turn = static_cast<size_t>(H) * blockDim.x * A::kBytes;
   Weights<V> wb;
   wb.load(a.w, a.b, at.c0, at.on);
-  float s = 0.0f;
+  const int64_t first = blockIdx.x / slabs;
+  if (first < a.n) A::copy(mine, x + first * a.xs_n, step, count);
+  cp_async_commit();
+  int odd = 0;
+  for (int64_t n = first; n < a.n; n += blocks, odd ^= 1) {
+    if (n + blocks < a.n) A::copy(mine + (odd ^ 1) * turn, x + (n + blocks) * a.xs_n, step, count);
+    cp_async_commit();
+    cp_async_wait<1>();
+    Piece<T, V> r[H];
+    A::take(r, mine + odd * turn, x + n * a.xs_n, step, count);
+    Nums<V> s = Nums<V>::all(0.0f);
 #pragma unroll
-  for (int k = 0; k < H; ++k) {
-    float v[V];
-    r[k].get(v);
+    for (int k = 0; k < H; ++k) s = s + r[k].get();
+    sum_groups(s.sum(), red, res, at.groups, at.per, at.per_group, at.walkers);
+    const float mean = res[at.own] * inv;
+    s = Nums<V>::all(0.0f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) s += v[j];
-  }
-  sum_groups(s, red, res, at.groups, at.per, at.per_group, at.walkers);
-  const float mean = res[at.own] * inv;
-  s = 0.0f;
+    for (int k = 0; k < H; ++k)
+      if (k < count) {
+        const Nums<V> d = r[k].get() + Nums<V>::all(-mean);
+        s = fma(d, d, s);
+      }
+    sum_groups(s.sum(), red, res, at.groups, at.per, at.per_group, at.walkers);
+    const float rstd = rsqrtf(res[at.own] * inv + a.eps);
+    if (a.stats && at.on && at.row == 0 && at.piece % at.per_group == 0)
+      *reinterpret_cast<float2*>(a.stats + (n * a.g + at.g0 + at.own) * 2) = make_float2(mean, rstd);
+    T* y = static_cast<T*>(a.y) + n * a.ys_n + at.row * a.ys_p + at.c0;
 #pragma unroll
-  for (int k = 0; k < H; ++k) {
-    float v[V];
-    r[k].get(v);
-    if (k < count)
-#pragma unroll
-      for (int j = 0; j < V; ++j) s = fmaf(v[j] - mean, v[j] - mean, s);
-  }
-  sum_groups(s, red, res, at.groups, at.per, at.per_group, at.walkers);
-  const float rstd = rsqrtf(res[at.own] * inv + a.eps);
-  if (a.stats && at.on && at.row == 0 && at.piece % at.per_group == 0)
-    *reinterpret_cast<float2*>(a.stats + (n * a.g + at.g0 + at.own) * 2) = make_float2(mean, rstd);
-  T* y = static_cast<T*>(a.y) + n * a.ys_n + at.row * a.ys_p + at.c0;
-#pragma unroll
-  for (int k = 0; k < H; ++k) {
-    if (k >= count) continue;
-    float v[V];
-    r[k].get(v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = apply(v[j], mean, rstd, wb.w[j], wb.b[j], a.act);
-    store_vec<T, V>(y + k * (at.rows * a.ys_p), v);
+    for (int k = 0; k < H; ++k)
+      if (k < count) store<T, V>(y + k * (at.rows * a.ys_p), apply<V>(r[k].get(), mean, rstd, wb.w, wb.b, a.act));
   }
 }
 
-// Gradient of a slab of samples blockIdx.x / slabs, + gridDim.x / slabs, ...
+// Its gradient, x and dy a sample ahead.
 template <typename T, int V, int H> __global__ void __launch_bounds__(kBlockThreads / 2, 2) norm_block_grad(NormArgs a) {
-  __shared__ float red[kBlockThreads], res[kBlockThreads];
+  using A = Ahead<T, V, H>;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float red[kBlockThreads / 2], res[kBlockThreads / 2];
   const int slabs = (a.g + a.slab - 1) / a.slab, blocks = gridDim.x / slabs, block = blockIdx.x / slabs;
   const Place at(a, blockIdx.x % slabs, V);
   const float inv = 1.0f / (static_cast<float>(a.p) * (a.c / a.g));
   const int count = at.on ? max(0, static_cast<int>((a.p - at.row + at.rows - 1) / at.rows)) : 0;
+  const T* x = static_cast<const T*>(a.x) + at.row * a.xs_p + at.c0;
+  const T* dy = static_cast<const T*>(a.dy) + at.row * a.ds_p + at.c0;
+  const int64_t xstep = at.rows * a.xs_p, dstep = at.rows * a.ds_p;
+  char* mine = smem + threadIdx.x * A::kBytes;
+  const size_t half = static_cast<size_t>(H) * blockDim.x * A::kBytes, turn = 2 * half;
   Weights<V> wb;
   wb.load(a.w, a.b, at.c0, at.on);
-  float sw[V] = {}, sb[V] = {};
-  for (int64_t n = block; n < a.n; n += blocks) {
-    Piece<T, V> rx[H], rd[H];
-    const T* x = static_cast<const T*>(a.x) + n * a.xs_n + at.row * a.xs_p + at.c0;
-    const T* dy = static_cast<const T*>(a.dy) + n * a.ds_n + at.row * a.ds_p + at.c0;
-#pragma unroll
-    for (int k = 0; k < H; ++k) {
-      if (k < count) {
-        rx[k].load(x + k * (at.rows * a.xs_p));
-        rd[k].load(dy + k * (at.rows * a.ds_p));
-      } else {
-        rx[k].zero();
-        rd[k].zero();
-      }
+  Nums<V> sw = Nums<V>::all(0.0f), sb = sw;
+  if (block < a.n) {
+    A::copy(mine, x + block * a.xs_n, xstep, count);
+    A::copy(mine + half, dy + block * a.ds_n, dstep, count);
+  }
+  cp_async_commit();
+  int odd = 0;
+  for (int64_t n = block; n < a.n; n += blocks, odd ^= 1) {
+    if (n + blocks < a.n) {
+      A::copy(mine + (odd ^ 1) * turn, x + (n + blocks) * a.xs_n, xstep, count);
+      A::copy(mine + (odd ^ 1) * turn + half, dy + (n + blocks) * a.ds_n, dstep, count);
     }
+    cp_async_commit();
     const float2 st = *reinterpret_cast<const float2*>(a.stats + (n * a.g + at.g0 + at.own) * 2);
-    float xh[H][V], d[H][V], s1 = 0.0f, s2 = 0.0f;
+    cp_async_wait<1>();
+    Piece<T, V> rx[H], rd[H];
+    A::take(rx, mine + odd * turn, x + n * a.xs_n, xstep, count);
+    A::take(rd, mine + odd * turn + half, dy + n * a.ds_n, dstep, count);
+    Nums<V> xh[H], d[H], s1 = Nums<V>::all(0.0f), s2 = s1;       // pieces that are not there have dy = 0
 #pragma unroll
     for (int k = 0; k < H; ++k) {
-      float v[V], e[V];
-      rx[k].get(v);
-      rd[k].get(e);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float g = gradient(v[j], e[j], st.x, st.y, wb.w[j], wb.b[j], a.act, xh[k][j]);
-        if (k < count) {
-          sw[j] = fmaf(g, xh[k][j], sw[j]);
-          sb[j] += g;
-        }
-        d[k][j] = k < count ? g * wb.w[j] : 0.0f;
-        s1 += d[k][j];
-        s2 = fmaf(d[k][j], xh[k][j], s2);
-      }
+      const Nums<V> e = gradient<V>(rx[k].get(), rd[k].get(), st.x, st.y, wb.w, wb.b, a.act, xh[k]);
+      sw = fma(e, xh[k], sw);
+      sb = sb + e;
+      d[k] = e * wb.w;
+      s1 = s1 + d[k];
+      s2 = fma(d[k], xh[k], s2);
     }
-    sum_groups(s1, red, res, at.groups, at.per, at.per_group, at.walkers);
+    sum_groups(s1.sum(), red, res, at.groups, at.per, at.per_group, at.walkers);
     const float m1 = res[at.own] * inv;
-    sum_groups(s2, red, res, at.groups, at.per, at.per_group, at.walkers);
+    sum_groups(s2.sum(), red, res, at.groups, at.per, at.per_group, at.walkers);
     const float m2 = res[at.own] * inv;
     T* y = static_cast<T*>(a.y) + n * a.ys_n + at.row * a.ys_p + at.c0;
 #pragma unroll
-    for (int k = 0; k < H; ++k) {
-      if (k >= count) continue;
-      float v[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = st.y * (d[k][j] - fmaf(xh[k][j], m2, m1));
-      store_vec<T, V>(y + k * (at.rows * a.ys_p), v);
-    }
+    for (int k = 0; k < H; ++k)
+      if (k < count)
+        store<T, V>(y + k * (at.rows * a.ys_p), (d[k] + fma(xh[k], Nums<V>::all(-m2), Nums<V>::all(-m1))) * Nums<V>::all(st.y));
   }
   // the channels' sums, the block's rows in order
   float* out = a.part + static_cast<int64_t>(block) * 2 * a.c + at.c0 - at.piece * V;
+  float both[2][V];
+  sw.put(both[0]);
+  sb.put(both[1]);
 #pragma unroll
   for (int j = 0; j < V; ++j)
 #pragma unroll
     for (int turn = 0; turn < 2; ++turn) {
       __syncthreads();
-      red[threadIdx.x] = at.on ? (turn ? sb[j] : sw[j]) : 0.0f;
+      red[threadIdx.x] = at.on ? both[turn][j] : 0.0f;
       __syncthreads();
       if (static_cast<int>(threadIdx.x) < at.per) {
         float s = 0.0f;
@@ -456,23 +524,16 @@ template <typename T, int V> __global__ void __launch_bounds__(kBlockThreads) no
     }
   };
   const int group_pieces = wide ? 1 : at.per_group, row_pieces = wide ? 1 : at.per, own = wide ? 0 : at.own;
-  float s = 0.0f;
-  each([&](const T* from) {
-    float v[V];
-    load_vec<T, V>(from, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) s += v[j];
-  });
-  sum_groups(s, red, res, at.groups, row_pieces, group_pieces, walkers);
+  Nums<V> s = Nums<V>::all(0.0f);
+  each([&](const T* from) { s = s + load<T, V>(from); });
+  sum_groups(s.sum(), red, res, at.groups, row_pieces, group_pieces, walkers);
   const float mean = res[own] * inv;
-  s = 0.0f;
+  s = Nums<V>::all(0.0f);
   each([&](const T* from) {
-    float v[V];
-    load_vec<T, V>(from, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) s = fmaf(v[j] - mean, v[j] - mean, s);
+    const Nums<V> d = load<T, V>(from) + Nums<V>::all(-mean);
+    s = fma(d, d, s);
   });
-  sum_groups(s, red, res, at.groups, row_pieces, group_pieces, walkers);
+  sum_groups(s.sum(), red, res, at.groups, row_pieces, group_pieces, walkers);
   if (wide ? threadIdx.x == 0 : at.on && at.row == 0 && at.piece % at.per_group == 0) {
     float* out = a.part + ((n * a.g + at.g0 + own) * a.parts + part) * 3;
     out[0] = static_cast<float>(last - first) * cg;
@@ -513,11 +574,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kBlockThreads) no
   const T* x = static_cast<const T*>(a.x) + n * a.xs_n + at.g0 * cg;
   T* y = static_cast<T*>(a.y) + n * a.ys_n + at.g0 * cg;
   auto one = [&](int64_t p, int i, const Weights<V>& wb) {
-    float v[V];
-    load_vec<T, V>(x + p * a.xs_p + i * V, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = apply(v[j], m.x, m.y, wb.w[j], wb.b[j], a.act);
-    store_vec<T, V>(y + p * a.ys_p + i * V, v);
+    store<T, V>(y + p * a.ys_p + i * V, apply<V>(load<T, V>(x + p * a.xs_p + i * V), m.x, m.y, wb.w, wb.b, a.act));
   };
   Weights<V> wb;
   if (wide) {
@@ -543,39 +600,31 @@ template <typename T, int V> __global__ void __launch_bounds__(kPartThreads) nor
   // 32 pieces of channels by 8 rows of positions
   const int col = (blockIdx.y * 32 + (threadIdx.x & 31)) * V, row = threadIdx.x >> 5;
   const bool on = col < a.c;
-  float sw[V], sb[V], w[V], b[V], mean = 0.0f, rstd = 0.0f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    sw[j] = sb[j] = 0.0f;
-    w[j] = a.w && on ? a.w[col + j] : 1.0f;
-    b[j] = a.b && on ? a.b[col + j] : 0.0f;
-  }
+  Nums<V> sw = Nums<V>::all(0.0f), sb = sw;
+  Weights<V> wb;
+  wb.load(a.w, a.b, col, on);
   if (on) {
-    mean = a.stats[(n * a.g + col / cg) * 2];
-    rstd = a.stats[(n * a.g + col / cg) * 2 + 1];
+    const float2 st = *reinterpret_cast<const float2*>(a.stats + (n * a.g + col / cg) * 2);
     const T* x = static_cast<const T*>(a.x) + n * a.xs_n + col;
     const T* dy = static_cast<const T*>(a.dy) + n * a.ds_n + col;
 #pragma unroll 2
     for (int64_t p = first + row; p < last; p += 8) {
-      float v[V], d[V];
-      load_vec<T, V>(x + p * a.xs_p, v);
-      load_vec<T, V>(dy + p * a.ds_p, d);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float xh;
-        const float e = gradient(v[j], d[j], mean, rstd, w[j], b[j], a.act, xh);
-        sw[j] = fmaf(e, xh, sw[j]);
-        sb[j] += e;
-      }
+      Nums<V> xh;
+      const Nums<V> e = gradient<V>(load<T, V>(x + p * a.xs_p), load<T, V>(dy + p * a.ds_p), st.x, st.y, wb.w, wb.b, a.act, xh);
+      sw = fma(e, xh, sw);
+      sb = sb + e;
     }
   }
+  float both[2][V];
+  sw.put(both[0]);
+  sb.put(both[1]);
   float* out = a.part + blockIdx.x * static_cast<int64_t>(2 * a.c);
 #pragma unroll
   for (int j = 0; j < V; ++j)
 #pragma unroll
     for (int turn = 0; turn < 2; ++turn) {
       __syncthreads();
-      red[threadIdx.x] = turn ? sb[j] : sw[j];
+      red[threadIdx.x] = both[turn][j];
       __syncthreads();
       if (row == 0 && on) {
         float s = 0.0f;
@@ -621,28 +670,18 @@ template <typename T, int V> __global__ void __launch_bounds__(kPartThreads) nor
   const int col = (blockIdx.y * 32 + (threadIdx.x & 31)) * V, row = threadIdx.x >> 5;
   if (col >= a.c) return;
   const int64_t at = (n * a.g + col / cg) * 2;
-  const float mean = a.stats[at], rstd = a.stats[at + 1], m1 = means[at], m2 = means[at + 1];
-  float w[V], b[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    w[j] = a.w ? a.w[col + j] : 1.0f;
-    b[j] = a.b ? a.b[col + j] : 0.0f;
-  }
+  const float2 st = *reinterpret_cast<const float2*>(a.stats + at);
+  const float m1 = means[at], m2 = means[at + 1];
+  Weights<V> wb;
+  wb.load(a.w, a.b, col, true);
   const T* x = static_cast<const T*>(a.x) + n * a.xs_n + col;
   const T* dy = static_cast<const T*>(a.dy) + n * a.ds_n + col;
   T* y = static_cast<T*>(a.y) + n * a.ys_n + col;
 #pragma unroll 2
   for (int64_t p = first + row; p < last; p += 8) {
-    float v[V], d[V];
-    load_vec<T, V>(x + p * a.xs_p, v);
-    load_vec<T, V>(dy + p * a.ds_p, d);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float xh;
-      const float e = gradient(v[j], d[j], mean, rstd, w[j], b[j], a.act, xh);
-      v[j] = rstd * (e * w[j] - fmaf(xh, m2, m1));
-    }
-    store_vec<T, V>(y + p * a.ys_p, v);
+    Nums<V> xh;
+    const Nums<V> e = gradient<V>(load<T, V>(x + p * a.xs_p), load<T, V>(dy + p * a.ds_p), st.x, st.y, wb.w, wb.b, a.act, xh);
+    store<T, V>(y + p * a.ys_p, (e * wb.w + fma(xh, Nums<V>::all(-m2), Nums<V>::all(-m1))) * Nums<V>::all(st.y));
   }
 }
 
@@ -713,11 +752,17 @@ template <typename T, int V> int forward(const NormArgs& a, int mode, int lanes,
   const int slabs = (a.g + a.slab - 1) / a.slab;
   if (threads > kBlockThreads || threads % 32) return static_cast<int>(cudaErrorInvalidValue);
   if (mode == 1) {
-    const unsigned grid = static_cast<unsigned>(a.n * slabs);
-    if (hold == 2) norm_block<T, V, 2><<<grid, threads, 0, s>>>(a);
-    else if (hold == 4) norm_block<T, V, 4><<<grid, threads, 0, s>>>(a);
-    else if (hold == 8) norm_block<T, V, 8><<<grid, threads, 0, s>>>(a);
-    else return static_cast<int>(cudaErrorInvalidValue);
+    auto go = [&](auto h) {
+      constexpr int H = decltype(h)::value;
+      const size_t bytes = 2 * static_cast<size_t>(H) * threads * V * sizeof(T);       // this sample's and the next one's
+      if (const int e = allow_smem<norm_block<T, V, H>>(2 * H * kBlockThreads * 16)) return e;
+      norm_block<T, V, H><<<static_cast<unsigned>(blocks) * slabs, threads, bytes, s>>>(a);
+      return static_cast<int>(cudaGetLastError());
+    };
+    if (hold == 2) return go(std::integral_constant<int, 2>());
+    if (hold == 4) return go(std::integral_constant<int, 4>());
+    if (hold == 8) return go(std::integral_constant<int, 8>());
+    return static_cast<int>(cudaErrorInvalidValue);
   } else {
     const dim3 grid(static_cast<unsigned>(a.n * a.parts), slabs);
     norm_part_stats<T, V><<<grid, threads, 0, s>>>(a);
@@ -733,9 +778,16 @@ template <typename T, int V> int backward(const NormArgs& a, int mode, int lanes
   } else if (mode == 1) {
     if (threads > kBlockThreads / 2 || threads % 32) return static_cast<int>(cudaErrorInvalidValue);
     const unsigned grid = static_cast<unsigned>(blocks) * ((a.g + a.slab - 1) / a.slab);
-    if (hold == 2) norm_block_grad<T, V, 2><<<grid, threads, 0, s>>>(a);
-    else if (hold == 4) norm_block_grad<T, V, 4><<<grid, threads, 0, s>>>(a);
-    else return static_cast<int>(cudaErrorInvalidValue);
+    auto go = [&](auto h) {
+      constexpr int H = decltype(h)::value;
+      const size_t bytes = 4 * static_cast<size_t>(H) * threads * V * sizeof(T);
+      if (const int e = allow_smem<norm_block_grad<T, V, H>>(4 * H * kBlockThreads / 2 * 16)) return e;
+      norm_block_grad<T, V, H><<<grid, threads, bytes, s>>>(a);
+      return static_cast<int>(cudaGetLastError());
+    };
+    const int e = hold == 2 ? go(std::integral_constant<int, 2>()) : hold == 4 ? go(std::integral_constant<int, 4>())
+                                                                             : static_cast<int>(cudaErrorInvalidValue);
+    if (e) return e;
   } else {
     rows = a.n * a.parts;
     float* means = a.part + rows * 2 * a.c;

@@ -538,7 +538,7 @@ def build_parser() -> argparse.ArgumentParser:
     rc.add_argument("--keys", type=int, default=32, help="keys of a head of the delta core")
     rc.add_argument("--objective", choices=("answers", "policy"), default="answers",
                     help="the asked-for answers, or what sampled answers earn (clipped policy loss)")
-    rc.add_argument("--lr", type=float, default=1e-2)
+    rc.add_argument("--lr", type=float, default=None, help="1e-2, and 2e-3 for the policy objective")
     rc.add_argument("--temperature", type=float, default=0.5)
     rc.add_argument("--top-p", type=float, default=0.9)
     rc.add_argument("--seed", type=int, default=0)

@@ -384,12 +384,13 @@ class _Answered:
 
 
 def train_recall(iterations: int = 400, envs: int = 128, length: int = 64, cfg: Optional[MemoryConfig] = None, device="cuda",
-                 lr: float = 1e-2, seed: int = 0, longest: int = 48, act_steps: int = 96, temperature: float = 0.5, top_p: float = 0.9,
+                 lr: Optional[float] = None, seed: int = 0, longest: int = 48, act_steps: int = 96, temperature: float = 0.5, top_p: float = 0.9,
                  objective: str = "answers", epochs: int = 2, log=None) -> dict:
     """Train a memory core on the recall task and let it answer, decision by decision, with
     sampled answers: {"loss": first and last, "accuracy": of the sampled answers}. The objective is the
     asked-for answers' cross-entropy ("answers") or what the core's own sampled answers earn ("policy": 1 for a right one,
-    ``epochs`` updates of ``ops.rl.policy_loss`` for each batch of rows). An error that
+    ``epochs`` updates of ``ops.rl.policy_loss`` for each batch of rows); ``lr`` None: 1e-2, and 2e-3 for the
+    policy, whose KL term grows with e^(its step). An error that
     a kernel reported (a wait that ran out, an index out of range) is raised every 25 iterations
     and at the end."""
     from ..ops import rl as R
@@ -400,7 +401,7 @@ def train_recall(iterations: int = 400, envs: int = 128, length: int = 64, cfg: 
     dev = torch.device(device)
     net = MemoryNet(cfg or MemoryConfig(), dev, seed)
     c = net.cfg
-    opt = R.Adam(net, lr=lr, max_norm=1.0)
+    opt = R.Adam(net, lr=lr if lr is not None else 1e-2 if objective == "answers" else 2e-3, max_norm=1.0)
     task = RecallTask(envs, c.answers, longest, c.features, seed)
     state = MemoryState(net, envs)
     gpu = dev.type == "cuda"

@@ -90,11 +90,11 @@ def _plan(n: int, p: int, c: int, g: int, e: int, v: int, grad: bool):
     if items <= 128:
         lanes = min(32, _pow2(items))
         hold = _pow2(-(-items // lanes))
-        blocks = min(-(-n // 8), max(1, 148 * (6 if grad else 24) // -(-g // (32 // lanes))), 65535)
+        blocks = min(-(-n // 8), max(1, 148 * 4 // -(-g // (32 // lanes))), 65535)
         return LANES, lanes, hold, 256, blocks, 1, 1, p
     # the narrowest slab of whole groups with rows of 32 bytes (a sector) that a block's registers
     # take, twice as wide where that still leaves three for every SM
-    threads, most = (256, 4) if grad else (512, 8)
+    threads, most = 256, 4 if grad else 8
     fits = [k for k in range(1, g + 1) if g % k == 0 and k * per_group <= threads and
             -(-p // (threads // (k * per_group))) <= most]
     slab = next((k for k in fits if k * cg * e >= 32), fits[-1] if fits else 0)
@@ -105,7 +105,7 @@ def _plan(n: int, p: int, c: int, g: int, e: int, v: int, grad: bool):
         # no more threads than the pieces take
         threads = -(-min(threads // per, -(-p // hold)) * per // 32) * 32
         hold = max(2, _pow2(-(-p // (threads // per))))
-        return BLOCK, 0, hold, threads, min(n, max(1, 148 * 4 // (g // slab))) if grad else n, slab, 1, p
+        return BLOCK, 0, hold, threads, min(n, max(1, 148 * (2 if grad else 3) // (g // slab))), slab, 1, p
     threads = 256
     slab = max((k for k in range(1, g + 1) if g % k == 0 and k * per_group <= threads), default=1)
     slabs = -(-(c // v) // 32) if grad else g // slab
