@@ -416,43 +416,58 @@ template <typename T, int LK> __global__ void __launch_bounds__(256) delta_step(
   const T* pv = static_cast<const T*>(a.v) + r * a.v_r + h * a.v_h;
   float* state = a.state + (static_cast<int64_t>(slot) * a.heads + h) * a.values * a.keys;
   const bool whole = a.keys % 4 == 0;
-  for (int v0 = 0; v0 < a.values; v0 += kRows) {
-    const int vr = v0 + lane / LK;
-    const bool on = vr < a.values;
-    float* p = state + static_cast<int64_t>(vr) * a.keys + k0;
-    float s[4] = {};
-    if (on && !fresh) {
+  // several rows of the state are on their way before the first is used
+  constexpr int kAhead = 4;
+  for (int v0 = lane / LK; v0 < a.values + lane / LK; v0 += kAhead * kRows) {
+    float s[kAhead][4];
+    float v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int vr = v0 + i * kRows;
+      const float* p = state + vr * a.keys + k0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+      v[i] = 0.0f;
+      if (vr >= a.values) continue;
+      v[i] = to_f(pv[vr]);
+      if (fresh) continue;
       if (whole) {
-        if (k0 < a.keys) *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(p);
+        if (k0 < a.keys) *reinterpret_cast<float4*>(s[i]) = *reinterpret_cast<const float4*>(p);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = k0 + j < a.keys ? p[j] : 0.0f;
+        for (int j = 0; j < 4; ++j)
+          if (k0 + j < a.keys) s[i][j] = p[j];
       }
     }
-    float sk = 0.0f, sq = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j] *= decay;
-      sk = fmaf(s[j], k[j], sk);
-      sq = fmaf(s[j], q[j], sq);
+    for (int i = 0; i < kAhead; ++i) {
+      const int vr = v0 + i * kRows;
+      float* p = state + vr * a.keys + k0;
+      float sk = 0.0f, sq = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] *= decay;
+        sk = fmaf(s[i][j], k[j], sk);
+        sq = fmaf(s[i][j], q[j], sq);
+      }
+#pragma unroll
+      for (int o = LK / 2; o; o >>= 1) {
+        sk += __shfl_xor_sync(0xffffffffu, sk, o);
+        sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      }
+      if (vr >= a.values) continue;
+      const float u = beta * (v[i] - sk);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = fmaf(u, k[j], s[i][j]);
+      if (whole) {
+        if (k0 < a.keys) *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(s[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k0 + j < a.keys) p[j] = s[i][j];
+      }
+      if (l == 0) out[vr] = from_f<T>(a.scale * fmaf(u, kq, sq));
     }
-#pragma unroll
-    for (int o = LK / 2; o; o >>= 1) {
-      sk += __shfl_xor_sync(0xffffffffu, sk, o);
-      sq += __shfl_xor_sync(0xffffffffu, sq, o);
-    }
-    if (!on) continue;
-    const float u = beta * (to_f(pv[vr]) - sk);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = fmaf(u, k[j], s[j]);
-    if (whole) {
-      if (k0 < a.keys) *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(s);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (k0 + j < a.keys) p[j] = s[j];
-    }
-    if (l == 0) out[vr] = from_f<T>(a.scale * fmaf(u, kq, sq));
   }
 }
 
