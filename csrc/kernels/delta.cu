@@ -279,22 +279,31 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
         }
     }
     // the state
-    {
+    if (marks) {                                       // of it the tokens behind the last reset alone are left
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (marks >> (8 * t + col + (e & 1) + 1)) w[t][e] = 0.0f;
+      each([&](float& x, float& y, int, int) { x = y = 0.0f; });
+    } else {
       const float end = c.head[kTile - 1];
+      each([&](float& x, float& y, int, int) {
+        x *= end;
+        y *= end;
+      });
+    }
+    {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const float2 tail = pair(c.tail_k, t), beta = pair(c.beta, t);
         const float fx = tail.x * beta.x, fy = tail.y * beta.y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[t][e] = marks >> (8 * t + col + (e & 1) + 1) ? 0.0f : w[t][e] * (e & 1 ? fy : fx);
+        for (int e = 0; e < 4; ++e) w[t][e] *= e & 1 ? fy : fx;
       }
       Frag<NI> f;
       f.from(w[0], w[1]);
       const uint32_t kt = smem_of(st.tk) + at_cols(lane, Keys::kPitch);
-      each([&](float& x, float& y, int, int) {
-        x = marks ? 0.0f : x * end;
-        y = marks ? 0.0f : y * end;
-      });
       // two steps at a time, so that four sums take turns
 #pragma unroll
       for (int i = 0; i < kSteps; i += 2) {

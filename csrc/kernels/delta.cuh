@@ -68,6 +68,10 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
+// four 8 x 8 tiles, one register of each lane's a tile, to rows of 16 bytes
+__device__ __forceinline__ void stsm4(uint32_t at, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -121,47 +125,20 @@ __device__ __forceinline__ uint32_t a_cols(int lane, int pitch) {
   return (((lane & 16) >> 1) + (lane & 7)) * pitch * 2 + (lane & 8) * 2;
 }
 
-// c0, c1 (columns 0-7 and 8-15) += A B over 16 of k, of the first PA and PB planes; products of
-// planes i and j with i + j >= max(PA, PB) are below what the planes leave out. An accumulator's
-// next product waits 22 cycles for the one before (one may start every 9): products of two
-// split numbers go to sums of their own by i + j.
+// c0, c1 (columns 0-7 and 8-15) += A B over 16 of k, of the first PA and PB planes, smaller products
+// first; products of planes i and j with i + j >= max(PA, PB) are below what the planes leave out.
 template <int PA, int PB, int NA, int NB>
 __device__ __forceinline__ void mma_planes(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
   static_assert(PA <= NA && PB <= NB, "planes that are there");
   constexpr int kLevels = PA > PB ? PA : PB;
-  if constexpr (PA == 1 || PB == 1) {
+#pragma unroll
+  for (int l = kLevels - 1; l >= 0; --l)
 #pragma unroll
     for (int i = 0; i < PA; ++i)
-#pragma unroll
-      for (int j = 0; j < PB; ++j) {
-        mma(c0, a[i], b[j][0], b[j][1]);
-        mma(c1, a[i], b[j][2], b[j][3]);
+      if (l - i >= 0 && l - i < PB) {
+        mma(c0, a[i], b[l - i][0], b[l - i][1]);
+        mma(c1, a[i], b[l - i][2], b[l - i][3]);
       }
-  } else {
-    float l0[kLevels - 1][4] = {}, l1[kLevels - 1][4] = {};
-#pragma unroll
-    for (int i = PA - 1; i >= 0; --i)
-#pragma unroll
-      for (int j = PB - 1; j >= 0; --j)
-        if (i + j < kLevels && i + j > 0) {
-          mma(l0[i + j - 1], a[i], b[j][0], b[j][1]);
-          mma(l1[i + j - 1], a[i], b[j][2], b[j][3]);
-        }
-    mma(c0, a[0], b[0][0], b[0][1]);
-    mma(c1, a[0], b[0][2], b[0][3]);
-#pragma unroll
-    for (int l = kLevels - 2; l > 0; --l)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        l0[l - 1][e] += l0[l][e];
-        l1[l - 1][e] += l1[l][e];
-      }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      c0[e] += l0[0][e];
-      c1[e] += l1[0][e];
-    }
-  }
 }
 // The same for one left operand and two right ones (c += A B, d += A D), planes in turn.
 template <int PC, int PD, int NA, int NB>
@@ -237,6 +214,17 @@ template <typename T> __device__ __forceinline__ float tile_at(const bf16* t, in
 #pragma unroll
   for (int i = 1; i < Planes<T>::kToken; ++i) v += to_f(t[i * plane + at]);
   return v;
+}
+
+// Two neighbouring ones, the first on an even place.
+template <typename T> __device__ __forceinline__ void tile_pair(const bf16* t, int plane, int at, float& x, float& y) {
+  x = y = 0.0f;
+#pragma unroll
+  for (int i = 0; i < Planes<T>::kToken; ++i) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(t + i * plane + at);
+    x += __uint_as_float(w << 16);
+    y += __uint_as_float(w & 0xffff0000u);
+  }
 }
 
 // By one warp: rows [0, n) of `cols` elements as they are, `pitch` apart; the rest of `rows` x `width` zero.

@@ -81,20 +81,18 @@ template <int N, int R, int P> __device__ __forceinline__ void put_planes(bf16 (
 #pragma unroll
   for (int n = 0; n < N; ++n) *reinterpret_cast<uint32_t*>(&m[n][i][j]) = p[n];
 }
+// A fragment's tiles (rows i .. i + 15, columns j .. j + 15) to rows of m; of w and z with swap8.
 template <int N, int NF, int R, int P> __device__ __forceinline__ void put_frag(bf16 (&m)[N][R][P], int i, int j, const Frag<NF>& f) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t at = smem_of(&m[0][i + (lane & 15)][j + ((lane & 16) >> 1)]);
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(&m[n][i + (e & 1) * 8][j + (e >> 1) * 8]) = f.r[n][e];
+  for (int n = 0; n < N; ++n) stsm4(at + n * R * P * 2, f.r[n]);
 }
-template <int N, int NF, int R> __device__ __forceinline__ void put_tokens(bf16 (&m)[N][R][kTile], int i, int j, const Frag<NF>& f) {
+template <int N, int NF, int R> __device__ __forceinline__ void put_tokens(bf16 (&m)[N][R][kTile], int i, const Frag<NF>& f) {
+  const int lane = threadIdx.x & 31, r = lane & 15;
+  const uint32_t at = smem_of(&m[0][i + r][swap8(r, (lane & 16) >> 1)]);
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = i + (e & 1) * 8;
-      *reinterpret_cast<uint32_t*>(&m[n][r][swap8(r, j + (e >> 1) * 8)]) = f.r[n][e];
-    }
+  for (int n = 0; n < N; ++n) stsm4(at + n * R * kTile * 2, f.r[n]);
 }
 // Addresses of ldmatrix in such rows, of a left operand's columns (a_cols) and a right one's (at_cols).
 __device__ __forceinline__ uint32_t tokens_a(int lane) {
@@ -421,7 +419,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
         uint32_t b[NT][4];
         load_planes<NT, false>(b, ka + x * 32, Keys::kPlane * 2);
         mma_planes<NI, NT>(ds[0], ds[1], f.r, b);
-        put_frag(sh.d, vl + row, 16 * x + col, f);
+        put_frag(sh.d, vl, 16 * x, f);
         if (!marks)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
@@ -449,16 +447,23 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
         load_planes<NT, true>(o, smem_of(st.tdo) + a_cols(lane, Values::kPitch) + vl * 2, Values::kPlane * 2);
         load_planes<NI, true>(b, smem_of(c.p) + at_cols(lane, kSide), kTile * kSide * 2);
         mma_planes<NT, NI>(du[0], du[1], o, b);
+        if (marks)                                     // no token before the last reset gets of dS
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (marks >> (t * 8 + col + (e & 1) + 1)) ds[t][e] = 0.0f;
         float x[2][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+          const float2 tail = *reinterpret_cast<const float2*>(&c.tail_k[t * 8 + col]), beta = *reinterpret_cast<const float2*>(&c.beta[t * 8 + col]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int tok = t * 8 + col + (e & 1);
-            ds[t][e] = marks >> (tok + 1) ? 0.0f : ds[t][e] * c.tail_k[tok];
+            ds[t][e] *= e & 1 ? tail.y : tail.x;
             du[t][e] += ds[t][e];
-            x[t][e] = c.beta[tok] * du[t][e];
+            x[t][e] = (e & 1 ? beta.y : beta.x) * du[t][e];
           }
+        }
         Frag<NI> f;
         load_planes<NI, true>(b, smem_of(c.inv) + at_cols(lane, kSide), kTile * kSide * 2);
         // A gradient of the state that is not finite reaches the last episode's tokens alone: with
@@ -490,9 +495,9 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
           }
         }
         f.from(z[0], z[1]);
-        put_tokens(sh.z, vl + row, col, f);
+        put_tokens(sh.z, vl, f);
         f.from(w[0], w[1]);
-        put_tokens(sh.w, vl + row, col, f);
+        put_tokens(sh.w, vl, f);
       }
       // sums over the warp's values, by tokens
       T (&so)[kTile][16 + 16 / sizeof(T)] = sh.part[warp].out;
@@ -539,27 +544,40 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
 #pragma unroll
           for (int e = 0; e < 4; ++e) d[x][e] = 0.0f;
       } else {
-        const float end = c.head[kTile - 1];
         float x[2][4];
+        if (marks) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (marks & ((2u << (t * 8 + col + (e & 1))) - 1u)) z[t][e] = 0.0f;
+#pragma unroll
+          for (int y = 0; y < DK / 8; ++y)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[y][e] = 0.0f;
+        } else {
+          const float end = c.head[kTile - 1];
+#pragma unroll
+          for (int y = 0; y < DK / 8; ++y)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[y][e] *= end;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float2 hk = *reinterpret_cast<const float2*>(&c.head_k[t * 8 + col]), hq = *reinterpret_cast<const float2*>(&c.head_q[t * 8 + col]);
+          const bf16* from = st.tdo + (t * 8 + col) * Values::kPitch + vl + row;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int tok = t * 8 + col + (e & 1), r = vl + row + (e >> 1) * 8;
-            z[t][e] = marks & ((2u << tok) - 1u) ? 0.0f : -c.head_k[tok] * z[t][e];
-            x[t][e] = c.head_q[tok] * tile_at<T>(st.tdo, Values::kPlane, tok * Values::kPitch + r);
+            z[t][e] *= e & 1 ? -hk.y : -hk.x;
+            x[t][e] = (e & 1 ? hq.y : hq.x) * tile_at<T>(from, Values::kPlane, (e & 1) * Values::kPitch + (e >> 1) * 8);
           }
+        }
         Frag<NI> fz, fo;
         fz.from(z[0], z[1]);
         fo.from(x[0], x[1]);
         const uint32_t kt = smem_of(st.tk) + at_cols(lane, Keys::kPitch), qt = smem_of(st.tq) + at_cols(lane, Keys::kPitch);
 #pragma unroll
         for (int y = 0; y < kSteps; ++y) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            d[2 * y][e] = marks ? 0.0f : d[2 * y][e] * end;
-            d[2 * y + 1][e] = marks ? 0.0f : d[2 * y + 1][e] * end;
-          }
           uint32_t b[NT][4];
           load_planes<NT, true>(b, kt + y * 32, Keys::kPlane * 2);
           mma_planes<NI, NT>(d[2 * y], d[2 * y + 1], fz.r, b);
@@ -604,18 +622,39 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
           }
         }
       }
-      float e0[2] = {};
+      float e0[2] = {}, hq[2], hk[2], tk[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int tok = row + 8 * e;
+        hk[e] = -c.head[tok];
+        hq[e] = a.scale * c.head[tok];
+        tk[e] = c.tail[tok] * c.beta[tok];
+        if (marks) {
+#pragma unroll
+          for (int p = 0; p < kPairs; ++p)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int x = 2 * e; x < 2 * e + 2; ++x) {
+                if (marks & ((2u << tok) - 1u)) aq[p][t][x] = ak[p][t][x] = 0.0f;
+                if (marks >> (tok + 1)) as[p][t][x] = 0.0f;
+              }
+        }
+      }
 #pragma unroll
       for (int p = 0; p < kPairs; ++p)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int tok = row + (e >> 1) * 8;
-            const bool seen = !(marks & ((2u << tok) - 1u)), sent = !(marks >> (tok + 1));
-            aq[p][t][e] = seen ? a.scale * c.head[tok] * aq[p][t][e] : 0.0f;
-            ak[p][t][e] = (seen ? -c.head[tok] * ak[p][t][e] : 0.0f) + (sent ? c.tail[tok] * c.beta[tok] * as[p][t][e] : 0.0f);
-            e0[e >> 1] = fmaf(aq[p][t][e], tile_at<T>(st.tq, Keys::kPlane, tok * Keys::kPitch + c0 + 16 * p + t * 8 + col + (e & 1)), e0[e >> 1]);
+          for (int e = 0; e < 2; ++e) {
+            float q0, q1;
+            tile_pair<T>(st.tq, Keys::kPlane, (row + 8 * e) * Keys::kPitch + c0 + 16 * p + t * 8 + col, q0, q1);
+#pragma unroll
+            for (int x = 2 * e; x < 2 * e + 2; ++x) {
+              aq[p][t][x] *= hq[e];
+              ak[p][t][x] = fmaf(hk[e], ak[p][t][x], tk[e] * as[p][t][x]);
+              e0[e] = fmaf(aq[p][t][x], x & 1 ? q1 : q0, e0[e]);
+            }
           }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -655,10 +694,15 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int x = (row + (e >> 1) * 8) * Keys::kPitch + cp + t * 8 + col + (e & 1);
-            aq[p][t][e] = rq[e >> 1] * (aq[p][t][e] - nq[e >> 1] * tile_at<T>(st.tq, Keys::kPlane, x));
-            ak[p][t][e] = rk[e >> 1] * (ak[p][t][e] - nk[e >> 1] * tile_at<T>(st.tk, Keys::kPlane, x));
+          for (int e = 0; e < 2; ++e) {
+            const int x = (row + 8 * e) * Keys::kPitch + cp + t * 8 + col;
+            float q0, q1, k0, k1;
+            tile_pair<T>(st.tq, Keys::kPlane, x, q0, q1);
+            tile_pair<T>(st.tk, Keys::kPlane, x, k0, k1);
+            aq[p][t][2 * e] = rq[e] * fmaf(-nq[e], q0, aq[p][t][2 * e]);
+            aq[p][t][2 * e + 1] = rq[e] * fmaf(-nq[e], q1, aq[p][t][2 * e + 1]);
+            ak[p][t][2 * e] = rk[e] * fmaf(-nk[e], k0, ak[p][t][2 * e]);
+            ak[p][t][2 * e + 1] = rk[e] * fmaf(-nk[e], k1, ak[p][t][2 * e + 1]);
           }
         if (a.part_q) {
 #pragma unroll
@@ -678,7 +722,10 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) so[row + (e >> 1) * 8][t * 8 + col + (e & 1)] = from_f<T>(turn2 ? ak[p][t][e] : aq[p][t][e]);
+              for (int e = 0; e < 2; ++e) {
+                const float pair[2] = {turn2 ? ak[p][t][2 * e] : aq[p][t][2 * e], turn2 ? ak[p][t][2 * e + 1] : aq[p][t][2 * e + 1]};
+                store_vec<T, 2>(&so[row + 8 * e][t * 8 + col], pair);
+              }
             __syncwarp();
             put_rows(static_cast<T*>(turn2 ? a.dk : a.dq) + qk_at + t0 * qk_t + cp, qk_t, so, n, a.keys - cp, pieces_k);
           }
