@@ -60,13 +60,15 @@ template <typename T> struct Planes { static constexpr int kToken = 1, kInner = 
 template <> struct Planes<float> { static constexpr int kToken = 3, kInner = 3, kShort = 3; };
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// What these read was written before a barrier of the warp or the block, across which the compiler moves
+// neither; without a memory clobber it may move other accesses about them.
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 // four 8 x 8 tiles, one register of each lane's a tile, to rows of 16 bytes
 __device__ __forceinline__ void stsm4(uint32_t at, const uint32_t (&r)[4]) {

@@ -24,10 +24,11 @@ namespace {
 using namespace delta;
 
 constexpr int kPrep = 2, kMain = 4, kValues = 64;      // warps of each kind (and one more); values of a block
-constexpr int kThreads = (kPrep + kMain + 1) * 32;
-// barriers: stage s ready (1 + s), stage s free (1 + kStages + s), S free for the warp of stage s (8 + s),
-// the chain's results, the matrices
-enum : int { kBarState = 8, kBarChain = 14, kBarMatrices = 15 };
+constexpr int kTeam = kPrep + kMain + 1;
+// A team's barriers: stage s ready (s), stage s free (2 + s), the chain's results, the matrices; one for
+// all of a block's main warps. And how many threads meet at them.
+enum : int { kBarReady = 0, kBarFree = 2, kBarChain = 4, kBarMatrices = 5, kBarTeam = 6, kBarAll = 13 };
+constexpr int kStageThreads = (kMain + 2) * 32, kMainThreads = (kMain + 1) * 32;
 
 template <typename T, int DK> struct Backward {
   static constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort;
@@ -46,7 +47,7 @@ template <typename T, int DK> struct Backward {
   };
   struct Shared {
     Stage stage[kStages];
-    // the forward pass's S and W (rows values, columns tokens), one chunk's: two blocks fit on an SM then
+    // the forward pass's S and W (rows values, columns tokens) of a tile
     alignas(16) float s[kValues][kPitchS];
     alignas(16) float saved_w[kValues][kMat];
     alignas(16) Scratch scratch[kStages];
@@ -59,9 +60,11 @@ template <typename T, int DK> struct Backward {
     float by_key[kMain][kTile];                        // the heads' terms of q
     float nq[kTile], nk[kTile];                        // q.dq and k.dk but for those
   };
-  static constexpr size_t kBytes = sizeof(Shared);
-  static_assert(kBytes <= 227 * 1024, "a block's shared memory");
-  static constexpr int kBlocks = kBytes <= 113 * 1024 ? 2 : 1;
+  // Two teams in a block, where they fit: warps of the same task then run the same instructions on the
+  // same quarter of the SM at the same time. As two blocks they spent a third of their time waiting for
+  // instructions (a tile's are 60 KB).
+  static constexpr int kTeams = 2 * sizeof(Shared) <= 227 * 1024 ? 2 : 1;
+  static_assert(sizeof(Shared) <= 227 * 1024, "a block's shared memory");
 };
 
 // Rows of 16 tokens lie 32 bytes apart, their halves swapped in every other four rows: eight rows of
@@ -119,30 +122,48 @@ __device__ __forceinline__ void put_rows(T* to, int64_t stride, const T (&out)[k
   }
 }
 
-template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backward<T, DK>::kBlocks) delta_backward(DeltaArgs a) {
+template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTeams * kTeam * 32) delta_backward(DeltaArgs a, int splits) {
   using B = Backward<T, DK>;
   constexpr int NT = B::NT, NI = B::NI, NS = B::NS, kSteps = DK / 16, kStages = B::kStages;
   using Keys = typename B::Keys;
   using Values = typename B::Values;
   extern __shared__ __align__(16) char smem[];
-  typename B::Shared& sh = *reinterpret_cast<typename B::Shared*>(smem);
-  const int bi = blockIdx.x / a.heads, h = blockIdx.x % a.heads, gr = h / (a.heads / a.groups);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = lane >> 2, col = (lane & 3) * 2;
-  const int vb = blockIdx.y * kValues, mine = min(kValues, a.values - vb), splits = gridDim.y;
-  const int length = a.lengths ? max(0, min(a.lengths[bi], a.length)) : a.length;
-  const int tiles = (a.length + kTile - 1) / kTile;
+  // main warps first (warp w of every team on the same quarter of the SM), then the ones that make
+  // chunks ready, then those of the matrices
+  int warp = threadIdx.x >> 5, team, role;
+  if (warp < kTeams * kMain) {
+    role = 0;
+    team = warp / kMain;
+    warp %= kMain;
+  } else if (warp < kTeams * (kMain + kPrep)) {
+    role = 1;
+    team = (warp - kTeams * kMain) / kPrep;
+    warp = (warp - kTeams * kMain) % kPrep;
+  } else {
+    role = 2;
+    team = warp - kTeams * (kMain + kPrep);
+  }
+  const int64_t items = static_cast<int64_t>(a.batch) * a.heads * splits, item = static_cast<int64_t>(blockIdx.x) * kTeams + team;
+  if (item >= items) return;
+  typename B::Shared& sh = reinterpret_cast<typename B::Shared*>(smem)[team];
+  const int bars = 1 + team * kBarTeam;
+  const int block = static_cast<int>(item % splits), bh = static_cast<int>(item / splits), bi = bh / a.heads, h = bh % a.heads, gr = h / (a.heads / a.groups);
+  const int lane = threadIdx.x & 31, row = lane >> 2, col = (lane & 3) * 2;
+  const int vb = block * kValues, mine = min(kValues, a.values - vb);
+  auto length_of = [&](int b) { return a.lengths ? max(0, min(a.lengths[b], a.length)) : a.length; };
+  const int length = length_of(bi);
+  const int tiles = (a.length + kTile - 1) / kTile, count = (length + kTile - 1) / kTile;
   const int64_t row0 = static_cast<int64_t>(bi) * a.length;
   const T* dt = static_cast<const T*>(a.dt) + bi * a.dt_b + h;
   const T* gb = static_cast<const T*>(a.b) + bi * a.b_b + h;
   const float rate = rate_at(a.A, h), bias = a.bias ? a.bias[h] : 0.0f;
 
-  if (warp >= kMain && warp < kMain + kPrep) {
-    const int w = warp - kMain, pitch = a.keys + kTile;
+  if (role == 1) {
+    const int w = warp, pitch = a.keys + kTile;
     const T* q = static_cast<const T*>(a.q) + bi * a.q_b + gr * a.q_g;
     const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
     const T* v = static_cast<const T*>(a.v) + bi * a.v_b + h * a.v_h + vb;
     const T* dout = static_cast<const T*>(a.dout) + bi * a.do_b + h * a.do_h + vb;
-    const int count = (length + kTile - 1) / kTile, stage_threads = kThreads - (kPrep - 1) * 32;
     Marks look{a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length, 0u};
     // resets and gates a tile of this warp's ahead of the rest
     T raw_dt = from_f<T>(0.0f), raw_b = raw_dt;
@@ -160,9 +181,8 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
       const unsigned marks = look.get();
       const float now_dt = to_f(raw_dt), now_b = to_f(raw_b);
       ahead(tile - kStages);
-      if (i >= kStages) bar_sync(1 + kStages + w, stage_threads);
+      if (i >= kStages) bar_sync(bars + kBarFree + w, kStageThreads);
       const float* saved = a.saved + (((static_cast<int64_t>(bi) * tiles + tile) * a.heads + h) * a.values + vb) * pitch;
-      const bool pieces = a.keys % 4 == 0;
       bool bad = false;
       auto fetch = [&](int from, int n, unsigned mark, float x, float y) {
         const int t0 = tile * kTile + from;
@@ -184,60 +204,52 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
         cp_async_wait<0>();
         __syncwarp();
       };
-      // matrices, then S and W as soon as the chunk before is done with its own
-      auto ready = [&](int from, int n, unsigned mark, bool first) {
+      auto ready = [&](unsigned mark) {
         prepare<T, DK, true>(st.c, sh.scratch[w], &st.wide, st.tk, st.tq, mark, a.scale, a.unit);
-        if (!first) bar_sync(kBarState + w, (kMain + 1) * 32);
-        load_rows(&sh.saved_w[0][0], kMat, kValues, kTile, saved + a.keys + from, pitch, mine, n, pieces && from % 4 == 0 && n % 4 == 0);
-        if (!(mark & 1u)) load_rows(&sh.s[0][0], B::kPitchS, kValues, DK, saved, pitch, mine, a.keys, pieces);
-        cp_async_commit();
-        cp_async_wait<0>();
-        __syncwarp();
-        bar_arrive(1 + w, stage_threads);
+        bar_arrive(bars + kBarReady + w, kStageThreads);
       };
       fetch(0, end, marks, now_dt, now_b);
       bool split = false;
       if (marks & ~1u) {
-        float w_bad = 0.0f;                            // W is looked at where it lies: its place here is still in use
+        float w_bad = 0.0f;
         for (int x = lane; x < mine * end; x += 32) w_bad = fmaf(saved[x / end * pitch + a.keys + x % end], 0.0f, w_bad);
         split = bad || __any_sync(0xffffffffu, w_bad != 0.0f) || not_finite(st.tk, Keys::kPitch, DK, end) ||
                 not_finite(st.tq, Keys::kPitch, DK, end) || not_finite(st.tdo, Values::kPitch, kValues, end) ||
                 not_finite(st.tv, B::kPitchV, kValues, end);
       }
       if (!split) {
-        ready(0, end, marks, i == 0);
+        ready(marks);
         continue;
       }
       for (int to = end; to > 0;) {                    // the last episode first
         const int from = 31 - __clz((marks | 1u) & ((1u << to) - 1u));
         const unsigned mark = (marks >> from) & 1u;
-        if (to < end) bar_sync(1 + kStages + w, stage_threads);
+        if (to < end) bar_sync(bars + kBarFree + w, kStageThreads);
         const int at = tile * kTile + from + lane;
         const bool on = from + lane < to;
         fetch(from, to - from, mark, on ? to_f(dt[at * a.dt_t]) : 0.0f, on ? to_f(gb[at * a.b_t]) : 0.0f);
         if (lane == 0) st.more = from > 0;
-        ready(from, to - from, mark, i == 0 && to == end);
+        ready(mark);
         to = from;
       }
     }
     return;
   }
 
-  const int stage_threads = kThreads - (kPrep - 1) * 32, team = (kMain + 1) * 32, count = (length + kTile - 1) / kTile;
-  if (warp == kMain + kPrep) {
+  if (role == 2) {
     // the matrices and gates of 16 x 16
-    const int64_t g_t = static_cast<int64_t>(a.heads) * splits, g_at = row0 * g_t + static_cast<int64_t>(h) * splits + blockIdx.y;
+    const int64_t g_t = static_cast<int64_t>(a.heads) * splits, g_at = row0 * g_t + static_cast<int64_t>(h) * splits + block;
     double sum_a = 0.0, sum_bias = 0.0;
     for (int i = 0, more = 0; i < count; i += more ? 0 : 1) {
       const int at = i % kStages;
       typename B::Stage& st = sh.stage[at];
-      bar_sync(1 + at, stage_threads);
+      bar_sync(bars + kBarReady + at, kStageThreads);
       const int t0 = st.t0, n = st.n;
       const unsigned marks = st.marks;
       more = st.more;
       Gate gate{};
       if (lane < n) gate = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
-      bar_sync(kBarChain, team);
+      bar_sync(bars + kBarChain, kMainThreads);
       // lane: row r, columns j0 .. j0 + 7 of Z W^T and dO W^T. By rows: sums of E's part of P, of M, and Z.R
       const int r = lane >> 1, j0 = (lane & 1) * 8;
       const float rqr = st.c.rq[r], rkr = st.c.rk[r];
@@ -330,7 +342,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
         sh.nq[c] = row_p;
         sh.nk[c] = keep + f + row_m + column;
       }
-      bar_sync(kBarMatrices, team);
+      bar_sync(bars + kBarMatrices, kMainThreads);
       float e = keep;
 #pragma unroll
       for (int x = 0; x < kMain; ++x) e += sh.by_key[x][c];
@@ -353,14 +365,14 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
         sum_bias += back;
       }
       __syncwarp();
-      bar_arrive(1 + kStages + at, stage_threads);
+      bar_arrive(bars + kBarFree + at, kStageThreads);
     }
     for (int o = 16; o; o >>= 1) {
       sum_a += __shfl_xor_sync(0xffffffffu, sum_a, o);
       sum_bias += __shfl_xor_sync(0xffffffffu, sum_bias, o);
     }
     if (lane == 0) {
-      const int64_t to = (static_cast<int64_t>(blockIdx.x) * splits + blockIdx.y) * 2;
+      const int64_t to = item * 2;
       a.part_h[to] = static_cast<float>(sum_a);
       a.part_h[to + 1] = static_cast<float>(sum_bias);
     }
@@ -373,7 +385,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
   }
 
   // gradients are dense; parts of dq and dk by heads and blocks
-  const int qk_heads = a.part_q ? a.heads * splits : a.groups, qk_head = a.part_q ? h * splits + static_cast<int>(blockIdx.y) : gr;
+  const int qk_heads = a.part_q ? a.heads * splits : a.groups, qk_head = a.part_q ? h * splits + block : gr;
   const int64_t qk_t = static_cast<int64_t>(qk_heads) * a.keys, qk_at = (row0 * qk_heads + qk_head) * a.keys;
   const int64_t v_t = static_cast<int64_t>(a.heads) * a.values;
   T* dv = static_cast<T*>(a.dv) + (row0 * a.heads + h) * a.values + vb;
@@ -399,15 +411,39 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
   if (lane == 0) sh.inner[warp] = 0.0f;
   __syncwarp();
 
-  for (int i = 0, more = 0; i < count; i += more ? 0 : 1) {
+  // S and W of the tiles from the last on, each warp's own rows, on their way while the tile before is finished
+  const int pitch = a.keys + kTile;
+  const bool pieces_s = a.keys % 4 == 0;
+  const int64_t saved_tile = static_cast<int64_t>(a.heads) * a.values * pitch;
+  const float* saved = a.saved + (static_cast<int64_t>(bi) * tiles * a.heads + h) * a.values * pitch + static_cast<int64_t>(vb + vl) * pitch;
+  auto take = [&](int tile) {
+    if (!by_v) return;
+    const float* from = saved + tile * saved_tile;
+    load_rows(&sh.s[vl][0], B::kPitchS, 16, DK, from, pitch, min(16, mine - vl), a.keys, pieces_s);
+    load_rows(&sh.saved_w[vl][0], kMat, 16, kTile, from + a.keys, pitch, min(16, mine - vl), kTile, pieces_s);
+    cp_async_commit();
+  };
+  if (count > 0) take(count - 1);
+  // tiles that all teams of the block have
+  int common = 0;
+  if constexpr (kTeams > 1) {
+    const int64_t other = item ^ 1;
+    if (other < items) common = min(count, (length_of(static_cast<int>(other / splits) / a.heads) + kTile - 1) / kTile);
+  }
+
+  for (int i = 0, more = 0, next = 1; i < count; i += more ? 0 : 1) {
     const int at = i % kStages;
     typename B::Stage& st = sh.stage[at];
     const Chunk<T, NI>& c = st.c;
-    bar_sync(1 + at, stage_threads);
+    if (next && i < common) bar_sync(kBarAll, kTeams * kMain * 32);
+    bar_sync(bars + kBarReady + at, kStageThreads);
     const int t0 = st.t0, n = st.n;
     const unsigned marks = st.marks;
     const bool fresh = marks & 1u;                     // no token sees S
     more = st.more;
+    next = !more;
+    cp_async_wait<0>();
+    __syncwarp();
     if (by_v) {
       // K dS^T (rows values, columns tokens), <dS, S>; dS's planes to shared memory
       float ds[2][4] = {}, inner = 0.0f;
@@ -442,6 +478,14 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
           w[t][2 * e] = y.x;
           w[t][2 * e + 1] = y.y;
         }
+      if (n < kTile)                                   // a part of the tile
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tok = 8 * t + col + (e & 1);
+            w[t][e] = tok < n ? sh.saved_w[vl + row + (e >> 1) * 8][t0 % kTile + tok] : 0.0f;
+          }
       {
         uint32_t o[NT][4], b[NI][4];
         load_planes<NT, true>(o, smem_of(st.tdo) + a_cols(lane, Values::kPitch) + vl * 2, Values::kPlane * 2);
@@ -588,7 +632,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
     }
     else
       for (int x = lane; x < 2 * kTile * kMat; x += 32) (&sh.part[warp].product[0][0][0])[x] = 0.0f;
-    bar_sync(kBarChain, team);
+    bar_sync(bars + kBarChain, kMainThreads);
 
     // by keys: rows tokens, columns c0 ..
     float aq[kPairs][2][4] = {}, ak[kPairs][2][4] = {};
@@ -662,8 +706,8 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
         if ((lane & 3) == 0) sh.by_key[warp][row + 8 * e] = e0[e] * c.rq[row + 8 * e];
       }
     }
-    bar_sync(kBarMatrices, team);
-    bar_arrive(kBarState + (more ? at : (i + 1) % kStages), team);       // S and W: the next chunk's warp may have their place
+    bar_sync(bars + kBarMatrices, kMainThreads);       // S is read no more
+    if (!more && i + 1 < count) take(count - 2 - i);
 
     if (by_k) {
       float nq[2] = {}, nk[2] = {}, rq[2], rk[2];
@@ -733,7 +777,7 @@ template <typename T, int DK> __global__ void __launch_bounds__(kThreads, Backwa
       }
     }
     __syncwarp();
-    bar_arrive(1 + kStages + at, stage_threads);
+    bar_arrive(bars + kBarFree + at, kStageThreads);
   }
 
   if (dstate && by_v) {
@@ -806,13 +850,20 @@ template <typename T, int DK> int backward(const DeltaArgs& a, cudaStream_t s) {
   using B = Backward<T, DK>;
   const int splits = (a.values + kValues - 1) / kValues;
   if ((splits > 1 && !a.part_g) || (splits * a.heads != a.groups && !a.part_q)) return static_cast<int>(cudaErrorInvalidValue);
-  if (const int e = allow_smem<delta_backward<T, DK>>(B::kBytes)) return e;
-  delta_backward<T, DK><<<dim3(a.batch * a.heads, splits), kThreads, B::kBytes, s>>>(a);
-  if (const cudaError_t e = cudaGetLastError()) return static_cast<int>(e);
+  // one team a block as long as every head has an SM to itself
+  const int64_t items = static_cast<int64_t>(a.batch) * a.heads * splits;
+  auto go = [&](auto n) {
+    constexpr int kTeams = decltype(n)::value;
+    constexpr size_t bytes = kTeams * sizeof(typename B::Shared);
+    if (const int e = allow_smem<delta_backward<T, DK, kTeams>>(bytes)) return e;
+    delta_backward<T, DK, kTeams><<<static_cast<unsigned>((items + kTeams - 1) / kTeams), kTeams * kTeam * 32, bytes, s>>>(a, splits);
+    return static_cast<int>(cudaGetLastError());
+  };
+  if (const int e = items > 148 ? go(std::integral_constant<int, B::kTeams>()) : go(std::integral_constant<int, 1>())) return e;
   delta_rates<<<a.heads, 32, 0, s>>>(a, splits);
   if (a.part_q && a.length > 0) {
-    const int64_t blocks = (static_cast<int64_t>(a.batch) * a.length * a.groups * a.keys + 255) / 256;
-    delta_parts<T><<<blocks < 148 * 16 ? static_cast<unsigned>(blocks) : 148 * 16, 256, 0, s>>>(a, splits);
+    const int64_t grid = (static_cast<int64_t>(a.batch) * a.length * a.groups * a.keys + 255) / 256;
+    delta_parts<T><<<grid < 148 * 16 ? static_cast<unsigned>(grid) : 148 * 16, 256, 0, s>>>(a, splits);
   }
   return static_cast<int>(cudaGetLastError());
 }
