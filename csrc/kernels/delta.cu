@@ -373,20 +373,21 @@ struct StepArgs {
 };
 static_assert(sizeof(StepArgs) == 12 * 8 + 10 * 8 + 8 * 4, "as the caller packs it");
 
-// A warp for a head of a row: its lanes hold the key and the query, LK lanes a value's row of the
-// state. S k and S q come from one look at the state:
+// A warp for `per` values of a head of a row (blockIdx.y): its lanes hold the key and the query, LK
+// lanes a value's row of the state. S k and S q come from one look at the state:
 //   u = beta (v - e^g S k),  S <- e^g S + u k^T,  o = scale (e^g S q + u k.q).
-template <typename T, int LK> __global__ void __launch_bounds__(256) delta_step(StepArgs a) {
+template <typename T, int LK> __global__ void __launch_bounds__(256) delta_step(StepArgs a, int per) {
   constexpr int kRows = 32 / LK;                       // values that a warp takes at once
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
   if (item >= static_cast<int64_t>(a.rows) * a.heads) return;
   const int r = static_cast<int>(item / a.heads), h = static_cast<int>(item % a.heads), gr = h / (a.heads / a.groups);
   T* out = static_cast<T*>(a.out) + r * a.o_r + h * a.o_h;
+  const int first = blockIdx.y * per, last = min(first + per, a.values);
   const int slot = a.slots ? a.slots[r] : r;
   if (slot < 0 || slot >= a.pools) {
-    if (slot >= a.pools && h == 0 && lane == 0) surfk::report_error(a.err, surfk::kErrSlotIndex);
-    for (int i = lane; i < a.values; i += 32) out[i] = from_f<T>(0.0f);
+    if (slot >= a.pools && h == 0 && first == 0 && lane == 0) surfk::report_error(a.err, surfk::kErrSlotIndex);
+    for (int i = first + lane; i < last; i += 32) out[i] = from_f<T>(0.0f);
     return;
   }
   const int l = lane % LK, k0 = l * 4;
@@ -427,7 +428,7 @@ template <typename T, int LK> __global__ void __launch_bounds__(256) delta_step(
   const bool whole = a.keys % 4 == 0;
   // several rows of the state are on their way before the first is used
   constexpr int kAhead = 4;
-  for (int v0 = lane / LK; v0 < a.values + lane / LK; v0 += kAhead * kRows) {
+  for (int v0 = first + lane / LK; v0 < last + lane / LK; v0 += kAhead * kRows) {
     float s[kAhead][4];
     float v[kAhead];
 #pragma unroll
@@ -437,7 +438,7 @@ template <typename T, int LK> __global__ void __launch_bounds__(256) delta_step(
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
       v[i] = 0.0f;
-      if (vr >= a.values) continue;
+      if (vr >= last) continue;
       v[i] = to_f(pv[vr]);
       if (fresh) continue;
       if (whole) {
@@ -464,7 +465,7 @@ template <typename T, int LK> __global__ void __launch_bounds__(256) delta_step(
         sk += __shfl_xor_sync(0xffffffffu, sk, o);
         sq += __shfl_xor_sync(0xffffffffu, sq, o);
       }
-      if (vr >= a.values) continue;
+      if (vr >= last) continue;
       const float u = beta * (v[i] - sk);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = fmaf(u, k[j], s[i][j]);
@@ -481,12 +482,22 @@ template <typename T, int LK> __global__ void __launch_bounds__(256) delta_step(
 }
 
 template <typename T> int step(const StepArgs& a, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.rows) * a.heads + 7) / 8);
-  if (a.keys <= 16) delta_step<T, 4><<<grid, 256, 0, s>>>(a);
-  else if (a.keys <= 32) delta_step<T, 8><<<grid, 256, 0, s>>>(a);
-  else if (a.keys <= 64) delta_step<T, 16><<<grid, 256, 0, s>>>(a);
-  else delta_step<T, 32><<<grid, 256, 0, s>>>(a);
-  return static_cast<int>(cudaGetLastError());
+  const int64_t heads = static_cast<int64_t>(a.rows) * a.heads;
+  auto go = [&](auto lanes) {
+    constexpr int LK = decltype(lanes)::value;
+    // a head's values in as many warps as give every SM 32, of at least the rows that are on their way
+    // at once: 64 rows of 8 heads of 64 x 64 in 1 and 8 warps a head
+    const int least = 4 * (32 / LK), most = (a.values + least - 1) / least;
+    int parts = static_cast<int>(heads >= 148 * 32 ? 1 : (148 * 32 + heads - 1) / heads);
+    parts = parts < most ? parts : most;
+    const int per = ((a.values + parts - 1) / parts + least - 1) / least * least;
+    delta_step<T, LK><<<dim3(static_cast<unsigned>((heads + 7) / 8), (a.values + per - 1) / per), 256, 0, s>>>(a, per);
+    return static_cast<int>(cudaGetLastError());
+  };
+  if (a.keys <= 16) return go(std::integral_constant<int, 4>());
+  if (a.keys <= 32) return go(std::integral_constant<int, 8>());
+  if (a.keys <= 64) return go(std::integral_constant<int, 16>());
+  return go(std::integral_constant<int, 32>());
 }
 
 }  // namespace
