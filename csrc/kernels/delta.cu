@@ -31,13 +31,15 @@ template <typename T, int DK> struct Forward {
   static __host__ __device__ constexpr size_t bytes(int warps) {
     return sizeof(Shared) + (static_cast<size_t>(kStages) * kTile * pitch_v(warps) + static_cast<size_t>(warps) * kTile * kRow) * sizeof(T);
   }
+  // and, where the state goes out by bulk copies, each warp's rows of it and of W
+  static __host__ __device__ constexpr size_t kept_bytes(int warps, int keys) { return static_cast<size_t>(warps) * 16 * (keys + kTile) * sizeof(float); }
 };
 
 // A block for up to 64 values of a sequence's value head. Two warps make the chunks ready in turn
 // (tiles, decays, P, the inverse: nothing of it waits for the state), the others hold 16 values'
 // rows of the state each, as accumulators from the first token to the last. They meet at
 // numbered barriers: stage s is ready (1 + s), stage s is free (1 + kStages + s).
-template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kPrep + kMain) * 32, kBlocks) delta_forward(DeltaArgs a) {
+template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kPrep + kMain) * 32, kBlocks) delta_forward(DeltaArgs a, int bulk) {
   constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort, kSteps = DK / 16;
   using F = Forward<T, DK>;
   using Keys = Tile<T, DK>;
@@ -178,7 +180,8 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
     }
   });
 
-  const int tiles = (a.length + kTile - 1) / kTile;
+  const int tiles = (a.length + kTile - 1) / kTile, pitch_s = a.keys + kTile;
+  float* kept = reinterpret_cast<float*>(smem + F::bytes(warps)) + warp * 16 * pitch_s;
   for (int i = 0, more = 0; i < (length + kTile - 1) / kTile; i += more ? 0 : 1) {
     const int at = i % kStages;
     typename F::Stage& st = sh.stage[at];
@@ -187,8 +190,20 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
     const unsigned marks = st.marks;
     more = st.more;
     const Chunk<T, NS>& c = st.c;
-    float* saved = a.saved ? a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values * (a.keys + kTile) : nullptr;
-    if (saved && t0 % kTile == 0) store(saved, a.keys + kTile);
+    // The state before the tile and W, for the gradient: rows of both side by side, as one bulk copy from
+    // shared memory where that is allowed (stored lane by lane they held the chain up: 2x4096x16x64x64
+    // 449 us).
+    float* saved = a.saved ? a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values * pitch_s : nullptr;
+    const bool copied = bulk && t0 % kTile == 0 && !more;
+    if (copied) {
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+      each([&](float x, float y, int r, int kc) {
+        if (kc < a.keys) *reinterpret_cast<float2*>(kept + (r - v0) * pitch_s + kc) = make_float2(x, y);
+      });
+    } else if (saved && t0 % kTile == 0) {
+      store(saved, pitch_s);
+    }
     if (marks & 1u) each([&](float& x, float& y, int, int) { x = y = 0.0f; });
     const T* tv = values + at * kTile * pitch_v;
 
@@ -268,14 +283,27 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
             sq[t][e] += y[t][e];
           }
     }
-    if (saved) {
+    if (copied) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float2*>(kept + (row + 8 * e) * pitch_s + a.keys + 8 * t + col) = make_float2(w[t][2 * e], w[t][2 * e + 1]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(saved + static_cast<int64_t>(v0) * pitch_s),
+                     "r"(smem_of(kept)), "r"(min(16, a.values - v0) * pitch_s * 4) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    } else if (saved) {
       float* p = saved + a.keys + t0 % kTile;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int tok = t * 8 + col + (e & 1), r = v0 + row + (e >> 1) * 8;
-          if (tok < n && r < a.values) p[r * (a.keys + kTile) + tok] = w[t][e];
+          if (tok < n && r < a.values) p[r * pitch_s + tok] = w[t][e];
         }
     }
     // the state
@@ -336,6 +364,7 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
     __syncwarp();
   }
   store(a.final_ + head_at, a.keys);
+  if (bulk && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   // tokens that are not there give zeros
   for (int t = length + warp; t < a.length; t += warps)
     for (int j = lane; j < mine; j += 32) out[t * a.o_t + vb + j] = from_f<T>(0.0f);
@@ -344,12 +373,19 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
 template <typename T, int DK> int forward(const DeltaArgs& a, cudaStream_t s) {
   using F = Forward<T, DK>;
   constexpr int kBlocks = sizeof(T) == 4 && DK == 128 ? 1 : 2;
-  if (const int e = allow_smem<delta_forward<T, DK, kBlocks>>(F::bytes(kMain))) return e;
   // values of a block: as many as it takes, or fewer where that leaves SMs without one
   const int all = (a.values + 15) / 16;
   int warps = all < kMain ? all : kMain;
   while (warps > 1 && static_cast<int64_t>(a.batch) * a.heads * ((all + warps - 1) / warps) < 148) warps = (warps + 1) / 2;
-  delta_forward<T, DK, kBlocks><<<dim3(a.batch * a.heads, (all + warps - 1) / warps), (warps + kPrep) * 32, F::bytes(warps), s>>>(a);
+  const int64_t blocks = static_cast<int64_t>(a.batch) * a.heads * ((all + warps - 1) / warps);
+  // bulk copies of what is kept want rows of whole 16 bytes, and shared memory that would cost many
+  // blocks their neighbour on the SM
+  const size_t kept = F::kept_bytes(warps, a.keys);
+  const bool bulk = a.saved && a.keys % 4 == 0 && F::bytes(warps) + kept <= (blocks > 148 && kBlocks > 1 ? 113 : 227) * 1024;
+  constexpr size_t kMost = F::bytes(kMain) + F::kept_bytes(kMain, DK);
+  if (const int e = allow_smem<delta_forward<T, DK, kBlocks>>(kMost < 227 * 1024 ? kMost : 227 * 1024)) return e;
+  delta_forward<T, DK, kBlocks><<<dim3(a.batch * a.heads, (all + warps - 1) / warps), (warps + kPrep) * 32,
+                                  F::bytes(warps) + (bulk ? kept : 0), s>>>(a, bulk);
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T> int forward_by(const DeltaArgs& a, cudaStream_t s) {

@@ -190,7 +190,7 @@ template <typename T, int H> __global__ void __launch_bounds__(kWarpThreads) los
 }
 
 // ---- a cluster of blocks for a row ------------------------------------------------------
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 384;
 
 __device__ __forceinline__ float max_of(const uint4& q, float m) {
   return fmaxf(fmaxf(m, fmaxf(__uint_as_float(q.x), __uint_as_float(q.y))), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
@@ -199,7 +199,7 @@ __device__ __forceinline__ __nv_bfloat162 pair_of(uint32_t w) { return *reinterp
 
 // A block takes candidates [first, first + count) of its row; shared memory mirrors their place within 16
 // bytes of global memory, so that all but the ends move in pieces of 16 bytes.
-template <typename T> __global__ void __launch_bounds__(kRowThreads) loss_row(LossArgs p, int per) {
+template <typename T> __global__ void __launch_bounds__(kRowThreads, 3) loss_row(LossArgs p, int per) {
   constexpr int V = kVec16<T>;
   extern __shared__ __align__(16) char smem[];
   __shared__ Sums part[kRowThreads / 32], mine;
