@@ -23,16 +23,28 @@ namespace {
 
 using namespace delta;
 
-constexpr int kPrep = 2, kMain = 4, kValues = 64;      // warps of each kind (and one more); values of a block
-constexpr int kTeam = kPrep + kMain + 1;
-// A team's barriers: stage s ready (s), stage s free (2 + s), the chain's results, the matrices; one for
-// all of a block's main warps. And how many threads meet at them.
-enum : int { kBarReady = 0, kBarFree = 2, kBarChain = 4, kBarMatrices = 5, kBarTeam = 6, kBarAll = 13 };
-constexpr int kStageThreads = (kMain + 2) * 32, kMainThreads = (kMain + 1) * 32;
+constexpr int kPrep = 2, kMain = 4, kValues = 64;      // warps that make chunks ready, of the chain and of the keys; values of a block
+
+// How a block is made up. Either teams of one head each, whose four main warps follow the chain and then the
+// keys; or (kApart) one head whose chain is four warps' and whose keys are four others', a chunk behind.
+template <int kTeams_, bool kApart_> struct Plan {
+  static constexpr int kTeams = kTeams_;
+  static constexpr bool kApart = kApart_;
+  static constexpr int kAll = (kApart ? 2 : 1) * kMain;                // main warps of a team
+  static constexpr int kThreads = kTeams * (kAll + kPrep + 1) * 32;
+  static constexpr int kStages = kApart ? 2 * kPrep : kPrep;           // a stage's barriers are one preparing warp's alone
+  static constexpr int kCopies = kApart ? 2 : 1;                       // of what the chain leaves
+  // a team's barriers, and how many threads meet at them: stage s ready (chain, matrices, the warp that made
+  // it), stage s free (all of them), the chain's results (main, matrices), their place free (the
+  // same), the matrices (keys, matrices); one for the main warps of all teams
+  static constexpr int kReady = 0, kFree = kStages, kChain = 2 * kStages, kPlace = kChain + kCopies, kMatrices = kPlace + (kApart ? 2 : 0);
+  static constexpr int kBars = kMatrices + 1, kEvery = 1 + kTeams * kBars;
+  static_assert(kEvery < 16, "barriers of a block");
+  static constexpr int kAtReady = (kMain + 2) * 32, kAtFree = (kAll + 2) * 32, kAtChain = (kAll + 1) * 32, kAtMatrices = (kMain + 1) * 32;
+};
 
 template <typename T, int DK> struct Backward {
   static constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort;
-  static constexpr int kStages = kPrep;                // one for each warp that makes chunks ready: its barriers are that warp's alone
   using Keys = Tile<T, DK>;
   using Values = Tile<T, kValues>;
   static constexpr int kPitchS = DK + 4, kPitchD = DK + 8, kPitchV = kValues + 16 / static_cast<int>(sizeof(T));
@@ -45,26 +57,28 @@ template <typename T, int DK> struct Backward {
     alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize], tdo[Values::kSize];
     alignas(16) T tv[kTile * kPitchV];
   };
-  struct Shared {
-    Stage stage[kStages];
-    // the forward pass's S and W (rows values, columns tokens) of a tile
-    alignas(16) float s[kValues][kPitchS];
-    alignas(16) float saved_w[kValues][kMat];
-    alignas(16) Scratch scratch[kStages];
-    alignas(16) bf16 w[NI][kValues][kTile], z[NI][kValues][kTile];       // rows values, columns tokens; see swap8
+  struct Chain {                                       // what the chain leaves of a chunk
+    alignas(16) bf16 w[NI][kValues][kTile], z[NI][kValues][kTile];     // rows values, columns tokens; see swap8
     alignas(16) bf16 d[NS][kValues][kPitchD];          // dS
-    alignas(16) bf16 x1[NS][kTile][kSide], x2[NS][kTile][kSide], x3[NS][kTile][kSide];
     // of each warp: Z W^T and dO W^T, or its outputs
     alignas(16) union { float product[2][kTile][kMat]; T out[kTile][16 + 16 / sizeof(T)]; } part[kMain];
     float by_value[kMain][3][kTile], inner[kMain];     // sums over its values: W.dU, Z.V, the tails' terms; <dS, S>
-    float by_key[kMain][kTile];                        // the heads' terms of q
+  };
+  template <typename P> struct Shared {
+    Stage stage[P::kStages];
+    // the forward pass's S and W (rows values, columns tokens) of a tile: the chain's, and where the keys' warps
+    // are others, theirs
+    alignas(16) float s[P::kCopies][kValues][kPitchS];
+    alignas(16) float saved_w[kValues][kMat];
+    alignas(16) Scratch scratch[kPrep];
+    Chain chain[P::kCopies];
+    alignas(16) bf16 x1[NS][kTile][kSide], x2[NS][kTile][kSide], x3[NS][kTile][kSide];
+    alignas(16) T out[P::kApart ? kMain : 1][kTile][16 + 16 / sizeof(T)];
+    float by_key[2][kMain][kTile];                     // the head's terms of q and k
     float nq[kTile], nk[kTile];                        // q.dq and k.dk but for those
   };
-  // Two teams in a block, where they fit: warps of the same task then run the same instructions on the
-  // same quarter of the SM at the same time. As two blocks they spent a third of their time waiting for
-  // instructions (a tile's are 60 KB).
-  static constexpr int kTeams = 2 * sizeof(Shared) <= 227 * 1024 ? 2 : 1;
-  static_assert(sizeof(Shared) <= 227 * 1024, "a block's shared memory");
+  template <typename P> static constexpr bool kFits = P::kTeams * sizeof(Shared<P>) <= 227 * 1024;
+  static_assert(kFits<Plan<1, false>>, "a block's shared memory");
 };
 
 // Rows of 16 tokens lie 32 bytes apart, their halves swapped in every other four rows: eight rows of
@@ -122,31 +136,33 @@ __device__ __forceinline__ void put_rows(T* to, int64_t stride, const T (&out)[k
   }
 }
 
-template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTeams * kTeam * 32) delta_backward(DeltaArgs a, int splits) {
+template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::kThreads) delta_backward(DeltaArgs a, int splits) {
   using B = Backward<T, DK>;
-  constexpr int NT = B::NT, NI = B::NI, NS = B::NS, kSteps = DK / 16, kStages = B::kStages;
+  constexpr int NT = B::NT, NI = B::NI, NS = B::NS, kSteps = DK / 16, kStages = P::kStages, kTeams = P::kTeams;
   using Keys = typename B::Keys;
   using Values = typename B::Values;
   extern __shared__ __align__(16) char smem[];
-  // main warps first (warp w of every team on the same quarter of the SM), then the ones that make
-  // chunks ready, then those of the matrices
+  // Main warps first (warp w of every team, and of the chain and the keys, on the same quarter of the SM:
+  // warps of the same task then run the same instructions at the same time), then the ones that
+  // make chunks ready, then those of the matrices.
+  enum { kFollow, kPrepare, kSquares };
   int warp = threadIdx.x >> 5, team, role;
-  if (warp < kTeams * kMain) {
-    role = 0;
-    team = warp / kMain;
-    warp %= kMain;
-  } else if (warp < kTeams * (kMain + kPrep)) {
-    role = 1;
-    team = (warp - kTeams * kMain) / kPrep;
-    warp = (warp - kTeams * kMain) % kPrep;
+  if (warp < kTeams * P::kAll) {
+    role = kFollow;
+    team = warp / P::kAll;
+    warp %= P::kAll;
+  } else if (warp < kTeams * (P::kAll + kPrep)) {
+    role = kPrepare;
+    team = (warp - kTeams * P::kAll) / kPrep;
+    warp = (warp - kTeams * P::kAll) % kPrep;
   } else {
-    role = 2;
-    team = warp - kTeams * (kMain + kPrep);
+    role = kSquares;
+    team = warp - kTeams * (P::kAll + kPrep);
   }
   const int64_t items = static_cast<int64_t>(a.batch) * a.heads * splits, item = static_cast<int64_t>(blockIdx.x) * kTeams + team;
   if (item >= items) return;
-  typename B::Shared& sh = reinterpret_cast<typename B::Shared*>(smem)[team];
-  const int bars = 1 + team * kBarTeam;
+  auto& sh = reinterpret_cast<typename B::template Shared<P>*>(smem)[team];
+  const int bars = 1 + team * P::kBars;
   const int block = static_cast<int>(item % splits), bh = static_cast<int>(item / splits), bi = bh / a.heads, h = bh % a.heads, gr = h / (a.heads / a.groups);
   const int lane = threadIdx.x & 31, row = lane >> 2, col = (lane & 3) * 2;
   const int vb = block * kValues, mine = min(kValues, a.values - vb);
@@ -158,7 +174,7 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
   const T* gb = static_cast<const T*>(a.b) + bi * a.b_b + h;
   const float rate = rate_at(a.A, h), bias = a.bias ? a.bias[h] : 0.0f;
 
-  if (role == 1) {
+  if (role == kPrepare) {
     const int w = warp, pitch = a.keys + kTile;
     const T* q = static_cast<const T*>(a.q) + bi * a.q_b + gr * a.q_g;
     const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
@@ -175,13 +191,14 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       }
     };
     ahead(count - 1 - w);
-    for (int i = w; i < count; i += kStages) {
-      typename B::Stage& st = sh.stage[w];
+    for (int i = w; i < count; i += kPrep) {
+      const int at = i % kStages;
+      typename B::Stage& st = sh.stage[at];
       const int tile = count - 1 - i, end = min(kTile, length - tile * kTile);
       const unsigned marks = look.get();
       const float now_dt = to_f(raw_dt), now_b = to_f(raw_b);
-      ahead(tile - kStages);
-      if (i >= kStages) bar_sync(bars + kBarFree + w, kStageThreads);
+      ahead(tile - kPrep);
+      if (i >= kStages) bar_sync(bars + P::kFree + at, P::kAtFree);
       const float* saved = a.saved + (((static_cast<int64_t>(bi) * tiles + tile) * a.heads + h) * a.values + vb) * pitch;
       bool bad = false;
       auto fetch = [&](int from, int n, unsigned mark, float x, float y) {
@@ -206,7 +223,7 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       };
       auto ready = [&](unsigned mark) {
         prepare<T, DK, true>(st.c, sh.scratch[w], &st.wide, st.tk, st.tq, mark, a.scale, a.unit);
-        bar_arrive(bars + kBarReady + w, kStageThreads);
+        bar_arrive(bars + P::kReady + at, P::kAtReady);
       };
       fetch(0, end, marks, now_dt, now_b);
       bool split = false;
@@ -224,10 +241,10 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       for (int to = end; to > 0;) {                    // the last episode first
         const int from = 31 - __clz((marks | 1u) & ((1u << to) - 1u));
         const unsigned mark = (marks >> from) & 1u;
-        if (to < end) bar_sync(bars + kBarFree + w, kStageThreads);
-        const int at = tile * kTile + from + lane;
+        if (to < end) bar_sync(bars + P::kFree + at, P::kAtFree);
+        const int token = tile * kTile + from + lane;
         const bool on = from + lane < to;
-        fetch(from, to - from, mark, on ? to_f(dt[at * a.dt_t]) : 0.0f, on ? to_f(gb[at * a.b_t]) : 0.0f);
+        fetch(from, to - from, mark, on ? to_f(dt[token * a.dt_t]) : 0.0f, on ? to_f(gb[token * a.b_t]) : 0.0f);
         if (lane == 0) st.more = from > 0;
         ready(mark);
         to = from;
@@ -236,20 +253,21 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
     return;
   }
 
-  if (role == 2) {
+  if (role == kSquares) {
     // the matrices and gates of 16 x 16
     const int64_t g_t = static_cast<int64_t>(a.heads) * splits, g_at = row0 * g_t + static_cast<int64_t>(h) * splits + block;
     double sum_a = 0.0, sum_bias = 0.0;
-    for (int i = 0, more = 0; i < count; i += more ? 0 : 1) {
-      const int at = i % kStages;
+    for (int i = 0, more = 0, unit = 0; i < count; i += more ? 0 : 1, ++unit) {
+      const int at = i % kStages, copy = unit % P::kCopies;
       typename B::Stage& st = sh.stage[at];
-      bar_sync(bars + kBarReady + at, kStageThreads);
+      const typename B::Chain& chain = sh.chain[copy];
+      bar_sync(bars + P::kReady + at, P::kAtReady);
       const int t0 = st.t0, n = st.n;
       const unsigned marks = st.marks;
       more = st.more;
       Gate gate{};
       if (lane < n) gate = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
-      bar_sync(bars + kBarChain, kMainThreads);
+      bar_sync(bars + P::kChain + copy, P::kAtChain);
       // lane: row r, columns j0 .. j0 + 7 of Z W^T and dO W^T. By rows: sums of E's part of P, of M, and Z.R
       const int r = lane >> 1, j0 = (lane & 1) * 8;
       const float rqr = st.c.rq[r], rkr = st.c.rk[r];
@@ -261,10 +279,10 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
 #pragma unroll
         for (int x = 0; x < kMain; ++x) {
           float y[4];
-          four(y, &sh.part[x].product[0][r][j]);
+          four(y, &chain.part[x].product[0][r][j]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) zw[e] += y[e];
-          four(y, &sh.part[x].product[1][r][j]);
+          four(y, &chain.part[x].product[1][r][j]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) ow[e] += y[e];
         }
@@ -318,10 +336,10 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       float wd = 0.0f, zv = 0.0f, f = 0.0f, inner = 0.0f;
 #pragma unroll
       for (int x = 0; x < kMain; ++x) {
-        wd += sh.by_value[x][0][c];
-        zv += sh.by_value[x][1][c];
-        f += sh.by_value[x][2][c];
-        inner += sh.inner[x];
+        wd += chain.by_value[x][0][c];
+        zv += chain.by_value[x][1][c];
+        f += chain.by_value[x][2][c];
+        inner += chain.inner[x];
       }
       float column = 0.0f, below = 0.0f, dbeta = wd;
 #pragma unroll
@@ -336,16 +354,19 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       row_p = __shfl_sync(0xffffffffu, row_p, 2 * c);
       row_m = __shfl_sync(0xffffffffu, row_m, 2 * c);
       zr = __shfl_sync(0xffffffffu, zr, 2 * c);
-      // the head's term of k, -Z.(head K S^T) = Z.R - Z.V
-      const float keep = marks & ((2u << c) - 1u) ? 0.0f : zr - zv;
+      // The head's term of k, -Z.(head K S^T): Z.R - Z.V with bfloat16 tokens, whose S^T Z has only two planes'
+      // digits; with 32-bit ones it comes from the keys, without the difference (ddt 1.3e-6 -> 4e-7 off
+      // where S is small).
+      const float keep = sizeof(T) == 4 || marks & ((2u << c) - 1u) ? 0.0f : zr - zv;
       if (lane < kTile) {
         sh.nq[c] = row_p;
         sh.nk[c] = keep + f + row_m + column;
       }
-      bar_sync(bars + kBarMatrices, kMainThreads);
+      bar_sync(bars + P::kMatrices, P::kAtMatrices);
+      if constexpr (P::kApart) bar_arrive(bars + P::kPlace + copy, P::kAtChain);
       float e = keep;
 #pragma unroll
-      for (int x = 0; x < kMain; ++x) e += sh.by_key[x][c];
+      for (int x = 0; x < kMain; ++x) e += sh.by_key[0][x][c] + sh.by_key[1][x][c];
       float dg = marks ? 0.0f : st.c.head[kTile - 1] * inner;
 #pragma unroll
       for (int j = 0; j < kTile; ++j) {
@@ -365,7 +386,7 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
         sum_bias += back;
       }
       __syncwarp();
-      bar_arrive(bars + kBarFree + at, kStageThreads);
+      bar_arrive(bars + P::kFree + at, P::kAtFree);
     }
     for (int o = 16; o; o >>= 1) {
       sum_a += __shfl_xor_sync(0xffffffffu, sum_a, o);
@@ -390,11 +411,26 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
   const int64_t v_t = static_cast<int64_t>(a.heads) * a.values;
   T* dv = static_cast<T*>(a.dv) + (row0 * a.heads + h) * a.values + vb;
   const bool pieces_v = a.values * sizeof(T) % 16 == 0, pieces_k = a.keys * sizeof(T) % 16 == 0;
+  const bool follows = !P::kApart || warp < kMain, keys = !P::kApart || warp >= kMain;       // the chain, the keys
+  warp %= kMain;
   const int vl = warp * 16, c0 = warp * B::kColumns, vsteps = (mine + 15) / 16;
   const bool by_v = vl < mine, by_k = c0 < DK && c0 < a.keys;
   constexpr int kPairs = B::kColumns / 16;
   float* dstate = a.dstate ? a.dstate + ((static_cast<int64_t>(bi) * a.heads + h) * a.values + vb) * a.keys : nullptr;
   const float* dfinal = a.dfinal ? a.dfinal + ((static_cast<int64_t>(bi) * a.heads + h) * a.values + vb) * a.keys : nullptr;
+
+  // S and W of the tiles from the last on, by the chain its own rows, on their way while the tile before is finished
+  const int pitch = a.keys + kTile;
+  const bool pieces_s = a.keys % 4 == 0;
+  const int64_t saved_tile = static_cast<int64_t>(a.heads) * a.values * pitch;
+  const float* saved = a.saved + (static_cast<int64_t>(bi) * tiles * a.heads + h) * a.values * pitch + static_cast<int64_t>(vb + vl) * pitch;
+  auto take = [&](int copy, int tile, bool w_too) {
+    if (!by_v) return;
+    const float* from = saved + tile * saved_tile;
+    load_rows(&sh.s[copy][vl][0], B::kPitchS, 16, DK, from, pitch, min(16, mine - vl), a.keys, pieces_s);
+    if (w_too) load_rows(&sh.saved_w[vl][0], kMat, 16, kTile, from + a.keys, pitch, min(16, mine - vl), kTile, pieces_s);
+    cp_async_commit();
+  };
 
   // d[n]: rows vl + row, + 8; keys 8 n + col, + 1
   float d[DK / 8][4];
@@ -406,24 +442,14 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       d[n][e] = dfinal && r < mine && kc < a.keys ? dfinal[r * a.keys + kc] : 0.0f;
     }
   // what a warp without values or columns leaves
-  for (int i = lane; i < 3 * kTile; i += 32) (&sh.by_value[warp][0][0])[i] = 0.0f;
-  if (lane < kTile) sh.by_key[warp][lane] = 0.0f;
-  if (lane == 0) sh.inner[warp] = 0.0f;
+  if (follows)
+    for (int copy = 0; copy < P::kCopies; ++copy) {
+      for (int i = lane; i < 3 * kTile; i += 32) (&sh.chain[copy].by_value[warp][0][0])[i] = 0.0f;
+      if (lane == 0) sh.chain[copy].inner[warp] = 0.0f;
+    }
+  if (keys && lane < kTile) sh.by_key[0][warp][lane] = sh.by_key[1][warp][lane] = 0.0f;
   __syncwarp();
 
-  // S and W of the tiles from the last on, each warp's own rows, on their way while the tile before is finished
-  const int pitch = a.keys + kTile;
-  const bool pieces_s = a.keys % 4 == 0;
-  const int64_t saved_tile = static_cast<int64_t>(a.heads) * a.values * pitch;
-  const float* saved = a.saved + (static_cast<int64_t>(bi) * tiles * a.heads + h) * a.values * pitch + static_cast<int64_t>(vb + vl) * pitch;
-  auto take = [&](int tile) {
-    if (!by_v) return;
-    const float* from = saved + tile * saved_tile;
-    load_rows(&sh.s[vl][0], B::kPitchS, 16, DK, from, pitch, min(16, mine - vl), a.keys, pieces_s);
-    load_rows(&sh.saved_w[vl][0], kMat, 16, kTile, from + a.keys, pitch, min(16, mine - vl), kTile, pieces_s);
-    cp_async_commit();
-  };
-  if (count > 0) take(count - 1);
   // tiles that all teams of the block have
   int common = 0;
   if constexpr (kTeams > 1) {
@@ -431,19 +457,11 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
     if (other < items) common = min(count, (length_of(static_cast<int>(other / splits) / a.heads) + kTile - 1) / kTile);
   }
 
-  for (int i = 0, more = 0, next = 1; i < count; i += more ? 0 : 1) {
-    const int at = i % kStages;
-    typename B::Stage& st = sh.stage[at];
+  auto follow_chain = [&](const typename B::Stage& st, typename B::Chain& chain) {
     const Chunk<T, NI>& c = st.c;
-    if (next && i < common) bar_sync(kBarAll, kTeams * kMain * 32);
-    bar_sync(bars + kBarReady + at, kStageThreads);
     const int t0 = st.t0, n = st.n;
     const unsigned marks = st.marks;
     const bool fresh = marks & 1u;                     // no token sees S
-    more = st.more;
-    next = !more;
-    cp_async_wait<0>();
-    __syncwarp();
     if (by_v) {
       // K dS^T (rows values, columns tokens), <dS, S>; dS's planes to shared memory
       float ds[2][4] = {}, inner = 0.0f;
@@ -455,19 +473,19 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
         uint32_t b[NT][4];
         load_planes<NT, false>(b, ka + x * 32, Keys::kPlane * 2);
         mma_planes<NI, NT>(ds[0], ds[1], f.r, b);
-        put_frag(sh.d, vl, 16 * x, f);
+        put_frag(chain.d, vl, 16 * x, f);
         if (!marks)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float2 s = *reinterpret_cast<const float2*>(&sh.s[vl + row + 8 * e][16 * x + 8 * t + col]);
+              const float2 s = *reinterpret_cast<const float2*>(&sh.s[0][vl + row + 8 * e][16 * x + 8 * t + col]);
               inner = fmaf(s.x, d[2 * x + t][2 * e], fmaf(s.y, d[2 * x + t][2 * e + 1], inner));
             }
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, o);
-      if (lane == 0) sh.inner[warp] = inner;
+      if (lane == 0) chain.inner[warp] = inner;
       // dU, Z
       float w[2][4], du[2][4] = {}, z[2][4] = {};
 #pragma unroll
@@ -539,12 +557,12 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
           }
         }
         f.from(z[0], z[1]);
-        put_tokens(sh.z, vl, f);
+        put_tokens(chain.z, vl, f);
         f.from(w[0], w[1]);
-        put_tokens(sh.w, vl, f);
+        put_tokens(chain.w, vl, f);
       }
       // sums over the warp's values, by tokens
-      T (&so)[kTile][16 + 16 / sizeof(T)] = sh.part[warp].out;
+      T (&so)[kTile][16 + 16 / sizeof(T)] = chain.part[warp].out;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -555,9 +573,9 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
           const float zv = column_sum(fmaf(z[t][e], v0, z[t][e + 2] * v1));
           const float send = column_sum(fmaf(w[t][e], ds[t][e], w[t][e + 2] * ds[t][e + 2]));
           if (row == 0) {
-            sh.by_value[warp][0][tok] = wd;
-            sh.by_value[warp][1][tok] = zv;
-            sh.by_value[warp][2][tok] = c.beta[tok] * send;
+            chain.by_value[warp][0][tok] = wd;
+            chain.by_value[warp][1][tok] = zv;
+            chain.by_value[warp][2][tok] = c.beta[tok] * send;
           }
           so[tok][row] = from_f<T>(z[t][e]);
           so[tok][row + 8] = from_f<T>(z[t][e + 2]);
@@ -568,8 +586,8 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       {
         uint32_t b[NI][4], x[NI][4], o[NT][4];
         float zw[2][4] = {}, ow[2][4] = {};
-        load_planes<NI, true>(b, smem_of(sh.w) + tokens_b(lane) + vl * kTile * 2, kValues * kTile * 2);
-        load_planes<NI, true>(x, smem_of(sh.z) + tokens_a(lane) + vl * kTile * 2, kValues * kTile * 2);
+        load_planes<NI, true>(b, smem_of(chain.w) + tokens_b(lane) + vl * kTile * 2, kValues * kTile * 2);
+        load_planes<NI, true>(x, smem_of(chain.z) + tokens_a(lane) + vl * kTile * 2, kValues * kTile * 2);
         mma_planes<NI, NI>(zw[0], zw[1], x, b);
         load_planes<NT, false>(o, smem_of(st.tdo) + a_rows(lane, Values::kPitch) + vl * 2, Values::kPlane * 2);
         mma_planes<NT, NI>(ow[0], ow[1], o, b);
@@ -577,8 +595,8 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            *reinterpret_cast<float2*>(&sh.part[warp].product[0][row + 8 * e][8 * t + col]) = make_float2(zw[t][2 * e], zw[t][2 * e + 1]);
-            *reinterpret_cast<float2*>(&sh.part[warp].product[1][row + 8 * e][8 * t + col]) = make_float2(ow[t][2 * e], ow[t][2 * e + 1]);
+            *reinterpret_cast<float2*>(&chain.part[warp].product[0][row + 8 * e][8 * t + col]) = make_float2(zw[t][2 * e], zw[t][2 * e + 1]);
+            *reinterpret_cast<float2*>(&chain.part[warp].product[1][row + 8 * e][8 * t + col]) = make_float2(ow[t][2 * e], ow[t][2 * e + 1]);
           }
       }
       // dS one chunk on
@@ -631,31 +649,37 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       }
     }
     else
-      for (int x = lane; x < 2 * kTile * kMat; x += 32) (&sh.part[warp].product[0][0][0])[x] = 0.0f;
-    bar_sync(bars + kBarChain, kMainThreads);
+      for (int x = lane; x < 2 * kTile * kMat; x += 32) (&chain.part[warp].product[0][0][0])[x] = 0.0f;
+  };
 
+  auto follow_keys = [&](const typename B::Stage& st, typename B::Chain& chain, int i, int copy) {
+    const Chunk<T, NI>& c = st.c;
+    const int t0 = st.t0, n = st.n;
+    const unsigned marks = st.marks;
+    const bool fresh = marks & 1u;                     // no token sees S
+    const int more = st.more;
     // by keys: rows tokens, columns c0 ..
     float aq[kPairs][2][4] = {}, ak[kPairs][2][4] = {};
     if (by_k) {
       float as[kPairs][2][4] = {};
       for (int x = 0; x < vsteps; ++x) {
         uint32_t o[NT][4], z[NS][4], w[NS][4];
-        load_planes<NS, true>(w, smem_of(sh.w) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
+        load_planes<NS, true>(w, smem_of(chain.w) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
         if (!fresh) {
           load_planes<NT, false>(o, smem_of(st.tdo) + a_rows(lane, Values::kPitch) + x * 32, Values::kPlane * 2);
-          load_planes<NS, true>(z, smem_of(sh.z) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
+          load_planes<NS, true>(z, smem_of(chain.z) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
         }
 #pragma unroll
         for (int p = 0; p < kPairs; ++p) {
           uint32_t b[NS][4];
-          load_planes<NS, true>(b, smem_of(sh.d) + at_cols(lane, B::kPitchD) + (x * 16 * B::kPitchD + c0 + 16 * p) * 2,
+          load_planes<NS, true>(b, smem_of(chain.d) + at_cols(lane, B::kPitchD) + (x * 16 * B::kPitchD + c0 + 16 * p) * 2,
                                 kValues * B::kPitchD * 2);
           mma_planes<NS, NS>(as[p][0], as[p][1], w, b);
           if (!fresh) {
             uint32_t s[NI][4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float* from = &sh.s[16 * x + (e & 1) * 8 + col][c0 + 16 * p + (e >> 1) * 8 + row];
+              const float* from = &sh.s[P::kCopies - 1][16 * x + (e & 1) * 8 + col][c0 + 16 * p + (e >> 1) * 8 + row];
               uint32_t y[NI];
               split2<NI>(from[0], from[B::kPitchS], y);
 #pragma unroll
@@ -666,7 +690,7 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
           }
         }
       }
-      float e0[2] = {}, hq[2], hk[2], tk[2];
+      float e0[2] = {}, e1[2] = {}, hq[2], hk[2], tk[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int tok = row + 8 * e;
@@ -693,6 +717,11 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
           for (int e = 0; e < 2; ++e) {
             float q0, q1;
             tile_pair<T>(st.tq, Keys::kPlane, (row + 8 * e) * Keys::kPitch + c0 + 16 * p + t * 8 + col, q0, q1);
+            if constexpr (sizeof(T) == 4) {
+              float k0, k1;
+              tile_pair<T>(st.tk, Keys::kPlane, (row + 8 * e) * Keys::kPitch + c0 + 16 * p + t * 8 + col, k0, k1);
+              e1[e] = fmaf(ak[p][t][2 * e], k0, fmaf(ak[p][t][2 * e + 1], k1, e1[e]));
+            }
 #pragma unroll
             for (int x = 2 * e; x < 2 * e + 2; ++x) {
               aq[p][t][x] *= hq[e];
@@ -703,11 +732,16 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         e0[e] = quad_sum(e0[e]);
-        if ((lane & 3) == 0) sh.by_key[warp][row + 8 * e] = e0[e] * c.rq[row + 8 * e];
+        if ((lane & 3) == 0) sh.by_key[0][warp][row + 8 * e] = e0[e] * c.rq[row + 8 * e];
+        if constexpr (sizeof(T) == 4) {
+          e1[e] = quad_sum(e1[e]);
+          if ((lane & 3) == 0) sh.by_key[1][warp][row + 8 * e] = e1[e] * hk[e] * c.rk[row + 8 * e];
+        }
       }
     }
-    bar_sync(bars + kBarMatrices, kMainThreads);       // S is read no more
-    if (!more && i + 1 < count) take(count - 2 - i);
+    bar_sync(bars + P::kMatrices, P::kAtMatrices);     // S is read no more
+    if constexpr (P::kApart) bar_arrive(bars + P::kPlace + copy, P::kAtChain);
+    if (!more && i + 1 < count) take(P::kCopies - 1, count - 2 - i, !P::kApart);
 
     if (by_k) {
       float nq[2] = {}, nk[2] = {}, rq[2], rk[2];
@@ -718,9 +752,12 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
         if (!a.unit) continue;
         nq[e] = sh.nq[row + 8 * e];
 #pragma unroll
-        for (int x = 0; x < kMain; ++x) nq[e] += sh.by_key[x][row + 8 * e];
+        for (int x = 0; x < kMain; ++x) {
+          nq[e] += sh.by_key[0][x][row + 8 * e];
+          nk[e] += sh.by_key[1][x][row + 8 * e];
+        }
         nq[e] *= rq[e];                                // what takes the part along q out of dq, for q itself
-        nk[e] = sh.nk[row + 8 * e] * rk[e];
+        nk[e] = (nk[e] + sh.nk[row + 8 * e]) * rk[e];
       }
       uint32_t x1[NS][4], x2[NS][4], x3[NS][4];
       load_planes<NS, false>(x1, smem_of(sh.x1) + a_rows(lane, kSide), kTile * kSide * 2);
@@ -759,7 +796,7 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
               a.part_k[qk_at + (t0 + tok) * qk_t + kc] = ak[p][t][e];
             }
         } else {
-          T (&so)[kTile][16 + 16 / sizeof(T)] = sh.part[warp].out;
+          T (&so)[kTile][16 + 16 / sizeof(T)] = *(P::kApart ? &sh.out[P::kApart ? warp : 0] : &chain.part[warp].out);
 #pragma unroll
           for (int turn2 = 0; turn2 < 2; ++turn2) {
             __syncwarp();
@@ -776,11 +813,55 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
         }
       }
     }
-    __syncwarp();
-    bar_arrive(bars + kBarFree + at, kStageThreads);
+  };
+
+  if constexpr (P::kApart) {
+    if (follows) {
+      if (count > 0) take(0, count - 1, true);
+      for (int i = 0, more = 0, unit = 0; i < count; i += more ? 0 : 1, ++unit) {
+        const int at = i % kStages, copy = unit & 1;
+        bar_sync(bars + P::kReady + at, P::kAtReady);
+        more = sh.stage[at].more;
+        if (unit > 1) bar_sync(bars + P::kPlace + copy, P::kAtChain);
+        cp_async_wait<0>();
+        __syncwarp();
+        follow_chain(sh.stage[at], sh.chain[copy]);
+        __syncwarp();
+        bar_arrive(bars + P::kChain + copy, P::kAtChain);
+        bar_arrive(bars + P::kFree + at, P::kAtFree);
+        if (!more && i + 1 < count) take(0, count - 2 - i, true);
+      }
+    } else {
+      if (count > 0) take(1, count - 1, false);
+      for (int i = 0, more = 0, unit = 0; i < count; i += more ? 0 : 1, ++unit) {
+        const int at = i % kStages, copy = unit & 1;
+        cp_async_wait<0>();                            // this warp's rows of S; all warps' with the barrier
+        bar_sync(bars + P::kChain + copy, P::kAtChain);
+        more = sh.stage[at].more;
+        follow_keys(sh.stage[at], sh.chain[copy], i, copy);
+        __syncwarp();
+        bar_arrive(bars + P::kFree + at, P::kAtFree);
+      }
+    }
+  } else {
+    if (count > 0) take(0, count - 1, true);
+    for (int i = 0, more = 0, next = 1; i < count; i += more ? 0 : 1) {
+      const int at = i % kStages;
+      if (next && i < common) bar_sync(P::kEvery, kTeams * kMain * 32);
+      bar_sync(bars + P::kReady + at, P::kAtReady);
+      more = sh.stage[at].more;
+      next = !more;
+      cp_async_wait<0>();
+      __syncwarp();
+      follow_chain(sh.stage[at], sh.chain[0]);
+      bar_sync(bars + P::kChain, P::kAtChain);
+      follow_keys(sh.stage[at], sh.chain[0], i, 0);
+      __syncwarp();
+      bar_arrive(bars + P::kFree + at, P::kAtFree);
+    }
   }
 
-  if (dstate && by_v) {
+  if (dstate && by_v && follows) {
 #pragma unroll
     for (int n = 0; n < DK / 8; ++n)
 #pragma unroll
@@ -790,6 +871,7 @@ template <typename T, int DK, int kTeams> __global__ void __launch_bounds__(kTea
       }
   }
   // tokens that are not there
+  if (!keys) return;
   for (int t = length + warp; t < a.length; t += kMain) {
     for (int x = lane; x < a.keys; x += 32) {
       const int64_t to = qk_at + t * qk_t + x;
@@ -850,16 +932,18 @@ template <typename T, int DK> int backward(const DeltaArgs& a, cudaStream_t s) {
   using B = Backward<T, DK>;
   const int splits = (a.values + kValues - 1) / kValues;
   if ((splits > 1 && !a.part_g) || (splits * a.heads != a.groups && !a.part_q)) return static_cast<int>(cudaErrorInvalidValue);
-  // one team a block as long as every head has an SM to itself
   const int64_t items = static_cast<int64_t>(a.batch) * a.heads * splits;
-  auto go = [&](auto n) {
-    constexpr int kTeams = decltype(n)::value;
-    constexpr size_t bytes = kTeams * sizeof(typename B::Shared);
-    if (const int e = allow_smem<delta_backward<T, DK, kTeams>>(bytes)) return e;
-    delta_backward<T, DK, kTeams><<<static_cast<unsigned>((items + kTeams - 1) / kTeams), kTeams * kTeam * 32, bytes, s>>>(a, splits);
+  auto go = [&](auto plan) {
+    using P = decltype(plan);
+    constexpr size_t bytes = P::kTeams * sizeof(typename B::template Shared<P>);
+    if (const int e = allow_smem<delta_backward<T, DK, P>>(bytes)) return e;
+    delta_backward<T, DK, P><<<static_cast<unsigned>((items + P::kTeams - 1) / P::kTeams), P::kThreads, bytes, s>>>(a, splits);
     return static_cast<int>(cudaGetLastError());
   };
-  if (const int e = items > 148 ? go(std::integral_constant<int, B::kTeams>()) : go(std::integral_constant<int, 1>())) return e;
+  using One = Plan<1, false>;
+  using Two = std::conditional_t<B::template kFits<Plan<2, false>>, Plan<2, false>, One>;
+  using Apart = std::conditional_t<B::template kFits<Plan<1, true>>, Plan<1, true>, One>;
+  if (const int e = items > 148 ? go(Two()) : go(Apart())) return e;
   delta_rates<<<a.heads, 32, 0, s>>>(a, splits);
   if (a.part_q && a.length > 0) {
     const int64_t grid = (static_cast<int64_t>(a.batch) * a.length * a.groups * a.keys + 255) / 256;
