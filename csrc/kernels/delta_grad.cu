@@ -34,13 +34,13 @@ template <int kTeams_, bool kApart_> struct Plan {
   static constexpr int kThreads = kTeams * (kAll + kPrep + 1) * 32;
   static constexpr int kStages = kApart ? 2 * kPrep : kPrep;           // a stage's barriers are one preparing warp's alone
   static constexpr int kCopies = kApart ? 2 : 1;                       // of what the chain leaves
-  // a team's barriers, and how many threads meet at them: stage s ready (chain, matrices, the warp that made
-  // it), stage s free (all of them), the chain's results (main, matrices), their place free (the
+  // a team's barriers, and how many threads meet at them: stage s ready (chain, the warp that made it),
+  // stage s free (all of them), the chain's results (main, matrices), their place free (the
   // same), the matrices (keys, matrices); one for the main warps of all teams
   static constexpr int kReady = 0, kFree = kStages, kChain = 2 * kStages, kPlace = kChain + kCopies, kMatrices = kPlace + (kApart ? 2 : 0);
   static constexpr int kBars = kMatrices + 1, kEvery = 1 + kTeams * kBars;
   static_assert(kEvery < 16, "barriers of a block");
-  static constexpr int kAtReady = (kMain + 2) * 32, kAtFree = (kAll + 2) * 32, kAtChain = (kAll + 1) * 32, kAtMatrices = (kMain + 1) * 32;
+  static constexpr int kAtReady = (kMain + 1) * 32, kAtFree = (kAll + 2) * 32, kAtChain = (kAll + 1) * 32, kAtMatrices = (kMain + 1) * 32;
 };
 
 template <typename T, int DK> struct Backward {
@@ -261,13 +261,13 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       const int at = i % kStages, copy = unit % P::kCopies;
       typename B::Stage& st = sh.stage[at];
       const typename B::Chain& chain = sh.chain[copy];
-      bar_sync(bars + P::kReady + at, P::kAtReady);
+      // the chunk was ready for the chain, which does not wait for this warp
+      bar_sync(bars + P::kChain + copy, P::kAtChain);
       const int t0 = st.t0, n = st.n;
       const unsigned marks = st.marks;
       more = st.more;
       Gate gate{};
       if (lane < n) gate = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
-      bar_sync(bars + P::kChain + copy, P::kAtChain);
       // lane: row r, columns j0 .. j0 + 7 of Z W^T and dO W^T. By rows: sums of E's part of P, of M, and Z.R
       const int r = lane >> 1, j0 = (lane & 1) * 8;
       const float rqr = st.c.rq[r], rkr = st.c.rk[r];
