@@ -47,6 +47,10 @@ template <typename T, int DK> struct Backward {
   static constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort;
   using Keys = Tile<T, DK>;
   using Values = Tile<T, kValues>;
+  // The head's term of k, -Z.(head K S^T): Z.R - Z.V with bfloat16 tokens, whose S^T Z has only two planes'
+  // digits; with 32-bit ones it comes from the keys, without the difference (ddt 1.3e-6 -> 3e-7 off
+  // where S is small).
+  static constexpr bool kByValues = sizeof(T) == 2;
   static constexpr int kPitchS = DK + 4, kPitchD = DK + 8, kPitchV = kValues + 16 / static_cast<int>(sizeof(T));
   static constexpr int kColumns = DK / kMain < 16 ? 16 : DK / kMain;     // of a warp by keys
   struct Stage {
@@ -55,14 +59,14 @@ template <typename T, int DK> struct Backward {
     int t0, n, more;                                   // more: the tile's next episode follows in this stage
     unsigned marks;
     alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize], tdo[Values::kSize];
-    alignas(16) T tv[kTile * kPitchV];
+    alignas(16) T tv[kByValues ? kTile * kPitchV : 8];
   };
   struct Chain {                                       // what the chain leaves of a chunk
     alignas(16) bf16 w[NI][kValues][kTile], z[NI][kValues][kTile];     // rows values, columns tokens; see swap8
     alignas(16) bf16 d[NS][kValues][kPitchD];          // dS
     // of each warp: Z W^T and dO W^T, or its outputs
     alignas(16) union { float product[2][kTile][kMat]; T out[kTile][16 + 16 / sizeof(T)]; } part[kMain];
-    float by_value[kMain][3][kTile], inner[kMain];     // sums over its values: W.dU, Z.V, the tails' terms; <dS, S>
+    float by_value[kMain][3][kTile], inner[kMain];     // sums over its values: W.dU, the tails' terms, Z.V; <dS, S>
   };
   template <typename P> struct Shared {
     Stage stage[P::kStages];
@@ -73,7 +77,8 @@ template <typename T, int DK> struct Backward {
     alignas(16) Scratch scratch[kPrep];
     Chain chain[P::kCopies];
     alignas(16) bf16 x1[NS][kTile][kSide], x2[NS][kTile][kSide], x3[NS][kTile][kSide];
-    alignas(16) T out[P::kApart ? kMain : 1][kTile][16 + 16 / sizeof(T)];
+    // outputs, where other warps have the chain's place in use: the chain's dV, the keys' dq and dk
+    alignas(16) T dv[P::kApart ? P::kCopies * kMain : 1][kTile][16 + 16 / sizeof(T)], out[P::kApart ? kMain : 1][kTile][16 + 16 / sizeof(T)];
     float by_key[2][kMain][kTile];                     // the head's terms of q and k
     float nq[kTile], nk[kTile];                        // q.dq and k.dk but for those
   };
@@ -88,11 +93,6 @@ __device__ __forceinline__ int swap8(int row, int token) { return token ^ ((row 
 __device__ __forceinline__ float quad_sum(float v) {   // over a row's four lanes
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
-}
-__device__ __forceinline__ float column_sum(float v) { // over a column's eight lanes
-  v += __shfl_xor_sync(0xffffffffu, v, 4);
-  v += __shfl_xor_sync(0xffffffffu, v, 8);
-  return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 template <int N, int R, int P> __device__ __forceinline__ void put_planes(bf16 (&m)[N][R][P], int i, int j, const uint32_t (&p)[N]) {
 #pragma unroll
@@ -206,7 +206,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
         Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k == 16);
         Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k == 16);
         Values::load(st.tdo, dout + t0 * a.do_t, a.do_t, n, mine, a.piece_v == 16);
-        load_rows(st.tv, B::kPitchV, kTile, kValues, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
+        if constexpr (B::kByValues) load_rows(st.tv, B::kPitchV, kTile, kValues, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
         cp_async_commit();
         Gate e{};
         if (lane < n) e = gate_of(x, y, bias, rate);
@@ -228,11 +228,10 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       fetch(0, end, marks, now_dt, now_b);
       bool split = false;
       if (marks & ~1u) {
-        float w_bad = 0.0f;
+        float w_bad = 0.0f;                            // a value that is not finite makes its token's W so
         for (int x = lane; x < mine * end; x += 32) w_bad = fmaf(saved[x / end * pitch + a.keys + x % end], 0.0f, w_bad);
         split = bad || __any_sync(0xffffffffu, w_bad != 0.0f) || not_finite(st.tk, Keys::kPitch, DK, end) ||
-                not_finite(st.tq, Keys::kPitch, DK, end) || not_finite(st.tdo, Values::kPitch, kValues, end) ||
-                not_finite(st.tv, B::kPitchV, kValues, end);
+                not_finite(st.tq, Keys::kPitch, DK, end) || not_finite(st.tdo, Values::kPitch, kValues, end);
       }
       if (!split) {
         ready(marks);
@@ -266,8 +265,11 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       const int t0 = st.t0, n = st.n;
       const unsigned marks = st.marks;
       more = st.more;
-      Gate gate{};
-      if (lane < n) gate = gate_of(to_f(dt[(t0 + lane) * a.dt_t]), to_f(gb[(t0 + lane) * a.b_t]), bias, rate);
+      T raw_dt = from_f<T>(0.0f), raw_b = raw_dt;      // on their way until the end
+      if (lane < n) {
+        raw_dt = dt[(t0 + lane) * a.dt_t];
+        raw_b = gb[(t0 + lane) * a.b_t];
+      }
       // lane: row r, columns j0 .. j0 + 7 of Z W^T and dO W^T. By rows: sums of E's part of P, of M, and Z.R
       const int r = lane >> 1, j0 = (lane & 1) * 8;
       const float rqr = st.c.rq[r], rkr = st.c.rk[r];
@@ -337,8 +339,8 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
 #pragma unroll
       for (int x = 0; x < kMain; ++x) {
         wd += chain.by_value[x][0][c];
-        zv += chain.by_value[x][1][c];
-        f += chain.by_value[x][2][c];
+        f += chain.by_value[x][1][c];
+        if constexpr (B::kByValues) zv += chain.by_value[x][2][c];
         inner += chain.inner[x];
       }
       float column = 0.0f, below = 0.0f, dbeta = wd;
@@ -354,10 +356,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       row_p = __shfl_sync(0xffffffffu, row_p, 2 * c);
       row_m = __shfl_sync(0xffffffffu, row_m, 2 * c);
       zr = __shfl_sync(0xffffffffu, zr, 2 * c);
-      // The head's term of k, -Z.(head K S^T): Z.R - Z.V with bfloat16 tokens, whose S^T Z has only two planes'
-      // digits; with 32-bit ones it comes from the keys, without the difference (ddt 1.3e-6 -> 4e-7 off
-      // where S is small).
-      const float keep = sizeof(T) == 4 || marks & ((2u << c) - 1u) ? 0.0f : zr - zv;
+      const float keep = !B::kByValues || marks & ((2u << c) - 1u) ? 0.0f : zr - zv;
       if (lane < kTile) {
         sh.nq[c] = row_p;
         sh.nk[c] = keep + f + row_m + column;
@@ -374,6 +373,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
         dg += j >= c ? ej : fj + st.wide.p[c][j];
       }
       if (lane < n) {
+        const Gate gate = gate_of(to_f(raw_dt), to_f(raw_b), bias, rate);
         const float back = dg * rate * sigmoid(gate.pre), b_back = dbeta * gate.beta * (1.0f - gate.beta);
         const int64_t to = g_at + (t0 + lane) * g_t;
         if (a.part_g) {
@@ -447,6 +447,22 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       for (int i = lane; i < 3 * kTile; i += 32) (&sh.chain[copy].by_value[warp][0][0])[i] = 0.0f;
       if (lane == 0) sh.chain[copy].inner[warp] = 0.0f;
     }
+  if (P::kApart && !by_v) {
+    for (int copy = 0; copy < P::kCopies; ++copy) {
+      auto zero = [&](auto& rows) {
+        for (int n = 0; n < NI; ++n)
+          for (int x = lane; x < 16 * kTile; x += 32) (&rows[n][vl][0])[x] = bf16(0.0f);
+      };
+      if (follows) {
+        zero(sh.chain[copy].w);
+        zero(sh.chain[copy].z);
+        for (int n = 0; n < NS; ++n)
+          for (int x = lane; x < 16 * B::kPitchD; x += 32) (&sh.chain[copy].d[n][vl][0])[x] = bf16(0.0f);
+      } else {
+        for (int x = lane; x < 16 * B::kPitchS; x += 32) (&sh.s[copy][vl][0])[x] = 0.0f;  // copy 1 is the keys'
+      }
+    }
+  }
   if (keys && lane < kTile) sh.by_key[0][warp][lane] = sh.by_key[1][warp][lane] = 0.0f;
   __syncwarp();
 
@@ -457,7 +473,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
     if (other < items) common = min(count, (length_of(static_cast<int>(other / splits) / a.heads) + kTile - 1) / kTile);
   }
 
-  auto follow_chain = [&](const typename B::Stage& st, typename B::Chain& chain) {
+  auto follow_chain = [&](const typename B::Stage& st, typename B::Chain& chain, int copy) {
     const Chunk<T, NI>& c = st.c;
     const int t0 = st.t0, n = st.n;
     const unsigned marks = st.marks;
@@ -561,27 +577,39 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
         f.from(w[0], w[1]);
         put_tokens(chain.w, vl, f);
       }
-      // sums over the warp's values, by tokens
-      T (&so)[kTile][16 + 16 / sizeof(T)] = chain.part[warp].out;
+      // sums over the warp's values, by tokens: halves of the sums change lanes until each has one token's
+      {
+        T (&so)[kTile][16 + 16 / sizeof(T)] = *(P::kApart ? &sh.dv[P::kApart ? copy * kMain + warp : 0] : &chain.part[warp].out);
+        float sum[3][2][2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int tok = t * 8 + col + e;
-          const float v0 = to_f(st.tv[tok * B::kPitchV + vl + row]), v1 = to_f(st.tv[tok * B::kPitchV + vl + row + 8]);
-          const float wd = column_sum(fmaf(w[t][e], du[t][e], w[t][e + 2] * du[t][e + 2]));
-          const float zv = column_sum(fmaf(z[t][e], v0, z[t][e + 2] * v1));
-          const float send = column_sum(fmaf(w[t][e], ds[t][e], w[t][e + 2] * ds[t][e + 2]));
-          if (row == 0) {
-            chain.by_value[warp][0][tok] = wd;
-            chain.by_value[warp][1][tok] = zv;
-            chain.by_value[warp][2][tok] = c.beta[tok] * send;
+          for (int e = 0; e < 2; ++e) {
+            const int tok = t * 8 + col + e;
+            sum[0][t][e] = fmaf(w[t][e], du[t][e], w[t][e + 2] * du[t][e + 2]);
+            sum[1][t][e] = fmaf(w[t][e], ds[t][e], w[t][e + 2] * ds[t][e + 2]);
+            if constexpr (B::kByValues)
+              sum[2][t][e] = fmaf(z[t][e], to_f(st.tv[tok * B::kPitchV + vl + row]), z[t][e + 2] * to_f(st.tv[tok * B::kPitchV + vl + row + 8]));
+            so[tok][row] = from_f<T>(z[t][e]);
+            so[tok][row + 8] = from_f<T>(z[t][e + 2]);
           }
-          so[tok][row] = from_f<T>(z[t][e]);
-          so[tok][row + 8] = from_f<T>(z[t][e + 2]);
+        const bool t1 = lane & 16, e1 = lane & 8;
+        const int tok = (t1 ? 8 : 0) + col + (e1 ? 1 : 0);
+#pragma unroll
+        for (int x = 0; x < (B::kByValues ? 3 : 2); ++x) {
+          float y[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) y[e] = (t1 ? sum[x][1][e] : sum[x][0][e]) + __shfl_xor_sync(0xffffffffu, t1 ? sum[x][0][e] : sum[x][1][e], 16);
+          float one = (e1 ? y[1] : y[0]) + __shfl_xor_sync(0xffffffffu, e1 ? y[0] : y[1], 8);
+          one += __shfl_xor_sync(0xffffffffu, one, 4);
+          if (!(lane & 4)) chain.by_value[warp][x][tok] = x == 1 ? c.beta[tok] * one : one;
         }
+        if constexpr (!P::kApart) {
+          __syncwarp();
+          put_rows(dv + t0 * v_t + vl, v_t, so, n, mine - vl, pieces_v);
+        }
+      }
       __syncwarp();
-      put_rows(dv + t0 * v_t + vl, v_t, so, n, mine - vl, pieces_v);
       // the warp's part of Z W^T and dO W^T
       {
         uint32_t b[NI][4], x[NI][4], o[NT][4];
@@ -660,9 +688,13 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
     const int more = st.more;
     // by keys: rows tokens, columns c0 ..
     float aq[kPairs][2][4] = {}, ak[kPairs][2][4] = {};
+    if (P::kApart && by_v) put_rows(dv + t0 * v_t + vl, v_t, sh.dv[P::kApart ? copy * kMain + warp : 0], n, mine - vl, pieces_v);
     if (by_k) {
       float as[kPairs][2][4] = {};
-      for (int x = 0; x < vsteps; ++x) {
+      // apart, all of a block's values unrolled, those that it does not have as zeros (864 -> 834 us at
+      // 2x4096x16x64x64); teams of two are bound by fetching instructions
+#pragma unroll (P::kApart ? kMain : 1)
+      for (int x = 0; x < (P::kApart ? kMain : vsteps); ++x) {
         uint32_t o[NT][4], z[NS][4], w[NS][4];
         load_planes<NS, true>(w, smem_of(chain.w) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
         if (!fresh) {
@@ -717,7 +749,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
           for (int e = 0; e < 2; ++e) {
             float q0, q1;
             tile_pair<T>(st.tq, Keys::kPlane, (row + 8 * e) * Keys::kPitch + c0 + 16 * p + t * 8 + col, q0, q1);
-            if constexpr (sizeof(T) == 4) {
+            if constexpr (!B::kByValues) {
               float k0, k1;
               tile_pair<T>(st.tk, Keys::kPlane, (row + 8 * e) * Keys::kPitch + c0 + 16 * p + t * 8 + col, k0, k1);
               e1[e] = fmaf(ak[p][t][2 * e], k0, fmaf(ak[p][t][2 * e + 1], k1, e1[e]));
@@ -733,7 +765,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       for (int e = 0; e < 2; ++e) {
         e0[e] = quad_sum(e0[e]);
         if ((lane & 3) == 0) sh.by_key[0][warp][row + 8 * e] = e0[e] * c.rq[row + 8 * e];
-        if constexpr (sizeof(T) == 4) {
+        if constexpr (!B::kByValues) {
           e1[e] = quad_sum(e1[e]);
           if ((lane & 3) == 0) sh.by_key[1][warp][row + 8 * e] = e1[e] * hk[e] * c.rk[row + 8 * e];
         }
@@ -825,7 +857,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
         if (unit > 1) bar_sync(bars + P::kPlace + copy, P::kAtChain);
         cp_async_wait<0>();
         __syncwarp();
-        follow_chain(sh.stage[at], sh.chain[copy]);
+        follow_chain(sh.stage[at], sh.chain[copy], copy);
         __syncwarp();
         bar_arrive(bars + P::kChain + copy, P::kAtChain);
         bar_arrive(bars + P::kFree + at, P::kAtFree);
@@ -853,7 +885,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       next = !more;
       cp_async_wait<0>();
       __syncwarp();
-      follow_chain(sh.stage[at], sh.chain[0]);
+      follow_chain(sh.stage[at], sh.chain[0], 0);
       bar_sync(bars + P::kChain, P::kAtChain);
       follow_keys(sh.stage[at], sh.chain[0], i, 0);
       __syncwarp();
