@@ -157,6 +157,11 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return bool(np.shares_memory(np.asarray(_Extent(a)), np.asarray(_Extent(b))))
 
 
+def within_float32(x: float) -> bool:
+    """A number that a kernel's float32 argument holds: finite there."""
+    return -3.4028234663852886e38 <= x <= 3.4028234663852886e38
+
+
 def require_apart(what: str, name: str, out: torch.Tensor, inputs: dict, in_place: tuple = ()) -> None:
     """Refuse an ``out`` whose elements share memory with one another or with an input: other
     threads read the inputs while it is written. It may be one of the inputs named in

@@ -83,6 +83,13 @@ def _check(what, q, k, v, dt, b, A, dt_bias, state, reset, lengths):
     return code, 4 - 2 * code, at, bsz, t, g, h, nk, nv
 
 
+def _scale(what: str, scale: Optional[float], keys: int) -> float:
+    scale = keys ** -0.5 if scale is None else float(scale)
+    if not _lib.within_float32(scale):
+        raise ValueError(f"{what}: scale must be finite in float32")
+    return scale
+
+
 def _piece(bits: int) -> int:
     return 16 if bits & 15 == 0 else 0
 
@@ -114,7 +121,7 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dt: torch.Ten
     args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt.data_ptr(), b.data_ptr(), A.data_ptr(), _p(dt_bias), _p(state),
                       _p(reset), _p(lengths), out.data_ptr(), final.data_ptr(), _p(saved), *(0,) * 14,
                       *_strides(q, k, v), *dt.stride()[:2], *b.stride()[:2], *_strides(out), 0, 0, 0,
-                      nk ** -0.5 if scale is None else scale, bsz, t, g, h, nk, nv, normalize,
+                      _scale(what, scale, nk), bsz, t, g, h, nk, nv, normalize,
                       _piece(_bits(e, q, k) | nk * e), _piece(_bits(e, v, out) | nv * e))
     launch(_lib.lib(DLIB).surf_delta, "surf_delta", at, args, code)
     return Delta(out, final, saved)
@@ -136,6 +143,8 @@ def gated_delta_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     if saved is None:
         raise ValueError(f"{what}: needs the states that gated_delta(train=True) saved")
     _dense(what, "saved", saved, (bsz, -(-t // TILE), h, nv, nk + TILE), f32, at)
+    if saved.data_ptr() & 15:
+        raise ValueError(f"{what}: saved must start on a 16-byte boundary")
     dq, dk, dv, ddt, db = (_like(x) for x in (q, k, v, dt, b))
     dA, dbias, dstate = torch.empty_like(A), None if dt_bias is None else torch.empty_like(dt_bias), \
         None if state is None else torch.empty_like(state)
@@ -151,7 +160,7 @@ def gated_delta_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
                       dv.data_ptr(), ddt.data_ptr(), db.data_ptr(), _p(dstate), base if n else 0,
                       base + 4 * n if n else 0, base + 8 * n if m else 0, base + 8 * n + 4 * m, dA.data_ptr(), _p(dbias),
                       *_strides(q, k, v), *dt.stride()[:2], *b.stride()[:2], 0, 0, 0, *_strides(dout),
-                      nk ** -0.5 if scale is None else scale, bsz, t, g, h, nk, nv, normalize,
+                      _scale(what, scale, nk), bsz, t, g, h, nk, nv, normalize,
                       _piece(_bits(e, q, k) | nk * e), _piece(_bits(e, v, dout) | nv * e))
     launch(_lib.lib(DLIB).surf_delta_grad, "surf_delta_grad", at, args, code)
     del ws                                     # the stream's next user comes after the launch
@@ -200,7 +209,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dt: torc
     args = _STEP.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt.data_ptr(), b.data_ptr(), A.data_ptr(), _p(dt_bias),
                       state.data_ptr(), _p(reset), _p(slots), out.data_ptr(), error_flag(q.device).data_ptr(), *q.stride()[:2],
                       *k.stride()[:2], *v.stride()[:2], dt.stride(0), b.stride(0), *out.stride()[:2],
-                      nk ** -0.5 if scale is None else scale, r, g, h, nk, nv, normalize, state.shape[0])
+                      _scale(what, scale, nk), r, g, h, nk, nv, normalize, state.shape[0])
     launch(_lib.lib(DLIB).surf_delta_step, "surf_delta_step", at, args, code)
     return out
 

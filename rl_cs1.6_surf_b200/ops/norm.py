@@ -60,8 +60,8 @@ def _check(what, x, groups, weight, bias, activation, eps):
         raise ValueError(f"{what}: the groups must divide the channels, {c} in {groups} do not")
     if activation not in ACTIVATIONS:
         raise ValueError(f"{what}: activation must be one of {', '.join(ACTIVATIONS)}, not {activation!r}")
-    if not eps > 0:
-        raise ValueError(f"{what}: eps must be positive")
+    if not 2.0 ** -126 <= eps or not _lib.within_float32(eps):
+        raise ValueError(f"{what}: eps must be positive and finite in float32")
     _tokens(what, "x", x, x.shape, x.dtype, at)
     _dense(what, "weight", weight, (c,), torch.float32, at)
     _dense(what, "bias", bias, (c,), torch.float32, at)
@@ -154,6 +154,8 @@ def group_norm_grad(dy: torch.Tensor, x: torch.Tensor, groups: int, weight: Opti
     if stats is None:
         raise ValueError(f"{what}: needs the statistics that group_norm(train=True) kept")
     _dense(what, "stats", stats, (x.shape[0], g, 2), torch.float32, at)
+    if stats.data_ptr() & 7:
+        raise ValueError(f"{what}: stats must start on an 8-byte boundary")
     n, p, xn, xp = _flat(what, "x", x)
     _, _, dn, dp = _flat(what, "dy", dy)
     dx = _like(x)

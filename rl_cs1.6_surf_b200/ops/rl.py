@@ -346,11 +346,11 @@ def policy_loss(logits: torch.Tensor, answers: torch.Tensor, old_logp: torch.Ten
     for name, t in (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp), ("weights", weights)):
         _loss_rows(name, t, rows, dev)
     high = clip if clip_high is None else clip_high
-    if not 0 <= clip <= 1 or not 0 <= high < math.inf:
+    if not 0 <= clip <= 1 or not (0 <= high and _lib.within_float32(high)):
         raise ValueError(f"{what}: clip lies in [0, 1], clip_high in [0, inf)")
-    if not 0 < temperature < math.inf:
+    if not (2.0 ** -126 <= temperature and _lib.within_float32(temperature)):
         raise ValueError(f"{what}: the temperature must be positive and finite")
-    if not (math.isfinite(kl_coef) and math.isfinite(ent_coef)):
+    if not (_lib.within_float32(kl_coef) and _lib.within_float32(ent_coef)):
         raise ValueError(f"{what}: kl_coef and ent_coef must be finite")
     if out is not None:
         if not grad:
@@ -359,6 +359,8 @@ def policy_loss(logits: torch.Tensor, answers: torch.Tensor, old_logp: torch.Ten
             raise ValueError(f"{what}: out must be like the logits, with a dense last axis")
         _lib.require_apart(what, "out", out, dict(logits=logits, answers=answers, old_logp=old_logp, advantages=advantages,
                                                   ref_logp=ref_logp, weights=weights), ("logits",))
+        if rows > 1 and out.stride(0) < v:
+            raise ValueError(f"{what}: out has rows that share memory")
     elif grad:
         out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(logits.shape)
     stats = torch.empty(4 * rows + 1, dtype=torch.float32, device=dev)

@@ -407,3 +407,89 @@ def test_refusals():
         DR.gated_delta_step(*one, A, torch.zeros(2 * 4 * 256 + 1, device="cuda")[1:].view(2, 4, 16, 16))
     with pytest.raises(ValueError, match="out shares memory"):
         DR.gated_delta_step(*one, A, c["state"].clone(), out=one[2])
+
+
+MANY = [  # more heads of sequences than SMs: two share a block in the gradient, the last may be alone
+    (151, 37, 1, 1, 16, 16, 0.1, True), (50, 70, 1, 3, 64, 64, 0.1, True), (77, 35, 2, 2, 32, 24, 0.0, True),
+    (40, 33, 2, 4, 64, 128, 0.2, True), (160, 20, 1, 1, 128, 64, 0.0, False), (149, 1, 1, 1, 40, 33, 0.0, False),
+    (151, 50, 1, 1, 65, 100, 0.3, True),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("case", MANY)
+def test_many_sequences(case, dtype):
+    test_sequences_and_gradients(case, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("which", ["token", "state", "dfinal"])
+def test_not_finite_stays_in_its_row_among_many(dtype, which):
+    """Row 6 is bad, between two episodes inside a tile for a token; row 7 shares its block in the gradient."""
+    c = make(151, 50, 1, 1, 32, 32, dtype, ragged=True)
+    c["reset"] = torch.zeros(151, 50, dtype=torch.bool, device="cuda")
+    c["reset"][:, [21, 26]] = True
+    c["lengths"][5:8] = torch.tensor([50, 50, 33], dtype=torch.int32, device="cuda")
+    c["tokens"] = tuple(torch.nan_to_num(x) for x in c["tokens"])
+    c["dout"] = torch.nan_to_num(c["dout"])
+    clean = call(c)
+    for name in ("state", "dfinal"):
+        if which == name:
+            c[name] = c[name].clone()
+            c[name][6] = float("nan")
+    if which == "token":
+        c["tokens"] = tuple(x.clone() for x in c["tokens"])
+        c["tokens"][2][6, 23] = float("inf")
+    r, d = call(c)
+    rows = torch.arange(151, device="cuda") != 6
+    assert torch.equal(r.out[rows], clean[0].out[rows]) and torch.equal(r.final[rows], clean[0].final[rows])
+    for x, y in zip(d[:5] + (d.dstate,), clean[1][:5] + (clean[1].dstate,)):
+        assert torch.equal(x[rows], y[rows])
+    # the row's own tokens of other episodes than the bad one
+    keep = {"token": [*range(21), *range(26, 50)], "state": [*range(21, 50)], "dfinal": [*range(26)]}[which]
+    tol = torch.finfo(dtype).eps
+    for x, y in zip(d[:5], clean[1][:5]):
+        assert rel(x[6, keep], y[6, keep]) < 2 * INNER[dtype] + tol
+
+
+def test_odd_saved_and_scales_past_float32_are_refused():
+    c = make(2, 10, 1, 1, 16, 16, BF)
+    saved = call(c)[0].saved
+    odd = torch.empty(1 + saved.numel(), device="cuda")[1:].view(saved.shape)
+    odd.copy_(saved)
+    with pytest.raises(ValueError, match="16-byte"):
+        DR.gated_delta_grad(c["dout"], *c["tokens"], c["A"], saved=odd)
+    for scale in (1e39, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            DR.gated_delta(*c["tokens"], c["A"], scale=scale)
+        with pytest.raises(ValueError, match="scale"):
+            DR.gated_delta_step(*(x[:, 0] for x in c["tokens"]), c["A"], c["state"], scale=scale)
+
+
+def test_two_calls_at_once():
+    for case in ((3, 60, 1, 2, 64, 64), (160, 40, 1, 1, 32, 48)):
+        c = make(*case, BF, reset=0.1, ragged=True)
+        want, grads = call(c)
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream() for _ in range(2)], []
+        for s in streams * 3:
+            with torch.cuda.stream(s):
+                got.append(call(c))
+        torch.cuda.synchronize()
+        for r, d in got:
+            assert torch.equal(r.out, want.out) and torch.equal(r.final, want.final)
+            for x, y in zip(d, grads):
+                assert torch.equal(x, y)
+
+
+def test_shared_rows_as_inputs():
+    """Views whose rows lie on one another: gradients are dense, each row's own."""
+    c = make(1, 40, 1, 2, 32, 32, F32)
+    c["tokens"] = tuple(x.expand(5, *x.shape[1:]) for x in c["tokens"])
+    c["dout"] = c["dout"].expand(5, *c["dout"].shape[1:])
+    c["state"], c["dfinal"] = (c[n].expand(5, *c[n].shape[1:]).contiguous() for n in ("state", "dfinal"))
+    r, d = call(c)
+    _, _, want = oracle(c)
+    assert rel(r.out[4], r.out[0]) == 0
+    for n, x in zip(NAMES, d):
+        assert rel(x, want[n]) < 2 * INNER[F32] + torch.finfo(F32).eps, n

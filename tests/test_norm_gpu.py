@@ -185,3 +185,37 @@ def test_refusals():
         N.group_norm_grad(dy, x, 4, stats=None)
     with pytest.raises(ValueError, match="stats has shape"):
         N.group_norm_grad(dy, x, 4, stats=torch.zeros(4, 2, 2, device="cuda"))
+
+
+def test_numbers_past_float32_and_odd_statistics_are_refused():
+    x = torch.randn(4, 6, 32, device="cuda")
+    for eps in (1e39, 1e-39, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="eps"):
+            N.group_norm(x, 4, eps=eps)
+    stats = N.group_norm(x, 4, train=True).stats
+    odd = torch.empty(1 + stats.numel(), device="cuda")[1:].view(stats.shape)
+    odd.copy_(stats)
+    with pytest.raises(ValueError, match="8-byte"):
+        N.group_norm_grad(x, x, 4, stats=odd)
+
+
+@pytest.mark.parametrize("shape,groups", [((40, 96), 3), ((300, 200, 32), 4), ((1, 5000, 24), 3)])
+def test_weights_at_odd_addresses_and_two_calls_at_once(shape, groups):
+    gen = torch.Generator("cuda").manual_seed(5)
+    c = shape[-1]
+    x, dy = (torch.randn(*shape, generator=gen, device="cuda") for _ in range(2))
+    flat = torch.randn(2 * c + 1, generator=gen, device="cuda")
+    w, b = flat[1:c + 1], flat[c + 1:]
+    whole = N.group_norm(x, groups, w.clone(), b.clone(), activation="silu", train=True)
+    grads = N.group_norm_grad(dy, x, groups, w.clone(), b.clone(), stats=whole.stats, activation="silu")
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams * 3:
+        with torch.cuda.stream(s):
+            y = N.group_norm(x, groups, w, b, activation="silu", train=True)
+            got.append((y, N.group_norm_grad(dy, x, groups, w, b, stats=y.stats, activation="silu")))
+    torch.cuda.synchronize()
+    for y, g in got:
+        assert torch.equal(y.out, whole.out) and torch.equal(y.stats, whole.stats)
+        for a, e in zip(g, grads):
+            assert torch.equal(a, e)

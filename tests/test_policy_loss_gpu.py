@@ -261,3 +261,30 @@ def test_refusals():
         call(c, out=torch.as_strided(c["logits"], (4, 20), (19, 1)))
     with pytest.raises(_lib.KernelError):
         R.policy_loss(*(c[k].cpu() for k in ("logits", "answers", "old_logp", "advantages")))
+
+
+def test_numbers_past_float32_and_rows_that_share_memory_are_refused():
+    c = make(4, 20, F32)
+    for bad in (dict(clip_high=1e39), dict(temperature=1e-39), dict(temperature=1e39), dict(kl_coef=1e39), dict(ent_coef=-1e300)):
+        with pytest.raises(ValueError):
+            call(c, **bad)
+    with pytest.raises(ValueError, match="share memory"):
+        call(c, out=torch.zeros(80, device="cuda").as_strided((4, 20), (10, 1)))
+    rows = torch.zeros(80, device="cuda").as_strided((4, 20), (10, 1))
+    with pytest.raises(ValueError, match="share memory"):
+        call(dict(c, logits=rows), out=rows)
+
+
+def test_two_calls_at_once():
+    # the same rows on two streams, neither waiting for the other
+    for v, dtype in ((15, F32), (700, BF), (60000, BF)):
+        c = make(64, v, dtype)
+        want = call(c, kl_coef=0.1)
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream() for _ in range(2)], []
+        for s in streams * 4:
+            with torch.cuda.stream(s):
+                got.append(call(c, kl_coef=0.1))
+        torch.cuda.synchronize()
+        for r in got:
+            assert torch.equal(r.loss, want.loss) and torch.equal(r.dlogits, want.dlogits) and torch.equal(r.logp, want.logp)
