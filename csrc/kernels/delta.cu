@@ -39,7 +39,9 @@ template <typename T, int DK> struct Forward {
 // (tiles, decays, P, the inverse: nothing of it waits for the state), the others hold 16 values'
 // rows of the state each, as accumulators from the first token to the last. They meet at
 // numbered barriers: stage s is ready (1 + s), stage s is free (1 + kStages + s).
-template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kPrep + kMain) * 32, kBlocks) delta_forward(DeltaArgs a, int bulk) {
+// kKeep: for the gradient. Calls that keep nothing are kernels of their own (1x8191x8x128x128 1054 -> XXX us).
+template <typename T, int DK, int kBlocks, bool kKeep>
+__global__ void __launch_bounds__((kPrep + kMain) * 32, kBlocks) delta_forward(DeltaArgs a, int bulk) {
   constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort, kSteps = DK / 16;
   using F = Forward<T, DK>;
   using Keys = Tile<T, DK>;
@@ -193,8 +195,8 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
     // The state before the tile and W, for the gradient: rows of both side by side, as one bulk copy from
     // shared memory where that is allowed (stored lane by lane they held the chain up: 2x4096x16x64x64
     // 449 us).
-    float* saved = a.saved ? a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values * pitch_s : nullptr;
-    const bool copied = bulk && t0 % kTile == 0 && !more;
+    float* saved = kKeep ? a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values * pitch_s : nullptr;
+    const bool copied = kKeep && bulk && t0 % kTile == 0 && !more;
     if (copied) {
       if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
@@ -364,7 +366,7 @@ template <typename T, int DK, int kBlocks> __global__ void __launch_bounds__((kP
     __syncwarp();
   }
   store(a.final_ + head_at, a.keys);
-  if (bulk && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (kKeep && bulk && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   // tokens that are not there give zeros
   for (int t = length + warp; t < a.length; t += warps)
     for (int j = lane; j < mine; j += 32) out[t * a.o_t + vb + j] = from_f<T>(0.0f);
@@ -383,10 +385,13 @@ template <typename T, int DK> int forward(const DeltaArgs& a, cudaStream_t s) {
   const size_t kept = F::kept_bytes(warps, a.keys);
   const bool bulk = a.saved && a.keys % 4 == 0 && F::bytes(warps) + kept <= (blocks > 148 && kBlocks > 1 ? 113 : 227) * 1024;
   constexpr size_t kMost = F::bytes(kMain) + F::kept_bytes(kMain, DK);
-  if (const int e = allow_smem<delta_forward<T, DK, kBlocks>>(kMost < 227 * 1024 ? kMost : 227 * 1024)) return e;
-  delta_forward<T, DK, kBlocks><<<dim3(a.batch * a.heads, (all + warps - 1) / warps), (warps + kPrep) * 32,
-                                  F::bytes(warps) + (bulk ? kept : 0), s>>>(a, bulk);
-  return static_cast<int>(cudaGetLastError());
+  auto go = [&](auto keep) {
+    constexpr auto kernel = delta_forward<T, DK, kBlocks, decltype(keep)::value>;
+    if (const int e = allow_smem<kernel>(kMost < 227 * 1024 ? kMost : 227 * 1024)) return e;
+    kernel<<<dim3(a.batch * a.heads, (all + warps - 1) / warps), (warps + kPrep) * 32, F::bytes(warps) + (bulk ? kept : 0), s>>>(a, bulk);
+    return static_cast<int>(cudaGetLastError());
+  };
+  return a.saved ? go(std::true_type()) : go(std::false_type());
 }
 template <typename T> int forward_by(const DeltaArgs& a, cudaStream_t s) {
   if (a.keys <= 32) return forward<T, 32>(a, s);

@@ -481,24 +481,31 @@ template <typename T, int V, int H> __global__ void __launch_bounds__(kBlockThre
       if (k < count)
         store<T, V>(y + k * (at.rows * a.ys_p), (d[k] + fma(xh[k], Nums<V>::all(-m2), Nums<V>::all(-m1))) * Nums<V>::all(st.y));
   }
-  // the channels' sums, the block's rows in order
-  float* out = a.part + static_cast<int64_t>(block) * 2 * a.c + at.c0 - at.piece * V;
+  // the channels' sums, from every row's in shared memory: as many lanes an output as there are rows, 32
+  // at most (by one thread an output the rows' chain took 15 us)
+  float* all = reinterpret_cast<float*>(smem);
   float both[2][V];
   sw.put(both[0]);
   sb.put(both[1]);
+  __syncthreads();
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-#pragma unroll
-    for (int turn = 0; turn < 2; ++turn) {
-      __syncthreads();
-      red[threadIdx.x] = at.on ? both[turn][j] : 0.0f;
-      __syncthreads();
-      if (static_cast<int>(threadIdx.x) < at.per) {
-        float s = 0.0f;
-        for (int i = 0; i < at.rows; ++i) s += red[i * at.per + threadIdx.x];
-        out[turn * a.c + threadIdx.x * V + j] = s;
-      }
-    }
+  for (int j = 0; j < V; ++j) {
+    all[j * blockDim.x + threadIdx.x] = both[0][j];
+    all[(V + j) * blockDim.x + threadIdx.x] = both[1][j];
+  }
+  __syncthreads();
+  float* out = a.part + static_cast<int64_t>(block) * 2 * a.c + at.c0 - at.piece * V;
+  int share = 32;
+  while (share > at.rows) share >>= 1;
+  const int outs = at.per * 2 * V, lane = threadIdx.x & 31;
+  for (int first = (threadIdx.x & ~31u) / share; first < outs; first += blockDim.x / share) {
+    const int o = first + lane / share, piece = o % at.per, slot = o / at.per;
+    float s = 0.0f;
+    if (o < outs)
+      for (int i = lane % share; i < at.rows; i += share) s += all[slot * blockDim.x + i * at.per + piece];
+    for (int x = share >> 1; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    if (o < outs && lane % share == 0) out[(slot >= V ? a.c : 0) + piece * V + slot % V] = s;
+  }
 }
 
 // ---- parts ------------------------------------------------------------------------------

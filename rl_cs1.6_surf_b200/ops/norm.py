@@ -99,7 +99,7 @@ def _plan(n: int, p: int, c: int, g: int, e: int, v: int, grad: bool):
             -(-p // (threads // (k * per_group))) <= most]
     slab = next((k for k in fits if k * cg * e >= 32), fits[-1] if fits else 0)
     slab = next((k for k in fits if k >= 2 * slab and n * (g // k) >= 148 * 3), slab)
-    if slab and n * (g // slab) >= 74:
+    if slab and n * (g // slab) >= (74 if grad else 1):
         per = slab * per_group
         hold = -(-p // (threads // per))
         # no more threads than the pieces take

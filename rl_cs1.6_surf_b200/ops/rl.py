@@ -305,7 +305,7 @@ def _loss_blocks(rows: int, v: int, e: int):
     if v <= 512:
         return 0, v
     ranks = 1
-    while ranks < 8 and (v * e > ranks * 100 * 1024 or (rows * ranks < 148 and v * e > ranks * 16384)):
+    while ranks < 8 and (v * e > ranks * 100 * 1024 or (rows * ranks * 2 <= 148 and v * e > ranks * 16384)):
         ranks *= 2
     return ranks, -(-v // (ranks * 16)) * 16
 
