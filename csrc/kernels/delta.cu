@@ -38,8 +38,12 @@ template <typename T, int DK> struct Forward {
 // A block for up to 64 values of a sequence's value head. Two warps make the chunks ready in turn
 // (tiles, decays, P, the inverse: nothing of it waits for the state), the others hold 16 values'
 // rows of the state each, as accumulators from the first token to the last. They meet at
-// numbered barriers: stage s is ready (1 + s), stage s is free (1 + kStages + s).
-// kKeep: for the gradient. Calls that keep nothing are kernels of their own (1x8191x8x128x128 1054 -> XXX us).
+// numbered barriers: stage s is ready (1 + s), stage s is free (1 + kStages + s). With few blocks the chain
+// from state to state bounds it (64 keys: 1.8 thousand cycles a chunk of one warp's products, each
+// waiting for the one before, against 0.1 of memory), with many the same warps' waits and instructions
+// (256x128x8x64x64: 0.38 a cycle and scheduler, tensor pipe 26%, 0.42 of the copy rate).
+// kKeep: for the gradient. Calls that keep nothing are kernels of their own (1x8191x8x128x128 1054 -> 745 us,
+// 2x4096x16x64x64 313 -> 248 us).
 template <typename T, int DK, int kBlocks, bool kKeep>
 __global__ void __launch_bounds__((kPrep + kMain) * 32, kBlocks) delta_forward(DeltaArgs a, int bulk) {
   constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort, kSteps = DK / 16;
@@ -375,13 +379,14 @@ __global__ void __launch_bounds__((kPrep + kMain) * 32, kBlocks) delta_forward(D
 template <typename T, int DK> int forward(const DeltaArgs& a, cudaStream_t s) {
   using F = Forward<T, DK>;
   constexpr int kBlocks = sizeof(T) == 4 && DK == 128 ? 1 : 2;
-  // values of a block: as many as it takes, or fewer where that leaves SMs without one
+  // values of a block: as many as it takes, or fewer where that leaves SMs without one (2x4096x16x64x64,
+  // states kept: 361 us; with 64 a block 385)
   const int all = (a.values + 15) / 16;
   int warps = all < kMain ? all : kMain;
   while (warps > 1 && static_cast<int64_t>(a.batch) * a.heads * ((all + warps - 1) / warps) < 148) warps = (warps + 1) / 2;
   const int64_t blocks = static_cast<int64_t>(a.batch) * a.heads * ((all + warps - 1) / warps);
-  // bulk copies of what is kept want rows of whole 16 bytes, and shared memory that would cost many
-  // blocks their neighbour on the SM
+  // bulk copies of what is kept want rows of whole 16 bytes, and no shared memory that would cost many
+  // blocks their neighbour on the SM (lane by lane 2x4096x16x64x64 takes 428 us, 361 so; 256x128x8x64x64 167, 158)
   const size_t kept = F::kept_bytes(warps, a.keys);
   const bool bulk = a.saved && a.keys % 4 == 0 && F::bytes(warps) + kept <= (blocks > 148 && kBlocks > 1 ? 113 : 227) * 1024;
   constexpr size_t kMost = F::bytes(kMain) + F::kept_bytes(kMain, DK);
@@ -417,6 +422,8 @@ static_assert(sizeof(StepArgs) == 12 * 8 + 10 * 8 + 8 * 4, "as the caller packs 
 // A warp for `per` values of a head of a row (blockIdx.y): its lanes hold the key and the query, LK
 // lanes a value's row of the state. S k and S q come from one look at the state:
 //   u = beta (v - e^g S k),  S <- e^g S + u k^T,  o = scale (e^g S q + u k.q).
+// Bound by the state's bytes: 2048x8x64x64 97 us, 0.86 of the copy rate, with four rows a lane on their way
+// (one: 119 us).
 template <typename T, int LK> __global__ void __launch_bounds__(256) delta_step(StepArgs a, int per) {
   constexpr int kRows = 32 / LK;                       // values that a warp takes at once
   const int lane = threadIdx.x & 31;
@@ -527,7 +534,7 @@ template <typename T> int step(const StepArgs& a, cudaStream_t s) {
   auto go = [&](auto lanes) {
     constexpr int LK = decltype(lanes)::value;
     // a head's values in as many warps as give every SM 32, of at least the rows that are on their way
-    // at once: 64 rows of 8 heads of 64 x 64 in 1 and 8 warps a head
+    // at once: 64 rows of 8 heads of 64 x 64 take 11.9 us in one warp a head and 5.5 in four
     const int least = 4 * (32 / LK), most = (a.values + least - 1) / least;
     int parts = static_cast<int>(heads >= 148 * 32 ? 1 : (148 * 32 + heads - 1) / heads);
     parts = parts < most ? parts : most;

@@ -427,6 +427,33 @@ template <typename T, int V, int H> __global__ void __launch_bounds__(kBlockThre
   }
 }
 
+// The rows' sums of each of `per` pieces, from threads row * per + piece, to out[0 .. ] and out[c .. ] for columns
+// below `cols`: through 2 V floats a thread of shared memory, with as many lanes an output as there are rows, 32 at
+// most (by one thread an output the rows' chain took 15 us at 128 rows).
+template <int V> __device__ __forceinline__ void sum_rows(const Nums<V>& sw, const Nums<V>& sb, float* all, int rows, int per, int cols,
+                                                          int c, float* out) {
+  float both[2][V];
+  sw.put(both[0]);
+  sb.put(both[1]);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    all[j * blockDim.x + threadIdx.x] = both[0][j];
+    all[(V + j) * blockDim.x + threadIdx.x] = both[1][j];
+  }
+  __syncthreads();
+  int share = 32;
+  while (share > rows) share >>= 1;
+  const int outs = per * 2 * V, lane = threadIdx.x & 31;
+  for (int first = (threadIdx.x & ~31u) / share; first < outs; first += blockDim.x / share) {
+    const int o = first + lane / share, piece = o % per, slot = o / per;
+    float s = 0.0f;
+    if (o < outs)
+      for (int i = lane % share; i < rows; i += share) s += all[slot * blockDim.x + i * per + piece];
+    for (int x = share >> 1; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    if (o < outs && lane % share == 0 && piece * V < cols) out[(slot >= V ? c : 0) + piece * V + slot % V] = s;
+  }
+}
+
 // Its gradient, x and dy a sample ahead.
 template <typename T, int V, int H> __global__ void __launch_bounds__(kBlockThreads / 2, 2) norm_block_grad(NormArgs a) {
   using A = Ahead<T, V, H>;
@@ -481,31 +508,10 @@ template <typename T, int V, int H> __global__ void __launch_bounds__(kBlockThre
       if (k < count)
         store<T, V>(y + k * (at.rows * a.ys_p), (d[k] + fma(xh[k], Nums<V>::all(-m2), Nums<V>::all(-m1))) * Nums<V>::all(st.y));
   }
-  // the channels' sums, from every row's in shared memory: as many lanes an output as there are rows, 32
-  // at most (by one thread an output the rows' chain took 15 us)
-  float* all = reinterpret_cast<float*>(smem);
-  float both[2][V];
-  sw.put(both[0]);
-  sb.put(both[1]);
+  // the channels' sums
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    all[j * blockDim.x + threadIdx.x] = both[0][j];
-    all[(V + j) * blockDim.x + threadIdx.x] = both[1][j];
-  }
-  __syncthreads();
-  float* out = a.part + static_cast<int64_t>(block) * 2 * a.c + at.c0 - at.piece * V;
-  int share = 32;
-  while (share > at.rows) share >>= 1;
-  const int outs = at.per * 2 * V, lane = threadIdx.x & 31;
-  for (int first = (threadIdx.x & ~31u) / share; first < outs; first += blockDim.x / share) {
-    const int o = first + lane / share, piece = o % at.per, slot = o / at.per;
-    float s = 0.0f;
-    if (o < outs)
-      for (int i = lane % share; i < at.rows; i += share) s += all[slot * blockDim.x + i * at.per + piece];
-    for (int x = share >> 1; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    if (o < outs && lane % share == 0) out[(slot >= V ? a.c : 0) + piece * V + slot % V] = s;
-  }
+  sum_rows<V>(sw, sb, reinterpret_cast<float*>(smem), at.rows, at.per, a.c - at.c0 + at.piece * V, a.c,
+              a.part + static_cast<int64_t>(block) * 2 * a.c + at.c0 - at.piece * V);
 }
 
 // ---- parts ------------------------------------------------------------------------------
@@ -596,16 +602,30 @@ template <typename T, int V> __global__ void __launch_bounds__(kBlockThreads) no
   }
 }
 
-// Sums of d xh and d over the positions of a part: [N, parts, 2, C].
+// A block of the gradient by parts: 32 pieces of channels by 8 positions, or fewer by more where
+// the channels are fewer.
 constexpr int kPartThreads = 256;
+struct Cells {
+  int cols, rows, piece, row;
+  __device__ __forceinline__ explicit Cells(int pieces) {
+    int log = 5;
+    while (log > 0 && 1 << (log - 1) >= pieces) --log;
+    cols = 1 << log;
+    rows = kPartThreads >> log;
+    piece = threadIdx.x & (cols - 1);
+    row = threadIdx.x >> log;
+  }
+};
+
+// Sums of d xh and d over the positions of a part: [N, parts, 2, C].
 template <typename T, int V> __global__ void __launch_bounds__(kPartThreads) norm_part_sums(NormArgs a) {
   const int cg = a.c / a.g;
   const int64_t n = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x % a.parts);
   const int64_t first = part * a.span, last = min(a.p, first + a.span);
-  __shared__ float red[kPartThreads];
-  // 32 pieces of channels by 8 rows of positions
-  const int col = (blockIdx.y * 32 + (threadIdx.x & 31)) * V, row = threadIdx.x >> 5;
+  __shared__ float all[2 * V * kPartThreads];
+  const Cells at(a.c / V);
+  const int col0 = blockIdx.y * 32 * V, col = col0 + at.piece * V;
   const bool on = col < a.c;
   Nums<V> sw = Nums<V>::all(0.0f), sb = sw;
   Weights<V> wb;
@@ -615,30 +635,14 @@ template <typename T, int V> __global__ void __launch_bounds__(kPartThreads) nor
     const T* x = static_cast<const T*>(a.x) + n * a.xs_n + col;
     const T* dy = static_cast<const T*>(a.dy) + n * a.ds_n + col;
 #pragma unroll 2
-    for (int64_t p = first + row; p < last; p += 8) {
+    for (int64_t p = first + at.row; p < last; p += at.rows) {
       Nums<V> xh;
       const Nums<V> e = gradient<V>(load<T, V>(x + p * a.xs_p), load<T, V>(dy + p * a.ds_p), st.x, st.y, wb.w, wb.b, a.act, xh);
       sw = fma(e, xh, sw);
       sb = sb + e;
     }
   }
-  float both[2][V];
-  sw.put(both[0]);
-  sb.put(both[1]);
-  float* out = a.part + blockIdx.x * static_cast<int64_t>(2 * a.c);
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-#pragma unroll
-    for (int turn = 0; turn < 2; ++turn) {
-      __syncthreads();
-      red[threadIdx.x] = both[turn][j];
-      __syncthreads();
-      if (row == 0 && on) {
-        float s = 0.0f;
-        for (int r = 0; r < 8; ++r) s += red[r * 32 + threadIdx.x];
-        out[turn * a.c + col + j] = s;
-      }
-    }
+  sum_rows<V>(sw, sb, all, at.rows, at.cols, a.c - col0, a.c, a.part + blockIdx.x * static_cast<int64_t>(2 * a.c) + col0);
 }
 
 // From those, of every (sample, group): mean(a), mean(a xh): [N, G, 2] behind the parts' sums.
@@ -674,7 +678,8 @@ template <typename T, int V> __global__ void __launch_bounds__(kPartThreads) nor
   const int64_t n = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x % a.parts);
   const int64_t first = part * a.span, last = min(a.p, first + a.span);
-  const int col = (blockIdx.y * 32 + (threadIdx.x & 31)) * V, row = threadIdx.x >> 5;
+  const Cells cell(a.c / V);
+  const int col = (blockIdx.y * 32 + cell.piece) * V;
   if (col >= a.c) return;
   const int64_t at = (n * a.g + col / cg) * 2;
   const float2 st = *reinterpret_cast<const float2*>(a.stats + at);
@@ -685,7 +690,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kPartThreads) nor
   const T* dy = static_cast<const T*>(a.dy) + n * a.ds_n + col;
   T* y = static_cast<T*>(a.y) + n * a.ys_n + col;
 #pragma unroll 2
-  for (int64_t p = first + row; p < last; p += 8) {
+  for (int64_t p = first + cell.row; p < last; p += cell.rows) {
     Nums<V> xh;
     const Nums<V> e = gradient<V>(load<T, V>(x + p * a.xs_p), load<T, V>(dy + p * a.ds_p), st.x, st.y, wb.w, wb.b, a.act, xh);
     store<T, V>(y + p * a.ys_p, (e * wb.w + fma(xh, Nums<V>::all(-m2), Nums<V>::all(-m1))) * Nums<V>::all(st.y));

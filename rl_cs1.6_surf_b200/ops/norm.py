@@ -87,19 +87,23 @@ def _plan(n: int, p: int, c: int, g: int, e: int, v: int, grad: bool):
     cg = c // g
     per_group = cg // v
     items = p * per_group
-    if items <= 128:
+    # a warp's registers: up to 4 pieces a lane, or 2 where positions are shorter than a 32-byte sector. Lanes and
+    # block, forward and gradient in us: 8192x64x64 g8 61 + 120 and 84 + 139, 8192x8192 g8 103 + 158 and
+    # 186 + 256; 2048x128x64 g8 31 + 105 and 28 + 40
+    if items <= 64 or (items <= 128 and cg * e >= 32):
         lanes = min(32, _pow2(items))
         hold = _pow2(-(-items // lanes))
         blocks = min(-(-n // 8), max(1, 148 * 4 // -(-g // (32 // lanes))), 65535)
         return LANES, lanes, hold, 256, blocks, 1, 1, p
     # the narrowest slab of whole groups with rows of 32 bytes (a sector) that a block's registers
-    # take, twice as wide where that still leaves three for every SM
+    # take, twice as wide where that still leaves three for every SM (2048x512x64 g8 97 -> 79 us forward).
+    # Block and parts, where both can be: 1x512x64 4.3 + 8.5 and 6.6 + 10.3, 24x512x64 4.6 + 9.1 and 12.3 + 21.3
     threads, most = 256, 4 if grad else 8
     fits = [k for k in range(1, g + 1) if g % k == 0 and k * per_group <= threads and
             -(-p // (threads // (k * per_group))) <= most]
     slab = next((k for k in fits if k * cg * e >= 32), fits[-1] if fits else 0)
     slab = next((k for k in fits if k >= 2 * slab and n * (g // k) >= 148 * 3), slab)
-    if slab and n * (g // slab) >= (74 if grad else 1):
+    if slab:
         per = slab * per_group
         hold = -(-p // (threads // per))
         # no more threads than the pieces take
