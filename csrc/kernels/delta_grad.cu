@@ -9,7 +9,8 @@
 //   dk_i = -head_i S^T Z_i + tail_i beta_i dS^T W_i + sum_j scale dP_ji D_ji q_j + (dM_ij D_ij + dM_ji D_ji) k_j
 // and of a token's log decay, with E = dP P + dM M, e_i = head_i's terms, f_j = tail_j's:
 //   dg_m = sum_{j < m <= i} E_ij + sum_{i >= m} e_i + sum_{j < m} f_j + end <dS, S>.
-// These are sums of what each pair's decay contributes; none is a difference of larger ones.
+// These are sums of what each pair's decay contributes; none is a difference of larger ones (but for
+// a term of bfloat16 tokens, kByValues).
 //
 // A block for up to 64 values of a sequence's value head: two warps make the chunks ready in turn, as
 // in the forward pass, four carry them out, one makes the matrices and gates of 16 x 16. By values
@@ -17,6 +18,10 @@
 // quarter of the columns): dq and dk, which sum over the values; the chain's results pass
 // through shared memory as planes. S and W are the forward pass's. Blocks of one head, and heads
 // that share keys, leave parts of dq and dk that a second kernel sums in order.
+//
+// Neither memory nor the tensor pipe bounds it (256x128x8x64x64: 496 us, 0.17 of the copy rate, tensor pipe
+// 19%): each warp's instructions wait for the ones before, and many warps with code of their own
+// for the instruction cache. See Plan.
 #include "delta.cuh"
 
 namespace {
@@ -26,7 +31,10 @@ using namespace delta;
 constexpr int kPrep = 2, kMain = 4, kValues = 64;      // warps that make chunks ready, of the chain and of the keys; values of a block
 
 // How a block is made up. Either teams of one head each, whose four main warps follow the chain and then the
-// keys; or (kApart) one head whose chain is four warps' and whose keys are four others', a chunk behind.
+// keys; or (kApart) one head whose chain is four warps' and whose keys are four others', a chunk behind. The
+// first where there are more heads of sequences than SMs: main warps of two teams meet before each tile and run the
+// same instructions at the same time, 256x128x8x64x64 500 us (apart 686), 16x2048x16x64x64 986 (1573); apart
+// where there are fewer, 2x4096x16x64x64 834 us (one head a block, nothing apart: 1326).
 template <int kTeams_, bool kApart_> struct Plan {
   static constexpr int kTeams = kTeams_;
   static constexpr bool kApart = kApart_;
@@ -975,7 +983,7 @@ template <typename T, int DK> int backward(const DeltaArgs& a, cudaStream_t s) {
   using One = Plan<1, false>;
   using Two = std::conditional_t<B::template kFits<Plan<2, false>>, Plan<2, false>, One>;
   using Apart = std::conditional_t<B::template kFits<Plan<1, true>>, Plan<1, true>, One>;
-  if (const int e = items > 148 ? go(Two()) : go(Apart())) return e;
+  if (const int e = items > 148 ? go(Two()) : go(Apart())) return e;            // see Plan
   delta_rates<<<a.heads, 32, 0, s>>>(a, splits);
   if (a.part_q && a.length > 0) {
     const int64_t grid = (static_cast<int64_t>(a.batch) * a.length * a.groups * a.keys + 255) / 256;
