@@ -9,8 +9,7 @@
 //   dk_i = -head_i S^T Z_i + tail_i beta_i dS^T W_i + sum_j scale dP_ji D_ji q_j + (dM_ij D_ij + dM_ji D_ji) k_j
 // and of a token's log decay, with E = dP P + dM M, e_i = head_i's terms, f_j = tail_j's:
 //   dg_m = sum_{j < m <= i} E_ij + sum_{i >= m} e_i + sum_{j < m} f_j + end <dS, S>.
-// These are sums of what each pair's decay contributes; none is a difference of larger ones (but for
-// a term of bfloat16 tokens, kByValues).
+// These are sums of what each pair's decay contributes; none is a difference of larger ones.
 //
 // A block for up to 64 values of a sequence's value head: two warps make the chunks ready in turn, as
 // in the forward pass, four carry them out, one makes the matrices and gates of 16 x 16. By values
@@ -19,7 +18,7 @@
 // through shared memory as planes. S and W are the forward pass's. Blocks of one head, and heads
 // that share keys, leave parts of dq and dk that a second kernel sums in order.
 //
-// Neither memory nor the tensor pipe bounds it (256x128x8x64x64: 496 us, 0.17 of the copy rate, tensor pipe
+// Neither memory nor the tensor pipe bounds it (256x128x8x64x64: 518 us, 0.16 of the copy rate, tensor pipe
 // 19%): each warp's instructions wait for the ones before, and many warps with code of their own
 // for the instruction cache. See Plan.
 #include "delta.cuh"
@@ -33,8 +32,8 @@ constexpr int kPrep = 2, kMain = 4, kValues = 64;      // warps that make chunks
 // How a block is made up. Either teams of one head each, whose four main warps follow the chain and then the
 // keys; or (kApart) one head whose chain is four warps' and whose keys are four others', a chunk behind. The
 // first where there are more heads of sequences than SMs: main warps of two teams meet before each tile and run the
-// same instructions at the same time, 256x128x8x64x64 500 us (apart 686), 16x2048x16x64x64 986 (1573); apart
-// where there are fewer, 2x4096x16x64x64 834 us (one head a block, nothing apart: 1326).
+// same instructions at the same time, 256x128x8x64x64 518 us (apart about 700), 16x2048x16x64x64 986 (1573); apart
+// where there are fewer, 2x4096x16x64x64 861 us (one head a block, nothing apart: 1326).
 template <int kTeams_, bool kApart_> struct Plan {
   static constexpr int kTeams = kTeams_;
   static constexpr bool kApart = kApart_;
@@ -55,11 +54,7 @@ template <typename T, int DK> struct Backward {
   static constexpr int NT = Planes<T>::kToken, NI = Planes<T>::kInner, NS = Planes<T>::kShort;
   using Keys = Tile<T, DK>;
   using Values = Tile<T, kValues>;
-  // The head's term of k, -Z.(head K S^T): Z.R - Z.V with bfloat16 tokens, whose S^T Z has only two planes'
-  // digits; with 32-bit ones it comes from the keys, without the difference (ddt 1.3e-6 -> 3e-7 off
-  // where S is small).
-  static constexpr bool kByValues = sizeof(T) == 2;
-  static constexpr int kPitchS = DK + 4, kPitchD = DK + 8, kPitchV = kValues + 16 / static_cast<int>(sizeof(T));
+  static constexpr int kPitchS = DK + 4, kPitchD = DK + 8;
   static constexpr int kColumns = DK / kMain < 16 ? 16 : DK / kMain;     // of a warp by keys
   struct Stage {
     Chunk<T, NI> c;
@@ -67,14 +62,13 @@ template <typename T, int DK> struct Backward {
     int t0, n, more;                                   // more: the tile's next episode follows in this stage
     unsigned marks;
     alignas(16) bf16 tk[Keys::kSize], tq[Keys::kSize], tdo[Values::kSize];
-    alignas(16) T tv[kByValues ? kTile * kPitchV : 8];
   };
   struct Chain {                                       // what the chain leaves of a chunk
     alignas(16) bf16 w[NI][kValues][kTile], z[NI][kValues][kTile];     // rows values, columns tokens; see swap8
     alignas(16) bf16 d[NS][kValues][kPitchD];          // dS
     // of each warp: Z W^T and dO W^T, or its outputs
     alignas(16) union { float product[2][kTile][kMat]; T out[kTile][16 + 16 / sizeof(T)]; } part[kMain];
-    float by_value[kMain][3][kTile], inner[kMain];     // sums over its values: W.dU, the tails' terms, Z.V; <dS, S>
+    float by_value[kMain][2][kTile], inner[kMain];     // sums over its values: W.dU, the tails' terms; <dS, S>
   };
   template <typename P> struct Shared {
     Stage stage[P::kStages];
@@ -186,7 +180,6 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
     const int w = warp, pitch = a.keys + kTile;
     const T* q = static_cast<const T*>(a.q) + bi * a.q_b + gr * a.q_g;
     const T* k = static_cast<const T*>(a.k) + bi * a.k_b + gr * a.k_g;
-    const T* v = static_cast<const T*>(a.v) + bi * a.v_b + h * a.v_h + vb;
     const T* dout = static_cast<const T*>(a.dout) + bi * a.do_b + h * a.do_h + vb;
     Marks look{a.reset ? a.reset + static_cast<int64_t>(bi) * a.length : nullptr, length, 0u};
     // resets and gates a tile of this warp's ahead of the rest
@@ -214,7 +207,6 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
         Keys::load(st.tk, k + t0 * a.k_t, a.k_t, n, a.keys, a.piece_k == 16);
         Keys::load(st.tq, q + t0 * a.q_t, a.q_t, n, a.keys, a.piece_k == 16);
         Values::load(st.tdo, dout + t0 * a.do_t, a.do_t, n, mine, a.piece_v == 16);
-        if constexpr (B::kByValues) load_rows(st.tv, B::kPitchV, kTile, kValues, v + t0 * a.v_t, a.v_t, n, mine, a.piece_v == 16);
         cp_async_commit();
         Gate e{};
         if (lane < n) e = gate_of(x, y, bias, rate);
@@ -278,10 +270,10 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
         raw_dt = dt[(t0 + lane) * a.dt_t];
         raw_b = gb[(t0 + lane) * a.b_t];
       }
-      // lane: row r, columns j0 .. j0 + 7 of Z W^T and dO W^T. By rows: sums of E's part of P, of M, and Z.R
+      // lane: row r, columns j0 .. j0 + 7 of Z W^T and dO W^T. By rows: sums of E's part of P, of M
       const int r = lane >> 1, j0 = (lane & 1) * 8;
       const float rqr = st.c.rq[r], rkr = st.c.rk[r];
-      float row_p = 0.0f, row_m = 0.0f, zr = 0.0f;
+      float row_p = 0.0f, row_m = 0.0f;
 #pragma unroll
       for (int j = j0; j < j0 + 8; j += 4) {
         auto four = [](float (&x)[4], const float* from) { *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from); };
@@ -313,7 +305,6 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
           mz[e] = one && c < r ? m[e] * zw[e] : 0.0f;
           row_p += ep[e];
           row_m += em[e];
-          zr += c == r ? zw[e] : mz[e] * bt[e];
         }
         *reinterpret_cast<float4*>(&st.wide.p[r][j]) = make_float4(ep[0], ep[1], ep[2], ep[3]);
         *reinterpret_cast<float4*>(&st.wide.m[r][j]) = make_float4(em[0], em[1], em[2], em[3]);
@@ -339,16 +330,14 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       }
       row_p += __shfl_xor_sync(0xffffffffu, row_p, 1);
       row_m += __shfl_xor_sync(0xffffffffu, row_m, 1);
-      zr += __shfl_xor_sync(0xffffffffu, zr, 1);
       __syncwarp();
       // lane: column and token c; columns from below
       const int c = lane & 15;
-      float wd = 0.0f, zv = 0.0f, f = 0.0f, inner = 0.0f;
+      float wd = 0.0f, f = 0.0f, inner = 0.0f;
 #pragma unroll
       for (int x = 0; x < kMain; ++x) {
         wd += chain.by_value[x][0][c];
         f += chain.by_value[x][1][c];
-        if constexpr (B::kByValues) zv += chain.by_value[x][2][c];
         inner += chain.inner[x];
       }
       float column = 0.0f, below = 0.0f, dbeta = wd;
@@ -363,15 +352,13 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       }
       row_p = __shfl_sync(0xffffffffu, row_p, 2 * c);
       row_m = __shfl_sync(0xffffffffu, row_m, 2 * c);
-      zr = __shfl_sync(0xffffffffu, zr, 2 * c);
-      const float keep = !B::kByValues || marks & ((2u << c) - 1u) ? 0.0f : zr - zv;
       if (lane < kTile) {
         sh.nq[c] = row_p;
-        sh.nk[c] = keep + f + row_m + column;
+        sh.nk[c] = f + row_m + column;
       }
       bar_sync(bars + P::kMatrices, P::kAtMatrices);
       if constexpr (P::kApart) bar_arrive(bars + P::kPlace + copy, P::kAtChain);
-      float e = keep;
+      float e = 0.0f;
 #pragma unroll
       for (int x = 0; x < kMain; ++x) e += sh.by_key[0][x][c] + sh.by_key[1][x][c];
       float dg = marks ? 0.0f : st.c.head[kTile - 1] * inner;
@@ -452,7 +439,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
   // what a warp without values or columns leaves
   if (follows)
     for (int copy = 0; copy < P::kCopies; ++copy) {
-      for (int i = lane; i < 3 * kTile; i += 32) (&sh.chain[copy].by_value[warp][0][0])[i] = 0.0f;
+      for (int i = lane; i < 2 * kTile; i += 32) (&sh.chain[copy].by_value[warp][0][0])[i] = 0.0f;
       if (lane == 0) sh.chain[copy].inner[warp] = 0.0f;
     }
   if (P::kApart && !by_v) {
@@ -588,7 +575,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       // sums over the warp's values, by tokens: halves of the sums change lanes until each has one token's
       {
         T (&so)[kTile][16 + 16 / sizeof(T)] = *(P::kApart ? &sh.dv[P::kApart ? copy * kMain + warp : 0] : &chain.part[warp].out);
-        float sum[3][2][2];
+        float sum[2][2][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -596,15 +583,13 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
             const int tok = t * 8 + col + e;
             sum[0][t][e] = fmaf(w[t][e], du[t][e], w[t][e + 2] * du[t][e + 2]);
             sum[1][t][e] = fmaf(w[t][e], ds[t][e], w[t][e + 2] * ds[t][e + 2]);
-            if constexpr (B::kByValues)
-              sum[2][t][e] = fmaf(z[t][e], to_f(st.tv[tok * B::kPitchV + vl + row]), z[t][e + 2] * to_f(st.tv[tok * B::kPitchV + vl + row + 8]));
             so[tok][row] = from_f<T>(z[t][e]);
             so[tok][row + 8] = from_f<T>(z[t][e + 2]);
           }
         const bool t1 = lane & 16, e1 = lane & 8;
         const int tok = (t1 ? 8 : 0) + col + (e1 ? 1 : 0);
 #pragma unroll
-        for (int x = 0; x < (B::kByValues ? 3 : 2); ++x) {
+        for (int x = 0; x < 2; ++x) {
           float y[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) y[e] = (t1 ? sum[x][1][e] : sum[x][0][e]) + __shfl_xor_sync(0xffffffffu, t1 ? sum[x][0][e] : sum[x][1][e], 16);
@@ -699,15 +684,15 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
     if (P::kApart && by_v) put_rows(dv + t0 * v_t + vl, v_t, sh.dv[P::kApart ? copy * kMain + warp : 0], n, mine - vl, pieces_v);
     if (by_k) {
       float as[kPairs][2][4] = {};
-      // apart, all of a block's values unrolled, those that it does not have as zeros (864 -> 834 us at
+      // apart, all of a block's values unrolled, those that it does not have as zeros (4% at
       // 2x4096x16x64x64); teams of two are bound by fetching instructions
 #pragma unroll (P::kApart ? kMain : 1)
       for (int x = 0; x < (P::kApart ? kMain : vsteps); ++x) {
-        uint32_t o[NT][4], z[NS][4], w[NS][4];
+        uint32_t o[NT][4], z[NI][4], w[NS][4];
         load_planes<NS, true>(w, smem_of(chain.w) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
         if (!fresh) {
           load_planes<NT, false>(o, smem_of(st.tdo) + a_rows(lane, Values::kPitch) + x * 32, Values::kPlane * 2);
-          load_planes<NS, true>(z, smem_of(chain.z) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
+          load_planes<NI, true>(z, smem_of(chain.z) + tokens_a(lane) + x * 16 * kTile * 2, kValues * kTile * 2);
         }
 #pragma unroll
         for (int p = 0; p < kPairs; ++p) {
@@ -726,7 +711,7 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
               for (int m = 0; m < NI; ++m) s[m][e] = y[m];
             }
             mma_planes<NT, NI>(aq[p][0], aq[p][1], o, s);
-            mma_planes<NS, NS>(ak[p][0], ak[p][1], z, s);
+            mma_planes<NI, NI>(ak[p][0], ak[p][1], z, s);    // all planes: the decays' gradients are made of it
           }
         }
       }
@@ -757,11 +742,9 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
           for (int e = 0; e < 2; ++e) {
             float q0, q1;
             tile_pair<T>(st.tq, Keys::kPlane, (row + 8 * e) * Keys::kPitch + c0 + 16 * p + t * 8 + col, q0, q1);
-            if constexpr (!B::kByValues) {
-              float k0, k1;
-              tile_pair<T>(st.tk, Keys::kPlane, (row + 8 * e) * Keys::kPitch + c0 + 16 * p + t * 8 + col, k0, k1);
-              e1[e] = fmaf(ak[p][t][2 * e], k0, fmaf(ak[p][t][2 * e + 1], k1, e1[e]));
-            }
+            float k0, k1;
+            tile_pair<T>(st.tk, Keys::kPlane, (row + 8 * e) * Keys::kPitch + c0 + 16 * p + t * 8 + col, k0, k1);
+            e1[e] = fmaf(ak[p][t][2 * e], k0, fmaf(ak[p][t][2 * e + 1], k1, e1[e]));
 #pragma unroll
             for (int x = 2 * e; x < 2 * e + 2; ++x) {
               aq[p][t][x] *= hq[e];
@@ -773,10 +756,8 @@ template <typename T, int DK, typename P> __global__ void __launch_bounds__(P::k
       for (int e = 0; e < 2; ++e) {
         e0[e] = quad_sum(e0[e]);
         if ((lane & 3) == 0) sh.by_key[0][warp][row + 8 * e] = e0[e] * c.rq[row + 8 * e];
-        if constexpr (!B::kByValues) {
-          e1[e] = quad_sum(e1[e]);
-          if ((lane & 3) == 0) sh.by_key[1][warp][row + 8 * e] = e1[e] * hk[e] * c.rk[row + 8 * e];
-        }
+        e1[e] = quad_sum(e1[e]);
+        if ((lane & 3) == 0) sh.by_key[1][warp][row + 8 * e] = e1[e] * hk[e] * c.rk[row + 8 * e];
       }
     }
     bar_sync(bars + P::kMatrices, P::kAtMatrices);     // S is read no more

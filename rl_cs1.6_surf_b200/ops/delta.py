@@ -161,7 +161,7 @@ def gated_delta_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
                       base + 4 * n if n else 0, base + 8 * n if m else 0, base + 8 * n + 4 * m, dA.data_ptr(), _p(dbias),
                       *_strides(q, k, v), *dt.stride()[:2], *b.stride()[:2], 0, 0, 0, *_strides(dout),
                       _scale(what, scale, nk), bsz, t, g, h, nk, nv, normalize,
-                      _piece(_bits(e, q, k) | nk * e), _piece(_bits(e, v, dout) | nv * e))
+                      _piece(_bits(e, q, k) | nk * e), _piece(_bits(e, dout) | nv * e))
     launch(_lib.lib(DLIB).surf_delta_grad, "surf_delta_grad", at, args, code)
     del ws                                     # the stream's next user comes after the launch
     _lib.add_launches(2 if n else 1)
