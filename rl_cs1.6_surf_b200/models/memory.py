@@ -398,6 +398,8 @@ def train_recall(iterations: int = 400, envs: int = 128, length: int = 64, cfg: 
     from ..ops.tokens import sample_tokens, sample_tokens_reference
     if objective not in ("answers", "policy"):
         raise ValueError(f"objective must be answers or policy, not {objective!r}")
+    if epochs < 1:
+        raise ValueError(f"epochs must be positive, not {epochs}")
     dev = torch.device(device)
     net = MemoryNet(cfg or MemoryConfig(), dev, seed)
     c = net.cfg

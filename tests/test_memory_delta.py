@@ -112,3 +112,8 @@ def test_policy_gradient_matches_the_reference():
         g = params[name].grad
         # as of the sequence's gradients; ratios near 1 amplify nothing
         assert float((net.g(name).cpu() - g).norm() / g.norm()) < 0.05, name
+
+
+def test_no_epochs_are_refused():
+    with pytest.raises(ValueError, match="epochs"):
+        M.train_recall(1, device="cpu", objective="policy", epochs=0)
