@@ -272,10 +272,10 @@ struct Wide { float m[kTile][kMat], p[kTile][kMat], d[kTile][kMat]; };   // M, P
 // The chunk's decays, by one warp, from each lane's gates (lane < 16: token lane's log decay and beta,
 // zero behind the chunk) and the chunk's resets. Running sums are kept as two floats, of which
 // differences lose nothing: the larger halves' is exact where they are close. Decays below e^-104 are
-// 0 in 32 bits; -10^4 stands for all of them.
+// 0 in 32 bits; -10^4 stands for all of them, and NaN stays.
 template <typename T, int NP> __device__ __forceinline__ void decays(Chunk<T, NP>& c, float g, float beta, unsigned marks) {
   const int lane = threadIdx.x & 31;
-  double sum = fmaxf(g, -1e4f);
+  double sum = g < -1e4f ? -1e4f : g;
 #pragma unroll
   for (int o = 1; o < kTile; o <<= 1) {
     const double x = __shfl_up_sync(0xffffffffu, sum, o, kTile);
