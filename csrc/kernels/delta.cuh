@@ -429,8 +429,8 @@ __device__ __forceinline__ Gate gate_of(float dt, float b, float bias, float rat
   r.beta = sigmoid(b);
   return r;
 }
-// A[h]; -inf as the lowest finite number, so that a step of zero decays by e^0
-__device__ __forceinline__ float rate_at(const float* A, int h) { return fmaxf(A[h], -3.4028235e38f); }
+// A[h]; -inf as the lowest finite number, so that a step of zero decays by e^0. NaN stays.
+__device__ __forceinline__ float rate_at(const float* A, int h) { return A[h] < -3.4028235e38f ? -3.4028235e38f : A[h]; }
 
 // The resets of the tile at t (bit i: token t + i), as each lane's own flag, on its way until it is
 // asked for by all lanes of the warp.

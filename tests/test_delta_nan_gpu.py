@@ -88,3 +88,14 @@ def check_head(c, clean, grads):
     state = c["state"].clone()
     out = DR.gated_delta_step(*tokens, c["A"], state, dt_bias=c["dt_bias"])
     assert out[:, 1].isnan().all() and state[:, 1].isnan().all() and torch.isfinite(out[:, 0]).all() and torch.isfinite(state[:, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("rows", [4, 151])
+def test_a_rate_that_is_nan_shows_in_its_head(rows, ragged, dtype):
+    c = make(rows, 40, 2, 2, 32, 48, dtype, reset=0.1, ragged=ragged)
+    clean, grads = call(c)
+    c["A"] = c["A"].clone()
+    c["A"][1] = float("nan")
+    check_head(c, clean, grads)
