@@ -100,10 +100,11 @@ __device__ __forceinline__ Slopes finish(const LossArgs& p, const Row& row, cons
     lp = static_cast<float>(l);
     ent = static_cast<float>(log_s - power * kLn2d);
     const float ratio = expf(static_cast<float>(l - p.old_logp[row.n]));
-    const float held = fminf(fmaxf(ratio, 1.0f - p.lo), 1.0f + p.hi);
-    const float free = adv == 0.0f ? 0.0f : ratio * adv, cut = held * adv;
-    float c = free <= cut ? -free : 0.0f;
-    each = -fminf(free, cut);
+    // by comparisons that NaN fails, so that it stays; no advantage makes nothing of an infinite ratio
+    const float held = ratio < 1.0f - p.lo ? 1.0f - p.lo : ratio > 1.0f + p.hi ? 1.0f + p.hi : ratio;
+    const float free = adv == 0.0f && ratio >= 0.0f ? 0.0f : ratio * adv, cut = held * adv;
+    float c = cut < free ? 0.0f : -free;
+    each = cut < free ? -cut : -free;
     if (p.ref) {
       const double d = p.ref[row.n] - l;
       const double e = expm1(d);
