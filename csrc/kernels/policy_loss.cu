@@ -109,8 +109,10 @@ __device__ __forceinline__ Slopes finish(const LossArgs& p, const Row& row, cons
       const double d = p.ref[row.n] - l;
       const double e = expm1(d);
       kl = static_cast<float>(e - d);
-      each = fmaf(p.kl, kl, each);
-      c = fmaf(p.kl, -static_cast<float>(e), c);
+      if (p.kl != 0.0f) {                              // e^d of a row may be infinite in 32 bits: 0 times it is not 0
+        each = fmaf(p.kl, kl, each);
+        c = fmaf(p.kl, -static_cast<float>(e), c);
+      }
     }
     each = w * fmaf(-p.ent, ent, each);
     c *= w;

@@ -323,10 +323,10 @@ def policy_loss(logits: torch.Tensor, answers: torch.Tensor, old_logp: torch.Ten
 
         loss = sum_n weights[n] (-min(r A, clip(r, 1 - clip, 1 + clip_high) A) + kl_coef (e^d - d - 1) - ent_coef H)
 
-    ``weights`` None: 1 / R each; ``clip_high`` None: ``clip``; ``ref_logp`` None: no KL term. Logits are
-    bfloat16 or float32, their rows any stride apart; NaN counts as -inf. A row whose answer is
-    negative or has a logit of -inf counts nothing and gets zeros. An answer past the row does too, and is
-    reported through ``ops.gemm.check_error_flag``. ``logp``, ``kl`` and ``entropy`` [R] are float32, ``dlogits`` has
+    ``weights`` None: 1 / R each; ``clip_high`` None: ``clip``; ``ref_logp`` None: no KL term, with a ``kl_coef`` of 0
+    it is reported but takes no part, infinite or not. Logits are bfloat16 or float32, their rows any
+    stride apart; NaN counts as -inf. A row whose answer is negative or has a logit of -inf counts nothing
+    and gets zeros. An answer past the row does too, and is reported through ``ops.gemm.check_error_flag``. ``logp``, ``kl`` and ``entropy`` [R] are float32, ``dlogits`` has
     the logits' type (None without ``grad``) and may be written to ``out``, the logits themselves among others. The
     temperature must be positive: an answer that was taken greedily has no probability to move.
     Where r A ties with its clipped value its gradient passes."""
@@ -398,7 +398,7 @@ def policy_loss_reference(logits, answers, old_logp, advantages, *, ref_logp=Non
     ratio = torch.exp(lp - old_logp)
     held = torch.clamp(ratio, 1 - clip, 1 + (clip if clip_high is None else clip_high))
     each = -torch.minimum(ratio * advantages, held * advantages) - ent_coef * ent
-    if ref_logp is not None:
+    if ref_logp is not None and kl_coef != 0:
         d = ref_logp - lp
         each = each + kl_coef * (torch.exp(d) - d - 1)
     w = weights if weights is not None else torch.full_like(each, 1.0 / max(1, rows))

@@ -51,3 +51,17 @@ def test_nan_of_rows_that_count_nothing_stays_out(v):
     assert torch.isfinite(r.loss) and not r.dlogits[2].any()
     for x, y in zip(r, want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("v", [9, 1001])
+def test_a_kl_term_that_is_only_reported(v):
+    """e^100 is infinite in 32 bits, and so is the KL term of a reference policy that gives an answer no probability."""
+    c = make(5, v, F32, masked=False)
+    plain = call(dict(c, ref_logp=None), ent_coef=0.01)
+    for far in (100.0, -float("inf"), float("nan")):
+        c["ref_logp"] = plain.logp + 0.3
+        want = call(c, ent_coef=0.01)
+        c["ref_logp"][1] = plain.logp[1] + far
+        r = call(c, ent_coef=0.01)
+        assert torch.equal(r.loss, plain.loss) and torch.equal(r.dlogits, plain.dlogits)
+        assert not torch.isfinite(r.kl[1]) and torch.equal(r.kl[2:], want.kl[2:])
