@@ -952,7 +952,8 @@ template <typename T> __global__ void __launch_bounds__(256) delta_parts(DeltaAr
 template <typename T, int DK> int backward(const DeltaArgs& a, cudaStream_t s) {
   using B = Backward<T, DK>;
   const int splits = (a.values + kValues - 1) / kValues;
-  if ((splits > 1 && !a.part_g) || (splits * a.heads != a.groups && !a.part_q)) return static_cast<int>(cudaErrorInvalidValue);
+  // parts of as many elements as there are tokens: rows of none need no memory for them
+  if (a.length > 0 && ((splits > 1 && !a.part_g) || (splits * a.heads != a.groups && !a.part_q))) return static_cast<int>(cudaErrorInvalidValue);
   const int64_t items = static_cast<int64_t>(a.batch) * a.heads * splits;
   auto go = [&](auto plan) {
     using P = decltype(plan);
