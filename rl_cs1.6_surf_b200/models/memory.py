@@ -85,9 +85,9 @@ class MemoryNet:
             raise ValueError("features, dim and rank must be multiples of 8, state of 4, answers at most out_pad")
         if c.core not in ("scan", "delta"):
             raise ValueError(f"core must be scan or delta, not {c.core!r}")
-        if c.core == "delta" and (c.heads % 4 or c.dim % c.heads or c.dim // c.heads > delta.MAX_HEAD or
+        if c.core == "delta" and (c.heads < 4 or c.heads % 4 or c.dim % c.heads or not 0 < c.dim // c.heads <= delta.MAX_HEAD or
                                   c.keys % 8 or not 0 < c.keys <= delta.MAX_HEAD):
-            raise ValueError(f"heads must be a multiple of 4 that divides dim, with at most {delta.MAX_HEAD} values and "
+            raise ValueError(f"heads must be a positive multiple of 4 that divides dim, with 1 to {delta.MAX_HEAD} values and "
                              f"8 to {delta.MAX_HEAD} keys, a multiple of 8")
         self.specs = [("in.w", (c.conv_dim, c.features)), ("gate.w", (2 * c.heads, c.features)), ("out.w", (c.out_pad, c.dim)),
                       ("conv.w", (c.conv_dim, c.width)), ("conv.b", (c.conv_dim,)), ("dt.b", (c.heads,)), ("a_log", (c.heads,)),
