@@ -53,6 +53,7 @@ _SIG = {
 _lib.register(NLIB, _SIG)
 
 _err_flags: dict = {}
+_clearing: dict = {}         # flags whose first clearing may still be on its way
 
 
 ERROR_CODES = {1: "GEMM producer wait timed out", 2: "GEMM MMA wait timed out", 3: "GEMM epilogue wait timed out",
@@ -68,8 +69,22 @@ def error_flag(device) -> torch.Tensor:
     if key.type == "cuda" and key.index is None:      # "cuda" and "cuda:<current>" share one flag
         key = torch.device("cuda", torch.cuda.current_device())
     if key not in _err_flags:
-        _err_flags[key] = torch.zeros(1, dtype=torch.int32, device=key)
+        _err_flags[key] = _new_flag(key)
+    elif key in _clearing and not torch.cuda.is_current_stream_capturing():
+        _clearing.pop(key).synchronize()
     return _err_flags[key]
+
+
+def _new_flag(device: torch.device) -> torch.Tensor:
+    if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+        return torch.zeros(1, dtype=torch.int32, device=device)
+    # Cleared on a stream of its own: the graph that is being captured would clear it, and what other calls have
+    # reported, at each replay. Nothing may be waited for during a capture: the next call outside of one does.
+    flag, side = torch.empty(1, dtype=torch.int32, device=device), torch.cuda.Stream(device)
+    with torch.cuda.stream(side):
+        flag.zero_()
+    _clearing[device] = side.record_event()
+    return flag
 
 
 def check_error_flag(device) -> None:
