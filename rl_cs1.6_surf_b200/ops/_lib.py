@@ -133,12 +133,19 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
 
 
 class _Extent:
-    """Where a tensor's elements lie, for numpy's overlap test; the memory is never touched."""
+    """Where elements lie, for numpy's overlap test; the memory is never touched."""
 
-    def __init__(self, t: torch.Tensor):
-        e = t.element_size()
-        self.__array_interface__ = {"version": 3, "typestr": f"|V{e}", "data": (t.data_ptr(), False),
-                                    "shape": tuple(t.shape), "strides": tuple(s * e for s in t.stride())}
+    def __init__(self, at: int, size: int, shape, strides):
+        self.__array_interface__ = {"version": 3, "typestr": f"|V{size}", "data": (at, False),
+                                    "shape": tuple(shape), "strides": tuple(s * size for s in strides)}
+
+
+def _extent(t: torch.Tensor) -> _Extent:
+    return _Extent(t.data_ptr(), t.element_size(), t.shape, t.stride())
+
+
+def _meet(a: _Extent, b: _Extent) -> bool:
+    return bool(np.shares_memory(np.asarray(a), np.asarray(b)))
 
 
 def _span(t: torch.Tensor) -> tuple:
@@ -154,7 +161,25 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     interleaved columns of one buffer do not count."""
     if not a.numel() or not b.numel():
         return False
-    return bool(np.shares_memory(np.asarray(_Extent(a)), np.asarray(_Extent(b))))
+    return _meet(_extent(a), _extent(b))
+
+
+def overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two of a tensor's elements share memory. Exact: by axes from the smallest stride on, whether the axes so
+    far meet themselves some steps along the next one, which takes a look only where they reach past its stride."""
+    if t.is_contiguous() or t.numel() < 2:
+        return False
+    at, e, reach = t.data_ptr(), t.element_size(), 0
+    axes = sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1)
+    for i, (s, n) in enumerate(axes):
+        if s == 0:
+            return True
+        for d in range(1, min(n - 1, reach // s) + 1):
+            shape, strides = [m for _, m in axes[:i]], [r for r, _ in axes[:i]]
+            if _meet(_Extent(at, e, shape, strides), _Extent(at + d * s * e, e, shape, strides)):
+                return True
+        reach += (n - 1) * s
+    return False
 
 
 def within_float32(x: float) -> bool:
@@ -166,8 +191,6 @@ def require_apart(what: str, name: str, out: torch.Tensor, inputs: dict, in_plac
     """Refuse an ``out`` whose elements share memory with one another or with an input: other
     threads read the inputs while it is written. It may be one of the inputs named in
     ``in_place`` itself, where a thread reads an element before it writes it."""
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-        raise ValueError(f"{what}: {name} has elements that share memory")
     lo, hi = _span(out)
     for key, t in inputs.items():
         if not isinstance(t, torch.Tensor):
@@ -179,3 +202,5 @@ def require_apart(what: str, name: str, out: torch.Tensor, inputs: dict, in_plac
             continue
         if overlap(out, t):
             raise ValueError(f"{what}: {name} shares memory with {key}")
+    if overlaps_itself(out):
+        raise ValueError(f"{what}: {name} has elements that share memory")
