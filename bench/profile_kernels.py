@@ -5,7 +5,8 @@
                                            conv2_iwgrad|conv2_idgrad|conv3_ifwd|conv3_iwgrad|conv3_idgrad|sample|gae|
                                            ppo_loss|reward|adam|p2p1|edt|geodesic|geodesic_race|surfnz|framestack|
                                            seq_conv|seq_scan|seq_scan_step|sample_tokens|
-                                           delta|delta_long|delta_step|group_norm|policy_loss [--reps 2]
+                                           delta|delta_prompt|delta_long|delta_step|
+                                           group_norm|group_norm_rows|group_norm_parts|policy_loss [--reps 2]
 
 Each case builds its inputs (a few GB on the device at most, larger than L2
 where the kernel streams memory), warms up once, then launches the kernel
@@ -13,7 +14,7 @@ where the kernel streams memory), warms up once, then launches the kernel
 ``ncu --set full --clock-control none -k regex:<kernel> -s 1 -c 1``.
 Shapes: the benchmark's 2048 envs x 128 x 64 rays, 2048-row sampling,
 128 x 2048 GAE, 32,768-row loss; a rollout's rows (256 x 128) for the sequence operators and the
-delta rule (long: 2 x 4096), forward and gradient in one case; the convolution cases use 4,096 images
+delta rule (long: 2 x 4096, a prompt of 8191 without its gradient), forward and gradient in one case; the convolution cases use 4,096 images
 (operands still larger than L2) to keep the captures small.
 """
 from __future__ import annotations
@@ -39,6 +40,15 @@ def _time(fn, reps):
     e1.record()
     torch.cuda.synchronize()
     return e0.elapsed_time(e1) / reps
+
+
+def _decays(heads, dev):
+    """Rates and biases of the delta rule's decays: e^(-16 * 0.1) to e^(-0.001) a token about a dt of 0."""
+    import math
+
+    import torch
+    step = torch.exp(torch.rand(heads, device=dev) * math.log(100.0) + math.log(0.001))
+    return -(1 + 15 * torch.rand(heads, device=dev)), torch.log(torch.expm1(step))
 
 
 def main():
@@ -319,29 +329,36 @@ def main():
         from surfb200.ops.tokens import sample_tokens
         logits, u = (2.5 * torch.randn(256, 131072, device=dev)).to(torch.bfloat16), torch.rand(256, 1, device=dev)
         info["ms"] = _time(lambda: sample_tokens(logits, u, top_p=0.95), args.reps)
-    elif k in ("delta", "delta_long"):
+    elif k in ("delta", "delta_prompt", "delta_long"):
         from surfb200.ops import delta
-        B, T, H = (256, 128, 8) if k == "delta" else (2, 4096, 16)
-        q, key, v, do = (torch.randn(B, T, H, 64, device=dev).to(torch.bfloat16) for _ in range(4))
+        B, T, H, N, resets = {"delta": (256, 128, 8, 64, 0.02), "delta_prompt": (1, 8191, 8, 128, 0.0),
+                              "delta_long": (2, 4096, 16, 64, 0.0005)}[k]
+        q, key, v, do = (torch.randn(B, T, H, N, device=dev).to(torch.bfloat16) for _ in range(4))
         dt, b = (torch.randn(B, T, H, device=dev).to(torch.bfloat16) for _ in range(2))
-        a = (q, key, v, dt, b, torch.rand(H, device=dev))
-        kw = dict(reset=torch.rand(B, T, device=dev) < 0.01)
-        saved = delta.gated_delta(*a, train=True, **kw).saved
-        info["ms"] = _time(lambda: delta.gated_delta(*a, train=True, **kw), args.reps)
-        info["grad_ms"] = _time(lambda: delta.gated_delta_grad(do, *a, saved=saved, **kw), args.reps)
+        A, bias = _decays(H, dev)
+        a, train = (q, key, v, dt, b, A), k != "delta_prompt"
+        kw = dict(dt_bias=bias, reset=torch.rand(B, T, device=dev) < resets if resets else None)
+        r = delta.gated_delta(*a, train=train, **kw)
+        assert torch.isfinite(r.final).all() and torch.isfinite(r.out).all()
+        info["ms"] = _time(lambda: delta.gated_delta(*a, train=train, **kw), args.reps)
+        if train:
+            info["grad_ms"] = _time(lambda: delta.gated_delta_grad(do, *a, saved=r.saved, **kw), args.reps)
     elif k == "delta_step":
         from surfb200.ops import delta
         q, key, v = (torch.randn(2048, 8, 64, device=dev).to(torch.bfloat16) for _ in range(3))
         dt, b = (torch.randn(2048, 8, device=dev).to(torch.bfloat16) for _ in range(2))
-        A, pool = torch.rand(8, device=dev), torch.randn(2048, 8, 64, 64, device=dev)
-        info["ms"] = _time(lambda: delta.gated_delta_step(q, key, v, dt, b, A, pool), args.reps)
-    elif k == "group_norm":
+        (A, bias), pool = _decays(8, dev), torch.randn(2048, 8, 64, 64, device=dev)
+        info["ms"] = _time(lambda: delta.gated_delta_step(q, key, v, dt, b, A, pool, dt_bias=bias), args.reps)
+        assert torch.isfinite(pool).all()
+    elif k in ("group_norm", "group_norm_rows", "group_norm_parts"):
         from surfb200.ops.norm import group_norm, group_norm_grad
-        x, dy = (torch.randn(2048, 512, 64, device=dev).to(torch.bfloat16) for _ in range(2))
-        w, b = torch.ones(64, device=dev), torch.zeros(64, device=dev)
-        stats = group_norm(x, 8, w, b, activation="silu", train=True).stats
-        info["ms"] = _time(lambda: group_norm(x, 8, w, b, activation="silu", train=True), args.reps)
-        info["grad_ms"] = _time(lambda: group_norm_grad(dy, x, 8, w, b, stats=stats, activation="silu"), args.reps)
+        shape, g, dtype = {"group_norm": ((2048, 512, 64), 8, torch.bfloat16), "group_norm_rows": ((32768, 512), 8, torch.bfloat16),
+                           "group_norm_parts": ((1, 12321, 120), 6, torch.float32)}[k]
+        x, dy = (torch.randn(*shape, device=dev).to(dtype) for _ in range(2))
+        w, b = torch.ones(shape[-1], device=dev), torch.zeros(shape[-1], device=dev)
+        stats = group_norm(x, g, w, b, activation="silu", train=True).stats
+        info["ms"] = _time(lambda: group_norm(x, g, w, b, activation="silu", train=True), args.reps)
+        info["grad_ms"] = _time(lambda: group_norm_grad(dy, x, g, w, b, stats=stats, activation="silu"), args.reps)
     elif k == "policy_loss":
         logits = (2.5 * torch.randn(4096, 32003, device=dev)).to(torch.bfloat16)
         ans, old = torch.randint(0, 32003, (4096,), device=dev), torch.full((4096,), -11.0, device=dev)
