@@ -41,7 +41,7 @@ template <typename T, int DK> struct Forward {
 // numbered barriers: stage s is ready (1 + s), stage s is free (1 + kStages + s). With few blocks the chain
 // from state to state bounds it (64 keys: 1.8 thousand cycles a chunk of one warp's products, each
 // waiting for the one before, against 0.1 of memory), with many the same warps' waits and instructions
-// (256x128x8x64x64: 0.38 a cycle and scheduler, tensor pipe 26%, 0.42 of the copy rate).
+// (256x128x8x64x64: 0.38 a cycle and scheduler, tensor pipe 26%, 0.41 of the copy rate).
 // kKeep: for the gradient. Calls that keep nothing are kernels of their own (1x8191x8x128x128 1054 -> 745 us,
 // 2x4096x16x64x64 313 -> 248 us).
 template <typename T, int DK, int kBlocks, bool kKeep>

@@ -19,7 +19,7 @@
 // that share keys, leave parts of dq and dk that a second kernel sums in order.
 //
 // Neither memory nor the tensor pipe bounds it (256x128x8x64x64: 518 us, 0.16 of the copy rate, tensor pipe
-// 19%): each warp's instructions wait for the ones before, and many warps with code of their own
+// 20%): each warp's instructions wait for the ones before, and many warps with code of their own
 // for the instruction cache. See Plan.
 #include "delta.cuh"
 
