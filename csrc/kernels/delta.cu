@@ -198,8 +198,8 @@ __global__ void __launch_bounds__((kPrep + kMain) * 32, kBlocks) delta_forward(D
     const Chunk<T, NS>& c = st.c;
     // The state before the tile and W, for the gradient: rows of both side by side, as one bulk copy from
     // shared memory where that is allowed (stored lane by lane they held the chain up: 2x4096x16x64x64
-    // 449 us). A warp behind the last value (its block's values are no multiple of 64) has none: a copy's size
-    // would be 0 or below.
+    // 449 us). A warp behind the last value (a head's values need not divide among its blocks' warps) has none: its
+    // copy's size would be 0 or below.
     float* saved = kKeep && v0 < a.values
                        ? a.saved + ((static_cast<int64_t>(bi) * tiles + t0 / kTile) * a.heads + h) * a.values * pitch_s : nullptr;
     const bool copied = saved && bulk && t0 % kTile == 0 && !more;

@@ -17,7 +17,7 @@ divided by their lengths, sqrt(|k|^2 + 1e-6); ``scale`` None: 1 / sqrt(K).
 state before its token (infinities and NaN end with their episode too), tokens past a row's
 length give zeros, change nothing and are never read; nothing here records a graph for autograd.
 NaN in a token, gate or weight is NaN in all that is made of it, and may reach up to 15 tokens
-before it in its episode (rows are taken 16 tokens at a time, what does not count as 0 times it).
+before it in its episode too: rows are taken 16 tokens at a time, later ones with a factor of 0.
 """
 from __future__ import annotations
 

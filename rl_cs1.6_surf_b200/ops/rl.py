@@ -326,9 +326,11 @@ def policy_loss(logits: torch.Tensor, answers: torch.Tensor, old_logp: torch.Ten
     ``weights`` None: 1 / R each; ``clip_high`` None: ``clip``; ``ref_logp`` None: no KL term, with a ``kl_coef`` of 0
     it is reported but takes no part, infinite or not. Logits are bfloat16 or float32, their rows any
     stride apart; NaN counts as -inf. A row whose answer is negative or has a logit of -inf counts nothing
-    and gets zeros. An answer past the row does too, and is reported through ``ops.gemm.check_error_flag``. ``logp``, ``kl`` and ``entropy`` [R] are float32, ``dlogits`` has
-    the logits' type (None without ``grad``) and may be written to ``out``, the logits themselves among others. The
-    temperature must be positive: an answer that was taken greedily has no probability to move.
+    and gets zeros. An answer past the row does too, and is reported through
+    ``ops.gemm.check_error_flag``. NaN elsewhere in a row that counts is NaN in the loss and the row's gradient.
+    ``logp``, ``kl`` and ``entropy`` [R] are float32, ``dlogits`` has the logits' type (None without ``grad``)
+    and may be written to ``out``, the logits themselves among others. The temperature must be positive: an
+    answer that was taken greedily has no probability to move.
     Where r A ties with its clipped value its gradient passes."""
     what = "policy_loss"
     _lib.require_cuda(logits, what)
